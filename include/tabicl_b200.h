@@ -404,6 +404,89 @@ enum { TCU_SHARD_PHASES = 7 };
  * over layers; waits for that call); then timing on for the following calls when `enable` is nonzero. */
 TCU_API int tcu_comm_breakdown(tcu_comm *c, int enable, double *ms);
 
+/* ---- four-bit operators ----------------------------------------------------------------------------------------
+ *
+ * A smaller resident form than the reference's f32, i16 and i8 (it has no counterpart there): keys, values and weights
+ * as four-bit codes. `group` neighbouring coordinates share (step, low), two f16 numbers; a coordinate stands for
+ * low + step * code, code 0..15. low is the group's smallest value and step a fifteenth of the span above it, both
+ * rounded to f16 (values beyond +-65504 are held there); codes are rounded to the nearest, ties to even. A group that
+ * holds a NaN or an infinity stands for NaN throughout.
+ *
+ * Order of the codes, for a width of 32 U coordinates, lowest nibble first: of a key, 32-bit word t U + u (t < 4) holds
+ * coordinates 32 u + 8 t + (0..7); of a value, 16-bit word g U + u (g < 8) holds coordinates 32 u + 4 g + (0..3).
+ *
+ * All pointers are device pointers, everything is queued on `stream` (a cudaStream_t; NULL = the context's stream, which
+ * does not wait for the legacy default stream: pass cudaStreamLegacy, the value 1, for that one), and nothing is
+ * allocated: where a call needs working memory the caller gives it (a `_workspace` call says how much; one such block
+ * serves one call at a time; its bytes must be zero before its first use, and every call leaves zero what it needs to
+ * be). Indexes that only the device sees (slots, page numbers, lengths, starts, labels) are checked there: one outside
+ * its range is not followed, and the next call on the context, or tcu_sync, reports it (TCU_ERR_ARG). */
+enum { TCU_F32 = 0, TCU_F16 = 1, TCU_BF16 = 2 }; /* element types of inputs and outputs */
+
+/* A cache in pages: pool is pages * tcu_kv4_page_bytes() bytes, 16-byte aligned. A page holds, for each head in turn,
+ * [page][width / 2] key codes, [page][width / group] key (step, low), [page][width / 2] value codes and
+ * [page][width / group] value (step, low). width 32, 64, 128 or 256; page (tokens) 16, 32, 64, 128 or 256; group 32, 64
+ * or 128, up to the width; heads 1..1024. */
+typedef struct tcu_kv4 {
+    void *pool;
+    int64_t pages;
+    int32_t heads, width, page, group;
+} tcu_kv4;
+TCU_API size_t tcu_kv4_page_bytes(int heads, int width, int page, int group); /* 0: sizes not taken */
+
+/* Quantise `tokens` rows of keys and values ([heads][width] each, by row and head strides in elements) into their slots
+ * (page number * tokens per page + place in the page; negative: the row is skipped). A call's slots are distinct. */
+TCU_API int tcu_kv4_store_device(tcu_ctx *ctx, const tcu_kv4 *cache, int dtype, int tokens, const int64_t *slots, const void *k,
+                                 int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, void *stream);
+/* The numbers that the slots' keys and values stand for (a negative slot's: zeros). */
+TCU_API int tcu_kv4_load_device(tcu_ctx *ctx, const tcu_kv4 *cache, int dtype, int tokens, const int64_t *slots, void *k,
+                                int64_t k_row, int64_t k_head, void *v, int64_t v_row, int64_t v_head, void *stream);
+
+/* Query rows against the cache: sequence s has lens[s] cached tokens (at most max_len), token j of it on page
+ * table[s * table_stride + j / page], and the query rows starts[s] .. starts[s + 1] of `rows` (at most max_rows each);
+ * starts NULL: max_rows rows each, one sequence after the other. */
+typedef struct tcu_kv4_batch {
+    int32_t seqs, rows, max_rows, max_len;
+    const int32_t *starts, *lens, *table;
+    int64_t table_stride;
+} tcu_kv4_batch;
+TCU_API size_t tcu_kv4_attend_workspace(tcu_ctx *ctx, const tcu_kv4 *cache, const tcu_kv4_batch *batch, int q_heads, int dtype); /* (size_t)-1: refused */
+/* Softmax attention: out = sum_j p_j v_j with p the softmax of scale * q . k_j over the keys a row sees. Query head h
+ * reads cache head h / (q_heads / heads). Without `causal` a row sees every cached token of its sequence; with it, row i
+ * of a sequence's n sees tokens up to lens - n + i (its own tokens are stored before the call), and with window > 0 only
+ * the last `window` of those. A row that sees nothing gives zeros. lse (may be NULL): [rows][q_heads], the logarithm of
+ * the sum of e^score, -infinity for such a row. Strides in elements. */
+TCU_API int tcu_kv4_attend_device(tcu_ctx *ctx, const tcu_kv4 *cache, const tcu_kv4_batch *batch, int dtype, int q_heads,
+                                  const void *q, int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head,
+                                  float scale, int causal, int window, float *lse, void *work, size_t work_bytes, void *stream);
+
+/* A weight matrix [n][k] in four bits: codes [n][k / 128 rounded up][64] (each block of 128 columns in the order of a key
+ * of that width, columns past k code 0), scales [n][k / 128 rounded up * 128 / group] (step, low), groups wholly past k
+ * zero. Both 16-byte aligned; group 32, 64 or 128. */
+typedef struct tcu_w4 {
+    const void *codes, *scales;
+    int32_t n, k, group;
+} tcu_w4;
+TCU_API size_t tcu_w4_code_bytes(int n, int k);
+TCU_API size_t tcu_w4_scale_bytes(int n, int k, int group);
+TCU_API int tcu_w4_pack_device(tcu_ctx *ctx, int dtype, int n, int k, int group, const void *w, int64_t ldw, void *codes,
+                               void *scales, void *stream);
+TCU_API size_t tcu_w4_linear_workspace(tcu_ctx *ctx, const tcu_w4 *w, int rows, int dtype); /* (size_t)-1: refused */
+/* y = act(x W^T + bias) + residual, act 0 (none) or 1 (GELU, src/kern.rs:285-290); bias [n] and residual [rows][n] may be
+ * NULL, and the residual may be y itself. x, y, bias and residual are of one type; sums are taken in f32. */
+TCU_API int tcu_w4_linear_device(tcu_ctx *ctx, const tcu_w4 *w, int dtype, int rows, const void *x, int64_t ldx, void *y,
+                                 int64_t ldy, const void *bias, int act, const void *residual, int64_t ldr, void *work,
+                                 size_t work_bytes, void *stream);
+
+/* Rows of scores: out [rows][per_row] the log probability of each given label under the softmax of logits / temperature
+ * (label -1: none, 0 is returned), entropy [rows] (may be NULL) in nats, and the `top` (0..32) classes of highest score,
+ * equal scores by the lower class: top_ids and their log probabilities top_values [rows][top]. -infinity masks a class:
+ * it is no alternative (id -1, value -infinity, where the others run out), and a row of nothing else gives -infinity for
+ * its labels and entropy 0. A NaN or +infinity in a row makes its log probabilities and entropy NaN. */
+TCU_API int tcu_label_logprobs_device(tcu_ctx *ctx, int dtype, const void *logits, int rows, int classes, int64_t stride,
+                                      const int32_t *labels, int per_row, float *out, float *entropy, int top, float *top_values,
+                                      int32_t *top_ids, double temperature, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

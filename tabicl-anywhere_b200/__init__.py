@@ -7,6 +7,7 @@ The objects mirror the reference's accelerator side (src/gpu.rs, src/predict.rs:
 * `VramModel` - one fitted problem's key/value cache resident on it (gpu::VramModel)
 * `VramMember` - a fitted member's problems and its class tree, predicted whole (predict::predict_raw)
 * `VramTier` / `VramHandle` - problems resident for many tenants within byte budgets; the handle is an AttendCached
+* `Kv4Cache`, `W4` - the four-bit cache and weights (fourbit.py; no counterpart in the reference)
 * `CudaAttend` - the `AttendCached` implementation: `attend`, `stage`, `rows`, each returning None to decline
 
 Everything computes on the GPU through libtabicl_b200.so; there is no CPU path here. The library is built in-tree
@@ -19,6 +20,7 @@ import numpy as np
 
 from . import tirs  # noqa: F401  (bundle reader/writer for callers)
 from .plan import Plan  # noqa: F401
+from . import fourbit
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtabicl_b200.so")
@@ -165,6 +167,7 @@ def lib():
         "tcu_stage_sharded_device": (_c_int, [_c_void, _c_void, _c_void, _c_int, _c_int, _c_void, _c_void]),
         "tcu_comm_breakdown": (_c_int, [_c_void, _c_int, P(ctypes.c_double)]),
         "tcu_comm_abort": (_c_int, [_c_void]),
+        **fourbit.signatures(),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -245,6 +248,14 @@ class Gpu:
         e = ctypes.c_double()
         self.check(lib().tcu_selftest_mma(self._h, ctypes.byref(e)))
         return e.value
+
+    def label_logprobs(self, dtype, logits_ptr, rows, classes, stride, labels_ptr, per_row, out_ptr, entropy=None, top=0,
+                       top_values=None, top_ids=None, temperature=1.0, stream=None):
+        """Log probabilities of the given labels [rows][per_row], the rows' entropy and their `top` alternatives
+        (log probabilities and ids), on device buffers (dtype F32, F16 or BF16 of the logits)."""
+        return self.check(lib().tcu_label_logprobs_device(self._h, dtype, logits_ptr, rows, classes, stride, labels_ptr,
+                                                          per_row, out_ptr, entropy, top, top_values, top_ids,
+                                                          temperature, stream))
 
     def pack(self, kv, d, rc, c_ptr, rec_ptr):
         return self.check(lib().tcu_pack_device(self._h, kv, d, rc, c_ptr, rec_ptr))
@@ -989,3 +1000,6 @@ class CudaAttend:
         """All three stages for a member of one node (predict.rs:642-652): None when the device declines (no column
         and row stages in the weights or the cache) or fails, as for the other hooks."""
         return self._or_cpu(lambda: self._model(prefix, 0).rows(x, out_n))
+
+
+from .fourbit import BF16, F16, F32, Kv4Cache, W4  # noqa: E402,F401  (they use lib() and Gpu)

@@ -24,6 +24,7 @@
 #include <string>
 #include <vector>
 
+#include "fourbit.cuh"
 #include "kernels.cuh"
 #include "engine.hpp"
 #include "tirs.hpp"
@@ -98,7 +99,8 @@ struct tcu_ctx {
 };
 
 // Which wait each report slot stands for.
-enum { ERR_ATTEND_TC = 0, ERR_GEMM_TC = 1, ERR_QMLP_TC = 2, ERR_ROWS = 3, ERR_PEER = 6, ERR_SLOTS = 8 };
+// (ERR_INDEX is no wait: a four-bit operator met an index outside its range, see check_device_error.)
+enum { ERR_ATTEND_TC = 0, ERR_GEMM_TC = 1, ERR_QMLP_TC = 2, ERR_ROWS = 3, ERR_PEER = 6, ERR_INDEX = 7, ERR_SLOTS = 8 };
 static const char *const err_slot_names[7] = {
     "tensor-core attention (matrix-unit or copy wait)", "tensor-core linear layer (matrix-unit or copy wait)",
     "tensor-core query MLP (matrix-unit wait)", "one-kernel stage (grid barrier)", "one-kernel stage (key tile copy)",
@@ -1018,6 +1020,11 @@ static void check_device_error(tcu_ctx *ctx) {
     if (!which.empty())
         fail(TCU_ERR_CUDA, "kernels gave up a bounded wait: " + which +
                                ". Outputs of the calls queued since the last report are invalid");
+    if (slot[ERR_INDEX]) {
+        slot[ERR_INDEX] = 0;
+        fail(TCU_ERR_ARG, "a four-bit operator or label_logprobs met a slot, page, length, start or label outside its range "
+                          "since the last report; nothing was read or written there");
+    }
 }
 
 // Largest |key| and |value| of a stored layer -> the tensor cores' power-of-two scalings (synchronises).
@@ -3220,6 +3227,211 @@ int tcu_profile(tcu_ctx *ctx, int enable, double *attend_ms, uint64_t *attend_la
         }
         ctx->prof = enable != 0;
         ctx->prof_used = 0;
+        return TCU_OK;
+    });
+}
+
+}  // extern "C"
+
+// ---- four-bit operators and label log-probabilities ---------------------------------------------------------------
+
+static size_t elem_size(int dtype) { return dtype == TCU_F32 ? 4 : 2; }
+
+static void check_dtype(const char *who, int dtype) {
+    if (dtype < TCU_F32 || dtype > TCU_BF16) fail(TCU_ERR_ARG, std::string(who) + ": dtype must be TCU_F32, TCU_F16 or TCU_BF16");
+}
+static void check_aligned(const char *who, const char *what, const void *p, size_t to) {
+    if ((uintptr_t)p % to) fail(TCU_ERR_ARG, std::string(who) + ": " + what + " must be " + std::to_string(to) + "-byte aligned");
+}
+static bool kv4_sizes(int heads, int width, int page, int group) {
+    const bool w = width == 32 || width == 64 || width == 128 || width == 256;
+    const bool g = group == 32 || group == 64 || group == 128;
+    const bool p = page == 16 || page == 32 || page == 64 || page == 128 || page == 256;
+    return heads >= 1 && heads <= 1024 && w && g && p && group <= width;
+}
+static Kv4 kv4_of(const char *who, const tcu_kv4 *c) {
+    if (!c) fail(TCU_ERR_ARG, std::string(who) + ": null cache");
+    if (!kv4_sizes(c->heads, c->width, c->page, c->group))
+        fail(TCU_ERR_ARG, std::string(who) + ": heads 1..1024, width 32, 64, 128 or 256, page 16, 32, 64, 128 or 256 tokens, "
+                                             "group 32, 64 or 128 up to the width");
+    if (!c->pool || c->pages < 1) fail(TCU_ERR_ARG, std::string(who) + ": the cache has no pool or no pages");
+    check_aligned(who, "the pool", c->pool, 16);
+    Kv4 k;
+    k.pool = (uint8_t *)c->pool, k.pages = c->pages, k.heads = c->heads, k.width = c->width, k.page = c->page, k.group = c->group;
+    return k;
+}
+
+extern "C" {
+
+size_t tcu_kv4_page_bytes(int heads, int width, int page, int group) {
+    return kv4_sizes(heads, width, page, group) ? (size_t)heads * kv4_head_bytes(width, page, group) : 0;
+}
+
+static int kv4_copy(tcu_ctx *ctx, const char *who, bool store, const tcu_kv4 *cache, int dtype, int tokens, const int64_t *slots,
+                    void *k, int64_t k_row, int64_t k_head, void *v, int64_t v_row, int64_t v_head, void *stream) {
+    return guarded(ctx, [&]() -> int {
+        check_device_error(ctx);
+        Kv4CopyArgs a;
+        a.c = kv4_of(who, cache);
+        check_dtype(who, dtype);
+        if (tokens < 0) fail(TCU_ERR_ARG, std::string(who) + ": tokens must not be negative");
+        if (tokens == 0) return TCU_OK;
+        if (!slots || !k || !v) fail(TCU_ERR_ARG, std::string(who) + ": null slots, keys or values");
+        if (k_row < 0 || k_head < 0 || v_row < 0 || v_head < 0) fail(TCU_ERR_ARG, std::string(who) + ": strides must not be negative");
+        check_aligned(who, "slots", slots, 8);
+        check_aligned(who, "keys", k, elem_size(dtype)), check_aligned(who, "values", v, elem_size(dtype));
+        a.tokens = tokens, a.slots = (const long long *)slots, a.k = k, a.v = v;
+        a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head, a.err = ctx->err_mapped + ERR_INDEX;
+        cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        Launch{ctx, s}(store ? launch_kv4_store(dtype, a, s, &ctx->launches) : launch_kv4_load(dtype, a, s, &ctx->launches), who);
+        return TCU_OK;
+    });
+}
+
+int tcu_kv4_store_device(tcu_ctx *ctx, const tcu_kv4 *cache, int dtype, int tokens, const int64_t *slots, const void *k,
+                         int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head, void *stream) {
+    return kv4_copy(ctx, "kv4_store", true, cache, dtype, tokens, slots, const_cast<void *>(k), k_row, k_head, const_cast<void *>(v),
+                    v_row, v_head, stream);
+}
+
+int tcu_kv4_load_device(tcu_ctx *ctx, const tcu_kv4 *cache, int dtype, int tokens, const int64_t *slots, void *k, int64_t k_row,
+                        int64_t k_head, void *v, int64_t v_row, int64_t v_head, void *stream) {
+    return kv4_copy(ctx, "kv4_load", false, cache, dtype, tokens, slots, k, k_row, k_head, v, v_row, v_head, stream);
+}
+
+static Kv4AttendArgs kv4_attend_args(const tcu_kv4 *cache, const tcu_kv4_batch *b, int q_heads, int dtype) {
+    Kv4AttendArgs a;
+    a.c = kv4_of("kv4_attend", cache);
+    check_dtype("kv4_attend", dtype);
+    if (!b) fail(TCU_ERR_ARG, "kv4_attend: null batch");
+    if (q_heads < 1 || q_heads > 65535 || q_heads % a.c.heads) fail(TCU_ERR_ARG, "kv4_attend: query heads must be a multiple of the cache's heads");
+    if (b->seqs < 0 || b->seqs > 65535 || b->rows < 0 || b->max_rows < 0 || b->max_len < 0)
+        fail(TCU_ERR_ARG, "kv4_attend: 0..65535 sequences, rows and lengths not negative");
+    if ((long long)b->rows * q_heads > 0x7fffffffLL / 256) fail(TCU_ERR_ARG, "kv4_attend: too many query rows for one call");
+    if (!b->starts && (long long)b->seqs * b->max_rows != b->rows) fail(TCU_ERR_ARG, "kv4_attend: without starts every sequence has max_rows rows");
+    if ((long long)b->table_stride * a.c.page < b->max_len) fail(TCU_ERR_ARG, "kv4_attend: the table's rows do not hold max_len tokens");
+    a.seqs = b->seqs, a.rows = b->rows, a.max_rows = b->max_rows, a.max_len = b->max_len, a.starts = b->starts, a.lens = b->lens;
+    a.table = b->table, a.table_stride = b->table_stride, a.q_heads = q_heads;
+    return a;
+}
+
+size_t tcu_kv4_attend_workspace(tcu_ctx *ctx, const tcu_kv4 *cache, const tcu_kv4_batch *batch, int q_heads, int dtype) {
+    size_t need = 0;
+    const int r = guarded(ctx, [&]() -> int {
+        kv4_attend_args(cache, batch, q_heads, dtype);
+        return TCU_OK;
+    });
+    return r == TCU_OK ? need : (size_t)-1;
+}
+
+int tcu_kv4_attend_device(tcu_ctx *ctx, const tcu_kv4 *cache, const tcu_kv4_batch *batch, int dtype, int q_heads, const void *q,
+                          int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head, float scale, int causal,
+                          int window, float *lse, void *work, size_t work_bytes, void *stream) {
+    return guarded(ctx, [&]() -> int {
+        check_device_error(ctx);
+        Kv4AttendArgs a = kv4_attend_args(cache, batch, q_heads, dtype);
+        if (window < 0 || (window && !causal)) fail(TCU_ERR_ARG, "kv4_attend: a window is not negative and goes with causal");
+        if (!std::isfinite(scale)) fail(TCU_ERR_ARG, "kv4_attend: scale must be finite");
+        if (q_row < 0 || q_head < 0 || o_row < 0 || o_head < 0) fail(TCU_ERR_ARG, "kv4_attend: strides must not be negative");
+        if (!a.seqs || !a.rows || !a.max_rows) return TCU_OK;
+        if (!q || !out || !a.lens || (a.max_len && !a.table)) fail(TCU_ERR_ARG, "kv4_attend: null queries, output, lengths or table");
+        check_aligned("kv4_attend", "queries", q, elem_size(dtype)), check_aligned("kv4_attend", "output", out, elem_size(dtype));
+        check_aligned("kv4_attend", "lengths", a.lens, 4), check_aligned("kv4_attend", "table", a.table, 4);
+        check_aligned("kv4_attend", "starts", a.starts, 4), check_aligned("kv4_attend", "lse", lse, 4);
+        a.q = q, a.out = out, a.q_row = q_row, a.q_head = q_head, a.o_row = o_row, a.o_head = o_head;
+        a.scale = scale, a.causal = causal != 0, a.window = window, a.lse = lse, a.err = ctx->err_mapped + ERR_INDEX;
+        cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        Launch{ctx, s}(launch_kv4_attend(dtype, a, s, &ctx->launches), "kv4_attend");
+        return TCU_OK;
+    });
+}
+
+static bool w4_sizes(int n, int k, int group) {
+    return n >= 1 && k >= 1 && k <= (1 << 24) && (group == 32 || group == 64 || group == 128);
+}
+size_t tcu_w4_code_bytes(int n, int k) { return w4_sizes(n, k, 32) ? (size_t)n * ((k + 127) / 128) * 64 : 0; }
+size_t tcu_w4_scale_bytes(int n, int k, int group) {
+    return w4_sizes(n, k, group) ? (size_t)n * ((k + 127) / 128) * (128 / group) * 4 : 0;
+}
+
+int tcu_w4_pack_device(tcu_ctx *ctx, int dtype, int n, int k, int group, const void *w, int64_t ldw, void *codes, void *scales,
+                       void *stream) {
+    return guarded(ctx, [&]() -> int {
+        check_device_error(ctx);
+        check_dtype("w4_pack", dtype);
+        if (!w4_sizes(n, k, group)) fail(TCU_ERR_ARG, "w4_pack: n and k at least 1, k up to 2^24, group 32, 64 or 128");
+        if (!w || !codes || !scales || ldw < k) fail(TCU_ERR_ARG, "w4_pack: null argument or a row stride below k");
+        check_aligned("w4_pack", "weights", w, elem_size(dtype));
+        check_aligned("w4_pack", "codes", codes, 16), check_aligned("w4_pack", "scales", scales, 16);
+        cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        Launch{ctx, s}(launch_w4_pack(dtype, w, ldw, n, k, group, (uint8_t *)codes, (__half2 *)scales, s, &ctx->launches), "w4_pack");
+        return TCU_OK;
+    });
+}
+
+static W4Args w4_args(const tcu_w4 *w, int dtype, int rows) {
+    if (!w) fail(TCU_ERR_ARG, "w4_linear: null weights");
+    check_dtype("w4_linear", dtype);
+    if (!w4_sizes(w->n, w->k, w->group)) fail(TCU_ERR_ARG, "w4_linear: n and k at least 1, k up to 2^24, group 32, 64 or 128");
+    if (!w->codes || !w->scales) fail(TCU_ERR_ARG, "w4_linear: null codes or scales");
+    check_aligned("w4_linear", "codes", w->codes, 16), check_aligned("w4_linear", "scales", w->scales, 16);
+    if (rows < 0 || rows > 65535) fail(TCU_ERR_ARG, "w4_linear: 0..65535 rows");
+    W4Args a;
+    a.codes = (const uint8_t *)w->codes, a.scales = (const __half2 *)w->scales, a.n = w->n, a.k = w->k, a.group = w->group, a.rows = rows;
+    return a;
+}
+
+size_t tcu_w4_linear_workspace(tcu_ctx *ctx, const tcu_w4 *w, int rows, int dtype) {
+    size_t need = 0;
+    const int r = guarded(ctx, [&]() -> int {
+        w4_args(w, dtype, rows);
+        return TCU_OK;
+    });
+    return r == TCU_OK ? need : (size_t)-1;
+}
+
+int tcu_w4_linear_device(tcu_ctx *ctx, const tcu_w4 *w, int dtype, int rows, const void *x, int64_t ldx, void *y, int64_t ldy,
+                         const void *bias, int act, const void *residual, int64_t ldr, void *work, size_t work_bytes, void *stream) {
+    return guarded(ctx, [&]() -> int {
+        check_device_error(ctx);
+        W4Args a = w4_args(w, dtype, rows);
+        if (act < 0 || act > 1) fail(TCU_ERR_ARG, "w4_linear: act must be 0 (none) or 1 (GELU)");
+        if (rows == 0) return TCU_OK;
+        if (!x || !y) fail(TCU_ERR_ARG, "w4_linear: null input or output");
+        if (ldx < a.k || ldy < a.n || (residual && ldr < a.n)) fail(TCU_ERR_ARG, "w4_linear: a row stride below the row");
+        check_aligned("w4_linear", "input", x, elem_size(dtype)), check_aligned("w4_linear", "output", y, elem_size(dtype));
+        check_aligned("w4_linear", "bias", bias, elem_size(dtype)), check_aligned("w4_linear", "residual", residual, elem_size(dtype));
+        a.x = x, a.ldx = ldx, a.y = y, a.ldy = ldy, a.bias = bias, a.act = act, a.residual = residual, a.ldr = ldr;
+        cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        Launch{ctx, s}(launch_w4_linear(dtype, a, s, &ctx->launches), "w4_linear");
+        return TCU_OK;
+    });
+}
+
+int tcu_label_logprobs_device(tcu_ctx *ctx, int dtype, const void *logits, int rows, int classes, int64_t stride, const int32_t *labels,
+                              int per_row, float *out, float *entropy, int top, float *top_values, int32_t *top_ids,
+                              double temperature, void *stream) {
+    return guarded(ctx, [&]() -> int {
+        check_device_error(ctx);
+        check_dtype("label_logprobs", dtype);
+        if (rows < 0 || classes < 1 || stride < classes) fail(TCU_ERR_ARG, "label_logprobs: rows not negative, classes at least 1, stride at least classes");
+        if (per_row < 0 || (per_row && rows && (!labels || !out))) fail(TCU_ERR_ARG, "label_logprobs: null labels or output");
+        if (top < 0 || top > LOGPROB_MAX_TOP || (top && rows && (!top_values || !top_ids)))
+            fail(TCU_ERR_ARG, "label_logprobs: 0.." + std::to_string(LOGPROB_MAX_TOP) + " alternatives, with their outputs");
+        if (!(temperature > 0) || !std::isfinite(temperature) || !std::isfinite((float)(1.0 / temperature)))
+            fail(TCU_ERR_ARG, "label_logprobs: temperature must be positive");
+        if (rows == 0) return TCU_OK;
+        if (!logits) fail(TCU_ERR_ARG, "label_logprobs: null logits");
+        check_aligned("label_logprobs", "logits", logits, elem_size(dtype));
+        check_aligned("label_logprobs", "labels", labels, 4), check_aligned("label_logprobs", "out", out, 4);
+        check_aligned("label_logprobs", "entropy", entropy, 4);
+        check_aligned("label_logprobs", "top_values", top_values, 4), check_aligned("label_logprobs", "top_ids", top_ids, 4);
+        LogprobArgs a;
+        a.logits = logits, a.rows = rows, a.classes = classes, a.stride = stride, a.labels = labels, a.per_row = per_row, a.top = top;
+        a.inv_t = (float)(1.0 / temperature), a.out = out, a.entropy = entropy, a.top_values = top_values, a.top_ids = top_ids;
+        a.err = ctx->err_mapped + ERR_INDEX;
+        cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        Launch{ctx, s}(launch_logprobs(dtype, a, s, &ctx->launches), "label_logprobs");
         return TCU_OK;
     });
 }

@@ -1,0 +1,183 @@
+// The four-bit operators (kv4.cu, w4.cu) and the label log-probabilities (logprobs.cu): what the host hands the
+// kernels, the stored format, and the conversions every kernel shares.
+//
+// Format: `group` neighbouring coordinates share (step, low), two f16 numbers; a coordinate is low + step * code with a
+// code of 0..15. Widths are made of 32-coordinate units (NU of them). A key's codes are words of 8: word t * NU + u
+// (t < 4) holds coordinates 32 u + 8 t + j in nibble j, so that a thread of a matrix fragment (t = lane % 4) reads its
+// part of every unit with one wide load. A value's codes are half-words of 4: half-word g * NU + u (g < 8) holds
+// coordinates 32 u + 4 g + j in nibble j, the same for a thread's row (g = lane / 4) of a transposed fragment.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cfloat>
+#include <cmath>
+#include <cstddef>
+#include <cstdint>
+
+namespace tcu {
+
+enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
+
+// A paged cache: pool [pages][heads]{key codes [page][width / 2], key (step, low) [page][width / group], value codes,
+// value (step, low)}.
+struct Kv4 {
+    uint8_t *pool = nullptr;
+    long long pages = 0;
+    int heads = 0, width = 0, page = 0, group = 0;
+};
+
+__host__ __device__ inline size_t kv4_head_bytes(int width, int page, int group) {
+    return (size_t)page * (width + 8 * (width / group));
+}
+// Byte offsets inside a head's part of a page.
+struct Kv4Offsets {
+    unsigned ks, vc, vs;  // key scales, value codes, value scales (key codes at 0)
+};
+__host__ __device__ inline Kv4Offsets kv4_offsets(int width, int page, int group) {
+    const unsigned c = (unsigned)page * (width / 2), s = (unsigned)page * (width / group) * 4;
+    return Kv4Offsets{c, c + s, 2 * c + s};
+}
+
+// Keys and values of `tokens` rows to (store) or from (load) their slots.
+struct Kv4CopyArgs {
+    Kv4 c;
+    int tokens = 0;
+    const long long *slots = nullptr;  // page * tokens per page + place in it; negative: no slot
+    void *k = nullptr, *v = nullptr;   // [tokens][heads][width] by row and head strides (elements)
+    long long k_row = 0, k_head = 0, v_row = 0, v_head = 0;
+    int *err = nullptr;  // report slot (host memory, mapped): set to 1 on a slot outside the cache
+};
+
+// Ragged query rows against the cache.
+struct Kv4AttendArgs {
+    Kv4 c;
+    int seqs = 0, rows = 0, max_rows = 0, max_len = 0;
+    const int *starts = nullptr, *lens = nullptr, *table = nullptr;
+    long long table_stride = 0;
+    int q_heads = 0;
+    const void *q = nullptr;
+    void *out = nullptr;
+    long long q_row = 0, q_head = 0, o_row = 0, o_head = 0;
+    float scale = 0.f;
+    int causal = 0, window = 0;
+    float *lse = nullptr;  // [rows][q_heads], or null
+    int *err = nullptr;    // report slot: set to 1 on a length, start or page outside its range
+};
+
+// y = act(x W^T + bias) + residual with four-bit weights.
+struct W4Args {
+    const uint8_t *codes = nullptr;  // [n][k / 128 rounded up][64]
+    const __half2 *scales = nullptr; // [n][k / 128 rounded up * 128 / group] (step, low)
+    int n = 0, k = 0, group = 0, rows = 0, act = 0;
+    const void *x = nullptr, *bias = nullptr, *residual = nullptr;
+    void *y = nullptr;
+    long long ldx = 0, ldy = 0, ldr = 0;
+};
+
+struct LogprobArgs {
+    const void *logits = nullptr;
+    int rows = 0, classes = 0;
+    long long stride = 0;
+    const int *labels = nullptr;  // [rows][per_row]
+    int per_row = 0, top = 0;
+    float inv_t = 1.f;
+    float *out = nullptr, *entropy = nullptr, *top_values = nullptr;
+    int *top_ids = nullptr;
+    int *err = nullptr;  // report slot: set to 1 on a label beyond the classes
+};
+constexpr int LOGPROB_MAX_TOP = 32;
+
+cudaError_t launch_kv4_store(int dtype, const Kv4CopyArgs &a, cudaStream_t s, uint64_t *launches);
+cudaError_t launch_kv4_load(int dtype, const Kv4CopyArgs &a, cudaStream_t s, uint64_t *launches);
+cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, cudaStream_t s, uint64_t *launches);
+// A weight matrix w [n][k] (row stride ldw) to codes and scales.
+cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k, int group, uint8_t *codes,
+                           __half2 *scales, cudaStream_t s, uint64_t *launches);
+cudaError_t launch_w4_linear(int dtype, const W4Args &a, cudaStream_t s, uint64_t *launches);
+cudaError_t launch_logprobs(int dtype, const LogprobArgs &a, cudaStream_t s, uint64_t *launches);
+
+#ifdef __CUDACC__
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<DT_F32> {
+    using T = float;
+    static __device__ __forceinline__ float get(float x) { return x; }
+    static __device__ __forceinline__ float put(float x) { return x; }
+};
+template <>
+struct Elem<DT_F16> {
+    using T = __half;
+    static __device__ __forceinline__ float get(__half x) { return __half2float(x); }
+    static __device__ __forceinline__ __half put(float x) { return __float2half_rn(x); }
+};
+template <>
+struct Elem<DT_BF16> {
+    using T = __nv_bfloat16;
+    static __device__ __forceinline__ float get(__nv_bfloat16 x) { return __bfloat162float(x); }
+    static __device__ __forceinline__ __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
+};
+
+// Eight consecutive elements; `wide` when the address is known to be 16-byte aligned.
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::T *p, bool wide, float (&v)[8]) {
+    using T = typename Elem<DT>::T;
+    if (wide) {
+        __align__(16) T e[8];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++)
+            reinterpret_cast<uint4 *>(e)[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = Elem<DT>::get(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = Elem<DT>::get(p[i]);
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store8(typename Elem<DT>::T *p, bool wide, const float (&v)[8]) {
+    using T = typename Elem<DT>::T;
+    __align__(16) T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) e[i] = Elem<DT>::put(v[i]);
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(e)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = e[i];
+    }
+}
+
+// (step, low) of a group with extremes mn, mx (`bad`: it holds a NaN or an infinity, and then stands for NaN
+// throughout). low is the smallest value and step a fifteenth of the span above it, each rounded to f16 (values beyond
+// f16's range are held at its largest): f16 keeps a group's overhead at 4 bytes and 11 bits of a 4-bit step.
+__device__ __forceinline__ void group_scale(float mn, float mx, bool bad, __half &step, __half &low) {
+    low = __float2half_rn(fminf(fmaxf(mn, -65504.f), 65504.f));
+    step = __float2half_rn(__fdiv_rn(fmaxf(__fsub_rn(fminf(mx, 65504.f), __half2float(low)), 0.f), 15.f));
+    if (bad) step = __ushort_as_half(0), low = __ushort_as_half(0x7e00);
+}
+// A value's code: its distance from low in steps, rounded to the nearest (ties to even), held to 0..15; 0 where the
+// step is 0. The quotient is the correctly rounded one, so equal inputs give equal codes everywhere.
+__device__ __forceinline__ uint32_t code_of(float x, float step, float low) {
+    if (!(step > 0.f)) return 0;
+    return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, low), step)), 0.f), 15.f);
+}
+__device__ __forceinline__ uint32_t pack8(const float (&x)[8], float step, float low) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) w |= code_of(x[j], step, low) << (4 * j);
+    return w;
+}
+// low + step * code, the product and the sum each rounded to f32 (step * code is exact: 11 + 4 bits).
+__device__ __forceinline__ float value_of(uint32_t w, int j, float step, float low) {
+    return __fadd_rn(__fmul_rn((float)((w >> (4 * j)) & 15u), step), low);
+}
+__device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+#endif
+
+}  // namespace tcu

@@ -1,0 +1,92 @@
+// The four-bit paged cache: quantise keys and values into their slots, and read them back.
+#include "fourbit.cuh"
+
+namespace tcu {
+
+// A thread takes 8 neighbouring coordinates (one word of a key, two half-words of a value) of one head of one token, of
+// the keys and of the values; width / 8 neighbouring lanes hold a token's head, group / 8 of them a group.
+template <int DT, bool STORE>
+__global__ void __launch_bounds__(256) k_kv4_copy(Kv4CopyArgs a, long long items, bool wide) {
+    using T = typename Elem<DT>::T;
+    const int W = a.c.width, NU = W / 32, per = W / 8, G8 = a.c.group / 8, NG = W / a.c.group, P = a.c.page;
+    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    const bool on = i < items;
+    const long long row = on ? i / per : 0;
+    const int part = (int)(i % per), u = part / 4, t = part % 4;
+    const int token = (int)(row / a.c.heads), head = (int)(row % a.c.heads);
+    const long long slot = on ? a.slots[token] : -1, page = slot / P;
+    const int at = (int)(slot % P);
+    const bool there = slot >= 0 && page < a.c.pages;
+    if (slot >= 0 && !there) *reinterpret_cast<volatile int *>(a.err) = 1;
+    const Kv4Offsets o = kv4_offsets(W, P, a.c.group);
+    uint8_t *base = a.c.pool + (there ? ((size_t)page * a.c.heads + head) * kv4_head_bytes(W, P, a.c.group) : 0);
+    T *kp = reinterpret_cast<T *>(a.k) + token * a.k_row + head * a.k_head + part * 8;
+    T *vp = reinterpret_cast<T *>(a.v) + token * a.v_row + head * a.v_head + part * 8;
+    uint32_t *kc = reinterpret_cast<uint32_t *>(base + (size_t)at * (W / 2)) + t * NU + u;
+    uint16_t *vc = reinterpret_cast<uint16_t *>(base + o.vc + (size_t)at * (W / 2)) + 2 * t * NU + u;
+    __half2 *ks = reinterpret_cast<__half2 *>(base + o.ks) + (size_t)at * NG + part / G8;
+    __half2 *vs = reinterpret_cast<__half2 *>(base + o.vs) + (size_t)at * NG + part / G8;
+    if (STORE) {
+        float x[2][8] = {};
+        if (there) load8<DT>(kp, wide, x[0]), load8<DT>(vp, wide, x[1]);
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            float mn = x[w][0], mx = x[w][0];
+            bool bad = !finite_f(x[w][0]);
+#pragma unroll
+            for (int j = 1; j < 8; j++) mn = fminf(mn, x[w][j]), mx = fmaxf(mx, x[w][j]), bad |= !finite_f(x[w][j]);
+            for (int d = 1; d < G8; d *= 2) {
+                mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                bad |= (bool)__shfl_xor_sync(0xffffffffu, (int)bad, d);
+            }
+            __half step, low;
+            group_scale(mn, mx, bad, step, low);
+            const uint32_t c = pack8(x[w], __half2float(step), __half2float(low));
+            if (there) {
+                if (w == 0) {
+                    *kc = c;
+                    if (part % G8 == 0) *ks = __halves2half2(step, low);
+                } else {
+                    vc[0] = (uint16_t)c, vc[NU] = (uint16_t)(c >> 16);
+                    if (part % G8 == 0) *vs = __halves2half2(step, low);
+                }
+            }
+        }
+    } else if (on) {
+        float x[2][8] = {};
+        if (there) {
+            const uint32_t c0 = *kc, c1 = (uint32_t)vc[0] | (uint32_t)vc[NU] << 16;
+            const float2 s0 = __half22float2(*ks), s1 = __half22float2(*vs);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[0][j] = value_of(c0, j, s0.x, s0.y), x[1][j] = value_of(c1, j, s1.x, s1.y);
+        }
+        store8<DT>(kp, wide, x[0]), store8<DT>(vp, wide, x[1]);
+    }
+}
+
+template <bool STORE>
+static cudaError_t launch_copy(int dtype, const Kv4CopyArgs &a, cudaStream_t s, uint64_t *launches) {
+    const long long items = (long long)a.tokens * a.c.heads * (a.c.width / 8);
+    if (!items) return cudaSuccess;
+    const int es = dtype == DT_F32 ? 4 : 2;
+    const bool wide = !((((uintptr_t)a.k | (uintptr_t)a.v) & 15) ||
+                        ((a.k_row | a.k_head | a.v_row | a.v_head) * es) % 16);
+    const unsigned grid = (unsigned)((items + 255) / 256);
+    if (dtype == DT_F32)
+        k_kv4_copy<DT_F32, STORE><<<grid, 256, 0, s>>>(a, items, wide);
+    else if (dtype == DT_F16)
+        k_kv4_copy<DT_F16, STORE><<<grid, 256, 0, s>>>(a, items, wide);
+    else
+        k_kv4_copy<DT_BF16, STORE><<<grid, 256, 0, s>>>(a, items, wide);
+    if (launches) ++*launches;
+    return cudaGetLastError();
+}
+cudaError_t launch_kv4_store(int dtype, const Kv4CopyArgs &a, cudaStream_t s, uint64_t *launches) {
+    return launch_copy<true>(dtype, a, s, launches);
+}
+cudaError_t launch_kv4_load(int dtype, const Kv4CopyArgs &a, cudaStream_t s, uint64_t *launches) {
+    return launch_copy<false>(dtype, a, s, launches);
+}
+
+}  // namespace tcu
