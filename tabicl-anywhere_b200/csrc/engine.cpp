@@ -3318,7 +3318,8 @@ static Kv4AttendArgs kv4_attend_args(const tcu_kv4 *cache, const tcu_kv4_batch *
 size_t tcu_kv4_attend_workspace(tcu_ctx *ctx, const tcu_kv4 *cache, const tcu_kv4_batch *batch, int q_heads, int dtype) {
     size_t need = 0;
     const int r = guarded(ctx, [&]() -> int {
-        kv4_attend_args(cache, batch, q_heads, dtype);
+        const Kv4AttendArgs a = kv4_attend_args(cache, batch, q_heads, dtype);
+        need = a.seqs && a.rows && a.max_rows ? kv4_attend_workspace(dtype, a, ctx->sms) : 0;
         return TCU_OK;
     });
     return r == TCU_OK ? need : (size_t)-1;
@@ -3341,7 +3342,10 @@ int tcu_kv4_attend_device(tcu_ctx *ctx, const tcu_kv4 *cache, const tcu_kv4_batc
         a.q = q, a.out = out, a.q_row = q_row, a.q_head = q_head, a.o_row = o_row, a.o_head = o_head;
         a.scale = scale, a.causal = causal != 0, a.window = window, a.lse = lse, a.err = ctx->err_mapped + ERR_INDEX;
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
-        Launch{ctx, s}(launch_kv4_attend(dtype, a, s, &ctx->launches), "kv4_attend");
+        const size_t need = kv4_attend_workspace(dtype, a, ctx->sms);
+        if (need && (!work || work_bytes < need)) fail(TCU_ERR_ARG, "kv4_attend: needs " + std::to_string(need) + " bytes of working memory");
+        check_aligned("kv4_attend", "working memory", work, 16);
+        Launch{ctx, s}(launch_kv4_attend(dtype, a, ctx->sms, work, work_bytes, s, &ctx->launches), "kv4_attend");
         return TCU_OK;
     });
 }

@@ -91,7 +91,12 @@ constexpr int LOGPROB_MAX_TOP = 32;
 
 cudaError_t launch_kv4_store(int dtype, const Kv4CopyArgs &a, cudaStream_t s, uint64_t *launches);
 cudaError_t launch_kv4_load(int dtype, const Kv4CopyArgs &a, cudaStream_t s, uint64_t *launches);
-cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, cudaStream_t s, uint64_t *launches);
+// Working memory of an attention call (its first ints zero between calls), and the call.
+size_t kv4_attend_workspace(int dtype, const Kv4AttendArgs &a, int sms);
+cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *work, size_t work_bytes, cudaStream_t s,
+                              uint64_t *launches);
+// kernels.cu: opt a kernel in to `bytes` of dynamic shared memory on the current device.
+cudaError_t allow_dynamic_smem(const void *kernel, size_t bytes);
 // A weight matrix w [n][k] (row stride ldw) to codes and scales.
 cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k, int group, uint8_t *codes,
                            __half2 *scales, cudaStream_t s, uint64_t *launches);

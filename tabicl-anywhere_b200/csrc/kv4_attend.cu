@@ -1,89 +1,606 @@
-// Attention of ragged query rows over a four-bit paged cache.
+// Attention of ragged query rows over a four-bit paged cache: few rows a cache head (decoding, short tails).
+//
+// The codes go into the matrix unit as they are. A nibble is a subnormal f16 (code * 2^-24, or 2^-20 from the second
+// nibble of a byte: one AND takes two of them out of a word), so a product with the codes is exact in everything but q and
+// the weights, and the group scales act on its f32 result:
+//     q . k_j   = sum over groups of  step * (q_g . codes)  +  low * (sum of q_g)
+//     sum p_j v = sum over groups of  (p_j step) . codes    +  sum p_j low
+// Per 32 keys a warp computes S^T = K Q^T with 16 keys as rows and 8 query rows as columns, so a key's codes are read in
+// the order they are stored in, and O^T = V^T P'^T with P' = p * step turned round in registers (movmatrix).
+#include <algorithm>
+
 #include "fourbit.cuh"
 
 namespace tcu {
 
-// One block per (query row, query head), one warp's lanes over a key's words: width / 8 lanes a key, several keys a
-// warp and step, each with its own running maximum and sum; joined at the end.
-template <int DT>
-__global__ void __launch_bounds__(128) k_kv4_attend(Kv4AttendArgs a) {
-    using T = typename Elem<DT>::T;
-    const int W = a.c.width, NU = W / 32, per = W / 8, NG = W / a.c.group, P = a.c.page;
-    const int seq = blockIdx.z, i = blockIdx.y, hq = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int first = seq * a.max_rows, n = a.max_rows;
-    if (a.starts) first = a.starts[seq], n = a.starts[seq + 1] - first;
-    int len = a.lens[seq];
-    if (first < 0 || n < 0 || n > a.max_rows || first > a.rows - n || len < 0 || len > a.max_len) {
-        if (threadIdx.x == 0) *reinterpret_cast<volatile int *>(a.err) = 1;
-        return;
-    }
-    if (i >= n) return;
-    const int head = hq / (a.q_heads / a.c.heads), row = first + i, pos = len - n + i;
-    const int end = a.causal ? min(len, pos + 1) : len, begin = a.window ? max(0, pos - a.window + 1) : 0;
-    const int part = lane % per, u = part / 4, t = part % 4, keys = 32 / per, mine = lane / per;
-    const size_t hb = kv4_head_bytes(W, P, a.c.group);
-    const Kv4Offsets o = kv4_offsets(W, P, a.c.group);
-    const T *qp = reinterpret_cast<const T *>(a.q) + row * a.q_row + hq * a.q_head + part * 8;
-    float q[8], acc[8] = {}, m = -INFINITY, l = 0.f;
+constexpr int KA_KEYS = 32;     // keys of a warp's step
+constexpr int KA_WARPS = 4;     // warps of a block, each over its own steps of the block's keys
+constexpr int KA_SPLITS = 128;  // most blocks along a sequence
+constexpr int KA_COUNTERS = 16384;  // arrival counters at the start of the working memory: in one place for every call
+
+template <int HD, int G>
+struct KaTile {
+    static constexpr int NU = HD / 32, NG = HD / G;
+    static constexpr int KC = KA_KEYS * HD / 2, SC = KA_KEYS * NG * 4;  // bytes of the codes and of the scales
+    static constexpr int BYTES = 2 * (KC + SC);
+    static constexpr int STAGES = BYTES > 6000 ? 2 : 3;
+};
+
+__device__ __forceinline__ uint32_t ka_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void cp16(void *dst, const void *src, bool on) {
+    const int n = on ? 16 : 0;  // 0: nothing is read, zeros are written
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ka_smem(dst)), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float2 bits_float2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ float exp2_sfu(float x) {  // relative error 2^-22; 0 for -infinity
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| < 127
+
+template <int N>
+__device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) {  // N consecutive words, aligned to 4 N up to 16
+    if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) q[j] = Elem<DT>::get(qp[j]) * a.scale;
-    for (int j0 = begin + warp * keys; j0 < end; j0 += 4 * keys) {
-        const int j = j0 + mine;
-        const int page = j < end ? a.table[seq * a.table_stride + j / P] : 0;
-        const bool ok = j < end && page >= 0 && page < a.c.pages;
-        if (j < end && !ok) *reinterpret_cast<volatile int *>(a.err) = 1;
-        float s = 0.f;
-        const uint8_t *base = a.c.pool + ((size_t)(ok ? page : 0) * a.c.heads + head) * hb;
-        const int at = j % P;
-        if (ok) {
-            const uint32_t c = *(reinterpret_cast<const uint32_t *>(base + (size_t)at * (W / 2)) + t * NU + u);
-            const float2 sc = __half22float2(*(reinterpret_cast<const __half2 *>(base + o.ks) + at * NG + part * 8 / a.c.group));
-#pragma unroll
-            for (int e = 0; e < 8; e++) s += q[e] * value_of(c, e, sc.x, sc.y);
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
         }
-        for (int d = 1; d < per; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if (ok) {
-            const float mn = fmaxf(m, s), f = expf(m - mn), p = expf(s - mn);
-            const uint16_t *vc = reinterpret_cast<const uint16_t *>(base + o.vc + (size_t)at * (W / 2)) + 2 * t * NU + u;
-            const uint32_t c = (uint32_t)vc[0] | (uint32_t)vc[NU] << 16;
-            const float2 sc = __half22float2(*(reinterpret_cast<const __half2 *>(base + o.vs) + at * NG + part * 8 / a.c.group));
-#pragma unroll
-            for (int e = 0; e < 8; e++) acc[e] = acc[e] * f + p * value_of(c, e, sc.x, sc.y);
-            l = l * f + p, m = mn;
-        }
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
     }
-    __shared__ float sm[4][8], sl[4][8], so[4][8][256];
-    if (part == 0) sm[warp][mine] = m, sl[warp][mine] = l;
-#pragma unroll
-    for (int e = 0; e < 8; e++) so[warp][mine][part * 8 + e] = acc[e];
-    __syncthreads();
-    float M = -INFINITY, L = 0.f;
-    for (int w = 0; w < 4; w++)
-        for (int k = 0; k < keys; k++) M = fmaxf(M, sm[w][k]);
-    const float M0 = M == -INFINITY ? 0.f : M;
-    for (int w = 0; w < 4; w++)
-        for (int k = 0; k < keys; k++) L += sl[w][k] * expf(sm[w][k] - M0);
-    T *op = reinterpret_cast<T *>(a.out) + row * a.o_row + hq * a.o_head;
-    for (int c = threadIdx.x; c < W; c += 128) {
-        float x = 0.f;
-        for (int w = 0; w < 4; w++)
-            for (int k = 0; k < keys; k++) x += so[w][k][c] * expf(sm[w][k] - M0);
-        op[c] = Elem<DT>::put(L != 0.f ? x / L : 0.f);  // L is 0 when no key is seen, NaN when a score is
-    }
-    if (a.lse && threadIdx.x == 0) a.lse[(size_t)row * a.q_heads + hq] = M0 + logf(L);
 }
 
-cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, cudaStream_t s, uint64_t *launches) {
-    if (!a.seqs || !a.rows || !a.max_rows) return cudaSuccess;
-    const dim3 grid(a.q_heads, a.max_rows, a.seqs);
-    if (dtype == DT_F32)
-        k_kv4_attend<DT_F32><<<grid, 128, 0, s>>>(a);
-    else if (dtype == DT_F16)
-        k_kv4_attend<DT_F16><<<grid, 128, 0, s>>>(a);
-    else
-        k_kv4_attend<DT_BF16><<<grid, 128, 0, s>>>(a);
-    if (launches) ++*launches;
+// What a sequence's rows of one block see, from the lengths that only the device has.
+struct KaRows {
+    int first, n, len;  // the sequence's first row, its rows and cached tokens
+    bool ok;
+};
+__device__ __forceinline__ KaRows ka_rows(const Kv4AttendArgs &a, int seq) {
+    KaRows r;
+    r.first = seq * a.max_rows, r.n = a.max_rows;
+    if (a.starts) r.first = a.starts[seq], r.n = a.starts[seq + 1] - r.first;
+    r.len = a.lens[seq];
+    r.ok = !(r.first < 0 || r.n < 0 || r.n > a.max_rows || r.first > a.rows - r.n || r.len < 0 || r.len > a.max_len);
+    return r;
+}
+
+// NT * 8 query rows (the rows of the heads that share a cache head, heads innermost) of one sequence and cache head over
+// `chunk` of its keys. SPLIT: q and P' as two f16 (f32 queries), else as one.
+template <int HD, int G, int NT, bool SPLIT>
+__global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, int dtype, int row_tiles, int chunk, float *part,
+                                                              int *arrived) {
+    using C = KaTile<HD, G>;
+    constexpr int NU = C::NU, NG = C::NG, UG = G / 32, R = 8 * NT, ST = C::STAGES, QS = SPLIT ? 2 : 1;
+    extern __shared__ __align__(16) uint8_t sm[];
+    __shared__ int s_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int unit = blockIdx.x, split = blockIdx.y;
+    const int rt = unit % row_tiles, head = unit / row_tiles % a.c.heads, seq = unit / row_tiles / a.c.heads;
+    const KaRows sr = ka_rows(a, seq);
+    if (!sr.ok) {
+        if (tid == 0) *reinterpret_cast<volatile int *>(a.err) = 1;
+        return;
+    }
+    const int each = a.q_heads / a.c.heads, total = sr.n * each, r0 = rt * R, rows = min(R, total - r0);
+    if (rows <= 0) return;
+    // row r of the block: query row i = (r0 + r) / each sees keys [lo(i), hi(i)); both grow with i
+    const int i_first = r0 / each, i_last = (r0 + rows - 1) / each;
+    auto hi_of = [&](int i) { return a.causal ? max(0, min(sr.len, sr.len - sr.n + i + 1)) : sr.len; };
+    auto lo_of = [&](int i) { return a.window ? max(0, sr.len - sr.n + i + 1 - a.window) : 0; };
+    const int lo_min = lo_of(i_first), lo_max = lo_of(i_last), hi_min = hi_of(i_first), hi_max = hi_of(i_last);
+    const int base = lo_min & ~(KA_KEYS - 1);
+    const int nsplits = hi_max > lo_min ? (hi_max - base + chunk - 1) / chunk : 1;
+    if (split >= nsplits) return;
+    const int k0 = base + split * chunk, k1 = hi_max > lo_min ? min(hi_max, k0 + chunk) : k0;
+    const int ntiles = (k1 - k0 + KA_KEYS - 1) / KA_KEYS, mine = (ntiles - warp + KA_WARPS - 1) / KA_WARPS;
+
+    uint8_t *ring = sm + warp * ST * C::BYTES;
+    const size_t hb = kv4_head_bytes(HD, a.c.page, G);
+    const Kv4Offsets off = kv4_offsets(HD, a.c.page, G);
+    const int page_shift = 31 - __clz(a.c.page);
+    // the 32 keys of a step lie on one page, or on two of 16; their numbers are read a step before they are needed
+    int pages[2];
+    auto find = [&](int it) {
+        const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            pages[h] = j0 + 16 * h < k1 ? a.table[seq * a.table_stride + ((j0 + 16 * h) >> page_shift)] : -1;
+    };
+    auto load = [&](int it) {  // this warp's it-th step into its ring
+        if (it < mine) {
+            const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
+            uint8_t *dst = ring + it % ST * C::BYTES;
+            const uint8_t *src[2];
+            bool ok[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int j = j0 + 16 * h, pg = pages[h];
+                ok[h] = pg >= 0 && pg < a.c.pages;
+                if (j < k1 && !ok[h] && (j + 16 > lo_min)) *reinterpret_cast<volatile int *>(a.err) = 1;
+                src[h] = a.c.pool + (ok[h] ? ((size_t)pg * a.c.heads + head) * hb : 0);
+            }
+            find(it + 1);
+            auto copy = [&](int at, int bytes, unsigned from) {
+                const int per = bytes / KA_KEYS;  // bytes of a key
+#pragma unroll
+                for (int b = 0; b < bytes; b += 512) {
+                    const int x = b + lane * 16;
+                    if (bytes % 512 == 0 || x < bytes) {
+                        const int h = x >= bytes / 2, j = j0 + 16 * h, in_page = j & (a.c.page - 1);
+                        cp16(dst + at + x, src[h] + (ok[h] ? from + in_page * per + x - h * (bytes / 2) : 0), ok[h]);
+                    }
+                }
+            };
+            copy(0, C::KC, 0), copy(C::KC, C::SC, off.ks);
+            copy(C::KC + C::SC, C::KC, off.vc), copy(2 * C::KC + C::SC, C::SC, off.vs);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    find(0);
+#pragma unroll
+    for (int it = 0; it < ST - 1; it++) load(it);
+
+    // Q^T fragments: column g of block nt is row nt * 8 + g, scaled by a power of two to at most 2^14; the coordinates of
+    // a word's second nibbles by 1/16 more
+    uint32_t qf[QS][NT][NU][4];
+    float qs[NT][NG][2], fq[NT][2];  // for this thread's columns 2 t, 2 t + 1: the groups' sums, the factor of a score
+    int hi[NT][2], lo[NT][2];
+    const int es = dtype == DT_F32 ? 4 : 2;
+    const bool wide = !(((uintptr_t)a.q & 15) || ((a.q_row | a.q_head) * es) % 16);
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = nt * 8 + g, i = (r0 + r) / each, hq = head * each + (r0 + r) % each;
+        float x[NU][8] = {}, mx = 0.f;
+        if (r < rows) {
+            const long long at = (long long)(sr.first + i) * a.q_row + (long long)hq * a.q_head + 8 * t;
+#pragma unroll
+            for (int u = 0; u < NU; u++) {
+                if (dtype == DT_F32)
+                    load8<DT_F32>(reinterpret_cast<const float *>(a.q) + at + 32 * u, wide, x[u]);
+                else if (dtype == DT_F16)
+                    load8<DT_F16>(reinterpret_cast<const __half *>(a.q) + at + 32 * u, wide, x[u]);
+                else
+                    load8<DT_BF16>(reinterpret_cast<const __nv_bfloat16 *>(a.q) + at + 32 * u, wide, x[u]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[u][j]));
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // mx * 2^e in [2^13, 2^14); queries above 2^114 pass f16 (their scores pass f32)
+        const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
+        const float up = pow2i(e);
+        float sum[NG] = {};
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[u][j] *= up;
+                sum[u / UG] += SPLIT ? x[u][j] : __half2float(__float2half_rn(x[u][j]));
+            }
+#pragma unroll
+            for (int w = 0; w < 4; w++) {  // word w of the unit: coordinates w and w + 4
+                const float f = w & 1 ? 0.0625f : 1.f, x0 = x[u][w] * f, x1 = x[u][w + 4] * f;
+                qf[0][nt][u][w] = half2_bits(x0, x1);
+                if (SPLIT) {
+                    const float2 b = bits_float2(qf[0][nt][u][w]);
+                    qf[QS - 1][nt][u][w] = half2_bits(x0 - b.x, x1 - b.y);
+                }
+            }
+        }
+        const float factor = a.scale * 1.44269504088896340736f * pow2i(-e) * 16777216.f;
+#pragma unroll
+        for (int k = 0; k < NG; k++) {
+            sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
+            sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
+            sum[k] *= 5.9604644775390625e-8f;  // 2^-24, as the products with the codes come
+        }
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const int from = (2 * t + c) * 4;
+            fq[nt][c] = __shfl_sync(0xffffffffu, factor, from);
+#pragma unroll
+            for (int k = 0; k < NG; k++) qs[nt][k][c] = __shfl_sync(0xffffffffu, sum[k], from);
+            const int ic = (r0 + nt * 8 + 2 * t + c) / each;
+            hi[nt][c] = hi_of(ic), lo[nt][c] = lo_of(ic);
+        }
+    }
+
+    // the running state, in units of 2^m for a column (m moves only when a score passes it by 8) and 2^ve for the weights
+    float m[NT][2], l[NT][2], ls[NT][NG][2], o[NT][NU][2][4];
+    float vtop = 0.f, vinv = 1.f;  // the largest step so far rounded up to a power of two, and 2^7 over it
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int k = 0; k < NG; k++) ls[nt][k][0] = ls[nt][k][1] = 0.f;
+#pragma unroll
+        for (int u = 0; u < NU; u++)
+#pragma unroll
+            for (int x = 0; x < 8; x++) o[nt][u][x >> 2][x & 3] = 0.f;
+    }
+
+    for (int it = 0; it < mine; it++) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+        __syncwarp();  // every lane's part has landed, and every lane is done with the slot that is filled next
+        load(it + ST - 1);
+        const uint8_t *tile = ring + it % ST * C::BYTES;
+        const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
+        const bool edge = j0 + KA_KEYS > hi_min || j0 < lo_max;
+        float s[2][NT][4];
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+            uint32_t kw[2][NU], sc[2][NG];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int key = kb * 16 + h * 8 + g;
+                lds_words<NU>(tile + key * (HD / 2) + t * NU * 4, kw[h]);
+                lds_words<NG>(tile + C::KC + key * NG * 4, sc[h]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[kb][nt][c] = 0.f;
+#pragma unroll
+            for (int k = 0; k < NG; k++) {
+                float acc[NT][4] = {};
+#pragma unroll
+                for (int u = k * UG; u < (k + 1) * UG; u++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t w0 = h ? kw[0][u] >> 8 : kw[0][u], w1 = h ? kw[1][u] >> 8 : kw[1][u];
+                        const uint32_t a0 = w0 & 0x000f000fu, a1 = w1 & 0x000f000fu, a2 = w0 & 0x00f000f0u, a3 = w1 & 0x00f000f0u;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int q = QS - 1; q >= 0; q--)
+                                mma16816(acc[nt], a0, a1, a2, a3, qf[q][nt][u][2 * h], qf[q][nt][u][2 * h + 1]);
+                    }
+                const float2 s0 = bits_float2(sc[0][k]), s1 = bits_float2(sc[1][k]);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        s[kb][nt][c] = fmaf(s0.x, acc[nt][c], fmaf(s0.y, qs[nt][k][c], s[kb][nt][c]));
+                        s[kb][nt][c + 2] = fmaf(s1.x, acc[nt][c + 2], fmaf(s1.y, qs[nt][k][c], s[kb][nt][c + 2]));
+                    }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    s[kb][nt][c] *= fq[nt][c & 1];
+                    const int key = j0 + kb * 16 + (c >> 1) * 8 + g;
+                    if (edge && (key >= hi[nt][c & 1] || key < lo[nt][c & 1])) s[kb][nt][c] = -INFINITY;
+                }
+        }
+        // the value scales of this thread's four keys; of keys that no row sees, nothing
+        uint32_t vs[2][2][NG];
+        __half2 smax = __half2half2(__ushort_as_half(0));
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int key = kb * 16 + h * 8 + g;
+                lds_words<NG>(tile + 2 * C::KC + C::SC + key * NG * 4, vs[kb][h]);
+                const bool none = edge && (j0 + key >= hi_max || j0 + key < lo_min);
+#pragma unroll
+                for (int k = 0; k < NG; k++) {
+                    if (none) vs[kb][h][k] = 0;
+                    smax = __hmax2(smax, *reinterpret_cast<const __half2 *>(&vs[kb][h][k]));
+                }
+            }
+        float step_max = __low2float(smax);
+        bool moves = step_max > vtop;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+                moves |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > m[nt][c] + 8.f;
+        if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) step_max = fmaxf(step_max, __shfl_xor_sync(0xffffffffu, step_max, d));
+            float vf = 1.f;
+            if (step_max > vtop) {
+                // the next power of two (steps are positive f16: at least 2^-24)
+                const float top = pow2i((int)(__float_as_uint(step_max) >> 23) - 126);
+                vf = vtop / top, vtop = top, vinv = 128.f / top;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    float x = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    x = fmaxf(x, m[nt][c]);
+                    const float f = x > m[nt][c] ? exp2_sfu(m[nt][c] - x) : 1.f, fo = f * vf;
+                    m[nt][c] = x, l[nt][c] *= f;
+#pragma unroll
+                    for (int k = 0; k < NG; k++) ls[nt][k][c] *= f;
+#pragma unroll
+                    for (int u = 0; u < NU; u++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) o[nt][u][i][c] *= fo, o[nt][u][i][c + 2] *= fo;
+                }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const float mm = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+#pragma unroll
+                for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                    for (int h = 0; h < 4; h += 2) {
+                        const float p = exp2_sfu(s[kb][nt][c + h] - mm);
+                        s[kb][nt][c + h] = p, l[nt][c] += p;
+                    }
+            }
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++) {
+            // the half-words of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9, a pair in one register
+            uint32_t pair[2][NU];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint8_t *p = tile + C::KC + C::SC + (kb * 16 + h * 8 + 2 * t) * (HD / 2) + g * NU * 2;
+                if constexpr (NU == 1) {
+                    pair[h][0] = (uint32_t)*reinterpret_cast<const uint16_t *>(p) |
+                                 (uint32_t)*reinterpret_cast<const uint16_t *>(p + HD / 2) << 16;
+                } else {
+                    uint32_t x[NU / 2], y[NU / 2];
+                    lds_words<NU / 2>(p, x), lds_words<NU / 2>(p + HD / 2, y);
+#pragma unroll
+                    for (int u = 0; u < NU; u++) pair[h][u] = __byte_perm(x[u / 2], y[u / 2], u & 1 ? 0x7632 : 0x5410);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < NG; k++) {
+                const float2 s0 = bits_float2(vs[kb][0][k]), s1 = bits_float2(vs[kb][1][k]);
+                const float w0 = s0.x * vinv, w1 = s1.x * vinv;
+                uint32_t b[QS][NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const float(&p)[4] = s[kb][nt];
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        // a weight of 0 meets a NaN only at a key that its row does not see
+                        const float y0 = edge && p[c] == 0.f ? 0.f : s0.y, y1 = edge && p[c + 2] == 0.f ? 0.f : s1.y;
+                        ls[nt][k][c] = fmaf(p[c], y0, fmaf(p[c + 2], y1, ls[nt][k][c]));
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float w = h ? w1 : w0, p0 = p[2 * h] * w, p1 = p[2 * h + 1] * w;
+                        const uint32_t x = half2_bits(p0, p1);
+                        b[0][nt][h] = transpose8(x);
+                        if (SPLIT) {
+                            const float2 f = bits_float2(x);
+                            b[QS - 1][nt][h] = transpose8(half2_bits(p0 - f.x, p1 - f.y));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = k * UG; u < (k + 1) * UG; u++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const uint32_t x = i ? pair[0][u] >> 8 : pair[0][u], y = i ? pair[1][u] >> 8 : pair[1][u];
+                        const uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int q = QS - 1; q >= 0; q--) mma16816(o[nt][u][i], a0, a1, a2, a3, b[q][nt][0], b[q][nt][1]);
+                    }
+            }
+        }
+    }
+
+    // ---- the warps' states joined ----
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    float *so = reinterpret_cast<float *>(sm);  // [warp][R][HD]
+    float *sms = so + KA_WARPS * R * HD;        // [warp][R]{m, l}
+    const float unv = vtop * (16777216.f / 128.f);
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            float x = l[nt][c], y[NG];
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+#pragma unroll
+            for (int k = 0; k < NG; k++) {
+                y[k] = ls[nt][k][c];
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) y[k] += __shfl_xor_sync(0xffffffffu, y[k], d);
+            }
+            const int r = nt * 8 + 2 * t + c;
+            if (g == 0) sms[(warp * R + r) * 2] = m[nt][c], sms[(warp * R + r) * 2 + 1] = x;
+            float *dst = so + (warp * R + r) * HD + 4 * g;
+#pragma unroll
+            for (int u = 0; u < NU; u++)
+                *reinterpret_cast<float4 *>(dst + 32 * u) =
+                    make_float4(fmaf(o[nt][u][0][c], unv, y[u / UG]), fmaf(o[nt][u][0][c + 2], unv * 0.0625f, y[u / UG]),
+                                fmaf(o[nt][u][1][c], unv, y[u / UG]), fmaf(o[nt][u][1][c + 2], unv * 0.0625f, y[u / UG]));
+        }
+    __syncthreads();
+    auto put = [&](int r, int x, float v) {
+        const int i = (r0 + r) / each, hq = head * each + (r0 + r) % each;
+        const long long at = (long long)(sr.first + i) * a.o_row + (long long)hq * a.o_head + x;
+        if (dtype == DT_F32)
+            reinterpret_cast<float *>(a.out)[at] = v;
+        else if (dtype == DT_F16)
+            reinterpret_cast<__half *>(a.out)[at] = __float2half_rn(v);
+        else
+            reinterpret_cast<__nv_bfloat16 *>(a.out)[at] = __float2bfloat16_rn(v);
+    };
+    auto put_lse = [&](int r, float M, float L) {
+        if (a.lse)
+            a.lse[(size_t)(sr.first + (r0 + r) / each) * a.q_heads + head * each + (r0 + r) % each] =
+                (M + log2f(L)) * 0.69314718055994530942f;
+    };
+    const size_t slot = ((size_t)unit * gridDim.y + split) * R;
+    float *pms = part + 2 * slot, *po = part + 2 * (size_t)gridDim.x * gridDim.y * R + slot * HD;
+    for (int x = tid; x < rows * HD; x += KA_WARPS * 32) {
+        const int r = x / HD, c = x % HD;
+        float M = -INFINITY, L = 0.f, v = 0.f;
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; w++) M = fmaxf(M, sms[(w * R + r) * 2]);
+        const float M0 = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; w++) {
+            const float f = exp2_sfu(sms[(w * R + r) * 2] - M0);
+            L = fmaf(sms[(w * R + r) * 2 + 1], f, L), v = fmaf(so[(w * R + r) * HD + c], f, v);
+        }
+        if (nsplits == 1) {
+            put(r, c, L != 0.f ? v / L : 0.f);  // L is 0 when no key is seen, NaN when a score is
+            if (c == 0) put_lse(r, M0, L);
+        } else {
+            __stcg(po + x, v);
+            if (c == 0) __stcg(pms + 2 * r, M), __stcg(pms + 2 * r + 1, L);
+        }
+    }
+    if (nsplits == 1) return;
+    // ---- the last block of the row tile to arrive joins the blocks' states, in their order ----
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+        s_last = atomicAdd(arrived + unit, 1) == nsplits - 1;
+        if (s_last) arrived[unit] = 0;  // ready for the next call
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    float *wt = reinterpret_cast<float *>(sm);  // [nsplits][rows] weights, then [rows]{1 / sum}
+    const float *ams = part + 2 * (size_t)unit * gridDim.y * R;
+    for (int r = warp; r < rows; r += KA_WARPS) {
+        float M = -INFINITY, L = 0.f;
+        for (int p = lane; p < nsplits; p += 32) M = fmaxf(M, __ldcg(ams + 2 * ((size_t)p * R + r)));
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+        const float M0 = M == -INFINITY ? 0.f : M;
+        for (int p = lane; p < nsplits; p += 32) {
+            const float2 x = __ldcg(reinterpret_cast<const float2 *>(ams) + (size_t)p * R + r);
+            const float f = exp2_sfu(x.x - M0);
+            wt[p * rows + r] = f, L = fmaf(x.y, f, L);
+        }
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) L += __shfl_xor_sync(0xffffffffu, L, d);
+        if (lane == 0) {
+            wt[nsplits * rows + r] = L != 0.f ? 1.f / L : 0.f;
+            put_lse(r, M0, L);
+        }
+    }
+    __syncthreads();
+    const float *ao = part + 2 * (size_t)gridDim.x * gridDim.y * R + (size_t)unit * gridDim.y * R * HD;
+    for (int x = tid; x < rows * HD; x += KA_WARPS * 32) {
+        const int r = x / HD;
+        float v = 0.f;
+        for (int p0 = 0; p0 < nsplits; p0 += 8) {
+            float y[8];
+#pragma unroll
+            for (int p = 0; p < 8; p++) y[p] = p0 + p < nsplits ? __ldcg(ao + (size_t)(p0 + p) * R * HD + x) : 0.f;
+#pragma unroll
+            for (int p = 0; p < 8; p++)
+                if (p0 + p < nsplits) v = fmaf(y[p], wt[(p0 + p) * rows + r], v);
+        }
+        put(r, x % HD, v * wt[nsplits * rows + r]);
+    }
+}
+
+struct KaPlan {
+    int nt, row_tiles, units, chunk, splits;
+};
+static KaPlan ka_plan(int dtype, const Kv4AttendArgs &a, int sms) {
+    KaPlan p;
+    const int rows = a.max_rows * (a.q_heads / a.c.heads);
+    // 16 rows a block where their fragments of q and of the output fit the registers
+    p.nt = rows > 8 && a.c.width * (dtype == DT_F32 ? 2 : 1) <= 128 ? 2 : 1;
+    p.row_tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
+    p.units = a.seqs * a.c.heads * p.row_tiles;
+    const int span = a.window ? (int)std::min<long long>(a.max_len, (long long)a.window + a.max_rows + KA_KEYS - 1) : a.max_len;
+    const int step = KA_WARPS * KA_KEYS, most = std::max(1, (span + step - 1) / step);  // steps of the longest
+    // enough blocks for two on every SM, at least one step of every warp a block and at most eight (a long sequence's
+    // blocks then start and end at different times, which hides their first loads and their joins)
+    int per = (int)std::min<long long>(8, ((long long)most * p.units + 2 * sms - 1) / (2 * sms));
+    per = std::max({per, 1, (most + KA_SPLITS - 1) / KA_SPLITS});
+    if (p.units > KA_COUNTERS) per = most;
+    p.chunk = per * step;
+    p.splits = (most + per - 1) / per;
+    return p;
+}
+
+static size_t ka_work_bytes(const Kv4AttendArgs &a, const KaPlan &p) {
+    return p.splits == 1 ? 0 : 4 * (KA_COUNTERS + (size_t)p.units * p.splits * 8 * p.nt * (a.c.width + 2));
+}
+size_t kv4_attend_workspace(int dtype, const Kv4AttendArgs &a, int sms) {
+    // A window shortens the span, and shorter spans are cut finer, up to two blocks an SM.
+    KaPlan p = ka_plan(dtype, a, sms);
+    const int most = (a.max_len + KA_WARPS * KA_KEYS - 1) / (KA_WARPS * KA_KEYS);
+    p.splits = std::max(p.splits, std::min({most, KA_SPLITS, 2 * sms / std::max(1, p.units) + 1}));
+    return ka_work_bytes(a, p);
+}
+
+template <int HD, int G, int NT, bool SPLIT>
+static cudaError_t launch_one(int dtype, const Kv4AttendArgs &a, const KaPlan &p, void *work, cudaStream_t s) {
+    using C = KaTile<HD, G>;
+    const size_t join = sizeof(float) * KA_WARPS * 8 * NT * (HD + 2);
+    const size_t smem = std::max({(size_t)KA_WARPS * C::STAGES * C::BYTES, join, sizeof(float) * 8 * NT * (KA_SPLITS + 2)});
+    cudaError_t e = allow_dynamic_smem((const void *)k_kv4_attend<HD, G, NT, SPLIT>, smem);
+    if (e != cudaSuccess) return e;
+    int *arrived = reinterpret_cast<int *>(work);
+    float *part = reinterpret_cast<float *>(work) + KA_COUNTERS;
+    k_kv4_attend<HD, G, NT, SPLIT><<<dim3(p.units, p.splits), KA_WARPS * 32, smem, s>>>(a, dtype, p.row_tiles, p.chunk, part, arrived);
     return cudaGetLastError();
+}
+template <int HD, int G>
+static cudaError_t launch_size(int dtype, const Kv4AttendArgs &a, const KaPlan &p, void *work, cudaStream_t s) {
+    const bool split = dtype == DT_F32;
+    if constexpr (HD <= 64) {
+        if (p.nt == 2 && split) return launch_one<HD, G, 2, true>(dtype, a, p, work, s);
+    }
+    if constexpr (HD <= 128) {
+        if (p.nt == 2) return launch_one<HD, G, 2, false>(dtype, a, p, work, s);
+    }
+    return split ? launch_one<HD, G, 1, true>(dtype, a, p, work, s) : launch_one<HD, G, 1, false>(dtype, a, p, work, s);
+}
+
+cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *work, size_t work_bytes, cudaStream_t s, uint64_t *launches) {
+    if (!a.seqs || !a.rows || !a.max_rows) return cudaSuccess;
+    const KaPlan p = ka_plan(dtype, a, sms);
+    if (ka_work_bytes(a, p) > work_bytes) return cudaErrorInvalidValue;
+    cudaError_t e = cudaErrorInvalidValue;
+    const int w = a.c.width, g = a.c.group;
+    if (w == 32) e = launch_size<32, 32>(dtype, a, p, work, s);
+    if (w == 64) e = g == 32 ? launch_size<64, 32>(dtype, a, p, work, s) : launch_size<64, 64>(dtype, a, p, work, s);
+    if (w == 128)
+        e = g == 32 ? launch_size<128, 32>(dtype, a, p, work, s)
+                    : g == 64 ? launch_size<128, 64>(dtype, a, p, work, s) : launch_size<128, 128>(dtype, a, p, work, s);
+    if (w == 256)
+        e = g == 32 ? launch_size<256, 32>(dtype, a, p, work, s)
+                    : g == 64 ? launch_size<256, 64>(dtype, a, p, work, s) : launch_size<256, 128>(dtype, a, p, work, s);
+    if (launches) ++*launches;
+    return e;
 }
 
 }  // namespace tcu

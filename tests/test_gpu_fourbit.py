@@ -535,3 +535,17 @@ def test_logprobs_refusals(gpu):
         with pytest.raises(tcu.TcuError, match=match):
             gpu.label_logprobs(*a, stream=1, **kw)
     gpu.label_logprobs(0, None, 0, 4, 4, None, 1, None)
+
+
+def test_attend_shares_working_memory_between_calls_of_different_shape(gpu):
+    """One block of working memory, calls that split their sequences differently one after the other."""
+    shapes = [([5000], 1, 1, [1]), ([300] * 40, 4, 8, [1] * 40), ([9000, 10], 2, 4, [1, 1]), ([2000], 1, 8, [3])]
+    caches = [Cached(gpu, i, lens, h, 64, 64, 32) for i, (lens, h, _, _) in enumerate(shapes)]
+    work = torch.zeros(64 << 20, dtype=torch.uint8, device="cuda")
+    for turn in range(2):
+        for c, (lens, h, hq, counts) in zip(caches, shapes):
+            q = rounded(np.random.default_rng(turn).normal(0, 1, (sum(counts), hq, 64)), torch.bfloat16)
+            for window in (0, 700):
+                out, lse = c.attend("bf16", q, counts, 0.125, causal=True, window=window, work=work)
+                sync(gpu)
+                c.check("bf16", q, counts, 0.125, True, window, out, lse)
