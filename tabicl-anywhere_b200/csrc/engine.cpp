@@ -3435,7 +3435,7 @@ int tcu_label_logprobs_device(tcu_ctx *ctx, int dtype, const void *logits, int r
         a.inv_t = (float)(1.0 / temperature), a.out = out, a.entropy = entropy, a.top_values = top_values, a.top_ids = top_ids;
         a.err = ctx->err_mapped + ERR_INDEX;
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
-        Launch{ctx, s}(launch_logprobs(dtype, a, s, &ctx->launches), "label_logprobs");
+        Launch{ctx, s}(launch_logprobs(dtype, a, ctx->sms, s, &ctx->launches), "label_logprobs");
         return TCU_OK;
     });
 }

@@ -101,7 +101,7 @@ cudaError_t allow_dynamic_smem(const void *kernel, size_t bytes);
 cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k, int group, uint8_t *codes,
                            __half2 *scales, cudaStream_t s, uint64_t *launches);
 cudaError_t launch_w4_linear(int dtype, const W4Args &a, cudaStream_t s, uint64_t *launches);
-cudaError_t launch_logprobs(int dtype, const LogprobArgs &a, cudaStream_t s, uint64_t *launches);
+cudaError_t launch_logprobs(int dtype, const LogprobArgs &a, int sms, cudaStream_t s, uint64_t *launches);
 
 #ifdef __CUDACC__
 
