@@ -3407,7 +3407,7 @@ int tcu_w4_linear_device(tcu_ctx *ctx, const tcu_w4 *w, int dtype, int rows, con
         check_aligned("w4_linear", "bias", bias, elem_size(dtype)), check_aligned("w4_linear", "residual", residual, elem_size(dtype));
         a.x = x, a.ldx = ldx, a.y = y, a.ldy = ldy, a.bias = bias, a.act = act, a.residual = residual, a.ldr = ldr;
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
-        Launch{ctx, s}(launch_w4_linear(dtype, a, s, &ctx->launches), "w4_linear");
+        Launch{ctx, s}(launch_w4_linear(dtype, a, ctx->sms, s, &ctx->launches), "w4_linear");
         return TCU_OK;
     });
 }

@@ -100,7 +100,7 @@ cudaError_t allow_dynamic_smem(const void *kernel, size_t bytes);
 // A weight matrix w [n][k] (row stride ldw) to codes and scales.
 cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k, int group, uint8_t *codes,
                            __half2 *scales, cudaStream_t s, uint64_t *launches);
-cudaError_t launch_w4_linear(int dtype, const W4Args &a, cudaStream_t s, uint64_t *launches);
+cudaError_t launch_w4_linear(int dtype, const W4Args &a, int sms, cudaStream_t s, uint64_t *launches);
 cudaError_t launch_logprobs(int dtype, const LogprobArgs &a, int sms, cudaStream_t s, uint64_t *launches);
 
 #ifdef __CUDACC__
