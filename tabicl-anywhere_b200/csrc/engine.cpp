@@ -3341,6 +3341,7 @@ int tcu_kv4_attend_device(tcu_ctx *ctx, const tcu_kv4 *cache, const tcu_kv4_batc
         check_aligned("kv4_attend", "starts", a.starts, 4), check_aligned("kv4_attend", "lse", lse, 4);
         a.q = q, a.out = out, a.q_row = q_row, a.q_head = q_head, a.o_row = o_row, a.o_head = o_head;
         a.scale = scale, a.causal = causal != 0, a.window = window, a.lse = lse, a.err = ctx->err_mapped + ERR_INDEX;
+        a.err_wait = ctx->err_mapped + ERR_ATTEND_TC;
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
         const size_t need = kv4_attend_workspace(dtype, a, ctx->sms);
         if (need && (!work || work_bytes < need)) fail(TCU_ERR_ARG, "kv4_attend: needs " + std::to_string(need) + " bytes of working memory");

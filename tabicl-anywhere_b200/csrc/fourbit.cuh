@@ -64,6 +64,7 @@ struct Kv4AttendArgs {
     int causal = 0, window = 0;
     float *lse = nullptr;  // [rows][q_heads], or null
     int *err = nullptr;    // report slot: set to 1 on a length, start or page outside its range
+    int *err_wait = nullptr;  // report slot: set to 1 when a kernel gave up waiting
 };
 
 // y = act(x W^T + bias) + residual with four-bit weights.

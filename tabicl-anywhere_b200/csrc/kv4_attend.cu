@@ -16,6 +16,7 @@ namespace tcu {
 constexpr int KA_KEYS = 32;     // keys of a warp's step
 constexpr int KA_WARPS = 4;     // warps of a block, each over its own steps of the block's keys
 constexpr int KA_SPLITS = 128;  // most blocks along a sequence
+constexpr long long KA_WAIT = 2000000000ll;  // cycles (about a second) that a warp waits for a copy before it gives up
 constexpr int KA_COUNTERS = 16384;  // arrival counters at the start of the working memory: in one place for every call
 
 template <int HD, int G>
@@ -24,18 +25,28 @@ struct KaTile {
     static constexpr int KC = KA_KEYS * HD / 2, SC = KA_KEYS * NG * 4;  // bytes of the codes and of the scales
     static constexpr int BYTES = 2 * (KC + SC);
     static constexpr int STAGES = BYTES > 6000 ? 2 : 3;
+    // the `low` part of the scores as a matrix product of the keys' lows with the groups' sums of q (as f16 hi and lo):
+    // one fragment of NG hi and NG lo columns; with one or two groups the multiply-adds are as few
+    static constexpr bool LOW_MMA = NG >= 4;
 };
 
 __device__ __forceinline__ uint32_t ka_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp16(void *dst, const void *src, bool on) {
-    const int n = on ? 16 : 0;  // 0: nothing is read, zeros are written
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(ka_smem(dst)), "l"(src), "r"(n) : "memory");
+// `bytes` (a multiple of 16) from global to shared memory, both 16-byte aligned; they count on the barrier.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma1688(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(b0));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -93,6 +104,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
     constexpr int NU = C::NU, NG = C::NG, UG = G / 32, R = 8 * NT, ST = C::STAGES, QS = SPLIT ? 2 : 1;
     extern __shared__ __align__(16) uint8_t sm[];
     __shared__ int s_last;
+    __shared__ __align__(8) unsigned long long bars[KA_WARPS][ST];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int unit = blockIdx.x, split = blockIdx.y;
     const int rt = unit % row_tiles, head = unit / row_tiles % a.c.heads, seq = unit / row_tiles / a.c.heads;
@@ -114,47 +126,48 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
     const int k0 = base + split * chunk, k1 = hi_max > lo_min ? min(hi_max, k0 + chunk) : k0;
     const int ntiles = (k1 - k0 + KA_KEYS - 1) / KA_KEYS, mine = (ntiles - warp + KA_WARPS - 1) / KA_WARPS;
 
+    // this warp's ring: each step's key codes, key scales, value codes and value scales come as four bulk copies (eight
+    // when the 32 keys lie on two pages of 16), one a lane, that count on the slot's barrier
     uint8_t *ring = sm + warp * ST * C::BYTES;
+    const uint32_t ring_at = ka_smem(ring), bar_at = ka_smem(&bars[warp][0]);
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < ST; i++) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar_at + 8 * i) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
     const size_t hb = kv4_head_bytes(HD, a.c.page, G);
     const Kv4Offsets off = kv4_offsets(HD, a.c.page, G);
-    const int page_shift = 31 - __clz(a.c.page);
-    // the 32 keys of a step lie on one page, or on two of 16; their numbers are read a step before they are needed
+    const int page_shift = 31 - __clz(a.c.page), halves = a.c.page == 16 ? 2 : 1;
+    const int cpart = lane & 3, chalf = (lane >> 2) & 1;
+    const uint32_t from = (cpart & 2 ? off.vc : 0) + (cpart & 1 ? off.ks : 0);  // ks = vs - vc: the codes before the scales
+    const uint32_t per_key = cpart & 1 ? NG * 4 : HD / 2, copy_bytes = per_key * KA_KEYS / halves;
+    const uint32_t to = (cpart & 2 ? C::KC + C::SC : 0) + (cpart & 1 ? C::KC : 0) + chalf * copy_bytes;
+    // the page numbers are read a step before they are needed
     int pages[2];
     auto find = [&](int it) {
         const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            pages[h] = j0 + 16 * h < k1 ? a.table[seq * a.table_stride + ((j0 + 16 * h) >> page_shift)] : -1;
+            pages[h] = h < halves && j0 + 16 * h < k1 ? a.table[seq * a.table_stride + ((j0 + 16 * h) >> page_shift)] : -1;
     };
     auto load = [&](int it) {  // this warp's it-th step into its ring
-        if (it < mine) {
-            const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
-            uint8_t *dst = ring + it % ST * C::BYTES;
-            const uint8_t *src[2];
-            bool ok[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int j = j0 + 16 * h, pg = pages[h];
-                ok[h] = pg >= 0 && pg < a.c.pages;
-                if (j < k1 && !ok[h] && (j + 16 > lo_min)) *reinterpret_cast<volatile int *>(a.err) = 1;
-                src[h] = a.c.pool + (ok[h] ? ((size_t)pg * a.c.heads + head) * hb : 0);
-            }
-            find(it + 1);
-            auto copy = [&](int at, int bytes, unsigned from) {
-                const int per = bytes / KA_KEYS;  // bytes of a key
-#pragma unroll
-                for (int b = 0; b < bytes; b += 512) {
-                    const int x = b + lane * 16;
-                    if (bytes % 512 == 0 || x < bytes) {
-                        const int h = x >= bytes / 2, j = j0 + 16 * h, in_page = j & (a.c.page - 1);
-                        cp16(dst + at + x, src[h] + (ok[h] ? from + in_page * per + x - h * (bytes / 2) : 0), ok[h]);
-                    }
-                }
-            };
-            copy(0, C::KC, 0), copy(C::KC, C::SC, off.ks);
-            copy(C::KC + C::SC, C::KC, off.vc), copy(2 * C::KC + C::SC, C::SC, off.vs);
+        if (it >= mine) return;
+        const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
+        const bool ok0 = pages[0] >= 0 && pages[0] < a.c.pages, ok1 = pages[1] >= 0 && pages[1] < a.c.pages;
+        const uint32_t bar = bar_at + 8 * (it % ST);
+        if (lane == 0) {
+            if ((!ok0 && j0 + KA_KEYS / halves > lo_min) || (halves == 2 && !ok1 && j0 + 16 < k1 && j0 + KA_KEYS > lo_min))
+                *reinterpret_cast<volatile int *>(a.err) = 1;
+            const uint32_t bytes = C::BYTES / halves * ((int)ok0 + (int)ok1);
+            asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}\n" ::"r"(bar), "r"(bytes) : "memory");
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (lane < 4 * halves && (chalf ? ok1 : ok0)) {
+            const uint8_t *src = a.c.pool + ((size_t)(chalf ? pages[1] : pages[0]) * a.c.heads + head) * hb + from +
+                                 ((j0 + 16 * chalf) & (a.c.page - 1)) * per_key;
+            bulk_copy(ring_at + it % ST * C::BYTES + to, src, copy_bytes, bar);
+        }
+        find(it + 1);
     };
     find(0);
 #pragma unroll
@@ -163,7 +176,9 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
     // Q^T fragments: column g of block nt is row nt * 8 + g, scaled by a power of two to at most 2^14; the coordinates of
     // a word's second nibbles by 1/16 more
     uint32_t qf[QS][NT][NU][4];
-    float qs[NT][NG][2], fq[NT][2];  // for this thread's columns 2 t, 2 t + 1: the groups' sums, the factor of a score
+    float fq[NT][2];                                // for this thread's columns 2 t, 2 t + 1: the factor of a score
+    float qs[NT][C::LOW_MMA ? 1 : NG][2];           // and the groups' sums,
+    uint32_t qlow[NT][2];                           // or their fragments: hi and lo of the sums times 2^-6
     int hi[NT][2], lo[NT][2];
     const int es = dtype == DT_F32 ? 4 : 2;
     const bool wide = !(((uintptr_t)a.q & 15) || ((a.q_row | a.q_head) * es) % 16);
@@ -213,14 +228,31 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
         for (int k = 0; k < NG; k++) {
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
-            sum[k] *= 5.9604644775390625e-8f;  // 2^-24, as the products with the codes come
+            sum[k] *= C::LOW_MMA ? 0.015625f : 5.9604644775390625e-8f;  // 2^-24: as the products with the codes come
+        }
+        if constexpr (C::LOW_MMA) {
+            uint32_t hi2[NG / 2], lo2[NG / 2];
+#pragma unroll
+            for (int k = 0; k < NG; k += 2) {
+                hi2[k / 2] = half2_bits(sum[k], sum[k + 1]);
+                const float2 b = bits_float2(hi2[k / 2]);
+                lo2[k / 2] = half2_bits(sum[k] - b.x, sum[k + 1] - b.y);
+            }
+            if constexpr (NG == 4) {  // columns 0-3 hi, 4-7 lo
+                qlow[nt][0] = t & 2 ? (t & 1 ? lo2[1] : lo2[0]) : (t & 1 ? hi2[1] : hi2[0]);
+            } else {  // columns 0-7 hi, 8-15 lo
+                qlow[nt][0] = t & 2 ? (t & 1 ? hi2[3] : hi2[2]) : (t & 1 ? hi2[1] : hi2[0]);
+                qlow[nt][1] = t & 2 ? (t & 1 ? lo2[3] : lo2[2]) : (t & 1 ? lo2[1] : lo2[0]);
+            }
         }
 #pragma unroll
         for (int c = 0; c < 2; c++) {
-            const int from = (2 * t + c) * 4;
-            fq[nt][c] = __shfl_sync(0xffffffffu, factor, from);
+            const int who = (2 * t + c) * 4;
+            fq[nt][c] = __shfl_sync(0xffffffffu, factor, who);
+            if constexpr (!C::LOW_MMA) {
 #pragma unroll
-            for (int k = 0; k < NG; k++) qs[nt][k][c] = __shfl_sync(0xffffffffu, sum[k], from);
+                for (int k = 0; k < NG; k++) qs[nt][k][c] = __shfl_sync(0xffffffffu, sum[k], who);
+            }
             const int ic = (r0 + nt * 8 + 2 * t + c) / each;
             hi[nt][c] = hi_of(ic), lo[nt][c] = lo_of(ic);
         }
@@ -240,10 +272,23 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
             for (int x = 0; x < 8; x++) o[nt][u][x >> 2][x & 3] = 0.f;
     }
 
+    __half2 vnorm = __float2half2_rn(1.f);  // one f16 of the weights: steps times 2^-ve (as far as f16 goes), weights times 2^7
+    bool gave_up = false;
     for (int it = 0; it < mine; it++) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
-        __syncwarp();  // every lane's part has landed, and every lane is done with the slot that is filled next
         load(it + ST - 1);
+        {
+            const uint32_t bar = bar_at + 8 * (it % ST), parity = (it / ST) & 1;
+            const long long began = clock64();
+            uint32_t done = 0;
+            while (!done) {
+                asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+                if (!done && clock64() - began > KA_WAIT) break;
+            }
+            if (__any_sync(0xffffffffu, !done)) {
+                gave_up = true;
+                break;
+            }
+        }
         const uint8_t *tile = ring + it % ST * C::BYTES;
         const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
         const bool edge = j0 + KA_KEYS > hi_min || j0 < lo_max;
@@ -257,10 +302,23 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                 lds_words<NU>(tile + key * (HD / 2) + t * NU * 4, kw[h]);
                 lds_words<NG>(tile + C::KC + key * NG * 4, sc[h]);
             }
+            float low[NT][4];
+            if constexpr (C::LOW_MMA) {
+                uint32_t lows[2];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                for (int h = 0; h < 2; h++) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(tile + C::KC + (kb * 16 + h * 8 + g) * NG * 4 + (NG == 4 ? t & 1 : t) * 8);
+                    lows[h] = __byte_perm(v.x, v.y, 0x7632);
+                }
 #pragma unroll
-                for (int c = 0; c < 4; c++) s[kb][nt][c] = 0.f;
+                for (int nt = 0; nt < NT; nt++) {
+                    low[nt][0] = low[nt][1] = low[nt][2] = low[nt][3] = 0.f;
+                    if constexpr (NG == 4)
+                        mma1688(low[nt], lows[0], lows[1], qlow[nt][0]);
+                    else
+                        mma16816(low[nt], lows[0], lows[1], lows[0], lows[1], qlow[nt][0], qlow[nt][1]);
+                }
+            }
 #pragma unroll
             for (int k = 0; k < NG; k++) {
                 float acc[NT][4] = {};
@@ -281,8 +339,14 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        s[kb][nt][c] = fmaf(s0.x, acc[nt][c], fmaf(s0.y, qs[nt][k][c], s[kb][nt][c]));
-                        s[kb][nt][c + 2] = fmaf(s1.x, acc[nt][c + 2], fmaf(s1.y, qs[nt][k][c], s[kb][nt][c + 2]));
+                        float &x = s[kb][nt][c], &y = s[kb][nt][c + 2];
+                        if constexpr (C::LOW_MMA) {
+                            x = k ? fmaf(s0.x, acc[nt][c], x) : s0.x * acc[nt][c];
+                            y = k ? fmaf(s1.x, acc[nt][c + 2], y) : s1.x * acc[nt][c + 2];
+                        } else {
+                            x = fmaf(s0.x, acc[nt][c], k ? fmaf(s0.y, qs[nt][k][c], x) : s0.y * qs[nt][k][c]);
+                            y = fmaf(s1.x, acc[nt][c + 2], k ? fmaf(s1.y, qs[nt][k][c], y) : s1.y * qs[nt][k][c]);
+                        }
                     }
                 }
             }
@@ -290,27 +354,37 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
+                    // the lows' products are 2^18 times the codes'
+                    if constexpr (C::LOW_MMA) s[kb][nt][c] = fmaf(low[nt][c], 3.814697265625e-6f, s[kb][nt][c]);
                     s[kb][nt][c] *= fq[nt][c & 1];
-                    const int key = j0 + kb * 16 + (c >> 1) * 8 + g;
-                    if (edge && (key >= hi[nt][c & 1] || key < lo[nt][c & 1])) s[kb][nt][c] = -INFINITY;
                 }
         }
-        // the value scales of this thread's four keys; of keys that no row sees, nothing
+        // the value scales of this thread's four keys
         uint32_t vs[2][2][NG];
-        __half2 smax = __half2half2(__ushort_as_half(0));
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int key = kb * 16 + h * 8 + g;
-                lds_words<NG>(tile + 2 * C::KC + C::SC + key * NG * 4, vs[kb][h]);
-                const bool none = edge && (j0 + key >= hi_max || j0 + key < lo_min);
+            for (int h = 0; h < 2; h++) lds_words<NG>(tile + 2 * C::KC + C::SC + (kb * 16 + h * 8 + g) * NG * 4, vs[kb][h]);
+        if (edge) {  // keys that a row does not see; of those that none sees, the scales may be anything
 #pragma unroll
-                for (int k = 0; k < NG; k++) {
-                    if (none) vs[kb][h][k] = 0;
-                    smax = __hmax2(smax, *reinterpret_cast<const __half2 *>(&vs[kb][h][k]));
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int key = j0 + kb * 16 + h * 8 + g;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++)
+                            if (key >= hi[nt][c] || key < lo[nt][c]) s[kb][nt][2 * h + c] = -INFINITY;
+                    if (key >= hi_max || key < lo_min) {
+#pragma unroll
+                        for (int k = 0; k < NG; k++) vs[kb][h][k] = 0;
+                    }
                 }
-            }
+        }
+        __half2 smax = *reinterpret_cast<const __half2 *>(&vs[0][0][0]);
+#pragma unroll
+        for (int i = 1; i < 4 * NG; i++) smax = __hmax2(smax, *reinterpret_cast<const __half2 *>(&vs[i / (2 * NG)][i / NG % 2][i % NG]));
         float step_max = __low2float(smax);
         bool moves = step_max > vtop;
 #pragma unroll
@@ -324,8 +398,10 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
             float vf = 1.f;
             if (step_max > vtop) {
                 // the next power of two (steps are positive f16: at least 2^-24)
-                const float top = pow2i((int)(__float_as_uint(step_max) >> 23) - 126);
+                const int e = (int)(__float_as_uint(step_max) >> 23) - 126;
+                const float top = SPLIT ? pow2i(e) : pow2i(max(e, -15));
                 vf = vtop / top, vtop = top, vinv = 128.f / top;
+                vnorm = __float2half2_rn(1.f / top);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -358,6 +434,23 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                         s[kb][nt][c + h] = p, l[nt][c] += p;
                     }
             }
+        // sum p low
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int k = 0; k < NG; k++) {
+                const float y0 = bits_float2(vs[kb][0][k]).y, y1 = bits_float2(vs[kb][1][k]).y;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const float p0 = s[kb][nt][c], p1 = s[kb][nt][c + 2];
+                        if (edge)  // a weight of 0 meets a NaN only at a key that its row does not see
+                            ls[nt][k][c] = fmaf(p0, p0 == 0.f ? 0.f : y0, fmaf(p1, p1 == 0.f ? 0.f : y1, ls[nt][k][c]));
+                        else
+                            ls[nt][k][c] = fmaf(p0, y0, fmaf(p1, y1, ls[nt][k][c]));
+                    }
+            }
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
             // the half-words of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9, a pair in one register
@@ -375,28 +468,36 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                     for (int u = 0; u < NU; u++) pair[h][u] = __byte_perm(x[u / 2], y[u / 2], u & 1 ? 0x7632 : 0x5410);
                 }
             }
+            __half2 p2[NT][2];
+            if (!SPLIT) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) p2[nt][h] = __floats2half2_rn(s[kb][nt][2 * h] * 128.f, s[kb][nt][2 * h + 1] * 128.f);
+            }
 #pragma unroll
             for (int k = 0; k < NG; k++) {
-                const float2 s0 = bits_float2(vs[kb][0][k]), s1 = bits_float2(vs[kb][1][k]);
-                const float w0 = s0.x * vinv, w1 = s1.x * vinv;
                 uint32_t b[QS][NT][2];
+                if constexpr (SPLIT) {
+                    const float w[2] = {bits_float2(vs[kb][0][k]).x * vinv, bits_float2(vs[kb][1][k]).x * vinv};
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const float(&p)[4] = s[kb][nt];
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        // a weight of 0 meets a NaN only at a key that its row does not see
-                        const float y0 = edge && p[c] == 0.f ? 0.f : s0.y, y1 = edge && p[c + 2] == 0.f ? 0.f : s1.y;
-                        ls[nt][k][c] = fmaf(p[c], y0, fmaf(p[c + 2], y1, ls[nt][k][c]));
-                    }
+                        for (int h = 0; h < 2; h++) {
+                            const float p0 = s[kb][nt][2 * h] * w[h], p1 = s[kb][nt][2 * h + 1] * w[h];
+                            const uint32_t x = half2_bits(p0, p1);
+                            const float2 f = bits_float2(x);
+                            b[0][nt][h] = transpose8(x), b[QS - 1][nt][h] = transpose8(half2_bits(p0 - f.x, p1 - f.y));
+                        }
+                } else {
+                    // one f16 of p 2^7 times one of the step: each rounds to 11 bits, as the results are to 11 or 8
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const float w = h ? w1 : w0, p0 = p[2 * h] * w, p1 = p[2 * h + 1] * w;
-                        const uint32_t x = half2_bits(p0, p1);
-                        b[0][nt][h] = transpose8(x);
-                        if (SPLIT) {
-                            const float2 f = bits_float2(x);
-                            b[QS - 1][nt][h] = transpose8(half2_bits(p0 - f.x, p1 - f.y));
+                        const __half2 w = __hmul2(__low2half2(*reinterpret_cast<const __half2 *>(&vs[kb][h][k])), vnorm);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            const __half2 x = __hmul2(p2[nt][h], w);
+                            b[0][nt][h] = transpose8(*reinterpret_cast<const uint32_t *>(&x));
                         }
                     }
                 }
@@ -413,10 +514,11 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                     }
             }
         }
+        __syncwarp();  // every lane is done with the slot that the next load fills
     }
+    if (gave_up && lane == 0) *reinterpret_cast<volatile int *>(a.err_wait) = 1;
 
     // ---- the warps' states joined ----
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
     float *so = reinterpret_cast<float *>(sm);  // [warp][R][HD]
     float *sms = so + KA_WARPS * R * HD;        // [warp][R]{m, l}
@@ -540,9 +642,9 @@ static KaPlan ka_plan(int dtype, const Kv4AttendArgs &a, int sms) {
     p.units = a.seqs * a.c.heads * p.row_tiles;
     const int span = a.window ? (int)std::min<long long>(a.max_len, (long long)a.window + a.max_rows + KA_KEYS - 1) : a.max_len;
     const int step = KA_WARPS * KA_KEYS, most = std::max(1, (span + step - 1) / step);  // steps of the longest
-    // enough blocks for two on every SM, at least one step of every warp a block and at most eight (a long sequence's
+    // enough blocks for two on every SM, at least one step of every warp a block and at most sixteen (a long sequence's
     // blocks then start and end at different times, which hides their first loads and their joins)
-    int per = (int)std::min<long long>(8, ((long long)most * p.units + 2 * sms - 1) / (2 * sms));
+    int per = (int)std::min<long long>(16, ((long long)most * p.units + 2 * sms - 1) / (2 * sms));
     per = std::max({per, 1, (most + KA_SPLITS - 1) / KA_SPLITS});
     if (p.units > KA_COUNTERS) per = most;
     p.chunk = per * step;
