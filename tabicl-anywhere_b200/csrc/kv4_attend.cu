@@ -8,6 +8,7 @@
 // Per 32 keys a warp computes S^T = K Q^T with 16 keys as rows and 8 query rows as columns, so a key's codes are read in
 // the order they are stored in, and O^T = V^T P'^T with P' = p * step turned round in registers (movmatrix).
 #include <algorithm>
+#include <atomic>
 
 #include "fourbit.cuh"
 
@@ -15,9 +16,9 @@ namespace tcu {
 
 constexpr int KA_KEYS = 32;     // keys of a warp's step
 constexpr int KA_WARPS = 4;     // warps of a block, each over its own steps of the block's keys
-constexpr int KA_SPLITS = 128;  // most blocks along a sequence
-constexpr long long KA_WAIT = 2000000000ll;  // cycles (about a second) that a warp waits for a copy before it gives up
-constexpr int KA_COUNTERS = 16384;  // arrival counters at the start of the working memory: in one place for every call
+constexpr int KA_STEP = KA_WARPS * KA_KEYS;  // keys of a block's step
+constexpr int KA_TRIES = 1 << 20;  // waits for a copy (each suspends the warp for a while) before a warp gives up
+constexpr int KA_BLOCKS = 2048;  // most blocks of a launch: as many arrival counters start the working memory of every call
 
 template <int HD, int G>
 struct KaTile {
@@ -95,36 +96,101 @@ __device__ __forceinline__ KaRows ka_rows(const Kv4AttendArgs &a, int seq) {
     return r;
 }
 
-// NT * 8 query rows (the rows of the heads that share a cache head, heads innermost) of one sequence and cache head over
-// `chunk` of its keys. SPLIT: q and P' as two f16 (f32 queries), else as one.
+// A unit of work is a row tile (R query rows: a sequence's rows, the heads that share a cache head innermost) of one cache
+// head, over the keys that its rows see, in steps of KA_STEP keys.
+struct KaSpan {
+    int lo_min, lo_max, hi_min, hi_max, base, steps;  // what the first and last rows see; where the steps begin
+};
+__device__ __forceinline__ int ka_hi(const Kv4AttendArgs &a, const KaRows &s, int i) {
+    return a.causal ? max(0, min(s.len, s.len - s.n + i + 1)) : s.len;
+}
+__device__ __forceinline__ int ka_lo(const Kv4AttendArgs &a, const KaRows &s, int i) {
+    return a.window ? max(0, s.len - s.n + i + 1 - a.window) : 0;
+}
+template <int R>
+__device__ __forceinline__ KaSpan ka_span(const Kv4AttendArgs &a, const KaRows &s, int each, int rt) {
+    const int first = rt * R / each, last = (min(s.n * each, (rt + 1) * R) - 1) / each;
+    KaSpan p;
+    p.lo_min = ka_lo(a, s, first), p.lo_max = ka_lo(a, s, last), p.hi_min = ka_hi(a, s, first), p.hi_max = ka_hi(a, s, last);
+    p.base = p.lo_min & ~(KA_KEYS - 1);
+    p.steps = p.hi_max > p.lo_min ? (p.hi_max - p.base + KA_STEP - 1) / KA_STEP : 1;  // no keys: a step that writes zeros
+    return p;
+}
+template <int R>
+__device__ __forceinline__ long long ka_seq_steps(const Kv4AttendArgs &a, int seq, int each) {  // a head's
+    const KaRows s = ka_rows(a, seq);
+    if (!s.ok) {
+        *reinterpret_cast<volatile int *>(a.err) = 1;
+        return 0;
+    }
+    const int tiles = (s.n * each + R - 1) / R;
+    if (!a.causal && tiles) return (long long)tiles * ka_span<R>(a, s, each, 0).steps;
+    long long n = 0;
+    for (int rt = 0; rt < tiles; rt++) n += ka_span<R>(a, s, each, rt).steps;
+    return n;
+}
+
+// The steps of all units in a row, cut evenly over the blocks: block b takes steps [T b / N, T (b + 1) / N), whole units
+// and at most one part of a unit at either end. Parts meet in the working memory; the last block of a unit to arrive joins
+// them in their order. SPLIT: q and the weights as two f16 (f32 queries), else as one.
 template <int HD, int G, int NT, bool SPLIT>
-__global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, int dtype, int row_tiles, int chunk, float *part,
-                                                              int *arrived) {
+__global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 : 1)
+    k_kv4_attend(Kv4AttendArgs a, int dtype, int min_steps, float *part, int *arrived) {
     using C = KaTile<HD, G>;
     constexpr int NU = C::NU, NG = C::NG, UG = G / 32, R = 8 * NT, ST = C::STAGES, QS = SPLIT ? 2 : 1;
     extern __shared__ __align__(16) uint8_t sm[];
-    __shared__ int s_last;
+    __shared__ int s_last, s_unit[4];
+    __shared__ long long s_sum[KA_STEP];
     __shared__ __align__(8) unsigned long long bars[KA_WARPS][ST];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int unit = blockIdx.x, split = blockIdx.y;
-    const int rt = unit % row_tiles, head = unit / row_tiles % a.c.heads, seq = unit / row_tiles / a.c.heads;
-    const KaRows sr = ka_rows(a, seq);
-    if (!sr.ok) {
-        if (tid == 0) *reinterpret_cast<volatile int *>(a.err) = 1;
-        return;
+    const int each = a.q_heads / a.c.heads;
+
+    // ---- this block's steps ----
+    const int share = (a.seqs + KA_STEP - 1) / KA_STEP, seq_lo = min(a.seqs, tid * share), seq_hi = min(a.seqs, seq_lo + share);
+    long long own = 0;
+    for (int q = seq_lo; q < seq_hi; q++) own += ka_seq_steps<R>(a, q, each) * a.c.heads;
+    long long before = own;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const long long x = __shfl_up_sync(0xffffffffu, before, d);
+        if (lane >= d) before += x;
     }
-    const int each = a.q_heads / a.c.heads, total = sr.n * each, r0 = rt * R, rows = min(R, total - r0);
-    if (rows <= 0) return;
-    // row r of the block: query row i = (r0 + r) / each sees keys [lo(i), hi(i)); both grow with i
-    const int i_first = r0 / each, i_last = (r0 + rows - 1) / each;
-    auto hi_of = [&](int i) { return a.causal ? max(0, min(sr.len, sr.len - sr.n + i + 1)) : sr.len; };
-    auto lo_of = [&](int i) { return a.window ? max(0, sr.len - sr.n + i + 1 - a.window) : 0; };
-    const int lo_min = lo_of(i_first), lo_max = lo_of(i_last), hi_min = hi_of(i_first), hi_max = hi_of(i_last);
-    const int base = lo_min & ~(KA_KEYS - 1);
-    const int nsplits = hi_max > lo_min ? (hi_max - base + chunk - 1) / chunk : 1;
-    if (split >= nsplits) return;
-    const int k0 = base + split * chunk, k1 = hi_max > lo_min ? min(hi_max, k0 + chunk) : k0;
-    const int ntiles = (k1 - k0 + KA_KEYS - 1) / KA_KEYS, mine = (ntiles - warp + KA_WARPS - 1) / KA_WARPS;
+    if (lane == 31) s_sum[warp] = before;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < KA_WARPS; w++) {
+        if (w == warp) before += total;
+        total += s_sum[w];
+    }
+    before -= own;
+    const long long blocks = min((long long)gridDim.x, (total + min_steps - 1) / min_steps);
+    if (blockIdx.x >= blocks) return;
+    long long pos = total * blockIdx.x / blocks;
+    const long long end = total * (blockIdx.x + 1) / blocks;
+    if (own && pos >= before && pos < before + own) {  // the thread whose sequences hold the first step
+        long long at = before;
+        for (int q = seq_lo; q < seq_hi; q++) {
+            const long long n = ka_seq_steps<R>(a, q, each) * a.c.heads;
+            if (pos >= at + n) {
+                at += n;
+                continue;
+            }
+            const KaRows r = ka_rows(a, q);
+            for (int rt = 0;; rt++) {
+                const int steps = ka_span<R>(a, r, each, rt).steps;
+                if (pos >= at + (long long)steps * a.c.heads) {
+                    at += (long long)steps * a.c.heads;
+                    continue;
+                }
+                s_unit[0] = q, s_unit[1] = rt, s_unit[2] = (int)((pos - at) / steps), s_unit[3] = (int)((pos - at) % steps);
+                break;
+            }
+            break;
+        }
+    }
+    __syncthreads();
+    int seq = s_unit[0], rt = s_unit[1], head = s_unit[2], skip = s_unit[3];
 
     // this warp's ring: each step's key codes, key scales, value codes and value scales come as four bulk copies (eight
     // when the 32 keys lie on two pages of 16), one a lane, that count on the slot's barrier
@@ -136,6 +202,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
+    uint32_t used = 0;  // steps of this warp so far: the ring's place and the barriers' phases
     const size_t hb = kv4_head_bytes(HD, a.c.page, G);
     const Kv4Offsets off = kv4_offsets(HD, a.c.page, G);
     const int page_shift = 31 - __clz(a.c.page), halves = a.c.page == 16 ? 2 : 1;
@@ -143,6 +210,13 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
     const uint32_t from = (cpart & 2 ? off.vc : 0) + (cpart & 1 ? off.ks : 0);  // ks = vs - vc: the codes before the scales
     const uint32_t per_key = cpart & 1 ? NG * 4 : HD / 2, copy_bytes = per_key * KA_KEYS / halves;
     const uint32_t to = (cpart & 2 ? C::KC + C::SC : 0) + (cpart & 1 ? C::KC : 0) + chalf * copy_bytes;
+    while (pos < end) {
+    const KaRows sr = ka_rows(a, seq);
+    const KaSpan sp = ka_span<R>(a, sr, each, rt);
+    const int piece = (int)min((long long)(sp.steps - skip), end - pos), r0 = rt * R, rows = min(R, sr.n * each - r0);
+    const int lo_min = sp.lo_min, lo_max = sp.lo_max, hi_min = sp.hi_min, hi_max = sp.hi_max;
+    const int k0 = sp.base + skip * KA_STEP, k1 = hi_max > lo_min ? min(hi_max, k0 + piece * KA_STEP) : k0;
+    const int ntiles = (k1 - k0 + KA_KEYS - 1) / KA_KEYS, mine = max(0, (ntiles - warp + KA_WARPS - 1) / KA_WARPS);
     // the page numbers are read a step before they are needed
     int pages[2];
     auto find = [&](int it) {
@@ -155,7 +229,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
         if (it >= mine) return;
         const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
         const bool ok0 = pages[0] >= 0 && pages[0] < a.c.pages, ok1 = pages[1] >= 0 && pages[1] < a.c.pages;
-        const uint32_t bar = bar_at + 8 * (it % ST);
+        const uint32_t slot = (used + it) % ST, bar = bar_at + 8 * slot;
         if (lane == 0) {
             if ((!ok0 && j0 + KA_KEYS / halves > lo_min) || (halves == 2 && !ok1 && j0 + 16 < k1 && j0 + KA_KEYS > lo_min))
                 *reinterpret_cast<volatile int *>(a.err) = 1;
@@ -165,7 +239,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
         if (lane < 4 * halves && (chalf ? ok1 : ok0)) {
             const uint8_t *src = a.c.pool + ((size_t)(chalf ? pages[1] : pages[0]) * a.c.heads + head) * hb + from +
                                  ((j0 + 16 * chalf) & (a.c.page - 1)) * per_key;
-            bulk_copy(ring_at + it % ST * C::BYTES + to, src, copy_bytes, bar);
+            bulk_copy(ring_at + slot * C::BYTES + to, src, copy_bytes, bar);
         }
         find(it + 1);
     };
@@ -210,7 +284,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
         for (int u = 0; u < NU; u++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                x[u][j] *= up;
+                x[u][j] *= a.scale < 0.f ? -up : up;
                 sum[u / UG] += SPLIT ? x[u][j] : __half2float(__float2half_rn(x[u][j]));
             }
 #pragma unroll
@@ -223,7 +297,8 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                 }
             }
         }
-        const float factor = a.scale * 1.44269504088896340736f * pow2i(-e) * 16777216.f;
+        // (a scale of 0 as 2^-100, so that the factor is positive: the scores' order is that of the products)
+        const float factor = fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * pow2i(-e) * 16777216.f;
 #pragma unroll
         for (int k = 0; k < NG; k++) {
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
@@ -254,16 +329,18 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                 for (int k = 0; k < NG; k++) qs[nt][k][c] = __shfl_sync(0xffffffffu, sum[k], who);
             }
             const int ic = (r0 + nt * 8 + 2 * t + c) / each;
-            hi[nt][c] = hi_of(ic), lo[nt][c] = lo_of(ic);
+            hi[nt][c] = ka_hi(a, sr, ic), lo[nt][c] = ka_lo(a, sr, ic);
         }
     }
 
     // the running state, in units of 2^m for a column (m moves only when a score passes it by 8) and 2^ve for the weights
-    float m[NT][2], l[NT][2], ls[NT][NG][2], o[NT][NU][2][4];
-    float vtop = 0.f, vinv = 1.f;  // the largest step so far rounded up to a power of two, and 2^7 over it
+    float m[NT][2], bound[NT][2], l[NT][2], ls[NT][NG][2], o[NT][NU][2][4];
+    float ol[NT][4] = {};  // sums of p low of group g, where they are taken as a matrix product
+    constexpr bool LOW_MMA_V = C::LOW_MMA && !SPLIT;
+    float vtop = 0.f, vinv = 1.f;  // the largest step so far rounded up to a power of two, and its reciprocal
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
+        m[nt][0] = m[nt][1] = bound[nt][0] = bound[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
         for (int k = 0; k < NG; k++) ls[nt][k][0] = ls[nt][k][1] = 0.f;
 #pragma unroll
@@ -272,24 +349,21 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
             for (int x = 0; x < 8; x++) o[nt][u][x >> 2][x & 3] = 0.f;
     }
 
-    __half2 vnorm = __float2half2_rn(1.f);  // one f16 of the weights: steps times 2^-ve (as far as f16 goes), weights times 2^7
+    __half2 vnorm = __float2half2_rn(1.f);  // 16-bit types: 1 / vtop, by which the steps come into f16's range
     bool gave_up = false;
     for (int it = 0; it < mine; it++) {
         load(it + ST - 1);
         {
-            const uint32_t bar = bar_at + 8 * (it % ST), parity = (it / ST) & 1;
-            const long long began = clock64();
+            const uint32_t bar = bar_at + 8 * ((used + it) % ST), parity = ((used + it) / ST) & 1;
             uint32_t done = 0;
-            while (!done) {
+            for (int tries = 0; !done && tries < KA_TRIES; tries++)
                 asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-                if (!done && clock64() - began > KA_WAIT) break;
-            }
             if (__any_sync(0xffffffffu, !done)) {
                 gave_up = true;
                 break;
             }
         }
-        const uint8_t *tile = ring + it % ST * C::BYTES;
+        const uint8_t *tile = ring + (used + it) % ST * C::BYTES;
         const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
         const bool edge = j0 + KA_KEYS > hi_min || j0 < lo_max;
         float s[2][NT][4];
@@ -356,7 +430,6 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                 for (int c = 0; c < 4; c++) {
                     // the lows' products are 2^18 times the codes'
                     if constexpr (C::LOW_MMA) s[kb][nt][c] = fmaf(low[nt][c], 3.814697265625e-6f, s[kb][nt][c]);
-                    s[kb][nt][c] *= fq[nt][c & 1];
                 }
         }
         // the value scales of this thread's four keys
@@ -391,7 +464,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int c = 0; c < 2; c++)
-                moves |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > m[nt][c] + 8.f;
+                moves |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > bound[nt][c];
         if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
             for (int d = 1; d < 32; d *= 2) step_max = fmaxf(step_max, __shfl_xor_sync(0xffffffffu, step_max, d));
@@ -400,7 +473,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                 // the next power of two (steps are positive f16: at least 2^-24)
                 const int e = (int)(__float_as_uint(step_max) >> 23) - 126;
                 const float top = SPLIT ? pow2i(e) : pow2i(max(e, -15));
-                vf = vtop / top, vtop = top, vinv = 128.f / top;
+                vf = vtop / top, vtop = top, vinv = 1.f / top;
                 vnorm = __float2half2_rn(1.f / top);
             }
 #pragma unroll
@@ -410,9 +483,10 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                     float x = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
 #pragma unroll
                     for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                    x = fmaxf(x, m[nt][c]);
+                    x = fmaxf(x * fq[nt][c], m[nt][c]);
+                    bound[nt][c] = x == -INFINITY ? x : (x + 8.f) / fq[nt][c];
                     const float f = x > m[nt][c] ? exp2_sfu(m[nt][c] - x) : 1.f, fo = f * vf;
-                    m[nt][c] = x, l[nt][c] *= f;
+                    m[nt][c] = x, l[nt][c] *= f, ol[nt][c] *= f;
 #pragma unroll
                     for (int k = 0; k < NG; k++) ls[nt][k][c] *= f;
 #pragma unroll
@@ -425,18 +499,20 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                const float mm = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+                // weights come 2^7 times as large (up to 2^15), so that small ones stay normal in f16
+                const float mm = m[nt][c] == -INFINITY ? 0.f : m[nt][c] - 7.f;
 #pragma unroll
                 for (int kb = 0; kb < 2; kb++)
 #pragma unroll
                     for (int h = 0; h < 4; h += 2) {
-                        const float p = exp2_sfu(s[kb][nt][c + h] - mm);
+                        const float p = exp2_sfu(fmaf(s[kb][nt][c + h], fq[nt][c], -mm));
                         s[kb][nt][c + h] = p, l[nt][c] += p;
                     }
             }
-        // sum p low
+        // sum p low: as a matrix product below, or in f32
+        if (!LOW_MMA_V || edge) {
 #pragma unroll
-        for (int kb = 0; kb < 2; kb++)
+            for (int kb = 0; kb < 2; kb++)
 #pragma unroll
             for (int k = 0; k < NG; k++) {
                 const float y0 = bits_float2(vs[kb][0][k]).y, y1 = bits_float2(vs[kb][1][k]).y;
@@ -451,6 +527,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                             ls[nt][k][c] = fmaf(p0, y0, fmaf(p1, y1, ls[nt][k][c]));
                     }
             }
+        }
 #pragma unroll
         for (int kb = 0; kb < 2; kb++) {
             // the half-words of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9, a pair in one register
@@ -473,7 +550,19 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) p2[nt][h] = __floats2half2_rn(s[kb][nt][2 * h] * 128.f, s[kb][nt][2 * h + 1] * 128.f);
+                    for (int h = 0; h < 2; h++) p2[nt][h] = __floats2half2_rn(s[kb][nt][2 * h], s[kb][nt][2 * h + 1]);
+            }
+            if (LOW_MMA_V && !edge) {  // rows: the groups' lows of keys 2 t, 2 t + 1 and 2 t + 8, 2 t + 9
+                uint32_t lows[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t *p = reinterpret_cast<const uint32_t *>(tile + 2 * C::KC + C::SC) + (kb * 16 + h * 8 + 2 * t) * NG + g % NG;
+                    lows[h] = g < NG ? __byte_perm(p[0], p[NG], 0x7632) : 0u;
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    mma16816(ol[nt], lows[0], 0u, lows[1], 0u, transpose8(*reinterpret_cast<const uint32_t *>(&p2[nt][0])),
+                             transpose8(*reinterpret_cast<const uint32_t *>(&p2[nt][1])));
             }
 #pragma unroll
             for (int k = 0; k < NG; k++) {
@@ -490,7 +579,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                             b[0][nt][h] = transpose8(x), b[QS - 1][nt][h] = transpose8(half2_bits(p0 - f.x, p1 - f.y));
                         }
                 } else {
-                    // one f16 of p 2^7 times one of the step: each rounds to 11 bits, as the results are to 11 or 8
+                    // p and p * step each round to 11 bits, as the results do to 11 or 8
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const __half2 w = __hmul2(__low2half2(*reinterpret_cast<const __half2 *>(&vs[kb][h][k])), vnorm);
@@ -516,13 +605,14 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
         }
         __syncwarp();  // every lane is done with the slot that the next load fills
     }
+    used += mine;
     if (gave_up && lane == 0) *reinterpret_cast<volatile int *>(a.err_wait) = 1;
 
     // ---- the warps' states joined ----
     __syncthreads();
     float *so = reinterpret_cast<float *>(sm);  // [warp][R][HD]
     float *sms = so + KA_WARPS * R * HD;        // [warp][R]{m, l}
-    const float unv = vtop * (16777216.f / 128.f);
+    const float unv = vtop * 16777216.f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -535,9 +625,10 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
                 y[k] = ls[nt][k][c];
 #pragma unroll
                 for (int d = 4; d < 32; d *= 2) y[k] += __shfl_xor_sync(0xffffffffu, y[k], d);
+                if (LOW_MMA_V) y[k] += __shfl_sync(0xffffffffu, ol[nt][c], k * 4 + t);
             }
             const int r = nt * 8 + 2 * t + c;
-            if (g == 0) sms[(warp * R + r) * 2] = m[nt][c], sms[(warp * R + r) * 2 + 1] = x;
+            if (g == 0) sms[(warp * R + r) * 2] = m[nt][c] - 7.f, sms[(warp * R + r) * 2 + 1] = x;
             float *dst = so + (warp * R + r) * HD + 4 * g;
 #pragma unroll
             for (int u = 0; u < NU; u++)
@@ -561,9 +652,11 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
             a.lse[(size_t)(sr.first + (r0 + r) / each) * a.q_heads + head * each + (r0 + r) % each] =
                 (M + log2f(L)) * 0.69314718055994530942f;
     };
-    const size_t slot = ((size_t)unit * gridDim.y + split) * R;
-    float *pms = part + 2 * slot, *po = part + 2 * (size_t)gridDim.x * gridDim.y * R + slot * HD;
-    for (int x = tid; x < rows * HD; x += KA_WARPS * 32) {
+    // a part that begins a unit goes to the block's second slot, one that goes on to its first
+    const bool whole = piece == sp.steps;
+    const size_t nslots = 2 * (size_t)gridDim.x, slot = 2 * (size_t)blockIdx.x + (skip == 0);
+    float *pms = part + 2 * slot * R, *po = part + 2 * nslots * R + slot * R * HD;
+    for (int x = tid; x < rows * HD; x += KA_STEP) {
         const int r = x / HD, c = x % HD;
         float M = -INFINITY, L = 0.f, v = 0.f;
 #pragma unroll
@@ -574,7 +667,7 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
             const float f = exp2_sfu(sms[(w * R + r) * 2] - M0);
             L = fmaf(sms[(w * R + r) * 2 + 1], f, L), v = fmaf(so[(w * R + r) * HD + c], f, v);
         }
-        if (nsplits == 1) {
+        if (whole) {
             put(r, c, L != 0.f ? v / L : 0.f);  // L is 0 when no key is seen, NaN when a score is
             if (c == 0) put_lse(r, M0, L);
         } else {
@@ -582,125 +675,134 @@ __global__ void __launch_bounds__(KA_WARPS * 32) k_kv4_attend(Kv4AttendArgs a, i
             if (c == 0) __stcg(pms + 2 * r, M), __stcg(pms + 2 * r + 1, L);
         }
     }
-    if (nsplits == 1) return;
-    // ---- the last block of the row tile to arrive joins the blocks' states, in their order ----
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        s_last = atomicAdd(arrived + unit, 1) == nsplits - 1;
-        if (s_last) arrived[unit] = 0;  // ready for the next call
+    if (!whole) {
+        // ---- the last of the unit's blocks to arrive joins their states, in their order ----
+        const long long u0 = pos - skip, u1 = u0 + sp.steps;
+        const int b0 = (int)(((u0 + 1) * blocks - 1) / total), b1 = (int)((u1 * blocks - 1) / total), np = b1 - b0 + 1;
+        __threadfence();
+        __syncthreads();
+        if (tid == 0) {
+            s_last = atomicAdd(arrived + b0, 1) == np - 1;  // (a block begins at most one unit that others go on with)
+            if (s_last) arrived[b0] = 0;                    // ready for the next call
+        }
+        __syncthreads();
+        if (s_last) {
+            __threadfence();
+            auto slot_of = [&](int p) { return 2 * (size_t)(b0 + p) + (p == 0); };
+            const float *po0 = part + 2 * nslots * R;
+            for (int r = warp; r < rows; r += KA_WARPS) {  // a warp a row: 32 parts' (maximum, sum) at a time
+                float M = -INFINITY, L = 0.f;
+                for (int p = lane; p < np; p += 32) M = fmaxf(M, __ldcg(part + 2 * (slot_of(p) * R + r)));
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+                const float M0 = M == -INFINITY ? 0.f : M;
+                float v[HD / 32] = {};
+                for (int p0 = 0; p0 < np; p0 += 32) {
+                    float f = 0.f;
+                    if (p0 + lane < np) {
+                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(part) + slot_of(p0 + lane) * R + r);
+                        f = exp2_sfu(x.x - M0), L = fmaf(x.y, f, L);
+                    }
+                    const int n = min(32, np - p0);
+                    for (int q0 = 0; q0 < n; q0 += 8) {
+                        float y[8][HD / 32];
+#pragma unroll
+                        for (int q = 0; q < 8; q++)
+#pragma unroll
+                            for (int k = 0; k < HD / 32; k++)
+                                y[q][k] = q0 + q < n ? __ldcg(po0 + (slot_of(p0 + q0 + q) * R + r) * HD + k * 32 + lane) : 0.f;
+#pragma unroll
+                        for (int q = 0; q < 8; q++) {
+                            const float w = __shfl_sync(0xffffffffu, f, q0 + q);
+                            if (q0 + q < n)
+#pragma unroll
+                                for (int k = 0; k < HD / 32; k++) v[k] = fmaf(y[q][k], w, v[k]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) L += __shfl_xor_sync(0xffffffffu, L, d);
+#pragma unroll
+                for (int k = 0; k < HD / 32; k++) put(r, k * 32 + lane, L != 0.f ? v[k] / L : 0.f);
+                if (lane == 0) put_lse(r, M0, L);
+            }
+        }
     }
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
-    float *wt = reinterpret_cast<float *>(sm);  // [nsplits][rows] weights, then [rows]{1 / sum}
-    const float *ams = part + 2 * (size_t)unit * gridDim.y * R;
-    for (int r = warp; r < rows; r += KA_WARPS) {
-        float M = -INFINITY, L = 0.f;
-        for (int p = lane; p < nsplits; p += 32) M = fmaxf(M, __ldcg(ams + 2 * ((size_t)p * R + r)));
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-        const float M0 = M == -INFINITY ? 0.f : M;
-        for (int p = lane; p < nsplits; p += 32) {
-            const float2 x = __ldcg(reinterpret_cast<const float2 *>(ams) + (size_t)p * R + r);
-            const float f = exp2_sfu(x.x - M0);
-            wt[p * rows + r] = f, L = fmaf(x.y, f, L);
-        }
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) L += __shfl_xor_sync(0xffffffffu, L, d);
-        if (lane == 0) {
-            wt[nsplits * rows + r] = L != 0.f ? 1.f / L : 0.f;
-            put_lse(r, M0, L);
+    // the next unit; its copies (the asynchronous proxy's) come after this one's reads and writes of the same memory
+    pos += piece, skip = 0;
+    if (++head == a.c.heads) {
+        head = 0;
+        if ((++rt) * R >= sr.n * each) {
+            rt = 0;
+            while (++seq < a.seqs) {
+                const KaRows next = ka_rows(a, seq);
+                if (next.ok && next.n) break;
+            }
         }
     }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
-    const float *ao = part + 2 * (size_t)gridDim.x * gridDim.y * R + (size_t)unit * gridDim.y * R * HD;
-    for (int x = tid; x < rows * HD; x += KA_WARPS * 32) {
-        const int r = x / HD;
-        float v = 0.f;
-        for (int p0 = 0; p0 < nsplits; p0 += 8) {
-            float y[8];
-#pragma unroll
-            for (int p = 0; p < 8; p++) y[p] = p0 + p < nsplits ? __ldcg(ao + (size_t)(p0 + p) * R * HD + x) : 0.f;
-#pragma unroll
-            for (int p = 0; p < 8; p++)
-                if (p0 + p < nsplits) v = fmaf(y[p], wt[(p0 + p) * rows + r], v);
-        }
-        put(r, x % HD, v * wt[nsplits * rows + r]);
     }
 }
 
-struct KaPlan {
-    int nt, row_tiles, units, chunk, splits;
-};
-static KaPlan ka_plan(int dtype, const Kv4AttendArgs &a, int sms) {
-    KaPlan p;
-    const int rows = a.max_rows * (a.q_heads / a.c.heads);
+static int ka_nt(int dtype, const Kv4AttendArgs &a) {
     // 16 rows a block where their fragments of q and of the output fit the registers
-    p.nt = rows > 8 && a.c.width * (dtype == DT_F32 ? 2 : 1) <= 128 ? 2 : 1;
-    p.row_tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
-    p.units = a.seqs * a.c.heads * p.row_tiles;
-    const int span = a.window ? (int)std::min<long long>(a.max_len, (long long)a.window + a.max_rows + KA_KEYS - 1) : a.max_len;
-    const int step = KA_WARPS * KA_KEYS, most = std::max(1, (span + step - 1) / step);  // steps of the longest
-    // enough blocks for two on every SM, at least one step of every warp a block and at most sixteen (a long sequence's
-    // blocks then start and end at different times, which hides their first loads and their joins)
-    int per = (int)std::min<long long>(16, ((long long)most * p.units + 2 * sms - 1) / (2 * sms));
-    per = std::max({per, 1, (most + KA_SPLITS - 1) / KA_SPLITS});
-    if (p.units > KA_COUNTERS) per = most;
-    p.chunk = per * step;
-    p.splits = (most + per - 1) / per;
-    return p;
+    return a.max_rows * (a.q_heads / a.c.heads) > 8 && a.c.width * (dtype == DT_F32 ? 2 : 1) <= 128 ? 2 : 1;
 }
 
-static size_t ka_work_bytes(const Kv4AttendArgs &a, const KaPlan &p) {
-    return p.splits == 1 ? 0 : 4 * (KA_COUNTERS + (size_t)p.units * p.splits * 8 * p.nt * (a.c.width + 2));
-}
 size_t kv4_attend_workspace(int dtype, const Kv4AttendArgs &a, int sms) {
-    // A window shortens the span, and shorter spans are cut finer, up to two blocks an SM.
-    KaPlan p = ka_plan(dtype, a, sms);
-    const int most = (a.max_len + KA_WARPS * KA_KEYS - 1) / (KA_WARPS * KA_KEYS);
-    p.splits = std::max(p.splits, std::min({most, KA_SPLITS, 2 * sms / std::max(1, p.units) + 1}));
-    return ka_work_bytes(a, p);
+    return 4 * (KA_BLOCKS + (size_t)std::min(KA_BLOCKS, 8 * sms) * 2 * 8 * ka_nt(dtype, a) * (a.c.width + 2));
 }
 
 template <int HD, int G, int NT, bool SPLIT>
-static cudaError_t launch_one(int dtype, const Kv4AttendArgs &a, const KaPlan &p, void *work, cudaStream_t s) {
+static cudaError_t launch_one(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
     using C = KaTile<HD, G>;
+    const auto kernel = k_kv4_attend<HD, G, NT, SPLIT>;
     const size_t join = sizeof(float) * KA_WARPS * 8 * NT * (HD + 2);
-    const size_t smem = std::max({(size_t)KA_WARPS * C::STAGES * C::BYTES, join, sizeof(float) * 8 * NT * (KA_SPLITS + 2)});
-    cudaError_t e = allow_dynamic_smem((const void *)k_kv4_attend<HD, G, NT, SPLIT>, smem);
+    const size_t smem = std::max((size_t)KA_WARPS * C::STAGES * C::BYTES, join);
+    cudaError_t e = allow_dynamic_smem((const void *)kernel, smem);
     if (e != cudaSuccess) return e;
-    int *arrived = reinterpret_cast<int *>(work);
-    float *part = reinterpret_cast<float *>(work) + KA_COUNTERS;
-    k_kv4_attend<HD, G, NT, SPLIT><<<dim3(p.units, p.splits), KA_WARPS * 32, smem, s>>>(a, dtype, p.row_tiles, p.chunk, part, arrived);
+    static std::atomic<int> resident{0};  // blocks an SM holds
+    if (!resident) {
+        int n = 0;
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, KA_STEP, smem);
+        if (e != cudaSuccess) return e;
+        resident = std::max(1, std::min(8, n));
+    }
+    // as many blocks as the GPU holds at once, at least one step each
+    const long long rows = (long long)a.max_rows * (a.q_heads / a.c.heads), tiles = (rows + 8 * NT - 1) / (8 * NT);
+    const long long most = std::max(1LL, ((long long)a.max_len + KA_STEP + KA_KEYS - 1) / KA_STEP) * tiles * a.seqs * a.c.heads;
+    const int grid = (int)std::min<long long>({most, (long long)resident * sms, KA_BLOCKS});
+    k_kv4_attend<HD, G, NT, SPLIT><<<grid, KA_STEP, smem, s>>>(a, dtype, 1, reinterpret_cast<float *>(work) + KA_BLOCKS,
+                                                               reinterpret_cast<int *>(work));
     return cudaGetLastError();
 }
 template <int HD, int G>
-static cudaError_t launch_size(int dtype, const Kv4AttendArgs &a, const KaPlan &p, void *work, cudaStream_t s) {
+static cudaError_t launch_size(int dtype, const Kv4AttendArgs &a, int nt, int sms, void *work, cudaStream_t s) {
     const bool split = dtype == DT_F32;
     if constexpr (HD <= 64) {
-        if (p.nt == 2 && split) return launch_one<HD, G, 2, true>(dtype, a, p, work, s);
+        if (nt == 2 && split) return launch_one<HD, G, 2, true>(dtype, a, sms, work, s);
     }
     if constexpr (HD <= 128) {
-        if (p.nt == 2) return launch_one<HD, G, 2, false>(dtype, a, p, work, s);
+        if (nt == 2) return launch_one<HD, G, 2, false>(dtype, a, sms, work, s);
     }
-    return split ? launch_one<HD, G, 1, true>(dtype, a, p, work, s) : launch_one<HD, G, 1, false>(dtype, a, p, work, s);
+    return split ? launch_one<HD, G, 1, true>(dtype, a, sms, work, s) : launch_one<HD, G, 1, false>(dtype, a, sms, work, s);
 }
 
 cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *work, size_t work_bytes, cudaStream_t s, uint64_t *launches) {
     if (!a.seqs || !a.rows || !a.max_rows) return cudaSuccess;
-    const KaPlan p = ka_plan(dtype, a, sms);
-    if (ka_work_bytes(a, p) > work_bytes) return cudaErrorInvalidValue;
+    if (kv4_attend_workspace(dtype, a, sms) > work_bytes) return cudaErrorInvalidValue;
+    const int nt = ka_nt(dtype, a);
     cudaError_t e = cudaErrorInvalidValue;
     const int w = a.c.width, g = a.c.group;
-    if (w == 32) e = launch_size<32, 32>(dtype, a, p, work, s);
-    if (w == 64) e = g == 32 ? launch_size<64, 32>(dtype, a, p, work, s) : launch_size<64, 64>(dtype, a, p, work, s);
+    if (w == 32) e = launch_size<32, 32>(dtype, a, nt, sms, work, s);
+    if (w == 64) e = g == 32 ? launch_size<64, 32>(dtype, a, nt, sms, work, s) : launch_size<64, 64>(dtype, a, nt, sms, work, s);
     if (w == 128)
-        e = g == 32 ? launch_size<128, 32>(dtype, a, p, work, s)
-                    : g == 64 ? launch_size<128, 64>(dtype, a, p, work, s) : launch_size<128, 128>(dtype, a, p, work, s);
+        e = g == 32 ? launch_size<128, 32>(dtype, a, nt, sms, work, s)
+                    : g == 64 ? launch_size<128, 64>(dtype, a, nt, sms, work, s) : launch_size<128, 128>(dtype, a, nt, sms, work, s);
     if (w == 256)
-        e = g == 32 ? launch_size<256, 32>(dtype, a, p, work, s)
-                    : g == 64 ? launch_size<256, 64>(dtype, a, p, work, s) : launch_size<256, 128>(dtype, a, p, work, s);
+        e = g == 32 ? launch_size<256, 32>(dtype, a, nt, sms, work, s)
+                    : g == 64 ? launch_size<256, 64>(dtype, a, nt, sms, work, s) : launch_size<256, 128>(dtype, a, nt, sms, work, s);
     if (launches) ++*launches;
     return e;
 }
