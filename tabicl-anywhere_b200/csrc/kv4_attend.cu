@@ -10,7 +10,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "fourbit.cuh"
+#include "kv4_plan.cuh"
 
 namespace tcu {
 
@@ -18,7 +18,6 @@ constexpr int KA_KEYS = 32;     // keys of a warp's step
 constexpr int KA_WARPS = 4;     // warps of a block, each over its own steps of the block's keys
 constexpr int KA_STEP = KA_WARPS * KA_KEYS;  // keys of a block's step
 constexpr int KA_TRIES = 1 << 20;  // waits for a copy (each suspends the warp for a while) before a warp gives up
-constexpr int KA_BLOCKS = 2048;  // most blocks of a launch: as many arrival counters start the working memory of every call
 
 template <int HD, int G>
 struct KaTile {
@@ -82,57 +81,7 @@ __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) { 
     }
 }
 
-// What a sequence's rows of one block see, from the lengths that only the device has.
-struct KaRows {
-    int first, n, len;  // the sequence's first row, its rows and cached tokens
-    bool ok;
-};
-__device__ __forceinline__ KaRows ka_rows(const Kv4AttendArgs &a, int seq) {
-    KaRows r;
-    r.first = seq * a.max_rows, r.n = a.max_rows;
-    if (a.starts) r.first = a.starts[seq], r.n = a.starts[seq + 1] - r.first;
-    r.len = a.lens[seq];
-    r.ok = !(r.first < 0 || r.n < 0 || r.n > a.max_rows || r.first > a.rows - r.n || r.len < 0 || r.len > a.max_len);
-    return r;
-}
-
-// A unit of work is a row tile (R query rows: a sequence's rows, the heads that share a cache head innermost) of one cache
-// head, over the keys that its rows see, in steps of KA_STEP keys.
-struct KaSpan {
-    int lo_min, lo_max, hi_min, hi_max, base, steps;  // what the first and last rows see; where the steps begin
-};
-__device__ __forceinline__ int ka_hi(const Kv4AttendArgs &a, const KaRows &s, int i) {
-    return a.causal ? max(0, min(s.len, s.len - s.n + i + 1)) : s.len;
-}
-__device__ __forceinline__ int ka_lo(const Kv4AttendArgs &a, const KaRows &s, int i) {
-    return a.window ? max(0, s.len - s.n + i + 1 - a.window) : 0;
-}
-template <int R>
-__device__ __forceinline__ KaSpan ka_span(const Kv4AttendArgs &a, const KaRows &s, int each, int rt) {
-    const int first = rt * R / each, last = (min(s.n * each, (rt + 1) * R) - 1) / each;
-    KaSpan p;
-    p.lo_min = ka_lo(a, s, first), p.lo_max = ka_lo(a, s, last), p.hi_min = ka_hi(a, s, first), p.hi_max = ka_hi(a, s, last);
-    p.base = p.lo_min & ~(KA_KEYS - 1);
-    p.steps = p.hi_max > p.lo_min ? (p.hi_max - p.base + KA_STEP - 1) / KA_STEP : 1;  // no keys: a step that writes zeros
-    return p;
-}
-template <int R>
-__device__ __forceinline__ long long ka_seq_steps(const Kv4AttendArgs &a, int seq, int each) {  // a head's
-    const KaRows s = ka_rows(a, seq);
-    if (!s.ok) {
-        *reinterpret_cast<volatile int *>(a.err) = 1;
-        return 0;
-    }
-    const int tiles = (s.n * each + R - 1) / R;
-    if (!a.causal && tiles) return (long long)tiles * ka_span<R>(a, s, each, 0).steps;
-    long long n = 0;
-    for (int rt = 0; rt < tiles; rt++) n += ka_span<R>(a, s, each, rt).steps;
-    return n;
-}
-
-// The steps of all units in a row, cut evenly over the blocks: block b takes steps [T b / N, T (b + 1) / N), whole units
-// and at most one part of a unit at either end. Parts meet in the working memory; the last block of a unit to arrive joins
-// them in their order. SPLIT: q and the weights as two f16 (f32 queries), else as one.
+// SPLIT: q and the weights as two f16 (f32 queries), else as one.
 template <int HD, int G, int NT, bool SPLIT>
 __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 : 1)
     k_kv4_attend(Kv4AttendArgs a, int dtype, int min_steps, float *part, int *arrived) {
@@ -140,57 +89,14 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
     constexpr int NU = C::NU, NG = C::NG, UG = G / 32, R = 8 * NT, ST = C::STAGES, QS = SPLIT ? 2 : 1;
     extern __shared__ __align__(16) uint8_t sm[];
     __shared__ int s_last, s_unit[4];
-    __shared__ long long s_sum[KA_STEP];
+    __shared__ long long s_sum[KA_WARPS];
     __shared__ __align__(8) unsigned long long bars[KA_WARPS][ST];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int each = a.q_heads / a.c.heads;
 
-    // ---- this block's steps ----
-    const int share = (a.seqs + KA_STEP - 1) / KA_STEP, seq_lo = min(a.seqs, tid * share), seq_hi = min(a.seqs, seq_lo + share);
-    long long own = 0;
-    for (int q = seq_lo; q < seq_hi; q++) own += ka_seq_steps<R>(a, q, each) * a.c.heads;
-    long long before = own;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        const long long x = __shfl_up_sync(0xffffffffu, before, d);
-        if (lane >= d) before += x;
-    }
-    if (lane == 31) s_sum[warp] = before;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < KA_WARPS; w++) {
-        if (w == warp) before += total;
-        total += s_sum[w];
-    }
-    before -= own;
-    const long long blocks = min((long long)gridDim.x, (total + min_steps - 1) / min_steps);
-    if (blockIdx.x >= blocks) return;
-    long long pos = total * blockIdx.x / blocks;
-    const long long end = total * (blockIdx.x + 1) / blocks;
-    if (own && pos >= before && pos < before + own) {  // the thread whose sequences hold the first step
-        long long at = before;
-        for (int q = seq_lo; q < seq_hi; q++) {
-            const long long n = ka_seq_steps<R>(a, q, each) * a.c.heads;
-            if (pos >= at + n) {
-                at += n;
-                continue;
-            }
-            const KaRows r = ka_rows(a, q);
-            for (int rt = 0;; rt++) {
-                const int steps = ka_span<R>(a, r, each, rt).steps;
-                if (pos >= at + (long long)steps * a.c.heads) {
-                    at += (long long)steps * a.c.heads;
-                    continue;
-                }
-                s_unit[0] = q, s_unit[1] = rt, s_unit[2] = (int)((pos - at) / steps), s_unit[3] = (int)((pos - at) % steps);
-                break;
-            }
-            break;
-        }
-    }
-    __syncthreads();
-    int seq = s_unit[0], rt = s_unit[1], head = s_unit[2], skip = s_unit[3];
+    using Cut = KaCut<R, KA_KEYS, KA_STEP>;
+    auto pl = Cut::template place<KA_STEP>(a, each, min_steps, s_sum, s_unit);
+    if (pl.pos >= pl.end) return;
 
     // this warp's ring: each step's key codes, key scales, value codes and value scales come as four bulk copies (eight
     // when the 32 keys lie on two pages of 16), one a lane, that count on the slot's barrier
@@ -210,10 +116,11 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
     const uint32_t from = (cpart & 2 ? off.vc : 0) + (cpart & 1 ? off.ks : 0);  // ks = vs - vc: the codes before the scales
     const uint32_t per_key = cpart & 1 ? NG * 4 : HD / 2, copy_bytes = per_key * KA_KEYS / halves;
     const uint32_t to = (cpart & 2 ? C::KC + C::SC : 0) + (cpart & 1 ? C::KC : 0) + chalf * copy_bytes;
-    while (pos < end) {
+    while (pl.pos < pl.end) {
+    const int seq = pl.seq, head = pl.head, skip = pl.skip, r0 = pl.rt * R;
     const KaRows sr = ka_rows(a, seq);
-    const KaSpan sp = ka_span<R>(a, sr, each, rt);
-    const int piece = (int)min((long long)(sp.steps - skip), end - pos), r0 = rt * R, rows = min(R, sr.n * each - r0);
+    const auto sp = Cut::span(a, sr, each, pl.rt);
+    const int piece = (int)min((long long)(sp.steps - skip), pl.end - pl.pos), rows = min(R, sr.n * each - r0);
     const int lo_min = sp.lo_min, lo_max = sp.lo_max, hi_min = sp.hi_min, hi_max = sp.hi_max;
     const int k0 = sp.base + skip * KA_STEP, k1 = hi_max > lo_min ? min(hi_max, k0 + piece * KA_STEP) : k0;
     const int ntiles = (k1 - k0 + KA_KEYS - 1) / KA_KEYS, mine = max(0, (ntiles - warp + KA_WARPS - 1) / KA_WARPS);
@@ -652,9 +559,8 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
             a.lse[(size_t)(sr.first + (r0 + r) / each) * a.q_heads + head * each + (r0 + r) % each] =
                 (M + log2f(L)) * 0.69314718055994530942f;
     };
-    // a part that begins a unit goes to the block's second slot, one that goes on to its first
     const bool whole = piece == sp.steps;
-    const size_t nslots = 2 * (size_t)gridDim.x, slot = 2 * (size_t)blockIdx.x + (skip == 0);
+    const size_t nslots = 2 * (size_t)gridDim.x, slot = Cut::slot(blockIdx.x, skip == 0);
     float *pms = part + 2 * slot * R, *po = part + 2 * nslots * R + slot * R * HD;
     for (int x = tid; x < rows * HD; x += KA_STEP) {
         const int r = x / HD, c = x % HD;
@@ -677,8 +583,8 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
     }
     if (!whole) {
         // ---- the last of the unit's blocks to arrive joins their states, in their order ----
-        const long long u0 = pos - skip, u1 = u0 + sp.steps;
-        const int b0 = (int)(((u0 + 1) * blocks - 1) / total), b1 = (int)((u1 * blocks - 1) / total), np = b1 - b0 + 1;
+        const int2 who = Cut::sharers(pl, pl.pos - skip, sp.steps);
+        const int b0 = who.x, np = who.y;
         __threadfence();
         __syncthreads();
         if (tid == 0) {
@@ -688,7 +594,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
         __syncthreads();
         if (s_last) {
             __threadfence();
-            auto slot_of = [&](int p) { return 2 * (size_t)(b0 + p) + (p == 0); };
+            auto slot_of = [&](int p) { return Cut::slot(b0 + p, p == 0); };
             const float *po0 = part + 2 * nslots * R;
             for (int r = warp; r < rows; r += KA_WARPS) {  // a warp a row: 32 parts' (maximum, sum) at a time
                 float M = -INFINITY, L = 0.f;
@@ -729,17 +635,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
         }
     }
     // the next unit; its copies (the asynchronous proxy's) come after this one's reads and writes of the same memory
-    pos += piece, skip = 0;
-    if (++head == a.c.heads) {
-        head = 0;
-        if ((++rt) * R >= sr.n * each) {
-            rt = 0;
-            while (++seq < a.seqs) {
-                const KaRows next = ka_rows(a, seq);
-                if (next.ok && next.n) break;
-            }
-        }
-    }
+    Cut::next(pl, a, each, sr.n, piece);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
     }
@@ -750,7 +646,11 @@ static int ka_nt(int dtype, const Kv4AttendArgs &a) {
     return a.max_rows * (a.q_heads / a.c.heads) > 8 && a.c.width * (dtype == DT_F32 ? 2 : 1) <= 128 ? 2 : 1;
 }
 
+// Many rows: tiles of 128 rows on the tensor cores.
+static bool ka_many(const Kv4AttendArgs &a) { return a.c.width <= 128 && a.max_rows * (a.q_heads / a.c.heads) > 32; }
+
 size_t kv4_attend_workspace(int dtype, const Kv4AttendArgs &a, int sms) {
+    if (ka_many(a)) return kv4_attend_tc_workspace(a, sms);
     return 4 * (KA_BLOCKS + (size_t)std::min(KA_BLOCKS, 8 * sms) * 2 * 8 * ka_nt(dtype, a) * (a.c.width + 2));
 }
 
@@ -792,6 +692,8 @@ static cudaError_t launch_size(int dtype, const Kv4AttendArgs &a, int nt, int sm
 cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *work, size_t work_bytes, cudaStream_t s, uint64_t *launches) {
     if (!a.seqs || !a.rows || !a.max_rows) return cudaSuccess;
     if (kv4_attend_workspace(dtype, a, sms) > work_bytes) return cudaErrorInvalidValue;
+    if (launches) ++*launches;
+    if (ka_many(a)) return launch_kv4_attend_tc(dtype, a, sms, work, s);
     const int nt = ka_nt(dtype, a);
     cudaError_t e = cudaErrorInvalidValue;
     const int w = a.c.width, g = a.c.group;
@@ -803,7 +705,6 @@ cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *
     if (w == 256)
         e = g == 32 ? launch_size<256, 32>(dtype, a, nt, sms, work, s)
                     : g == 64 ? launch_size<256, 64>(dtype, a, nt, sms, work, s) : launch_size<256, 128>(dtype, a, nt, sms, work, s);
-    if (launches) ++*launches;
     return e;
 }
 
