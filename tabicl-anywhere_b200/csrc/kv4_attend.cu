@@ -65,22 +65,6 @@ __device__ __forceinline__ float exp2_sfu(float x) {  // relative error 2^-22; 0
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| < 127
 
-template <int N>
-__device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) {  // N consecutive words, aligned to 4 N up to 16
-    if constexpr (N % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < N / 4; i++) {
-            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
-            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-        }
-    } else if constexpr (N == 2) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        w[0] = v.x, w[1] = v.y;
-    } else {
-        w[0] = *reinterpret_cast<const uint32_t *>(p);
-    }
-}
-
 // SPLIT: q and the weights as two f16 (f32 queries), else as one.
 template <int HD, int G, int NT, bool SPLIT>
 __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 : 1)

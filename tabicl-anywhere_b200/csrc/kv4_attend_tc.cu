@@ -316,29 +316,41 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 wait_warp(&mRaw[rs], (uint32_t)(i / NR) & 1u);
                 const uint8_t *kraw = raw + rs * C::RAW, *vraw = kraw + C::KC + C::SC;
                 const bool seen = j >= sp.lo_min && j < sp.hi_max;
-                // the step's power of two, for keys and values: from each group's largest magnitude
+                // the codes of this thread's halves and the scales of its key, all asked for at once
+                uint32_t kw[2 * NU], vw[2 * NU], kc[NG], vc[NG];
+                lds_words<2 * NU>(kraw + key * (HD / 2) + half * NU * 8, kw);
+                lds_words<2 * NU>(vraw + key * (HD / 2) + half * NU * 8, vw);
+                lds_words<NG>(kraw + C::KC + key * NG * 4, kc);
+                lds_words<NG>(vraw + C::KC + key * NG * 4, vc);
+                // the step's power of two, for keys and values: from each group's ends
                 float2 ks[NG], vs[NG];
                 float mx[2] = {0.f, 0.f};
                 bool nan = false;
 #pragma unroll
                 for (int k = 0; k < NG; k++) {
-                    ks[k] = seen ? __half22float2(*(reinterpret_cast<const __half2 *>(kraw + C::KC) + key * NG + k)) : make_float2(0.f, 0.f);
-                    vs[k] = seen ? __half22float2(*(reinterpret_cast<const __half2 *>(vraw + C::KC) + key * NG + k)) : make_float2(0.f, 0.f);
-                    mx[0] = fmaxf(mx[0], fmaxf(fabsf(ks[k].y), fmaxf(fabsf(fmaf(15.f, ks[k].x, ks[k].y)), 15.f * ks[k].x)));
-                    mx[1] = fmaxf(mx[1], fmaxf(fabsf(vs[k].y), fmaxf(fabsf(fmaf(15.f, vs[k].x, vs[k].y)), 15.f * vs[k].x)));
-                    // a group of values that stands for NaN is left out here and put into the rows that see it by the fold
-                    const bool bad = vs[k].y != vs[k].y;
-                    const unsigned who = __ballot_sync(0xffffffffu, bad);
-                    if (half == 0 && lane == 0) nan_keys[i & 7][k][w4] = who;
-                    if (bad) vs[k].y = 0.f;
-                    nan |= who != 0;
+                    ks[k] = seen ? __half22float2(kt_h2(kc[k])) : make_float2(0.f, 0.f);
+                    vs[k] = seen ? __half22float2(kt_h2(vc[k])) : make_float2(0.f, 0.f);
+                    mx[0] = fmaxf(mx[0], fmaxf(fabsf(ks[k].y), fabsf(fmaf(15.f, ks[k].x, ks[k].y))));
+                    mx[1] = fmaxf(mx[1], fmaxf(fabsf(vs[k].y), fabsf(fmaf(15.f, vs[k].x, vs[k].y))));
+                    nan |= vs[k].y != vs[k].y;
                 }
+                // a group of values that stands for NaN is left out here and put into the rows that see it by the fold
+                nan = __any_sync(0xffffffffu, nan);
+                if (nan) {
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-#pragma unroll
-                    for (int d = 16; d > 0; d >>= 1) mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], d));
-                    if (lane == 0) red[i & 1][x][w4] = x && nan ? -mx[x] - 1.f : mx[x];  // a NaN shows as the sign
+                    for (int k = 0; k < NG; k++) {
+                        const bool bad = vs[k].y != vs[k].y;
+                        const unsigned who = __ballot_sync(0xffffffffu, bad);
+                        if (half == 0 && lane == 0) nan_keys[i & 7][k][w4] = who;
+                        if (bad) vs[k].y = 0.f;
+                    }
+                } else if (half == 0 && lane < NG) {
+                    nan_keys[i & 7][lane][w4] = 0;
                 }
+                mx[0] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[0])));  // (not negative: ordered as their bits)
+                mx[1] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[1])));
+                if (lane == 0) red[i & 1][0][w4] = mx[0], red[i & 1][1][w4] = nan ? -mx[1] - 1.f : mx[1];  // a NaN shows as the sign
+                mbar_arrive(&mRawFree[rs]);
                 kt_bar(3, 128);
                 int e[2];
                 bool any = false;
@@ -350,7 +362,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                         const float r = red[i & 1][x][w];
                         any |= r < 0.f, m = fmaxf(m, r < 0.f ? -1.f - r : r);
                     }
-                    e[x] = m > 0.f ? min(40, (int)(__float_as_uint(m) >> 23) - 126) : 0;  // m < 2^e
+                    e[x] = m > 0.f ? min(40, (int)(__float_as_uint(m) >> 23) - 125) : 0;  // m < 2^(e - 1): a span, 15 steps, below 2^e
                 }
                 if (tid % 128 == 0) teK[i & 7] = e[0], teV[i & 7] = e[1], has_nan[i & 7] = any;
                 if (i >= NS) wait_warp(&mKfree[sl], ph ^ 1u);
@@ -362,11 +374,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
                         const int t = 2 * half + x;
-                        const uint32_t *w = reinterpret_cast<const uint32_t *>(kraw + key * (HD / 2)) + t * NU;
 #pragma unroll
                         for (int u = 0; u < NU; u++) {
                             const int o = kmajor_off(key, 32 * u + 8 * t, BK);
-                            kt_widen(w[u], s[u / UG], hi + o, lo + o);
+                            kt_widen(kw[x * NU + u], s[u / UG], hi + o, lo + o);
                         }
                     }
                 }
@@ -381,14 +392,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
                         const int q = 2 * half + x;  // half-words g = 2 q and 2 q + 1 of every unit: coordinates 32 u + 8 q + (0..7)
-                        const uint32_t *w = reinterpret_cast<const uint32_t *>(vraw + key * (HD / 2)) + q * NU;
 #pragma unroll
                         for (int u = 0; u < NU; u++) {
                             uint32_t c;
                             if constexpr (NU == 1)
-                                c = w[0];
+                                c = vw[x];
                             else
-                                c = __byte_perm(w[u / 2], w[NU / 2 + u / 2], u & 1 ? 0x7632 : 0x5410);
+                                c = __byte_perm(vw[x * NU + u / 2], vw[x * NU + NU / 2 + u / 2], u & 1 ? 0x7632 : 0x5410);
                             const int o = mnmajor_off(32 * u + 8 * q, key, HD);
                             kt_widen(c, s[u / UG], hi + o, lo + o);
                         }
@@ -396,7 +406,6 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 }
                 fence_async_smem();
                 mbar_arrive(&mV[sl]);
-                mbar_arrive(&mRawFree[rs]);
             }
             at += n;
             Cut::next(pl, a, each, sr.n, n);

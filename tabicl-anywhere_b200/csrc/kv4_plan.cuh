@@ -12,6 +12,22 @@ namespace tcu {
 
 constexpr int KA_BLOCKS = 2048;  // most blocks of a launch: as many arrival counters start the working memory of every call
 
+template <int N>
+__device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) {  // N consecutive words, aligned to 4 N up to 16
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 v = reinterpret_cast<const uint4 *>(p)[i];
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+}
+
 // A sequence's first row, its rows and cached tokens.
 struct KaRows {
     int first, n, len;
