@@ -13,9 +13,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtabicl_b200.so")
 SOURCES = ["kernels.cu", "attend_tc.cu", "gemm_tc.cu", "stage_rows.cu", "rows.cu", "qmlp_tc.cu", "tree.cu", "peer.cu", "fitcol.cu", "engine.cpp", "tier.cpp", "tirs.cpp", "noalloc.cu",
-           "kv4.cu", "kv4_attend.cu", "kv4_attend_tc.cu", "w4.cu", "logprobs.cu"]
+           "kv4.cu", "kv4_attend.cu", "kv4_attend_tc.cu", "kv4_attend_tc16.cu", "w4.cu", "logprobs.cu"]
 HEADERS = ["device.cuh", "kernels.cuh", "tirs.hpp", "tc.cuh", "stage_common.cuh", "engine.hpp", "fourbit.cuh",
-           "kv4_plan.cuh", "pdl.cuh"]
+           "kv4_plan.cuh", "kv4_tc.cuh", "pdl.cuh"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-O3", "-std=c++17", "-lineinfo",

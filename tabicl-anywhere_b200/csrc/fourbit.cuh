@@ -98,9 +98,11 @@ cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *
                               uint64_t *launches);
 // kernels.cu: opt a kernel in to `bytes` of dynamic shared memory on the current device.
 cudaError_t allow_dynamic_smem(const void *kernel, size_t bytes);
-// The same by tensor-core tiles of 128 rows: for many rows a cache head (widths up to 128).
+// The same on the tensor cores, for many rows a cache head (widths up to 128): f32, and 16-bit types.
 size_t kv4_attend_tc_workspace(const Kv4AttendArgs &a, int sms);
-cudaError_t launch_kv4_attend_tc(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s);
+cudaError_t launch_kv4_attend_tc(const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s);
+size_t kv4_attend_tc16_workspace(const Kv4AttendArgs &a, int sms);
+cudaError_t launch_kv4_attend_tc16(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s);
 // A weight matrix w [n][k] (row stride ldw) to codes and scales.
 cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k, int group, uint8_t *codes,
                            __half2 *scales, cudaStream_t s, uint64_t *launches);

@@ -634,7 +634,7 @@ static int ka_nt(int dtype, const Kv4AttendArgs &a) {
 static bool ka_many(const Kv4AttendArgs &a) { return a.c.width <= 128 && a.max_rows * (a.q_heads / a.c.heads) > 32; }
 
 size_t kv4_attend_workspace(int dtype, const Kv4AttendArgs &a, int sms) {
-    if (ka_many(a)) return kv4_attend_tc_workspace(a, sms);
+    if (ka_many(a)) return dtype == DT_F32 ? kv4_attend_tc_workspace(a, sms) : kv4_attend_tc16_workspace(a, sms);
     return 4 * (KA_BLOCKS + (size_t)std::min(KA_BLOCKS, 8 * sms) * 2 * 8 * ka_nt(dtype, a) * (a.c.width + 2));
 }
 
@@ -677,7 +677,7 @@ cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *
     if (!a.seqs || !a.rows || !a.max_rows) return cudaSuccess;
     if (kv4_attend_workspace(dtype, a, sms) > work_bytes) return cudaErrorInvalidValue;
     if (launches) ++*launches;
-    if (ka_many(a)) return launch_kv4_attend_tc(dtype, a, sms, work, s);
+    if (ka_many(a)) return dtype == DT_F32 ? launch_kv4_attend_tc(a, sms, work, s) : launch_kv4_attend_tc16(dtype, a, sms, work, s);
     const int nt = ka_nt(dtype, a);
     cudaError_t e = cudaErrorInvalidValue;
     const int w = a.c.width, g = a.c.group;

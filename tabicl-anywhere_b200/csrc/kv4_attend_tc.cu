@@ -12,15 +12,11 @@
 #include <algorithm>
 #include <atomic>
 
-#include "kv4_plan.cuh"
-#include "tc.cuh"
+#include "kv4_tc.cuh"
 
 namespace tcu {
 
-using namespace tc;
-
-constexpr int KT_BQ = 128, KT_BK = 64, KT_NS = 3, KT_NR = 2, KT_THREADS = 512;
-constexpr long long KT_WAIT = 2000000000ll;  // about a second at boost clock
+constexpr int KT_BQ = 128, KT_BK = 64, KT_NS = 3, KT_THREADS = 512;
 constexpr uint32_t KT_TQ = 0, KT_TS = 128, KT_TO = 384;
 
 template <int HD, int G, bool SPLIT>
@@ -28,56 +24,10 @@ struct KtShape {
     static constexpr int NU = HD / 32, NG = HD / G, QS = SPLIT ? 2 : 1;
     static constexpr int BLOCK = KT_BK * HD;                            // f16 of one operand block
     static constexpr int KC = KT_BK * HD / 2, SC = KT_BK * NG * 4, RAW = 2 * (KC + SC);
+    static constexpr int NR = SPLIT ? 2 : 4;                            // slots of stored codes: what shared memory leaves
     static constexpr int T = SPLIT ? 13 : -5;                           // widened values are below 2^T
-    static constexpr size_t SMEM = (size_t)2 * KT_NS * QS * BLOCK * 2 + (size_t)KT_NR * RAW + 1024;
+    static constexpr size_t SMEM = (size_t)2 * KT_NS * QS * BLOCK * 2 + (size_t)NR * RAW + 1024;
 };
-
-__device__ __forceinline__ float kt_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| < 127
-__device__ __forceinline__ float kt_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ void kt_bar(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ __half2 kt_h2(uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); }
-__device__ __forceinline__ uint32_t kt_u32(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
-
-// One group's scales for widening: value = code nibble as f16 * even (a byte's first nibble) or * odd (its second) + low.
-template <bool SPLIT>
-struct KtScale;
-template <>
-struct KtScale<false> {
-    __half2 even, odd, low;
-    __device__ __forceinline__ void set(float step, float l, float up) {
-        const float s = step * up * 16777216.f;
-        even = __float2half2_rn(s), odd = __float2half2_rn(s * 0.0625f), low = __float2half2_rn(l * up);
-    }
-};
-template <>
-struct KtScale<true> {
-    float even, odd, low;
-    __device__ __forceinline__ void set(float step, float l, float up) {
-        even = step * up * 16777216.f, odd = even * 0.0625f, low = l * up;
-    }
-};
-// A word's eight values as f16 (and what remains of them) into 16 bytes each.
-__device__ __forceinline__ void kt_widen(uint32_t w, const KtScale<false> &s, __half *hi, __half *) {
-    const uint32_t v = w >> 8;
-    *reinterpret_cast<uint4 *>(hi) = make_uint4(kt_u32(__hfma2(kt_h2(w & 0x000f000fu), s.even, s.low)), kt_u32(__hfma2(kt_h2(w & 0x00f000f0u), s.odd, s.low)),
-                                                kt_u32(__hfma2(kt_h2(v & 0x000f000fu), s.even, s.low)), kt_u32(__hfma2(kt_h2(v & 0x00f000f0u), s.odd, s.low)));
-}
-__device__ __forceinline__ void kt_widen(uint32_t w, const KtScale<true> &s, __half *hi, __half *lo) {
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t v = i & 2 ? w >> 8 : w;
-        const float2 c = __half22float2(kt_h2(i & 1 ? v & 0x00f000f0u : v & 0x000f000fu));
-        const float f = i & 1 ? s.odd : s.even;
-        split_pair(fmaf(c.x, f, s.low), fmaf(c.y, f, s.low), h[i], l[i]);
-    }
-    *reinterpret_cast<uint4 *>(hi) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4 *>(lo) = make_uint4(l[0], l[1], l[2], l[3]);
-}
 
 // Warps 0-3: softmax, a thread a query row; warps 4-7: the fold of each step's P V, a thread a row; warps 8-11: widening;
 // warp 12, 13: one thread each issues the S products of even and odd steps; warp 14: one thread the P V products; warp 15:
@@ -87,7 +37,7 @@ template <int HD, int G, bool SPLIT>
 __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a, int dtype, float *part, int *arrived) {
     using C = KtShape<HD, G, SPLIT>;
     using Cut = KaCut<KT_BQ, KT_BK, KT_BK>;
-    constexpr int NU = C::NU, NG = C::NG, UG = G / 32, QS = C::QS, BQ = KT_BQ, BK = KT_BK, NS = KT_NS, NR = KT_NR, BLOCK = C::BLOCK;
+    constexpr int NU = C::NU, NG = C::NG, UG = G / 32, QS = C::QS, BQ = KT_BQ, BK = KT_BK, NS = KT_NS, NR = C::NR, BLOCK = C::BLOCK;
     extern __shared__ __align__(1024) uint8_t smraw[];
     __half *Kring = reinterpret_cast<__half *>(smraw);                // [NS][QS][64 x HD], K-major
     __half *Vring = Kring + NS * QS * BLOCK;                          // [NS][QS][64 x HD], coordinate-major
@@ -213,10 +163,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 const KaRows sr = ka_rows(a, pl.seq);
                 const auto sp = Cut::span(a, sr, each, pl.rt);
                 const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), j0 = sp.base + pl.skip * BK;
+                auto find = [&](int i) {  // a step's page, read two steps before it is needed; -2: nothing there to be seen
+                    const int j = j0 + i * BK + cp * keys;
+                    return i < n && cp < pieces && j < sp.hi_max && j + keys > sp.lo_min ? a.table[pl.seq * a.table_stride + (j >> shift)] : -2;
+                };
+                int next = find(0), after = find(1);
                 for (int i = 0; i < n; i++, at++) {
-                    const int j = j0 + i * BK + cp * keys, slot = at % NR;
-                    const bool there = cp < pieces && j < sp.hi_max && j + keys > sp.lo_min;
-                    const int pg = there ? a.table[pl.seq * a.table_stride + (j >> shift)] : -1;
+                    const int j = j0 + i * BK + cp * keys, slot = at % NR, pg = next;
+                    const bool there = pg != -2 || (i < n && cp < pieces && j < sp.hi_max && j + keys > sp.lo_min);
+                    next = after, after = find(i + 2);
                     const bool ok = pg >= 0 && pg < a.c.pages;
                     if (there && !ok) *reinterpret_cast<volatile int *>(a.err) = 1;
                     const unsigned mask = __ballot_sync(0xffffffffu, ok && cpart == 0);
@@ -604,24 +559,22 @@ size_t kv4_attend_tc_workspace(const Kv4AttendArgs &a, int sms) {
     return 4 * (KA_BLOCKS + (size_t)2 * std::min(KA_BLOCKS, sms) * KT_BQ * (a.c.width + 2));
 }
 
-template <int HD, int G, bool SPLIT>
-static cudaError_t launch_tc(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
-    const size_t smem = KtShape<HD, G, SPLIT>::SMEM;
-    cudaError_t e = allow_dynamic_smem((const void *)k_kv4_attend_tc<HD, G, SPLIT>, smem);
+template <int HD, int G>
+static cudaError_t launch_tc(const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
+    const size_t smem = KtShape<HD, G, true>::SMEM;
+    cudaError_t e = allow_dynamic_smem((const void *)k_kv4_attend_tc<HD, G, true>, smem);
     if (e != cudaSuccess) return e;
-    k_kv4_attend_tc<HD, G, SPLIT><<<std::min(sms, KA_BLOCKS), KT_THREADS, smem, s>>>(a, dtype, reinterpret_cast<float *>(work) + KA_BLOCKS,
-                                                                                    reinterpret_cast<int *>(work));
+    k_kv4_attend_tc<HD, G, true><<<std::min(sms, KA_BLOCKS), KT_THREADS, smem, s>>>(a, DT_F32, reinterpret_cast<float *>(work) + KA_BLOCKS,
+                                                                                   reinterpret_cast<int *>(work));
     return cudaGetLastError();
 }
 
-cudaError_t launch_kv4_attend_tc(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
-    const bool f32 = dtype == DT_F32;
+cudaError_t launch_kv4_attend_tc(const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
     const int g = a.c.group;
-#define TCU_KT(hd, gr) (f32 ? launch_tc<hd, gr, true>(dtype, a, sms, work, s) : launch_tc<hd, gr, false>(dtype, a, sms, work, s))
-    if (a.c.width == 32) return TCU_KT(32, 32);
-    if (a.c.width == 64) return g == 32 ? TCU_KT(64, 32) : TCU_KT(64, 64);
-    if (a.c.width == 128) return g == 32 ? TCU_KT(128, 32) : g == 64 ? TCU_KT(128, 64) : TCU_KT(128, 128);
-#undef TCU_KT
+    if (a.c.width == 32) return launch_tc<32, 32>(a, sms, work, s);
+    if (a.c.width == 64) return g == 32 ? launch_tc<64, 32>(a, sms, work, s) : launch_tc<64, 64>(a, sms, work, s);
+    if (a.c.width == 128)
+        return g == 32 ? launch_tc<128, 32>(a, sms, work, s) : g == 64 ? launch_tc<128, 64>(a, sms, work, s) : launch_tc<128, 128>(a, sms, work, s);
     return cudaErrorInvalidValue;
 }
 

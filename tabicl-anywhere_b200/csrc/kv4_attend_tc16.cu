@@ -1,0 +1,567 @@
+// Attention of many query rows of a 16-bit type over the four-bit cache on the 5th-generation tensor cores (tcgen05).
+//
+// 256 query rows of one cache head (the heads that share it side by side) as two tiles of 128, against 64 keys at a time:
+// S = Q K^T with Q and the keys, widened to f16, in shared memory; the weights P go to tensor memory over S and multiply
+// the widened values; the output stays in tensor memory. Keys, values and weights are one f16 each (11 bits; the results
+// have 11 or 8), sums are f32. What bounds it is the exponentials (16 a cycle and SM) beside the instructions that feed
+// them, so the two tiles have a warpgroup each, and widening, which serves both, two that take the steps in turn.
+//
+// A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8, so the output
+// in tensor memory is rarely rescaled. A step's keys and values are scaled by a power of two of their own that keeps them
+// inside f16, whatever the cache holds; the output is in units of the largest step's. Coordinates keep the order the codes
+// are unpacked in, (0, 4, 1, 5, 2, 6, 3, 7) of every eight: Q takes the same order, and the output's columns are put back
+// when they are written.
+#include <algorithm>
+
+#include "kv4_tc.cuh"
+
+namespace tcu {
+
+constexpr int KU_R = 256, KU_BQ = 128, KU_BK = 64, KU_NS = 3, KU_NR = 4, KU_THREADS = 640;
+constexpr int KU_T = -5;  // widened values are below 2^T
+constexpr uint32_t KU_TS = 0, KU_TO = 256;  // tensor memory: [tile][2 slots] of S / P, then [tile] of O
+
+template <int HD, int G>
+struct KuShape {
+    static constexpr int NU = HD / 32, NG = HD / G, BLOCK = KU_BK * HD;
+    static constexpr int KC = KU_BK * HD / 2, SC = KU_BK * NG * 4, RAW = 2 * (KC + SC);
+    static constexpr size_t SMEM = (size_t)KU_R * HD * 2 + (size_t)2 * KU_NS * BLOCK * 2 + (size_t)KU_NR * RAW + 1024;
+};
+
+// Warps 0-3, 4-7: softmax of the first and second tile, a thread a query row; warps 8-11, 12-15: widening of even and odd
+// steps; warp 16: one thread issues the S products; warp 17: one thread the P V products; warp 18: the copies of the stored
+// codes. They hand over through mbarriers; every wait is bounded, and one that gives up raises the block's abort flag, after
+// which every wait returns at once and the roles run to the end without results.
+template <int HD, int G>
+__global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs a, int dtype, float *part, int *arrived) {
+    using C = KuShape<HD, G>;
+    using Cut = KaCut<KU_R, KU_BK, KU_BK>;
+    constexpr int NU = C::NU, NG = C::NG, UG = G / 32, BQ = KU_BQ, BK = KU_BK, NS = KU_NS, NR = KU_NR, BLOCK = C::BLOCK;
+    extern __shared__ __align__(1024) uint8_t smraw[];
+    __half *Qs = reinterpret_cast<__half *>(smraw);   // [2][128 x HD], K-major
+    __half *Kring = Qs + KU_R * HD;                   // [NS][64 x HD], K-major
+    __half *Vring = Kring + NS * BLOCK;               // [NS][64 x HD], coordinate-major
+    uint8_t *raw = reinterpret_cast<uint8_t *>(Vring + NS * BLOCK);  // [NR]{key codes, key scales, value codes, value scales}
+    __shared__ float red[2][2][2][4];  // [turn][step][keys, values][warp]
+    __shared__ int teK[8], teV[8], has_nan[8];
+    __shared__ uint32_t nan_keys[8][NG][2];
+    __shared__ __align__(8) uint64_t mK[NS], mV[NS], mKfree[NS], mVfree[NS], mS[2][2], mP[2][2], mSlot[2][2], mQ[2], mDone[2], mRaw[NR],
+        mRawFree[NR];
+    __shared__ uint32_t tslot;
+    __shared__ volatile int abort_flag;
+    __shared__ int s_unit[4], s_last[2];
+    __shared__ long long s_sum[KU_THREADS / 32];
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
+    const int each = a.q_heads / a.c.heads;
+    auto pl = Cut::template place<KU_THREADS>(a, each, 1, s_sum, s_unit);
+    if (pl.pos >= pl.end) return;
+    if (warp == 0) {
+        tmem_alloc(&tslot, 512);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        for (int i = 0; i < NS; i++) mbar_init(&mK[i], 128), mbar_init(&mV[i], 128), mbar_init(&mKfree[i], 1), mbar_init(&mVfree[i], 1);
+        for (int q = 0; q < 2; q++) {
+            for (int i = 0; i < 2; i++) mbar_init(&mS[q][i], 1), mbar_init(&mP[q][i], BQ), mbar_init(&mSlot[q][i], 1);
+            mbar_init(&mQ[q], BQ), mbar_init(&mDone[q], 1);
+        }
+        for (int i = 0; i < NR; i++) mbar_init(&mRaw[i], 1), mbar_init(&mRawFree[i], 128);
+        mbar_init_fence();
+        abort_flag = 0;
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = tslot;
+
+    auto wait = [&](uint64_t *m, uint32_t parity) {
+        if (mbar_test_wait(m, parity)) return true;
+        if (abort_flag) return false;
+        if (!mbar_wait(m, parity, KT_WAIT)) {
+            abort_flag = 1;
+            return false;
+        }
+        return true;
+    };
+    auto wait_warp = [&](uint64_t *m, uint32_t parity) {  // warp-uniform: warp-wide instructions follow
+        bool ok = mbar_test_wait(m, parity) || (!abort_flag && mbar_wait(m, parity, KT_WAIT));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) abort_flag = 1;
+        return ok;
+    };
+    // Every role walks the block's pieces of units alike: n steps; `at` counts the steps before them, at1 those of the second
+    // tile (a piece of at most 128 rows has none).
+    int at = 0, at1 = 0;
+
+    if (wg == 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 18) {
+            // ---- copies: lane part + 4 * piece brings one of the four arrays of one page's share of the 64 keys ----
+            const Kv4Offsets off = kv4_offsets(HD, a.c.page, G);
+            const size_t hb = kv4_head_bytes(HD, a.c.page, G);
+            const int page = a.c.page, shift = 31 - __clz(page), keys = min(page, BK), pieces = BK / keys;
+            const int cpart = lane & 3, cp = lane >> 2;
+            const uint32_t per_key = cpart & 1 ? NG * 4 : HD / 2, bytes = per_key * keys;
+            const uint32_t from = (cpart & 2 ? off.vc : 0) + (cpart & 1 ? off.ks : 0);
+            const uint32_t to = (cpart & 2 ? C::KC + C::SC : 0) + (cpart & 1 ? C::KC : 0) + cp * bytes;
+            while (pl.pos < pl.end) {
+                const KaRows sr = ka_rows(a, pl.seq);
+                const auto sp = Cut::span(a, sr, each, pl.rt);
+                const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), j0 = sp.base + pl.skip * BK + cp * keys;
+                const int *table = a.table + pl.seq * a.table_stride;
+                auto there = [&](int i) { return i < n && cp < pieces && j0 + i * BK < sp.hi_max && j0 + i * BK + keys > sp.lo_min; };
+                auto find = [&](int i) { return there(i) ? table[(j0 + i * BK) >> shift] : -1; };  // a page number, two steps ahead
+                int next = find(0), after = find(1);
+                for (int i = 0; i < n; i++, at++) {
+                    const int slot = at % NR, pg = next;
+                    next = after, after = find(i + 2);
+                    const bool ok = pg >= 0 && pg < a.c.pages;
+                    if (there(i) && !ok) *reinterpret_cast<volatile int *>(a.err) = 1;
+                    const unsigned mask = __ballot_sync(0xffffffffu, ok && cpart == 0);
+                    if (at >= NR && !wait_warp(&mRawFree[slot], (uint32_t)(at / NR - 1) & 1u)) break;
+                    if (lane == 0)
+                        asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}\n" ::"r"(smem_addr(&mRaw[slot])),
+                                     "r"((uint32_t)(__popc(mask) * (C::RAW / pieces)))
+                                     : "memory");
+                    if (ok)
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                         smem_addr(raw + slot * C::RAW + to)),
+                                     "l"(a.c.pool + ((size_t)pg * a.c.heads + pl.head) * hb + from + ((j0 + i * BK) & (page - 1)) * per_key),
+                                     "r"(bytes), "r"(smem_addr(&mRaw[slot]))
+                                     : "memory");
+                }
+                Cut::next(pl, a, each, sr.n, n);
+            }
+            // what was asked for lands before the block lets go of shared memory
+            for (int i = max(0, at - NR); i < at; i++) mbar_wait(&mRaw[i % NR], (uint32_t)(i / NR) & 1u, KT_WAIT);
+        } else if (warp < 18 && lane == 0) {
+            // ---- the products ----
+            const uint32_t idS = idesc_f16(BQ, BK, 0, 0), idO = idesc_f16(BQ, HD, 0, 1);
+            const uint64_t dQ0 = kstep_desc(Qs, BQ, 0), dK0 = kstep_desc(Kring, BK, 0), dV0 = kstep_desc(Vring, HD, 0);
+            const uint64_t stQ = (2 * (BQ / 8) * 128) >> 4, stK = (2 * (BK / 8) * 128) >> 4, stV = (2 * (HD / 8) * 128) >> 4;
+            constexpr uint64_t q_off = (BQ * HD * 2) >> 4, slot_off = (BLOCK * 2) >> 4;
+            int units[2] = {0, 0};  // pieces of each tile so far
+            while (pl.pos < pl.end) {
+                const KaRows sr = ka_rows(a, pl.seq);
+                const auto sp = Cut::span(a, sr, each, pl.rt);
+                const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), nq = sr.n * each - pl.rt * KU_R > BQ ? 2 : 1;
+                for (int i = 0; i < n; i++) {
+                    const int sl = (at + i) % NS;
+                    const uint32_t ph = (uint32_t)((at + i) / NS) & 1u;
+                    if (warp == 16) {
+                        // S(i) of both tiles from the keys of step i, once P V(i - 2) has read the slot
+                        if (!wait(&mK[sl], ph)) break;
+                        bool ok = true;
+                        for (int q = 0; q < nq && ok; q++) {
+                            const int c = (q ? at1 : at) + i;
+                            if (i == 0 && !(ok = wait(&mQ[q], (uint32_t)units[q] & 1u))) break;
+                            if (c >= 2 && !(ok = wait(&mSlot[q][c & 1], (uint32_t)((c >> 1) - 1) & 1u))) break;
+                            fence_after_sync();
+#pragma unroll
+                            for (int k = 0; k < HD / 16; k++)
+                                mma_f16(tmem + KU_TS + (2 * q + (c & 1)) * BK, dQ0 + q * q_off + k * stQ, dK0 + sl * slot_off + k * stK, idS, k > 0 ? 1u : 0u);
+                            mma_commit(&mS[q][c & 1]);
+                        }
+                        if (!ok) break;
+                        mma_commit(&mKfree[sl]);
+                    } else {
+                        // P V(i) of both tiles, from the values of step i
+                        if (!wait(&mV[sl], ph)) break;
+                        bool ok = true;
+                        for (int q = 0; q < nq && ok; q++) {
+                            const int c = (q ? at1 : at) + i;
+                            if (!(ok = wait(&mP[q][c & 1], (uint32_t)(c >> 1) & 1u))) break;
+                            fence_after_sync();
+#pragma unroll
+                            for (int k = 0; k < BK / 16; k++)
+                                mma_f16_ta(tmem + KU_TO + q * HD, tmem + KU_TS + (2 * q + (c & 1)) * BK + 8 * k, dV0 + sl * slot_off + k * stV, idO,
+                                           i > 0 || k > 0 ? 1u : 0u);
+                            mma_commit(&mSlot[q][c & 1]);
+                        }
+                        if (!ok) break;
+                        mma_commit(&mVfree[sl]);
+                    }
+                }
+                units[0]++, units[1] += nq == 2;
+                at += n, at1 += nq == 2 ? n : 0;
+                Cut::next(pl, a, each, sr.n, n);
+            }
+            // every product issued here completes before the block lets go of its memory
+            mma_commit(&mDone[warp - 16]);
+            mbar_wait(&mDone[warp - 16], 0, KT_WAIT);
+        }
+    } else if (wg >= 2) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // ---- widening: a thread half a key's coordinates and half a value's, of every other step ----
+        // (a wait that gave up does not end the loop: the four warps meet at a barrier in every step)
+        const int key = tid & 63, half = (tid >> 6) & 1, w4 = warp & 3, turn = wg - 2;
+        while (pl.pos < pl.end) {
+            const KaRows sr = ka_rows(a, pl.seq);
+            const auto sp = Cut::span(a, sr, each, pl.rt);
+            const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), j0 = sp.base + pl.skip * BK;
+            for (int i = at + ((at ^ turn) & 1); i < at + n; i += 2) {
+                const int sl = i % NS, rs = i % NR, j = j0 + (i - at) * BK + key;
+                const uint32_t ph = (uint32_t)(i / NS) & 1u;
+                wait_warp(&mRaw[rs], (uint32_t)(i / NR) & 1u);
+                const uint8_t *kraw = raw + rs * C::RAW, *vraw = kraw + C::KC + C::SC;
+                const bool seen = j >= sp.lo_min && j < sp.hi_max;
+                // the codes of this thread's halves and the scales of its key, all asked for at once
+                uint32_t kw[2 * NU], vw[2 * NU], kc[NG], vc[NG];
+                lds_words<2 * NU>(kraw + key * (HD / 2) + half * NU * 8, kw);
+                lds_words<2 * NU>(vraw + key * (HD / 2) + half * NU * 8, vw);
+                lds_words<NG>(kraw + C::KC + key * NG * 4, kc);
+                lds_words<NG>(vraw + C::KC + key * NG * 4, vc);
+                // the step's power of two, for keys and values: from each group's ends
+                float mx[2] = {0.f, 0.f};
+                bool nan = false;
+#pragma unroll
+                for (int k = 0; k < NG; k++) {
+                    if (!seen) kc[k] = vc[k] = 0;
+                    const float2 ks = __half22float2(kt_h2(kc[k])), vs = __half22float2(kt_h2(vc[k]));
+                    mx[0] = fmaxf(mx[0], fmaxf(fabsf(ks.y), fabsf(fmaf(15.f, ks.x, ks.y))));
+                    mx[1] = fmaxf(mx[1], fmaxf(fabsf(vs.y), fabsf(fmaf(15.f, vs.x, vs.y))));
+                    nan |= vs.y != vs.y;
+                }
+                // a group of values that stands for NaN is left out here and put into the rows that see it at the end
+                nan = __any_sync(0xffffffffu, nan);
+                if (nan) {
+#pragma unroll
+                    for (int k = 0; k < NG; k++) {
+                        const bool bad = (vc[k] & 0x7fff0000u) > 0x7c000000u;
+                        const unsigned who = __ballot_sync(0xffffffffu, bad);
+                        if (half == 0 && lane == 0) nan_keys[i & 7][k][w4] = who;
+                        if (bad) vc[k] = 0;
+                    }
+                } else if (half == 0 && lane < NG) {
+                    nan_keys[i & 7][lane][w4] = 0;
+                }
+                mx[0] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[0])));  // (not negative: ordered as their bits)
+                mx[1] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[1])));
+                if (lane == 0) red[turn][i >> 1 & 1][0][w4] = mx[0], red[turn][i >> 1 & 1][1][w4] = nan ? -mx[1] - 1.f : mx[1];  // a NaN shows as the sign
+                mbar_arrive(&mRawFree[rs]);
+                kt_bar(1 + turn, 128);
+                int e[2];
+                bool any = false;
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    float m = 0.f;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const float r = red[turn][i >> 1 & 1][x][w];
+                        any |= r < 0.f, m = fmaxf(m, r < 0.f ? -1.f - r : r);
+                    }
+                    e[x] = m > 0.f ? min(40, (int)(__float_as_uint(m) >> 23) - 125) : 0;  // m < 2^(e - 1): a span, 15 steps, below 2^e
+                }
+                if (tid % 128 == 0) teK[i & 7] = e[0], teV[i & 7] = e[1], has_nan[i & 7] = any;
+                if (i >= NS) wait_warp(&mKfree[sl], ph ^ 1u);
+#pragma unroll
+                for (int k = 0; k < NG; k++) {
+                    KtScale<false> s;
+                    const float2 f = __half22float2(kt_h2(kc[k]));
+                    s.set(f.x, f.y, kt_pow2(KU_T - e[0]));
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int u = k * UG; u < (k + 1) * UG; u++)
+                            kt_widen(kw[x * NU + u], s, Kring + sl * BLOCK + kmajor_off(key, 32 * u + 8 * (2 * half + x), BK), nullptr);
+                }
+                fence_async_smem();
+                mbar_arrive(&mK[sl]);
+                if (i >= NS) wait_warp(&mVfree[sl], ph ^ 1u);
+#pragma unroll
+                for (int k = 0; k < NG; k++) {
+                    KtScale<false> s;
+                    const float2 f = __half22float2(kt_h2(vc[k]));
+                    s.set(f.x, f.y, kt_pow2(KU_T - e[1]));
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int u = k * UG; u < (k + 1) * UG; u++) {
+                            // half-words g = 2 q and 2 q + 1 of a unit: coordinates 32 u + 8 q + (0..7)
+                            uint32_t c;
+                            if constexpr (NU == 1)
+                                c = vw[x];
+                            else
+                                c = __byte_perm(vw[x * NU + u / 2], vw[x * NU + NU / 2 + u / 2], u & 1 ? 0x7632 : 0x5410);
+                            kt_widen(c, s, Vring + sl * BLOCK + mnmajor_off(32 * u + 8 * (2 * half + x), key, HD), nullptr);
+                        }
+                }
+                fence_async_smem();
+                mbar_arrive(&mV[sl]);
+            }
+            at += n;
+            Cut::next(pl, a, each, sr.n, n);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        const int q = wg, row = tid & (BQ - 1);
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const int es = 2;
+        const bool wide_q = !(((uintptr_t)a.q & 15) || ((a.q_row | a.q_head) * es) % 16);
+        const bool wide_o = !(((uintptr_t)a.out & 15) || ((a.o_row | a.o_head) * es) % 16);
+        while (pl.pos < pl.end) {
+            const KaRows sr = ka_rows(a, pl.seq);
+            const auto sp = Cut::span(a, sr, each, pl.rt);
+            const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), j0 = sp.base + pl.skip * BK;
+            const int r0 = pl.rt * KU_R + q * BQ, rows = min(BQ, sr.n * each - r0);
+            if (rows <= 0) {
+                at += n;
+                Cut::next(pl, a, each, sr.n, n);
+                continue;
+            }
+            const int r = min(row, rows - 1), ri = (r0 + r) / each, hq = pl.head * each + (r0 + r) % each;  // rows past the end repeat the last
+            const int my_hi = ka_hi(a, sr, ri), my_lo = ka_lo(a, sr, ri);
+            const int hi_min = ka_hi(a, sr, r0 / each), lo_max = ka_lo(a, sr, (r0 + rows - 1) / each);
+            int c = q ? at1 : at;  // this tile's steps so far
+
+            // ---- Q: a thread a row, scaled by a power of two of the row's to at most 2^14 ----
+            float rowfac;
+            {
+                uint32_t w[HD / 2];
+                const long long from = (long long)(sr.first + ri) * a.q_row + (long long)hq * a.q_head;
+                const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + from;
+                if (wide_q) {
+#pragma unroll
+                    for (int b = 0; b < HD / 8; b++) {
+                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src) + b);
+                        w[4 * b] = v.x, w[4 * b + 1] = v.y, w[4 * b + 2] = v.z, w[4 * b + 3] = v.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < HD / 2; b++) w[b] = (uint32_t)src[2 * b] | (uint32_t)src[2 * b + 1] << 16;
+                }
+                auto get = [&](uint32_t x) {
+                    return dtype == DT_BF16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : __half22float2(kt_h2(x));
+                };
+                float mx = 0.f;
+#pragma unroll
+                for (int b = 0; b < HD / 2; b++) {
+                    const float2 v = get(w[b]);
+                    mx = fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y)));
+                }
+                const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
+                const float up = a.scale < 0.f ? -kt_pow2(e) : kt_pow2(e);
+                // a score in units of log2: the product with the widened keys times this and the step's power of two (a scale of
+                // 0 as 2^-100, so that the factor is positive)
+                rowfac = fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * kt_pow2(-e);
+#pragma unroll
+                for (int b = 0; b < HD / 8; b++) {
+                    float v[8];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const float2 f = get(w[4 * b + x]);
+                        v[2 * x] = f.x * up, v[2 * x + 1] = f.y * up;
+                    }
+                    uint32_t h[4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) h[x] = kt_u32(__floats2half2_rn(v[x], v[x + 4]));
+                    *reinterpret_cast<uint4 *>(Qs + q * BQ * HD + kmajor_off(row, 8 * b, BQ)) = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+                fence_async_smem();
+                mbar_arrive(&mQ[q]);
+            }
+
+            // ---- softmax: S(i) -> P(i) over S(i) ----
+            float m = -INFINITY, l = 0.f;  // the row's reference (log2), its sum of weights times 2^7
+            int unit = 0;                  // the output is in units of 2^(unit - T - 7)
+            uint32_t nans = 0;             // groups whose output is NaN
+            for (int i = 0; i < n; i++, c++) {
+                const int key0 = j0 + i * BK, x8 = (at + i) & 7;
+                const uint32_t tsp = tmem + lane_base + KU_TS + (2 * q + (c & 1)) * BK;
+                if (!wait_warp(&mS[q][c & 1], (uint32_t)(c >> 1) & 1u)) break;
+                fence_after_sync();
+                const float c1 = rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_T);
+                const int e = *reinterpret_cast<volatile int *>(&teV[x8]);
+                float s[64];
+                {
+                    float x[32], y[32];
+                    tmem_ld32(tsp, x);
+                    tmem_ld32(tsp + 32, y);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 32; k++) s[k] = x[k], s[32 + k] = y[k];
+                }
+                if (key0 < lo_max || key0 + BK > hi_min) {
+#pragma unroll
+                    for (int k = 0; k < 64; k++)
+                        if (key0 + k < my_lo || key0 + k >= my_hi) s[k] = -INFINITY;
+                }
+                float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int k = 4; k < 64; k++) top[k & 3] = fmaxf(top[k & 3], s[k]);
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c1;
+                if (i == 0) unit = e;
+                if (__any_sync(0xffffffffu, mx > m + 8.f) || e > unit) {
+                    const float mnew = fmaxf(m, mx), f = m == -INFINITY ? 0.f : kt_ex2(m - mnew);
+                    const int unew = max(unit, e);
+                    if (i > 0) {  // O, once the product before has been added to it
+                        if (!wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u)) break;
+                        fence_after_sync();
+                        const float fo = f * kt_pow2(unit - unew);
+#pragma unroll 1
+                        for (int b = 0; b < HD / 32; b++) {
+                            float x[32];
+                            tmem_ld32(tmem + lane_base + KU_TO + q * HD + 32 * b, x);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; k++) x[k] *= fo;
+                            tmem_st32(tmem + lane_base + KU_TO + q * HD + 32 * b, x);
+                        }
+                        tmem_wait_st();
+                    }
+                    l *= f, m = mnew, unit = unew;
+                }
+                // weights times 2^7 (up to 2^15), in units of the step's values
+                const float mm = (m == -INFINITY ? 0.f : m) - 7.f - (float)(e - unit);
+                float sum[4] = {};
+                uint32_t h[32];
+#pragma unroll
+                for (int k = 0; k < 32; k++) {
+                    const float p0 = kt_ex2(fmaf(s[2 * k], c1, -mm)), p1 = kt_ex2(fmaf(s[2 * k + 1], c1, -mm));
+                    sum[(2 * k) & 3] += p0, sum[(2 * k + 1) & 3] += p1;
+                    h[k] = kt_u32(__floats2half2_rn(p0, p1));
+                }
+                tmem_st32u(tsp, h);
+                tmem_wait_st();
+                fence_before_sync();
+                mbar_arrive(&mP[q][c & 1]);
+                l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), kt_pow2(unit - e), l);
+                if (*reinterpret_cast<volatile int *>(&has_nan[x8])) {
+                    for (int k = 0; k < NG; k++)
+                        for (int b = 0; b < 64; b++)
+                            if ((nan_keys[x8][k][b >> 5] >> (b & 31) & 1) && key0 + b >= my_lo && key0 + b < my_hi) nans |= 1u << k;
+                }
+            }
+
+            // ---- the row's output, or its part of it ----
+            const bool whole = n == sp.steps;
+            bool write = row < rows;
+            float M = m, L = l * 0.0078125f;
+            const float un = kt_pow2(unit - KU_T - 7);
+            if (c > 0) wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u);
+            fence_after_sync();
+            const uint32_t to_o = tmem + lane_base + KU_TO + q * HD;
+            auto put = [&](int b, const float (&o)[32], float inv) {  // 32 columns from 32 b on
+                const long long at_o = (long long)(sr.first + ri) * a.o_row + (long long)hq * a.o_head + 32 * b;
+#pragma unroll
+                for (int y = 0; y < 32; y += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        v[x] = L != 0.f ? o[y + 2 * x] * inv : 0.f, v[x + 4] = L != 0.f ? o[y + 2 * x + 1] * inv : 0.f;
+                    }
+                    if (dtype == DT_F16)
+                        store8<DT_F16>(reinterpret_cast<__half *>(a.out) + at_o + y, wide_o, v);
+                    else
+                        store8<DT_BF16>(reinterpret_cast<__nv_bfloat16 *>(a.out) + at_o + y, wide_o, v);
+                }
+            };
+            auto put_lse = [&]() {
+                if (a.lse) a.lse[(size_t)(sr.first + ri) * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M) + log2f(L)) * 0.69314718055994530942f;
+            };
+            const int2 who = Cut::sharers(pl, pl.pos - pl.skip, sp.steps);
+            float *po = part + 2 * (size_t)2 * gridDim.x * KU_R;
+            const int prow = q * BQ + row;
+            const size_t mine = Cut::slot(blockIdx.x, pl.skip == 0) * KU_R + prow;
+            const float inv = L != 0.f ? un / L : 0.f;  // L is 0 when no key is seen, NaN when a score is
+#pragma unroll 1
+            for (int b = 0; b < HD / 32; b++) {
+                float o[32];
+                tmem_ld32(to_o + 32 * b, o);
+                tmem_wait_ld();
+                if (nans >> (32 * b / G) & 1) {
+#pragma unroll
+                    for (int k = 0; k < 32; k++) o[k] = NAN;
+                }
+                if (whole) {
+                    if (write) put(b, o, inv);
+                } else if (write) {
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4)
+                        __stcg(reinterpret_cast<float4 *>(po + mine * HD + 32 * b + k), make_float4(o[k] * un, o[k + 1] * un, o[k + 2] * un, o[k + 3] * un));
+                }
+            }
+            fence_before_sync();
+            if (whole) {
+                if (write) put_lse();
+            } else {
+                if (write) __stcg(reinterpret_cast<float2 *>(part) + mine, make_float2(M, L));
+                __threadfence();
+                kt_bar(3 + q, 128);
+                if (row == 0) {
+                    // (a counter for each tile: the second tile's behind the first's)
+                    int *count = arrived + q * (KA_BLOCKS / 2) + who.x;
+                    s_last[q] = atomicAdd(count, 1) == who.y - 1;
+                    if (s_last[q]) *count = 0;  // ready for the next call
+                }
+                kt_bar(3 + q, 128);
+                write = write && s_last[q];
+                kt_bar(3 + q, 128);  // (read before a next piece writes it)
+                if (write) {
+                    __threadfence();
+                    M = -INFINITY, L = 0.f;
+                    for (int p = 0; p < who.y; p++)
+                        M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(part) + Cut::slot(who.x + p, p == 0) * KU_R + prow).x);
+                    auto weight = [&](float2 x) { return x.x == -INFINITY ? (x.y != 0.f ? x.y : 0.f) : kt_ex2(x.x - M); };  // (a NaN sum stays one)
+                    for (int p = 0; p < who.y; p++) {
+                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(part) + Cut::slot(who.x + p, p == 0) * KU_R + prow);
+                        L = fmaf(x.y, weight(x), L);
+                    }
+                    const float w = L != 0.f ? 1.f / L : 0.f;
+#pragma unroll 1
+                    for (int b = 0; b < HD / 32; b++) {
+                        float o[32];
+#pragma unroll
+                        for (int k = 0; k < 32; k++) o[k] = 0.f;
+                        for (int p = 0; p < who.y; p++) {
+                            const size_t src = Cut::slot(who.x + p, p == 0) * KU_R + prow;
+                            const float f = weight(__ldcg(reinterpret_cast<const float2 *>(part) + src));
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4) {
+                                const float4 y = __ldcg(reinterpret_cast<const float4 *>(po + src * HD + 32 * b + k));
+                                o[k] = fmaf(y.x, f, o[k]), o[k + 1] = fmaf(y.y, f, o[k + 1]);
+                                o[k + 2] = fmaf(y.z, f, o[k + 2]), o[k + 3] = fmaf(y.w, f, o[k + 3]);
+                            }
+                        }
+                        put(b, o, w);
+                    }
+                    put_lse();
+                }
+            }
+            at += n, at1 += q ? n : 0;
+            Cut::next(pl, a, each, sr.n, n);
+        }
+    }
+    if (abort_flag && tid == 0) *reinterpret_cast<volatile int *>(a.err_wait) = 1;
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+size_t kv4_attend_tc16_workspace(const Kv4AttendArgs &a, int sms) {
+    return 4 * (KA_BLOCKS + (size_t)2 * std::min(KA_BLOCKS / 2, sms) * KU_R * (a.c.width + 2));
+}
+
+template <int HD, int G>
+static cudaError_t launch_tc16(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
+    const size_t smem = KuShape<HD, G>::SMEM;
+    cudaError_t e = allow_dynamic_smem((const void *)k_kv4_attend_tc16<HD, G>, smem);
+    if (e != cudaSuccess) return e;
+    k_kv4_attend_tc16<HD, G><<<std::min(sms, KA_BLOCKS / 2), KU_THREADS, smem, s>>>(a, dtype, reinterpret_cast<float *>(work) + KA_BLOCKS,
+                                                                                   reinterpret_cast<int *>(work));
+    return cudaGetLastError();
+}
+
+cudaError_t launch_kv4_attend_tc16(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
+    const int g = a.c.group;
+    if (a.c.width == 32) return launch_tc16<32, 32>(dtype, a, sms, work, s);
+    if (a.c.width == 64) return g == 32 ? launch_tc16<64, 32>(dtype, a, sms, work, s) : launch_tc16<64, 64>(dtype, a, sms, work, s);
+    if (a.c.width == 128)
+        return g == 32   ? launch_tc16<128, 32>(dtype, a, sms, work, s)
+               : g == 64 ? launch_tc16<128, 64>(dtype, a, sms, work, s)
+                         : launch_tc16<128, 128>(dtype, a, sms, work, s);
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace tcu

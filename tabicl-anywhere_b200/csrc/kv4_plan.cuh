@@ -98,7 +98,7 @@ struct KaCut {
         __syncthreads();
         Place p;
         p.total = 0;
-#pragma unroll
+#pragma unroll 1
         for (int w = 0; w < THREADS / 32; w++) {
             if (w == warp) before += p.total;
             p.total += sums[w];

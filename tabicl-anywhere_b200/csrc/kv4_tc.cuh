@@ -1,0 +1,59 @@
+// What the two tensor-core kernels of the four-bit attention share: widening stored codes into operand blocks, waits.
+#pragma once
+#include "kv4_plan.cuh"
+#include "tc.cuh"
+
+namespace tcu {
+
+using namespace tc;
+
+constexpr long long KT_WAIT = 2000000000ll;  // about a second at boost clock
+
+__device__ __forceinline__ float kt_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| < 127
+__device__ __forceinline__ float kt_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void kt_bar(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ __half2 kt_h2(uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); }
+__device__ __forceinline__ uint32_t kt_u32(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
+
+// One group's scales for widening: value = code nibble as f16 * even (a byte's first nibble) or * odd (its second) + low.
+template <bool SPLIT>
+struct KtScale;
+template <>
+struct KtScale<false> {
+    __half2 even, odd, low;
+    __device__ __forceinline__ void set(float step, float l, float up) {
+        const float s = step * up * 16777216.f;
+        even = __float2half2_rn(s), odd = __float2half2_rn(s * 0.0625f), low = __float2half2_rn(l * up);
+    }
+};
+template <>
+struct KtScale<true> {
+    float even, odd, low;
+    __device__ __forceinline__ void set(float step, float l, float up) {
+        even = step * up * 16777216.f, odd = even * 0.0625f, low = l * up;
+    }
+};
+// A word's eight values as f16 (and what remains of them) into 16 bytes each.
+__device__ __forceinline__ void kt_widen(uint32_t w, const KtScale<false> &s, __half *hi, __half *) {
+    const uint32_t v = w >> 8;
+    *reinterpret_cast<uint4 *>(hi) = make_uint4(kt_u32(__hfma2(kt_h2(w & 0x000f000fu), s.even, s.low)), kt_u32(__hfma2(kt_h2(w & 0x00f000f0u), s.odd, s.low)),
+                                                kt_u32(__hfma2(kt_h2(v & 0x000f000fu), s.even, s.low)), kt_u32(__hfma2(kt_h2(v & 0x00f000f0u), s.odd, s.low)));
+}
+__device__ __forceinline__ void kt_widen(uint32_t w, const KtScale<true> &s, __half *hi, __half *lo) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t v = i & 2 ? w >> 8 : w;
+        const float2 c = __half22float2(kt_h2(i & 1 ? v & 0x00f000f0u : v & 0x000f000fu));
+        const float f = i & 1 ? s.odd : s.even;
+        split_pair(fmaf(c.x, f, s.low), fmaf(c.y, f, s.low), h[i], l[i]);
+    }
+    *reinterpret_cast<uint4 *>(hi) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4 *>(lo) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+}  // namespace tcu
