@@ -203,18 +203,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos);
                 kt_bar(1, 352);  // Q is in tensor memory
                 fence_after_sync();
-                if (lane == 0) {
+                {
                     for (int i = at; i < at + n; i++) {
                         const int sl = i % NS;
                         const uint32_t ph = (uint32_t)(i / NS) & 1u;
                         if (warp < 14) {
                             if ((i & 1) != warp - 12) continue;
                             // S(i) once P V(i - NS) has read its slot, from the keys of step i
-                            if (i >= NS && !wait(&mSlot[sl], ph ^ 1u)) break;
-                            if (!wait(&mK[sl], ph)) break;
+                            if (i >= NS) wait_warp(&mSlot[sl], ph ^ 1u);
+                            wait_warp(&mK[sl], ph);
                             fence_after_sync();
                             const uint32_t tS = tmem + KT_TS + BK * sl;
                             const uint64_t dh = dK0 + sl * slot_off, dl = dh + lo_off;
+                            if (elect_one()) {
                             if (SPLIT) {
 #pragma unroll
                                 for (int k = 0; k < HD / 16; k++) mma_f16_ta(tS, tmem + KT_TQ + 8 * k, dl + k * stK, idS, k > 0 ? 1u : 0u);
@@ -225,14 +226,17 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                             for (int k = 0; k < HD / 16; k++) mma_f16_ta(tS, tmem + KT_TQ + 8 * k, dh + k * stK, idS, SPLIT || k > 0 ? 1u : 0u);
                             mma_commit(&mS[sl]);
                             mma_commit(&mKfree[sl]);
+                            }
+                            __syncwarp();
                         } else {
                             // P V of step i: its weights and values there, the fold of step i - 1 done
-                            if (!wait(&mP[sl], ph)) break;
-                            if (!wait(&mV[sl], ph)) break;
-                            if (i >= 1 && !wait(&mOfree, (uint32_t)(i - 1) & 1u)) break;
+                            wait_warp(&mP[sl], ph);
+                            wait_warp(&mV[sl], ph);
+                            if (i >= 1) wait_warp(&mOfree, (uint32_t)(i - 1) & 1u);
                             fence_after_sync();
                             const uint32_t pA = tmem + KT_TS + BK * sl, tO = tmem + KT_TO;
                             const uint64_t dh = dV0 + sl * slot_off, dl = dh + lo_off;
+                            if (elect_one()) {
                             if (SPLIT) {
 #pragma unroll
                                 for (int k = 0; k < BK / 16; k++) mma_f16_ta(tO, pA + 8 * k, dl + k * stV, idO, k > 0 ? 1u : 0u);
@@ -244,6 +248,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                             mma_commit(&mPV);
                             mma_commit(&mVfree[sl]);
                             mma_commit(&mSlot[sl]);
+                            }
+                            __syncwarp();
                         }
                     }
                 }
@@ -251,7 +257,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 at += n;
                 Cut::next(pl, a, each, sr.n, n);
             }
-            if (lane == 0) {  // every product issued here completes before the block lets go of its memory
+            if (elect_one()) {  // every product issued here completes before the block lets go of its memory
                 mma_commit(&mDone[warp - 12]);
                 mbar_wait(&mDone[warp - 12], 0, KT_WAIT);
             }

@@ -135,11 +135,11 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
             }
             // what was asked for lands before the block lets go of shared memory
             for (int i = max(0, at - NR); i < at; i++) mbar_wait(&mRaw[i % NR], (uint32_t)(i / NR) & 1u, KT_WAIT);
-        } else if (warp < 18 && lane == 0) {
+        } else if (warp < 18) {
             // ---- the products ----
             const uint32_t idS = idesc_f16(BQ, BK, 0, 0), idO = idesc_f16(BQ, HD, 0, 1);
             const uint64_t dQ0 = kstep_desc(Qs, BQ, 0), dK0 = kstep_desc(Kring, BK, 0), dV0 = kstep_desc(Vring, HD, 0);
-            const uint64_t stQ = (2 * (BQ / 8) * 128) >> 4, stK = (2 * (BK / 8) * 128) >> 4, stV = (2 * (HD / 8) * 128) >> 4;
+            constexpr uint64_t stQ = (2 * (BQ / 8) * 128) >> 4, stK = (2 * (BK / 8) * 128) >> 4, stV = (2 * (HD / 8) * 128) >> 4;
             constexpr uint64_t q_off = (BQ * HD * 2) >> 4, slot_off = (BLOCK * 2) >> 4;
             int units[2] = {0, 0};  // pieces of each tile so far
             while (pl.pos < pl.end) {
@@ -151,36 +151,44 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     const uint32_t ph = (uint32_t)((at + i) / NS) & 1u;
                     if (warp == 16) {
                         // S(i) of both tiles from the keys of step i, once P V(i - 2) has read the slot
-                        if (!wait(&mK[sl], ph)) break;
-                        bool ok = true;
-                        for (int q = 0; q < nq && ok; q++) {
-                            const int c = (q ? at1 : at) + i;
-                            if (i == 0 && !(ok = wait(&mQ[q], (uint32_t)units[q] & 1u))) break;
-                            if (c >= 2 && !(ok = wait(&mSlot[q][c & 1], (uint32_t)((c >> 1) - 1) & 1u))) break;
-                            fence_after_sync();
+                        wait_warp(&mK[sl], ph);
+                        const uint64_t dK = dK0 + sl * slot_off;
 #pragma unroll
-                            for (int k = 0; k < HD / 16; k++)
-                                mma_f16(tmem + KU_TS + (2 * q + (c & 1)) * BK, dQ0 + q * q_off + k * stQ, dK0 + sl * slot_off + k * stK, idS, k > 0 ? 1u : 0u);
-                            mma_commit(&mS[q][c & 1]);
+                        for (int q = 0; q < 2; q++) {
+                            if (q >= nq) break;
+                            const int c = (q ? at1 : at) + i;
+                            if (i == 0) wait_warp(&mQ[q], (uint32_t)units[q] & 1u);
+                            if (c >= 2) wait_warp(&mSlot[q][c & 1], (uint32_t)((c >> 1) - 1) & 1u);
+                            fence_after_sync();
+                            const uint32_t tS = tmem + KU_TS + (2 * q + (c & 1)) * BK;
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = 0; k < HD / 16; k++) mma_f16(tS, dQ0 + q * q_off + k * stQ, dK + k * stK, idS, k > 0 ? 1u : 0u);
+                                mma_commit(&mS[q][c & 1]);
+                                if (q == nq - 1) mma_commit(&mKfree[sl]);
+                            }
+                            __syncwarp();
                         }
-                        if (!ok) break;
-                        mma_commit(&mKfree[sl]);
                     } else {
                         // P V(i) of both tiles, from the values of step i
-                        if (!wait(&mV[sl], ph)) break;
-                        bool ok = true;
-                        for (int q = 0; q < nq && ok; q++) {
-                            const int c = (q ? at1 : at) + i;
-                            if (!(ok = wait(&mP[q][c & 1], (uint32_t)(c >> 1) & 1u))) break;
-                            fence_after_sync();
+                        wait_warp(&mV[sl], ph);
+                        const uint64_t dV = dV0 + sl * slot_off;
 #pragma unroll
-                            for (int k = 0; k < BK / 16; k++)
-                                mma_f16_ta(tmem + KU_TO + q * HD, tmem + KU_TS + (2 * q + (c & 1)) * BK + 8 * k, dV0 + sl * slot_off + k * stV, idO,
-                                           i > 0 || k > 0 ? 1u : 0u);
-                            mma_commit(&mSlot[q][c & 1]);
+                        for (int q = 0; q < 2; q++) {
+                            if (q >= nq) break;
+                            const int c = (q ? at1 : at) + i;
+                            wait_warp(&mP[q][c & 1], (uint32_t)(c >> 1) & 1u);
+                            fence_after_sync();
+                            const uint32_t tP = tmem + KU_TS + (2 * q + (c & 1)) * BK;
+                            if (elect_one()) {
+#pragma unroll
+                                for (int k = 0; k < BK / 16; k++)
+                                    mma_f16_ta(tmem + KU_TO + q * HD, tP + 8 * k, dV + k * stV, idO, i > 0 || k > 0 ? 1u : 0u);
+                                mma_commit(&mSlot[q][c & 1]);
+                                if (q == nq - 1) mma_commit(&mVfree[sl]);
+                            }
+                            __syncwarp();
                         }
-                        if (!ok) break;
-                        mma_commit(&mVfree[sl]);
                     }
                 }
                 units[0]++, units[1] += nq == 2;
@@ -188,8 +196,11 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 Cut::next(pl, a, each, sr.n, n);
             }
             // every product issued here completes before the block lets go of its memory
-            mma_commit(&mDone[warp - 16]);
-            mbar_wait(&mDone[warp - 16], 0, KT_WAIT);
+            if (elect_one()) {
+                mma_commit(&mDone[warp - 16]);
+                mbar_wait(&mDone[warp - 16], 0, KT_WAIT);
+            }
+            __syncwarp();
         }
     } else if (wg >= 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -315,48 +326,59 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
             const int hi_min = ka_hi(a, sr, r0 / each), lo_max = ka_lo(a, sr, (r0 + rows - 1) / each);
             int c = q ? at1 : at;  // this tile's steps so far
 
-            // ---- Q: a thread a row, scaled by a power of two of the row's to at most 2^14 ----
-            float rowfac;
+            // ---- Q: a warp its 32 rows, 8 rows x 4 chunks of 8 coordinates at a time; a row scaled by a power of two of its own
+            // to at most 2^14 ----
+            float rowfac = 0.f;
             {
-                uint32_t w[HD / 2];
-                const long long from = (long long)(sr.first + ri) * a.q_row + (long long)hq * a.q_head;
-                const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + from;
-                if (wide_q) {
-#pragma unroll
-                    for (int b = 0; b < HD / 8; b++) {
-                        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src) + b);
-                        w[4 * b] = v.x, w[4 * b + 1] = v.y, w[4 * b + 2] = v.z, w[4 * b + 3] = v.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int b = 0; b < HD / 2; b++) w[b] = (uint32_t)src[2 * b] | (uint32_t)src[2 * b + 1] << 16;
-                }
+                constexpr int NC = HD / 32;  // chunks of a row a lane reads
                 auto get = [&](uint32_t x) {
                     return dtype == DT_BF16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : __half22float2(kt_h2(x));
                 };
-                float mx = 0.f;
 #pragma unroll
-                for (int b = 0; b < HD / 2; b++) {
-                    const float2 v = get(w[b]);
-                    mx = fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y)));
-                }
-                const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
-                const float up = a.scale < 0.f ? -kt_pow2(e) : kt_pow2(e);
-                // a score in units of log2: the product with the widened keys times this and the step's power of two (a scale of
-                // 0 as 2^-100, so that the factor is positive)
-                rowfac = fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * kt_pow2(-e);
+                for (int x = 0; x < 4; x++) {
+                    const int qrow = (warp & 3) * 32 + x * 8 + (lane & 7), qr = r0 + min(qrow, rows - 1);
+                    const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + (long long)(sr.first + qr / each) * a.q_row +
+                                          (long long)(pl.head * each + qr % each) * a.q_head + (lane >> 3) * 8;
+                    uint32_t w[NC][4];
+                    float mx = 0.f;
 #pragma unroll
-                for (int b = 0; b < HD / 8; b++) {
-                    float v[8];
+                    for (int y = 0; y < NC; y++) {
+                        if (wide_q) {
+                            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src + 32 * y));
+                            w[y][0] = v.x, w[y][1] = v.y, w[y][2] = v.z, w[y][3] = v.w;
+                        } else {
 #pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        const float2 f = get(w[4 * b + x]);
-                        v[2 * x] = f.x * up, v[2 * x + 1] = f.y * up;
+                            for (int z = 0; z < 4; z++) w[y][z] = (uint32_t)src[32 * y + 2 * z] | (uint32_t)src[32 * y + 2 * z + 1] << 16;
+                        }
                     }
-                    uint32_t h[4];
 #pragma unroll
-                    for (int x = 0; x < 4; x++) h[x] = kt_u32(__floats2half2_rn(v[x], v[x + 4]));
-                    *reinterpret_cast<uint4 *>(Qs + q * BQ * HD + kmajor_off(row, 8 * b, BQ)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    for (int y = 0; y < NC; y++)
+#pragma unroll
+                        for (int z = 0; z < 4; z++) {
+                            const float2 v = get(w[y][z]);
+                            mx = fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y)));
+                        }
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
+                    const float up = a.scale < 0.f ? -kt_pow2(e) : kt_pow2(e);
+                    // a score in units of log2: the product with the widened keys times this and the step's power of two (a scale
+                    // of 0 as 2^-100, so that the factor is positive)
+                    const float fac = __shfl_sync(0xffffffffu, fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * kt_pow2(-e), lane & 7);
+                    if (lane >> 3 == x) rowfac = fac;
+#pragma unroll
+                    for (int y = 0; y < NC; y++) {
+                        float v[8];
+#pragma unroll
+                        for (int z = 0; z < 4; z++) {
+                            const float2 f = get(w[y][z]);
+                            v[2 * z] = f.x * up, v[2 * z + 1] = f.y * up;
+                        }
+                        uint32_t h[4];
+#pragma unroll
+                        for (int z = 0; z < 4; z++) h[z] = kt_u32(__floats2half2_rn(v[z], v[z + 4]));
+                        *reinterpret_cast<uint4 *>(Qs + q * BQ * HD + kmajor_off(qrow, 32 * y + (lane >> 3) * 8, BQ)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    }
                 }
                 fence_async_smem();
                 mbar_arrive(&mQ[q]);
@@ -442,8 +464,8 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
             if (c > 0) wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u);
             fence_after_sync();
             const uint32_t to_o = tmem + lane_base + KU_TO + q * HD;
-            auto put = [&](int b, const float (&o)[32], float inv) {  // 32 columns from 32 b on
-                const long long at_o = (long long)(sr.first + ri) * a.o_row + (long long)hq * a.o_head + 32 * b;
+            // 32 columns from 32 b on into the row's place in Q's memory (its products are done), 16 bytes of 8 coordinates each
+            auto put = [&](int b, const float (&o)[32], float inv) {
 #pragma unroll
                 for (int y = 0; y < 32; y += 8) {
                     float v[8];
@@ -451,11 +473,35 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     for (int x = 0; x < 4; x++) {
                         v[x] = L != 0.f ? o[y + 2 * x] * inv : 0.f, v[x + 4] = L != 0.f ? o[y + 2 * x + 1] * inv : 0.f;
                     }
+                    uint16_t *to = reinterpret_cast<uint16_t *>(Qs) + q * BQ * HD + kmajor_off(row, 32 * b + y, BQ);
                     if (dtype == DT_F16)
-                        store8<DT_F16>(reinterpret_cast<__half *>(a.out) + at_o + y, wide_o, v);
+                        store8<DT_F16>(reinterpret_cast<__half *>(to), true, v);
                     else
-                        store8<DT_BF16>(reinterpret_cast<__nv_bfloat16 *>(a.out) + at_o + y, wide_o, v);
+                        store8<DT_BF16>(reinterpret_cast<__nv_bfloat16 *>(to), true, v);
                 }
+            };
+            // the warp's rows from there to memory, 8 rows x 4 chunks at a time
+            auto flush = [&]() {
+                __syncwarp();
+#pragma unroll 1
+                for (int x = 0; x < 4; x++) {
+                    const int orow = (warp & 3) * 32 + x * 8 + (lane & 7), orr = r0 + orow;
+                    uint16_t *dst = reinterpret_cast<uint16_t *>(a.out) + (long long)(sr.first + orr / each) * a.o_row +
+                                    (long long)(pl.head * each + orr % each) * a.o_head + (lane >> 3) * 8;
+#pragma unroll
+                    for (int y = 0; y < HD / 32; y++) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(Qs + q * BQ * HD + kmajor_off(orow, 32 * y + (lane >> 3) * 8, BQ));
+                        if (orow >= rows) continue;
+                        if (wide_o) {
+                            *reinterpret_cast<uint4 *>(dst + 32 * y) = v;
+                        } else {
+                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int z = 0; z < 4; z++) dst[32 * y + 2 * z] = (uint16_t)w[z], dst[32 * y + 2 * z + 1] = (uint16_t)(w[z] >> 16);
+                        }
+                    }
+                }
+                __syncwarp();
             };
             auto put_lse = [&]() {
                 if (a.lse) a.lse[(size_t)(sr.first + ri) * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M) + log2f(L)) * 0.69314718055994530942f;
@@ -475,7 +521,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     for (int k = 0; k < 32; k++) o[k] = NAN;
                 }
                 if (whole) {
-                    if (write) put(b, o, inv);
+                    put(b, o, inv);
                 } else if (write) {
 #pragma unroll
                     for (int k = 0; k < 32; k += 4)
@@ -484,6 +530,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
             }
             fence_before_sync();
             if (whole) {
+                flush();
                 if (write) put_lse();
             } else {
                 if (write) __stcg(reinterpret_cast<float2 *>(part) + mine, make_float2(M, L));
@@ -496,7 +543,8 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     if (s_last[q]) *count = 0;  // ready for the next call
                 }
                 kt_bar(3 + q, 128);
-                write = write && s_last[q];
+                const bool s_last_seen = s_last[q];
+                write = write && s_last_seen;
                 kt_bar(3 + q, 128);  // (read before a next piece writes it)
                 if (write) {
                     __threadfence();
@@ -528,6 +576,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     }
                     put_lse();
                 }
+                if (s_last_seen) flush();
             }
             at += n, at1 += q ? n : 0;
             Cut::next(pl, a, each, sr.n, n);

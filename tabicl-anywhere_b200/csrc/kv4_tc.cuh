@@ -9,6 +9,13 @@ using namespace tc;
 
 constexpr long long KT_WAIT = 2000000000ll;  // about a second at boost clock
 
+// One lane of a converged warp. The products are issued under it by a warp whose lanes all run the issuing loop: their
+// operands are then uniform, and an issue takes a few cycles (under `lane == 0` of a diverged warp about 130 were measured).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ float kt_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| < 127
 __device__ __forceinline__ float kt_ex2(float x) {
     float y;
