@@ -3389,7 +3389,7 @@ static W4Args w4_args(const tcu_w4 *w, int dtype, int rows) {
 size_t tcu_w4_linear_workspace(tcu_ctx *ctx, const tcu_w4 *w, int rows, int dtype) {
     size_t need = 0;
     const int r = guarded(ctx, [&]() -> int {
-        w4_args(w, dtype, rows);
+        need = w4_linear_workspace(dtype, w4_args(w, dtype, rows), ctx->sms);
         return TCU_OK;
     });
     return r == TCU_OK ? need : (size_t)-1;
@@ -3408,7 +3408,10 @@ int tcu_w4_linear_device(tcu_ctx *ctx, const tcu_w4 *w, int dtype, int rows, con
         check_aligned("w4_linear", "bias", bias, elem_size(dtype)), check_aligned("w4_linear", "residual", residual, elem_size(dtype));
         a.x = x, a.ldx = ldx, a.y = y, a.ldy = ldy, a.bias = bias, a.act = act, a.residual = residual, a.ldr = ldr;
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
-        Launch{ctx, s}(launch_w4_linear(dtype, a, ctx->sms, s, &ctx->launches), "w4_linear");
+        const size_t need = w4_linear_workspace(dtype, a, ctx->sms);
+        if (need && (!work || work_bytes < need)) fail(TCU_ERR_ARG, "w4_linear: needs " + std::to_string(need) + " bytes of working memory");
+        check_aligned("w4_linear", "working memory", work, 16);
+        Launch{ctx, s}(launch_w4_linear(dtype, a, ctx->sms, work, work_bytes, s, &ctx->launches), "w4_linear");
         return TCU_OK;
     });
 }

@@ -106,7 +106,9 @@ cudaError_t launch_kv4_attend_tc16(int dtype, const Kv4AttendArgs &a, int sms, v
 // A weight matrix w [n][k] (row stride ldw) to codes and scales.
 cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k, int group, uint8_t *codes,
                            __half2 *scales, cudaStream_t s, uint64_t *launches);
-cudaError_t launch_w4_linear(int dtype, const W4Args &a, int sms, cudaStream_t s, uint64_t *launches);
+size_t w4_linear_workspace(int dtype, const W4Args &a, int sms);
+cudaError_t launch_w4_linear(int dtype, const W4Args &a, int sms, void *work, size_t work_bytes, cudaStream_t s,
+                             uint64_t *launches);
 cudaError_t launch_logprobs(int dtype, const LogprobArgs &a, int sms, cudaStream_t s, uint64_t *launches);
 
 #ifdef __CUDACC__

@@ -334,23 +334,28 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 auto get = [&](uint32_t x) {
                     return dtype == DT_BF16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)) : __half22float2(kt_h2(x));
                 };
+                uint32_t raw_q[4][NC][4];
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
-                    const int qrow = (warp & 3) * 32 + x * 8 + (lane & 7), qr = r0 + min(qrow, rows - 1);
+                    const int qr = r0 + min((warp & 3) * 32 + x * 8 + (lane & 7), rows - 1);
                     const uint16_t *src = reinterpret_cast<const uint16_t *>(a.q) + (long long)(sr.first + qr / each) * a.q_row +
                                           (long long)(pl.head * each + qr % each) * a.q_head + (lane >> 3) * 8;
-                    uint32_t w[NC][4];
-                    float mx = 0.f;
 #pragma unroll
                     for (int y = 0; y < NC; y++) {
                         if (wide_q) {
                             const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src + 32 * y));
-                            w[y][0] = v.x, w[y][1] = v.y, w[y][2] = v.z, w[y][3] = v.w;
+                            raw_q[x][y][0] = v.x, raw_q[x][y][1] = v.y, raw_q[x][y][2] = v.z, raw_q[x][y][3] = v.w;
                         } else {
 #pragma unroll
-                            for (int z = 0; z < 4; z++) w[y][z] = (uint32_t)src[32 * y + 2 * z] | (uint32_t)src[32 * y + 2 * z + 1] << 16;
+                            for (int z = 0; z < 4; z++) raw_q[x][y][z] = (uint32_t)src[32 * y + 2 * z] | (uint32_t)src[32 * y + 2 * z + 1] << 16;
                         }
                     }
+                }
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int qrow = (warp & 3) * 32 + x * 8 + (lane & 7);
+                    const uint32_t(&w)[NC][4] = raw_q[x];
+                    float mx = 0.f;
 #pragma unroll
                     for (int y = 0; y < NC; y++)
 #pragma unroll

@@ -49,6 +49,10 @@ __device__ __forceinline__ int ka_lo(const Kv4AttendArgs &a, const KaRows &s, in
     return a.window ? max(0, s.len - s.n + i + 1 - a.window) : 0;
 }
 
+__device__ __forceinline__ long long ka_div(long long a, long long b) {  // not negative; 64-bit division only where it is needed
+    return ((a | b) >> 32) ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+
 template <int R, int ALIGN, int STEP>
 struct KaCut {
     struct Span {
@@ -85,52 +89,92 @@ struct KaCut {
     static __device__ __forceinline__ Place place(const Kv4AttendArgs &a, int each, int min_steps, long long (&sums)[THREADS / 32],
                                                   int (&unit)[4]) {
         const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-        const int share = (a.seqs + THREADS - 1) / THREADS, seq_lo = min(a.seqs, tid * share), seq_hi = min(a.seqs, seq_lo + share);
-        long long own = 0;
-        for (int q = seq_lo; q < seq_hi; q++) own += seq_steps(a, q, each) * a.c.heads;
-        long long before = own;
+        // the threads' numbers before this one's, and all of them
+        auto scan = [&](long long own, long long &total) {
+            long long before = own;
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const long long x = __shfl_up_sync(0xffffffffu, before, d);
-            if (lane >= d) before += x;
-        }
-        if (lane == 31) sums[warp] = before;
-        __syncthreads();
-        Place p;
-        p.total = 0;
+            for (int d = 1; d < 32; d *= 2) {
+                const long long x = __shfl_up_sync(0xffffffffu, before, d);
+                if (lane >= d) before += x;
+            }
+            __syncthreads();
+            if (lane == 31) sums[warp] = before;
+            __syncthreads();
+            total = 0;
 #pragma unroll 1
-        for (int w = 0; w < THREADS / 32; w++) {
-            if (w == warp) before += p.total;
-            p.total += sums[w];
-        }
-        before -= own;
-        p.blocks = min((long long)gridDim.x, (p.total + min_steps - 1) / min_steps);
+            for (int w = 0; w < THREADS / 32; w++) {
+                if (w == warp) before += total;
+                total += sums[w];
+            }
+            return before - own;
+        };
+        Place p;
         p.pos = p.end = 0;
-        if (blockIdx.x < p.blocks) p.pos = p.total * blockIdx.x / p.blocks, p.end = p.total * (blockIdx.x + 1) / p.blocks;
-        if (p.end && own && p.pos >= before && p.pos < before + own) {  // the thread whose sequences hold the first step
-            long long at = before;
-            for (int q = seq_lo; q < seq_hi; q++) {
-                const long long n = seq_steps(a, q, each) * a.c.heads;
-                if (p.pos >= at + n) {
-                    at += n;
-                    continue;
+        if ((long long)a.max_rows * each > 8 * R && a.seqs <= 16) {
+            // few sequences of many row tiles: all threads share each sequence's tiles
+            long long total = 0;
+            for (int turn = 0; turn < 2; turn++) {  // the sum of all, then this block's place in it
+                long long at = 0;
+                for (int q = 0; q < a.seqs; q++) {
+                    const KaRows s = ka_rows(a, q);
+                    if (!s.ok && tid == 0) *reinterpret_cast<volatile int *>(a.err) = 1;
+                    const int tiles = s.ok ? (s.n * each + R - 1) / R : 0, share = (tiles + THREADS - 1) / THREADS;
+                    const int lo = min(tiles, tid * share), hi = min(tiles, lo + share);
+                    long long own = 0, all;
+                    for (int rt = lo; rt < hi; rt++) own += (long long)span(a, s, each, rt).steps * a.c.heads;
+                    const long long before = at + scan(own, all);
+                    if (turn && p.end && p.pos >= before && p.pos < before + own) {
+                        long long x = before;
+                        for (int rt = lo;; rt++) {
+                            const int steps = span(a, s, each, rt).steps;
+                            if (p.pos < x + (long long)steps * a.c.heads) {
+                                unit[0] = q, unit[1] = rt, unit[2] = (int)ka_div(p.pos - x, steps);
+                                unit[3] = (int)(p.pos - x - (long long)unit[2] * steps);
+                                break;
+                            }
+                            x += (long long)steps * a.c.heads;
+                        }
+                    }
+                    at += all;
                 }
-                const KaRows r = ka_rows(a, q);
-                for (int rt = 0;; rt++) {
-                    const int steps = span(a, r, each, rt).steps;
-                    if (p.pos >= at + (long long)steps * a.c.heads) {
-                        at += (long long)steps * a.c.heads;
+                if (!turn) total = at, cut(p, total, min_steps);
+            }
+        } else {
+            const int share = (a.seqs + THREADS - 1) / THREADS, seq_lo = min(a.seqs, tid * share), seq_hi = min(a.seqs, seq_lo + share);
+            long long own = 0, total;
+            for (int q = seq_lo; q < seq_hi; q++) own += seq_steps(a, q, each) * a.c.heads;
+            const long long before = scan(own, total);
+            cut(p, total, min_steps);
+            if (p.end && own && p.pos >= before && p.pos < before + own) {  // the thread whose sequences hold the first step
+                long long at = before;
+                for (int q = seq_lo; q < seq_hi; q++) {
+                    const long long n = seq_steps(a, q, each) * a.c.heads;
+                    if (p.pos >= at + n) {
+                        at += n;
                         continue;
                     }
-                    unit[0] = q, unit[1] = rt, unit[2] = (int)((p.pos - at) / steps), unit[3] = (int)((p.pos - at) % steps);
+                    const KaRows r = ka_rows(a, q);
+                    for (int rt = 0;; rt++) {
+                        const int steps = span(a, r, each, rt).steps;
+                        if (p.pos >= at + (long long)steps * a.c.heads) {
+                            at += (long long)steps * a.c.heads;
+                            continue;
+                        }
+                        unit[0] = q, unit[1] = rt, unit[2] = (int)ka_div(p.pos - at, steps);
+                        unit[3] = (int)(p.pos - at - (long long)unit[2] * steps);
+                        break;
+                    }
                     break;
                 }
-                break;
             }
         }
         __syncthreads();
         p.seq = unit[0], p.rt = unit[1], p.head = unit[2], p.skip = unit[3];
         return p;
+    }
+    static __device__ __forceinline__ void cut(Place &p, long long total, int min_steps) {
+        p.total = total, p.blocks = min((long long)gridDim.x, ka_div(total + min_steps - 1, min_steps));
+        if (blockIdx.x < p.blocks) p.pos = ka_div(total * blockIdx.x, p.blocks), p.end = ka_div(total * (blockIdx.x + 1), p.blocks);
     }
     // On to the next unit, `piece` steps on.
     static __device__ __forceinline__ void next(Place &p, const Kv4AttendArgs &a, int each, int n, int piece) {
@@ -146,7 +190,7 @@ struct KaCut {
     }
     // The blocks [first, first + count) that share the unit whose first step is u0.
     static __device__ __forceinline__ int2 sharers(const Place &p, long long u0, int steps) {
-        const int b0 = (int)(((u0 + 1) * p.blocks - 1) / p.total), b1 = (int)(((u0 + steps) * p.blocks - 1) / p.total);
+        const int b0 = (int)ka_div((u0 + 1) * p.blocks - 1, p.total), b1 = (int)ka_div((u0 + steps) * p.blocks - 1, p.total);
         return make_int2(b0, b1 - b0 + 1);
     }
     // Where block b's part of a unit lies: a part that begins the unit in its second slot, one that goes on in its first.

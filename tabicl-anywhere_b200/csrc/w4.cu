@@ -64,14 +64,17 @@ cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k
 // the sum of two for f32; the group scales act on the f32 result:
 //     sum over groups of  step * (x_g . codes)  +  low * (sum of x_g)
 //
-// A warp takes 16 outputs (the rows of the matrix fragments, read 16 bytes a thread straight from memory) over a part of
-// K; the rows of x are the 8 NT columns, laid out once a block as fragments in shared memory. K is cut over the blocks of
-// a cluster (each lays out its own slice of x only) and over `parts` of a block's warps; the partial outputs meet in
-// shared memory, in a fixed order.
-constexpr int W4_WARPS = 8, W4_X_BYTES = 65536, W4_Y_UNITS = 128;
+// A warp takes 16 outputs (the rows of the matrix fragments) over a part of K, its weights arriving in a ring of its own a
+// few blocks ahead; the rows of x are the 8 NT columns, as fragments in shared memory: up to 8 rows are laid out by every
+// block for itself, more by a kernel before. K is cut over the blocks of a cluster (each holds its own slice of x only)
+// and over `parts` of a block's warps; the partial outputs meet in shared memory, in a fixed order.
+constexpr int W4_WARPS = 8, W4_X_BYTES = 65536, W4_Y_UNITS = 64;
+constexpr int W4_DEPTH = 3;   // steps a warp's ring holds
+constexpr int W4_SLICE = 16;  // most blocks of columns of x that a block holds at once
 
 struct W4Plan {
-    int nt, cs, groups, tiles, parts, slice, pass, row_tiles;  // tiles: of 16 outputs, a block's at a time; slice, pass: blocks of 128 columns
+    // tiles: of 16 outputs, a block's at a time; parts: log2 of the parts of a pass; slice, pass: blocks of 128 columns
+    int nt, cs, groups, tiles, parts, slice, pass, row_tiles;
 };
 
 __device__ __forceinline__ uint32_t w4_half2(float a, float b) {
@@ -110,195 +113,279 @@ __device__ __forceinline__ float w4_get(int dtype, const void *p, long long i) {
     return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i]);
 }
 
-// One block of 128 columns of the two weight rows of a thread.
-template <int G>
-struct W4Block {
-    static constexpr int NG = 128 / G;
-    uint4 c[2];
-    uint32_t s[2][NG];
-};
-template <int G>
-__device__ __forceinline__ void w4_load(W4Block<G> &w, const uint8_t *const (&codes)[2], const uint32_t *const (&scales)[2], int b, int t) {
-    constexpr int NG = W4Block<G>::NG;
+// x as fragments: word k of a unit and lane (row m % 8, quarter q of the unit) holds columns k and k + 4 of 8, scaled by
+// `up`; a weight word's second nibbles come 16 times as large, so every other word is 1/16 of it. Returns the columns' sum.
+template <int QS>
+__device__ __forceinline__ float w4_fragment(const float (&v)[8], float up, uint4 (&h)[QS]) {
+    float s = 0.f;
+    uint32_t w[QS][4];
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-        w.c[r] = __ldcs(reinterpret_cast<const uint4 *>(codes[r] + (size_t)b * 64) + t);
-        const uint32_t *s = scales[r] + (size_t)b * NG;
-        if constexpr (NG == 4) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(s));
-            w.s[r][0] = v.x, w.s[r][1] = v.y, w.s[r][2] = v.z, w.s[r][3] = v.w;
-        } else if constexpr (NG == 2) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(s));
-            w.s[r][0] = v.x, w.s[r][1] = v.y;
-        } else {
-            w.s[r][0] = __ldg(s);
+    for (int k = 0; k < 4; k++) {
+        const float f = k & 1 ? 0.0625f : 1.f, x0 = v[k] * up, x1 = v[k + 4] * up;
+        w[0][k] = w4_half2(x0 * f, x1 * f);
+        if constexpr (QS == 2) {
+            const float2 o = w4_float2(w[0][k]);
+            w[1][k] = w4_half2(fmaf(x0, f, -o.x), fmaf(x1, f, -o.y));
         }
+        s += x0 + x1;
+    }
+#pragma unroll
+    for (int k = 0; k < QS; k++) h[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+    return s;
+}
+// The power of two that brings a row's largest magnitude into [2^13, 2^14), and what undoes it on the sums (with 2^24 for
+// the codes).
+__device__ __forceinline__ float w4_up(float mx, float &undo) {
+    const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
+    undo = __uint_as_float((uint32_t)(127 - e) << 23) * 16777216.f;
+    return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+// Words of fragments and floats of sums of one block of 128 columns of 8 NT rows.
+__host__ __device__ constexpr int w4_frag_words(int nt, int qs) { return nt * qs * 512; }
+
+// Fragments of more than 8 rows, laid out once for all blocks of the product: one block a row.
+template <int G, int NT, int QS>
+__global__ void __launch_bounds__(256) k_w4_x(W4Args a, int dtype, uint32_t *xf, float *xs, float *fx) {
+    constexpr int NG = 128 / G, R = 8 * NT;
+    __shared__ float red[8];
+    const int blocks = (a.k + 127) / 128, m = blockIdx.x % R, rt = blockIdx.x / R, lane = threadIdx.x & 31;
+    const bool there = (int)blockIdx.x < a.rows;
+    const int es = dtype == DT_F32 ? 4 : 2;
+    const bool wide = !(((uintptr_t)a.x & 15) || (a.ldx * es) % 16);
+    const void *row = reinterpret_cast<const uint8_t *>(a.x) + (long long)(there ? blockIdx.x : 0) * a.ldx * es;
+    float mx = 0.f, v[8];
+    if (there)
+        for (int c = threadIdx.x * 8; c < a.k; c += 2048) {
+            w4_x8(dtype, row, c, a.k, wide, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[j]));
+        }
+    mx = warp_max(mx);
+    if (lane == 0) red[threadIdx.x >> 5] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; w++) mx = fmaxf(mx, red[w]);
+    float undo;
+    const float up = w4_up(mx, undo);
+    if (threadIdx.x == 0) fx[rt * R + m] = undo;
+    for (int i0 = 0; i0 < blocks * 16; i0 += 256) {
+        const int i = i0 + threadIdx.x, b = i / 16, u = i % 16 / 4, q = i % 4;
+        const bool on = i < blocks * 16;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = 0.f;
+        if (on && there) w4_x8(dtype, row, i * 8, a.k, wide, v);
+        uint4 h[QS];
+        float s = w4_fragment<QS>(v, up, h);
+#pragma unroll
+        for (int k = 0; k < QS; k++)
+            if (on)
+                *reinterpret_cast<uint4 *>(xf + ((size_t)(rt * blocks + b) * NT * QS + (m / 8) * QS + k) * 512 + u * 128 + (m % 8 * 4 + q) * 4) = h[k];
+#pragma unroll
+        for (int d = 1; d < G / 8; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if (on && i % (G / 8) == 0) xs[((size_t)(rt * blocks + b) * NG + i % 16 / (G / 8)) * R + m] = s * 5.9604644775390625e-8f;  // 2^-24
     }
 }
 
+__device__ __forceinline__ uint32_t w4_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int N>
+__device__ __forceinline__ void w4_cp(void *dst, const void *src) {
+    if constexpr (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(w4_smem(dst)), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(w4_smem(dst)), "l"(src), "n"(N) : "memory");
+}
+
+// One slot of a warp's ring: two blocks of 128 columns of 16 rows, 128 bytes of codes a row (of odd rows the two halves
+// changed places, so that eight lanes' 16 bytes of two rows fall on different banks), then the rows' scales.
+template <int G>
+struct W4Ring {
+    static constexpr int NG = 128 / G, BYTES = 2048 + 32 * NG * 4;
+};
+
 template <int G, int NT, int QS>
-__global__ void __launch_bounds__(W4_WARPS * 32) k_w4_linear(W4Args a, int dtype, W4Plan p) {
-    constexpr int NG = 128 / G, R = 8 * NT;
+__global__ void __launch_bounds__(W4_WARPS * 32, NT < 8 ? 2 : 1) k_w4_linear(W4Args a, int dtype, W4Plan p, const uint32_t *gxf, const float *gxs,
+                                                             const float *gfx) {
+    constexpr int NG = 128 / G, R = 8 * NT, D = W4_DEPTH;
+    using Ring = W4Ring<G>;
     extern __shared__ __align__(16) uint8_t sm[];
-    uint32_t *xf = reinterpret_cast<uint32_t *>(sm);                             // [pass][NT][QS][4 units][32 lanes][4]
-    float *xs = reinterpret_cast<float *>(xf + (size_t)p.pass * NT * QS * 512);  // [pass][NG][R] sums of a group's x
-    float *fx = xs + p.pass * NG * R;                                            // [R] undoes x's scaling
-    float *ybuf = fx + R;                                                        // [parts][tiles][R][16]
+    uint8_t *rings = sm;                                                               // [warps][D][Ring::BYTES]
+    uint32_t *xf = reinterpret_cast<uint32_t *>(sm + W4_WARPS * D * Ring::BYTES);      // [pass][NT][QS][4 units][32 lanes][4]
+    float *xs = reinterpret_cast<float *>(xf + (size_t)p.pass * w4_frag_words(NT, QS));  // [pass][NG][R] sums of a group's x
+    float *fx = xs + p.pass * NG * R;                                                  // [R] undoes x's scaling
+    float *ybuf = fx + R;                                                              // [parts][tiles][R][16]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int slice = blockIdx.x % p.cs, group = blockIdx.x / p.cs, r0 = blockIdx.y * R, rows = min(R, a.rows - r0);
+    const int slice = blockIdx.x % p.cs, group = blockIdx.x / p.cs, rt = blockIdx.y, r0 = rt * R, rows = min(R, a.rows - r0);
     const int blocks = (a.k + 127) / 128, b_lo = min(blocks, slice * p.slice), b_hi = min(blocks, b_lo + p.slice);
     const int all = (a.n + 15) / 16;
-    const int es = dtype == DT_F32 ? 4 : 2;
-    const bool wide = !(((uintptr_t)a.x & 15) || (a.ldx * es) % 16);
+    uint8_t *ring = rings + warp * D * Ring::BYTES;
 
     for (int tile0 = group * p.tiles; tile0 < all; tile0 += p.groups * p.tiles) {
-        const int tiles = min(p.tiles, all - tile0), units = tiles * p.parts;
+        const int tiles = min(p.tiles, all - tile0), units = tiles << p.parts;
         for (int b0 = b_lo; b0 == b_lo || b0 < b_hi; b0 += p.pass) {
-            const int nb = max(0, min(p.pass, b_hi - b0)), per = (nb + p.parts - 1) / p.parts;
-            // a warp's units (tile, part of the pass) run on without a break: the next two blocks are on their way while
-            // two are computed
-            const int steps = (per + 1) / 2, mine = warp < units ? (units - warp + W4_WARPS - 1) / W4_WARPS : 0;
-            W4Block<G> w[2][2];
-            auto fetch = [&](int step, W4Block<G>(&to)[2]) {
-                const int unit = warp + step / steps * W4_WARPS, tile = tile0 + unit / p.parts;
-                const int b = b0 + unit % p.parts * per + step % steps * 2;
-                const uint8_t *codes[2];
-                const uint32_t *scales[2];
+            const int nb = max(0, min(p.pass, b_hi - b0)), parts = 1 << p.parts, per = ((nb + 1) / 2 + parts - 1) >> p.parts;
+            // A warp's units (tile, part of the pass) run on without a break, two blocks of columns a step: the next D - 1 steps
+            // are on their way while one is computed.
+            const int mine = warp < units ? (units - warp + W4_WARPS - 1) / W4_WARPS : 0, total = per * mine;
+            int fu = warp, fb = 0, fetched = 0, fslot = 0;
+            const uint8_t *src[4], *ssrc;  // this lane's rows of the unit fetched next, its 16 bytes and its scales of the first block
+            const int half = lane >> 4;
+            auto fetch = [&]() {
+                if (fetched < total) {
+                    const int b = b0 + ((fu & (parts - 1)) * per + fb) * 2;
+                    if (fb == 0) {
+                        const int tile = tile0 + (fu >> p.parts);
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const size_t n = min(tile * 16 + r * 8 + g, a.n - 1);  // rows past n are read as the last, and not used
-                    codes[r] = a.codes + n * blocks * 64;
-                    scales[r] = reinterpret_cast<const uint32_t *>(a.scales) + n * blocks * NG;
+                        for (int x = 0; x < 4; x++)  // rows past n are read as the last, and not used
+                            src[x] = a.codes + (size_t)min(tile * 16 + x * 4 + (lane >> 3), a.n - 1) * blocks * 64;
+                        ssrc = reinterpret_cast<const uint8_t *>(a.scales + (size_t)min(tile * 16 + (lane & 15), a.n - 1) * blocks * NG);
+                    }
+                    uint8_t *to = ring + fslot * Ring::BYTES;
+                    // (a last block without a second is read twice)
+                    const int c = lane & 7, at = min(b + (c >> 2), blocks - 1) * 64 + (c & 3) * 16;
+#pragma unroll
+                    for (int x = 0; x < 4; x++) w4_cp<16>(to + (x * 4 + (lane >> 3)) * 128 + (c ^ ((lane >> 3 & 1) << 2)) * 16, src[x] + at);
+                    w4_cp<NG * 4>(to + 2048 + ((lane & 15) * 2 + half) * NG * 4, ssrc + min(b + half, blocks - 1) * NG * 4);
+                    if (++fb == per) fb = 0, fu += W4_WARPS;
                 }
-                w4_load<G>(to[0], codes, scales, min(b, blocks - 1), t);
-                w4_load<G>(to[1], codes, scales, min(b + 1, blocks - 1), t);
+                fetched++, fslot = fslot + 1 == D ? 0 : fslot + 1;
+                asm volatile("cp.async.commit_group;" ::: "memory");
             };
-            const int total = steps * mine;
-            if (total) fetch(0, w[0]);
 
             // the pass's x as fragments, unless they are there from the tiles before
-            if (tile0 == group * p.tiles || b_hi - b_lo > p.pass) {
-                __syncthreads();
-                for (int m = warp; m < R; m += W4_WARPS) {
-                    const uint8_t *row = reinterpret_cast<const uint8_t *>(a.x) + (long long)(r0 + min(m, rows - 1)) * a.ldx * es;
-                    float mx = 0.f, v[8];
-                    if (m < rows)
-                        for (int c = b0 * 128 + lane * 8; c < min(a.k, (b0 + nb) * 128); c += 256) {
-                            w4_x8(dtype, row, c, a.k, wide, v);
+            const bool lay = tile0 == group * p.tiles || b_hi - b_lo > p.pass;
+            if (lay) __syncthreads();  // (the warps are done with those of the pass before)
+            if (lay && NT > 1) {
+                for (int i = tid; i < nb * w4_frag_words(NT, QS) / 4; i += W4_WARPS * 32)
+                    w4_cp<16>(xf + 4 * i, gxf + ((size_t)rt * blocks + b0) * w4_frag_words(NT, QS) + 4 * i);
+                for (int i = tid; i < nb * NG * R / 4; i += W4_WARPS * 32) w4_cp<16>(xs + 4 * i, gxs + ((size_t)rt * blocks + b0) * NG * R + 4 * i);
+                if (tid < R) fx[tid] = gfx[rt * R + tid];
+            }
 #pragma unroll
-                            for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[j]));
-                        }
-                    mx = warp_max(mx);
-                    // mx * 2^e in [2^13, 2^14)
-                    const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
-                    const float up = __uint_as_float((uint32_t)(e + 127) << 23);
-                    if (lane == 0) fx[m] = __uint_as_float((uint32_t)(127 - e) << 23) * 16777216.f;
-                    for (int i0 = 0; i0 < nb * 16; i0 += 32) {
-                        const int i = i0 + lane, b = i / 16, u = i % 16 / 4, q = i % 4;
-                        const bool on = i < nb * 16;
-                        float s = 0.f;
-                        if (on && m < rows)
-                            w4_x8(dtype, row, (b0 + b) * 128 + i % 16 * 8, a.k, wide, v);
-                        else
+            for (int i = 0; i < D - 1; i++) fetch();
+            if (lay && NT == 1) {
+                // a warp a row; its part is read once, into registers (up to 8 x 8 columns a lane)
+                const int es = dtype == DT_F32 ? 4 : 2;
+                const bool wide = !(((uintptr_t)a.x & 15) || (a.ldx * es) % 16);
+                const uint8_t *row = reinterpret_cast<const uint8_t *>(a.x) + (long long)(r0 + min(warp, rows - 1)) * a.ldx * es;
+                float v[W4_SLICE / 2][8], mx = 0.f;
 #pragma unroll
-                            for (int j = 0; j < 8; j++) v[j] = 0.f;
-                        uint32_t h[2][4];
+                for (int x = 0; x < W4_SLICE / 2; x++) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {  // word k: columns k and k + 4; a word's second nibbles are 16 times as large
-                            const float f = k & 1 ? 0.0625f : 1.f, x0 = v[k] * up, x1 = v[k + 4] * up;
-                            h[0][k] = w4_half2(x0 * f, x1 * f);
-                            const float2 o = w4_float2(h[0][k]);
-                            if (QS == 2) h[1][k] = w4_half2(fmaf(x0, f, -o.x), fmaf(x1, f, -o.y));
-                            s += x0 + x1;
-                        }
-#pragma unroll
-                        for (int k = 0; k < QS; k++)
-                            if (on) *reinterpret_cast<uint4 *>(xf + (((b * NT + m / 8) * QS + k) * 4 + u) * 128 + (m % 8 * 4 + q) * 4) =
-                                make_uint4(h[k][0], h[k][1], h[k][2], h[k][3]);
-#pragma unroll
-                        for (int d = 1; d < G / 8; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-                        if (on && i % (G / 8) == 0) xs[(b * NG + i % 16 / (G / 8)) * R + m] = s * 5.9604644775390625e-8f;  // 2^-24
-                    }
+                    for (int j = 0; j < 8; j++) v[x][j] = 0.f;
+                    if (warp < rows && x * 32 + lane < nb * 16) w4_x8(dtype, row, b0 * 128 + (x * 32 + lane) * 8, a.k, wide, v[x]);
                 }
+#pragma unroll
+                for (int x = 0; x < W4_SLICE / 2; x++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[x][j]));
+                float undo;
+                const float up = w4_up(warp_max(mx), undo);
+                if (lane == 0) fx[warp] = undo;
+#pragma unroll
+                for (int x = 0; x < W4_SLICE / 2; x++) {
+                    const int i = x * 32 + lane, b = i / 16, u = i % 16 / 4, q = i % 4;
+                    const bool on = i < nb * 16;
+                    uint4 h[QS];
+                    float s = w4_fragment<QS>(v[x], up, h);
+#pragma unroll
+                    for (int k = 0; k < QS; k++)
+                        if (on) *reinterpret_cast<uint4 *>(xf + (b * QS + k) * 512 + u * 128 + (warp * 4 + q) * 4) = h[k];
+#pragma unroll
+                    for (int d = 1; d < G / 8; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+                    if (on && i % (G / 8) == 0) xs[(b * NG + i % 16 / (G / 8)) * R + warp] = s * 5.9604644775390625e-8f;  // 2^-24
+                }
+            }
+            if (lay) {
+                // (x's copies are the oldest group of every thread)
+                if (NT > 1) asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
                 __syncthreads();
             }
 
             float y[NT][4];
-            for (int step = 0; step < total; step += 2) {
+            int unit = warp, in = 0, slot = 0;
+            for (int now = 0; now < total; now++) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(D - 2) : "memory");
+                __syncwarp();  // every lane's part has landed, and every lane is done with the slot that is filled next
+                fetch();
+                if (in == 0) {
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const int now = step + half;
-                    if (now >= total) break;
-                    if (now + 1 < total) fetch(now + 1, w[half ^ 1]);
-                    const int unit = warp + now / steps * W4_WARPS, in = now % steps;
-                    if (in == 0) {
+                    for (int nt = 0; nt < NT; nt++) y[nt][0] = y[nt][1] = y[nt][2] = y[nt][3] = 0.f;
+                }
+                const uint8_t *wb = ring + slot * Ring::BYTES;
+                slot = slot + 1 == D ? 0 : slot + 1;
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) y[nt][0] = y[nt][1] = y[nt][2] = y[nt][3] = 0.f;
-                    }
-                    const int lo = unit % p.parts * per, hi = min(nb, lo + per);
+                for (int k = 0; k < 2; k++) {
+                    const int b = ((unit & (parts - 1)) * per + in) * 2 + k;
+                    if (b >= nb) break;
+                    const int c = (k * 4 + t) ^ ((g & 1) << 2);
+                    const uint4 k0 = *reinterpret_cast<const uint4 *>(wb + g * 128 + c * 16), k1 = *reinterpret_cast<const uint4 *>(wb + (g + 8) * 128 + c * 16);
+                    const uint32_t c0[4] = {k0.x, k0.y, k0.z, k0.w}, c1[4] = {k1.x, k1.y, k1.z, k1.w};
+                    const uint32_t *sc = reinterpret_cast<const uint32_t *>(wb + 2048) + k * NG;
+                    const uint32_t *xb = xf + b * w4_frag_words(NT, QS) + lane * 4;
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int b = lo + in * 2 + k;
-                        if (b >= hi) break;
-                        const W4Block<G> &wb = w[half][k];
-                        const uint32_t c0[4] = {wb.c[0].x, wb.c[0].y, wb.c[0].z, wb.c[0].w};
-                        const uint32_t c1[4] = {wb.c[1].x, wb.c[1].y, wb.c[1].z, wb.c[1].w};
+                    for (int q = 0; q < NG; q++) {
+                        float acc[NT][4] = {};
 #pragma unroll
-                        for (int q = 0; q < NG; q++) {
-                            float acc[NT][4] = {};
+                        for (int u = q * (G / 32); u < (q + 1) * (G / 32); u++) {
+                            const uint32_t v0 = c0[u] >> 8, v1 = c1[u] >> 8;
 #pragma unroll
-                            for (int u = q * (G / 32); u < (q + 1) * (G / 32); u++) {
-                                const uint32_t v0 = c0[u] >> 8, v1 = c1[u] >> 8;
+                            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                                for (int nt = 0; nt < NT; nt++)
+                                for (int z = QS - 1; z >= 0; z--) {
+                                    const uint4 x = *reinterpret_cast<const uint4 *>(xb + ((nt * QS + z) * 4 + u) * 128);
+                                    w4_mma(acc[nt], c0[u] & 0x000f000fu, c1[u] & 0x000f000fu, c0[u] & 0x00f000f0u, c1[u] & 0x00f000f0u, x.x, x.y);
+                                    w4_mma(acc[nt], v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, x.z, x.w);
+                                }
+                        }
+                        const float2 s0 = w4_float2(sc[g * 2 * NG + q]), s1 = w4_float2(sc[(g + 8) * 2 * NG + q]);
 #pragma unroll
-                                    for (int z = QS - 1; z >= 0; z--) {
-                                        const uint4 x = *reinterpret_cast<const uint4 *>(xf + (((b * NT + nt) * QS + z) * 4 + u) * 128 + lane * 4);
-                                        w4_mma(acc[nt], c0[u] & 0x000f000fu, c1[u] & 0x000f000fu, c0[u] & 0x00f000f0u, c1[u] & 0x00f000f0u, x.x, x.y);
-                                        w4_mma(acc[nt], v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, x.z, x.w);
-                                    }
-                            }
-                            const float2 s0 = w4_float2(wb.s[0][q]), s1 = w4_float2(wb.s[1][q]);
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                const float2 sx = *reinterpret_cast<const float2 *>(xs + (b * NG + q) * R + nt * 8 + 2 * t);
-                                y[nt][0] = fmaf(s0.x, acc[nt][0], fmaf(s0.y, sx.x, y[nt][0]));
-                                y[nt][1] = fmaf(s0.x, acc[nt][1], fmaf(s0.y, sx.y, y[nt][1]));
-                                y[nt][2] = fmaf(s1.x, acc[nt][2], fmaf(s1.y, sx.x, y[nt][2]));
-                                y[nt][3] = fmaf(s1.x, acc[nt][3], fmaf(s1.y, sx.y, y[nt][3]));
-                            }
+                        for (int nt = 0; nt < NT; nt++) {
+                            const float2 sx = *reinterpret_cast<const float2 *>(xs + (b * NG + q) * R + nt * 8 + 2 * t);
+                            y[nt][0] = fmaf(s0.x, acc[nt][0], fmaf(s0.y, sx.x, y[nt][0]));
+                            y[nt][1] = fmaf(s0.x, acc[nt][1], fmaf(s0.y, sx.y, y[nt][1]));
+                            y[nt][2] = fmaf(s1.x, acc[nt][2], fmaf(s1.y, sx.x, y[nt][2]));
+                            y[nt][3] = fmaf(s1.x, acc[nt][3], fmaf(s1.y, sx.y, y[nt][3]));
                         }
                     }
-                    if (in == steps - 1) {  // the unit's partial outputs, added to those of the passes before (the same warp's)
-                        float *yb = ybuf + ((unit % p.parts) * p.tiles + unit / p.parts) * R * 16;
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int c = 0; c < 4; c++) {
-                                const int m = nt * 8 + 2 * t + (c & 1);
-                                float *at = yb + m * 16 + (c >> 1) * 8 + g;
-                                const float v = y[nt][c] * fx[m];
-                                *at = b0 == b_lo ? v : *at + v;
-                            }
-                    }
                 }
+                if (++in < per) continue;
+                // the unit's partial outputs, added to those of the passes before (the same warp's)
+                float *yb = ybuf + ((unit & (parts - 1)) * p.tiles + (unit >> p.parts)) * R * 16;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const int m = nt * 8 + 2 * t + (c & 1);
+                        float *at = yb + m * 16 + (c >> 1) * 8 + g;
+                        const float v = y[nt][c] * fx[m];
+                        *at = b0 == b_lo ? v : *at + v;
+                    }
+                in = 0, unit += W4_WARPS;
             }
         }
-        // ---- the partial outputs joined: each block of the cluster takes a share ----
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        // ---- the partial outputs joined: the parts' by the block, the slices' by the cluster, each block a share ----
+        __syncthreads();
+        const int wide_n = tiles * 16;
+        if (p.parts && b_lo < b_hi) {
+            for (int i = tid; i < wide_n * R; i += W4_WARPS * 32) {
+                float v = ybuf[i];
+                for (int q = 1; q < 1 << p.parts; q++) v += ybuf[q * p.tiles * R * 16 + i];
+                ybuf[i] = v;
+            }
+        }
         cg::cluster_group cl = cg::this_cluster();
         if (p.cs > 1)
             cl.sync();
         else
             __syncthreads();
-        const int wide_n = tiles * 16, count = wide_n * rows;
-        for (int i = slice * W4_WARPS * 32 + tid; i < count; i += p.cs * W4_WARPS * 32) {
+        for (int i = slice * W4_WARPS * 32 + tid; i < wide_n * rows; i += p.cs * W4_WARPS * 32) {
             const int m = i / wide_n, nn = i % wide_n, n = tile0 * 16 + nn;
             if (n >= a.n) continue;
             float v = 0.f;
-            for (int c = 0; c < p.cs; c++) {
-                if (c * p.slice >= blocks) break;  // no columns left for it
+            for (int c = 0; c < p.cs && c * p.slice < blocks; c++) {  // (blocks past the last column have nothing)
                 const float *from = p.cs > 1 ? cl.map_shared_rank(ybuf, c) : ybuf;
-                for (int q = 0; q < p.parts; q++) v += from[((q * p.tiles + nn / 16) * R + m) * 16 + nn % 16];
+                v += from[(nn / 16 * R + m) * 16 + nn % 16];
             }
             if (a.bias) v += w4_get(dtype, a.bias, n);
             if (a.act) v = gelu1(v);
@@ -323,52 +410,75 @@ static W4Plan w4_plan(int dtype, const W4Args &a, int sms) {
     const int qs = dtype == DT_F32 ? 2 : 1, blocks = (a.k + 127) / 128, tiles = (a.n + 15) / 16;
     p.nt = a.rows <= 8 ? 1 : a.rows <= 16 ? 2 : a.rows <= 32 || qs == 2 ? 4 : 8;
     p.row_tiles = (a.rows + 8 * p.nt - 1) / (8 * p.nt);
-    // a slice of at most 16 blocks of columns (its x takes a block longer to lay out than its weights to stream beyond
-    // that), up to 8 slices; more where there are too few outputs to fill the GPU
+    // a slice of at most 16 blocks of columns, up to 8 slices; more where there are too few outputs to fill the GPU
     p.cs = 1;
-    while (p.cs < 8 && (blocks > 16 * p.cs || (blocks >= 16 * p.cs && tiles * p.cs * 2 <= sms))) p.cs *= 2;
+    while (p.cs < 8 && (blocks > W4_SLICE * p.cs || (blocks >= 16 * p.cs && tiles * p.cs * 2 <= sms))) p.cs *= 2;
     p.slice = (blocks + p.cs - 1) / p.cs;
-    p.pass = std::min(p.slice, std::max(1, W4_X_BYTES / (2048 * p.nt * qs)));
+    p.pass = std::min({p.slice, W4_SLICE, std::max(1, W4_X_BYTES / (4 * w4_frag_words(p.nt, qs)))});
     p.groups = std::min(tiles, std::max(1, 2 * sms / (p.cs * p.row_tiles)));
     p.tiles = std::min((tiles + p.groups - 1) / p.groups, W4_Y_UNITS / p.nt);
     p.groups = std::min(p.groups, (tiles + p.tiles - 1) / p.tiles);
-    // parts of a slice so that the warps share the tiles evenly
-    p.parts = 1;
-    for (int h = 2; h <= 8 && h <= p.pass && p.tiles * h <= W4_Y_UNITS / p.nt; h *= 2) {
-        auto cost = [&](int x) { return (p.tiles * x + W4_WARPS - 1) / W4_WARPS * ((p.pass + x - 1) / x); };
+    // a power of two of parts of a slice, so that the warps share the tiles evenly
+    p.parts = 0;
+    for (int h = 1; h <= 3 && 2 << h <= p.pass + 1 && p.tiles << h <= W4_Y_UNITS / p.nt; h++) {
+        auto cost = [&](int x) { return (((p.tiles << x) + W4_WARPS - 1) / W4_WARPS) * (((p.pass + 1) / 2 + (1 << x) - 1) >> x); };
         if (cost(h) < cost(p.parts)) p.parts = h;
     }
     return p;
 }
 
+// More than 8 rows: the fragments, the groups' sums and the rows' factors, one after the other.
+static size_t w4_frag_bytes(const W4Args &a, const W4Plan &p, int qs) { return (size_t)p.row_tiles * ((a.k + 127) / 128) * w4_frag_words(p.nt, qs) * 4; }
+static size_t w4_sum_bytes(const W4Args &a, const W4Plan &p) { return (size_t)p.row_tiles * ((a.k + 127) / 128) * (128 / a.group) * 8 * p.nt * 4; }
+size_t w4_linear_workspace(int dtype, const W4Args &a, int sms) {
+    if (a.rows <= 8) return 0;
+    const W4Plan p = w4_plan(dtype, a, sms);
+    return w4_frag_bytes(a, p, dtype == DT_F32 ? 2 : 1) + w4_sum_bytes(a, p) + (size_t)p.row_tiles * 8 * p.nt * 4;
+}
+
 template <int G, int NT, int QS>
-static cudaError_t launch_w4(int dtype, const W4Args &a, const W4Plan &p, cudaStream_t s) {
-    const size_t smem = (size_t)p.pass * NT * QS * 2048 + sizeof(float) * (p.pass * (128 / G) * 8 * NT + 8 * NT + p.parts * p.tiles * 8 * NT * 16);
+static cudaError_t launch_w4(int dtype, const W4Args &a, const W4Plan &p, void *work, cudaStream_t s, uint64_t *launches) {
+    const size_t smem = (size_t)W4_WARPS * W4_DEPTH * W4Ring<G>::BYTES + (size_t)p.pass * w4_frag_words(NT, QS) * 4 +
+                        sizeof(float) * (p.pass * (128 / G) * 8 * NT + 8 * NT + ((p.tiles * 8 * NT * 16) << p.parts));
     cudaError_t e = allow_dynamic_smem((const void *)k_w4_linear<G, NT, QS>, smem);
     if (e != cudaSuccess) return e;
+    uint32_t *xf = reinterpret_cast<uint32_t *>(work);
+    float *xs = nullptr, *fx = nullptr;
+    if constexpr (NT > 1) {
+        xs = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(work) + w4_frag_bytes(a, p, QS));
+        fx = xs + w4_sum_bytes(a, p) / 4;
+        k_w4_x<G, NT, QS><<<p.row_tiles * 8 * NT, 256, 0, s>>>(a, dtype, xf, xs, fx);
+        if (launches) ++*launches;
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.groups * p.cs, p.row_tiles), cfg.blockDim = dim3(W4_WARPS * 32), cfg.dynamicSmemBytes = smem, cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = p.cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
     cfg.attrs = at, cfg.numAttrs = p.cs > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, k_w4_linear<G, NT, QS>, a, dtype, p);
+    if (launches) ++*launches;
+    return cudaLaunchKernelEx(&cfg, k_w4_linear<G, NT, QS>, a, dtype, p, (const uint32_t *)xf, (const float *)xs, (const float *)fx);
 }
 template <int G>
-static cudaError_t launch_w4(int dtype, const W4Args &a, const W4Plan &p, cudaStream_t s) {
+static cudaError_t launch_w4(int dtype, const W4Args &a, const W4Plan &p, void *work, cudaStream_t s, uint64_t *launches) {
     if (dtype == DT_F32)
-        return p.nt == 1 ? launch_w4<G, 1, 2>(dtype, a, p, s) : p.nt == 2 ? launch_w4<G, 2, 2>(dtype, a, p, s) : launch_w4<G, 4, 2>(dtype, a, p, s);
-    return p.nt == 1   ? launch_w4<G, 1, 1>(dtype, a, p, s)
-           : p.nt == 2 ? launch_w4<G, 2, 1>(dtype, a, p, s)
-           : p.nt == 4 ? launch_w4<G, 4, 1>(dtype, a, p, s)
-                       : launch_w4<G, 8, 1>(dtype, a, p, s);
+        return p.nt == 1   ? launch_w4<G, 1, 2>(dtype, a, p, work, s, launches)
+               : p.nt == 2 ? launch_w4<G, 2, 2>(dtype, a, p, work, s, launches)
+                           : launch_w4<G, 4, 2>(dtype, a, p, work, s, launches);
+    return p.nt == 1   ? launch_w4<G, 1, 1>(dtype, a, p, work, s, launches)
+           : p.nt == 2 ? launch_w4<G, 2, 1>(dtype, a, p, work, s, launches)
+           : p.nt == 4 ? launch_w4<G, 4, 1>(dtype, a, p, work, s, launches)
+                       : launch_w4<G, 8, 1>(dtype, a, p, work, s, launches);
 }
 
-cudaError_t launch_w4_linear(int dtype, const W4Args &a, int sms, cudaStream_t s, uint64_t *launches) {
+cudaError_t launch_w4_linear(int dtype, const W4Args &a, int sms, void *work, size_t work_bytes, cudaStream_t s, uint64_t *launches) {
     if (!a.rows) return cudaSuccess;
+    if (w4_linear_workspace(dtype, a, sms) > work_bytes) return cudaErrorInvalidValue;
     const W4Plan p = w4_plan(dtype, a, sms);
-    if (launches) ++*launches;
-    return a.group == 32 ? launch_w4<32>(dtype, a, p, s) : a.group == 64 ? launch_w4<64>(dtype, a, p, s) : launch_w4<128>(dtype, a, p, s);
+    return a.group == 32   ? launch_w4<32>(dtype, a, p, work, s, launches)
+           : a.group == 64 ? launch_w4<64>(dtype, a, p, work, s, launches)
+                           : launch_w4<128>(dtype, a, p, work, s, launches);
 }
 
 }  // namespace tcu
