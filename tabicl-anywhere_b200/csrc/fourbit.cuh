@@ -175,14 +175,20 @@ __device__ __forceinline__ void group_scale(float mn, float mx, bool bad, __half
 }
 // A value's code: its distance from low in steps, rounded to the nearest (ties to even), held to 0..15; 0 where the
 // step is 0. The quotient is the correctly rounded one, so equal inputs give equal codes everywhere.
-__device__ __forceinline__ uint32_t code_of(float x, float step, float low) {
-    if (!(step > 0.f)) return 0;
-    return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(x, low), step)), 0.f), 15.f);
+// It is found as a product with the step's reciprocal, which is within 2^-21 of it; only where that is near a tie is the
+// division itself taken (it costs as much as all the rest).
+__device__ __forceinline__ uint32_t code_of(float x, float step, float inverse, float low) {
+    const float d = __fsub_rn(x, low), t = d * inverse;
+    float c = rintf(t);
+    if (fabsf(fabsf(t - c) - 0.5f) < 1e-4f) c = rintf(__fdiv_rn(d, step));
+    return (uint32_t)(int)fminf(fmaxf(c, 0.f), 15.f);
 }
 __device__ __forceinline__ uint32_t pack8(const float (&x)[8], float step, float low) {
+    if (!(step > 0.f)) return 0;
+    const float inverse = __frcp_rn(step);
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) w |= code_of(x[j], step, low) << (4 * j);
+    for (int j = 0; j < 8; j++) w |= code_of(x[j], step, inverse, low) << (4 * j);
     return w;
 }
 // low + step * code, the product and the sum each rounded to f32 (step * code is exact: 11 + 4 bits).

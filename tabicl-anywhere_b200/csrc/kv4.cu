@@ -1,4 +1,6 @@
 // The four-bit paged cache: quantise keys and values into their slots, and read them back.
+#include <algorithm>
+
 #include "fourbit.cuh"
 
 namespace tcu {
@@ -6,26 +8,26 @@ namespace tcu {
 // A thread takes 8 neighbouring coordinates (one word of a key, two half-words of a value) of one head of one token, of
 // the keys and of the values; width / 8 neighbouring lanes hold a token's head, group / 8 of them a group.
 template <int DT, bool STORE>
-__global__ void __launch_bounds__(256) k_kv4_copy(Kv4CopyArgs a, long long items, bool wide) {
+__global__ void __launch_bounds__(256) k_kv4_copy(Kv4CopyArgs a, uint32_t items, int per_log2, int page_log2, int group_log2, bool wide) {
     using T = typename Elem<DT>::T;
-    const int W = a.c.width, NU = W / 32, per = W / 8, G8 = a.c.group / 8, NG = W / a.c.group, P = a.c.page;
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    const int W = a.c.width, NU = W / 32, G8 = a.c.group / 8, NG = W / a.c.group, P = a.c.page;
+    const uint32_t i = blockIdx.x * 256u + threadIdx.x;
     const bool on = i < items;
-    const long long row = on ? i / per : 0;
-    const int part = (int)(i % per), u = part / 4, t = part % 4;
-    const int token = (int)(row / a.c.heads), head = (int)(row % a.c.heads);
-    const long long slot = on ? a.slots[token] : -1, page = slot / P;
-    const int at = (int)(slot % P);
+    const uint32_t row = on ? i >> per_log2 : 0;
+    const int part = (int)(i & ((1u << per_log2) - 1)), u = part / 4, t = part % 4;
+    const uint32_t token = row / (uint32_t)a.c.heads, head = row - token * a.c.heads;
+    const long long slot = on ? __ldg(a.slots + token) : -1, page = slot >> page_log2;
+    const int at = (int)slot & (P - 1);
     const bool there = slot >= 0 && page < a.c.pages;
     if (slot >= 0 && !there) *reinterpret_cast<volatile int *>(a.err) = 1;
     const Kv4Offsets o = kv4_offsets(W, P, a.c.group);
     uint8_t *base = a.c.pool + (there ? ((size_t)page * a.c.heads + head) * kv4_head_bytes(W, P, a.c.group) : 0);
     T *kp = reinterpret_cast<T *>(a.k) + token * a.k_row + head * a.k_head + part * 8;
     T *vp = reinterpret_cast<T *>(a.v) + token * a.v_row + head * a.v_head + part * 8;
-    uint32_t *kc = reinterpret_cast<uint32_t *>(base + (size_t)at * (W / 2)) + t * NU + u;
-    uint16_t *vc = reinterpret_cast<uint16_t *>(base + o.vc + (size_t)at * (W / 2)) + 2 * t * NU + u;
-    __half2 *ks = reinterpret_cast<__half2 *>(base + o.ks) + (size_t)at * NG + part / G8;
-    __half2 *vs = reinterpret_cast<__half2 *>(base + o.vs) + (size_t)at * NG + part / G8;
+    uint32_t *kc = reinterpret_cast<uint32_t *>(base + at * (W / 2)) + t * NU + u;
+    uint16_t *vc = reinterpret_cast<uint16_t *>(base + o.vc + at * (W / 2)) + 2 * t * NU + u;
+    __half2 *ks = reinterpret_cast<__half2 *>(base + o.ks) + at * NG + (part >> group_log2);
+    __half2 *vs = reinterpret_cast<__half2 *>(base + o.vs) + at * NG + (part >> group_log2);
     if (STORE) {
         float x[2][8] = {};
         if (there) load8<DT>(kp, wide, x[0]), load8<DT>(vp, wide, x[1]);
@@ -46,10 +48,10 @@ __global__ void __launch_bounds__(256) k_kv4_copy(Kv4CopyArgs a, long long items
             if (there) {
                 if (w == 0) {
                     *kc = c;
-                    if (part % G8 == 0) *ks = __halves2half2(step, low);
+                    if (!(part & (G8 - 1))) *ks = __halves2half2(step, low);
                 } else {
                     vc[0] = (uint16_t)c, vc[NU] = (uint16_t)(c >> 16);
-                    if (part % G8 == 0) *vs = __halves2half2(step, low);
+                    if (!(part & (G8 - 1))) *vs = __halves2half2(step, low);
                 }
             }
         }
@@ -65,22 +67,32 @@ __global__ void __launch_bounds__(256) k_kv4_copy(Kv4CopyArgs a, long long items
     }
 }
 
+static int log2_of(int x) { return x <= 1 ? 0 : 1 + log2_of(x / 2); }
+
 template <bool STORE>
-static cudaError_t launch_copy(int dtype, const Kv4CopyArgs &a, cudaStream_t s, uint64_t *launches) {
-    const long long items = (long long)a.tokens * a.c.heads * (a.c.width / 8);
-    if (!items) return cudaSuccess;
-    const int es = dtype == DT_F32 ? 4 : 2;
+static cudaError_t launch_copy(int dtype, Kv4CopyArgs a, cudaStream_t s, uint64_t *launches) {
+    const int es = dtype == DT_F32 ? 4 : 2, per = a.c.width / 8;
     const bool wide = !((((uintptr_t)a.k | (uintptr_t)a.v) & 15) ||
                         ((a.k_row | a.k_head | a.v_row | a.v_head) * es) % 16);
-    const unsigned grid = (unsigned)((items + 255) / 256);
-    if (dtype == DT_F32)
-        k_kv4_copy<DT_F32, STORE><<<grid, 256, 0, s>>>(a, items, wide);
-    else if (dtype == DT_F16)
-        k_kv4_copy<DT_F16, STORE><<<grid, 256, 0, s>>>(a, items, wide);
-    else
-        k_kv4_copy<DT_BF16, STORE><<<grid, 256, 0, s>>>(a, items, wide);
-    if (launches) ++*launches;
-    return cudaGetLastError();
+    // indexes are 32 bits wide: very long calls in parts
+    const int most = (int)std::min<long long>(0x7fffffff, 0x7fffff00LL / ((long long)a.c.heads * per));
+    for (int left = a.tokens; left > 0;) {
+        const int n = std::min(left, most);
+        const uint32_t items = (uint32_t)n * a.c.heads * per, grid = (items + 255) / 256;
+        const int pl = log2_of(per), gl = log2_of(a.c.page), ul = log2_of(a.c.group / 8);
+        if (dtype == DT_F32)
+            k_kv4_copy<DT_F32, STORE><<<grid, 256, 0, s>>>(a, items, pl, gl, ul, wide);
+        else if (dtype == DT_F16)
+            k_kv4_copy<DT_F16, STORE><<<grid, 256, 0, s>>>(a, items, pl, gl, ul, wide);
+        else
+            k_kv4_copy<DT_BF16, STORE><<<grid, 256, 0, s>>>(a, items, pl, gl, ul, wide);
+        if (launches) ++*launches;
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return e;
+        left -= n, a.tokens = left, a.slots += n;
+        a.k = (uint8_t *)a.k + (long long)n * a.k_row * es, a.v = (uint8_t *)a.v + (long long)n * a.v_row * es;
+    }
+    return cudaSuccess;
 }
 cudaError_t launch_kv4_store(int dtype, const Kv4CopyArgs &a, cudaStream_t s, uint64_t *launches) {
     return launch_copy<true>(dtype, a, s, launches);

@@ -9,6 +9,7 @@
 // and the scores that reach it are ranked by counting. Where more than 256 do (rows of equal scores) the row is read again
 // by warps that keep sorted lists.
 #include <algorithm>
+#include <type_traits>
 
 #include <cooperative_groups.h>
 
@@ -56,6 +57,42 @@ __device__ __forceinline__ void add_score(Stats &a, float x, float c) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(t) : "f"((x - a.m) * c), "f"(-1000.f));  // a NaN stays one, and makes S NaN
     const float p = lp_exp2(t);
     a.s += p, a.e = fmaf(p, t, a.e);
+}
+// Two scores at a time: the sums in pairs, which the FMA pipe takes in one instruction.
+struct Pair {
+    unsigned long long v;
+};
+__device__ __forceinline__ Pair pair_of(float x, float y) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
+    return p;
+}
+__device__ __forceinline__ float2 floats_of(Pair p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+__device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
+    Pair p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+    return p;
+}
+__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
+    Pair p;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+    return p;
+}
+__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
+    Pair p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return p;
+}
+__device__ __forceinline__ void add_scores(Pair &s, Pair &e, float x, float y, Pair minus_m, Pair c) {
+    float2 t = floats_of(pair_mul(pair_add(pair_of(x, y), minus_m), c));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(t.x) : "f"(t.x), "f"(-1000.f));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(t.y) : "f"(t.y), "f"(-1000.f));
+    const Pair p = pair_of(lp_exp2(t.x), lp_exp2(t.y));
+    s = pair_add(s, p), e = pair_fma(p, pair_of(t.x, t.y), e);
 }
 __device__ __forceinline__ void join(Stats &a, Stats b, float c) {
     const float m = fmaxf(a.m, b.m);
@@ -207,24 +244,42 @@ __global__ void __launch_bounds__(LP_THREADS) k_logprobs(LogprobArgs a, int cs) 
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         if constexpr (DT == DT_F32) return __uint_as_float(w[j]);
         if constexpr (DT == DT_BF16) return __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[j / 2]));
-        return j & 1 ? f.y : f.x;
+        const __half2 h = *reinterpret_cast<const __half2 *>(&w[j / 2]);
+        return __half2float(j & 1 ? __high2half(h) : __low2half(h));
     };
+    const Pair cc = pair_of(c, c);
+    int keep = 0, fill = 0;
     for (int s = s0; s < s1; s++) {
         uint4 v[VEC];
         strip_load(s, v);
-        float mx = -INFINITY;
+        // the strip's largest, 16-bit types two at a time (a NaN is passed over)
+        float mx;
+        if constexpr (DT == DT_F32) {
+            mx = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < VEC; k++)
+            for (int k = 0; k < VEC; k++) mx = fmaxf(fmaxf(fmaxf(mx, get(v[k], 0)), get(v[k], 1)), fmaxf(get(v[k], 2), get(v[k], 3)));
+        } else {
+            using T2 = typename std::conditional<DT == DT_F16, __half2, __nv_bfloat162>::type;
+            T2 m2 = *reinterpret_cast<const T2 *>(&v[0].x);
 #pragma unroll
-            for (int j = 0; j < PER; j++) mx = fmaxf(mx, get(v[k], j));
+            for (int k = 0; k < VEC; k++) {
+                const T2 *w = reinterpret_cast<const T2 *>(&v[k]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) m2 = __hmax2(m2, w[j]);
+            }
+            mx = fmaxf(Elem<DT>::get(m2.x), Elem<DT>::get(m2.y));
+        }
         if (mx > st.m) rebase(st, mx, c);
+        const Pair minus_m = pair_of(-st.m, -st.m);
+        Pair ps = pair_of(0.f, 0.f), pe = ps;
 #pragma unroll
         for (int k = 0; k < VEC; k++)
 #pragma unroll
-            for (int j = 0; j < PER; j++) add_score(st, get(v[k], j), c);
+            for (int j = 0; j < PER; j += 2) add_scores(ps, pe, get(v[k], j), get(v[k], j + 1), minus_m, cc);
+        const float2 fs = floats_of(ps), fe = floats_of(pe);
+        st.s += fs.x + fs.y, st.e += fe.x + fe.y;
         top = fmaxf(top, mx), kept = fmaxf(kept, mx);
-        if ((s - s0) % share == share - 1 || s == s1 - 1) strip_max[(s - s0) / share][tid] = kept, kept = -INFINITY;
+        if (++fill == share || s == s1 - 1) strip_max[keep][tid] = kept, kept = -INFINITY, fill = 0, keep++;
     }
     // ---- the threads' and blocks' sums joined ----
     warp_join(st, c);

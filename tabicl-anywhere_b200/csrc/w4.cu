@@ -1,5 +1,6 @@
 // Linear layers with four-bit weights and group scales.
 #include <algorithm>
+#include <atomic>
 
 #include <cooperative_groups.h>
 
@@ -405,6 +406,28 @@ __global__ void __launch_bounds__(W4_WARPS * 32, NT < 8 ? 2 : 1) k_w4_linear(W4A
     }
 }
 
+// How many clusters of cs blocks of two an SM the GPU holds at once: a cluster lies within one of the GPU's processing
+// clusters, so it is fewer than their blocks over cs (with one cluster too many the product takes twice as long).
+static int w4_clusters(int cs, int sms) {
+    static std::atomic<int> known[4];
+    const int i = cs == 1 ? 0 : cs == 2 ? 1 : cs == 4 ? 2 : 3;
+    int n = known[i];
+    if (!n) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * sms / cs * cs), cfg.blockDim = dim3(W4_WARPS * 32), cfg.dynamicSmemBytes = 100 << 10;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+        cfg.attrs = at, cfg.numAttrs = 1;
+        const auto kernel = k_w4_linear<128, 1, 1>;
+        if (allow_dynamic_smem((const void *)kernel, cfg.dynamicSmemBytes) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1)
+            n = std::max(1, 2 * sms / cs);
+        known[i] = n;
+    }
+    return n;
+}
+
 static W4Plan w4_plan(int dtype, const W4Args &a, int sms) {
     W4Plan p;
     const int qs = dtype == DT_F32 ? 2 : 1, blocks = (a.k + 127) / 128, tiles = (a.n + 15) / 16;
@@ -415,7 +438,7 @@ static W4Plan w4_plan(int dtype, const W4Args &a, int sms) {
     while (p.cs < 8 && (blocks > W4_SLICE * p.cs || (blocks >= 16 * p.cs && tiles * p.cs * 2 <= sms))) p.cs *= 2;
     p.slice = (blocks + p.cs - 1) / p.cs;
     p.pass = std::min({p.slice, W4_SLICE, std::max(1, W4_X_BYTES / (4 * w4_frag_words(p.nt, qs)))});
-    p.groups = std::min(tiles, std::max(1, 2 * sms / (p.cs * p.row_tiles)));
+    p.groups = std::min(tiles, std::max(1, w4_clusters(p.cs, sms) / p.row_tiles));
     p.tiles = std::min((tiles + p.groups - 1) / p.groups, W4_Y_UNITS / p.nt);
     p.groups = std::min(p.groups, (tiles + p.tiles - 1) / p.tiles);
     // a power of two of parts of a slice, so that the warps share the tiles evenly
