@@ -47,9 +47,16 @@ def signatures():
     }
 
 
+_loaded = None
+
+
 def _lib():
-    from . import lib
-    return lib()
+    """The library (kept here: a call's own time on the host is a few microseconds)."""
+    global _loaded
+    if _loaded is None:
+        from . import lib
+        _loaded = lib()
+    return _loaded
 
 
 class Kv4Cache:
@@ -67,13 +74,15 @@ class Kv4Cache:
     def store(self, dtype, tokens, slots_ptr, k_ptr, k_row, k_head, v_ptr, v_row, v_head, stream=None):
         """Quantise rows of keys and values ([heads][width] by row and head strides) into their slots (int64; negative:
         skipped)."""
-        return self.gpu.check(_lib().tcu_kv4_store_device(self.gpu._h, self._c, dtype, tokens, slots_ptr, k_ptr, k_row, k_head,
-                                                          v_ptr, v_row, v_head, stream))
+        r = _lib().tcu_kv4_store_device(self.gpu._h, self._c, dtype, tokens, slots_ptr, k_ptr, k_row, k_head, v_ptr, v_row,
+                                        v_head, stream)
+        return r if r == 0 else self.gpu.check(r)
 
     def load(self, dtype, tokens, slots_ptr, k_ptr, k_row, k_head, v_ptr, v_row, v_head, stream=None):
         """The numbers that the slots' keys and values stand for (zeros for a negative slot)."""
-        return self.gpu.check(_lib().tcu_kv4_load_device(self.gpu._h, self._c, dtype, tokens, slots_ptr, k_ptr, k_row, k_head,
-                                                         v_ptr, v_row, v_head, stream))
+        r = _lib().tcu_kv4_load_device(self.gpu._h, self._c, dtype, tokens, slots_ptr, k_ptr, k_row, k_head, v_ptr, v_row,
+                                       v_head, stream)
+        return r if r == 0 else self.gpu.check(r)
 
     @staticmethod
     def batch(seqs, max_rows, max_len, lens_ptr, table_ptr, table_stride, starts_ptr=None, rows=None):
@@ -92,9 +101,9 @@ class Kv4Cache:
     def attend(self, batch, dtype, q_heads, q_ptr, q_row, q_head, out_ptr, o_row, o_head, scale, causal=False, window=0,
                lse=None, work=None, work_bytes=0, stream=None):
         """Softmax attention of the batch's query rows; lse (optional): f32 [rows][q_heads]."""
-        return self.gpu.check(_lib().tcu_kv4_attend_device(self.gpu._h, self._c, batch, dtype, q_heads, q_ptr, q_row, q_head,
-                                                           out_ptr, o_row, o_head, scale, causal, window, lse, work,
-                                                           work_bytes, stream))
+        r = _lib().tcu_kv4_attend_device(self.gpu._h, self._c, batch, dtype, q_heads, q_ptr, q_row, q_head, out_ptr, o_row,
+                                         o_head, scale, causal, window, lse, work, work_bytes, stream)
+        return r if r == 0 else self.gpu.check(r)
 
 
 class W4:
@@ -128,5 +137,6 @@ class W4:
     def linear(self, dtype, rows, x_ptr, ldx, y_ptr, ldy, bias=None, act=0, residual=None, ldr=0, work=None, work_bytes=0,
                stream=None):
         """y = act(x W^T + bias) + residual; act 1 is GELU, the residual may be y itself."""
-        return self.gpu.check(_lib().tcu_w4_linear_device(self.gpu._h, self._w, dtype, rows, x_ptr, ldx, y_ptr, ldy, bias, act,
-                                                          residual, ldr, work, work_bytes, stream))
+        r = _lib().tcu_w4_linear_device(self.gpu._h, self._w, dtype, rows, x_ptr, ldx, y_ptr, ldy, bias, act, residual, ldr, work,
+                                        work_bytes, stream)
+        return r if r == 0 else self.gpu.check(r)
