@@ -224,13 +224,18 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
         }
     }
 
-    // the running state, in units of 2^m for a column (m moves only when a score passes it by 8) and 2^ve for the weights
-    float m[NT][2], bound[NT][2], l[NT][2], ls[NT][NG][2], o[NT][NU][2][4];
+    // the running state of a column, in units of 2^off: off = m - 7 + ve, m the column's reference (it moves only when a score
+    // passes it by 8), 2^ve the largest value step so far or more. So a weight is at most 2^(15 - ve), and with its step at
+    // most 2^15: inside f16, and 2^7 above where the largest would leave small ones the least room. A 16-bit type's weights
+    // are f16 before they meet their step too, so there ve stays at 0 or above; f32's are not.
+    float m[NT][2], off_m[NT][2], bound[NT][2], l[NT][2], ls[NT][NG][2], o[NT][NU][2][4];
     float ol[NT][4] = {};  // sums of p low of group g, where they are taken as a matrix product
     constexpr bool LOW_MMA_V = C::LOW_MMA && !SPLIT;
-    float vtop = 0.f, vinv = 1.f;  // the largest step so far rounded up to a power of two, and its reciprocal
+    int ve = SPLIT ? -24 : 0;  // (steps are f16: at least 2^-24)
+    float vtop = pow2i(ve);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
+        off_m[nt][0] = off_m[nt][1] = (float)(ve - 7);
         m[nt][0] = m[nt][1] = bound[nt][0] = bound[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
         for (int k = 0; k < NG; k++) ls[nt][k][0] = ls[nt][k][1] = 0.f;
@@ -240,7 +245,6 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
             for (int x = 0; x < 8; x++) o[nt][u][x >> 2][x & 3] = 0.f;
     }
 
-    __half2 vnorm = __float2half2_rn(1.f);  // 16-bit types: 1 / vtop, by which the steps come into f16's range
     bool gave_up = false;
     for (int it = 0; it < mine; it++) {
         load(it + ST - 1);
@@ -346,10 +350,17 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
                     }
                 }
         }
-        __half2 smax = *reinterpret_cast<const __half2 *>(&vs[0][0][0]);
+        // the largest value step: a lane looks at one key's
+        float step_max;
+        {
+            uint32_t w[NG];
+            lds_words<NG>(tile + 2 * C::KC + C::SC + lane * NG * 4, w);
+            __half2 x = *reinterpret_cast<const __half2 *>(&w[0]);
 #pragma unroll
-        for (int i = 1; i < 4 * NG; i++) smax = __hmax2(smax, *reinterpret_cast<const __half2 *>(&vs[i / (2 * NG)][i / NG % 2][i % NG]));
-        float step_max = __low2float(smax);
+            for (int k = 1; k < NG; k++) x = __hmax2(x, *reinterpret_cast<const __half2 *>(&w[k]));
+            step_max = __low2float(x);
+            if (edge && (j0 + lane >= hi_max || j0 + lane < lo_min)) step_max = 0.f;
+        }
         bool moves = step_max > vtop;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -359,13 +370,10 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
         if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
             for (int d = 1; d < 32; d *= 2) step_max = fmaxf(step_max, __shfl_xor_sync(0xffffffffu, step_max, d));
-            float vf = 1.f;
-            if (step_max > vtop) {
-                // the next power of two (steps are positive f16: at least 2^-24)
+            int grow = 0;
+            if (step_max > vtop) {  // the next power of two above
                 const int e = (int)(__float_as_uint(step_max) >> 23) - 126;
-                const float top = SPLIT ? pow2i(e) : pow2i(max(e, -15));
-                vf = vtop / top, vtop = top, vinv = 1.f / top;
-                vnorm = __float2half2_rn(1.f / top);
+                grow = e - ve, ve = e, vtop = pow2i(e);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -376,27 +384,25 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
                     for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
                     x = fmaxf(x * fq[nt][c], m[nt][c]);
                     bound[nt][c] = x == -INFINITY ? x : (x + 8.f) / fq[nt][c];
-                    const float f = x > m[nt][c] ? exp2_sfu(m[nt][c] - x) : 1.f, fo = f * vf;
-                    m[nt][c] = x, l[nt][c] *= f, ol[nt][c] *= f;
+                    const float f = (x > m[nt][c] ? exp2_sfu(m[nt][c] - x) : 1.f) * pow2i(-grow);
+                    m[nt][c] = x, off_m[nt][c] = (x == -INFINITY ? 0.f : x) + (float)(ve - 7), l[nt][c] *= f, ol[nt][c] *= f;
 #pragma unroll
                     for (int k = 0; k < NG; k++) ls[nt][k][c] *= f;
 #pragma unroll
                     for (int u = 0; u < NU; u++)
 #pragma unroll
-                        for (int i = 0; i < 2; i++) o[nt][u][i][c] *= fo, o[nt][u][i][c + 2] *= fo;
+                        for (int i = 0; i < 2; i++) o[nt][u][i][c] *= f, o[nt][u][i][c + 2] *= f;
                 }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                // weights come 2^7 times as large (up to 2^15), so that small ones stay normal in f16
-                const float mm = m[nt][c] == -INFINITY ? 0.f : m[nt][c] - 7.f;
 #pragma unroll
                 for (int kb = 0; kb < 2; kb++)
 #pragma unroll
                     for (int h = 0; h < 4; h += 2) {
-                        const float p = exp2_sfu(fmaf(s[kb][nt][c + h], fq[nt][c], -mm));
+                        const float p = exp2_sfu(fmaf(s[kb][nt][c + h], fq[nt][c], -off_m[nt][c]));
                         s[kb][nt][c + h] = p, l[nt][c] += p;
                     }
             }
@@ -459,7 +465,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
             for (int k = 0; k < NG; k++) {
                 uint32_t b[QS][NT][2];
                 if constexpr (SPLIT) {
-                    const float w[2] = {bits_float2(vs[kb][0][k]).x * vinv, bits_float2(vs[kb][1][k]).x * vinv};
+                    const float w[2] = {bits_float2(vs[kb][0][k]).x, bits_float2(vs[kb][1][k]).x};
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -473,7 +479,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
                     // p and p * step each round to 11 bits, as the results do to 11 or 8
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const __half2 w = __hmul2(__low2half2(*reinterpret_cast<const __half2 *>(&vs[kb][h][k])), vnorm);
+                        const __half2 w = __low2half2(*reinterpret_cast<const __half2 *>(&vs[kb][h][k]));
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             const __half2 x = __hmul2(p2[nt][h], w);
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
     __syncthreads();
     float *so = reinterpret_cast<float *>(sm);  // [warp][R][HD]
     float *sms = so + KA_WARPS * R * HD;        // [warp][R]{m, l}
-    const float unv = vtop * 16777216.f;
+    constexpr float unv = 16777216.f;  // 2^24
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -519,7 +525,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
                 if (LOW_MMA_V) y[k] += __shfl_sync(0xffffffffu, ol[nt][c], k * 4 + t);
             }
             const int r = nt * 8 + 2 * t + c;
-            if (g == 0) sms[(warp * R + r) * 2] = m[nt][c] - 7.f, sms[(warp * R + r) * 2 + 1] = x;
+            if (g == 0) sms[(warp * R + r) * 2] = m[nt][c] == -INFINITY ? -INFINITY : off_m[nt][c], sms[(warp * R + r) * 2 + 1] = x;
             float *dst = so + (warp * R + r) * HD + 4 * g;
 #pragma unroll
             for (int u = 0; u < NU; u++)
@@ -580,41 +586,49 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
             __threadfence();
             auto slot_of = [&](int p) { return Cut::slot(b0 + p, p == 0); };
             const float *po0 = part + 2 * nslots * R;
-            for (int r = warp; r < rows; r += KA_WARPS) {  // a warp a row: 32 parts' (maximum, sum) at a time
+            // row by row; a warp sums every fourth part (eight in flight), the warps' sums are joined in shared memory
+            float *sv = reinterpret_cast<float *>(sm);  // [2][warps][HD + 1]
+            for (int r = 0; r < rows; r++) {
                 float M = -INFINITY, L = 0.f;
                 for (int p = lane; p < np; p += 32) M = fmaxf(M, __ldcg(part + 2 * (slot_of(p) * R + r)));
 #pragma unroll
                 for (int d = 1; d < 32; d *= 2) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
                 const float M0 = M == -INFINITY ? 0.f : M;
                 float v[HD / 32] = {};
-                for (int p0 = 0; p0 < np; p0 += 32) {
-                    float f = 0.f;
-                    if (p0 + lane < np) {
-                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(part) + slot_of(p0 + lane) * R + r);
-                        f = exp2_sfu(x.x - M0), L = fmaf(x.y, f, L);
+                for (int p0 = warp; p0 < np; p0 += 8 * KA_WARPS) {
+                    float y[8][HD / 32];
+                    float2 x[8];
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {
+                        const int p = p0 + q * KA_WARPS;
+                        x[q] = p < np ? __ldcg(reinterpret_cast<const float2 *>(part) + slot_of(p) * R + r) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                        for (int k = 0; k < HD / 32; k++) y[q][k] = p < np ? __ldcg(po0 + (slot_of(p) * R + r) * HD + k * 32 + lane) : 0.f;
                     }
-                    const int n = min(32, np - p0);
-                    for (int q0 = 0; q0 < n; q0 += 8) {
-                        float y[8][HD / 32];
 #pragma unroll
-                        for (int q = 0; q < 8; q++)
+                    for (int q = 0; q < 8; q++) {
+                        const float f = exp2_sfu(x[q].x - M0);
+                        L = fmaf(x[q].y, f, L);
 #pragma unroll
-                            for (int k = 0; k < HD / 32; k++)
-                                y[q][k] = q0 + q < n ? __ldcg(po0 + (slot_of(p0 + q0 + q) * R + r) * HD + k * 32 + lane) : 0.f;
-#pragma unroll
-                        for (int q = 0; q < 8; q++) {
-                            const float w = __shfl_sync(0xffffffffu, f, q0 + q);
-                            if (q0 + q < n)
-#pragma unroll
-                                for (int k = 0; k < HD / 32; k++) v[k] = fmaf(y[q][k], w, v[k]);
-                        }
+                        for (int k = 0; k < HD / 32; k++) v[k] = fmaf(y[q][k], f, v[k]);
                     }
                 }
+                float *mine_v = sv + ((r & 1) * KA_WARPS + warp) * (HD + 1);
 #pragma unroll
-                for (int d = 1; d < 32; d *= 2) L += __shfl_xor_sync(0xffffffffu, L, d);
+                for (int k = 0; k < HD / 32; k++) mine_v[k * 32 + lane] = v[k];
+                if (lane == 0) mine_v[HD] = L;
+                __syncthreads();
+                const float *all = sv + (r & 1) * KA_WARPS * (HD + 1);
+                L = 0.f;
 #pragma unroll
-                for (int k = 0; k < HD / 32; k++) put(r, k * 32 + lane, L != 0.f ? v[k] / L : 0.f);
-                if (lane == 0) put_lse(r, M0, L);
+                for (int w = 0; w < KA_WARPS; w++) L += all[w * (HD + 1) + HD];
+                for (int c = tid; c < HD; c += KA_STEP) {
+                    float x = 0.f;
+#pragma unroll
+                    for (int w = 0; w < KA_WARPS; w++) x += all[w * (HD + 1) + c];
+                    put(r, c, L != 0.f ? x / L : 0.f);
+                }
+                if (tid == 0) put_lse(r, M0, L);
             }
         }
     }
