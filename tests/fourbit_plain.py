@@ -34,6 +34,11 @@ def pack(code, values):
     return nib[..., 0::2] | (nib[..., 1::2] << 4)
 
 
+def unpack(raw, values):
+    nib = np.stack([raw & 15, raw >> 4], -1).reshape(*raw.shape[:-1], -1)
+    return nib[..., places(nib.shape[-1], values)]
+
+
 def scales(step, low):
     return np.stack([step, low], -1)
 

@@ -549,3 +549,45 @@ def test_attend_shares_working_memory_between_calls_of_different_shape(gpu):
                 out, lse = c.attend("bf16", q, counts, 0.125, causal=True, window=window, work=work)
                 sync(gpu)
                 c.check("bf16", q, counts, 0.125, True, window, out, lse)
+
+
+@pytest.mark.parametrize("test_rows", [1, 40])
+def test_the_example_runs_the_operators_together(test_rows):
+    """examples/four_bit_member.py on a small member, against the same stage in 64 bits over what its caches and weights stand
+    for: within the bar of every cached stage here (5e-5 on raw decoder scores)."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "four_bit_member.py")
+    spec = importlib.util.spec_from_file_location("four_bit_member", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    member, h, scores = example.main(["--rows", "700", "--test", str(test_rows)])
+
+    def values(lin):
+        """A four-bit layer's weights in 64 bits."""
+        g = example.GROUP
+        codes = lin.codes.cpu().numpy().reshape(lin.n, -1, 64)
+        sc = lin.scales.cpu().numpy().view(np.float16).reshape(lin.n, codes.shape[1], 128 // g, 2)
+        w = plain.value(plain.unpack(codes, False), sc[..., 0], sc[..., 1], g).reshape(lin.n, -1)[:, :lin.k]
+        return torch.from_numpy(w).cuda(), lin.bias.double()
+
+    def linear(x, lin, gelu=False):
+        w, b = values(lin)
+        y = x @ w.T + b
+        return torch.nn.functional.gelu(y) if gelu else y
+
+    norm = lambda x, p: torch.nn.functional.layer_norm(x, (member.d,), p[0].double(), p[1].double())  # noqa: E731
+    x, n, d, w = h.double(), h.shape[0], member.d, member.width
+    slots = torch.arange(member.rows, dtype=torch.int64, device="cuda")
+    for l, b in enumerate(member.blocks):
+        k, v = (torch.empty(member.rows, d, device="cuda") for _ in range(2))
+        member.caches[l].load(0, member.rows, slots.data_ptr(), k.data_ptr(), d, w, v.data_ptr(), d, w, stream=1)
+        heads = lambda t: t.double().view(-1, member.heads, w).transpose(0, 1)  # noqa: E731
+        q = linear(norm(x, b["n1"]), b["wq"])
+        m = linear(linear(q.view(-1, w), b["q0"], True), b["q2"]).view(n, d)
+        q = q * member.scale[l].double() * (1 + torch.tanh(m))
+        att = (torch.softmax(heads(q) @ heads(k).transpose(1, 2), -1) @ heads(v)).transpose(0, 1).reshape(n, d)
+        x = x + linear(att, b["wo"])
+        x = x + linear(linear(norm(x, b["n2"]), b["w1"], True), b["w2"])
+    want = linear(linear(norm(x, member.ln), member.dec0, True), member.dec2)
+    assert float((scores.double() - want).abs().max()) <= 5e-5
