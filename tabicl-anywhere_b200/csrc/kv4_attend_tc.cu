@@ -16,7 +16,7 @@
 
 namespace tcu {
 
-constexpr int KT_BQ = 128, KT_BK = 64, KT_NS = 3, KT_THREADS = 512;
+constexpr int KT_BQ = 128, KT_BK = 64, KT_NS = 3, KT_THREADS = 640;
 constexpr uint32_t KT_TQ = 0, KT_TS = 128, KT_TO = 384;
 
 template <int HD, int G, bool SPLIT>
@@ -29,8 +29,8 @@ struct KtShape {
     static constexpr size_t SMEM = (size_t)2 * KT_NS * QS * BLOCK * 2 + (size_t)NR * RAW + 1024;
 };
 
-// Warps 0-3: softmax, a thread a query row; warps 4-7: the fold of each step's P V, a thread a row; warps 8-11: widening;
-// warp 12, 13: one thread each issues the S products of even and odd steps; warp 14: one thread the P V products; warp 15:
+// Warps 0-3: softmax, a thread a query row; warps 4-7: the fold of each step's P V, a thread a row; warps 8-11, 12-15:
+// widening of even and odd steps; warps 16, 17 issue the S products of even and odd steps, warp 18 the P V products; warp 19:
 // the copies of the stored codes. They hand over through mbarriers; every wait is bounded, and one that gives up raises the
 // block's abort flag, after which every wait returns at once and the roles run to the end without results.
 template <int HD, int G, bool SPLIT>
@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
     __half *Kring = reinterpret_cast<__half *>(smraw);                // [NS][QS][64 x HD], K-major
     __half *Vring = Kring + NS * QS * BLOCK;                          // [NS][QS][64 x HD], coordinate-major
     uint8_t *raw = reinterpret_cast<uint8_t *>(Vring + NS * QS * BLOCK);  // [NR]{key codes, key scales, value codes, value scales}
-    __shared__ float fr[4][BQ], rowx[2][BQ], qmax[2][BQ], red[2][2][4];
+    __shared__ float fr[4][BQ], rowx[2][BQ], qmax[2][BQ], red[2][2][2][4];  // red: [turn][step][keys, values][warp]
     __shared__ int teK[8], teV[8], has_nan[8];
     __shared__ uint32_t nan_keys[8][NG][2];
     __shared__ __align__(8) uint64_t mK[NS], mV[NS], mKfree[NS], mVfree[NS], mS[NS], mP[NS], mSlot[NS], mF[4], mPV, mOfree, mDone[3],
@@ -148,9 +148,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
     // the pieces of units that are this block's, in every role alike: n steps from key j0 on, `at` steps before them
     int at = 0;
 
-    if (wg == 3) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == 15) {
+    if (wg == 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+        if (warp == 19) {
             // ---- copies: lane part + 4 * piece brings one of the four arrays of one page's share of the 64 keys ----
             const Kv4Offsets off = kv4_offsets(HD, a.c.page, G);
             const size_t hb = kv4_head_bytes(HD, a.c.page, G);
@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                     for (int i = at; i < at + n; i++) {
                         const int sl = i % NS;
                         const uint32_t ph = (uint32_t)(i / NS) & 1u;
-                        if (warp < 14) {
-                            if ((i & 1) != warp - 12) continue;
+                        if (warp < 18) {
+                            if ((i & 1) != warp - 16) continue;
                             // S(i) once P V(i - NS) has read its slot, from the keys of step i
                             if (i >= NS) wait_warp(&mSlot[sl], ph ^ 1u);
                             wait_warp(&mK[sl], ph);
@@ -258,20 +258,20 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 Cut::next(pl, a, each, sr.n, n);
             }
             if (elect_one()) {  // every product issued here completes before the block lets go of its memory
-                mma_commit(&mDone[warp - 12]);
-                mbar_wait(&mDone[warp - 12], 0, KT_WAIT);
+                mma_commit(&mDone[warp - 16]);
+                mbar_wait(&mDone[warp - 16], 0, KT_WAIT);
             }
         }
-    } else if (wg == 2) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-        // ---- widening: a thread half a key's coordinates and half a value's ----
+    } else if (wg >= 2) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        // ---- widening: a thread half a key's coordinates and half a value's, of every other step ----
         // (a wait that gave up does not end the loop: the four warps meet at a barrier in every step)
-        const int key = tid & 63, half = (tid >> 6) & 1, w4 = warp & 3;
+        const int key = tid & 63, half = (tid >> 6) & 1, w4 = warp & 3, turn = wg - 2;
         while (pl.pos < pl.end) {
             const KaRows sr = ka_rows(a, pl.seq);
             const auto sp = Cut::span(a, sr, each, pl.rt);
             const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), j0 = sp.base + pl.skip * BK;
-            for (int i = at; i < at + n; i++) {
+            for (int i = at + ((at ^ turn) & 1); i < at + n; i += 2) {
                 const int sl = i % NS, rs = i % NR, j = j0 + (i - at) * BK + key;
                 const uint32_t ph = (uint32_t)(i / NS) & 1u;
                 wait_warp(&mRaw[rs], (uint32_t)(i / NR) & 1u);
@@ -284,35 +284,34 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 lds_words<NG>(kraw + C::KC + key * NG * 4, kc);
                 lds_words<NG>(vraw + C::KC + key * NG * 4, vc);
                 // the step's power of two, for keys and values: from each group's ends
-                float2 ks[NG], vs[NG];
                 float mx[2] = {0.f, 0.f};
                 bool nan = false;
 #pragma unroll
                 for (int k = 0; k < NG; k++) {
-                    ks[k] = seen ? __half22float2(kt_h2(kc[k])) : make_float2(0.f, 0.f);
-                    vs[k] = seen ? __half22float2(kt_h2(vc[k])) : make_float2(0.f, 0.f);
-                    mx[0] = fmaxf(mx[0], fmaxf(fabsf(ks[k].y), fabsf(fmaf(15.f, ks[k].x, ks[k].y))));
-                    mx[1] = fmaxf(mx[1], fmaxf(fabsf(vs[k].y), fabsf(fmaf(15.f, vs[k].x, vs[k].y))));
-                    nan |= vs[k].y != vs[k].y;
+                    if (!seen) kc[k] = vc[k] = 0;
+                    const float2 ks = __half22float2(kt_h2(kc[k])), vs = __half22float2(kt_h2(vc[k]));
+                    mx[0] = fmaxf(mx[0], fmaxf(fabsf(ks.y), fabsf(fmaf(15.f, ks.x, ks.y))));
+                    mx[1] = fmaxf(mx[1], fmaxf(fabsf(vs.y), fabsf(fmaf(15.f, vs.x, vs.y))));
+                    nan |= vs.y != vs.y;
                 }
                 // a group of values that stands for NaN is left out here and put into the rows that see it by the fold
                 nan = __any_sync(0xffffffffu, nan);
                 if (nan) {
 #pragma unroll
                     for (int k = 0; k < NG; k++) {
-                        const bool bad = vs[k].y != vs[k].y;
+                        const bool bad = (vc[k] & 0x7fff0000u) > 0x7c000000u;
                         const unsigned who = __ballot_sync(0xffffffffu, bad);
                         if (half == 0 && lane == 0) nan_keys[i & 7][k][w4] = who;
-                        if (bad) vs[k].y = 0.f;
+                        if (bad) vc[k] = 0;
                     }
                 } else if (half == 0 && lane < NG) {
                     nan_keys[i & 7][lane][w4] = 0;
                 }
                 mx[0] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[0])));  // (not negative: ordered as their bits)
                 mx[1] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[1])));
-                if (lane == 0) red[i & 1][0][w4] = mx[0], red[i & 1][1][w4] = nan ? -mx[1] - 1.f : mx[1];  // a NaN shows as the sign
+                if (lane == 0) red[turn][i >> 1 & 1][0][w4] = mx[0], red[turn][i >> 1 & 1][1][w4] = nan ? -mx[1] - 1.f : mx[1];  // a NaN shows as the sign
                 mbar_arrive(&mRawFree[rs]);
-                kt_bar(3, 128);
+                kt_bar(3 + turn, 128);
                 int e[2];
                 bool any = false;
 #pragma unroll
@@ -320,7 +319,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                     float m = 0.f;
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
-                        const float r = red[i & 1][x][w];
+                        const float r = red[turn][i >> 1 & 1][x][w];
                         any |= r < 0.f, m = fmaxf(m, r < 0.f ? -1.f - r : r);
                     }
                     e[x] = m > 0.f ? min(40, (int)(__float_as_uint(m) >> 23) - 125) : 0;  // m < 2^(e - 1): a span, 15 steps, below 2^e
@@ -329,17 +328,18 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 if (i >= NS) wait_warp(&mKfree[sl], ph ^ 1u);
                 {
                     __half *hi = Kring + sl * QS * BLOCK, *lo = hi + (SPLIT ? BLOCK : 0);
-                    KtScale<SPLIT> s[NG];
 #pragma unroll
-                    for (int k = 0; k < NG; k++) s[k].set(ks[k].x, ks[k].y, kt_pow2(C::T - e[0]));
+                    for (int k = 0; k < NG; k++) {
+                        KtScale<SPLIT> s;
+                        const float2 f = __half22float2(kt_h2(kc[k]));
+                        s.set(f.x, f.y, kt_pow2(C::T - e[0]));
 #pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const int t = 2 * half + x;
+                        for (int x = 0; x < 2; x++)
 #pragma unroll
-                        for (int u = 0; u < NU; u++) {
-                            const int o = kmajor_off(key, 32 * u + 8 * t, BK);
-                            kt_widen(kw[x * NU + u], s[u / UG], hi + o, lo + o);
-                        }
+                            for (int u = k * UG; u < (k + 1) * UG; u++) {
+                                const int o = kmajor_off(key, 32 * u + 8 * (2 * half + x), BK);
+                                kt_widen(kw[x * NU + u], s, hi + o, lo + o);
+                            }
                     }
                 }
                 fence_async_smem();
@@ -347,22 +347,24 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 if (i >= NS) wait_warp(&mVfree[sl], ph ^ 1u);
                 {
                     __half *hi = Vring + sl * QS * BLOCK, *lo = hi + (SPLIT ? BLOCK : 0);
-                    KtScale<SPLIT> s[NG];
 #pragma unroll
-                    for (int k = 0; k < NG; k++) s[k].set(vs[k].x, vs[k].y, kt_pow2(C::T - e[1]));
+                    for (int k = 0; k < NG; k++) {
+                        KtScale<SPLIT> s;
+                        const float2 f = __half22float2(kt_h2(vc[k]));
+                        s.set(f.x, f.y, kt_pow2(C::T - e[1]));
 #pragma unroll
-                    for (int x = 0; x < 2; x++) {
-                        const int q = 2 * half + x;  // half-words g = 2 q and 2 q + 1 of every unit: coordinates 32 u + 8 q + (0..7)
+                        for (int x = 0; x < 2; x++)
 #pragma unroll
-                        for (int u = 0; u < NU; u++) {
-                            uint32_t c;
-                            if constexpr (NU == 1)
-                                c = vw[x];
-                            else
-                                c = __byte_perm(vw[x * NU + u / 2], vw[x * NU + NU / 2 + u / 2], u & 1 ? 0x7632 : 0x5410);
-                            const int o = mnmajor_off(32 * u + 8 * q, key, HD);
-                            kt_widen(c, s[u / UG], hi + o, lo + o);
-                        }
+                            for (int u = k * UG; u < (k + 1) * UG; u++) {
+                                // half-words g = 2 q and 2 q + 1 of a unit: coordinates 32 u + 8 q + (0..7)
+                                uint32_t c;
+                                if constexpr (NU == 1)
+                                    c = vw[x];
+                                else
+                                    c = __byte_perm(vw[x * NU + u / 2], vw[x * NU + NU / 2 + u / 2], u & 1 ? 0x7632 : 0x5410);
+                                const int o = mnmajor_off(32 * u + 8 * (2 * half + x), key, HD);
+                                kt_widen(c, s, hi + o, lo + o);
+                            }
                     }
                 }
                 fence_async_smem();
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
             Cut::next(pl, a, each, sr.n, n);
         }
     } else if (wg == 0) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         while (pl.pos < pl.end) {
             const KaRows sr = ka_rows(a, pl.seq);
             const auto sp = Cut::span(a, sr, each, pl.rt);
@@ -503,12 +505,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                                         __stcg(reinterpret_cast<float4 *>(po + mine * HD + k), make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
                                 }
                                 __threadfence();
-                                kt_bar(4, 128);
+                                kt_bar(5, 128);
                                 if (row == 0) {
                                     s_last = atomicAdd(arrived + who.x, 1) == who.y - 1;
                                     if (s_last) arrived[who.x] = 0;  // ready for the next call
                                 }
-                                kt_bar(4, 128);
+                                kt_bar(5, 128);
                                 write = write && s_last;
                                 if (write) {
                                     __threadfence();
