@@ -269,11 +269,36 @@ __global__ void __launch_bounds__(W4_WARPS * 32, NT < 8 ? 2 : 1) k_w4_linear(W4A
                 const bool wide = !(((uintptr_t)a.x & 15) || (a.ldx * es) % 16);
                 const uint8_t *row = reinterpret_cast<const uint8_t *>(a.x) + (long long)(r0 + min(warp, rows - 1)) * a.ldx * es;
                 float v[W4_SLICE / 2][8], mx = 0.f;
+                if (wide && (b0 + nb) * 128 <= a.k) {  // whole vectors, all asked for before any is used
+                    uint4 raw[W4_SLICE / 2][QS];
+                    const uint4 *src = reinterpret_cast<const uint4 *>(row + (size_t)b0 * 128 * es) + lane * QS;
 #pragma unroll
-                for (int x = 0; x < W4_SLICE / 2; x++) {
+                    for (int x = 0; x < W4_SLICE / 2; x++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[x][j] = 0.f;
-                    if (warp < rows && x * 32 + lane < nb * 16) w4_x8(dtype, row, b0 * 128 + (x * 32 + lane) * 8, a.k, wide, v[x]);
+                        for (int k = 0; k < QS; k++)
+                            raw[x][k] = warp < rows && x * 32 + lane < nb * 16 ? __ldg(src + x * 32 * QS + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int x = 0; x < W4_SLICE / 2; x++) {
+                        const uint32_t w[4] = {raw[x][0].x, raw[x][0].y, raw[x][0].z, raw[x][0].w};
+                        if constexpr (QS == 2) {
+                            const uint32_t z[4] = {raw[x][1].x, raw[x][1].y, raw[x][1].z, raw[x][1].w};
+#pragma unroll
+                            for (int j = 0; j < 4; j++) v[x][j] = __uint_as_float(w[j]), v[x][j + 4] = __uint_as_float(z[j]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const float2 f = dtype == DT_BF16 ? make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u)) : w4_float2(w[j]);
+                                v[x][2 * j] = f.x, v[x][2 * j + 1] = f.y;
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < W4_SLICE / 2; x++) {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) v[x][j] = 0.f;
+                        if (warp < rows && x * 32 + lane < nb * 16) w4_x8(dtype, row, b0 * 128 + (x * 32 + lane) * 8, a.k, wide, v[x]);
+                    }
                 }
 #pragma unroll
                 for (int x = 0; x < W4_SLICE / 2; x++)
@@ -441,11 +466,12 @@ static W4Plan w4_plan(int dtype, const W4Args &a, int sms) {
     p.groups = std::min(tiles, std::max(1, w4_clusters(p.cs, sms) / p.row_tiles));
     p.tiles = std::min((tiles + p.groups - 1) / p.groups, W4_Y_UNITS / p.nt);
     p.groups = std::min(p.groups, (tiles + p.tiles - 1) / p.tiles);
-    // a power of two of parts of a slice, so that the warps share the tiles evenly
+    // a power of two of parts of a slice where the warps share the tiles more evenly by it: a warp that streams a whole slice
+    // of its rows reads memory in longer runs (14336 x 8192: 25.4 us with one part of 16 steps, 27.2 us with four of 14)
     p.parts = 0;
     for (int h = 1; h <= 3 && 2 << h <= p.pass + 1 && p.tiles << h <= W4_Y_UNITS / p.nt; h++) {
         auto cost = [&](int x) { return (((p.tiles << x) + W4_WARPS - 1) / W4_WARPS) * (((p.pass + 1) / 2 + (1 << x) - 1) >> x); };
-        if (cost(h) < cost(p.parts)) p.parts = h;
+        if (cost(h) * 8 < cost(p.parts) * 7) p.parts = h;
     }
     return p;
 }
