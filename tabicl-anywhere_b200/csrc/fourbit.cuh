@@ -165,6 +165,48 @@ __device__ __forceinline__ void store8(typename Elem<DT>::T *p, bool wide, const
     }
 }
 
+// N runs of eight elements, `step` elements apart, of a type known at run time: where they are whole aligned vectors all are
+// asked for before any is used (a branch between two loads makes the second wait for the first).
+template <int N>
+__device__ __forceinline__ void load_runs(int dtype, const void *base, long long at, int step, bool wide, float (&v)[N][8]) {
+    if (wide && dtype == DT_F32) {
+        const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(base) + at);
+        float4 raw[N][2];
+#pragma unroll
+        for (int i = 0; i < N; i++) raw[i][0] = __ldg(p + i * (step / 4)), raw[i][1] = __ldg(p + i * (step / 4) + 1);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            v[i][0] = raw[i][0].x, v[i][1] = raw[i][0].y, v[i][2] = raw[i][0].z, v[i][3] = raw[i][0].w;
+            v[i][4] = raw[i][1].x, v[i][5] = raw[i][1].y, v[i][6] = raw[i][1].z, v[i][7] = raw[i][1].w;
+        }
+    } else if (wide) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(base) + at);
+        uint4 raw[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) raw[i] = __ldg(p + i * (step / 8));
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 f = dtype == DT_BF16 ? make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u))
+                                                  : __half22float2(*reinterpret_cast<const __half2 *>(&w[j]));
+                v[i][2 * j] = f.x, v[i][2 * j + 1] = f.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (dtype == DT_F32)
+                load8<DT_F32>(reinterpret_cast<const float *>(base) + at + i * step, false, v[i]);
+            else if (dtype == DT_F16)
+                load8<DT_F16>(reinterpret_cast<const __half *>(base) + at + i * step, false, v[i]);
+            else
+                load8<DT_BF16>(reinterpret_cast<const __nv_bfloat16 *>(base) + at + i * step, false, v[i]);
+        }
+    }
+}
+
 // (step, low) of a group with extremes mn, mx (`bad`: it holds a NaN or an infinity, and then stands for NaN
 // throughout). low is the smallest value and step a fifteenth of the span above it, each rounded to f16 (values beyond
 // f16's range are held at its largest): f16 keeps a group's overhead at 4 bytes and 11 bits of a 4-bit step.

@@ -153,17 +153,11 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
         float x[NU][8] = {}, mx = 0.f;
         if (r < rows) {
             const long long at = (long long)(sr.first + i) * a.q_row + (long long)hq * a.q_head + 8 * t;
+            load_runs<NU>(dtype, a.q, at, 32, wide, x);
 #pragma unroll
-            for (int u = 0; u < NU; u++) {
-                if (dtype == DT_F32)
-                    load8<DT_F32>(reinterpret_cast<const float *>(a.q) + at + 32 * u, wide, x[u]);
-                else if (dtype == DT_F16)
-                    load8<DT_F16>(reinterpret_cast<const __half *>(a.q) + at + 32 * u, wide, x[u]);
-                else
-                    load8<DT_BF16>(reinterpret_cast<const __nv_bfloat16 *>(a.q) + at + 32 * u, wide, x[u]);
+            for (int u = 0; u < NU; u++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(x[u][j]));
-            }
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));

@@ -97,22 +97,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
     // score in units of log2.
     auto put_q = [&](const KaRows &sr, int ri, int hq) {
                         constexpr int H = HD / 2;
-                        float q[H], mx = 0.f;
+                        float q[H / 8][8], mx = 0.f;
                         const int es = dtype == DT_F32 ? 4 : 2;
                         const bool wide = !(((uintptr_t)a.q & 15) || ((a.q_row | a.q_head) * es) % 16);
                         const long long from = (long long)(sr.first + ri) * a.q_row + (long long)hq * a.q_head + wg * H;
-        #pragma unroll
-                        for (int b = 0; b < H / 8; b++) {
-                            float v[8];
-                            if (dtype == DT_F32)
-                                load8<DT_F32>(reinterpret_cast<const float *>(a.q) + from + 8 * b, wide, v);
-                            else if (dtype == DT_F16)
-                                load8<DT_F16>(reinterpret_cast<const __half *>(a.q) + from + 8 * b, wide, v);
-                            else
-                                load8<DT_BF16>(reinterpret_cast<const __nv_bfloat16 *>(a.q) + from + 8 * b, wide, v);
-        #pragma unroll
-                            for (int x = 0; x < 8; x++) q[8 * b + x] = v[x], mx = fmaxf(mx, fabsf(v[x]));
-                        }
+                                load_runs<H / 8>(dtype, a.q, from, 8, wide, q);
+#pragma unroll
+                        for (int b = 0; b < H / 8; b++)
+#pragma unroll
+                            for (int x = 0; x < 8; x++) mx = fmaxf(mx, fabsf(q[b][x]));
                         kt_bar(2, 256);  // the last piece's epilogue is done with the exchange
                         qmax[wg][row] = mx;
                         kt_bar(2, 256);
@@ -127,7 +120,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                         for (int b = 0; b < H / 8; b++)
         #pragma unroll
                             for (int x = 0; x < 4; x++)
-                                split_pair(q[8 * b + x] * up, q[8 * b + x + 4] * up, hi[4 * b + x], lo[4 * b + x]);
+                                split_pair(q[b][x] * up, q[b][x + 4] * up, hi[4 * b + x], lo[4 * b + x]);
                         const uint32_t tq = tmem + lane_base + KT_TQ + wg * (H / 2);
                         if constexpr (H / 2 == 32) {
                             tmem_st32u(tq, hi);

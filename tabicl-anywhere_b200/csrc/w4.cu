@@ -453,6 +453,13 @@ static int w4_clusters(int cs, int sms) {
     return n;
 }
 
+static size_t w4_smem_bytes(const W4Plan &p, int group, int qs) {
+    const int ng = 128 / group, r = 8 * p.nt;
+    return (size_t)W4_WARPS * W4_DEPTH * (2048 + 32 * ng * 4) + (size_t)p.pass * w4_frag_words(p.nt, qs) * 4 +
+           sizeof(float) * (p.pass * ng * r + r + (((size_t)p.tiles * r * 16) << p.parts));
+}
+
+// (the largest of these shared-memory sizes is 216,320 bytes: 32-wide groups, 7 blocks of 64 rows, 64 units of outputs)
 static W4Plan w4_plan(int dtype, const W4Args &a, int sms) {
     W4Plan p;
     const int qs = dtype == DT_F32 ? 2 : 1, blocks = (a.k + 127) / 128, tiles = (a.n + 15) / 16;
@@ -462,16 +469,22 @@ static W4Plan w4_plan(int dtype, const W4Args &a, int sms) {
     p.cs = 1;
     while (p.cs < 8 && (blocks > W4_SLICE * p.cs || (blocks >= 16 * p.cs && tiles * p.cs * 2 <= sms))) p.cs *= 2;
     p.slice = (blocks + p.cs - 1) / p.cs;
-    p.pass = std::min({p.slice, W4_SLICE, std::max(1, W4_X_BYTES / (4 * w4_frag_words(p.nt, qs)))});
-    p.groups = std::min(tiles, std::max(1, w4_clusters(p.cs, sms) / p.row_tiles));
-    p.tiles = std::min((tiles + p.groups - 1) / p.groups, W4_Y_UNITS / p.nt);
-    p.groups = std::min(p.groups, (tiles + p.tiles - 1) / p.tiles);
-    // a power of two of parts of a slice where the warps share the tiles more evenly by it: a warp that streams a whole slice
-    // of its rows reads memory in longer runs (14336 x 8192: 25.4 us with one part of 16 steps, 27.2 us with four of 14)
-    p.parts = 0;
-    for (int h = 1; h <= 3 && 2 << h <= p.pass + 1 && p.tiles << h <= W4_Y_UNITS / p.nt; h++) {
-        auto cost = [&](int x) { return (((p.tiles << x) + W4_WARPS - 1) / W4_WARPS) * (((p.pass + 1) / 2 + (1 << x) - 1) >> x); };
-        if (cost(h) * 8 < cost(p.parts) * 7) p.parts = h;
+    for (int resident = 2; resident >= 1; resident--) {  // blocks an SM: one may hold more of x at once
+        const int most = std::min(W4_SLICE, std::max(1, (resident == 1 ? W4_X_BYTES * 7 / 4 : W4_X_BYTES) / (4 * w4_frag_words(p.nt, qs))));
+        const int passes = (p.slice + most - 1) / most;
+        p.pass = (p.slice + passes - 1) / passes;
+        p.groups = std::min(tiles, std::max(1, w4_clusters(p.cs, sms) * resident / 2 / p.row_tiles));
+        p.tiles = std::min((tiles + p.groups - 1) / p.groups, W4_Y_UNITS / p.nt);
+        p.groups = std::min(p.groups, (tiles + p.tiles - 1) / p.tiles);
+        // a power of two of parts of a slice where the warps share the tiles more evenly by it: a warp that streams a whole
+        // slice of its rows reads memory in longer runs (14336 x 8192: 25.4 us with one part of 16 steps, 27.2 us with four
+        // of 14)
+        p.parts = 0;
+        for (int h = 1; h <= 3 && 2 << h <= p.pass + 1 && p.tiles << h <= W4_Y_UNITS / p.nt; h++) {
+            auto cost = [&](int x) { return (((p.tiles << x) + W4_WARPS - 1) / W4_WARPS) * (((p.pass + 1) / 2 + (1 << x) - 1) >> x); };
+            if (cost(h) * 8 < cost(p.parts) * 7) p.parts = h;
+        }
+        if (w4_smem_bytes(p, a.group, qs) <= 113 * 1024 && passes == 1) break;
     }
     return p;
 }
@@ -487,8 +500,7 @@ size_t w4_linear_workspace(int dtype, const W4Args &a, int sms) {
 
 template <int G, int NT, int QS>
 static cudaError_t launch_w4(int dtype, const W4Args &a, const W4Plan &p, void *work, cudaStream_t s, uint64_t *launches) {
-    const size_t smem = (size_t)W4_WARPS * W4_DEPTH * W4Ring<G>::BYTES + (size_t)p.pass * w4_frag_words(NT, QS) * 4 +
-                        sizeof(float) * (p.pass * (128 / G) * 8 * NT + 8 * NT + ((p.tiles * 8 * NT * 16) << p.parts));
+    const size_t smem = w4_smem_bytes(p, G, QS);
     cudaError_t e = allow_dynamic_smem((const void *)k_w4_linear<G, NT, QS>, smem);
     if (e != cudaSuccess) return e;
     uint32_t *xf = reinterpret_cast<uint32_t *>(work);
