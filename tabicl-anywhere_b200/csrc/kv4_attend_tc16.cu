@@ -400,24 +400,27 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 fence_after_sync();
                 const float c1 = rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_T);
                 const int e = *reinterpret_cast<volatile int *>(&teV[x8]);
-                float s[64];
+                const bool edge = key0 < lo_max || key0 + BK > hi_min;
+                // Two passes over the step's scores in tensor memory, 32 at a time in loops that are not unrolled further: the code
+                // of a step is then short enough for the instruction caches, which the two kinds of warpgroups share.
+                float mx;
                 {
-                    float x[32], y[32];
-                    tmem_ld32(tsp, x);
-                    tmem_ld32(tsp + 32, y);
-                    tmem_wait_ld();
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int b = 0; b < 2; b++) {
+                        float x[32];
+                        tmem_ld32(tsp + 32 * b, x);
+                        tmem_wait_ld32(x);
+                        if (edge) {
 #pragma unroll
-                    for (int k = 0; k < 32; k++) s[k] = x[k], s[32 + k] = y[k];
+                            for (int k = 0; k < 32; k++)
+                                if (key0 + 32 * b + k < my_lo || key0 + 32 * b + k >= my_hi) x[k] = -INFINITY;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; k++) top[k & 3] = fmaxf(top[k & 3], x[k]);
+                    }
+                    mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c1;
                 }
-                if (key0 < lo_max || key0 + BK > hi_min) {
-#pragma unroll
-                    for (int k = 0; k < 64; k++)
-                        if (key0 + k < my_lo || key0 + k >= my_hi) s[k] = -INFINITY;
-                }
-                float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int k = 4; k < 64; k++) top[k & 3] = fmaxf(top[k & 3], s[k]);
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c1;
                 if (i == 0) unit = e;
                 if (__any_sync(0xffffffffu, mx > m + 8.f) || e > unit) {
                     const float mnew = fmaxf(m, mx), f = m == -INFINITY ? 0.f : kt_ex2(m - mnew);
@@ -430,7 +433,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                         for (int b = 0; b < HD / 32; b++) {
                             float x[32];
                             tmem_ld32(tmem + lane_base + KU_TO + q * HD + 32 * b, x);
-                            tmem_wait_ld();
+                            tmem_wait_ld32(x);
 #pragma unroll
                             for (int k = 0; k < 32; k++) x[k] *= fo;
                             tmem_st32(tmem + lane_base + KU_TO + q * HD + 32 * b, x);
@@ -441,19 +444,31 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 }
                 // weights times 2^7 (up to 2^15), in units of the step's values
                 const float mm = (m == -INFINITY ? 0.f : m) - 7.f - (float)(e - unit);
-                float sum[4] = {};
-                uint32_t h[32];
+                float part_sum[4] = {};
+#pragma unroll 1
+                for (int b = 0; b < 2; b++) {
+                    float x[32];
+                    tmem_ld32(tsp + 32 * b, x);
+                    tmem_wait_ld32(x);
+                    if (edge) {
 #pragma unroll
-                for (int k = 0; k < 32; k++) {
-                    const float p0 = kt_ex2(fmaf(s[2 * k], c1, -mm)), p1 = kt_ex2(fmaf(s[2 * k + 1], c1, -mm));
-                    sum[(2 * k) & 3] += p0, sum[(2 * k + 1) & 3] += p1;
-                    h[k] = kt_u32(__floats2half2_rn(p0, p1));
+                        for (int k = 0; k < 32; k++)
+                            if (key0 + 32 * b + k < my_lo || key0 + 32 * b + k >= my_hi) x[k] = -INFINITY;
+                    }
+                    uint32_t h[16];
+#pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const float p0 = kt_ex2(fmaf(x[2 * k], c1, -mm)), p1 = kt_ex2(fmaf(x[2 * k + 1], c1, -mm));
+                        part_sum[(2 * k) & 3] += p0, part_sum[(2 * k + 1) & 3] += p1;
+                        h[k] = kt_u32(__floats2half2_rn(p0, p1));
+                    }
+                    tmem_st16u(tsp + 16 * b, h);  // over scores that have been read
                 }
-                tmem_st32u(tsp, h);
+                const float sum = (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
                 tmem_wait_st();
                 fence_before_sync();
                 mbar_arrive(&mP[q][c & 1]);
-                l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), kt_pow2(unit - e), l);
+                l = fmaf(sum, kt_pow2(unit - e), l);
                 if (*reinterpret_cast<volatile int *>(&has_nan[x8])) {
                     for (int k = 0; k < NG; k++)
                         for (int b = 0; b < 64; b++)
@@ -520,7 +535,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
             for (int b = 0; b < HD / 32; b++) {
                 float o[32];
                 tmem_ld32(to_o + 32 * b, o);
-                tmem_wait_ld();
+                tmem_wait_ld32(o);
                 if (nans >> (32 * b / G) & 1) {
 #pragma unroll
                     for (int k = 0; k < 32; k++) o[k] = NAN;
