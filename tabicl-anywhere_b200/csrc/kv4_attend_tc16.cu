@@ -217,10 +217,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 wait_warp(&mRaw[rs], (uint32_t)(i / NR) & 1u);
                 const uint8_t *kraw = raw + rs * C::RAW, *vraw = kraw + C::KC + C::SC;
                 const bool seen = j >= sp.lo_min && j < sp.hi_max;
-                // the codes of this thread's halves and the scales of its key, all asked for at once
-                uint32_t kw[2 * NU], vw[2 * NU], kc[NG], vc[NG];
-                lds_words<2 * NU>(kraw + key * (HD / 2) + half * NU * 8, kw);
-                lds_words<2 * NU>(vraw + key * (HD / 2) + half * NU * 8, vw);
+                uint32_t kc[NG], vc[NG];  // the key's scales
                 lds_words<NG>(kraw + C::KC + key * NG * 4, kc);
                 lds_words<NG>(vraw + C::KC + key * NG * 4, vc);
                 // the step's power of two, for keys and values: from each group's ends
@@ -250,7 +247,6 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 mx[0] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[0])));  // (not negative: ordered as their bits)
                 mx[1] = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx[1])));
                 if (lane == 0) red[turn][i >> 1 & 1][0][w4] = mx[0], red[turn][i >> 1 & 1][1][w4] = nan ? -mx[1] - 1.f : mx[1];  // a NaN shows as the sign
-                mbar_arrive(&mRawFree[rs]);
                 kt_bar(1 + turn, 128);
                 int e[2];
                 bool any = false;
@@ -265,41 +261,44 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     e[x] = m > 0.f ? min(40, (int)(__float_as_uint(m) >> 23) - 125) : 0;  // m < 2^(e - 1): a span, 15 steps, below 2^e
                 }
                 if (tid % 128 == 0) teK[i & 7] = e[0], teV[i & 7] = e[1], has_nan[i & 7] = any;
-                if (i >= NS) wait_warp(&mKfree[sl], ph ^ 1u);
+                KtScale<false> ks[NG], vs[NG];
 #pragma unroll
                 for (int k = 0; k < NG; k++) {
-                    KtScale<false> s;
-                    const float2 f = __half22float2(kt_h2(kc[k]));
-                    s.set(f.x, f.y, kt_pow2(KU_T - e[0]));
+                    const float2 f = __half22float2(kt_h2(kc[k])), g = __half22float2(kt_h2(vc[k]));
+                    ks[k].set(f.x, f.y, kt_pow2(KU_T - e[0])), vs[k].set(g.x, g.y, kt_pow2(KU_T - e[1]));
+                }
+                // (loops that are not unrolled over the halves: short code, see the softmax)
+                if (i >= NS) wait_warp(&mKfree[sl], ph ^ 1u);
+#pragma unroll 1
+                for (int x = 2 * half; x < 2 * half + 2; x++) {
+                    uint32_t w[NU];
+                    lds_words<NU>(kraw + key * (HD / 2) + x * NU * 4, w);
+                    __half *to = Kring + sl * BLOCK + kmajor_off(key, 8 * x, BK);
 #pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int u = k * UG; u < (k + 1) * UG; u++)
-                            kt_widen(kw[x * NU + u], s, Kring + sl * BLOCK + kmajor_off(key, 32 * u + 8 * (2 * half + x), BK), nullptr);
+                    for (int u = 0; u < NU; u++) kt_widen(w[u], ks[u / UG], to + kmajor_off(0, 32, BK) * u, nullptr);
                 }
                 fence_async_smem();
                 mbar_arrive(&mK[sl]);
                 if (i >= NS) wait_warp(&mVfree[sl], ph ^ 1u);
+#pragma unroll 1
+                for (int x = 2 * half; x < 2 * half + 2; x++) {
+                    uint32_t w[NU];
+                    lds_words<NU>(vraw + key * (HD / 2) + x * NU * 4, w);
+                    __half *to = Vring + sl * BLOCK + mnmajor_off(8 * x, key, HD);
 #pragma unroll
-                for (int k = 0; k < NG; k++) {
-                    KtScale<false> s;
-                    const float2 f = __half22float2(kt_h2(vc[k]));
-                    s.set(f.x, f.y, kt_pow2(KU_T - e[1]));
-#pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int u = k * UG; u < (k + 1) * UG; u++) {
-                            // half-words g = 2 q and 2 q + 1 of a unit: coordinates 32 u + 8 q + (0..7)
-                            uint32_t c;
-                            if constexpr (NU == 1)
-                                c = vw[x];
-                            else
-                                c = __byte_perm(vw[x * NU + u / 2], vw[x * NU + NU / 2 + u / 2], u & 1 ? 0x7632 : 0x5410);
-                            kt_widen(c, s, Vring + sl * BLOCK + mnmajor_off(32 * u + 8 * (2 * half + x), key, HD), nullptr);
-                        }
+                    for (int u = 0; u < NU; u++) {
+                        // half-words g = 2 x and 2 x + 1 of a unit: coordinates 32 u + 8 x + (0..7)
+                        uint32_t c;
+                        if constexpr (NU == 1)
+                            c = w[0];
+                        else
+                            c = __byte_perm(w[u / 2], w[NU / 2 + u / 2], u & 1 ? 0x7632 : 0x5410);
+                        kt_widen(c, vs[u / UG], to + mnmajor_off(32, 0, HD) * u, nullptr);
+                    }
                 }
                 fence_async_smem();
                 mbar_arrive(&mV[sl]);
+                mbar_arrive(&mRawFree[rs]);
             }
             at += n;
             Cut::next(pl, a, each, sr.n, n);
