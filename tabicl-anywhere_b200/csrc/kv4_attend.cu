@@ -638,11 +638,17 @@ static int ka_nt(int dtype, const Kv4AttendArgs &a) {
     return a.max_rows * (a.q_heads / a.c.heads) > 8 && a.c.width * (dtype == DT_F32 ? 2 : 1) <= 128 ? 2 : 1;
 }
 
-// Many rows: tiles of 128 rows on the tensor cores.
-static bool ka_many(const Kv4AttendArgs &a) { return a.c.width <= 128 && a.max_rows * (a.q_heads / a.c.heads) > 32; }
+// Many rows go to the tensor cores' kernels, whose tiles hold 128 or 256 rows: from 41 rows a cache head on (32 sequences of
+// 4096 bf16 keys, 8 heads: 32 rows 164 us here and 176 us there, 48 rows 223 and 179), where their units are many or long
+// enough. Units that are fewer than a quarter of the SMs are cut into parts, whose joining costs more there: 512 rows over
+// 2048 keys of 8 heads take 63 us here and 94 us there, 1024 rows 98 and 94; 512 over 8192 keys 140 and 152 (f32 214 and 117).
+static bool ka_many(const Kv4AttendArgs &a, int sms) {
+    const long long rows = (long long)a.max_rows * (a.q_heads / a.c.heads), heads = (long long)a.seqs * a.c.heads;
+    return a.c.width <= 128 && rows > 40 && (heads * ((rows + 255) / 256) * 4 >= sms || heads * rows * a.max_len >= 16000000LL);
+}
 
 size_t kv4_attend_workspace(int dtype, const Kv4AttendArgs &a, int sms) {
-    if (ka_many(a)) return dtype == DT_F32 ? kv4_attend_tc_workspace(a, sms) : kv4_attend_tc16_workspace(a, sms);
+    if (ka_many(a, sms)) return dtype == DT_F32 ? kv4_attend_tc_workspace(a, sms) : kv4_attend_tc16_workspace(a, sms);
     return 4 * (KA_BLOCKS + (size_t)std::min(KA_BLOCKS, 8 * sms) * 2 * 8 * ka_nt(dtype, a) * (a.c.width + 2));
 }
 
@@ -685,7 +691,7 @@ cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *
     if (!a.seqs || !a.rows || !a.max_rows) return cudaSuccess;
     if (kv4_attend_workspace(dtype, a, sms) > work_bytes) return cudaErrorInvalidValue;
     if (launches) ++*launches;
-    if (ka_many(a)) return dtype == DT_F32 ? launch_kv4_attend_tc(a, sms, work, s) : launch_kv4_attend_tc16(dtype, a, sms, work, s);
+    if (ka_many(a, sms)) return dtype == DT_F32 ? launch_kv4_attend_tc(a, sms, work, s) : launch_kv4_attend_tc16(dtype, a, sms, work, s);
     const int nt = ka_nt(dtype, a);
     cudaError_t e = cudaErrorInvalidValue;
     const int w = a.c.width, g = a.c.group;

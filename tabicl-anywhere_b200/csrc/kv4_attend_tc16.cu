@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
     const int each = a.q_heads / a.c.heads;
-    auto pl = Cut::template place<KU_THREADS>(a, each, 1, s_sum, s_unit);
+    auto pl = Cut::template place<KU_THREADS>(a, each, KA_TC_STEPS, s_sum, s_unit);
     if (pl.pos >= pl.end) return;
     if (warp == 0) {
         tmem_alloc(&tslot, 512);

@@ -591,3 +591,88 @@ def test_the_example_runs_the_operators_together(test_rows):
         x = x + linear(linear(norm(x, b["n2"]), b["w1"], True), b["w2"])
     want = linear(linear(norm(x, member.ln), member.dec0, True), member.dec2)
     assert float((scores.double() - want).abs().max()) <= 5e-5
+
+
+# ---- many rows: shapes that reach the tensor cores' kernels (more than 40 rows a cache head, in many units or long ones) ----
+
+def check_many(c, dtype, q, n, scale, causal, window, out, lse):
+    """As Cached.check, every sequence with n rows, on the device in 64 bits."""
+    for s, length in enumerate(c.lens):
+        rows = slice(s * n, (s + 1) * n)
+        got, gl = out[rows].double(), lse[rows].double()
+        if not length:
+            assert not got.any() and bool((gl == -np.inf).all())
+            continue
+        k, v = (torch.from_numpy(x).cuda().transpose(0, 1) for x in (c.k[s], c.v[s]))
+        each = q.shape[1] // c.heads
+        x = torch.from_numpy(q[rows].astype(np.float64)).cuda().transpose(0, 1)
+        i, j = torch.arange(n, device="cuda")[:, None], torch.arange(length, device="cuda")[None]
+        seen = torch.ones(n, length, dtype=torch.bool, device="cuda")
+        if causal:
+            seen &= j <= length - n + i
+        if window:
+            seen &= j > length - n + i - window
+        u = 2.0**-11 if dtype != "f32" else 2.0**-20
+        for h in range(q.shape[1]):
+            kk, vv = k[h // each], v[h // each]
+            sc = (x[h] @ kk.T * scale).masked_fill(~seen, -np.inf)
+            want_lse = torch.logsumexp(sc, -1)
+            some = want_lse > -np.inf
+            p = torch.exp(sc - torch.where(some, want_lse, torch.zeros_like(want_lse))[:, None])
+            want = torch.where(some[:, None], p @ torch.nan_to_num(vv), torch.zeros_like(x[h]))
+            reach = (x[h].abs() @ kk.abs().T * abs(scale)).masked_fill(~seen, 0).amax(-1)
+            score = (u + 2.0**-20) * reach
+            tol = torch.nan_to_num(vv).abs().max() * (torch.expm1(2 * score) + 3 * u)[:, None] + 2 * ULP[dtype] * want.abs() + 1e-7
+            bad = torch.isnan(vv)  # a value that is NaN reaches the rows that see it, and no others
+            nan = (seen.double() @ bad.double()) > 0
+            assert torch.equal(torch.isnan(got[:, h]), nan)
+            assert bool(((got[:, h] - want).abs() <= tol)[~nan].all()), (s, h)
+            assert bool((gl[:, h][~some] == -np.inf).all())
+            assert bool(((gl[:, h] - want_lse).abs() <= score + 2.0**-20 * (1 + want_lse.abs()))[some].all())
+
+
+MANY = [
+    # width, group, page, heads, q_heads, rows, lens, causal, window
+    (64, 32, 16, 1, 2, 30, [0, 1, 29, 30, 31, 63, 64, 65, 127, 200] * 4, True, 0),
+    (128, 64, 64, 5, 5, 43, [300, 43, 1, 77, 512, 64, 200, 129], True, 50),
+    (32, 32, 32, 8, 24, 17, [100, 16, 17, 18, 130], False, 0),
+    (64, 64, 256, 8, 8, 1030, [2050], True, 0),
+    (128, 128, 128, 4, 8, 1100, [4000], False, 0),
+    (128, 32, 64, 8, 8, 300, [7100], True, 1000),
+    (32, 32, 16, 10, 10, 257, [700, 513, 0, 256], True, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("width,group,page,heads,q_heads,rows,lens,causal,window", MANY)
+def test_attend_many_rows(gpu, dtype, width, group, page, heads, q_heads, rows, lens, causal, window):
+    c = Cached(gpu, rows, lens, heads, width, page, group)
+    counts = [rows] * len(lens)
+    q = rounded(np.random.default_rng(7).normal(0, 1, (sum(counts), q_heads, width)), DT[dtype][1])
+    scale = -1 / np.sqrt(width) if rows == 43 else 1 / np.sqrt(width)
+    first, _ = c.attend(dtype, q, counts, scale, causal, window)
+    out, lse = c.attend(dtype, q, counts, scale, causal, window)
+    sync(gpu)
+    assert torch.equal(first, out)
+    check_many(c, dtype, q, rows, scale, causal, window, out, lse)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,seqs", [(5, 1), (60, 40)])
+def test_attend_a_nan_reaches_only_the_rows_that_see_it(gpu, dtype, rows, seqs):
+    """Groups of values that stand for NaN, at tokens that some rows of a step see and others do not."""
+    page, group, width = 32, 32, 64
+    c = Cached(gpu, 21, [200] * seqs, 1, width, page, group)
+    raw = c.pool.cpu().numpy().reshape(c.pages, -1)
+    low = page * width // 2 * 2 + page * 4 * 2  # value (step, low) behind key codes, key scales and value codes
+    table = c.table.cpu().numpy()
+    for s in range(seqs):
+        for token, g in ((200 - rows // 2, 1), (199, 0)):
+            p, at = table[s, token // page], low + (token % page) * 8 + g * 4
+            raw[p, at:at + 4] = np.array([0.0, np.nan], np.float16).view(np.uint8)
+            c.v[s][token, 0, g * group:(g + 1) * group] = np.nan
+    c.pool.copy_(dev(raw))
+    q = rounded(np.random.default_rng(7).normal(0, 1, (rows * seqs, 2, width)), DT[dtype][1])
+    out, lse = c.attend(dtype, q, [rows] * seqs, 0.125, causal=True)
+    sync(gpu)
+    check_many(c, dtype, q, rows, 0.125, True, 0, out, lse)
