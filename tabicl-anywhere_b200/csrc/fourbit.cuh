@@ -237,6 +237,19 @@ __device__ __forceinline__ uint32_t pack8(const float (&x)[8], float step, float
 __device__ __forceinline__ float value_of(uint32_t w, int j, float step, float low) {
     return __fadd_rn(__fmul_rn((float)((w >> (4 * j)) & 15u), step), low);
 }
+// Two codes of a word as f16 operands of a product: the first (SECOND false) or second nibbles of its even bytes. As they
+// are, subnormals: code * 2^-24, code * 2^-20, one AND. CENTRED: code - 8, 16 (code - 8), with the AND's result in the low
+// bits of 1024 and one subtraction, exact. The products' f32 sums are not rounded to nearest by the matrix unit, and with
+// codes of one sign they are large beside what is left when the groups' lows are added, so for f32 and f16 results the
+// codes are centred and the lows taken as low + 8 step.
+template <bool CENTRED, bool SECOND>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+    const uint32_t c = w & (SECOND ? 0x00f000f0u : 0x000f000fu);
+    if constexpr (!CENTRED) return c;
+    const uint32_t v = c | 0x64006400u, m = SECOND ? 0x64806480u : 0x64086408u;
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&m));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
 __device__ __forceinline__ bool finite_f(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 #endif

@@ -5,6 +5,11 @@
 // the weights, and the group scales act on its f32 result:
 //     q . k_j   = sum over groups of  step * (q_g . codes)  +  low * (sum of q_g)
 //     sum p_j v = sum over groups of  (p_j step) . codes    +  sum p_j low
+// What bounds it: issue. Taking a code out of its word is one logic instruction for two, and a step of 32 keys with 8 query
+// rows some 600 instructions a warp, at 0.55 a cycle and scheduler with the 12 warps that the registers of q, the output
+// and the sums leave an SM. 64 bf16 rows (32 heads of 128 on 8, groups of 32) over 0..16384 cached tokens: 0.19 ms, 3.8 TB/s
+// of codes and scales, 57% of a copy's rate; with 16 warps and spills 0.225 ms.
+//
 // Per 32 keys a warp computes S^T = K Q^T with 16 keys as rows and 8 query rows as columns, so a key's codes are read in
 // the order they are stored in, and O^T = V^T P'^T with P' = p * step turned round in registers (movmatrix).
 #include <algorithm>
@@ -65,12 +70,15 @@ __device__ __forceinline__ float exp2_sfu(float x) {  // relative error 2^-22; 0
 }
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| < 127
 
-// SPLIT: q and the weights as two f16 (f32 queries), else as one.
-template <int HD, int G, int NT, bool SPLIT>
-__global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 : 1)
+// TYPE: the queries' type. f32: q and the weights as two f16, else as one; bf16: codes as they are, and the weights' products
+// with their steps in f16 pairs, each rounded to the 11 bits that 8-bit results do not show.
+template <int HD, int G, int NT, int TYPE>
+__global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F32) ? 3 : 1)
     k_kv4_attend(Kv4AttendArgs a, int dtype, int min_steps, float *part, int *arrived) {
     using C = KaTile<HD, G>;
-    constexpr int NU = C::NU, NG = C::NG, UG = G / 32, R = 8 * NT, ST = C::STAGES, QS = SPLIT ? 2 : 1;
+    constexpr int NU = C::NU, NG = C::NG, UG = G / 32, R = 8 * NT, ST = C::STAGES, QS = TYPE == DT_F32 ? 2 : 1;
+    constexpr bool SPLIT = TYPE == DT_F32, CENTRED = TYPE != DT_BF16, LOW_MMA = C::LOW_MMA && !CENTRED;
+    constexpr float UNIT = CENTRED ? 1.f : 16777216.f;  // undoes the codes' 2^-24
     extern __shared__ __align__(16) uint8_t sm[];
     __shared__ int s_last, s_unit[4];
     __shared__ long long s_sum[KA_WARPS];
@@ -142,7 +150,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
     // a word's second nibbles by 1/16 more
     uint32_t qf[QS][NT][NU][4];
     float fq[NT][2];                                // for this thread's columns 2 t, 2 t + 1: the factor of a score
-    float qs[NT][C::LOW_MMA ? 1 : NG][2];           // and the groups' sums,
+    float qs[NT][LOW_MMA ? 1 : NG][2];           // and the groups' sums,
     uint32_t qlow[NT][2];                           // or their fragments: hi and lo of the sums times 2^-6
     int hi[NT][2], lo[NT][2];
     const int es = dtype == DT_F32 ? 4 : 2;
@@ -183,14 +191,14 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
             }
         }
         // (a scale of 0 as 2^-100, so that the factor is positive: the scores' order is that of the products)
-        const float factor = fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * pow2i(-e) * 16777216.f;
+        const float factor = fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * pow2i(-e) * UNIT;
 #pragma unroll
         for (int k = 0; k < NG; k++) {
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
-            sum[k] *= C::LOW_MMA ? 0.015625f : 5.9604644775390625e-8f;  // 2^-24: as the products with the codes come
+            sum[k] *= LOW_MMA ? 0.015625f : 1.f / UNIT;  // as the products with the codes come
         }
-        if constexpr (C::LOW_MMA) {
+        if constexpr (LOW_MMA) {
             uint32_t hi2[NG / 2], lo2[NG / 2];
 #pragma unroll
             for (int k = 0; k < NG; k += 2) {
@@ -209,7 +217,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
         for (int c = 0; c < 2; c++) {
             const int who = (2 * t + c) * 4;
             fq[nt][c] = __shfl_sync(0xffffffffu, factor, who);
-            if constexpr (!C::LOW_MMA) {
+            if constexpr (!LOW_MMA) {
 #pragma unroll
                 for (int k = 0; k < NG; k++) qs[nt][k][c] = __shfl_sync(0xffffffffu, sum[k], who);
             }
@@ -220,12 +228,12 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
 
     // the running state of a column, in units of 2^off: off = m - 7 + ve, m the column's reference (it moves only when a score
     // passes it by 8), 2^ve the largest value step so far or more. So a weight is at most 2^(15 - ve), and with its step at
-    // most 2^15: inside f16, and 2^7 above where the largest would leave small ones the least room. A 16-bit type's weights
-    // are f16 before they meet their step too, so there ve stays at 0 or above; f32's are not.
+    // most 2^15: inside f16, and 2^7 above where the largest would leave small ones the least room. bf16's weights are
+    // f16 before they meet their step too, so there ve stays at 0 or above.
     float m[NT][2], off_m[NT][2], bound[NT][2], l[NT][2], ls[NT][NG][2], o[NT][NU][2][4];
     float ol[NT][4] = {};  // sums of p low of group g, where they are taken as a matrix product
-    constexpr bool LOW_MMA_V = C::LOW_MMA && !SPLIT;
-    int ve = SPLIT ? -24 : 0;  // (steps are f16: at least 2^-24)
+    constexpr bool LOW_MMA_V = LOW_MMA;
+    int ve = CENTRED ? -24 : 0;  // (steps are f16: at least 2^-24)
     float vtop = pow2i(ve);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -266,7 +274,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
                 lds_words<NG>(tile + C::KC + key * NG * 4, sc[h]);
             }
             float low[NT][4];
-            if constexpr (C::LOW_MMA) {
+            if constexpr (LOW_MMA) {
                 uint32_t lows[2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -290,20 +298,22 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const uint32_t w0 = h ? kw[0][u] >> 8 : kw[0][u], w1 = h ? kw[1][u] >> 8 : kw[1][u];
-                        const uint32_t a0 = w0 & 0x000f000fu, a1 = w1 & 0x000f000fu, a2 = w0 & 0x00f000f0u, a3 = w1 & 0x00f000f0u;
+                        const uint32_t a0 = code_pair<CENTRED, false>(w0), a1 = code_pair<CENTRED, false>(w1);
+                        const uint32_t a2 = code_pair<CENTRED, true>(w0), a3 = code_pair<CENTRED, true>(w1);
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                             for (int q = QS - 1; q >= 0; q--)
                                 mma16816(acc[nt], a0, a1, a2, a3, qf[q][nt][u][2 * h], qf[q][nt][u][2 * h + 1]);
                     }
-                const float2 s0 = bits_float2(sc[0][k]), s1 = bits_float2(sc[1][k]);
+                float2 s0 = bits_float2(sc[0][k]), s1 = bits_float2(sc[1][k]);
+                if (CENTRED) s0.y = fmaf(8.f, s0.x, s0.y), s1.y = fmaf(8.f, s1.x, s1.y);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         float &x = s[kb][nt][c], &y = s[kb][nt][c + 2];
-                        if constexpr (C::LOW_MMA) {
+                        if constexpr (LOW_MMA) {
                             x = k ? fmaf(s0.x, acc[nt][c], x) : s0.x * acc[nt][c];
                             y = k ? fmaf(s1.x, acc[nt][c + 2], y) : s1.x * acc[nt][c + 2];
                         } else {
@@ -318,7 +328,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     // the lows' products are 2^18 times the codes'
-                    if constexpr (C::LOW_MMA) s[kb][nt][c] = fmaf(low[nt][c], 3.814697265625e-6f, s[kb][nt][c]);
+                    if constexpr (LOW_MMA) s[kb][nt][c] = fmaf(low[nt][c], 3.814697265625e-6f, s[kb][nt][c]);
                 }
         }
         // the value scales of this thread's four keys
@@ -406,7 +416,8 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
             for (int kb = 0; kb < 2; kb++)
 #pragma unroll
             for (int k = 0; k < NG; k++) {
-                const float y0 = bits_float2(vs[kb][0][k]).y, y1 = bits_float2(vs[kb][1][k]).y;
+                const float2 v0 = bits_float2(vs[kb][0][k]), v1 = bits_float2(vs[kb][1][k]);
+                const float y0 = CENTRED ? fmaf(8.f, v0.x, v0.y) : v0.y, y1 = CENTRED ? fmaf(8.f, v1.x, v1.y) : v1.y;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -437,7 +448,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
                 }
             }
             __half2 p2[NT][2];
-            if (!SPLIT) {
+            if (!CENTRED) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -458,7 +469,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
 #pragma unroll
             for (int k = 0; k < NG; k++) {
                 uint32_t b[QS][NT][2];
-                if constexpr (SPLIT) {
+                if constexpr (CENTRED) {
                     const float w[2] = {bits_float2(vs[kb][0][k]).x, bits_float2(vs[kb][1][k]).x};
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
@@ -466,8 +477,11 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
                         for (int h = 0; h < 2; h++) {
                             const float p0 = s[kb][nt][2 * h] * w[h], p1 = s[kb][nt][2 * h + 1] * w[h];
                             const uint32_t x = half2_bits(p0, p1);
-                            const float2 f = bits_float2(x);
-                            b[0][nt][h] = transpose8(x), b[QS - 1][nt][h] = transpose8(half2_bits(p0 - f.x, p1 - f.y));
+                            b[0][nt][h] = transpose8(x);
+                            if constexpr (SPLIT) {
+                                const float2 f = bits_float2(x);
+                                b[QS - 1][nt][h] = transpose8(half2_bits(p0 - f.x, p1 - f.y));
+                            }
                         }
                 } else {
                     // p and p * step each round to 11 bits, as the results do to 11 or 8
@@ -486,7 +500,8 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         const uint32_t x = i ? pair[0][u] >> 8 : pair[0][u], y = i ? pair[1][u] >> 8 : pair[1][u];
-                        const uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+                        const uint32_t a0 = code_pair<CENTRED, false>(x), a1 = code_pair<CENTRED, true>(x);
+                        const uint32_t a2 = code_pair<CENTRED, false>(y), a3 = code_pair<CENTRED, true>(y);
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -503,7 +518,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && !SPLIT) ? 3 
     __syncthreads();
     float *so = reinterpret_cast<float *>(sm);  // [warp][R][HD]
     float *sms = so + KA_WARPS * R * HD;        // [warp][R]{m, l}
-    constexpr float unv = 16777216.f;  // 2^24
+    constexpr float unv = UNIT;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -652,10 +667,10 @@ size_t kv4_attend_workspace(int dtype, const Kv4AttendArgs &a, int sms) {
     return 4 * (KA_BLOCKS + (size_t)std::min(KA_BLOCKS, 8 * sms) * 2 * 8 * ka_nt(dtype, a) * (a.c.width + 2));
 }
 
-template <int HD, int G, int NT, bool SPLIT>
-static cudaError_t launch_one(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
+template <int HD, int G, int NT, int TYPE>
+static cudaError_t launch_one(const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
     using C = KaTile<HD, G>;
-    const auto kernel = k_kv4_attend<HD, G, NT, SPLIT>;
+    const auto kernel = k_kv4_attend<HD, G, NT, TYPE>;
     const size_t join = sizeof(float) * KA_WARPS * 8 * NT * (HD + 2);
     const size_t smem = std::max((size_t)KA_WARPS * C::STAGES * C::BYTES, join);
     cudaError_t e = allow_dynamic_smem((const void *)kernel, smem);
@@ -671,20 +686,21 @@ static cudaError_t launch_one(int dtype, const Kv4AttendArgs &a, int sms, void *
     const long long rows = (long long)a.max_rows * (a.q_heads / a.c.heads), tiles = (rows + 8 * NT - 1) / (8 * NT);
     const long long most = std::max(1LL, ((long long)a.max_len + KA_STEP + KA_KEYS - 1) / KA_STEP) * tiles * a.seqs * a.c.heads;
     const int grid = (int)std::min<long long>({most, (long long)resident * sms, KA_BLOCKS});
-    k_kv4_attend<HD, G, NT, SPLIT><<<grid, KA_STEP, smem, s>>>(a, dtype, 1, reinterpret_cast<float *>(work) + KA_BLOCKS,
+    k_kv4_attend<HD, G, NT, TYPE><<<grid, KA_STEP, smem, s>>>(a, TYPE, 1, reinterpret_cast<float *>(work) + KA_BLOCKS,
                                                                reinterpret_cast<int *>(work));
     return cudaGetLastError();
 }
+template <int HD, int G, int TYPE>
+static cudaError_t launch_type(const Kv4AttendArgs &a, int nt, int sms, void *work, cudaStream_t s) {
+    if constexpr (HD * (TYPE == DT_F32 ? 2 : 1) <= 128) {
+        if (nt == 2) return launch_one<HD, G, 2, TYPE>(a, sms, work, s);
+    }
+    return launch_one<HD, G, 1, TYPE>(a, sms, work, s);
+}
 template <int HD, int G>
 static cudaError_t launch_size(int dtype, const Kv4AttendArgs &a, int nt, int sms, void *work, cudaStream_t s) {
-    const bool split = dtype == DT_F32;
-    if constexpr (HD <= 64) {
-        if (nt == 2 && split) return launch_one<HD, G, 2, true>(dtype, a, sms, work, s);
-    }
-    if constexpr (HD <= 128) {
-        if (nt == 2) return launch_one<HD, G, 2, false>(dtype, a, sms, work, s);
-    }
-    return split ? launch_one<HD, G, 1, true>(dtype, a, sms, work, s) : launch_one<HD, G, 1, false>(dtype, a, sms, work, s);
+    if (dtype == DT_F32) return launch_type<HD, G, DT_F32>(a, nt, sms, work, s);
+    return dtype == DT_F16 ? launch_type<HD, G, DT_F16>(a, nt, sms, work, s) : launch_type<HD, G, DT_BF16>(a, nt, sms, work, s);
 }
 
 cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *work, size_t work_bytes, cudaStream_t s, uint64_t *launches) {

@@ -2,7 +2,9 @@
 //
 // With m the largest score and d = (x - m) / T:  S = sum e^d, log p(label) = d_label - log S,
 // entropy = log S - (sum e^d d) / S. A thread keeps (m, S, sum e^d d) of what it has seen and rescales them when a strip
-// of 32 of its scores holds a larger one, so scores are read once; the bound is memory (one ex2 a score comes next).
+// of 32 of its scores holds a larger one, so scores are read once; the bound is memory, one ex2 a score next. 4096 rows of
+// 131,071 bf16 scores with five alternatives: 0.194 ms (1.07 GB, 5.5 TB/s); 16 rows of 128,000 with twenty: 13 us, the
+// latency of two strips, the ranking and the cluster's join; 2048 rows of 10 classes: 3.9 us.
 //
 // Top alternatives: a strip's largest score is kept beside. The n-th largest of 32 disjoint parts' maxima is a bound that
 // at least n scores reach and hardly more than n do, so after the pass only the few strips that reach it are read again

@@ -61,14 +61,19 @@ cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k
 
 // y = act(x W^T + bias) + residual for a few rows of x: the weights stream from memory once, as codes, and go into the
 // matrix unit as they are. A nibble is a subnormal f16 (code * 2^-24, or 2^-20 from a byte's second nibble: one AND takes
-// two out of a word), so a product with the codes is exact in everything but x, which is one f16 for the 16-bit types and
-// the sum of two for f32; the group scales act on the f32 result:
+// two out of a word; f32 takes code - 8 instead, see code_pair), so a product with the codes is exact in everything but x,
+// which is one f16 for the 16-bit types and the sum of two for f32; the group scales act on the f32 result:
 //     sum over groups of  step * (x_g . codes)  +  low * (sum of x_g)
 //
 // A warp takes 16 outputs (the rows of the matrix fragments) over a part of K, its weights arriving in a ring of its own a
 // few blocks ahead; the rows of x are the 8 NT columns, as fragments in shared memory: up to 8 rows are laid out by every
 // block for itself, more by a kernel before. K is cut over the blocks of a cluster (each holds its own slice of x only)
 // and over `parts` of a block's warps; the partial outputs meet in shared memory, in a fixed order.
+//
+// What bounds it: launch, laying out x and joining take 8 to 10 us of a call; the weights then stream at 4 to 5 TB/s, the
+// rest of the time going into the codes (about 150 instructions a warp and 16 x 128 weights). 14336 x 8192 weights in groups
+// of 128 by 8 bf16 rows: 23.5 us (63 MB, floor 9.6); 4097 x 2050 in groups of 32 by 50 f16 rows: 20.5 us; 1024 x 512 by one
+// f32 row with GELU: 4.8 us.
 constexpr int W4_WARPS = 8, W4_X_BYTES = 65536, W4_Y_UNITS = 64;
 constexpr int W4_DEPTH = 3;   // steps a warp's ring holds
 constexpr int W4_SLICE = 16;  // most blocks of columns of x that a block holds at once
@@ -134,11 +139,13 @@ __device__ __forceinline__ float w4_fragment(const float (&v)[8], float up, uint
     for (int k = 0; k < QS; k++) h[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
     return s;
 }
-// The power of two that brings a row's largest magnitude into [2^13, 2^14), and what undoes it on the sums (with 2^24 for
-// the codes).
+// The power of two that brings a row's largest magnitude into [2^13, 2^14), and what undoes it on the sums (with the codes'
+// unit).
+__device__ __forceinline__ constexpr float w4_unit(int qs) { return qs == 2 ? 1.f : 5.9604644775390625e-8f; }  // centred codes, or 2^-24
+template <int QS>
 __device__ __forceinline__ float w4_up(float mx, float &undo) {
     const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
-    undo = __uint_as_float((uint32_t)(127 - e) << 23) * 16777216.f;
+    undo = __uint_as_float((uint32_t)(127 - e) << 23) / w4_unit(QS);
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 // Words of fragments and floats of sums of one block of 128 columns of 8 NT rows.
@@ -167,7 +174,7 @@ __global__ void __launch_bounds__(256) k_w4_x(W4Args a, int dtype, uint32_t *xf,
 #pragma unroll
     for (int w = 0; w < 8; w++) mx = fmaxf(mx, red[w]);
     float undo;
-    const float up = w4_up(mx, undo);
+    const float up = w4_up<QS>(mx, undo);
     if (threadIdx.x == 0) fx[rt * R + m] = undo;
     for (int i0 = 0; i0 < blocks * 16; i0 += 256) {
         const int i = i0 + threadIdx.x, b = i / 16, u = i % 16 / 4, q = i % 4;
@@ -183,7 +190,7 @@ __global__ void __launch_bounds__(256) k_w4_x(W4Args a, int dtype, uint32_t *xf,
                 *reinterpret_cast<uint4 *>(xf + ((size_t)(rt * blocks + b) * NT * QS + (m / 8) * QS + k) * 512 + u * 128 + (m % 8 * 4 + q) * 4) = h[k];
 #pragma unroll
         for (int d = 1; d < G / 8; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-        if (on && i % (G / 8) == 0) xs[((size_t)(rt * blocks + b) * NG + i % 16 / (G / 8)) * R + m] = s * 5.9604644775390625e-8f;  // 2^-24
+        if (on && i % (G / 8) == 0) xs[((size_t)(rt * blocks + b) * NG + i % 16 / (G / 8)) * R + m] = s * w4_unit(QS);
     }
 }
 
@@ -305,7 +312,7 @@ __global__ void __launch_bounds__(W4_WARPS * 32, NT < 8 ? 2 : 1) k_w4_linear(W4A
 #pragma unroll
                     for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[x][j]));
                 float undo;
-                const float up = w4_up(warp_max(mx), undo);
+                const float up = w4_up<QS>(warp_max(mx), undo);
                 if (lane == 0) fx[warp] = undo;
 #pragma unroll
                 for (int x = 0; x < W4_SLICE / 2; x++) {
@@ -318,7 +325,7 @@ __global__ void __launch_bounds__(W4_WARPS * 32, NT < 8 ? 2 : 1) k_w4_linear(W4A
                         if (on) *reinterpret_cast<uint4 *>(xf + (b * QS + k) * 512 + u * 128 + (warp * 4 + q) * 4) = h[k];
 #pragma unroll
                     for (int d = 1; d < G / 8; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-                    if (on && i % (G / 8) == 0) xs[(b * NG + i % 16 / (G / 8)) * R + warp] = s * 5.9604644775390625e-8f;  // 2^-24
+                    if (on && i % (G / 8) == 0) xs[(b * NG + i % 16 / (G / 8)) * R + warp] = s * w4_unit(QS);
                 }
             }
             if (lay) {
@@ -359,11 +366,12 @@ __global__ void __launch_bounds__(W4_WARPS * 32, NT < 8 ? 2 : 1) k_w4_linear(W4A
 #pragma unroll
                                 for (int z = QS - 1; z >= 0; z--) {
                                     const uint4 x = *reinterpret_cast<const uint4 *>(xb + ((nt * QS + z) * 4 + u) * 128);
-                                    w4_mma(acc[nt], c0[u] & 0x000f000fu, c1[u] & 0x000f000fu, c0[u] & 0x00f000f0u, c1[u] & 0x00f000f0u, x.x, x.y);
-                                    w4_mma(acc[nt], v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, x.z, x.w);
+                                    w4_mma(acc[nt], code_pair<QS == 2, false>(c0[u]), code_pair<QS == 2, false>(c1[u]), code_pair<QS == 2, true>(c0[u]), code_pair<QS == 2, true>(c1[u]), x.x, x.y);
+                                    w4_mma(acc[nt], code_pair<QS == 2, false>(v0), code_pair<QS == 2, false>(v1), code_pair<QS == 2, true>(v0), code_pair<QS == 2, true>(v1), x.z, x.w);
                                 }
                         }
-                        const float2 s0 = w4_float2(sc[g * 2 * NG + q]), s1 = w4_float2(sc[(g + 8) * 2 * NG + q]);
+                        float2 s0 = w4_float2(sc[g * 2 * NG + q]), s1 = w4_float2(sc[(g + 8) * 2 * NG + q]);
+                        if (QS == 2) s0.y = fmaf(8.f, s0.x, s0.y), s1.y = fmaf(8.f, s1.x, s1.y);  // the codes came less 8
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             const float2 sx = *reinterpret_cast<const float2 *>(xs + (b * NG + q) * R + nt * 8 + 2 * t);

@@ -245,6 +245,32 @@ def test_attend_scales_of_very_different_size(gpu, rows):
     c.check("f32", q, [rows], 0.125, False, 0, out, lse)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,width,group", [(1, 128, 64), (3, 128, 32), (2, 64, 32), (1, 256, 128), (200, 128, 64)])
+def test_attend_values_that_cancel(gpu, dtype, rows, width, group):
+    """Flat scores over thousands of keys whose values have no mean: outputs far below the values and their lows."""
+    n = 6000
+    c = Cached(gpu, 14, [16], 1, width, 256, group, extra=n // 256 + 1)
+    rng = np.random.default_rng(7)
+    k, v = rng.normal(0, 1, (2, n, 1, width))
+    order = rng.permutation(c.pages)[:-(-n // 256)]
+    raw, kk, vv = plain.pool_of(k.astype(np.float32), v.astype(np.float32), order[np.arange(n) // 256] * 256 + np.arange(n) % 256,
+                                c.pages, 256, group, 0xFF)
+    c.pool.copy_(dev(raw))
+    c.table, c.stride, c.lens = dev(order.astype(np.int32)[None]), len(order), [n]
+    c.lens_dev.fill_(n)
+    q = rounded(rng.normal(0, 1, (rows, 2, width)), DT[dtype][1])
+    out, lse = c.attend(dtype, q, [rows], 0.5 / np.sqrt(width))
+    sync(gpu)
+    o, l, _ = plain.attend(q, kk, vv, rows, n, 0.5 / np.sqrt(width), False, 0)
+    # weights are off by 2^-20 for f32 and 2^-11 (keys, or twice 2^-12) else, each by itself, so a sum of values without a
+    # mean by no more than that share of itself; an f32 sum by 2^-23 of its size a step, some ten steps' worth; the result
+    # by its own rounding
+    off = np.linalg.norm(host(out) - o) / np.linalg.norm(o)
+    assert off <= {"f32": 1e-5, "f16": 2.0**-11, "bf16": 2.0**-8}[dtype], off
+    assert np.abs(host(lse) - l).max() <= {"f32": 1e-5, "f16": 2.0**-9, "bf16": 2.0**-9}[dtype]
+
+
 @pytest.mark.parametrize("dtype,rows", [("f32", 1), ("bf16", 1), ("f32", 200), ("bf16", 200)])
 def test_attend_strides_and_repeat(gpu, dtype, rows):
     """Query and output rows inside wider buffers at odd places; the same call again gives the same bits."""
@@ -416,6 +442,22 @@ def test_linear(gpu, dtype, n, k, group, rows, act, bias, residual):
     got = host(yd)
     assert (np.abs(got[:, :n] - y) <= 2.0**-20 * size + 2 * ULP[dtype] * np.abs(y) + 1e-7).all()
     assert (got[:, n:] == 9).all()
+
+
+@pytest.mark.parametrize("rows", [1, 5, 20, 70])
+@pytest.mark.parametrize("k,group", [(512, 64), (4000, 32), (3000, 128)])
+def test_linear_keeps_32_bits(gpu, rows, k, group):
+    """f32 sums of products of either sign: a group's sum is rounded some ten times by at most 2^-23 of its size."""
+    rng = np.random.default_rng(k + rows)
+    w4, keep, w = weights(rng, gpu, 64, k, group, "f32")
+    x = rng.normal(0, 1, (rows, k)).astype(np.float32)
+    xd, yd = dev(x), torch.zeros(rows, 64, device="cuda")
+    work = torch.zeros(max(16, w4.linear_workspace(rows, 0)), dtype=torch.uint8, device="cuda")
+    w4.linear(0, rows, xd.data_ptr(), k, yd.data_ptr(), 64, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    y = x.astype(np.float64) @ w.T
+    off = np.linalg.norm(host(yd) - y) / np.linalg.norm(y)
+    assert off <= 1e-6, off
 
 
 def test_linear_keeps_rows_apart(gpu):
