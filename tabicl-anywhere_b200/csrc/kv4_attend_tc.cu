@@ -15,7 +15,6 @@
 // turn took 2048 rows over 10,000 keys (4 heads of 128) from 0.28 to 0.19 ms, loops short enough for the instruction caches
 // to 0.17 ms: 0.24 PFLOP/s of scores and sums, 0.73 of products.
 #include <algorithm>
-#include <atomic>
 
 #include "kv4_tc.cuh"
 

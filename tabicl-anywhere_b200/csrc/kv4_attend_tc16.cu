@@ -3,11 +3,11 @@
 // 256 query rows of one cache head (the heads that share it side by side) as two tiles of 128, against 64 keys at a time:
 // S = Q K^T with Q and the keys, widened to f16, in shared memory; the weights P go to tensor memory over S and multiply
 // the widened values; the output stays in tensor memory. Keys, values and weights are one f16 each (11 bits; the results
-// have 11 or 8), sums are f32. What bounds it is the exponentials (16 a cycle and SM, 1024 cycles a step) beside the
-// instructions that feed them, so the two tiles have a warpgroup each, and widening, which serves both, two that take the
-// steps in turn. A step takes about 2300 cycles; the products issued from one diverged thread took it to 2800, loops
-// unrolled over a whole step (which the instruction caches do not hold beside widening) to 2700. A prompt of 4096 bf16
-// tokens after 1000 cached ones, 32 heads of 128 on 8: 0.40 ms, 0.51 PFLOP/s.
+// have 11 or 8; the log-sum-exp carries the keys' 11 bits), sums are f32. What bounds it is the exponentials (16 a cycle and
+// SM, 1024 cycles a step) beside the instructions that feed them, so the two tiles have a warpgroup each, and widening,
+// which serves both, two that take the steps in turn. A step takes about 2300 cycles; the products issued from one diverged
+// thread took it to 2800, loops unrolled over a whole step (which the instruction caches do not hold beside widening) to
+// 2700. A prompt of 4096 bf16 tokens after 1000 cached ones, 32 heads of 128 on 8: 0.40 ms, 0.51 PFLOP/s.
 //
 // A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8, so the output
 // in tensor memory is rarely rescaled. A step's keys and values are scaled by a power of two of their own that keeps them

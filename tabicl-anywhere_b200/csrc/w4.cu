@@ -73,7 +73,7 @@ cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k
 // What bounds it: launch, laying out x and joining take 8 to 10 us of a call; the weights then stream at 4 to 5 TB/s, the
 // rest of the time going into the codes (about 150 instructions a warp and 16 x 128 weights). 14336 x 8192 weights in groups
 // of 128 by 8 bf16 rows: 23.5 us (63 MB, floor 9.6); 4097 x 2050 in groups of 32 by 50 f16 rows: 20.5 us; 1024 x 512 by one
-// f32 row with GELU: 4.8 us.
+// f32 row with GELU: 5.1 us.
 constexpr int W4_WARPS = 8, W4_X_BYTES = 65536, W4_Y_UNITS = 64;
 constexpr int W4_DEPTH = 3;   // steps a warp's ring holds
 constexpr int W4_SLICE = 16;  // most blocks of columns of x that a block holds at once
