@@ -134,11 +134,16 @@ struct Elem<DT_BF16> {
     static __device__ __forceinline__ __nv_bfloat16 put(float x) { return __float2bfloat16_rn(x); }
 };
 
-// Eight consecutive elements; `wide` when the address is known to be 16-byte aligned.
+// Eight consecutive elements; `wide`: the address is known to be 16-byte aligned (1) or, f32, 32-byte aligned (2: one access of
+// 32 bytes, so a warp's accesses are whole lines).
 template <int DT>
-__device__ __forceinline__ void load8(const typename Elem<DT>::T *p, bool wide, float (&v)[8]) {
+__device__ __forceinline__ void load8(const typename Elem<DT>::T *p, int wide, float (&v)[8]) {
     using T = typename Elem<DT>::T;
-    if (wide) {
+    if (DT == DT_F32 && wide == 2) {
+        asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "l"(p));
+    } else if (wide) {
         __align__(16) T e[8];
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; i++)
@@ -151,8 +156,14 @@ __device__ __forceinline__ void load8(const typename Elem<DT>::T *p, bool wide, 
     }
 }
 template <int DT>
-__device__ __forceinline__ void store8(typename Elem<DT>::T *p, bool wide, const float (&v)[8]) {
+__device__ __forceinline__ void store8(typename Elem<DT>::T *p, int wide, const float (&v)[8]) {
     using T = typename Elem<DT>::T;
+    if (DT == DT_F32 && wide == 2) {
+        asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                     "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                     : "memory");
+        return;
+    }
     __align__(16) T e[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) e[i] = Elem<DT>::put(v[i]);

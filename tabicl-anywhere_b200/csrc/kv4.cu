@@ -12,7 +12,7 @@ namespace tcu {
 // A thread takes 8 neighbouring coordinates (one word of a key, two half-words of a value) of one head of one token, of
 // the keys and of the values; width / 8 neighbouring lanes hold a token's head, group / 8 of them a group.
 template <int DT, bool STORE>
-__global__ void __launch_bounds__(256) k_kv4_copy(Kv4CopyArgs a, uint32_t items, int per_log2, int page_log2, int group_log2, bool wide) {
+__global__ void __launch_bounds__(256) k_kv4_copy(Kv4CopyArgs a, uint32_t items, int per_log2, int page_log2, int group_log2, int wide) {
     using T = typename Elem<DT>::T;
     const int W = a.c.width, NU = W / 32, G8 = a.c.group / 8, NG = W / a.c.group, P = a.c.page;
     const uint32_t i = blockIdx.x * 256u + threadIdx.x;
@@ -76,8 +76,8 @@ static int log2_of(int x) { return x <= 1 ? 0 : 1 + log2_of(x / 2); }
 template <bool STORE>
 static cudaError_t launch_copy(int dtype, Kv4CopyArgs a, cudaStream_t s, uint64_t *launches) {
     const int es = dtype == DT_F32 ? 4 : 2, per = a.c.width / 8;
-    const bool wide = !((((uintptr_t)a.k | (uintptr_t)a.v) & 15) ||
-                        ((a.k_row | a.k_head | a.v_row | a.v_head) * es) % 16);
+    const uint64_t places = (uintptr_t)a.k | (uintptr_t)a.v | (uint64_t)((a.k_row | a.k_head | a.v_row | a.v_head) * es);
+    const int wide = dtype == DT_F32 && places % 32 == 0 ? 2 : places % 16 == 0 ? 1 : 0;
     // indexes are 32 bits wide: very long calls in parts
     const int most = (int)std::min<long long>(0x7fffffff, 0x7fffff00LL / ((long long)a.c.heads * per));
     for (int left = a.tokens; left > 0;) {
