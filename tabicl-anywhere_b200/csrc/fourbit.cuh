@@ -226,22 +226,32 @@ __device__ __forceinline__ void group_scale(float mn, float mx, bool bad, __half
     step = __float2half_rn(__fdiv_rn(fmaxf(__fsub_rn(fminf(mx, 65504.f), __half2float(low)), 0.f), 15.f));
     if (bad) step = __ushort_as_half(0), low = __ushort_as_half(0x7e00);
 }
-// A value's code: its distance from low in steps, rounded to the nearest (ties to even), held to 0..15; 0 where the
+// Eight values' codes: a value's distance from low in steps, rounded to the nearest (ties to even), held to 0..15; 0 where the
 // step is 0. The quotient is the correctly rounded one, so equal inputs give equal codes everywhere.
-// It is found as a product with the step's reciprocal, which is within 2^-21 of it; only where that is near a tie is the
-// division itself taken (it costs as much as all the rest).
-__device__ __forceinline__ uint32_t code_of(float x, float step, float inverse, float low) {
-    const float d = __fsub_rn(x, low), t = d * inverse;
-    float c = rintf(t);
-    if (fabsf(fabsf(t - c) - 0.5f) < 1e-4f) c = rintf(__fdiv_rn(d, step));
-    return (uint32_t)(int)fminf(fmaxf(c, 0.f), 15.f);
-}
+// It is found as a product with the step's reciprocal, within 2^-20 of it (so 1.5e-5 at most), and rounded by adding 1.5 * 2^23, whose sum's low
+// bits are the code; only where one of the eight is near a tie are they divided (which costs as much as all the rest).
 __device__ __forceinline__ uint32_t pack8(const float (&x)[8], float step, float low) {
     if (!(step > 0.f)) return 0;
-    const float inverse = __frcp_rn(step);
+    constexpr float MAGIC = 12582912.f;
+    float inverse, near = 0.f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(step));  // (an f16's range: no subnormal f32)
     uint32_t w = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) w |= code_of(x[j], step, inverse, low) << (4 * j);
+    for (int j = 0; j < 8; j++) {
+        const float t = fminf(fmaxf(__fmul_rn(__fsub_rn(x[j], low), inverse), 0.f), 15.f), c = __fadd_rn(t, MAGIC);
+        near = fmaxf(near, fabsf(__fsub_rn(t, __fsub_rn(c, MAGIC))));
+        w += (__float_as_uint(c) - 0x4b400000u) << (4 * j);
+    }
+    if (near > 0.49997f) {
+        w = 0;
+#pragma unroll 1
+        for (int j = 0; j < 8; j++) {
+            float v = x[0];
+#pragma unroll
+            for (int k = 1; k < 8; k++) v = k == j ? x[k] : v;
+            w |= (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(v, low), step)), 0.f), 15.f) << (4 * j);
+        }
+    }
     return w;
 }
 // low + step * code, the product and the sum each rounded to f32 (step * code is exact: 11 + 4 bits).
