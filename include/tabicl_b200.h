@@ -418,8 +418,8 @@ TCU_API int tcu_comm_breakdown(tcu_comm *c, int enable, double *ms);
  * All pointers are device pointers, everything is queued on `stream` (a cudaStream_t; NULL = the context's stream, which
  * does not wait for the legacy default stream: pass cudaStreamLegacy, the value 1, for that one), and nothing is
  * allocated: where a call needs working memory the caller gives it (a `_workspace` call says how much; one such block
- * serves one call at a time; its bytes must be zero before its first use, and every call leaves zero what it needs to
- * be). Indexes that only the device sees (slots, page numbers, lengths, starts, labels) are checked there: one outside
+ * serves one call at a time, of any of these operators; its bytes must be zero before its first use, and every call
+ * leaves zero what any of them needs to be). Indexes that only the device sees (slots, page numbers, lengths, starts, labels) are checked there: one outside
  * its range is not followed, and the next call on the context, or tcu_sync, reports it (TCU_ERR_ARG). */
 enum { TCU_F32 = 0, TCU_F16 = 1, TCU_BF16 = 2 }; /* element types of inputs and outputs */
 

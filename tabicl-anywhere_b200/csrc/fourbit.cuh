@@ -20,6 +20,10 @@ namespace tcu {
 
 enum { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };
 
+// Most blocks of an attention launch. As many arrival counters (ints, zero between calls) start the working memory of every
+// operator, so that one block of it serves them all: attention counts there, the others leave them alone.
+constexpr int KA_BLOCKS = 2048;
+
 // A paged cache: pool [pages][heads]{key codes [page][width / 2], key (step, low) [page][width / group], value codes,
 // value (step, low)}.
 struct Kv4 {
@@ -106,6 +110,7 @@ cudaError_t launch_kv4_attend_tc16(int dtype, const Kv4AttendArgs &a, int sms, v
 // A weight matrix w [n][k] (row stride ldw) to codes and scales.
 cudaError_t launch_w4_pack(int dtype, const void *w, long long ldw, int n, int k, int group, uint8_t *codes,
                            __half2 *scales, cudaStream_t s, uint64_t *launches);
+// Working memory of a linear layer (what it uses comes after the KA_BLOCKS counters), and the call.
 size_t w4_linear_workspace(int dtype, const W4Args &a, int sms);
 cudaError_t launch_w4_linear(int dtype, const W4Args &a, int sms, void *work, size_t work_bytes, cudaStream_t s,
                              uint64_t *launches);

@@ -10,8 +10,6 @@
 
 namespace tcu {
 
-constexpr int KA_BLOCKS = 2048;  // most blocks of a launch: as many arrival counters start the working memory of every call
-
 template <int N>
 __device__ __forceinline__ void lds_words(const uint8_t *p, uint32_t (&w)[N]) {  // N consecutive words, aligned to 4 N up to 16
     if constexpr (N % 4 == 0) {

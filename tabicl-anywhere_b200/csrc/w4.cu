@@ -497,13 +497,13 @@ static W4Plan w4_plan(int dtype, const W4Args &a, int sms) {
     return p;
 }
 
-// More than 8 rows: the fragments, the groups' sums and the rows' factors, one after the other.
+// More than 8 rows: after attention's counters the fragments, the groups' sums and the rows' factors, one after the other.
 static size_t w4_frag_bytes(const W4Args &a, const W4Plan &p, int qs) { return (size_t)p.row_tiles * ((a.k + 127) / 128) * w4_frag_words(p.nt, qs) * 4; }
 static size_t w4_sum_bytes(const W4Args &a, const W4Plan &p) { return (size_t)p.row_tiles * ((a.k + 127) / 128) * (128 / a.group) * 8 * p.nt * 4; }
 size_t w4_linear_workspace(int dtype, const W4Args &a, int sms) {
     if (a.rows <= 8) return 0;
     const W4Plan p = w4_plan(dtype, a, sms);
-    return w4_frag_bytes(a, p, dtype == DT_F32 ? 2 : 1) + w4_sum_bytes(a, p) + (size_t)p.row_tiles * 8 * p.nt * 4;
+    return 4 * KA_BLOCKS + w4_frag_bytes(a, p, dtype == DT_F32 ? 2 : 1) + w4_sum_bytes(a, p) + (size_t)p.row_tiles * 8 * p.nt * 4;
 }
 
 template <int G, int NT, int QS>
@@ -511,10 +511,11 @@ static cudaError_t launch_w4(int dtype, const W4Args &a, const W4Plan &p, void *
     const size_t smem = w4_smem_bytes(p, G, QS);
     cudaError_t e = allow_dynamic_smem((const void *)k_w4_linear<G, NT, QS>, smem);
     if (e != cudaSuccess) return e;
-    uint32_t *xf = reinterpret_cast<uint32_t *>(work);
+    uint32_t *xf = nullptr;
     float *xs = nullptr, *fx = nullptr;
     if constexpr (NT > 1) {
-        xs = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(work) + w4_frag_bytes(a, p, QS));
+        xf = reinterpret_cast<uint32_t *>(work) + KA_BLOCKS;
+        xs = reinterpret_cast<float *>(xf + w4_frag_bytes(a, p, QS) / 4);
         fx = xs + w4_sum_bytes(a, p) / 4;
         k_w4_x<G, NT, QS><<<p.row_tiles * 8 * NT, 256, 0, s>>>(a, dtype, xf, xs, fx);
         if (launches) ++*launches;

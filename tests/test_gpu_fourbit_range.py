@@ -1,0 +1,93 @@
+"""The four-bit operators where types, sizes and values reach their ends, on the GPU against plain numpy or torch in 64 bits:
+very different magnitudes side by side, masks to the key, odd places and orders, working memory that all of them share,
+graph capture. Attention is tried on each of its kernels; `kernels` asserts which one a call takes."""
+import numpy as np
+import pytest
+
+import fourbit_plain as plain
+import test_gpu_fourbit as base
+from conftest import tcu
+from test_gpu_fourbit import DT, ULP, Cached, check_many, dev, host, rounded, sync, weights
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+gpu = base.gpu
+
+
+def kernels(c, dtype, rows, q_heads):
+    """Which attention kernels the call takes, by the working memory it asks for: "few" or "many" rows. (Of f32 at widths up
+    to 64 both ask for the same.)"""
+    assert dtype != "f32" or c.width > 64
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    batch = c.cache.batch(len(c.lens), rows, max(c.lens + [1]), c.lens_dev.data_ptr(), c.table.data_ptr(), c.stride)
+    many = 4 * (2048 + 2 * sms * (128 if dtype == "f32" else 256) * (c.width + 2))
+    return "many" if c.cache.attend_workspace(batch, q_heads, DT[dtype][0]) == many else "few"
+
+
+def set_tokens(c, k, v, page, group):
+    """The same keys k and values v [tokens][heads][width] in every sequence of c."""
+    n, seqs = k.shape[0], len(c.lens)
+    table = c.table.cpu().numpy()
+    slots = [int(table[s, j // page]) * page + j % page for s in range(seqs) for j in range(n)]
+    tile = lambda x: np.tile(np.asarray(x, np.float32), (seqs, 1, 1))  # noqa: E731
+    raw, kk, vv = plain.pool_of(tile(k), tile(v), slots, c.pages, page, group, 0xFF)
+    c.pool.copy_(dev(raw))
+    c.k, c.v = [kk[:n]] * seqs, [vv[:n]] * seqs
+
+
+def exact(q, k, v, scale, seen):
+    """Rows q [n][q_heads][width] against keys and values [length][heads][width] in 64 bits, `seen` [n][length]: the outputs,
+    the sums of |p v| behind them, lse, and the scores' largest sums of magnitudes."""
+    each = q.shape[1] // k.shape[1]
+    out, size = np.zeros(q.shape), np.zeros(q.shape)
+    lse, reach = np.full(q.shape[:2], -np.inf), np.zeros(q.shape[:2])
+    some = seen.any(1)
+    for h in range(q.shape[1]):
+        x, kk, vv = q[:, h].astype(np.float64), k[:, h // each], v[:, h // each]
+        s = np.where(seen, x @ kk.T * scale, -np.inf)
+        m = np.where(some, s.max(1), 0.0)
+        p = np.exp(s - m[:, None])
+        total = np.where(some, p.sum(1), 1.0)
+        out[:, h], size[:, h] = p @ vv / total[:, None], p @ np.abs(vv) / total[:, None]
+        lse[some, h] = (m + np.log(total))[some]
+        reach[:, h] = np.where(seen, np.abs(x) @ np.abs(kk).T * abs(scale), 0.0).max(1)
+    return out, size, lse, reach
+
+
+def visible(n, length, causal, window):
+    i, j = np.arange(n)[:, None], np.arange(length)[None]
+    seen = np.ones((n, length), bool)
+    if causal:
+        seen &= j <= length - n + i
+    if window:
+        seen &= j > length - n + i - window
+    return seen
+
+
+@pytest.mark.parametrize("dtype,width,heads,q_heads,rows,length,which", [
+    ("bf16", 64, 1, 1, 1, 5000, "few"), ("f32", 128, 1, 4, 2, 3000, "few"), ("bf16", 128, 4, 8, 1100, 4000, "many"),
+    ("f32", 128, 4, 8, 1100, 4000, "many")])
+def test_working_memory_serves_every_operator(gpu, dtype, width, heads, q_heads, rows, length, which):
+    """One block of working memory for attention whose units are cut into parts and linear layers of more than 8 rows, in
+    turn: the same bits as with a block of their own."""
+    code, tt = DT[dtype]
+    c = Cached(gpu, 30, [length], heads, width, 64, 32)
+    assert kernels(c, dtype, rows, q_heads) == which
+    rng = np.random.default_rng(1)
+    q = rounded(rng.normal(0, 1, (rows, q_heads, width)), tt)
+    w4, keep, _ = weights(rng, gpu, 300, 1000, 32, dtype)
+    x = dev(rng.normal(0, 1, (20, 1000)).astype(np.float32), tt)
+    shared = torch.zeros(64 << 20, dtype=torch.uint8, device="cuda")
+
+    def linear(work):
+        y = torch.full((20, 300), 9.0, dtype=tt, device="cuda")
+        w4.linear(code, 20, x.data_ptr(), 1000, y.data_ptr(), 300, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+        return y
+
+    own = torch.zeros(w4.linear_workspace(20, code), dtype=torch.uint8, device="cuda")
+    want_y, (want, want_lse) = linear(own), c.attend(dtype, q, [rows], 0.125, causal=True)
+    for _ in range(3):
+        y, (out, lse) = linear(shared), c.attend(dtype, q, [rows], 0.125, causal=True, work=shared)
+        sync(gpu)
+        assert torch.equal(y, want_y) and torch.equal(out, want) and torch.equal(lse, want_lse)
+    c.check(dtype, q[-3:], [min(rows, 3)], 0.125, True, 0, want[-3:], want_lse[-3:])
