@@ -3340,6 +3340,8 @@ int tcu_kv4_attend_device(tcu_ctx *ctx, const tcu_kv4 *cache, const tcu_kv4_batc
         check_aligned("kv4_attend", "lengths", a.lens, 4), check_aligned("kv4_attend", "table", a.table, 4);
         check_aligned("kv4_attend", "starts", a.starts, 4), check_aligned("kv4_attend", "lse", lse, 4);
         a.q = q, a.out = out, a.q_row = q_row, a.q_head = q_head, a.o_row = o_row, a.o_head = o_head;
+        // (no row sees more than max_len tokens: a wider window hides nothing, and would pass 32 bits in the rows' bounds)
+        if (window >= a.max_len) window = 0;
         a.scale = scale, a.causal = causal != 0, a.window = window, a.lse = lse, a.err = ctx->err_mapped + ERR_INDEX;
         a.err_wait = ctx->err_mapped + ERR_ATTEND_TC;
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;

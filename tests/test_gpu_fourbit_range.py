@@ -91,3 +91,22 @@ def test_working_memory_serves_every_operator(gpu, dtype, width, heads, q_heads,
         sync(gpu)
         assert torch.equal(y, want_y) and torch.equal(out, want) and torch.equal(lse, want_lse)
     c.check(dtype, q[-3:], [min(rows, 3)], 0.125, True, 0, want[-3:], want_lse[-3:])
+
+
+# sequences and heads that reach each kernel with a few dozen rows (f32 has its own for many rows)
+BOTH = [("f32", "few"), ("f16", "few"), ("bf16", "few"), ("f32", "many"), ("f16", "many"), ("bf16", "many")]
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+def test_a_window_wider_than_any_sequence_hides_nothing(gpu, dtype, which):
+    """Windows up to the largest number, where a sequence has fewer tokens than rows."""
+    lens, rows = ([5, 1, 40, 0], 10) if which == "few" else ([5, 1, 40, 0] * 10, 45)
+    c = Cached(gpu, 31, lens, 1 if which == "few" else 4, 128, 32, 64)
+    assert kernels(c, dtype, rows, c.heads) == which
+    q = rounded(np.random.default_rng(2).normal(0, 1, (rows * len(lens), c.heads, 128)), DT[dtype][1])
+    want, want_lse = c.attend(dtype, q, [rows] * len(lens), 0.1, causal=True)
+    for window in (41, 1 << 20, 2**31 - 1):
+        out, lse = c.attend(dtype, q, [rows] * len(lens), 0.1, causal=True, window=window)
+        sync(gpu)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse), window
+    check_many(c, dtype, q, rows, 0.1, True, 0, want, want_lse)
