@@ -2,12 +2,17 @@
 //
 // 256 query rows of one cache head (the heads that share it side by side) as two tiles of 128, against 64 keys at a time:
 // S = Q K^T with Q and the keys, widened to f16, in shared memory; the weights P go to tensor memory over S and multiply
-// the widened values; the output stays in tensor memory. Keys, values and weights are one f16 each (11 bits; the results
-// have 11 or 8; the log-sum-exp carries the keys' 11 bits), sums are f32. What bounds it is the exponentials (16 a cycle and
-// SM, 1024 cycles a step) beside the instructions that feed them, so the two tiles have a warpgroup each, and widening,
-// which serves both, two that take the steps in turn. A step takes about 2300 cycles; the products issued from one diverged
-// thread took it to 2800, loops unrolled over a whole step (which the instruction caches do not hold beside widening) to
-// 2700. A prompt of 4096 bf16 tokens after 1000 cached ones, 32 heads of 128 on 8: 0.40 ms, 0.51 PFLOP/s.
+// the widened values; the output stays in tensor memory. Values and weights are one f16 each (11 bits; the results have 11
+// or 8), sums are f32. Keys are exact, so that the log-sum-exp is f32 as in the other kernels: a key is low + 8 step +
+// step (code - 8), the step the sum of its upper 7 and its lower 4 bits, whose products with code - 8 f16 holds; two operand
+// blocks have those, and 16 columns beside the first the lows and 8 steps, which meet the sums of q over each group (as two
+// f16).
+// What bounds it is shared memory beside the instruction issue: a step's operands are some 290 KB read and written (2300
+// cycles at 128 bytes), the exponentials 1024 cycles (16 a cycle and SM), and a step takes about 2750. The two tiles have a
+// warpgroup each, and widening, which serves both, two that take the steps in turn. Keys rounded to one f16 took 2300 cycles
+// a step (0.40 ms for the prompt below, its lse 4e-6 off), as two f16 split in f32 2980. The products issued from one
+// diverged thread cost 500 cycles more, loops unrolled over a whole step (which the instruction caches do not hold beside
+// widening) 400. A prompt of 4096 bf16 tokens after 1000 cached ones, 32 heads of 128 on 8: 0.48 ms, 0.43 PFLOP/s.
 //
 // A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8, so the output
 // in tensor memory is rarely rescaled. A step's keys and values are scaled by a power of two of their own that keeps them
@@ -20,15 +25,19 @@
 
 namespace tcu {
 
-constexpr int KU_R = 256, KU_BQ = 128, KU_BK = 64, KU_NS = 3, KU_NR = 4, KU_THREADS = 640;
-constexpr int KU_T = -5;  // widened values are below 2^T
+constexpr int KU_R = 256, KU_BQ = 128, KU_BK = 64, KU_THREADS = 640;
+constexpr int KU_NK = 2, KU_NS = 3, KU_NR = 3;  // slots of widened keys, of widened values, of stored codes
+constexpr int KU_T = -5;   // widened values are below 2^T
+constexpr int KU_TK = 15;  // widened keys are below 2^TK
+constexpr int KU_X = 16;   // columns beside the coordinates in which the groups' lows meet the sums of q
 constexpr uint32_t KU_TS = 0, KU_TO = 256;  // tensor memory: [tile][2 slots] of S / P, then [tile] of O
 
 template <int HD, int G>
 struct KuShape {
     static constexpr int NU = HD / 32, NG = HD / G, BLOCK = KU_BK * HD;
     static constexpr int KC = KU_BK * HD / 2, SC = KU_BK * NG * 4, RAW = 2 * (KC + SC);
-    static constexpr size_t SMEM = (size_t)KU_R * HD * 2 + (size_t)2 * KU_NS * BLOCK * 2 + (size_t)KU_NR * RAW + 1024;
+    static constexpr int KSLOT = 2 * BLOCK + KU_BK * KU_X;  // f16 of a step's keys
+    static constexpr size_t SMEM = (size_t)KU_R * (HD + KU_X) * 2 + (size_t)(KU_NK * KSLOT + KU_NS * BLOCK) * 2 + (size_t)KU_NR * RAW + 1024;
 };
 
 // Warps 0-3, 4-7: softmax of the first and second tile, a thread a query row; warps 8-11, 12-15: widening of even and odd
@@ -39,16 +48,16 @@ template <int HD, int G>
 __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs a, int dtype, float *part, int *arrived) {
     using C = KuShape<HD, G>;
     using Cut = KaCut<KU_R, KU_BK, KU_BK>;
-    constexpr int NU = C::NU, NG = C::NG, UG = G / 32, BQ = KU_BQ, BK = KU_BK, NS = KU_NS, NR = KU_NR, BLOCK = C::BLOCK;
+    constexpr int NU = C::NU, NG = C::NG, UG = G / 32, BQ = KU_BQ, BK = KU_BK, NK = KU_NK, NS = KU_NS, NR = KU_NR, BLOCK = C::BLOCK, HX = HD + KU_X, KSLOT = C::KSLOT;
     extern __shared__ __align__(1024) uint8_t smraw[];
-    __half *Qs = reinterpret_cast<__half *>(smraw);   // [2][128 x HD], K-major
-    __half *Kring = Qs + KU_R * HD;                   // [NS][64 x HD], K-major
-    __half *Vring = Kring + NS * BLOCK;               // [NS][64 x HD], coordinate-major
+    __half *Qs = reinterpret_cast<__half *>(smraw);   // [2][128 x HX], K-major
+    __half *Kring = Qs + KU_R * HX;                   // [NK]{[64 x HX], [64 x HD]}, K-major: the keys, and what remains of them
+    __half *Vring = Kring + NK * KSLOT;               // [NS][64 x HD], coordinate-major
     uint8_t *raw = reinterpret_cast<uint8_t *>(Vring + NS * BLOCK);  // [NR]{key codes, key scales, value codes, value scales}
     __shared__ float red[2][2][2][4];  // [turn][step][keys, values][warp]
     __shared__ int teK[8], teV[8], has_nan[8];
     __shared__ uint32_t nan_keys[8][NG][2];
-    __shared__ __align__(8) uint64_t mK[NS], mV[NS], mKfree[NS], mVfree[NS], mS[2][2], mP[2][2], mSlot[2][2], mQ[2], mDone[2], mRaw[NR],
+    __shared__ __align__(8) uint64_t mK[NK], mV[NS], mKfree[NK], mVfree[NS], mS[2][2], mP[2][2], mSlot[2][2], mQ[2], mDone[2], mRaw[NR],
         mRawFree[NR];
     __shared__ uint32_t tslot;
     __shared__ volatile int abort_flag;
@@ -64,7 +73,8 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
         tmem_relinquish();
     }
     if (tid == 0) {
-        for (int i = 0; i < NS; i++) mbar_init(&mK[i], 128), mbar_init(&mV[i], 128), mbar_init(&mKfree[i], 1), mbar_init(&mVfree[i], 1);
+        for (int i = 0; i < NK; i++) mbar_init(&mK[i], 128), mbar_init(&mKfree[i], 1);
+        for (int i = 0; i < NS; i++) mbar_init(&mV[i], 128), mbar_init(&mVfree[i], 1);
         for (int q = 0; q < 2; q++) {
             for (int i = 0; i < 2; i++) mbar_init(&mS[q][i], 1), mbar_init(&mP[q][i], BQ), mbar_init(&mSlot[q][i], 1);
             mbar_init(&mQ[q], BQ), mbar_init(&mDone[q], 1);
@@ -143,19 +153,18 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
             const uint32_t idS = idesc_f16(BQ, BK, 0, 0), idO = idesc_f16(BQ, HD, 0, 1);
             const uint64_t dQ0 = kstep_desc(Qs, BQ, 0), dK0 = kstep_desc(Kring, BK, 0), dV0 = kstep_desc(Vring, HD, 0);
             constexpr uint64_t stQ = (2 * (BQ / 8) * 128) >> 4, stK = (2 * (BK / 8) * 128) >> 4, stV = (2 * (HD / 8) * 128) >> 4;
-            constexpr uint64_t q_off = (BQ * HD * 2) >> 4, slot_off = (BLOCK * 2) >> 4;
+            constexpr uint64_t q_off = (BQ * HX * 2) >> 4, k_off = (KSLOT * 2) >> 4, lo_off = (BK * HX * 2) >> 4, v_off = (BLOCK * 2) >> 4;
             int units[2] = {0, 0};  // pieces of each tile so far
             while (pl.pos < pl.end) {
                 const KaRows sr = ka_rows(a, pl.seq);
                 const auto sp = Cut::span(a, sr, each, pl.rt);
                 const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), nq = sr.n * each - pl.rt * KU_R > BQ ? 2 : 1;
                 for (int i = 0; i < n; i++) {
-                    const int sl = (at + i) % NS;
-                    const uint32_t ph = (uint32_t)((at + i) / NS) & 1u;
                     if (warp == 16) {
                         // S(i) of both tiles from the keys of step i, once P V(i - 2) has read the slot
-                        wait_warp(&mK[sl], ph);
-                        const uint64_t dK = dK0 + sl * slot_off;
+                        const int sl = (at + i) % NK;
+                        wait_warp(&mK[sl], (uint32_t)((at + i) / NK) & 1u);
+                        const uint64_t dK = dK0 + sl * k_off;
 #pragma unroll
                         for (int q = 0; q < 2; q++) {
                             if (q >= nq) break;
@@ -166,7 +175,9 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                             const uint32_t tS = tmem + KU_TS + (2 * q + (c & 1)) * BK;
                             if (elect_one()) {
 #pragma unroll
-                                for (int k = 0; k < HD / 16; k++) mma_f16(tS, dQ0 + q * q_off + k * stQ, dK + k * stK, idS, k > 0 ? 1u : 0u);
+                                for (int k = 0; k < HD / 16; k++) mma_f16(tS, dQ0 + q * q_off + k * stQ, dK + lo_off + k * stK, idS, k > 0 ? 1u : 0u);
+#pragma unroll
+                                for (int k = 0; k < HX / 16; k++) mma_f16(tS, dQ0 + q * q_off + k * stQ, dK + k * stK, idS, 1);
                                 mma_commit(&mS[q][c & 1]);
                                 if (q == nq - 1) mma_commit(&mKfree[sl]);
                             }
@@ -174,8 +185,9 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                         }
                     } else {
                         // P V(i) of both tiles, from the values of step i
-                        wait_warp(&mV[sl], ph);
-                        const uint64_t dV = dV0 + sl * slot_off;
+                        const int sl = (at + i) % NS;
+                        wait_warp(&mV[sl], (uint32_t)((at + i) / NS) & 1u);
+                        const uint64_t dV = dV0 + sl * v_off;
 #pragma unroll
                         for (int q = 0; q < 2; q++) {
                             if (q >= nq) break;
@@ -215,8 +227,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
             const auto sp = Cut::span(a, sr, each, pl.rt);
             const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), j0 = sp.base + pl.skip * BK;
             for (int i = at + ((at ^ turn) & 1); i < at + n; i += 2) {
-                const int sl = i % NS, rs = i % NR, j = j0 + (i - at) * BK + key;
-                const uint32_t ph = (uint32_t)(i / NS) & 1u;
+                const int kl = i % NK, sl = i % NS, rs = i % NR, j = j0 + (i - at) * BK + key;
                 wait_warp(&mRaw[rs], (uint32_t)(i / NR) & 1u);
                 const uint8_t *kraw = raw + rs * C::RAW, *vraw = kraw + C::KC + C::SC;
                 const bool seen = j >= sp.lo_min && j < sp.hi_max;
@@ -264,25 +275,39 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     e[x] = m > 0.f ? min(40, (int)(__float_as_uint(m) >> 23) - 125) : 0;  // m < 2^(e - 1): a span, 15 steps, below 2^e
                 }
                 if (tid % 128 == 0) teK[i & 7] = e[0], teV[i & 7] = e[1], has_nan[i & 7] = any;
-                KtScale<false> ks[NG], vs[NG];
+                KtScale<false> vs[NG];
 #pragma unroll
                 for (int k = 0; k < NG; k++) {
-                    const float2 f = __half22float2(kt_h2(kc[k])), g = __half22float2(kt_h2(vc[k]));
-                    ks[k].set(f.x, f.y, kt_pow2(KU_T - e[0])), vs[k].set(g.x, g.y, kt_pow2(KU_T - e[1]));
+                    const float2 f = __half22float2(kt_h2(kc[k]));  // (in the step's unit from here on: exact, but for steps below 2^-28 of its largest)
+                    kc[k] = kt_u32(__floats2half2_rn(f.x * kt_pow2(KU_TK - e[0]), f.y * kt_pow2(KU_TK - e[0])));
+                    const float2 g = __half22float2(kt_h2(vc[k]));
+                    vs[k].set(g.x, g.y, kt_pow2(KU_T - e[1]));
                 }
                 // (loops that are not unrolled over the halves: short code, see the softmax)
-                if (i >= NS) wait_warp(&mKfree[sl], ph ^ 1u);
+                if (i >= NK) wait_warp(&mKfree[kl], ((uint32_t)(i / NK) & 1u) ^ 1u);
 #pragma unroll 1
                 for (int x = 2 * half; x < 2 * half + 2; x++) {
                     uint32_t w[NU];
                     lds_words<NU>(kraw + key * (HD / 2) + x * NU * 4, w);
-                    __half *to = Kring + sl * BLOCK + kmajor_off(key, 8 * x, BK);
+                    __half *hi = Kring + kl * KSLOT + kmajor_off(key, 8 * x, BK), *lo = hi + BK * HX;
 #pragma unroll
-                    for (int u = 0; u < NU; u++) kt_widen(w[u], ks[u / UG], to + kmajor_off(0, 32, BK) * u, nullptr);
+                    for (int u = 0; u < NU; u++)
+                        kt_exact(w[u], __low2half2(kt_h2(kc[u / UG])), hi + kmajor_off(0, 32, BK) * u, lo + kmajor_off(0, 32, BK) * u);
+                }
+                {
+                    // beside them low, low, 8 step, 8 step of the four groups that there may be; here those of two
+                    uint32_t x[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < NG; k++)
+                        if (k / 2 == half) {
+                            const __half2 s = kt_h2(kc[k]);
+                            x[k % 2 * 2] = kt_u32(__high2half2(s)), x[k % 2 * 2 + 1] = kt_u32(__hmul2(__low2half2(s), kt_h2(0x48004800u)));
+                        }
+                    *reinterpret_cast<uint4 *>(Kring + kl * KSLOT + kmajor_off(key, HD + 8 * half, BK)) = make_uint4(x[0], x[1], x[2], x[3]);
                 }
                 fence_async_smem();
-                mbar_arrive(&mK[sl]);
-                if (i >= NS) wait_warp(&mVfree[sl], ph ^ 1u);
+                mbar_arrive(&mK[kl]);
+                if (i >= NS) wait_warp(&mVfree[sl], ((uint32_t)(i / NS) & 1u) ^ 1u);
 #pragma unroll 1
                 for (int x = 2 * half; x < 2 * half + 2; x++) {
                     uint32_t w[NU];
@@ -329,7 +354,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
             int c = q ? at1 : at;  // this tile's steps so far
 
             // ---- Q: a warp its 32 rows, 8 rows x 4 chunks of 8 coordinates at a time; a row scaled by a power of two of its own
-            // to at most 2^14 ----
+            // to at most 2^8 (so that the groups' sums beside it stay inside f16) ----
             float rowfac = 0.f;
             {
                 constexpr int NC = HD / 32;  // chunks of a row a lane reads
@@ -367,12 +392,13 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                         }
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
+                    const int e = mx > 0.f ? min(100, max(-100, 134 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
                     const float up = a.scale < 0.f ? -kt_pow2(e) : kt_pow2(e);
                     // a score in units of log2: the product with the widened keys times this and the step's power of two (a scale
                     // of 0 as 2^-100, so that the factor is positive)
                     const float fac = __shfl_sync(0xffffffffu, fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * kt_pow2(-e), lane & 7);
                     if (lane >> 3 == x) rowfac = fac;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};  // of the groups
 #pragma unroll
                     for (int y = 0; y < NC; y++) {
                         float v[8];
@@ -383,9 +409,24 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                         }
                         uint32_t h[4];
 #pragma unroll
-                        for (int z = 0; z < 4; z++) h[z] = kt_u32(__floats2half2_rn(v[z], v[z + 4]));
-                        *reinterpret_cast<uint4 *>(Qs + q * BQ * HD + kmajor_off(qrow, 32 * y + (lane >> 3) * 8, BQ)) = make_uint4(h[0], h[1], h[2], h[3]);
+                        for (int z = 0; z < 4; z++) {
+                            h[z] = kt_u32(__floats2half2_rn(v[z], v[z + 4]));
+                            const float2 f = __half22float2(kt_h2(h[z]));
+                            sum[y / UG] += f.x + f.y;
+                        }
+                        *reinterpret_cast<uint4 *>(Qs + q * BQ * HX + kmajor_off(qrow, 32 * y + (lane >> 3) * 8, BQ)) = make_uint4(h[0], h[1], h[2], h[3]);
                     }
+                    uint32_t both[4];  // a group's sum and what remains of it
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 8);
+                        sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 16);
+                        const float f = __half2float(__float2half_rn(sum[k]));
+                        both[k] = kt_u32(__floats2half2_rn(f, sum[k] - f));
+                    }
+                    if (lane < 16)  // as the keys' lows and steps lie: two groups in 8 columns
+                        *reinterpret_cast<uint4 *>(Qs + q * BQ * HX + kmajor_off(qrow, HD + (lane >> 3) * 8, BQ)) =
+                            lane < 8 ? make_uint4(both[0], both[0], both[1], both[1]) : make_uint4(both[2], both[2], both[3], both[3]);
                 }
                 fence_async_smem();
                 mbar_arrive(&mQ[q]);
@@ -400,7 +441,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 const uint32_t tsp = tmem + lane_base + KU_TS + (2 * q + (c & 1)) * BK;
                 if (!wait_warp(&mS[q][c & 1], (uint32_t)(c >> 1) & 1u)) break;
                 fence_after_sync();
-                const float c1 = rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_T);
+                const float c1 = rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_TK);
                 const int e = *reinterpret_cast<volatile int *>(&teV[x8]);
                 const bool edge = key0 < lo_max || key0 + BK > hi_min;
                 // Two passes over the step's scores in tensor memory, 32 at a time in loops that are not unrolled further: the code
@@ -495,7 +536,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     for (int x = 0; x < 4; x++) {
                         v[x] = L != 0.f ? o[y + 2 * x] * inv : 0.f, v[x + 4] = L != 0.f ? o[y + 2 * x + 1] * inv : 0.f;
                     }
-                    uint16_t *to = reinterpret_cast<uint16_t *>(Qs) + q * BQ * HD + kmajor_off(row, 32 * b + y, BQ);
+                    uint16_t *to = reinterpret_cast<uint16_t *>(Qs) + q * BQ * HX + kmajor_off(row, 32 * b + y, BQ);
                     if (dtype == DT_F16)
                         store8<DT_F16>(reinterpret_cast<__half *>(to), true, v);
                     else
@@ -512,7 +553,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                                     (long long)(pl.head * each + orr % each) * a.o_head + (lane >> 3) * 8;
 #pragma unroll
                     for (int y = 0; y < HD / 32; y++) {
-                        const uint4 v = *reinterpret_cast<const uint4 *>(Qs + q * BQ * HD + kmajor_off(orow, 32 * y + (lane >> 3) * 8, BQ));
+                        const uint4 v = *reinterpret_cast<const uint4 *>(Qs + q * BQ * HX + kmajor_off(orow, 32 * y + (lane >> 3) * 8, BQ));
                         if (orow >= rows) continue;
                         if (wide_o) {
                             *reinterpret_cast<uint4 *>(dst + 32 * y) = v;

@@ -66,6 +66,21 @@ struct KtScale<true> {
         even = step * up * 16777216.f, odd = even * 0.0625f, low = l * up;
     }
 };
+// A word's eight codes less 8 as f16 pairs, exact: a code under the bits of 1024, or of 1024 sixteenths.
+__device__ __forceinline__ void kt_codes(uint32_t w, __half2 (&c)[4]) {
+    const uint32_t v = w >> 8;
+    const __half2 up = kt_h2(0x64086408u), sixteenth = kt_h2(0x2c002c00u), off = kt_h2(0xd480d480u);  // 1032, 1 / 16, -72
+    c[0] = __hsub2(kt_h2((w & 0x000f000fu) | 0x64006400u), up), c[1] = __hfma2(kt_h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, off);
+    c[2] = __hsub2(kt_h2((v & 0x000f000fu) | 0x64006400u), up), c[3] = __hfma2(kt_h2((v & 0x00f000f0u) | 0x64006400u), sixteenth, off);
+}
+// step * (code - 8) of a word's eight codes as the sum of two f16, each exact: the step's upper 7 bits and its lower 4.
+__device__ __forceinline__ void kt_exact(uint32_t w, __half2 step, __half *hi, __half *lo) {
+    const __half2 s1 = kt_h2(kt_u32(step) & 0xfff0fff0u), s2 = __hsub2(step, s1);
+    __half2 c[4];
+    kt_codes(w, c);
+    *reinterpret_cast<uint4 *>(hi) = make_uint4(kt_u32(__hmul2(c[0], s1)), kt_u32(__hmul2(c[1], s1)), kt_u32(__hmul2(c[2], s1)), kt_u32(__hmul2(c[3], s1)));
+    *reinterpret_cast<uint4 *>(lo) = make_uint4(kt_u32(__hmul2(c[0], s2)), kt_u32(__hmul2(c[1], s2)), kt_u32(__hmul2(c[2], s2)), kt_u32(__hmul2(c[3], s2)));
+}
 // A word's eight values as f16 (and what remains of them) into 16 bytes each.
 __device__ __forceinline__ void kt_widen(uint32_t w, const KtScale<false> &s, __half *hi, __half *) {
     const uint32_t v = w >> 8;

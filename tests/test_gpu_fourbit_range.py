@@ -110,3 +110,24 @@ def test_a_window_wider_than_any_sequence_hides_nothing(gpu, dtype, which):
         sync(gpu)
         assert torch.equal(out, want) and torch.equal(lse, want_lse), window
     check_many(c, dtype, q, rows, 0.1, True, 0, want, want_lse)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("width,group,rows,seqs,which", [(128, 32, 2, 5, "few"), (128, 32, 50, 10, "many"), (64, 64, 50, 10, "many"),
+                                                         (32, 32, 50, 10, "many")])
+def test_attend_lse_keeps_32_bits(gpu, dtype, width, group, rows, seqs, which):
+    """The log-sum-exp is f32 whatever the queries' type: keys of 21 bits or more and sums in f32, so a score is off by at
+    most 2^-20 of its sum of magnitudes, and log-sum-exp rounds a few times."""
+    n = 300
+    c = Cached(gpu, 32, [n] * seqs, 4, width, 64, group, spread=1.0)
+    assert kernels(c, dtype, rows, 8) == which
+    q = rounded(np.random.default_rng(3).normal(0, 1, (rows * seqs, 8, width)), DT[dtype][1])
+    scale = 1 / np.sqrt(width)
+    out, lse = c.attend(dtype, q, [rows] * seqs, scale, causal=True)
+    sync(gpu)
+    for s in range(seqs):
+        r = slice(s * rows, (s + 1) * rows)
+        _, _, want, reach = exact(q[r], c.k[s], c.v[s], scale, visible(rows, n, True, 0))
+        assert (np.abs(host(lse)[r] - want) <= 2.0**-20 * (reach + 1 + np.abs(want))).all()
+        # and as a whole: roundings of either sign, here held to a quarter of the worst
+        assert np.linalg.norm(host(lse)[r] - want) <= 2.0**-22 * np.linalg.norm(reach + 1 + np.abs(want))
