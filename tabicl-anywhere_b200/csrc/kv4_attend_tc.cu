@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                     __half *hi = Kring + sl * QS * BLOCK + kmajor_off(key, 8 * x, BK), *lo = hi + BLOCK;
 #pragma unroll
                     for (int u = 0; u < NU; u++) {
-                        KtScale<true> s;
+                        KtScale s;
                         const float2 f = __half22float2(kt_h2(kc[u / UG]));
                         s.set(f.x, f.y, kt_pow2(C::T - e[0]));
                         kt_widen(w[u], s, hi + kmajor_off(0, 32, BK) * u, lo + kmajor_off(0, 32, BK) * u);
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                             c = w[0];
                         else
                             c = __byte_perm(w[u / 2], w[NU / 2 + u / 2], u & 1 ? 0x7632 : 0x5410);
-                        KtScale<true> s;
+                        KtScale s;
                         const float2 f = __half22float2(kt_h2(vc[u / UG]));
                         s.set(f.x, f.y, kt_pow2(C::T - e[1]));
                         kt_widen(c, s, hi + mnmajor_off(32, 0, HD) * u, lo + mnmajor_off(32, 0, HD) * u);

@@ -8,17 +8,17 @@
 // blocks have those, and 16 columns beside the first the lows and 8 steps, which meet the sums of q over each group (as two
 // f16).
 // What bounds it is shared memory beside the instruction issue: a step's operands are some 290 KB read and written (2300
-// cycles at 128 bytes), the exponentials 1024 cycles (16 a cycle and SM), and a step takes about 2750. The two tiles have a
+// cycles at 128 bytes), the exponentials 1024 cycles (16 a cycle and SM), and a step takes about 2730. The two tiles have a
 // warpgroup each, and widening, which serves both, two that take the steps in turn. Keys rounded to one f16 took 2300 cycles
 // a step (0.40 ms for the prompt below, its lse 4e-6 off), as two f16 split in f32 2980. The products issued from one
 // diverged thread cost 500 cycles more, loops unrolled over a whole step (which the instruction caches do not hold beside
-// widening) 400. A prompt of 4096 bf16 tokens after 1000 cached ones, 32 heads of 128 on 8: 0.48 ms, 0.43 PFLOP/s.
+// widening) 400. A prompt of 4096 bf16 tokens after 1000 cached ones, 32 heads of 128 on 8: 0.475 ms, 0.43 PFLOP/s.
 //
 // A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8, so the output
 // in tensor memory is rarely rescaled. A step's keys and values are scaled by a power of two of their own that keeps them
-// inside f16, whatever the cache holds; the output is in units of the largest step's. Coordinates keep the order the codes
-// are unpacked in, (0, 4, 1, 5, 2, 6, 3, 7) of every eight: Q takes the same order, and the output's columns are put back
-// when they are written.
+// inside f16: beside a value of 2^16 one of 1 keeps its 11 bits, and any is held to 2^-33 of its step's largest. The output
+// is in units that follow the steps'. Coordinates keep the order the codes are unpacked in, (0, 4, 1, 5, 2, 6, 3, 7) of every
+// eight: Q takes the same order, and the output's columns are put back when they are written.
 #include <algorithm>
 
 #include "kv4_tc.cuh"
@@ -27,9 +27,9 @@ namespace tcu {
 
 constexpr int KU_R = 256, KU_BQ = 128, KU_BK = 64, KU_THREADS = 640;
 constexpr int KU_NK = 2, KU_NS = 3, KU_NR = 3;  // slots of widened keys, of widened values, of stored codes
-constexpr int KU_T = -5;   // widened values are below 2^T
-constexpr int KU_TK = 15;  // widened keys are below 2^TK
-constexpr int KU_X = 16;   // columns beside the coordinates in which the groups' lows meet the sums of q
+constexpr int KU_T = 15;    // widened keys and values are below 2^T
+constexpr int KU_LAG = 3;   // powers of two that a step's values may lie below the output's unit
+constexpr int KU_X = 16;    // columns beside the coordinates in which the groups' lows meet the sums of q
 constexpr uint32_t KU_TS = 0, KU_TO = 256;  // tensor memory: [tile][2 slots] of S / P, then [tile] of O
 
 template <int HD, int G>
@@ -275,13 +275,12 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     e[x] = m > 0.f ? min(40, (int)(__float_as_uint(m) >> 23) - 125) : 0;  // m < 2^(e - 1): a span, 15 steps, below 2^e
                 }
                 if (tid % 128 == 0) teK[i & 7] = e[0], teV[i & 7] = e[1], has_nan[i & 7] = any;
-                KtScale<false> vs[NG];
 #pragma unroll
                 for (int k = 0; k < NG; k++) {
-                    const float2 f = __half22float2(kt_h2(kc[k]));  // (in the step's unit from here on: exact, but for steps below 2^-28 of its largest)
-                    kc[k] = kt_u32(__floats2half2_rn(f.x * kt_pow2(KU_TK - e[0]), f.y * kt_pow2(KU_TK - e[0])));
-                    const float2 g = __half22float2(kt_h2(vc[k]));
-                    vs[k].set(g.x, g.y, kt_pow2(KU_T - e[1]));
+                    // in the step's unit from here on: exact, but for steps and lows below 2^-28 of its largest
+                    const float2 f = __half22float2(kt_h2(kc[k])), g = __half22float2(kt_h2(vc[k]));
+                    const float uk = kt_pow2(KU_T - e[0]), uv = kt_pow2(KU_T - e[1]);
+                    kc[k] = kt_u32(__floats2half2_rn(f.x * uk, f.y * uk)), vc[k] = kt_u32(__floats2half2_rn(g.x * uv, g.y * uv));
                 }
                 // (loops that are not unrolled over the halves: short code, see the softmax)
                 if (i >= NK) wait_warp(&mKfree[kl], ((uint32_t)(i / NK) & 1u) ^ 1u);
@@ -321,7 +320,8 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                             c = w[0];
                         else
                             c = __byte_perm(w[u / 2], w[NU / 2 + u / 2], u & 1 ? 0x7632 : 0x5410);
-                        kt_widen(c, vs[u / UG], to + mnmajor_off(32, 0, HD) * u, nullptr);
+                        const __half2 g = kt_h2(vc[u / UG]);
+                        kt_round(c, __low2half2(g), __high2half2(g), to + mnmajor_off(32, 0, HD) * u);
                     }
                 }
                 fence_async_smem();
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 const uint32_t tsp = tmem + lane_base + KU_TS + (2 * q + (c & 1)) * BK;
                 if (!wait_warp(&mS[q][c & 1], (uint32_t)(c >> 1) & 1u)) break;
                 fence_after_sync();
-                const float c1 = rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_TK);
+                const float c1 = rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_T);
                 const int e = *reinterpret_cast<volatile int *>(&teV[x8]);
                 const bool edge = key0 < lo_max || key0 + BK > hi_min;
                 // Two passes over the step's scores in tensor memory, 32 at a time in loops that are not unrolled further: the code
@@ -465,9 +465,12 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c1;
                 }
                 if (i == 0) unit = e;
-                if (__any_sync(0xffffffffu, mx > m + 8.f) || e > unit) {
+                // (the output's unit follows steps of much smaller values down too: weights scaled down for them would leave f16's
+                // normal numbers, f32 has room for whatever the output is then)
+                const bool other = e > unit || e < unit - KU_LAG;
+                if (__any_sync(0xffffffffu, mx > m + 8.f) || other) {
                     const float mnew = fmaxf(m, mx), f = m == -INFINITY ? 0.f : kt_ex2(m - mnew);
-                    const int unew = max(unit, e);
+                    const int unew = other ? e : unit;
                     if (i > 0) {  // O, once the product before has been added to it
                         if (!wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u)) break;
                         fence_after_sync();
@@ -485,7 +488,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                     }
                     l *= f, m = mnew, unit = unew;
                 }
-                // weights times 2^7 (up to 2^15), in units of the step's values
+                // weights times 2^7 (up to 2^15), in units of the step's values (which are at most LAG powers of two smaller)
                 const float mm = (m == -INFINITY ? 0.f : m) - 7.f - (float)(e - unit);
                 float part_sum[4] = {};
 #pragma unroll 1

@@ -48,46 +48,40 @@ __device__ __forceinline__ void kt_bar(int id, int threads) { asm volatile("bar.
 __device__ __forceinline__ __half2 kt_h2(uint32_t w) { return *reinterpret_cast<const __half2 *>(&w); }
 __device__ __forceinline__ uint32_t kt_u32(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
 
-// One group's scales for widening: value = code nibble as f16 * even (a byte's first nibble) or * odd (its second) + low.
-template <bool SPLIT>
-struct KtScale;
-template <>
-struct KtScale<false> {
-    __half2 even, odd, low;
-    __device__ __forceinline__ void set(float step, float l, float up) {
-        const float s = step * up * 16777216.f;
-        even = __float2half2_rn(s), odd = __float2half2_rn(s * 0.0625f), low = __float2half2_rn(l * up);
-    }
-};
-template <>
-struct KtScale<true> {
+// One group's scales for widening in f32: value = code nibble as f16 * even (a byte's first nibble) or * odd (its second) + low.
+struct KtScale {
     float even, odd, low;
     __device__ __forceinline__ void set(float step, float l, float up) {
         even = step * up * 16777216.f, odd = even * 0.0625f, low = l * up;
     }
 };
-// A word's eight codes less 8 as f16 pairs, exact: a code under the bits of 1024, or of 1024 sixteenths.
+// A word's eight codes, CENTRED: less 8, as f16 pairs, exact: a code under the bits of 1024, or of 1024 sixteenths. (A nibble
+// as a subnormal f16 would take no subtraction, but the step that it meets 24 powers of two more of f16's range.)
+template <bool CENTRED>
 __device__ __forceinline__ void kt_codes(uint32_t w, __half2 (&c)[4]) {
     const uint32_t v = w >> 8;
-    const __half2 up = kt_h2(0x64086408u), sixteenth = kt_h2(0x2c002c00u), off = kt_h2(0xd480d480u);  // 1032, 1 / 16, -72
+    // 1024 or 1032, 1 / 16, -64 or -72
+    const __half2 up = kt_h2(CENTRED ? 0x64086408u : 0x64006400u), sixteenth = kt_h2(0x2c002c00u), off = kt_h2(CENTRED ? 0xd480d480u : 0xd400d400u);
     c[0] = __hsub2(kt_h2((w & 0x000f000fu) | 0x64006400u), up), c[1] = __hfma2(kt_h2((w & 0x00f000f0u) | 0x64006400u), sixteenth, off);
     c[2] = __hsub2(kt_h2((v & 0x000f000fu) | 0x64006400u), up), c[3] = __hfma2(kt_h2((v & 0x00f000f0u) | 0x64006400u), sixteenth, off);
+}
+// A word's eight values, each rounded once to f16.
+__device__ __forceinline__ void kt_round(uint32_t w, __half2 step, __half2 low, __half *to) {
+    __half2 c[4];
+    kt_codes<false>(w, c);
+    *reinterpret_cast<uint4 *>(to) = make_uint4(kt_u32(__hfma2(c[0], step, low)), kt_u32(__hfma2(c[1], step, low)), kt_u32(__hfma2(c[2], step, low)),
+                                                kt_u32(__hfma2(c[3], step, low)));
 }
 // step * (code - 8) of a word's eight codes as the sum of two f16, each exact: the step's upper 7 bits and its lower 4.
 __device__ __forceinline__ void kt_exact(uint32_t w, __half2 step, __half *hi, __half *lo) {
     const __half2 s1 = kt_h2(kt_u32(step) & 0xfff0fff0u), s2 = __hsub2(step, s1);
     __half2 c[4];
-    kt_codes(w, c);
+    kt_codes<true>(w, c);
     *reinterpret_cast<uint4 *>(hi) = make_uint4(kt_u32(__hmul2(c[0], s1)), kt_u32(__hmul2(c[1], s1)), kt_u32(__hmul2(c[2], s1)), kt_u32(__hmul2(c[3], s1)));
     *reinterpret_cast<uint4 *>(lo) = make_uint4(kt_u32(__hmul2(c[0], s2)), kt_u32(__hmul2(c[1], s2)), kt_u32(__hmul2(c[2], s2)), kt_u32(__hmul2(c[3], s2)));
 }
-// A word's eight values as f16 (and what remains of them) into 16 bytes each.
-__device__ __forceinline__ void kt_widen(uint32_t w, const KtScale<false> &s, __half *hi, __half *) {
-    const uint32_t v = w >> 8;
-    *reinterpret_cast<uint4 *>(hi) = make_uint4(kt_u32(__hfma2(kt_h2(w & 0x000f000fu), s.even, s.low)), kt_u32(__hfma2(kt_h2(w & 0x00f000f0u), s.odd, s.low)),
-                                                kt_u32(__hfma2(kt_h2(v & 0x000f000fu), s.even, s.low)), kt_u32(__hfma2(kt_h2(v & 0x00f000f0u), s.odd, s.low)));
-}
-__device__ __forceinline__ void kt_widen(uint32_t w, const KtScale<true> &s, __half *hi, __half *lo) {
+// A word's eight values as f16, and what remains of them, into 16 bytes each.
+__device__ __forceinline__ void kt_widen(uint32_t w, const KtScale &s, __half *hi, __half *lo) {
     uint32_t h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {

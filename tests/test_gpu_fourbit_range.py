@@ -131,3 +131,35 @@ def test_attend_lse_keeps_32_bits(gpu, dtype, width, group, rows, seqs, which):
         assert (np.abs(host(lse)[r] - want) <= 2.0**-20 * (reach + 1 + np.abs(want))).all()
         # and as a whole: roundings of either sign, here held to a quarter of the worst
         assert np.linalg.norm(host(lse)[r] - want) <= 2.0**-22 * np.linalg.norm(reach + 1 + np.abs(want))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,which", [(3, "few"), (60, "many")])
+@pytest.mark.parametrize("big", [256.0, 4096.0, 60000.0])
+def test_attend_small_values_beside_a_large_one(gpu, dtype, rows, which, big):
+    """Values of size 1 beside large ones that a row does not see, or that lie in another group of its tokens' coordinates,
+    late in the sequence and early: as near as the type rounds, by each row's own values."""
+    n, seqs, heads, width, page, group = 200, 10, 4, 64, 64, 32
+    c = Cached(gpu, 33, [n] * seqs, heads, width, page, group)
+    assert kernels(c, dtype, rows, heads) == which
+    rng = np.random.default_rng(5)
+    k, v = rng.normal(0, 1, (2, n, heads, width))
+    v[n - 1] = big * rng.choice([-1, 1], (heads, width))       # seen by the last row only
+    for token in (10, n - rows - 5):
+        v[token, :, group:] = -big
+    set_tokens(c, k, v, page, group)
+    q = rounded(rng.normal(0, 1, (rows * seqs, heads, width)), DT[dtype][1])
+    scale = 0.25 / np.sqrt(width)
+    out, _ = c.attend(dtype, q, [rows] * seqs, scale, causal=True)
+    sync(gpu)
+    seen = visible(rows, n, True, 0)
+    for s in range(0, seqs, 3):
+        r = slice(s * rows, s * rows + rows - 1)
+        want, size, _, reach = exact(q[r], c.k[s], c.v[s], scale, seen[:-1])
+        got, want, size = host(out)[r, :, :group], want[..., :group], size[..., :group]
+        # a weight and a value round to 11 bits each, scores as in f32; values that the large one pushes below f16's normal
+        # numbers by 17 halves of its smallest step, which is 2^-37 of the largest value or less
+        tol = size * (2.0**-10 + np.expm1(2.0**-19 * reach))[..., None] + 2 * ULP[dtype] * np.abs(want) + 2.0**-33 * big
+        assert (np.abs(got - want) <= tol).all(), (s, np.abs(got - want).max())
+        off = np.linalg.norm(got - want) / np.linalg.norm(want)
+        assert off <= 2.0**-10 + ULP[dtype] + 2.0**-33 * big, off
