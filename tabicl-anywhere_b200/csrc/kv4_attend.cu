@@ -231,15 +231,18 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
     // the running state of a column, in units of 2^off: off = m - 7 + ve, m the column's reference (it moves only when a score
     // passes it by 8), 2^ve the largest value step so far or more. So a weight is at most 2^(15 - ve), and with its step at
     // most 2^15: inside f16, and 2^7 above where the largest would leave small ones the least room. bf16's weights are
-    // f16 before they meet their step too, so there ve stays at 0 or above.
+    // f16 before they meet their step too, so there `off` does not follow ve below 0; where it is below -6 the steps are taken
+    // 2^steps_up as large instead, up to 2^15 (values of 4e-6 would lose all but 7 bits), and so is the output.
     float m[NT][2], off_m[NT][2], bound[NT][2], l[NT][2], ls[NT][NG][2], o[NT][NU][2][4];
     float ol[NT][4] = {};  // sums of p low of group g, where they are taken as a matrix product
     constexpr bool LOW_MMA_V = LOW_MMA;
-    int ve = CENTRED ? -24 : 0;  // (steps are f16: at least 2^-24)
+    int ve = -24;  // (steps are f16: at least 2^-24)
     float vtop = pow2i(ve);
+    auto weight_unit = [](int e) { return CENTRED ? e : max(e, 0); };
+    auto steps_up = [](int e) { return CENTRED || e >= -6 ? 0 : min(-e, 15); };
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        off_m[nt][0] = off_m[nt][1] = (float)(ve - 7);
+        off_m[nt][0] = off_m[nt][1] = (float)(weight_unit(ve) - 7);
         m[nt][0] = m[nt][1] = bound[nt][0] = bound[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
         for (int k = 0; k < NG; k++) ls[nt][k][0] = ls[nt][k][1] = 0.f;
@@ -377,9 +380,12 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
 #pragma unroll
             for (int d = 1; d < 32; d *= 2) step_max = fmaxf(step_max, __shfl_xor_sync(0xffffffffu, step_max, d));
             int grow = 0;
+            float out_f = 1.f;
             if (step_max > vtop) {  // the next power of two above
                 const int e = (int)(__float_as_uint(step_max) >> 23) - 126;
-                grow = e - ve, ve = e, vtop = pow2i(e);
+                grow = weight_unit(e) - weight_unit(ve);
+                if (!CENTRED) out_f = pow2i(steps_up(e) - steps_up(ve));
+                ve = e, vtop = pow2i(e);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -391,14 +397,26 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
                     x = fmaxf(x * fq[nt][c], m[nt][c]);
                     bound[nt][c] = x == -INFINITY ? x : (x + 8.f) / fq[nt][c];
                     const float f = (x > m[nt][c] ? exp2_sfu(m[nt][c] - x) : 1.f) * pow2i(-grow);
-                    m[nt][c] = x, off_m[nt][c] = (x == -INFINITY ? 0.f : x) + (float)(ve - 7), l[nt][c] *= f, ol[nt][c] *= f;
+                    m[nt][c] = x, off_m[nt][c] = (x == -INFINITY ? 0.f : x) + (float)(weight_unit(ve) - 7), l[nt][c] *= f, ol[nt][c] *= f;
 #pragma unroll
                     for (int k = 0; k < NG; k++) ls[nt][k][c] *= f;
 #pragma unroll
                     for (int u = 0; u < NU; u++)
 #pragma unroll
-                        for (int i = 0; i < 2; i++) o[nt][u][i][c] *= f, o[nt][u][i][c + 2] *= f;
+                        for (int i = 0; i < 2; i++) o[nt][u][i][c] *= f * out_f, o[nt][u][i][c + 2] *= f * out_f;
                 }
+        }
+        if (!CENTRED && steps_up(ve)) {
+            const __half2 up = __floats2half2_rn(pow2i(steps_up(ve)), 1.f);
+#pragma unroll
+            for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int k = 0; k < NG; k++) {
+                        const __half2 x = __hmul2(*reinterpret_cast<const __half2 *>(&vs[kb][h][k]), up);
+                        vs[kb][h][k] = *reinterpret_cast<const uint32_t *>(&x);
+                    }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -486,7 +504,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
                             }
                         }
                 } else {
-                    // p and p * step each round to 11 bits, as the results do to 11 or 8
+                    // p and p * step each round to 11 bits, the results to 8
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const __half2 w = __low2half2(*reinterpret_cast<const __half2 *>(&vs[kb][h][k]));
@@ -520,7 +538,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
     __syncthreads();
     float *so = reinterpret_cast<float *>(sm);  // [warp][R][HD]
     float *sms = so + KA_WARPS * R * HD;        // [warp][R]{m, l}
-    constexpr float unv = UNIT;
+    const float unv = UNIT * pow2i(-steps_up(ve));
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll

@@ -163,3 +163,28 @@ def test_attend_small_values_beside_a_large_one(gpu, dtype, rows, which, big):
         assert (np.abs(got - want) <= tol).all(), (s, np.abs(got - want).max())
         off = np.linalg.norm(got - want) / np.linalg.norm(want)
         assert off <= 2.0**-10 + ULP[dtype] + 2.0**-33 * big, off
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,seqs,which", [(1, 3, "few"), (1, 100, "few"), (12, 40, "few"), (50, 40, "many")])
+@pytest.mark.parametrize("size", [1e-3, 1e-5, 4e-6])
+def test_attend_values_of_small_steps(gpu, dtype, rows, seqs, which, size):
+    """Values far below 1, down to steps among f16's smallest, under uneven weights: a share of their own size. (Many
+    sequences, here on the same pages, let a warp see many keys.)"""
+    n, heads, width, page, group = 4000, 2, 128, 64, 32
+    c = Cached(gpu, 34, [n], heads, width, page, group)
+    rng = np.random.default_rng(6)
+    k, v = rng.normal(0, 1, (2, n, heads, width))
+    set_tokens(c, k, v * size, page, group)
+    c.lens = [n] * seqs
+    c.table, c.lens_dev = c.table.repeat(seqs, 1).contiguous(), c.lens_dev.repeat(seqs)
+    assert kernels(c, dtype, rows, heads) == which
+    q = rounded(rng.normal(0, 2, (rows * seqs, heads, width)), DT[dtype][1])
+    out, _ = c.attend(dtype, q, [rows] * seqs, 1 / np.sqrt(width))
+    sync(gpu)
+    want, _, _, _ = exact(q, c.k[0], c.v[0], 1 / np.sqrt(width), np.ones((len(q), n), bool))
+    off = np.linalg.norm(host(out) - want) / np.linalg.norm(want)
+    # 16-bit types: a weight rounds to 11 bits, its product with the step or the value again, keys to 21 or more; f16 results
+    # below its normal numbers by half of 2^-24 besides. f32: 2^-20 each, sums of some ten steps
+    floor = 2.0**-25 * np.sqrt(want.size) / np.linalg.norm(want) if dtype == "f16" else 0.0
+    assert off <= {"f32": 1e-5, "f16": 2.0**-10 + 2.0**-11, "bf16": 2.0**-8}[dtype] + floor, off
