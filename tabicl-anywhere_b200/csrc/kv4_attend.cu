@@ -192,8 +192,9 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
                 }
             }
         }
-        // (a scale of 0 as 2^-100, so that the factor is positive: the scores' order is that of the products)
-        const float factor = fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * pow2i(-e) * UNIT;
+        // (a scale of 0 as 2^-100 and never less than the smallest normal number, so that the factor is positive: the scores'
+        // order is that of the products, and -infinity stays itself)
+        const float factor = fmaxf(fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * pow2i(-e) * UNIT, FLT_MIN);
 #pragma unroll
         for (int k = 0; k < NG; k++) {
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);

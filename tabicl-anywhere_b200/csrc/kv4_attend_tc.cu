@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 if (!wait_warp(&mS[sl], (uint32_t)(i / NS) & 1u)) break;
                 fence_after_sync();
                 const uint32_t tsp = tmem + lane_base + KT_TS + BK * sl;
-                const float c1 = rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[i & 7]) - C::T);
+                const float c1 = fmaxf(rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[i & 7]) - C::T), FLT_MIN);  // (positive: -infinity stays itself)
                 // Two passes over the step's scores in tensor memory, 32 at a time in loops that are not unrolled further (short code
                 // for the instruction caches, which all roles share). P goes where the scores were: of every 16 keys, hi and lo.
                 const bool edge = key0 < sp.lo_max || key0 + BK > sp.hi_min;

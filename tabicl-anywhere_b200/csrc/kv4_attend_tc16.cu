@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 const uint32_t tsp = tmem + lane_base + KU_TS + (2 * q + (c & 1)) * BK;
                 if (!wait_warp(&mS[q][c & 1], (uint32_t)(c >> 1) & 1u)) break;
                 fence_after_sync();
-                const float c1 = rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_T);
+                const float c1 = fmaxf(rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_T), FLT_MIN);  // (positive: -infinity stays itself)
                 const int e = *reinterpret_cast<volatile int *>(&teV[x8]);
                 const bool edge = key0 < lo_max || key0 + BK > hi_min;
                 // Two passes over the step's scores in tensor memory, 32 at a time in loops that are not unrolled further: the code

@@ -188,3 +188,19 @@ def test_attend_values_of_small_steps(gpu, dtype, rows, seqs, which, size):
     # below its normal numbers by half of 2^-24 besides. f32: 2^-20 each, sums of some ten steps
     floor = 2.0**-25 * np.sqrt(want.size) / np.linalg.norm(want) if dtype == "f16" else 0.0
     assert off <= {"f32": 1e-5, "f16": 2.0**-10 + 2.0**-11, "bf16": 2.0**-8}[dtype] + floor, off
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+def test_attend_scale_of_nothing(gpu, dtype, which):
+    """A scale of 0, or one that leaves scores of nothing, gives every seen key the same weight, whatever the queries' size."""
+    lens, rows = ([70, 9], 3) if which == "few" else ([70, 9] * 20, 45)
+    c = Cached(gpu, 35, lens, 1 if which == "few" else 4, 128, 32, 64)
+    assert kernels(c, dtype, rows, c.heads) == which
+    q = np.random.default_rng(2).normal(0, 1, (rows * len(lens), c.heads, 128))
+    sizes = [1.0, 2.0**-24] if dtype == "f16" else [1.0, 2.0**-40, 2.0**-90, 2.0**-124]
+    for size in sizes:
+        for scale in (0.0, 1e-30, -1e-38):
+            x = rounded(q * size, DT[dtype][1])
+            out, lse = c.attend(dtype, x, [rows] * len(lens), scale, causal=True)
+            sync(gpu)
+            check_many(c, dtype, x, rows, scale, True, 0, out, lse)
