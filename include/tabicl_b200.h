@@ -479,10 +479,11 @@ TCU_API int tcu_w4_linear_device(tcu_ctx *ctx, const tcu_w4 *w, int dtype, int r
                                  size_t work_bytes, void *stream);
 
 /* Rows of scores: out [rows][per_row] the log probability of each given label under the softmax of logits / temperature
- * (label -1: none, 0 is returned), entropy [rows] (may be NULL) in nats, and the `top` (0..32) classes of highest score,
+ * (a negative label: none, 0 is returned), entropy [rows] (may be NULL) in nats, and the `top` (0..32) classes of highest score,
  * equal scores by the lower class: top_ids and their log probabilities top_values [rows][top]. -infinity masks a class:
  * it is no alternative (id -1, value -infinity, where the others run out), and a row of nothing else gives -infinity for
- * its labels and entropy 0. A NaN or +infinity in a row makes its log probabilities and entropy NaN. */
+ * its labels and entropy 0. A NaN or +infinity in a row makes its log probabilities and entropy NaN. Temperatures from
+ * 5e-39 to 8e37. */
 TCU_API int tcu_label_logprobs_device(tcu_ctx *ctx, int dtype, const void *logits, int rows, int classes, int64_t stride,
                                       const int32_t *labels, int per_row, float *out, float *entropy, int top, float *top_values,
                                       int32_t *top_ids, double temperature, void *stream);

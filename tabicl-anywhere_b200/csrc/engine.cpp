@@ -3428,8 +3428,11 @@ int tcu_label_logprobs_device(tcu_ctx *ctx, int dtype, const void *logits, int r
         if (per_row < 0 || (per_row && rows && (!labels || !out))) fail(TCU_ERR_ARG, "label_logprobs: null labels or output");
         if (top < 0 || top > LOGPROB_MAX_TOP || (top && rows && (!top_values || !top_ids)))
             fail(TCU_ERR_ARG, "label_logprobs: 0.." + std::to_string(LOGPROB_MAX_TOP) + " alternatives, with their outputs");
-        if (!(temperature > 0) || !std::isfinite(temperature) || !std::isfinite((float)(1.0 / temperature)))
-            fail(TCU_ERR_ARG, "label_logprobs: temperature must be positive");
+        // (the kernels multiply by its reciprocal and by that times log2 e in f32: neither may overflow, nor be so small that
+        // a masked class's -infinity times it is not one)
+        if (!(temperature > 0) || !std::isfinite(temperature) || !std::isnormal((float)(1.0 / temperature)) ||
+            !std::isfinite((float)(1.0 / temperature) * 1.44269504088896340736f))
+            fail(TCU_ERR_ARG, "label_logprobs: temperature must be positive, and f32 must hold its reciprocal (5e-39 to 8e37)");
         if (rows == 0) return TCU_OK;
         if (!logits) fail(TCU_ERR_ARG, "label_logprobs: null logits");
         check_aligned("label_logprobs", "logits", logits, elem_size(dtype));

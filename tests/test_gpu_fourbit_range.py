@@ -204,3 +204,33 @@ def test_attend_scale_of_nothing(gpu, dtype, which):
             out, lse = c.attend(dtype, x, [rows] * len(lens), scale, causal=True)
             sync(gpu)
             check_many(c, dtype, x, rows, scale, True, 0, out, lse)
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-39, 3e-39, 1e38, 1e60, float("inf"), -1.0])
+def test_logprobs_refuse_a_temperature_beyond_f32(gpu, temperature):
+    """Temperatures whose reciprocal, or its product with log2 e, 32 bits do not hold."""
+    t = torch.zeros(64, device="cuda")
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    with pytest.raises(tcu.TcuError, match="temperature"):
+        gpu.label_logprobs(0, t.data_ptr(), 1, 4, 4, i.data_ptr(), 1, t.data_ptr() + 64, temperature=temperature, stream=1)
+
+
+@pytest.mark.parametrize("temperature", [1e-37, 1e-20, 1e20, 1e37])
+@pytest.mark.parametrize("classes", [7, 700])
+def test_logprobs_of_extreme_temperatures(gpu, classes, temperature):
+    """The largest alone where it is cold, every class that is not masked alike where it is hot."""
+    x = np.random.default_rng(3).normal(0, 3, (3, classes)).astype(np.float32)
+    x[0, ::3] = -np.inf
+    x[1, 1:] = -np.inf
+    labels = np.tile(np.array([[1, 0, 2]]), (3, 1))
+    out, ent, tv, ti = base.logprobs(gpu, "f32", x, labels, 3, temperature)
+    gpu.sync()
+    for r in range(3):
+        with np.errstate(over="ignore"):
+            o, e, v, i = plain.logprobs(x[r], labels[r], 3, temperature)
+            o, v = (np.where(np.abs(a) > np.finfo(np.float32).max, -np.inf, a) for a in (o, v))
+        assert np.array_equal(ti[r], i)
+        for got, want in ((out[r], o), (tv[r], v), (ent[r:r + 1], np.array([e]))):
+            fin = np.isfinite(want)
+            assert np.array_equal(got[~fin], want[~fin])
+            assert (np.abs(got - np.where(fin, want, 0))[fin] <= (2.0**-20 * (1 + np.abs(want)))[fin]).all()
