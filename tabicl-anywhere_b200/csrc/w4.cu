@@ -139,13 +139,12 @@ __device__ __forceinline__ float w4_fragment(const float (&v)[8], float up, uint
     for (int k = 0; k < QS; k++) h[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
     return s;
 }
-// The power of two that brings a row's largest magnitude into [2^13, 2^14), and what undoes it on the sums (with the codes'
-// unit).
-__device__ __forceinline__ constexpr float w4_unit(int qs) { return qs == 2 ? 1.f : 5.9604644775390625e-8f; }  // centred codes, or 2^-24
-template <int QS>
+__device__ __forceinline__ constexpr float w4_unit(int qs) { return qs == 2 ? 1.f : 5.9604644775390625e-8f; }  // the codes': centred, or 2^-24
+// The power of two that brings a row's largest magnitude into [2^13, 2^14) (below 2^-113 as near as f32 holds its inverse),
+// and what undoes it on the sums.
 __device__ __forceinline__ float w4_up(float mx, float &undo) {
-    const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
-    undo = __uint_as_float((uint32_t)(127 - e) << 23) / w4_unit(QS);
+    const int e = mx > 0.f ? min(126, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff)) : 0;
+    undo = __uint_as_float((uint32_t)(127 - e) << 23);
     return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 // Words of fragments and floats of sums of one block of 128 columns of 8 NT rows.
@@ -174,7 +173,7 @@ __global__ void __launch_bounds__(256) k_w4_x(W4Args a, int dtype, uint32_t *xf,
 #pragma unroll
     for (int w = 0; w < 8; w++) mx = fmaxf(mx, red[w]);
     float undo;
-    const float up = w4_up<QS>(mx, undo);
+    const float up = w4_up(mx, undo);
     if (threadIdx.x == 0) fx[rt * R + m] = undo;
     for (int i0 = 0; i0 < blocks * 16; i0 += 256) {
         const int i = i0 + threadIdx.x, b = i / 16, u = i % 16 / 4, q = i % 4;
@@ -312,7 +311,7 @@ __global__ void __launch_bounds__(W4_WARPS * 32, NT < 8 ? 2 : 1) k_w4_linear(W4A
 #pragma unroll
                     for (int j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(v[x][j]));
                 float undo;
-                const float up = w4_up<QS>(warp_max(mx), undo);
+                const float up = w4_up(warp_max(mx), undo);
                 if (lane == 0) fx[warp] = undo;
 #pragma unroll
                 for (int x = 0; x < W4_SLICE / 2; x++) {
@@ -391,7 +390,7 @@ __global__ void __launch_bounds__(W4_WARPS * 32, NT < 8 ? 2 : 1) k_w4_linear(W4A
                     for (int c = 0; c < 4; c++) {
                         const int m = nt * 8 + 2 * t + (c & 1);
                         float *at = yb + m * 16 + (c >> 1) * 8 + g;
-                        const float v = y[nt][c] * fx[m];
+                        const float v = y[nt][c] * (1.f / w4_unit(QS)) * fx[m];
                         *at = b0 == b_lo ? v : *at + v;
                     }
                 in = 0, unit += W4_WARPS;

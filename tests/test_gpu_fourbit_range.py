@@ -234,3 +234,22 @@ def test_logprobs_of_extreme_temperatures(gpu, classes, temperature):
             fin = np.isfinite(want)
             assert np.array_equal(got[~fin], want[~fin])
             assert (np.abs(got - np.where(fin, want, 0))[fin] <= (2.0**-20 * (1 + np.abs(want)))[fin]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 5, 20])
+@pytest.mark.parametrize("size", [2.0**118, 2.0**102, 2.0**-100, 2.0**-118])
+def test_linear_of_very_large_and_small_inputs(gpu, dtype, rows, size):
+    """Inputs near the ends of the type whose outputs it holds."""
+    code, tt = DT[dtype]
+    rng = np.random.default_rng(rows)
+    n, k = 70, 300
+    w4, keep, w = weights(rng, gpu, n, k, 64, dtype)
+    x = rounded(rng.normal(0, 1, (rows, k)) * size, tt)
+    xd, yd = dev(x, tt), torch.full((rows, n), 9.0, dtype=tt, device="cuda")
+    work = torch.zeros(max(16, w4.linear_workspace(rows, code)), dtype=torch.uint8, device="cuda")
+    w4.linear(code, rows, xd.data_ptr(), k, yd.data_ptr(), n, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    y = x.astype(np.float64) @ w.T
+    tol = 2.0**-20 * (np.abs(x.astype(np.float64)) @ np.abs(w).T) + 2 * ULP[dtype] * np.abs(y)
+    assert (np.abs(yd.double().cpu().numpy() - y) <= tol).all()
