@@ -70,7 +70,7 @@ __device__ __forceinline__ float exp2_sfu(float x) {  // relative error 2^-22; 0
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| < 127
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -127 < e < 128
 
 // TYPE: the queries' type. f32: q and the weights as two f16, else as one; bf16: codes as they are, and the weights' products
 // with their steps in f16 pairs, each rounded to the 11 bits that 8-bit results do not show.
@@ -171,8 +171,8 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        // mx * 2^e in [2^13, 2^14); queries above 2^114 pass f16 (their scores pass f32)
-        const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
+        // mx * 2^e in [2^13, 2^14) (below 2^-113 as near as f32 holds 2^-e)
+        const int e = mx > 0.f ? min(126, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff)) : 0;
         const float up = pow2i(e);
         float sum[NG] = {};
 #pragma unroll
@@ -192,9 +192,9 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
                 }
             }
         }
-        // (a scale of 0 as 2^-100 and never less than the smallest normal number, so that the factor is positive: the scores'
-        // order is that of the products, and -infinity stays itself)
-        const float factor = fmaxf(fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * pow2i(-e) * UNIT, FLT_MIN);
+        // (held to the normal numbers: positive for a scale of 0 too, so that the scores' order is that of the products and
+        // -infinity stays itself)
+        const float factor = fminf(fmaxf(fabsf(a.scale) * 1.44269504088896340736f * pow2i(-e) * UNIT, FLT_MIN), FLT_MAX);
 #pragma unroll
         for (int k = 0; k < NG; k++) {
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);

@@ -114,11 +114,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
         qmax[wg][row] = mx;
         kt_bar(2, 256);
         mx = fmaxf(qmax[0][row], qmax[1][row]);
-        const int e = mx > 0.f ? min(100, max(-100, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
+        const int e = mx > 0.f ? min(126, 140 - (int)((__float_as_uint(mx) >> 23) & 0xff)) : 0;
         const float up = a.scale < 0.f ? -kt_pow2(e) : kt_pow2(e);
-        // a score in units of log2: the product with the widened keys times this and the step's power of two (a scale
-        // of 0 as 2^-100, so that the factor is positive)
-        const float rowfac = fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * kt_pow2(-e);
+        // a score in units of log2: the product with the widened keys times this and the step's power of two
+        const float rowfac = fabsf(a.scale) * 1.44269504088896340736f * kt_pow2(-e);
         uint32_t hi[H / 2], lo[H / 2];
 #pragma unroll
         for (int b = 0; b < H / 8; b++)
@@ -373,7 +372,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) k_kv4_attend_tc(Kv4AttendArgs a
                 if (!wait_warp(&mS[sl], (uint32_t)(i / NS) & 1u)) break;
                 fence_after_sync();
                 const uint32_t tsp = tmem + lane_base + KT_TS + BK * sl;
-                const float c1 = fmaxf(rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[i & 7]) - C::T), FLT_MIN);  // (positive: -infinity stays itself)
+                // (held to the normal numbers: positive for a scale of 0 too, so that -infinity stays itself)
+                const float c1 = fminf(fmaxf(rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[i & 7]) - C::T), FLT_MIN), FLT_MAX);
                 // Two passes over the step's scores in tensor memory, 32 at a time in loops that are not unrolled further (short code
                 // for the instruction caches, which all roles share). P goes where the scores were: of every 16 keys, hi and lo.
                 const bool edge = key0 < sp.lo_max || key0 + BK > sp.hi_min;

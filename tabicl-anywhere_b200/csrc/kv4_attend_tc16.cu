@@ -392,11 +392,10 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                         }
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const int e = mx > 0.f ? min(100, max(-100, 134 - (int)((__float_as_uint(mx) >> 23) & 0xff))) : 0;
+                    const int e = mx > 0.f ? min(126, 134 - (int)((__float_as_uint(mx) >> 23) & 0xff)) : 0;
                     const float up = a.scale < 0.f ? -kt_pow2(e) : kt_pow2(e);
-                    // a score in units of log2: the product with the widened keys times this and the step's power of two (a scale
-                    // of 0 as 2^-100, so that the factor is positive)
-                    const float fac = __shfl_sync(0xffffffffu, fmaxf(fabsf(a.scale), 7.8886e-31f) * 1.44269504088896340736f * kt_pow2(-e), lane & 7);
+                    // a score in units of log2: the product with the widened keys times this and the step's power of two
+                    const float fac = __shfl_sync(0xffffffffu, fabsf(a.scale) * 1.44269504088896340736f * kt_pow2(-e), lane & 7);
                     if (lane >> 3 == x) rowfac = fac;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};  // of the groups
 #pragma unroll
@@ -441,7 +440,8 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                 const uint32_t tsp = tmem + lane_base + KU_TS + (2 * q + (c & 1)) * BK;
                 if (!wait_warp(&mS[q][c & 1], (uint32_t)(c >> 1) & 1u)) break;
                 fence_after_sync();
-                const float c1 = fmaxf(rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_T), FLT_MIN);  // (positive: -infinity stays itself)
+                // (held to the normal numbers: positive for a scale of 0 too, so that -infinity stays itself)
+                const float c1 = fminf(fmaxf(rowfac * kt_pow2(*reinterpret_cast<volatile int *>(&teK[x8]) - KU_T), FLT_MIN), FLT_MAX);
                 const int e = *reinterpret_cast<volatile int *>(&teV[x8]);
                 const bool edge = key0 < lo_max || key0 + BK > hi_min;
                 // Two passes over the step's scores in tensor memory, 32 at a time in loops that are not unrolled further: the code

@@ -19,7 +19,7 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
     return p != 0;
 }
-__device__ __forceinline__ float kt_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // |e| < 127
+__device__ __forceinline__ float kt_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -127 < e < 128
 __device__ __forceinline__ float kt_ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

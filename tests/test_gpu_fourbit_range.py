@@ -253,3 +253,17 @@ def test_linear_of_very_large_and_small_inputs(gpu, dtype, rows, size):
     y = x.astype(np.float64) @ w.T
     tol = 2.0**-20 * (np.abs(x.astype(np.float64)) @ np.abs(w).T) + 2 * ULP[dtype] * np.abs(y)
     assert (np.abs(yd.double().cpu().numpy() - y) <= tol).all()
+
+
+@pytest.mark.parametrize("dtype,which", [("f32", "few"), ("bf16", "few"), ("f32", "many"), ("bf16", "many")])
+@pytest.mark.parametrize("size", [2.0**118, 2.0**-118])
+def test_attend_queries_of_very_large_and_small_size(gpu, dtype, which, size):
+    """Queries near the ends of the type with a scale that brings their scores back."""
+    lens, rows = ([70, 9], 3) if which == "few" else ([70, 9] * 20, 45)
+    c = Cached(gpu, 36, lens, 1 if which == "few" else 4, 128, 32, 64)
+    assert kernels(c, dtype, rows, c.heads) == which
+    q = rounded(np.random.default_rng(2).normal(0, 1, (rows * len(lens), c.heads, 128)) * size, DT[dtype][1])
+    scale = float(np.float32(0.09 / size))
+    out, lse = c.attend(dtype, q, [rows] * len(lens), scale, causal=True)
+    sync(gpu)
+    check_many(c, dtype, q, rows, scale, True, 0, out, lse)
