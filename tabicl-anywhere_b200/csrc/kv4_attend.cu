@@ -24,7 +24,7 @@ namespace tcu {
 constexpr int KA_KEYS = 32;     // keys of a warp's step
 constexpr int KA_WARPS = 4;     // warps of a block, each over its own steps of the block's keys
 constexpr int KA_STEP = KA_WARPS * KA_KEYS;  // keys of a block's step
-constexpr int KA_TRIES = 1 << 20;  // waits for a copy (each suspends the warp for a while) before a warp gives up
+constexpr long long KA_WAIT = 2000000000ll;  // a warp gives up a copy after about a second at boost clock
 
 template <int HD, int G>
 struct KaTile {
@@ -43,6 +43,19 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void *src, uint32_
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
                  "r"(bytes), "r"(bar)
                  : "memory");
+}
+// Waits for the barrier's phase; false after KA_WAIT.
+__device__ __forceinline__ bool ka_wait(uint32_t bar, uint32_t parity) {
+    auto done = [&] {
+        uint32_t p;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p) : "r"(bar), "r"(parity) : "memory");
+        return p != 0;
+    };
+    if (done()) return true;
+    const long long t0 = clock64();
+    while (!done())
+        if (clock64() - t0 > KA_WAIT) return false;
+    return true;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -103,6 +116,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
     }
     __syncwarp();
     uint32_t used = 0;  // steps of this warp so far: the ring's place and the barriers' phases
+    bool gave_up = false;  // a copy did not come: the warp reads no more
     const size_t hb = kv4_head_bytes(HD, a.c.page, G);
     const Kv4Offsets off = kv4_offsets(HD, a.c.page, G);
     const int page_shift = 31 - __clz(a.c.page), halves = a.c.page == 16 ? 2 : 1;
@@ -117,7 +131,7 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
     const int piece = (int)min((long long)(sp.steps - skip), pl.end - pl.pos), rows = min(R, sr.n * each - r0);
     const int lo_min = sp.lo_min, lo_max = sp.lo_max, hi_min = sp.hi_min, hi_max = sp.hi_max;
     const int k0 = sp.base + skip * KA_STEP, k1 = hi_max > lo_min ? min(hi_max, k0 + piece * KA_STEP) : k0;
-    const int ntiles = (k1 - k0 + KA_KEYS - 1) / KA_KEYS, mine = max(0, (ntiles - warp + KA_WARPS - 1) / KA_WARPS);
+    const int ntiles = (k1 - k0 + KA_KEYS - 1) / KA_KEYS, mine = gave_up ? 0 : max(0, (ntiles - warp + KA_WARPS - 1) / KA_WARPS);
     // the page numbers are read a step before they are needed
     int pages[2];
     auto find = [&](int it) {
@@ -253,18 +267,13 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
             for (int x = 0; x < 8; x++) o[nt][u][x >> 2][x & 3] = 0.f;
     }
 
-    bool gave_up = false;
     for (int it = 0; it < mine; it++) {
         load(it + ST - 1);
-        {
-            const uint32_t bar = bar_at + 8 * ((used + it) % ST), parity = ((used + it) / ST) & 1;
-            uint32_t done = 0;
-            for (int tries = 0; !done && tries < KA_TRIES; tries++)
-                asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-            if (__any_sync(0xffffffffu, !done)) {
-                gave_up = true;
-                break;
-            }
+        if (__any_sync(0xffffffffu, !ka_wait(bar_at + 8 * ((used + it) % ST), ((used + it) / ST) & 1))) {
+            // copies on their way land before the memory holds anything else, or the block leaves it
+            for (int x = it; x < min(mine, it + ST); x++) ka_wait(bar_at + 8 * ((used + x) % ST), ((used + x) / ST) & 1);
+            gave_up = true;
+            break;
         }
         const uint8_t *tile = ring + (used + it) % ST * C::BYTES;
         const int j0 = k0 + (warp + it * KA_WARPS) * KA_KEYS;
