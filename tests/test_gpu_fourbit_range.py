@@ -267,3 +267,324 @@ def test_attend_queries_of_very_large_and_small_size(gpu, dtype, which, size):
     out, lse = c.attend(dtype, q, [rows] * len(lens), scale, causal=True)
     sync(gpu)
     check_many(c, dtype, q, rows, scale, True, 0, out, lse)
+
+
+# ---- each kernel of attention at the masks, orders, places and values where it could go wrong --------------------------
+
+def check_rows(c, dtype, group, q, counts, scale, causal, window, out, lse, leave=()):
+    """Every row by its own values: 16-bit types round a weight and its product with a step or a value to 11 bits each, f32
+    to 21 or more; a code's part of a value is as large as its group's span; scores and sums are f32. Sequences in `leave`
+    are not looked at."""
+    out, lse, at = host(out), host(lse), 0
+    two = 2.0**-10 if dtype != "f32" else 2.0**-19
+    off = ref = 0.0
+    for s, n in enumerate(counts):
+        if not n:
+            continue
+        r = slice(at, at + n)
+        at += n
+        if s in leave:
+            continue
+        k, v = c.k[s], c.v[s]
+        seen = visible(n, c.lens[s], causal, window)
+        if not c.lens[s]:
+            assert not out[r].any() and (lse[r] == -np.inf).all()
+            continue
+        want, _, l, reach = exact(q[r], k, v, scale, seen)
+        g = v.reshape(*v.shape[:-1], -1, group)
+        span = np.repeat(g.max(-1) - g.min(-1), group, -1)
+        _, size, _, _ = exact(q[r], k, np.abs(v) + span, scale, seen)
+        none = ~np.isfinite(l)
+        assert (lse[r][none] == -np.inf).all() and not out[r][none].any()
+        with np.errstate(over="ignore"):
+            tol = size * (two + np.expm1(2.0**-19 * reach))[..., None] + 2 * ULP[dtype] * np.abs(want) + 1e-30
+        assert (np.abs(out[r] - want) <= tol).all(), (s, np.abs(out[r] - want).max())
+        some = ~none
+        assert (np.abs(lse[r] - l)[some] <= (2.0**-20 * (reach + 1 + np.abs(np.where(some, l, 0))))[some]).all(), s
+        off, ref = off + np.sum((out[r] - want) ** 2), ref + np.sum(want**2)
+    # roundings of either sign: as a whole a share of the result
+    assert off <= {"f32": 1e-5, "f16": 2.0**-10, "bf16": 2.0**-8}[dtype] ** 2 * ref, (off / ref) ** 0.5
+
+
+def shape_of(which):
+    """Sequences, heads and most rows that reach the kernel at width 128."""
+    return (4, 2, 7) if which == "few" else (40, 4, 47)
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_attend_counts_its_keys(gpu, dtype, which, page):
+    """All scores equal, and the values one-hot: an output is the number of seen tokens with that coordinate over the number
+    of all, so one key too many or too few at either end of a mask moves it by a part of eight or more."""
+    seqs, heads, rows = shape_of(which)
+    width, group = 128, 32
+    lens = [n for _ in range(seqs) for n in (0, 1, 46, 47, 64, 200, 333, 512)][:seqs]
+    c = Cached(gpu, 40, lens, heads, width, page, group)
+    assert kernels(c, dtype, rows, heads) == which
+    n = max(lens)
+    v = np.zeros((n, heads, width))
+    v[np.arange(n), :, np.arange(n) % width] = 1.0
+    rng = np.random.default_rng(1)
+    cut = np.cumsum([0] + lens)
+    all_v, all_k = np.concatenate([v[:m] for m in lens]), rng.normal(0, 1, (cut[-1], heads, width))
+    table = c.table.cpu().numpy()
+    slots = [int(table[s, j // page]) * page + j % page for s in range(seqs) for j in range(lens[s])]
+    raw, kk, vv = plain.pool_of(all_k.astype(np.float32), all_v.astype(np.float32), slots, c.pages, page, group, 0xFF)
+    c.pool.copy_(dev(raw))
+    one = vv.max()
+    q = np.zeros((rows * seqs, heads, width), np.float32)
+    for causal, window in ((False, 0), (True, 0), (True, 1), (True, 31), (True, 63), (True, 64), (True, 65), (True, 300)):
+        out, lse = (host(t) for t in c.attend(dtype, q, [rows] * seqs, 0.1, causal, window))
+        sync(gpu)
+        for s in range(seqs):
+            seen = visible(rows, lens[s], causal, window)
+            total = np.maximum(seen.sum(1), 1)
+            per = np.zeros((rows, width))
+            for j in range(lens[s]):
+                per[:, j % width] += seen[:, j]
+            r = slice(s * rows, (s + 1) * rows)
+            want = (per * one / total[:, None])[:, None]
+            assert (np.abs(out[r] - want) <= 0.1 / total[:, None, None] + 2.0**-8 * want).all(), (causal, window, s)
+            with np.errstate(divide="ignore"):
+                l = np.log(seen.sum(1).astype(float))[:, None]
+            assert (np.abs(lse[r] - l)[seen.any(1)] <= 2.0**-19 * (1 + l[seen.any(1)])).all() and (lse[r][~seen.any(1)] == -np.inf).all()
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+def test_attend_ragged_rows_on_each_kernel(gpu, dtype, which):
+    seqs, heads, rows = shape_of(which)
+    lens = [n for _ in range(seqs) for n in (120, 60, 0, 200)][:seqs]
+    counts = [n for _ in range(seqs) for n in (rows, 0, 3, rows - 1)][:seqs]
+    c = Cached(gpu, 41, lens, heads, 128, 32, 64)
+    assert kernels(c, dtype, rows, 3 * heads) == which
+    q = rounded(np.random.default_rng(2).normal(0, 1, (sum(counts), 3 * heads, 128)), DT[dtype][1])
+    for window in (0, 33):
+        out, lse = c.attend(dtype, q, counts, 0.088, causal=True, window=window, ragged=True)
+        sync(gpu)
+        check_rows(c, dtype, 64, q, counts, 0.088, True, window, out, lse)
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+@pytest.mark.parametrize("size", [6.0, 0.5])
+def test_attend_sharp_and_even_scores_on_each_kernel(gpu, dtype, which, size):
+    """Scores over a span of hundreds, growing along the sequence in places (references move), and nearly even ones."""
+    seqs, heads, rows = shape_of(which)
+    c = Cached(gpu, 42, [333] * seqs, heads, 128, 64, 32)
+    assert kernels(c, dtype, rows, heads) == which
+    rng = np.random.default_rng(3)
+    k, v = rng.normal(0, 1, (2, 333, heads, 128))
+    k *= np.where(np.arange(333) % 100 > 70, np.arange(333) / 100.0, 0.3)[:, None, None]
+    set_tokens(c, k, v, 64, 32)
+    q = rounded(rng.normal(0, size, (rows * seqs, heads, 128)), DT[dtype][1])
+    out, lse = c.attend(dtype, q, [rows] * seqs, -0.0884, causal=True)
+    sync(gpu)
+    check_rows(c, dtype, 32, q, [rows] * seqs, -0.0884, True, 0, out, lse)
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+def test_attend_scores_up_to_two_to_the_23(gpu, dtype, which):
+    """Scores as large as f32 still resolves: the largest takes all."""
+    seqs, heads, rows = shape_of(which)
+    c = Cached(gpu, 43, [200] * seqs, heads, 128, 64, 32)
+    assert kernels(c, dtype, rows, heads) == which
+    q = rounded(np.random.default_rng(3).normal(0, 30, (rows * seqs, heads, 128)), DT[dtype][1])
+    scale = 2.0**23 / 3e3
+    out, lse = (host(t) for t in c.attend(dtype, q, [rows] * seqs, scale))
+    sync(gpu)
+    for s in range(0, seqs, 5):
+        for h in range(heads):
+            r = slice(s * rows, (s + 1) * rows)
+            x = q[r, h].astype(np.float64) @ c.k[s][:, h].T * scale
+            order = np.sort(x, 1)
+            sure = order[:, -1] - order[:, -2] > 2.0**-18 * np.abs(x).max()  # of scores nearer than they round either may win
+            best, v = x.argmax(1), c.v[s][:, h]
+            assert sure.sum() > rows / 2 and np.abs(x).max() < 2.0**24
+            assert (np.abs(lse[r, h] - order[:, -1]) <= 2.0**-19 * np.abs(q[r, h]).astype(np.float64) @ np.abs(c.k[s][:, h]).T.max(1) * scale).all()
+            assert (np.abs(out[r, h] - v[best]) <= 2.0**-9 * (4 + np.abs(v[best])) + 2 * ULP[dtype] * np.abs(v[best]))[sure].all()
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+def test_attend_values_of_many_sizes_on_each_kernel(gpu, dtype, which):
+    """Tokens whose values go from 1e-4 to 1e4, keys over three powers of ten."""
+    seqs, heads, rows = shape_of(which)
+    c = Cached(gpu, 44, [400] * seqs, heads, 128, 16, 32)
+    assert kernels(c, dtype, rows, heads) == which
+    rng = np.random.default_rng(4)
+    k = rng.normal(0, 1, (400, heads, 128)) * 10.0 ** rng.uniform(-3, 0, (400, 1, 1))
+    v = rng.normal(0, 1, (400, heads, 128)) * 10.0 ** rng.uniform(-4, 4, (400, 1, 1))
+    set_tokens(c, k, v, 16, 32)
+    q = rounded(rng.normal(0, 1, (rows * seqs, heads, 128)), DT[dtype][1])
+    out, lse = c.attend(dtype, q, [rows] * seqs, 0.088, causal=True)
+    sync(gpu)
+    check_rows(c, dtype, 32, q, [rows] * seqs, 0.088, True, 0, out, lse)
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+@pytest.mark.parametrize("width", [64, 128])
+def test_attend_strides_and_orders_on_each_kernel(gpu, dtype, which, width):
+    """Queries and outputs by row and by head, at odd places of wider buffers; the same call again gives the same bits, and
+    nothing beside the outputs is written."""
+    if dtype == "f32" and width == 64:
+        width = 128
+    code, tt = DT[dtype]
+    seqs, heads, rows = shape_of(which)
+    c = Cached(gpu, 45, [150] * seqs, heads, width, 64, 32)
+    assert kernels(c, dtype, rows, heads) == which
+    q = rounded(np.random.default_rng(3).normal(0, 1, (rows * seqs, heads, width)), tt)
+    n, w = rows * seqs, width
+    batch = c.cache.batch(seqs, rows, 150, c.lens_dev.data_ptr(), c.table.data_ptr(), c.stride)
+    work = torch.zeros(max(16, c.cache.attend_workspace(batch, heads, code)), dtype=torch.uint8, device="cuda")
+    for row, head, lead in ((heads * (w + 3), w + 3, 1), (w, n * w, 0), (w + 1, n * (w + 1), 5), (heads * w + 8, w, 8)):
+        total = (n - 1) * row + (heads - 1) * head + w + lead + 9
+        wide, outs = torch.full((total,), 3e4, dtype=tt, device="cuda"), []
+        torch.as_strided(wide, (n, heads, w), (row, head, 1), lead).copy_(dev(q, tt))
+        for _ in range(2):
+            o = torch.full((total,), 9.0, dtype=tt, device="cuda")
+            at = lead * o.element_size()
+            c.cache.attend(batch, code, heads, wide.data_ptr() + at, row, head, o.data_ptr() + at, row, head, 0.1,
+                           work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+            sync(gpu)
+            outs.append(o)
+        assert torch.equal(outs[0], outs[1])
+        got = torch.as_strided(outs[0], (n, heads, w), (row, head, 1), lead).clone()
+        torch.as_strided(outs[0], (n, heads, w), (row, head, 1), lead).fill_(9.0)
+        assert bool((outs[0] == 9).all())
+        if lead == 1:
+            _, lse = c.attend(dtype, q, [rows] * seqs, 0.1)
+            sync(gpu)
+            check_rows(c, dtype, 32, q, [rows] * seqs, 0.1, False, 0, got, lse)
+            first = got
+        assert torch.equal(got, first)
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+def test_attend_past_four_gigabytes_on_each_kernel(gpu, dtype, which):
+    seqs, heads, rows = shape_of(which)
+    page, group = 64, 32
+    c = Cached(gpu, 46, [150] * seqs, heads, 128, page, group, extra=0)
+    assert kernels(c, dtype, rows, heads) == which
+    size = tcu.Kv4Cache.page_bytes(heads, 128, page, group)
+    pages = (9 << 30) // 2 // size + c.pages
+    pool = torch.empty(pages, size, dtype=torch.uint8, device="cuda")
+    pool[-c.pages:] = c.pool
+    c.table[c.table >= 0] += pages - c.pages
+    c.cache = tcu.Kv4Cache(gpu, pool.data_ptr(), pages, heads=heads, width=128, page=page, group=group)
+    q = rounded(np.random.default_rng(3).normal(0, 1, (rows * seqs, heads, 128)), DT[dtype][1])
+    out, lse = c.attend(dtype, q, [rows] * seqs, 0.09, causal=True)
+    sync(gpu)
+    check_rows(c, dtype, group, q, [rows] * seqs, 0.09, True, 0, out, lse)
+
+
+@pytest.mark.parametrize("dtype,which", BOTH)
+def test_attend_reports_indexes_on_each_kernel(gpu, dtype, which):
+    """A page, length or start outside its range is reported once, other sequences' rows are what they are."""
+    seqs, heads, rows = shape_of(which)
+
+    def call(change, bad, ragged=False):
+        c = Cached(gpu, 47, [100, 70] * (seqs // 2), heads, 128, 32, 64)
+        assert kernels(c, dtype, rows, heads) == which
+        q = rounded(np.random.default_rng(3).normal(0, 1, (rows * seqs, heads, 128)), DT[dtype][1])
+        starts = torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * rows
+        change(c, starts)
+        if ragged:
+            code = DT[dtype][0]
+            qd, out = dev(q, DT[dtype][1]), torch.full(q.shape, 9.0, dtype=DT[dtype][1], device="cuda")
+            lse = torch.full(q.shape[:2], 9.0, device="cuda")
+            b = c.cache.batch(seqs, rows, 101, c.lens_dev.data_ptr(), c.table.data_ptr(), c.stride, starts.data_ptr(), rows * seqs)
+            work = torch.zeros(max(16, c.cache.attend_workspace(b, heads, code)), dtype=torch.uint8, device="cuda")
+            c.cache.attend(b, code, heads, qd.data_ptr(), heads * 128, 128, out.data_ptr(), heads * 128, 128, 0.1, causal=True,
+                           lse=lse.data_ptr(), work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+        else:
+            out, lse = c.attend(dtype, q, [rows] * seqs, 0.1, causal=True)
+        torch.cuda.synchronize()
+        with pytest.raises(tcu.TcuError, match="outside its range"):
+            gpu.sync()
+        gpu.sync()
+        check_rows(c, dtype, 64, q, [rows] * seqs, 0.1, True, 0, out, lse, bad)
+
+    call(lambda c, st: c.table[0, 1].fill_(c.pages), [0])
+    call(lambda c, st: c.table[1, 0].fill_(-5), [1])
+    call(lambda c, st: c.lens_dev[0].fill_(101), [0])
+    call(lambda c, st: c.lens_dev[1].fill_(-1), [1])
+    call(lambda c, st: st[seqs].fill_(rows * seqs + 1), [seqs - 1], True)
+    call(lambda c, st: st[0].fill_(-1), [0], True)
+
+
+def test_working_memory_serves_every_kernel_in_turn(gpu):
+    """One block for calls of every kernel and type, whose units are cut differently, in turn."""
+    shapes = [("bf16", [5000], 1, 1, [1]), ("f32", [4000], 4, 8, [1100]), ("f16", [4000], 4, 8, [1100]), ("f32", [3000], 2, 8, [2]),
+              ("bf16", [300] * 40, 4, 4, [47] * 40), ("f32", [300] * 40, 4, 4, [47] * 40), ("f16", [2000], 1, 8, [3])]
+    calls = []
+    for i, (dtype, lens, heads, hq, counts) in enumerate(shapes):
+        c = Cached(gpu, i, lens, heads, 128, 64, 32)
+        q = rounded(np.random.default_rng(i).normal(0, 1, (sum(counts), hq, 128)), DT[dtype][1])
+        calls.append((c, dtype, q, counts, c.attend(dtype, q, counts, 0.1, causal=True)))
+    work = torch.zeros(64 << 20, dtype=torch.uint8, device="cuda")
+    for turn in range(2):
+        for c, dtype, q, counts, want in calls if turn else reversed(calls):
+            got = c.attend(dtype, q, counts, 0.1, causal=True, work=work)
+            sync(gpu)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---- streams and graphs ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,seqs", [(1, 3), (47, 40)])
+def test_every_operator_in_a_graph(gpu, dtype, rows, seqs):
+    """Store, load, attention, linear layers and log-probabilities captured on a stream of their own, replayed over new
+    inputs: the bits of the same calls without a graph."""
+    code, tt = DT[dtype]
+    heads, width, page, group, n = 4, 128, 64, 32, 90
+    pages = seqs * 2
+    pool = torch.zeros(pages * tcu.Kv4Cache.page_bytes(heads, width, page, group), dtype=torch.uint8, device="cuda")
+    cache = tcu.Kv4Cache(gpu, pool.data_ptr(), pages, heads=heads, width=width, page=page, group=group)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").view(seqs, 2)
+    lens = torch.full((seqs,), n, dtype=torch.int32, device="cuda")
+    slots = (torch.arange(seqs, device="cuda")[:, None] * 2 * page + torch.arange(n, device="cuda")).flatten()
+    batch = cache.batch(seqs, rows, n, lens.data_ptr(), table.data_ptr(), 2)
+    d, r = heads * width, rows * seqs
+    weight = torch.empty(700, d, dtype=tt, device="cuda")
+    codes = torch.empty(tcu.W4.code_bytes(700, d), dtype=torch.uint8, device="cuda")
+    scales = torch.empty(tcu.W4.scale_bytes(700, d, group), dtype=torch.uint8, device="cuda")
+    w4 = tcu.W4(gpu, 700, d, group, codes.data_ptr(), scales.data_ptr())
+    k, v = (torch.empty(seqs * n, d, dtype=tt, device="cuda") for _ in range(2))
+    q = torch.empty(r, d, dtype=tt, device="cuda")
+    labels = (torch.arange(r, dtype=torch.int32, device="cuda") * 7 % 700).contiguous()
+    outs = dict(k=torch.empty_like(k), v=torch.empty_like(v), o=torch.empty_like(q), lse=torch.empty(r, heads, device="cuda"),
+                y=torch.empty(r, 700, dtype=tt, device="cuda"), y8=torch.empty(1, 700, dtype=tt, device="cuda"), lp=torch.empty(r, device="cuda"),
+                tv=torch.empty(r, 3, device="cuda"), ti=torch.empty(r, 3, dtype=torch.int32, device="cuda"))
+    work = torch.zeros(max(cache.attend_workspace(batch, heads, code), w4.linear_workspace(r, code)), dtype=torch.uint8, device="cuda")
+
+    def step(stream):
+        w4.pack(code, weight.data_ptr(), d, stream=stream)
+        cache.store(code, seqs * n, slots.data_ptr(), k.data_ptr(), d, width, v.data_ptr(), d, width, stream=stream)
+        cache.load(code, seqs * n, slots.data_ptr(), outs["k"].data_ptr(), d, width, outs["v"].data_ptr(), d, width, stream=stream)
+        cache.attend(batch, code, heads, q.data_ptr(), d, width, outs["o"].data_ptr(), d, width, 0.1, causal=True, lse=outs["lse"].data_ptr(),
+                     work=work.data_ptr(), work_bytes=work.numel(), stream=stream)
+        for m, y in ((r, "y"), (1, "y8")):
+            w4.linear(code, m, outs["o"].data_ptr(), d, outs[y].data_ptr(), 700, act=1, work=work.data_ptr(), work_bytes=work.numel(), stream=stream)
+        gpu.label_logprobs(code, outs["y"].data_ptr(), r, 700, 700, labels.data_ptr(), 1, outs["lp"].data_ptr(), top=3,
+                           top_values=outs["tv"].data_ptr(), top_ids=outs["ti"].data_ptr(), stream=stream)
+
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        step(side.cuda_stream)
+    for seed in (1, 2):
+        gen = torch.Generator("cuda").manual_seed(seed)
+        for x in (weight, k, v, q):
+            x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        for x in outs.values():
+            x.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = {name: x.clone() for name, x in outs.items()}
+        for x in outs.values():
+            x.zero_()
+        step(1)
+        sync(gpu)
+        for name, x in outs.items():
+            assert torch.equal(x, got[name]), name
+        assert float(got["lp"].max()) < 0 and bool(torch.isfinite(got["lse"]).all()) and float(got["o"].float().abs().max()) > 0.01
