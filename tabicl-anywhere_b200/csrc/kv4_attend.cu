@@ -683,17 +683,24 @@ static int ka_nt(int dtype, const Kv4AttendArgs &a) {
     return a.max_rows * (a.q_heads / a.c.heads) > 8 && a.c.width * (dtype == DT_F32 ? 2 : 1) <= 128 ? 2 : 1;
 }
 
-// Many rows go to the tensor cores' kernels, whose tiles hold 128 or 256 rows: from 41 rows a cache head on (32 sequences of
-// 4096 bf16 keys, 8 heads: 32 rows 164 us here and 176 us there, 48 rows 223 and 179), where their units are many or long
-// enough. Units that are fewer than a quarter of the SMs are cut into parts, whose joining costs more there: 512 rows over
-// 2048 keys of 8 heads take 63 us here and 94 us there, 1024 rows 98 and 94; 512 over 8192 keys 140 and 152 (f32 214 and 117).
-static bool ka_many(const Kv4AttendArgs &a, int sms) {
+// Many rows go to the tensor cores' kernels, from 41 rows a cache head on (32 sequences of 4096 keys, 8 heads: 24 rows take
+// 149 us here and 186 there in bf16, 192 and 250 in f32; 48 rows 206 and 191, 361 and 256), where their units (row tiles of 128
+// for f32, 256 for 16 bits) fill the GPU, or nearly and with work enough, or where the work outweighs the joining of units cut
+// into many parts, which costs more there. us here and there, 8 heads of 128:
+//     units 64 and more:  f32 1024 x 512  66, 53;  16 bits 2048 x 512  93, 59
+//     32:                 f32 512 x 512  42, 51, 512 x 2048  82, 60;  16 bits 1024 x 512  61, 57, 1024 x 2048  95, 75
+//     fewer:              f32 128 x 8192  76, 92, 256 x 8192  135, 93;  16 bits 256 x 8192  85, 130, 512 x 8192  131, 132;
+//                         4 heads, f32 256 x 10,000  99, 119, 512 x 10,000  160, 119;  16 bits 512 x 10,000  95, 178
+// (Working memory is asked for before causal and window are known, so the rule does not go by them.)
+static bool ka_many(int dtype, const Kv4AttendArgs &a, int sms) {
     const long long rows = (long long)a.max_rows * (a.q_heads / a.c.heads), heads = (long long)a.seqs * a.c.heads;
-    return a.c.width <= 128 && rows > 40 && (heads * ((rows + 255) / 256) * 4 >= sms || heads * rows * a.max_len >= 16000000LL);
+    const long long tile = dtype == DT_F32 ? 128 : 256, units = heads * ((rows + tile - 1) / tile), pairs = heads * rows * a.max_len;
+    return a.c.width <= 128 && rows > 40 &&
+           (units * 4 >= sms || (units * 5 >= sms && pairs >= 3000000) || pairs >= (dtype == DT_F32 ? 12000000 : 36000000));
 }
 
 size_t kv4_attend_workspace(int dtype, const Kv4AttendArgs &a, int sms) {
-    if (ka_many(a, sms)) return dtype == DT_F32 ? kv4_attend_tc_workspace(a, sms) : kv4_attend_tc16_workspace(a, sms);
+    if (ka_many(dtype, a, sms)) return dtype == DT_F32 ? kv4_attend_tc_workspace(a, sms) : kv4_attend_tc16_workspace(a, sms);
     return 4 * (KA_BLOCKS + (size_t)std::min(KA_BLOCKS, 8 * sms) * 2 * 8 * ka_nt(dtype, a) * (a.c.width + 2));
 }
 
@@ -737,7 +744,7 @@ cudaError_t launch_kv4_attend(int dtype, const Kv4AttendArgs &a, int sms, void *
     if (!a.seqs || !a.rows || !a.max_rows) return cudaSuccess;
     if (kv4_attend_workspace(dtype, a, sms) > work_bytes) return cudaErrorInvalidValue;
     if (launches) ++*launches;
-    if (ka_many(a, sms)) return dtype == DT_F32 ? launch_kv4_attend_tc(a, sms, work, s) : launch_kv4_attend_tc16(dtype, a, sms, work, s);
+    if (ka_many(dtype, a, sms)) return dtype == DT_F32 ? launch_kv4_attend_tc(a, sms, work, s) : launch_kv4_attend_tc16(dtype, a, sms, work, s);
     const int nt = ka_nt(dtype, a);
     cudaError_t e = cudaErrorInvalidValue;
     const int w = a.c.width, g = a.c.group;

@@ -588,3 +588,19 @@ def test_every_operator_in_a_graph(gpu, dtype, rows, seqs):
         for name, x in outs.items():
             assert torch.equal(x, got[name]), name
         assert float(got["lp"].max()) < 0 and bool(torch.isfinite(got["lse"]).all()) and float(got["o"].float().abs().max()) > 0.01
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,length,heads,q_heads,window", [(2048, 7100, 8, 8, 1000), (1300, 1300, 4, 12, 100), (300, 5000, 16, 32, 0)])
+def test_attend_long_prompts(gpu, dtype, rows, length, heads, q_heads, window):
+    """Units cut into parts that several blocks share, with and without a window, causal."""
+    c = Cached(gpu, 48, [length], heads, 128, 64, 32)
+    assert kernels(c, dtype, rows, q_heads) == "many"
+    q = rounded(np.random.default_rng(7).normal(0, 1, (rows, q_heads, 128)), DT[dtype][1])
+    out, lse = c.attend(dtype, q, [rows], 0.088, causal=True, window=window)
+    again, _ = c.attend(dtype, q, [rows], 0.088, causal=True, window=window)
+    sync(gpu)
+    assert torch.equal(out, again)
+    check_many(c, dtype, q, rows, 0.088, True, window, out, lse)
+    last = slice(rows - 64, rows)  # and by each row's own values
+    check_rows(c, dtype, 32, q[last], [64], 0.088, True, window, out[last], lse[last])
