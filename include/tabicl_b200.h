@@ -455,7 +455,8 @@ TCU_API size_t tcu_kv4_attend_workspace(tcu_ctx *ctx, const tcu_kv4 *cache, cons
  * reads cache head h / (q_heads / heads). Without `causal` a row sees every cached token of its sequence; with it, row i
  * of a sequence's n sees tokens up to lens - n + i (its own tokens are stored before the call), and with window > 0 only
  * the last `window` of those. A row that sees nothing gives zeros. lse (may be NULL): [rows][q_heads], the logarithm of
- * the sum of e^score, -infinity for such a row. Strides in elements. */
+ * the sum of e^score, -infinity for such a row. Sums, weights' sums and lse are f32 for every type; scores are resolved up
+ * to 2^23 in magnitude. The outputs of 16-bit types come from weights and values of 11 bits. Strides in elements. */
 TCU_API int tcu_kv4_attend_device(tcu_ctx *ctx, const tcu_kv4 *cache, const tcu_kv4_batch *batch, int dtype, int q_heads,
                                   const void *q, int64_t q_row, int64_t q_head, void *out, int64_t o_row, int64_t o_head,
                                   float scale, int causal, int window, float *lse, void *work, size_t work_bytes, void *stream);
@@ -473,7 +474,8 @@ TCU_API int tcu_w4_pack_device(tcu_ctx *ctx, int dtype, int n, int k, int group,
                                void *scales, void *stream);
 TCU_API size_t tcu_w4_linear_workspace(tcu_ctx *ctx, const tcu_w4 *w, int rows, int dtype); /* (size_t)-1: refused */
 /* y = act(x W^T + bias) + residual, act 0 (none) or 1 (GELU, src/kern.rs:285-290); bias [n] and residual [rows][n] may be
- * NULL, and the residual may be y itself. x, y, bias and residual are of one type; sums are taken in f32. */
+ * NULL, and the residual may be y itself. x, y, bias and residual are of one type; sums are taken in f32. A NaN or an
+ * infinity in a row of x makes that row's outputs NaN or infinite, and no other's. */
 TCU_API int tcu_w4_linear_device(tcu_ctx *ctx, const tcu_w4 *w, int dtype, int rows, const void *x, int64_t ldx, void *y,
                                  int64_t ldy, const void *bias, int act, const void *residual, int64_t ldr, void *work,
                                  size_t work_bytes, void *stream);

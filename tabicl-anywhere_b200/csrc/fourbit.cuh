@@ -266,8 +266,9 @@ __device__ __forceinline__ float value_of(uint32_t w, int j, float step, float l
 // Two codes of a word as f16 operands of a product: the first (SECOND false) or second nibbles of its even bytes. As they
 // are, subnormals: code * 2^-24, code * 2^-20, one AND. CENTRED: code - 8, 16 (code - 8), with the AND's result in the low
 // bits of 1024 and one subtraction, exact. The products' f32 sums are not rounded to nearest by the matrix unit, and with
-// codes of one sign they are large beside what is left when the groups' lows are added, so for f32 and f16 results the
-// codes are centred and the lows taken as low + 8 step.
+// codes of one sign they are large beside what is left when the groups' lows are added, so for f32 results, and f16 ones of
+// attention, the codes are centred and the lows taken as low + 8 step (f16 linear layers are off by 1e-6, which 11 bits do
+// not show).
 template <bool CENTRED, bool SECOND>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
     const uint32_t c = w & (SECOND ? 0x00f000f0u : 0x000f000fu);

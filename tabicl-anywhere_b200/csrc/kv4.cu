@@ -1,7 +1,7 @@
 // The four-bit paged cache: quantise keys and values into their slots, and read them back.
 //
 // One pass over the rows: a thread's 8 coordinates are 16 or 32 bytes read and 4 written, a group's extremes meet in a few
-// lanes. 100,000 rows of 4 heads of 128 in f32 are stored and read back in 0.192 ms (936 MB, 4.9 TB/s): the store, 0.119 ms,
+// lanes. 100,000 rows of 4 heads of 128 in f32 are stored and read back in 0.193 ms (936 MB, 4.8 TB/s): the store, 0.119 ms,
 // is bound by the quantiser's instructions, the load, 0.082 ms, by memory. Two accesses of 16 bytes instead of one of 32
 // took both to 0.234 ms; conversions for rounding (a quarter of the rate of an addition) and a division test a value the
 // store alone to 0.143 ms.

@@ -9,8 +9,8 @@
 // (13.5 with codes as they are, and then off by 1.3e-4 of an output of values that cancel; now 4e-7).
 // What bounds it: issue. Taking a code out of its word is one logic instruction for two, and a step of 32 keys with 8 query
 // rows some 600 instructions a warp, at 0.55 a cycle and scheduler with the 12 warps that the registers of q, the output
-// and the sums leave an SM. 64 bf16 rows (32 heads of 128 on 8, groups of 32) over 0..16384 cached tokens: 0.19 ms, 3.8 TB/s
-// of codes and scales, 57% of a copy's rate; with 16 warps and spills 0.225 ms.
+// and the sums leave an SM. 64 bf16 rows (32 heads of 128 on 8, groups of 32) over 0..16384 cached tokens: 0.191 ms, 3.8 TB/s
+// of codes and scales, 58% of a copy's rate; with 16 warps and spills 0.225 ms.
 //
 // Per 32 keys a warp computes S^T = K Q^T with 16 keys as rows and 8 query rows as columns, so a key's codes are read in
 // the order they are stored in, and O^T = V^T P'^T with P' = p * step turned round in registers (movmatrix).

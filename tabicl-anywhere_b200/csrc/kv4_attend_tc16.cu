@@ -7,12 +7,13 @@
 // step (code - 8), the step the sum of its upper 7 and its lower 4 bits, whose products with code - 8 f16 holds; two operand
 // blocks have those, and 16 columns beside the first the lows and 8 steps, which meet the sums of q over each group (as two
 // f16).
-// What bounds it is shared memory beside the instruction issue: a step's operands are some 290 KB read and written (2300
-// cycles at 128 bytes), the exponentials 1024 cycles (16 a cycle and SM), and a step takes about 2730. The two tiles have a
-// warpgroup each, and widening, which serves both, two that take the steps in turn. Keys rounded to one f16 took 2300 cycles
-// a step (0.40 ms for the prompt below, its lse 4e-6 off), as two f16 split in f32 2980. The products issued from one
-// diverged thread cost 500 cycles more, loops unrolled over a whole step (which the instruction caches do not hold beside
-// widening) 400. A prompt of 4096 bf16 tokens after 1000 cached ones, 32 heads of 128 on 8: 0.475 ms, 0.43 PFLOP/s.
+// What bounds it is latency: of a step's 2700 cycles the exponentials need 1024 (16 a cycle and SM), the products 1630, and
+// issue is active in 46%; warps wait most for tensor memory, then for one another. So the two tiles have a warpgroup each, and
+// widening, which serves both, two that take the steps in turn. Keys rounded to one f16 took 2300 cycles a step (0.40 ms for
+// the prompt below, its lse 4e-6 off); of the 400 more half are the products with the steps' lower bits, half the widening;
+// keys as two f16 split in f32 took 2980. The products issued from one diverged thread cost 500 cycles more, loops unrolled
+// over a whole step (which the instruction caches do not hold beside widening) 400. A prompt of 4096 bf16 tokens after 1000
+// cached ones, 32 heads of 128 on 8: 0.47 ms, 0.44 PFLOP/s.
 //
 // A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8, so the output
 // in tensor memory is rarely rescaled. A step's keys and values are scaled by a power of two of their own that keeps them

@@ -2,9 +2,10 @@
 //
 // With m the largest score and d = (x - m) / T:  S = sum e^d, log p(label) = d_label - log S,
 // entropy = log S - (sum e^d d) / S. A thread keeps (m, S, sum e^d d) of what it has seen and rescales them when a strip
-// of 32 of its scores holds a larger one, so scores are read once; the bound is memory, one ex2 a score next. 4096 rows of
-// 131,071 bf16 scores with five alternatives: 0.194 ms (1.07 GB, 5.5 TB/s); 16 rows of 128,000 with twenty: 13 us, the
-// latency of two strips, the ranking and the cluster's join; 2048 rows of 10 classes: 3.9 us.
+// of 32 of its scores holds a larger one, so scores are read once. 4096 rows of 131,071 bf16 scores with five alternatives:
+// 0.195 ms (1.07 GB, 5.5 TB/s) in runs of up to 40 ms, 0.224 in longer ones, when the power cap holds the SMs at 1680 MHz
+// instead of 1965: instructions bound it (issue active 86%, an ex2 a score 65% of its pipe), not memory (64%). 16 rows of
+// 128,000 with twenty: 13 us, the latency of two strips, the ranking and the cluster's join; 2048 rows of 10 classes: 3.9 us.
 //
 // Top alternatives: a strip's largest score is kept beside. The n-th largest of 32 disjoint parts' maxima is a bound that
 // at least n scores reach and hardly more than n do, so after the pass only the few strips that reach it are read again
@@ -22,7 +23,7 @@ namespace tcu {
 namespace cg = cooperative_groups;
 
 // LP_KEEP: strips a thread keeps a maximum of (longer rows share). 16, and at most 32 registers, let an SM hold eight blocks:
-// 4096 rows of 131071 bf16 scores take 194 us (85% of a copy's rate), with 32 and five blocks 239 us.
+// 4096 rows of 131071 bf16 scores take 195 us in a short run (85% of a copy's rate), with 32 and five blocks 239 us.
 constexpr int LP_THREADS = 256, LP_STRIP = 32, LP_KEEP = 16;
 
 // A score as a whole number in the scores' order (-0 as +0), the index behind it so that of equal scores the lower
