@@ -5,8 +5,10 @@
 // the weights, and the group scales act on its f32 result:
 //     q . k_j   = sum over groups of  step * (q_g . codes)  +  low * (sum of q_g)
 //     sum p_j v = sum over groups of  (p_j step) . codes    +  sum p_j low
-// f32 and f16 queries take code - 8 and low + 8 step instead (code_pair). One f32 row over 10,000 keys, 4 heads of 128: 14.1 us
-// (13.5 with codes as they are, and then off by 1.3e-4 of an output of values that cancel; now 4e-7).
+// f32 and f16 queries take code - 8 and low + 8 step instead (code_pair), and f32 adds each step's products to the output by
+// itself. One f32 row over 10,000 keys, 4 heads of 128: 14.2 us (13.5 with codes as they are, and then off by 1.3e-4 of an
+// output of values that cancel; now 6e-7). 64 f32 rows over 8000 keys, 8 heads of 128: 256 us, and 2e-6 off or less; with the
+// matrix unit's own sums over the steps 244 us, and up to 1e-5 off.
 // What bounds it: issue. Taking a code out of its word is one logic instruction for two, and a step of 32 keys with 8 query
 // rows some 600 instructions a warp, at 0.55 a cycle and scheduler with the 12 warps that the registers of q, the output
 // and the sums leave an SM. 64 bf16 rows (32 heads of 128 on 8, groups of 32) over 0..16384 cached tokens: 0.191 ms, 3.8 TB/s
@@ -533,9 +535,17 @@ __global__ void __launch_bounds__(KA_STEP, (HD <= 128 && NT == 1 && TYPE != DT_F
                         const uint32_t a0 = code_pair<CENTRED, false>(x), a1 = code_pair<CENTRED, true>(x);
                         const uint32_t a2 = code_pair<CENTRED, false>(y), a3 = code_pair<CENTRED, true>(y);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
+                        for (int nt = 0; nt < NT; nt++) {
+                            if constexpr (SPLIT) {  // summed over the steps with rounding to nearest, which the matrix unit's sums are not
+                                float y[4] = {};
 #pragma unroll
-                            for (int q = QS - 1; q >= 0; q--) mma16816(o[nt][u][i], a0, a1, a2, a3, b[q][nt][0], b[q][nt][1]);
+                                for (int q = QS - 1; q >= 0; q--) mma16816(y, a0, a1, a2, a3, b[q][nt][0], b[q][nt][1]);
+#pragma unroll
+                                for (int x = 0; x < 4; x++) o[nt][u][i][x] += y[x];
+                            } else {
+                                mma16816(o[nt][u][i], a0, a1, a2, a3, b[0][nt][0], b[0][nt][1]);
+                            }
+                        }
                     }
             }
         }

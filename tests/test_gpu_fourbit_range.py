@@ -604,3 +604,36 @@ def test_attend_long_prompts(gpu, dtype, rows, length, heads, q_heads, window):
     check_many(c, dtype, q, rows, 0.088, True, window, out, lse)
     last = slice(rows - 64, rows)  # and by each row's own values
     check_rows(c, dtype, 32, q[last], [64], 0.088, True, window, out[last], lse[last])
+
+
+@pytest.mark.parametrize("rows,seqs,length,heads,q_heads,width,group,which", [
+    (1, 17, 20000, 1, 4, 32, 32, "few"), (1, 60, 9000, 2, 4, 128, 128, "few"), (40, 60, 3000, 2, 2, 256, 64, "few"), (1, 1, 20000, 1, 1, 128, 32, "few"),
+    (300, 20, 3000, 2, 2, 128, 64, "many")])
+def test_attend_f32_sums_over_long_sequences(gpu, rows, seqs, length, heads, q_heads, width, group, which):
+    """Thousands of values of either sign: every weighted value is good to 2^-20, and a sum over the steps rounds to nearest, so
+    that its errors, of either sign too, stay below a few 2^-24 of the values' root of squares."""
+    page = 256
+    c = Cached(gpu, 49, [16], heads, width, page, group, extra=length // page + 1)
+    rng = np.random.default_rng(7)
+    k, v = rng.normal(0, 1, (2, length, heads, width))
+    order = rng.permutation(c.pages)[:-(-length // page)]
+    at = order[np.arange(length) // page] * page + np.arange(length) % page
+    raw, kk, vv = plain.pool_of(k.astype(np.float32), v.astype(np.float32), at, c.pages, page, group, 0xFF)
+    c.pool.copy_(dev(raw))
+    c.stride, c.lens = len(order), [length] * seqs
+    c.table = dev(np.tile(order.astype(np.int32), (seqs, 1)))
+    c.lens_dev = torch.full((seqs,), length, dtype=torch.int32, device="cuda")
+    assert width < 128 or kernels(c, "f32", rows, q_heads) == which
+    q = rng.normal(0, 1, (rows * seqs, q_heads, width)).astype(np.float32)
+    out, lse = c.attend("f32", q, [rows] * seqs, 0.5 / np.sqrt(width))
+    sync(gpu)
+    worst = 0.0
+    for h in range(q_heads):
+        x, a, b = (torch.from_numpy(t).cuda().double() for t in (q[:, h], kk[:, h * heads // q_heads], vv[:, h * heads // q_heads]))
+        s = x @ a.T * (0.5 / np.sqrt(width))
+        want = torch.softmax(s, -1) @ b
+        worst = max(worst, float((out[:, h].double() - want).norm() / want.norm()))
+        assert float((lse[:, h].double() - torch.logsumexp(s, -1)).abs().max()) <= 2e-5
+    # a weight's error is that of its score (2^-20 of a sum of magnitudes of about 5, of either sign: 1e-6 and less as a
+    # whole) beside 2^-21 of each product, and ten roundings of a sum
+    assert worst <= 2e-6, worst
