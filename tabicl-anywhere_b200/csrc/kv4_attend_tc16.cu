@@ -2,18 +2,18 @@
 //
 // 256 query rows of one cache head (the heads that share it side by side) as two tiles of 128, against 64 keys at a time:
 // S = Q K^T with Q and the keys, widened to f16, in shared memory; the weights P go to tensor memory over S and multiply
-// the widened values; the output stays in tensor memory. Values and weights are one f16 each (11 bits; the results have 11
-// or 8), sums are f32. Keys are exact, so that the log-sum-exp is f32 as in the other kernels: a key is low + 8 step +
+// the widened values; the output stays in tensor memory. Values are one f16 each (11 bits; the results have 11
+// or 8), weights two for f16 and one for bf16, sums are f32. Keys are exact, so that the log-sum-exp is f32 as in the other kernels: a key is low + 8 step +
 // step (code - 8), the step the sum of its upper 7 and its lower 4 bits, whose products with code - 8 f16 holds; two operand
 // blocks have those, and 16 columns beside the first the lows and 8 steps, which meet the sums of q over each group (as two
 // f16).
-// What bounds it is latency: of a step's 2700 cycles the exponentials need 1024 (16 a cycle and SM), the products 1630, and
+// What bounds it is latency: of a step's 2650 cycles the exponentials need 1024 (16 a cycle and SM), the products 1630, and
 // issue is active in 46%; warps wait most for tensor memory, then for one another. So the two tiles have a warpgroup each, and
 // widening, which serves both, two that take the steps in turn. Keys rounded to one f16 took 2300 cycles a step (0.40 ms for
 // the prompt below, its lse 4e-6 off); of the 400 more half are the products with the steps' lower bits, half the widening;
 // keys as two f16 split in f32 took 2980. The products issued from one diverged thread cost 500 cycles more, loops unrolled
 // over a whole step (which the instruction caches do not hold beside widening) 400. A prompt of 4096 bf16 tokens after 1000
-// cached ones, 32 heads of 128 on 8: 0.47 ms, 0.44 PFLOP/s.
+// cached ones, 32 heads of 128 on 8: 0.46 ms, 0.44 PFLOP/s; f16 0.50.
 //
 // A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8, so the output
 // in tensor memory is rarely rescaled. A step's keys and values are scaled by a power of two of their own that keeps them
@@ -45,8 +45,12 @@ struct KuShape {
 // steps; warp 16: one thread issues the S products; warp 17: one thread the P V products; warp 18: the copies of the stored
 // codes. They hand over through mbarriers; every wait is bounded, and one that gives up raises the block's abort flag, after
 // which every wait returns at once and the roles run to the end without results.
-template <int HD, int G>
-__global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs a, int dtype, float *part, int *arrived) {
+// DT: the queries' type. For f16 a weight is the sum of two f16 (of every 16 keys, hi and lo): rounded to one, and the values
+// too, results were 1.6 times as far from 64 bits as the plain form's, now 1.35 times; bf16's 8 bits do not show it.
+template <int HD, int G, int DT>
+__global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs a, float *part, int *arrived) {
+    constexpr bool SPLIT = DT == DT_F16;
+    constexpr int dtype = DT;
     using C = KuShape<HD, G>;
     using Cut = KaCut<KU_R, KU_BK, KU_BK>;
     constexpr int NU = C::NU, NG = C::NG, UG = G / 32, BQ = KU_BQ, BK = KU_BK, NK = KU_NK, NS = KU_NS, NR = KU_NR, BLOCK = C::BLOCK, HX = HD + KU_X, KSLOT = C::KSLOT;
@@ -199,7 +203,11 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                             if (elect_one()) {
 #pragma unroll
                                 for (int k = 0; k < BK / 16; k++)
-                                    mma_f16_ta(tmem + KU_TO + q * HD, tP + 8 * k, dV + k * stV, idO, i > 0 || k > 0 ? 1u : 0u);
+                                    mma_f16_ta(tmem + KU_TO + q * HD, tP + (SPLIT ? 16 : 8) * k, dV + k * stV, idO, i > 0 || k > 0 ? 1u : 0u);
+                                if constexpr (SPLIT) {
+#pragma unroll
+                                    for (int k = 0; k < BK / 16; k++) mma_f16_ta(tmem + KU_TO + q * HD, tP + 16 * k + 8, dV + k * stV, idO, 1);
+                                }
                                 mma_commit(&mSlot[q][c & 1]);
                                 if (q == nq - 1) mma_commit(&mVfree[sl]);
                             }
@@ -502,14 +510,21 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
                         for (int k = 0; k < 32; k++)
                             if (key0 + 32 * b + k < my_lo || key0 + 32 * b + k >= my_hi) x[k] = -INFINITY;
                     }
-                    uint32_t h[16];
+                    uint32_t h[SPLIT ? 32 : 16];
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
                         const float p0 = kt_ex2(fmaf(x[2 * k], c1, -mm)), p1 = kt_ex2(fmaf(x[2 * k + 1], c1, -mm));
                         part_sum[(2 * k) & 3] += p0, part_sum[(2 * k + 1) & 3] += p1;
-                        h[k] = kt_u32(__floats2half2_rn(p0, p1));
+                        if constexpr (SPLIT)
+                            split_pair(p0, p1, h[k / 8 * 16 + k % 8], h[k / 8 * 16 + 8 + k % 8]);
+                        else
+                            h[k] = kt_u32(__floats2half2_rn(p0, p1));
                     }
-                    tmem_st16u(tsp + 16 * b, h);  // over scores that have been read
+                    // over scores that have been read
+                    if constexpr (SPLIT)
+                        tmem_st32u(tsp + 32 * b, h);
+                    else
+                        tmem_st16u(tsp + 16 * b, h);
                 }
                 const float sum = (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]);
                 tmem_wait_st();
@@ -659,14 +674,18 @@ size_t kv4_attend_tc16_workspace(const Kv4AttendArgs &a, int sms) {
     return 4 * (KA_BLOCKS + (size_t)2 * std::min(KA_BLOCKS / 2, sms) * KU_R * (a.c.width + 2));
 }
 
+template <int HD, int G, int DT>
+static cudaError_t launch_type(const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
+    const size_t smem = KuShape<HD, G>::SMEM;
+    cudaError_t e = allow_dynamic_smem((const void *)k_kv4_attend_tc16<HD, G, DT>, smem);
+    if (e != cudaSuccess) return e;
+    k_kv4_attend_tc16<HD, G, DT><<<std::min(sms, KA_BLOCKS / 2), KU_THREADS, smem, s>>>(a, reinterpret_cast<float *>(work) + KA_BLOCKS,
+                                                                                        reinterpret_cast<int *>(work));
+    return cudaGetLastError();
+}
 template <int HD, int G>
 static cudaError_t launch_tc16(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {
-    const size_t smem = KuShape<HD, G>::SMEM;
-    cudaError_t e = allow_dynamic_smem((const void *)k_kv4_attend_tc16<HD, G>, smem);
-    if (e != cudaSuccess) return e;
-    k_kv4_attend_tc16<HD, G><<<std::min(sms, KA_BLOCKS / 2), KU_THREADS, smem, s>>>(a, dtype, reinterpret_cast<float *>(work) + KA_BLOCKS,
-                                                                                   reinterpret_cast<int *>(work));
-    return cudaGetLastError();
+    return dtype == DT_F16 ? launch_type<HD, G, DT_F16>(a, sms, work, s) : launch_type<HD, G, DT_BF16>(a, sms, work, s);
 }
 
 cudaError_t launch_kv4_attend_tc16(int dtype, const Kv4AttendArgs &a, int sms, void *work, cudaStream_t s) {

@@ -637,3 +637,23 @@ def test_attend_f32_sums_over_long_sequences(gpu, rows, seqs, length, heads, q_h
     # a weight's error is that of its score (2^-20 of a sum of magnitudes of about 5, of either sign: 1e-6 and less as a
     # whole) beside 2^-21 of each product, and ten roundings of a sum
     assert worst <= 2e-6, worst
+
+
+@pytest.mark.parametrize("rows,seqs,which", [(2, 30, "few"), (60, 40, "many")])
+def test_attend_f16_is_near_the_result_rounded_once(gpu, rows, seqs, which):
+    """Values of either sign, one rounding to 11 bits (of weights times steps, or of values) beside the result's own: together
+    the root of two of the latter, so below 1.5 of it."""
+    n, heads = 1500, 4
+    c = Cached(gpu, 50, [n], heads, 128, 64, 32)
+    rng = np.random.default_rng(8)
+    k, v = rng.normal(0, 1, (2, n, heads, 128))
+    set_tokens(c, k, v, 64, 32)
+    c.lens = [n] * seqs
+    c.table, c.lens_dev = c.table.repeat(seqs, 1).contiguous(), c.lens_dev.repeat(seqs)
+    assert kernels(c, "f16", rows, heads) == which
+    q = rounded(rng.normal(0, 1, (rows * seqs, heads, 128)), torch.float16)
+    out, _ = c.attend("f16", q, [rows] * seqs, 0.088)
+    sync(gpu)
+    want, _, _, _ = exact(q, c.k[0], c.v[0], 0.088, np.ones((len(q), n), bool))
+    once = np.linalg.norm(want.astype(np.float16).astype(np.float64) - want)
+    assert np.linalg.norm(host(out) - want) <= 1.5 * once, np.linalg.norm(host(out) - want) / once
