@@ -93,15 +93,6 @@ __global__ void __launch_bounds__(KU_THREADS, 1) k_kv4_attend_tc16(Kv4AttendArgs
     fence_after_sync();
     const uint32_t tmem = tslot;
 
-    auto wait = [&](uint64_t *m, uint32_t parity) {
-        if (mbar_test_wait(m, parity)) return true;
-        if (abort_flag) return false;
-        if (!mbar_wait(m, parity, KT_WAIT)) {
-            abort_flag = 1;
-            return false;
-        }
-        return true;
-    };
     auto wait_warp = [&](uint64_t *m, uint32_t parity) {  // warp-uniform: warp-wide instructions follow
         bool ok = mbar_test_wait(m, parity) || (!abort_flag && mbar_wait(m, parity, KT_WAIT));
         ok = __all_sync(0xffffffffu, ok);
