@@ -7,7 +7,7 @@
 //     sum p_j v = sum over groups of  (p_j step) . codes    +  sum p_j low
 // f32 and f16 queries take code - 8 and low + 8 step instead (code_pair), and f32 adds each step's products to the output by
 // itself. One f32 row over 10,000 keys, 4 heads of 128: 14.2 us (13.5 with codes as they are, and then off by 1.3e-4 of an
-// output of values that cancel; now 6e-7). 64 f32 rows over 8000 keys, 8 heads of 128: 256 us, and 2e-6 off or less; with the
+// output of values that cancel; now 4e-7). 64 f32 rows over 8000 keys, 8 heads of 128: 256 us, and 2e-6 off or less; with the
 // matrix unit's own sums over the steps 244 us, and up to 1e-5 off.
 // What bounds it: issue. Taking a code out of its word is one logic instruction for two, and a step of 32 keys with 8 query
 // rows some 600 instructions a warp, at 0.55 a cycle and scheduler with the 12 warps that the registers of q, the output
