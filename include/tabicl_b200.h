@@ -490,6 +490,43 @@ TCU_API int tcu_label_logprobs_device(tcu_ctx *ctx, int dtype, const void *logit
                                       const int32_t *labels, int per_row, float *out, float *entropy, int top, float *top_values,
                                       int32_t *top_ids, double temperature, void *stream);
 
+/* ---- a prompt's operators ---------------------------------------------------------------------------------------
+ *
+ * What the rows of a prompt need beside the operators above, which serve a step's few rows best: matrices whose rows are four
+ * bits on both sides of a product, and attention over keys and values as they are. Streams, working memory, indexes that only
+ * the device sees and their reports are as for the four-bit operators; one block of working memory serves all of them. */
+
+/* A matrix [rows][k] in microscaled four-bit floating point. A number is 0, 0.5, 1, 1.5, 2, 3, 4 or 6 (codes 0..7) or its
+ * negative (8..15), and stands for unit * scale * number; neighbours of a row share the scale:
+ *   TCU_FP4_MX: 32 share a power of two, a byte of its exponent plus 127 (255: NaN); unit is 1;
+ *   TCU_FP4_NV: 16 share an e4m3 float (four exponent bits, three of mantissa; 127: NaN); unit is a number of the whole matrix,
+ *               1e-30 to 1e30, such as its largest magnitude / (448 * 6).
+ * codes: tcu_fp4_code_bytes(), [rows][k / 128 rounded up][64], the earlier of two neighbours in the low half of a byte, columns
+ * past k zeros. scales: tcu_fp4_scale_bytes(), blocks of 128 rows x 4 scales of 512 bytes each, a row's blocks beside one
+ * another, then the next 128 rows'; row r and scale s of a block at byte 16 (r % 32) + 4 (r / 32) + s. Both 16-byte aligned.
+ * rows * (k rounded up to 128) below 2^35. */
+enum { TCU_FP4_MX = 0, TCU_FP4_NV = 1 };
+typedef struct tcu_fp4 {
+    void *codes, *scales;
+    int32_t rows, k, format;
+    float unit;
+} tcu_fp4;
+TCU_API size_t tcu_fp4_code_bytes(int rows, int k);               /* 0: sizes not taken */
+TCU_API size_t tcu_fp4_scale_bytes(int rows, int k, int format);
+/* Quantise x [rows][k] (row stride ldx, elements) into m. A scale: of MX 2^(floor(log2 of the block's largest magnitude) - 2),
+ * at least 2^-127; of NV that magnitude / (6 unit) rounded to e4m3 (to the nearest, ties to even, held to 448). A number: the
+ * one nearest to x / (scale * unit), ties to the even code, held to 6; 0 where the scale is 0. Both as if worked out exactly.
+ * A block that holds a NaN or an infinity has scale NaN. Every byte of codes, and of the scales those of the rows, is written. */
+TCU_API int tcu_fp4_pack_device(tcu_ctx *ctx, const tcu_fp4 *m, int dtype, const void *x, int64_t ldx, void *stream);
+/* What m stands for, y [rows][k]: (number * scale) * unit in f32, rounded to the type. */
+TCU_API int tcu_fp4_load_device(tcu_ctx *ctx, const tcu_fp4 *m, int dtype, void *y, int64_t ldy, void *stream);
+TCU_API size_t tcu_fp4_linear_workspace(tcu_ctx *ctx, const tcu_fp4 *w, const tcu_fp4 *x, int dtype); /* (size_t)-1: refused */
+/* y = act(x W^T + bias) + residual [x's rows][W's rows], act 0 (none) or 1 (GELU, src/kern.rs:285-290); bias and residual may
+ * be NULL, and the residual may be y itself. y, bias and residual are of one type; sums are taken in f32. x and W are of one
+ * format and k. A scale NaN in a row of x, or of W, makes that row's, or column's, outputs NaN, and no other. */
+TCU_API int tcu_fp4_linear_device(tcu_ctx *ctx, const tcu_fp4 *w, const tcu_fp4 *x, int dtype, void *y, int64_t ldy, const void *bias,
+                                  int act, const void *residual, int64_t ldr, void *work, size_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,6 +8,7 @@ The objects mirror the reference's accelerator side (src/gpu.rs, src/predict.rs:
 * `VramMember` - a fitted member's problems and its class tree, predicted whole (predict::predict_raw)
 * `VramTier` / `VramHandle` - problems resident for many tenants within byte budgets; the handle is an AttendCached
 * `Kv4Cache`, `W4` - the four-bit cache and weights (fourbit.py; no counterpart in the reference)
+* `Fp4` - matrices in four-bit floating point and their products (prompt.py; no counterpart in the reference)
 * `CudaAttend` - the `AttendCached` implementation: `attend`, `stage`, `rows`, each returning None to decline
 
 Everything computes on the GPU through libtabicl_b200.so; there is no CPU path here. The library is built in-tree
@@ -20,7 +21,7 @@ import numpy as np
 
 from . import tirs  # noqa: F401  (bundle reader/writer for callers)
 from .plan import Plan  # noqa: F401
-from . import fourbit
+from . import fourbit, prompt
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtabicl_b200.so")
@@ -168,6 +169,7 @@ def lib():
         "tcu_comm_breakdown": (_c_int, [_c_void, _c_int, P(ctypes.c_double)]),
         "tcu_comm_abort": (_c_int, [_c_void]),
         **fourbit.signatures(),
+        **prompt.signatures(),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -1003,3 +1005,4 @@ class CudaAttend:
 
 
 from .fourbit import BF16, F16, F32, Kv4Cache, W4  # noqa: E402,F401  (they use lib() and Gpu)
+from .prompt import MX, NV, Fp4  # noqa: E402,F401

@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "fourbit.cuh"
+#include "fp4.cuh"
 #include "kernels.cuh"
 #include "engine.hpp"
 #include "tirs.hpp"
@@ -3445,6 +3446,93 @@ int tcu_label_logprobs_device(tcu_ctx *ctx, int dtype, const void *logits, int r
         a.err = ctx->err_mapped + ERR_INDEX;
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
         Launch{ctx, s}(launch_logprobs(dtype, a, ctx->sms, s, &ctx->launches), "label_logprobs");
+        return TCU_OK;
+    });
+}
+
+}  // extern "C"
+
+// ---- a prompt's operators -------------------------------------------------------------------------------------------
+
+static bool fp4_sizes(int rows, int k) {
+    return rows >= 1 && k >= 1 && k <= (1 << 24) && (long long)rows * fp4_padded(k) < 1LL << 35;
+}
+static void check_fp4(const char *who, const tcu_fp4 *m) {
+    const std::string w = who;
+    if (!m) fail(TCU_ERR_ARG, w + ": null matrix");
+    if (!fp4_sizes(m->rows, m->k)) fail(TCU_ERR_ARG, w + ": rows and k at least 1, k up to 2^24, rows * k below 2^35");
+    if (m->format != TCU_FP4_MX && m->format != TCU_FP4_NV) fail(TCU_ERR_ARG, w + ": format must be TCU_FP4_MX or TCU_FP4_NV");
+    if (m->format == TCU_FP4_MX ? m->unit != 1.f : !(m->unit >= 1e-30f && m->unit <= 1e30f))
+        fail(TCU_ERR_ARG, w + ": unit must be 1 (TCU_FP4_MX) or 1e-30 to 1e30 (TCU_FP4_NV)");
+    if (!m->codes || !m->scales) fail(TCU_ERR_ARG, w + ": null codes or scales");
+    check_aligned(who, "codes", m->codes, 16), check_aligned(who, "scales", m->scales, 16);
+}
+static int fp4_copy(tcu_ctx *ctx, const char *who, bool pack, const tcu_fp4 *m, int dtype, void *x, int64_t ldx, void *stream) {
+    return guarded(ctx, [&]() -> int {
+        check_device_error(ctx);
+        check_fp4(who, m);
+        check_dtype(who, dtype);
+        if (!x || ldx < m->k) fail(TCU_ERR_ARG, std::string(who) + ": null argument or a row stride below k");
+        check_aligned(who, "rows", x, elem_size(dtype));
+        Fp4Args a;
+        a.codes = (uint8_t *)m->codes, a.scales = (uint8_t *)m->scales, a.rows = m->rows, a.k = m->k, a.format = m->format, a.unit = m->unit;
+        a.x = x, a.ldx = ldx;
+        cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        Launch{ctx, s}(pack ? launch_fp4_pack(dtype, a, s, &ctx->launches) : launch_fp4_load(dtype, a, s, &ctx->launches), who);
+        return TCU_OK;
+    });
+}
+static Fp4LinearArgs fp4_linear_args(const tcu_fp4 *w, const tcu_fp4 *x, int dtype) {
+    check_fp4("fp4_linear", w), check_fp4("fp4_linear", x);
+    check_dtype("fp4_linear", dtype);
+    if (w->format != x->format || w->k != x->k) fail(TCU_ERR_ARG, "fp4_linear: both matrices must be of one format and k");
+    Fp4LinearArgs a;
+    a.w = (const uint8_t *)w->codes, a.w_scales = (const uint8_t *)w->scales, a.x = (const uint8_t *)x->codes, a.x_scales = (const uint8_t *)x->scales;
+    a.n = w->rows, a.k = w->k, a.rows = x->rows, a.format = w->format;
+    a.alpha = w->unit * x->unit;
+    return a;
+}
+
+extern "C" {
+
+size_t tcu_fp4_code_bytes(int rows, int k) { return fp4_sizes(rows, k) ? (size_t)rows * (fp4_padded(k) / 2) : 0; }
+size_t tcu_fp4_scale_bytes(int rows, int k, int format) {
+    return fp4_sizes(rows, k) && (format == TCU_FP4_MX || format == TCU_FP4_NV) ? (size_t)(rows + 127) / 128 * fp4_quads(k, format) * 512 : 0;
+}
+
+int tcu_fp4_pack_device(tcu_ctx *ctx, const tcu_fp4 *m, int dtype, const void *x, int64_t ldx, void *stream) {
+    return fp4_copy(ctx, "fp4_pack", true, m, dtype, const_cast<void *>(x), ldx, stream);
+}
+int tcu_fp4_load_device(tcu_ctx *ctx, const tcu_fp4 *m, int dtype, void *y, int64_t ldy, void *stream) {
+    return fp4_copy(ctx, "fp4_load", false, m, dtype, y, ldy, stream);
+}
+
+size_t tcu_fp4_linear_workspace(tcu_ctx *ctx, const tcu_fp4 *w, const tcu_fp4 *x, int dtype) {
+    size_t need = 0;
+    const int r = guarded(ctx, [&]() -> int {
+        need = fp4_linear_workspace(dtype, fp4_linear_args(w, x, dtype), ctx->sms);
+        return TCU_OK;
+    });
+    return r == TCU_OK ? need : (size_t)-1;
+}
+
+int tcu_fp4_linear_device(tcu_ctx *ctx, const tcu_fp4 *w, const tcu_fp4 *x, int dtype, void *y, int64_t ldy, const void *bias, int act,
+                          const void *residual, int64_t ldr, void *work, size_t work_bytes, void *stream) {
+    return guarded(ctx, [&]() -> int {
+        check_device_error(ctx);
+        Fp4LinearArgs a = fp4_linear_args(w, x, dtype);
+        if (act < 0 || act > 1) fail(TCU_ERR_ARG, "fp4_linear: act must be 0 (none) or 1 (GELU)");
+        if (!y) fail(TCU_ERR_ARG, "fp4_linear: null output");
+        if (ldy < a.n || (residual && ldr < a.n)) fail(TCU_ERR_ARG, "fp4_linear: a row stride below the row");
+        if (!(a.alpha >= FLT_MIN && a.alpha <= FLT_MAX)) fail(TCU_ERR_ARG, "fp4_linear: f32 does not hold the product of the units");
+        check_aligned("fp4_linear", "output", y, elem_size(dtype));
+        check_aligned("fp4_linear", "bias", bias, elem_size(dtype)), check_aligned("fp4_linear", "residual", residual, elem_size(dtype));
+        a.y = y, a.ldy = ldy, a.bias = bias, a.act = act, a.residual = residual, a.ldr = ldr, a.err_wait = ctx->err_mapped + ERR_GEMM_TC;
+        const size_t need = fp4_linear_workspace(dtype, a, ctx->sms);
+        if (need && (!work || work_bytes < need)) fail(TCU_ERR_ARG, "fp4_linear: needs " + std::to_string(need) + " bytes of working memory");
+        check_aligned("fp4_linear", "working memory", work, 16);
+        cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        Launch{ctx, s}(launch_fp4_linear(dtype, a, ctx->sms, (void *)tensor_map_encoder(), work, s, &ctx->launches), "fp4_linear");
         return TCU_OK;
     });
 }

@@ -1,0 +1,341 @@
+// Products of matrices in microscaled four-bit floating point on the 5th-generation tensor cores (tcgen05, block-scaled):
+// y = act(x W^T + bias) + residual.
+//
+// The matrix unit takes the stored codes and scales as they are: a tile is 128 outputs (rows of W, the unit's A) by up to 256
+// rows of x (its B), K in steps of 256 columns, 128 bytes of codes a row, by TMA into shared memory; the scales come by bulk
+// copies and go on to tensor memory. W on the unit's side of 128 serves one row and thousands alike: few rows make a narrow
+// tile, and the weights stream at the memory's rate with no instruction of a thread's spent on them.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "device.cuh"
+#include "fp4.cuh"
+#include "kv4_tc.cuh"
+
+namespace tcu {
+
+constexpr int FL_THREADS = 384, FL_M = 128, FL_STEP = 256, FL_STAGES = 8;
+constexpr int FL_A = FL_M * FL_STEP / 2;  // bytes of a step's weights
+constexpr size_t FL_SMEM = 225 * 1024;
+// Steps a block takes at least where a product has fewer tiles than SMs.
+constexpr int FL_MIN_STEPS = 2;
+
+struct FlPlan {
+    int nt, row_tiles, feat_tiles, steps, stages, nacc, chunk, blocks, quads, group;
+    unsigned stage_bytes, sf_a, sf_b, slot, acc_cols;
+    long long total;
+};
+
+// Instruction descriptor of a block-scaled product of two e2m1 operands, 128 x N: bits 4-5 and 29-30 which scales of a word
+// B and A use, 7-9 and 10-11 the operands' type, 17-22 N / 8, 23 the scales' type (1: powers of two), 27-28 M / 128.
+__device__ __forceinline__ uint32_t fl_idesc(int n, bool nv, int part) {
+    return (uint32_t)part << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (nv ? 0u : 1u << 23) | 1u << 27 | (uint32_t)part << 29;
+}
+// 128-byte rows swizzled by 128 bytes, groups of 8 rows 1024 bytes apart; K-major.
+__device__ __forceinline__ uint64_t fl_desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+template <bool NV>
+__device__ __forceinline__ void fl_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t acc) {
+    if constexpr (NV)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(acc)
+            : "memory");
+}
+// 512 bytes of scales (32 rows of 16) to 4 columns of tensor memory, once for each warp's lanes.
+__device__ __forceinline__ void fl_scales(uint32_t to, uint32_t from) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(smem_desc(from, 16, 128)) : "memory");
+}
+__device__ __forceinline__ void fl_expect(uint64_t *m, uint32_t bytes) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}\n" ::"r"(smem_addr(m)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void fl_tile(uint32_t to, const CUtensorMap *map, int x, int y, uint64_t *m) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(to),
+                 "l"(map), "r"(x), "r"(y), "r"(smem_addr(m))
+                 : "memory");
+}
+__device__ __forceinline__ void fl_bulk(uint32_t to, const void *from, uint32_t bytes, uint64_t *m) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes),
+                 "r"(smem_addr(m))
+                 : "memory");
+}
+
+// Tile t's place: groups of `group` row tiles, in them the row tiles innermost, so that blocks at work at the same time share
+// weights and rows in L2.
+__device__ __forceinline__ int2 fl_place(const FlPlan &p, int t) {
+    const int per = p.group * p.feat_tiles, g = t / per, in = t - g * per, rows = min(p.group, p.row_tiles - g * p.group);
+    return make_int2(g * p.group + in % rows, in / rows);
+}
+
+// Warp 0: the copies; warp 1: the products; warps 4-11: sums from tensor memory, joining and output, a thread one output of
+// half the tile's rows. The steps of all tiles in a row are cut evenly over the blocks; parts of a tile meet in the working
+// memory, and the last block to arrive joins them in order.
+template <int DT, bool NV>
+__global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, FlPlan p, const __grid_constant__ CUtensorMap map_w,
+                                                              const __grid_constant__ CUtensorMap map_x, float *part, int *arrived) {
+    using T = typename Elem<DT>::T;
+    constexpr int QS = NV ? 4 : 2;  // blocks of 4 scales in a step
+    extern __shared__ uint8_t smraw[];
+    __shared__ __align__(8) uint64_t m_full[FL_STAGES], m_empty[FL_STAGES], m_acc[2], m_free[2], m_done;
+    __shared__ uint32_t tslot;
+    __shared__ volatile int abort_flag;
+    __shared__ int s_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = (smem_addr(smraw) + 1023u) & ~1023u;
+    if (warp == 2) {
+        tmem_alloc(&tslot, 512);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        for (int i = 0; i < FL_STAGES; i++) mbar_init(&m_full[i], 1), mbar_init(&m_empty[i], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&m_acc[i], 1), mbar_init(&m_free[i], 256);
+        mbar_init(&m_done, 1);
+        mbar_init_fence();
+        abort_flag = 0;
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = tslot, sf0 = tmem + p.acc_cols;
+    auto wait_warp = [&](uint64_t *m, uint32_t parity) {
+        bool ok = mbar_test_wait(m, parity) || (!abort_flag && mbar_wait(m, parity, KT_WAIT));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) abort_flag = 1;
+        return ok;
+    };
+    long long pos = ka_div(p.total * blockIdx.x, gridDim.x);
+    const long long end = ka_div(p.total * (blockIdx.x + 1), gridDim.x);
+
+    if (warp == 0) {
+        int at = 0;
+        bool on = true;
+        while (pos < end && on) {
+            const int t = (int)ka_div(pos, p.steps), s0 = (int)(pos - (long long)t * p.steps), s1 = (int)min((long long)p.steps, s0 + end - pos);
+            const int2 place = fl_place(p, t);
+            const uint8_t *wa = a.w_scales + (size_t)place.y * p.quads * 512;
+            const int row_block = place.x * p.nt / 128, blocks = min((p.nt + 127) / 128, (a.rows + 127) / 128 - row_block);
+            const uint8_t *xa = a.x_scales + (size_t)row_block * p.quads * 512;
+            for (int s = s0; s < s1; s++, at++) {
+                const int slot = at % p.stages;
+                if (at >= p.stages && !wait_warp(&m_empty[slot], (uint32_t)(at / p.stages - 1) & 1u)) {
+                    on = false;
+                    break;
+                }
+                const int quads = min(QS, p.quads - s * QS);
+                if (elect_one()) {
+                    const uint32_t to = base + slot * p.stage_bytes;
+                    fl_expect(&m_full[slot], FL_A + p.nt * 128 + quads * 512 * (1 + blocks));
+                    fl_tile(to, &map_w, s * 128, place.y * FL_M, &m_full[slot]);
+                    fl_tile(to + FL_A, &map_x, s * 128, place.x * p.nt, &m_full[slot]);
+                    fl_bulk(to + p.sf_a, wa + (size_t)s * QS * 512, quads * 512, &m_full[slot]);
+                    for (int b = 0; b < blocks; b++)
+                        fl_bulk(to + p.sf_b + b * QS * 512, xa + ((size_t)b * p.quads + s * QS) * 512, quads * 512, &m_full[slot]);
+                }
+                __syncwarp();
+            }
+            pos += s1 - s0;
+        }
+        // what was asked for lands before the block lets go of shared memory
+        for (int i = max(0, at - p.stages); i < at; i++) mbar_wait(&m_full[i % p.stages], (uint32_t)(i / p.stages) & 1u, KT_WAIT);
+    } else if (warp == 1) {
+        int at = 0, c = 0;
+        const bool two = p.nt > 128;
+        while (pos < end) {
+            const int t = (int)ka_div(pos, p.steps), s0 = (int)(pos - (long long)t * p.steps), s1 = (int)min((long long)p.steps, s0 + end - pos);
+            for (int from = s0; from < s1; from += p.chunk, c++) {
+                const int to = min(s1, from + p.chunk), acc = c % p.nacc;
+                if (c >= p.nacc) wait_warp(&m_free[acc], (uint32_t)(c / p.nacc - 1) & 1u);
+                fence_after_sync();
+                const uint32_t d = tmem + acc * (p.acc_cols / p.nacc);
+                for (int s = from; s < to; s++, at++) {
+                    const int slot = at % p.stages;
+                    wait_warp(&m_full[slot], (uint32_t)(at / p.stages) & 1u);
+                    fence_after_sync();
+                    const int quads = min(QS, p.quads - s * QS);
+                    if (elect_one()) {
+                        const uint32_t in = base + slot * p.stage_bytes, sa = sf0 + slot * p.slot, sb = sa + QS * 4;
+                        for (int q = 0; q < quads; q++) {
+                            fl_scales(sa + q * 4, in + p.sf_a + q * 512);
+                            fl_scales(sb + q * (two ? 8 : 4), in + p.sf_b + q * 512);
+                            if (two) fl_scales(sb + q * 8 + 4, in + p.sf_b + (QS + q) * 512);
+                        }
+                        const uint64_t da = fl_desc(in), db = fl_desc(in + FL_A);
+                        for (int q = 0; q < quads; q++) {
+                            const uint32_t qa = sa + q * 4, qb = sb + q * (two ? 8 : 4);
+                            if constexpr (NV) {
+                                fl_mma<NV>(d, da + q * 2, db + q * 2, fl_idesc(p.nt, true, 0), qa, qb, s > from || q > 0);
+                            } else {
+                                fl_mma<NV>(d, da + q * 4, db + q * 4, fl_idesc(p.nt, false, 0), qa, qb, s > from || q > 0);
+                                fl_mma<NV>(d, da + q * 4 + 2, db + q * 4 + 2, fl_idesc(p.nt, false, 2), qa, qb, 1);
+                            }
+                        }
+                        mma_commit(&m_empty[slot]);
+                        if (s == to - 1) mma_commit(&m_acc[acc]);
+                    }
+                    __syncwarp();
+                }
+            }
+            pos += s1 - s0;
+        }
+        if (elect_one()) {
+            mma_commit(&m_done);
+            mbar_wait(&m_done, 0, KT_WAIT);
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        const int quad = warp & 3, half = (warp - 4) >> 2, cols = p.nt > 16 ? (p.nt / 2 + 15) & ~15 : 16, c0 = half * cols, own = min(cols, p.nt - c0);
+        int c = 0;
+        while (pos < end) {
+            const int t = (int)ka_div(pos, p.steps), s0 = (int)(pos - (long long)t * p.steps), s1 = (int)min((long long)p.steps, s0 + end - pos);
+            const int2 place = fl_place(p, t);
+            float v[128];
+#pragma unroll
+            for (int i = 0; i < 128; i++) v[i] = 0.f;
+            for (int from = s0; from < s1; from += p.chunk, c++) {
+                const int acc = c % p.nacc;
+                wait_warp(&m_acc[acc], (uint32_t)(c / p.nacc) & 1u);
+                fence_after_sync();
+                const uint32_t d = tmem + acc * (p.acc_cols / p.nacc) + c0 + ((uint32_t)(quad * 32) << 16);
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    if (g * 16 < own) {
+                        float x[16];
+                        tmem_ld16(d + g * 16, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 16; i++) v[g * 16 + i] += x[i];
+                    }
+                }
+                fence_before_sync();
+                mbar_arrive(&m_free[acc]);
+            }
+            const bool whole = s0 == 0 && s1 == p.steps;
+            bool last = true;
+            if (!whole && !abort_flag) {
+                // parts: each block's into its slot (the tile's first block's into its second slot, the others' into their first)
+                const long long u0 = (long long)t * p.steps;
+                const int b0 = (int)ka_div((u0 + 1) * gridDim.x - 1, p.total), b1 = (int)ka_div((u0 + p.steps) * gridDim.x - 1, p.total);
+                const size_t size = (size_t)FL_M * p.nt;
+                const int at = c0 * FL_M + quad * 32 + lane;
+                float *to = part + (2 * (size_t)blockIdx.x + (s0 == 0)) * size + at;
+#pragma unroll
+                for (int i = 0; i < 128; i++)
+                    if (i < own) __stcg(to + i * FL_M, v[i]);
+                __threadfence();
+                kt_bar(1, 256);
+                if (tid == 128) {
+                    const int n = atomicAdd(&arrived[b0], 1);
+                    s_last = n == b1 - b0;
+                    if (s_last) arrived[b0] = 0;
+                    __threadfence();
+                }
+                kt_bar(1, 256);
+                last = s_last != 0;
+                if (last) {
+#pragma unroll
+                    for (int i = 0; i < 128; i++) v[i] = 0.f;
+                    for (int b = b0; b <= b1; b++) {
+                        const float *in = part + (2 * (size_t)b + (b == b0)) * size + at;
+#pragma unroll
+                        for (int i = 0; i < 128; i++)
+                            if (i < own) v[i] += __ldcg(in + i * FL_M);
+                    }
+                }
+            }
+            const int n = place.y * FL_M + quad * 32 + lane, row0 = place.x * p.nt + c0;
+            if (last && n < a.n && !abort_flag) {
+                const float bias = a.bias ? Elem<DT>::get(reinterpret_cast<const T *>(a.bias)[n]) : 0.f;
+                T *y = reinterpret_cast<T *>(a.y) + (size_t)row0 * a.ldy + n;
+                const T *r = reinterpret_cast<const T *>(a.residual) + (a.residual ? (size_t)row0 * a.ldr + n : 0);
+                const int rows = min(own, a.rows - row0);
+#pragma unroll
+                for (int i = 0; i < 128; i++) {
+                    if (i < rows) {
+                        float f = fmaf(v[i], a.alpha, bias);
+                        if (a.act) f = gelu1(f);
+                        if (a.residual) f += Elem<DT>::get(r[(size_t)i * a.ldr]);
+                        y[(size_t)i * a.ldy] = Elem<DT>::put(f);
+                    }
+                }
+            }
+            pos += s1 - s0;
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (tid == 0 && abort_flag) *reinterpret_cast<volatile int *>(a.err_wait) = 1;
+    fence_after_sync();
+    if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+static FlPlan fl_plan(int dtype, const Fp4LinearArgs &a, int sms) {
+    FlPlan p;
+    const bool nv = a.format == FP4_NV;
+    const int kp = fp4_padded(a.k), qs = nv ? 4 : 2;
+    p.quads = fp4_quads(a.k, a.format), p.steps = (kp + FL_STEP - 1) / FL_STEP;
+    // f32 results: the matrix unit does not round its sums to nearest, so a sum runs over 4 steps in it, from there on in
+    // registers; two narrower accumulators in turn, so that the unit does not wait for them to be read
+    const int most = dtype == DT_F32 ? 128 : 256;
+    p.nt = a.rows > most ? most : a.rows > 128 ? 256 : a.rows > 64 ? 128 : (a.rows + 15) / 16 * 16;
+    p.chunk = dtype == DT_F32 ? 4 : p.steps;
+    p.nacc = p.nt > 128 ? 1 : 2;
+    int cols = 32;
+    while (cols < p.nt) cols *= 2;
+    p.acc_cols = (unsigned)(cols * p.nacc);
+    p.row_tiles = (a.rows + p.nt - 1) / p.nt, p.feat_tiles = (a.n + FL_M - 1) / FL_M;
+    p.sf_a = (unsigned)(FL_A + p.nt * 128), p.sf_b = p.sf_a + qs * 512;
+    p.stage_bytes = (p.sf_b + qs * 512 * (p.nt > 128 ? 2 : 1) + 1023) / 1024 * 1024;
+    p.slot = (unsigned)(qs * (4 + (p.nt > 128 ? 8 : 4)));
+    p.stages = (int)std::min<size_t>(FL_STAGES, (FL_SMEM - 1024) / p.stage_bytes);
+    p.stages = std::min<int>(p.stages, (int)((512 - p.acc_cols) / p.slot));
+    p.group = 8;
+    p.total = (long long)p.row_tiles * p.feat_tiles * p.steps;
+    p.blocks = (int)std::min<long long>(sms, (p.total + FL_MIN_STEPS - 1) / FL_MIN_STEPS);
+    return p;
+}
+
+size_t fp4_linear_workspace(int dtype, const Fp4LinearArgs &a, int sms) {
+    const FlPlan p = fl_plan(dtype, a, sms);
+    return sizeof(int) * KA_BLOCKS + (size_t)p.blocks * 2 * FL_M * p.nt * sizeof(float);
+}
+
+static bool fl_map(void *encode, CUtensorMap *m, const uint8_t *codes, int rows, int k, int box) {
+    const cuuint64_t dims[2] = {(cuuint64_t)fp4_padded(k) / 2, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)fp4_padded(k) / 2};
+    const cuuint32_t boxes[2] = {FL_STEP / 2, (cuuint32_t)box}, one[2] = {1, 1};
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(encode)(
+               m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DT, bool NV>
+static cudaError_t launch(const Fp4LinearArgs &a, const FlPlan &p, const CUtensorMap &w, const CUtensorMap &x, void *work, cudaStream_t s) {
+    const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
+    const cudaError_t e = allow_dynamic_smem((const void *)k_fp4_linear<DT, NV>, FL_SMEM);
+    if (e != cudaSuccess) return e;
+    int *arrived = reinterpret_cast<int *>(work);
+    k_fp4_linear<DT, NV><<<p.blocks, FL_THREADS, smem, s>>>(a, p, w, x, reinterpret_cast<float *>(arrived + KA_BLOCKS), arrived);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_fp4_linear(int dtype, const Fp4LinearArgs &a, int sms, void *encode, void *work, cudaStream_t s, uint64_t *launches) {
+    const FlPlan p = fl_plan(dtype, a, sms);
+    CUtensorMap w, x;
+    if (!encode || !fl_map(encode, &w, a.w, a.n, a.k, FL_M) || !fl_map(encode, &x, a.x, a.rows, a.k, p.nt)) return cudaErrorNotSupported;
+    (*launches)++;
+    const bool nv = a.format == FP4_NV;
+    return dtype == DT_F32   ? (nv ? launch<DT_F32, true>(a, p, w, x, work, s) : launch<DT_F32, false>(a, p, w, x, work, s))
+           : dtype == DT_F16 ? (nv ? launch<DT_F16, true>(a, p, w, x, work, s) : launch<DT_F16, false>(a, p, w, x, work, s))
+                             : (nv ? launch<DT_BF16, true>(a, p, w, x, work, s) : launch<DT_BF16, false>(a, p, w, x, work, s));
+}
+
+}  // namespace tcu

@@ -1,0 +1,222 @@
+"""A prompt's operators on the GPU against plain numpy in 64 bits."""
+import numpy as np
+import pytest
+
+import prompt_plain as plain
+from conftest import tcu
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": (0, torch.float32), "f16": (1, torch.float16), "bf16": (2, torch.bfloat16)}
+# half a unit in the last place of a result of each type, relative, and the smallest subnormal's half
+ULP = {"f32": 2.0**-24, "f16": 2.0**-11, "bf16": 2.0**-8}
+TINY = {"f32": 2.0**-150, "f16": 2.0**-25, "bf16": 2.0**-134}
+FORMATS = {"mx": plain.MX, "nv": plain.NV}
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    return tcu.Gpu(0)
+
+
+def dev(a, dtype=None):
+    t = torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return t if dtype is None else t.to(dtype)
+
+
+def host(t):
+    return t.double().cpu().numpy()
+
+
+def rounded(a, dtype):
+    """The numbers of a as the type holds them (f64 array)."""
+    return torch.from_numpy(np.ascontiguousarray(a, np.float64)).to(dtype).double().numpy()
+
+
+def sync(gpu):
+    torch.cuda.synchronize()
+    gpu.sync()
+
+
+class Matrix:
+    """An Fp4 with its buffers: packed by the library from x, or holding codes and scale bytes made by the plain form."""
+
+    def __init__(self, gpu, rows, k, fmt, unit=1.0, fill=0):
+        self.fmt, self.k, self.unit = fmt, k, unit
+        self.codes = torch.full((tcu.Fp4.code_bytes(rows, k),), fill, dtype=torch.uint8, device="cuda")
+        self.scales = torch.full((tcu.Fp4.scale_bytes(rows, k, fmt),), fill, dtype=torch.uint8, device="cuda")
+        self.m = tcu.Fp4(gpu, rows, k, fmt, self.codes.data_ptr(), self.scales.data_ptr(), unit=unit)
+
+    def put(self, code, byte):
+        packed, place = plain.stored(code, byte)
+        self.codes.copy_(dev(packed).flatten())
+        s = np.zeros(self.scales.numel(), np.uint8)
+        s[place] = byte
+        self.scales.copy_(dev(s))
+        return plain.values(code, byte, self.fmt, self.unit, self.k)
+
+
+def random_matrix(rng, gpu, rows, k, fmt, unit=1.0, spread=6):
+    """Codes of any number and scales over `spread` powers of two."""
+    kp = plain.padded(k)
+    code = rng.integers(0, 16, (rows, kp)).astype(np.uint8)
+    code[:, k:] = 0
+    count = kp // plain.BLOCK[fmt]
+    byte = rng.integers(127 - spread, 128, (rows, count)) if fmt == plain.MX else rng.integers(56 - 8 * spread, 57, (rows, count))
+    byte[:, -(-k // plain.BLOCK[fmt]):] = 0
+    m = Matrix(gpu, rows, k, fmt, unit)
+    return m, m.put(code, byte.astype(np.uint8))
+
+
+# ---- four-bit floating point ----------------------------------------------------------------------------------------
+
+def hard_rows(rng, k, fmt, unit, tt):
+    """Rows that meet the format's corners."""
+    x = rng.normal(0, 1, (200, k)) * 10.0 ** rng.uniform(-3, 3, (200, 1))
+    x[3] = 0
+    x[4, ::2] = -0.0
+    x[5, k // 2], x[6, 0], x[7, k - 1] = np.nan, np.inf, -np.inf
+    x[8] = 3e38 * rng.uniform(-1, 1, k)      # near f32's end
+    x[9] = 1e-40 * rng.normal(0, 1, k)       # subnormal in f32 and bf16
+    x[10] = 1e-30 * rng.normal(0, 1, k)
+    x[11], x[11, 1::2] = 1e-3, 1.0           # small beside large
+    # every border of a number, both sides: one number of magnitude 6 a block, the others on borders
+    b = np.concatenate([plain.MIDDLES, -plain.MIDDLES])
+    for i, off in enumerate((0, 2.0**-9, -2.0**-9, 2.0**-22, -2.0**-22)):
+        row = np.resize(b * (1 + off), k)
+        row[::8] = 6
+        x[12 + i] = row * unit
+        x[17 + i] = row * unit * 1.125
+        x[22 + i] = row * unit * 448
+        x[27 + i] = row * unit * 2.0**-9
+    # borders of a scale: the largest of a block 6 unit times the middle of two scales
+    mid = (plain.E4M3[1:] + plain.E4M3[:-1]) / 2
+    for i in range(60):
+        x[40 + i] = rng.uniform(-1, 1, k) * mid[2 * i] * 6 * unit
+        x[40 + i, ::16] = mid[2 * i] * 6 * unit * (1, 1, 1 + 2.0**-23, 1 - 2.0**-23)[i % 4]
+    with np.errstate(over="ignore"):
+        return rounded(x, tt)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("name", ["mx", "nv"])
+@pytest.mark.parametrize("k,unit", [(128, 1.0), (16, 1.0), (1, 2.0**-7), (130, 0.3), (2050, 0.0123), (200, 1e-30), (256, 1e30)])
+def test_pack_and_load(gpu, dtype, name, k, unit):
+    code, tt = DT[dtype]
+    fmt = FORMATS[name]
+    unit = float(np.float32(unit)) if fmt == plain.NV else 1.0
+    x = hard_rows(np.random.default_rng(k), k, fmt, unit, tt)
+    rows = len(x)
+    for pad, at in ((0, 0), (3, 1)):  # aligned where the width is, and not
+        buf = torch.full((rows * (k + pad) + at,), 7.0, dtype=tt, device="cuda")
+        xd = torch.as_strided(buf, (rows, k), (k + pad, 1), at)
+        xd.copy_(dev(x))
+        m = Matrix(gpu, rows, k, fmt, unit, fill=0xA5)
+        m.m.pack(code, xd.data_ptr(), k + pad, stream=1)
+        out = torch.full_like(buf, 9.0)
+        yd = torch.as_strided(out, (rows, k), (k + pad, 1), at)
+        m.m.load(code, yd.data_ptr(), k + pad, stream=1)
+        sync(gpu)
+        want_codes, byte = plain.quantise(x, fmt, unit)
+        packed, place = plain.stored(want_codes, byte)
+        got_codes, got_byte = m.codes.cpu().numpy().reshape(rows, -1), m.scales.cpu().numpy()[place]
+        assert np.array_equal(got_byte, byte)
+        assert np.array_equal(got_codes, packed)
+        n = plain.values(want_codes, byte, fmt, 1.0, k)          # number * scale: exact in f32
+        with np.errstate(over="ignore"):
+            want = rounded(rounded(n * unit, torch.float32), tt)  # one rounding to f32, one to the type
+        assert np.array_equal(host(yd), want, equal_nan=True)
+        rest = torch.ones_like(out, dtype=torch.bool)
+        torch.as_strided(rest, (rows, k), (k + pad, 1), at).fill_(False)
+        assert (out[rest] == 9).all()                            # nothing beside the rows
+
+
+def test_pack_writes_no_row_behind_the_last(gpu):
+    """Scales of rows that the matrix does not have are left as they were."""
+    m = Matrix(gpu, 130, 64, plain.NV, fill=0xA5)
+    x = torch.ones(130, 64, device="cuda")
+    m.m.pack(0, x.data_ptr(), 64, stream=1)
+    sync(gpu)
+    s = m.scales.cpu().numpy()
+    _, place = plain.stored(np.zeros((130, 128), np.uint8), np.zeros((130, 8), np.uint8))
+    rest = np.ones(s.size, bool)
+    rest[place] = False
+    assert (s[rest] == 0xA5).all() and rest.sum() == 2 * 2 * 512 - 130 * 8
+
+
+LINEAR = [  # rows, n, k
+    (1, 1, 1), (1, 128, 128), (1, 1024, 512), (3, 200, 130), (8, 4097, 700), (16, 256, 256), (17, 130, 2050), (33, 100, 512),
+    (64, 1000, 1000), (65, 129, 384), (127, 300, 100), (128, 512, 1024), (129, 513, 640), (256, 128, 64), (257, 1000, 2000), (600, 700, 900),
+]
+
+
+def check_linear(gpu, rng, dtype, fmt, rows, n, k, act, bias, residual, ux=1.0, uw=1.0, exact=False):
+    code, tt = DT[dtype]
+    spread = 2 if exact else 6
+    x, xv = random_matrix(rng, gpu, rows, k, fmt, ux, spread)
+    w, wv = random_matrix(rng, gpu, n, k, fmt, uw, spread)
+    b = rounded(rng.normal(0, 1, n), tt) if bias else None
+    r = rounded(rng.normal(0, 1, (rows, n)), tt) if residual else None
+    yd = torch.full((rows, n + 3), 9.0, dtype=tt, device="cuda")
+    if residual:
+        yd[:, :n] = dev(r, tt)  # in place: the residual is the output's own buffer
+    bd = dev(b, tt) if bias else None
+    work = torch.zeros(w.m.linear_workspace(x.m, code), dtype=torch.uint8, device="cuda")
+    w.m.linear(x.m, code, yd.data_ptr(), n + 3, bias=bd.data_ptr() if bias else None, act=act, residual=yd.data_ptr() if residual else None,
+               ldr=n + 3, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    y, size = xv @ wv.T, np.abs(xv) @ np.abs(wv).T
+    got = host(yd)
+    assert (got[:, n:] == 9).all()
+    if exact:
+        assert np.array_equal(got[:, :n], rounded(y, tt))
+        return
+    # a sum of 64 products is added to the one before at a time, each addition off by a unit in the last place of f32 (the matrix
+    # unit does not round to nearest); f32 results add four steps of 4 such sums at a time
+    adds = -(-k // 64) + 8 if dtype != "f32" else 16 + -(-k // 1024) + 8
+    tol = adds * 2.0**-23 * size
+    if bias:
+        y, tol = y + b, tol + 2.0**-23 * np.abs(b)
+    if act:
+        erf = torch.erf(torch.from_numpy(y / np.sqrt(2))).numpy()
+        y, tol = 0.5 * y * (1 + erf), 1.13 * tol + 2.0**-20 * np.abs(y)  # the slope of GELU is below 1.13; its erf is good to 2^-21
+    if residual:
+        y, tol = y + r, tol + 2.0**-23 * np.abs(r)
+    assert (np.abs(got[:, :n] - y) <= tol + 2 * ULP[dtype] * np.abs(y) + TINY[dtype]).all()
+    counters = work[:8192].cpu().numpy()
+    assert not counters.any()  # left as the next call needs them
+
+
+@pytest.mark.parametrize("name", ["mx", "nv"])
+@pytest.mark.parametrize("rows,n,k", [(1, 128, 128), (16, 128, 128), (16, 256, 256), (130, 140, 256), (300, 200, 512), (20, 300, 2050)])
+def test_linear_exact(gpu, name, rows, n, k):
+    """Scales of a few powers of two: every sum of products is a number that f32 holds, whatever the order."""
+    rng = np.random.default_rng(rows + n + k)
+    fmt = FORMATS[name]
+    x, xv = random_matrix(rng, gpu, rows, k, fmt, spread=2)
+    w, wv = random_matrix(rng, gpu, n, k, fmt, spread=2)
+    if fmt == plain.NV:  # whole powers of two among the e4m3 floats
+        for m, rws in ((x, rows), (w, n)):
+            code = rng.integers(0, 16, (rws, plain.padded(k))).astype(np.uint8)
+            code[:, k:] = 0
+            byte = (rng.integers(5, 8, (rws, plain.padded(k) // 16)) * 8).astype(np.uint8)
+            if m is x:
+                xv = m.put(code, byte)
+            else:
+                wv = m.put(code, byte)
+    y = torch.full((rows, n), 9.0, device="cuda")
+    work = torch.zeros(w.m.linear_workspace(x.m, 0), dtype=torch.uint8, device="cuda")
+    w.m.linear(x.m, 0, y.data_ptr(), n, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    # products are multiples of 2^-2 * 2^-4, sums below 36 * 4 * k: 22 bits at most
+    assert np.array_equal(host(y), xv @ wv.T)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("name", ["mx", "nv"])
+@pytest.mark.parametrize("rows,n,k", LINEAR)
+def test_linear(gpu, dtype, name, rows, n, k):
+    rng = np.random.default_rng(rows * 7 + n + k)
+    ux, uw = (0.37, 0.0021) if name == "nv" else (1.0, 1.0)
+    check_linear(gpu, rng, dtype, FORMATS[name], rows, n, k, act=rows % 2, bias=n % 3 > 0, residual=k % 3 > 0, ux=ux, uw=uw)
