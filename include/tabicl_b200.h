@@ -527,6 +527,26 @@ TCU_API size_t tcu_fp4_linear_workspace(tcu_ctx *ctx, const tcu_fp4 *w, const tc
 TCU_API int tcu_fp4_linear_device(tcu_ctx *ctx, const tcu_fp4 *w, const tcu_fp4 *x, int dtype, void *y, int64_t ldy, const void *bias,
                                   int act, const void *residual, int64_t ldr, void *work, size_t work_bytes, void *stream);
 
+/* Packed sequences: query rows q_starts[s] .. q_starts[s + 1] of q_rows belong to sequence s, and keys and values k_starts[s] ..
+ * k_starts[s + 1] of k_rows (k_starts NULL: the queries' own rows); at most max_q rows and max_k keys each. Starts are device
+ * memory, seqs + 1 of them, not decreasing. Rows that no sequence has are left as they were. */
+typedef struct tcu_packed {
+    int32_t seqs, q_rows, k_rows, max_q, max_k;
+    const int32_t *q_starts, *k_starts;
+} tcu_packed;
+TCU_API size_t tcu_packed_attend_workspace(tcu_ctx *ctx, const tcu_packed *p, int dtype, int q_heads, int heads, int width); /* (size_t)-1: refused */
+/* Softmax attention: out = sum_j p_j v_j with p the softmax of scale * q . k_j over the keys of its sequence that a row sees.
+ * Query head h reads key and value head h / (q_heads / heads). Without `causal` a row sees all of them; with it, row i of a
+ * sequence's n sees the keys up to (keys - n + i), and with window > 0 only the last `window` of those. A row that sees nothing
+ * gives zeros. What a row does not see has no part in its result, NaN and infinities neither. lse (may be NULL): [q_rows][q_heads],
+ * the logarithm of the sum of e^score, -infinity for a row that sees nothing. width: a multiple of 8, up to 256. Sums, weights'
+ * sums and lse are f32 for every type; the weights that multiply 16-bit values are rounded to their type, f32 values and weights
+ * are taken as two tf32 (22 bits). Strides in elements. */
+TCU_API int tcu_packed_attend_device(tcu_ctx *ctx, const tcu_packed *p, int dtype, int q_heads, int heads, int width, const void *q,
+                                     int64_t q_row, int64_t q_head, const void *k, int64_t k_row, int64_t k_head, const void *v,
+                                     int64_t v_row, int64_t v_head, void *out, int64_t o_row, int64_t o_head, float scale, int causal,
+                                     int window, float *lse, void *work, size_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

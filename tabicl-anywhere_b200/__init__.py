@@ -8,7 +8,8 @@ The objects mirror the reference's accelerator side (src/gpu.rs, src/predict.rs:
 * `VramMember` - a fitted member's problems and its class tree, predicted whole (predict::predict_raw)
 * `VramTier` / `VramHandle` - problems resident for many tenants within byte budgets; the handle is an AttendCached
 * `Kv4Cache`, `W4` - the four-bit cache and weights (fourbit.py; no counterpart in the reference)
-* `Fp4` - matrices in four-bit floating point and their products (prompt.py; no counterpart in the reference)
+* `Fp4`, `Packed` - matrices in four-bit floating point and their products, and attention of packed rows (prompt.py; no
+  counterpart in the reference)
 * `CudaAttend` - the `AttendCached` implementation: `attend`, `stage`, `rows`, each returning None to decline
 
 Everything computes on the GPU through libtabicl_b200.so; there is no CPU path here. The library is built in-tree
@@ -1005,4 +1006,4 @@ class CudaAttend:
 
 
 from .fourbit import BF16, F16, F32, Kv4Cache, W4  # noqa: E402,F401  (they use lib() and Gpu)
-from .prompt import MX, NV, Fp4  # noqa: E402,F401
+from .prompt import MX, NV, Fp4, Packed  # noqa: E402,F401

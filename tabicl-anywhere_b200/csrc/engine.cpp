@@ -28,6 +28,7 @@
 #include "fp4.cuh"
 #include "kernels.cuh"
 #include "engine.hpp"
+#include "packed.cuh"
 #include "tirs.hpp"
 
 namespace tcu {
@@ -1023,7 +1024,7 @@ static void check_device_error(tcu_ctx *ctx) {
                                ". Outputs of the calls queued since the last report are invalid");
     if (slot[ERR_INDEX]) {
         slot[ERR_INDEX] = 0;
-        fail(TCU_ERR_ARG, "a four-bit operator or label_logprobs met a slot, page, length, start or label outside its range "
+        fail(TCU_ERR_ARG, "a four-bit or prompt operator or label_logprobs met a slot, page, length, start or label outside its range "
                           "since the last report; nothing was read or written there");
     }
 }
@@ -3533,6 +3534,66 @@ int tcu_fp4_linear_device(tcu_ctx *ctx, const tcu_fp4 *w, const tcu_fp4 *x, int 
         check_aligned("fp4_linear", "working memory", work, 16);
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
         Launch{ctx, s}(launch_fp4_linear(dtype, a, ctx->sms, (void *)tensor_map_encoder(), work, s, &ctx->launches), "fp4_linear");
+        return TCU_OK;
+    });
+}
+
+static PackedArgs packed_args(const tcu_packed *p, int dtype, int q_heads, int heads, int width) {
+    if (!p) fail(TCU_ERR_ARG, "packed_attend: null batch");
+    check_dtype("packed_attend", dtype);
+    if (heads < 1 || heads > 1024 || q_heads < 1 || q_heads > 65535 || q_heads % heads)
+        fail(TCU_ERR_ARG, "packed_attend: heads 1..1024, and query heads a multiple of them");
+    if (width < 8 || width > 256 || width % 8) fail(TCU_ERR_ARG, "packed_attend: width must be a multiple of 8, up to 256");
+    if (p->seqs < 0 || p->seqs > 65535 || p->q_rows < 0 || p->k_rows < 0 || p->max_q < 0 || p->max_k < 0)
+        fail(TCU_ERR_ARG, "packed_attend: 0..65535 sequences, rows and lengths not negative");
+    if ((long long)p->q_rows * q_heads > 0x7fffffffLL / 256) fail(TCU_ERR_ARG, "packed_attend: too many query rows for one call");
+    PackedArgs a;
+    a.c.heads = heads, a.seqs = p->seqs, a.rows = p->q_rows, a.k_rows = p->k_starts ? p->k_rows : p->q_rows;
+    // (no sequence has more rows than there are)
+    a.max_rows = std::min(p->max_q, a.rows), a.max_len = std::min(p->max_k, a.k_rows), a.q_starts = p->q_starts;
+    a.k_starts = p->k_starts ? p->k_starts : p->q_starts, a.q_heads = q_heads, a.width = width;
+    return a;
+}
+
+size_t tcu_packed_attend_workspace(tcu_ctx *ctx, const tcu_packed *p, int dtype, int q_heads, int heads, int width) {
+    size_t need = 0;
+    const int r = guarded(ctx, [&]() -> int {
+        const PackedArgs a = packed_args(p, dtype, q_heads, heads, width);
+        need = a.seqs && a.rows && a.max_rows ? packed_attend_workspace(dtype, a, ctx->sms) : 0;
+        return TCU_OK;
+    });
+    return r == TCU_OK ? need : (size_t)-1;
+}
+
+int tcu_packed_attend_device(tcu_ctx *ctx, const tcu_packed *p, int dtype, int q_heads, int heads, int width, const void *q, int64_t q_row,
+                             int64_t q_head, const void *k, int64_t k_row, int64_t k_head, const void *v, int64_t v_row, int64_t v_head,
+                             void *out, int64_t o_row, int64_t o_head, float scale, int causal, int window, float *lse, void *work,
+                             size_t work_bytes, void *stream) {
+    return guarded(ctx, [&]() -> int {
+        check_device_error(ctx);
+        PackedArgs a = packed_args(p, dtype, q_heads, heads, width);
+        if (window < 0 || (window && !causal)) fail(TCU_ERR_ARG, "packed_attend: a window is not negative and goes with causal");
+        if (!std::isfinite(scale)) fail(TCU_ERR_ARG, "packed_attend: scale must be finite");
+        if (q_row < 0 || q_head < 0 || k_row < 0 || k_head < 0 || v_row < 0 || v_head < 0 || o_row < 0 || o_head < 0)
+            fail(TCU_ERR_ARG, "packed_attend: strides must not be negative");
+        if (!a.seqs || !a.rows || !a.max_rows) return TCU_OK;
+        if (!q || !out || !a.q_starts || (a.max_len && (!k || !v))) fail(TCU_ERR_ARG, "packed_attend: null queries, keys, values, output or starts");
+        const size_t size = elem_size(dtype);
+        check_aligned("packed_attend", "queries", q, size), check_aligned("packed_attend", "keys", k, size);
+        check_aligned("packed_attend", "values", v, size), check_aligned("packed_attend", "output", out, size);
+        check_aligned("packed_attend", "starts", a.q_starts, 4), check_aligned("packed_attend", "starts", a.k_starts, 4);
+        check_aligned("packed_attend", "lse", lse, 4);
+        a.q = q, a.k = k, a.v = v, a.out = out, a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row;
+        a.v_head = v_head, a.o_row = o_row, a.o_head = o_head;
+        // (no row sees more than max_k keys: a wider window hides nothing, and would pass 32 bits in the rows' bounds)
+        if (window >= a.max_len) window = 0;
+        a.scale = scale, a.causal = causal != 0, a.window = window, a.lse = lse, a.err = ctx->err_mapped + ERR_INDEX;
+        a.err_wait = ctx->err_mapped + ERR_ATTEND_TC;
+        const size_t need = packed_attend_workspace(dtype, a, ctx->sms);
+        if (need && (!work || work_bytes < need)) fail(TCU_ERR_ARG, "packed_attend: needs " + std::to_string(need) + " bytes of working memory");
+        check_aligned("packed_attend", "working memory", work, 16);
+        cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        Launch{ctx, s}(launch_packed_attend(dtype, a, ctx->sms, (void *)tensor_map_encoder(), work, s, &ctx->launches), "packed_attend");
         return TCU_OK;
     });
 }

@@ -1,4 +1,4 @@
-// How the attention over the four-bit cache is cut into work, from lengths that only the device has.
+// How attention, over the four-bit cache or over packed keys, is cut into work, from lengths that only the device has.
 //
 // A unit of work is a row tile (R query rows: a sequence's rows, the heads that share a cache head innermost) of one cache
 // head, over the keys that its rows see, in steps of STEP keys that begin at a multiple of ALIGN. The steps of all units in
@@ -40,10 +40,12 @@ __device__ __forceinline__ KaRows ka_rows(const Kv4AttendArgs &a, int seq) {
     return r;
 }
 // Row i of a sequence sees the tokens [ka_lo, ka_hi); both grow with i.
-__device__ __forceinline__ int ka_hi(const Kv4AttendArgs &a, const KaRows &s, int i) {
+template <class A>
+__device__ __forceinline__ int ka_hi(const A &a, const KaRows &s, int i) {
     return a.causal ? max(0, min(s.len, s.len - s.n + i + 1)) : s.len;
 }
-__device__ __forceinline__ int ka_lo(const Kv4AttendArgs &a, const KaRows &s, int i) {
+template <class A>
+__device__ __forceinline__ int ka_lo(const A &a, const KaRows &s, int i) {
     return a.window ? max(0, s.len - s.n + i + 1 - a.window) : 0;
 }
 
@@ -56,7 +58,8 @@ struct KaCut {
     struct Span {
         int lo_min, lo_max, hi_min, hi_max, base, steps;  // what the tile's first and last rows see; where its steps begin
     };
-    static __device__ __forceinline__ Span span(const Kv4AttendArgs &a, const KaRows &s, int each, int rt) {
+    template <class A>
+    static __device__ __forceinline__ Span span(const A &a, const KaRows &s, int each, int rt) {
         const int first = rt * R / each, last = (min(s.n * each, (rt + 1) * R) - 1) / each;
         Span p;
         p.lo_min = ka_lo(a, s, first), p.lo_max = ka_lo(a, s, last), p.hi_min = ka_hi(a, s, first), p.hi_max = ka_hi(a, s, last);
@@ -64,7 +67,8 @@ struct KaCut {
         p.steps = p.hi_max > p.lo_min ? (p.hi_max - p.base + STEP - 1) / STEP : 1;  // no keys: a step that writes zeros
         return p;
     }
-    static __device__ __forceinline__ long long seq_steps(const Kv4AttendArgs &a, int seq, int each) {  // a head's
+    template <class A>
+    static __device__ __forceinline__ long long seq_steps(const A &a, int seq, int each) {  // a head's
         const KaRows s = ka_rows(a, seq);
         if (!s.ok) {
             *reinterpret_cast<volatile int *>(a.err) = 1;
@@ -83,8 +87,8 @@ struct KaCut {
         int seq, rt, head, skip;
     };
     // Called by all THREADS threads of the block (of which it uses the barrier); sums and unit are shared memory.
-    template <int THREADS>
-    static __device__ __forceinline__ Place place(const Kv4AttendArgs &a, int each, int min_steps, long long (&sums)[THREADS / 32],
+    template <int THREADS, class A>
+    static __device__ __forceinline__ Place place(const A &a, int each, int min_steps, long long (&sums)[THREADS / 32],
                                                   int (&unit)[4]) {
         const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
         // the threads' numbers before this one's, and all of them
@@ -175,7 +179,8 @@ struct KaCut {
         if (blockIdx.x < p.blocks) p.pos = ka_div(total * blockIdx.x, p.blocks), p.end = ka_div(total * (blockIdx.x + 1), p.blocks);
     }
     // On to the next unit, `piece` steps on.
-    static __device__ __forceinline__ void next(Place &p, const Kv4AttendArgs &a, int each, int n, int piece) {
+    template <class A>
+    static __device__ __forceinline__ void next(Place &p, const A &a, int each, int n, int piece) {
         p.pos += piece, p.skip = 0;
         if (++p.head < a.c.heads) return;
         p.head = 0;

@@ -1,0 +1,420 @@
+// Attention of packed rows over keys and values as they are, for few rows of any type, and for what the tensor-core kernel
+// (packed_attend_tc.cu) does not take: f32, widths above 128, rows that TMA cannot fetch.
+//
+// 16 or 64 query rows of one key head (the heads that share it side by side) against steps of 64 keys (f32: 32) that come by
+// asynchronous copies. With 16 rows the four warps share a step's keys, with 64 its rows. One pass: running maxima and sums, the
+// output in registers, the matrix products by warp (16-bit operands as they are; f32 as two tf32, of 11 bits each, in three
+// products). A call of few rows streams its keys and values, so it is bound by memory; the steps of all sequences are cut evenly
+// over the blocks (kv4_plan.cuh), whose parts the last of them joins in order.
+#include <algorithm>
+#include <type_traits>
+
+#include "packed.cuh"
+
+namespace tcu {
+
+constexpr int PA_THREADS = 128;
+// Steps a block takes at least: shorter parts of a unit are more to join.
+constexpr int PA_STEPS = 4;
+
+template <int DT, int HD, int WR>
+struct PaShape {
+    using T = typename Elem<DT>::T;
+    static constexpr bool F32 = DT == DT_F32;
+    using Raw = std::conditional_t<F32, uint32_t, uint16_t>;
+    static constexpr int R = 16 * WR, KW = 4 / WR, BK = F32 ? 32 : 64, OWN = BK / KW;
+    static constexpr int PITCH = HD * (int)sizeof(T) + 16;  // bytes of a row: rows 4 banks apart
+    static constexpr int STAGES = !F32 && WR == 1 && HD <= 128 ? 3 : 2;
+    static constexpr int TILE = BK * PITCH, CP = HD + 4;
+    static constexpr size_t SMEM = (size_t)STAGES * 2 * TILE + R * PITCH;
+    static constexpr size_t PART = (size_t)R * (HD + 2);  // floats of a part: outputs, maxima, sums
+    static_assert((size_t)64 * CP * 4 + 512 <= (size_t)STAGES * 2 * TILE, "the warps' outputs meet where keys and values were");
+};
+
+__device__ __forceinline__ uint32_t pa_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void pa_ldsm(uint32_t at, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void pa_ldsm_t(uint32_t at, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <int DT>
+__device__ __forceinline__ void pa_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (DT == DT_F16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else if constexpr (DT == DT_BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo, two tf32 (11 bits each, rounded to nearest).
+__device__ __forceinline__ void pa_split(float x, uint32_t &hi, uint32_t &lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+__device__ __forceinline__ float pa_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pa_pair(float x, float y) {
+    if constexpr (DT == DT_F16) {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+// Rows [0, n) of `width` elements, `row` elements apart, into shared rows of PITCH bytes, by all threads; rows outside [lo, hi)
+// are zeros. Whole 16-byte pieces asynchronously where they are aligned.
+template <class C>
+__device__ __forceinline__ void pa_copy(uint8_t *to, const void *base, long long first, long long row, int lo, int hi, int width, bool wide) {
+    using Raw = typename C::Raw;
+    constexpr int PER = 16 / (int)sizeof(Raw);
+    const Raw *from = reinterpret_cast<const Raw *>(base);
+    if (wide) {
+        const int pieces = width / PER;
+        for (int i = threadIdx.x; i < C::BK * pieces; i += PA_THREADS) {
+            const int r = i / pieces, c = i - r * pieces;
+            const bool in = r >= lo && r < hi;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(pa_smem(to + r * C::PITCH + c * 16)),
+                         "l"(in ? from + first + r * row + c * PER : from), "r"(in ? 16 : 0)
+                         : "memory");
+        }
+    } else {
+        for (int i = threadIdx.x; i < C::BK * width; i += PA_THREADS) {
+            const int r = i / width, c = i - r * width;
+            *reinterpret_cast<Raw *>(to + r * C::PITCH + c * sizeof(Raw)) = r >= lo && r < hi ? from[first + r * row + c] : Raw(0);
+        }
+    }
+}
+
+template <int DT, int HD, int WR>
+__global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int wide, float *part, int *arrived) {
+    using C = PaShape<DT, HD, WR>;
+    using T = typename C::T;
+    using Raw = typename C::Raw;
+    using Cut = KaCut<C::R, 1, C::BK>;
+    constexpr int R = C::R, KW = C::KW, BK = C::BK, OWN = C::OWN, NT = OWN / 8, NO = HD / 8, STAGES = C::STAGES, PITCH = C::PITCH, CP = C::CP;
+    extern __shared__ __align__(16) uint8_t sm[];
+    uint8_t *Qs = sm + (size_t)STAGES * 2 * C::TILE;
+    __shared__ long long s_sum[PA_THREADS / 32];
+    __shared__ int s_unit[4], s_last;
+    __shared__ int s_bad[R];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, wr = warp % WR, kw = warp / WR;
+    const int each = a.q_heads / a.c.heads;
+    const float sl = a.scale * 1.44269504088896340736f;
+    auto pl = Cut::template place<PA_THREADS>(a, each, PA_STEPS, s_sum, s_unit);
+    while (pl.pos < pl.end) {
+        const KaRows sr = ka_rows(a, pl.seq);
+        const auto sp = Cut::span(a, sr, each, pl.rt);
+        const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), j0 = sp.base + pl.skip * BK, k0 = a.k_starts[pl.seq];
+        const int r0 = pl.rt * R, rows = min(R, sr.n * each - r0);
+        __syncthreads();  // the piece before is done with shared memory
+        if (a.width < HD) {
+            for (int i = tid; i < (int)(C::SMEM / 16); i += PA_THREADS) reinterpret_cast<uint4 *>(sm)[i] = make_uint4(0, 0, 0, 0);
+            __syncthreads();
+        }
+        for (int i = tid; i < rows * a.width; i += PA_THREADS) {
+            const int r = i / a.width, c = i - r * a.width, p = r0 + r;
+            *reinterpret_cast<Raw *>(Qs + r * PITCH + c * sizeof(T)) =
+                reinterpret_cast<const Raw *>(a.q)[(long long)(sr.first + p / each) * a.q_row + (long long)(pl.head * each + p % each) * a.q_head + c];
+        }
+        auto load = [&](int i) {
+            const int at = j0 + i * BK, slot = i % STAGES;
+            if (i < n) {
+                pa_copy<C>(sm + (size_t)slot * 2 * C::TILE, a.k, (long long)(k0 + at) * a.k_row + pl.head * a.k_head, a.k_row, 0, sp.hi_max - at, a.width, wide & 1);
+                pa_copy<C>(sm + (size_t)(slot * 2 + 1) * C::TILE, a.v, (long long)(k0 + at) * a.v_row + pl.head * a.v_head, a.v_row, 0, sp.hi_max - at, a.width,
+                           wide & 2);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; i++) load(i);
+
+        // this thread's rows of a fragment: g and g + 8
+        int lo[2], hi[2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int r = 16 * wr + g + 8 * x, i = (r0 + r) / each;
+            lo[x] = r < rows ? ka_lo(a, sr, i) : 0, hi[x] = r < rows ? ka_hi(a, sr, i) : 0;
+        }
+        float o[NO][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < NO; i++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) o[i][x] = 0.f;
+
+        for (int i = 0; i < n; i++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+            __syncthreads();
+            load(i + STAGES - 1);
+            const uint8_t *ks = sm + (size_t)(i % STAGES) * 2 * C::TILE + kw * OWN * PITCH, *vs = ks + C::TILE;
+            float s[NT][4];
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) s[x][y] = 0.f;
+            if constexpr (C::F32) {
+                const float *qf = reinterpret_cast<const float *>(Qs + (16 * wr + g) * PITCH);
+#pragma unroll 2
+                for (int c = 0; c < HD; c += 8) {
+                    uint32_t h[4], lw[4];
+                    pa_split(qf[c + t], h[0], lw[0]), pa_split(qf[8 * PITCH / 4 + c + t], h[1], lw[1]);
+                    pa_split(qf[c + t + 4], h[2], lw[2]), pa_split(qf[8 * PITCH / 4 + c + t + 4], h[3], lw[3]);
+#pragma unroll
+                    for (int x = 0; x < NT; x++) {
+                        const float *kf = reinterpret_cast<const float *>(ks + (8 * x + g) * PITCH) + c + t;
+                        uint32_t bh[2], bl[2];
+                        pa_split(kf[0], bh[0], bl[0]), pa_split(kf[4], bh[1], bl[1]);
+                        pa_mma<DT>(s[x], lw, bh[0], bh[1]);
+                        pa_mma<DT>(s[x], h, bl[0], bl[1]);
+                        pa_mma<DT>(s[x], h, bh[0], bh[1]);
+                    }
+                }
+            } else {
+                const uint32_t qa = pa_smem(Qs + (16 * wr + (lane & 15)) * PITCH + (lane >> 4) * 16);
+                const uint32_t ka = pa_smem(ks + ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16);
+#pragma unroll
+                for (int c = 0; c < HD / 16; c++) {
+                    uint32_t q[4];
+                    pa_ldsm(qa + c * 32, q);
+#pragma unroll
+                    for (int x = 0; x < NT; x += 2) {
+                        uint32_t b[4];
+                        pa_ldsm(ka + 8 * x * PITCH + c * 32, b);
+                        pa_mma<DT>(s[x], q, b[0], b[1]), pa_mma<DT>(s[x + 1], q, b[2], b[3]);
+                    }
+                }
+            }
+            // scores in units of log2; what a row does not see goes, whatever it is
+            const int at = j0 + i * BK + kw * OWN + 2 * t;
+            const bool edge = j0 + i * BK < sp.lo_max || j0 + (i + 1) * BK > sp.hi_min || rows < R;
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const int j = at + 8 * x + (y & 1);
+                    float v = s[x][y] * sl;
+                    if (edge && (j < lo[y >> 1] || j >= hi[y >> 1])) v = -INFINITY;
+                    s[x][y] = v, top[y >> 1] = fmaxf(top[y >> 1], v);
+                }
+            float f[2], ref[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+                top[x] = fmaxf(fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2)), m[x]);
+                ref[x] = top[x] == -INFINITY ? 0.f : top[x];
+                f[x] = m[x] == -INFINITY ? 0.f : pa_ex2(m[x] - ref[x]);
+            }
+            if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+#pragma unroll
+                for (int x = 0; x < NO; x++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        if (m[y >> 1] != -INFINITY) o[x][y] *= f[y >> 1];
+                l[0] *= f[0], l[1] *= f[1], m[0] = top[0], m[1] = top[1];
+            }
+#pragma unroll
+            for (int x = 0; x < NT; x++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) s[x][y] = pa_ex2(s[x][y] - ref[y >> 1]), l[y >> 1] += s[x][y];
+            if constexpr (C::F32) {
+                // A fragment's k takes the keys in the order in which a thread has their weights: k = t key 2 t, k = t + 4 key 2 t + 1.
+                // The unit does not round its sums to nearest, so each step's are its own, added here (over 10,000 keys 2.8e-5 of
+                // an output otherwise).
+                uint32_t h[NT][4], lw[NT][4];
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+                    pa_split(s[x][0], h[x][0], lw[x][0]), pa_split(s[x][2], h[x][1], lw[x][1]), pa_split(s[x][1], h[x][2], lw[x][2]), pa_split(s[x][3], h[x][3], lw[x][3]);
+#pragma unroll
+                for (int c = 0; c < NO; c++) {
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int x = 0; x < NT; x++) {
+                        const float *vf = reinterpret_cast<const float *>(vs + (8 * x + 2 * t) * PITCH) + 8 * c + g;
+                        uint32_t bh[2], bl[2];
+                        pa_split(vf[0], bh[0], bl[0]), pa_split(vf[PITCH / 4], bh[1], bl[1]);
+                        pa_mma<DT>(sum, lw[x], bh[0], bh[1]);
+                        pa_mma<DT>(sum, h[x], bl[0], bl[1]);
+                        pa_mma<DT>(sum, h[x], bh[0], bh[1]);
+                    }
+#pragma unroll
+                    for (int y = 0; y < 4; y++) o[c][y] += sum[y];
+                }
+            } else {
+                const uint32_t va = pa_smem(vs + (lane & 15) * PITCH + (lane >> 4) * 16);
+#pragma unroll
+                for (int x = 0; x < NT; x += 2) {
+                    const uint32_t p[4] = {pa_pair<DT>(s[x][0], s[x][1]), pa_pair<DT>(s[x][2], s[x][3]), pa_pair<DT>(s[x + 1][0], s[x + 1][1]),
+                                           pa_pair<DT>(s[x + 1][2], s[x + 1][3])};
+#pragma unroll
+                    for (int c = 0; c < NO; c += 2) {
+                        uint32_t b[4];
+                        pa_ldsm_t(va + 8 * x * PITCH + c * 16, b);
+                        pa_mma<DT>(o[c], p, b[0], b[1]), pa_mma<DT>(o[c + 1], p, b[2], b[3]);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+        }
+        __syncthreads();
+
+        // ---- the warps' outputs meet: [KW][R][HD], and maxima and sums [KW][R] ----
+        float *oc = reinterpret_cast<float *>(sm), *mc = oc + 64 * CP, *lc = mc + 64;
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int r = kw * R + 16 * wr + g + 8 * x;
+            if (t == 0) mc[r] = m[x], lc[r] = l[x];
+#pragma unroll
+            for (int c = 0; c < NO; c++) *reinterpret_cast<float2 *>(oc + r * CP + 8 * c + 2 * t) = make_float2(o[c][2 * x], o[c][2 * x + 1]);
+        }
+        __syncthreads();
+        const bool whole = n == sp.steps;
+        const int2 who = Cut::sharers(pl, pl.pos - pl.skip, sp.steps);
+        const int cols = (a.width + 3) / 4;
+        // one row's `parts` states joined in 4 columns; at(p): where part p's outputs of the row lie, its maximum and its sum
+        auto join = [&](int parts, auto at, float4 &v, float &M, float &L) {
+            M = -INFINITY, L = 0.f, v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int p = 0; p < parts; p++) M = fmaxf(M, *at(p).m);
+            const float ref = M == -INFINITY ? 0.f : M;
+            for (int p = 0; p < parts; p++) {
+                const auto from = at(p);
+                if (*from.m == -INFINITY && *from.l == 0.f) continue;
+                const float w = pa_ex2(*from.m - ref);
+                const float4 x = *reinterpret_cast<const float4 *>(from.o);
+                L = fmaf(w, *from.l, L), v.x = fmaf(w, x.x, v.x), v.y = fmaf(w, x.y, v.y), v.z = fmaf(w, x.z, v.z), v.w = fmaf(w, x.w, v.w);
+            }
+        };
+        struct From {
+            const float *o, *m, *l;
+        };
+        bool write = true;
+        if (!whole) {
+            float *mine = part + Cut::slot(blockIdx.x, pl.skip == 0) * C::PART;
+            for (int i = tid; i < rows * cols; i += PA_THREADS) {
+                const int r = i / cols, c = (i - r * cols) * 4;
+                float4 v;
+                float M, L;
+                join(KW, [&](int p) { return From{oc + (p * R + r) * CP + c, mc + p * R + r, lc + p * R + r}; }, v, M, L);
+                __stcg(reinterpret_cast<float4 *>(mine + r * HD + c), v);
+                if (c == 0) __stcg(mine + R * HD + r, M), __stcg(mine + R * HD + R + r, L);
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const int before = atomicAdd(&arrived[who.x], 1);
+                s_last = before == who.y - 1;
+                if (s_last) arrived[who.x] = 0;
+                __threadfence();
+            }
+            __syncthreads();
+            write = s_last;
+        }
+        if (write) {
+            for (int i = tid; i < R; i += PA_THREADS) s_bad[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < rows * cols; i += PA_THREADS) {
+                const int r = i / cols, c = (i - r * cols) * 4, p = r0 + r, hq = pl.head * each + p % each, row = sr.first + p / each;
+                float4 v;
+                float M, L;
+                if (whole)
+                    join(KW, [&](int p) { return From{oc + (p * R + r) * CP + c, mc + p * R + r, lc + p * R + r}; }, v, M, L);
+                else
+                    join(who.y, [&](int p) {
+                        const float *b = part + Cut::slot(who.x + p, p == 0) * C::PART;
+                        return From{b + r * HD + c, b + R * HD + r, b + R * HD + R + r};
+                    }, v, M, L);
+                const float inv = L != 0.f ? 1.f / L : 0.f;
+                const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+                T *out = reinterpret_cast<T *>(a.out) + row * a.o_row + hq * a.o_head + c;
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (c + x < a.width) {
+                        out[x] = Elem<DT>::put(y[x]);
+                        if (y[x] != y[x]) s_bad[r] = 1;
+                    }
+                if (c == 0 && a.lse) a.lse[(size_t)row * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M) + log2f(L)) * 0.69314718055994530942f;
+            }
+            __syncthreads();
+            for (int r = warp; r < rows; r += PA_THREADS / 32)
+                if (s_bad[r]) pa_repair<DT>(a, sr, pl.seq, (r0 + r) / each, pl.head * each + (r0 + r) % each);
+        }
+        Cut::next(pl, a, each, sr.n, n);
+    }
+}
+
+struct PaPlan {
+    int hd, wr, blocks;
+    size_t smem, part;
+};
+template <int DT, int HD, int WR>
+static PaPlan pa_plan(int sms) {
+    using C = PaShape<DT, HD, WR>;
+    return PaPlan{HD, WR, std::min(KA_BLOCKS, sms * std::max(1, std::min(4, (int)(224 * 1024 / (C::SMEM + 2048))))), C::SMEM, C::PART};
+}
+template <int DT, int HD>
+static PaPlan pa_plan(const PackedArgs &a, int sms) {
+    // 16 rows where every sequence's fit: the steps' keys then take turns on the warps
+    return (long long)a.max_rows * (a.q_heads / a.c.heads) <= 16 ? pa_plan<DT, HD, 1>(sms) : pa_plan<DT, HD, 4>(sms);
+}
+template <int DT>
+static PaPlan pa_plan(const PackedArgs &a, int sms) {
+    return a.width <= 32 ? pa_plan<DT, 32>(a, sms) : a.width <= 64 ? pa_plan<DT, 64>(a, sms) : a.width <= 128 ? pa_plan<DT, 128>(a, sms) : pa_plan<DT, 256>(a, sms);
+}
+
+template <int DT, int HD, int WR>
+static cudaError_t pa_launch(const PackedArgs &a, const PaPlan &p, void *work, cudaStream_t s) {
+    const size_t size = sizeof(typename Elem<DT>::T);
+    // keys' and values' rows in whole 16-byte pieces: bits 0 and 1
+    auto whole = [&](const void *x, long long row, long long head) {
+        return ((uintptr_t)x | (size_t)row * size | (size_t)head * size | (size_t)a.width * size) % 16 == 0;
+    };
+    const int wide = (whole(a.k, a.k_row, a.k_head) ? 1 : 0) | (whole(a.v, a.v_row, a.v_head) ? 2 : 0);
+    const cudaError_t e = allow_dynamic_smem((const void *)k_packed_attend<DT, HD, WR>, p.smem);
+    if (e != cudaSuccess) return e;
+    int *arrived = reinterpret_cast<int *>(work);
+    k_packed_attend<DT, HD, WR><<<p.blocks, PA_THREADS, p.smem, s>>>(a, wide, reinterpret_cast<float *>(arrived + KA_BLOCKS), arrived);
+    return cudaGetLastError();
+}
+template <int DT, int HD>
+static cudaError_t pa_launch(const PackedArgs &a, const PaPlan &p, void *work, cudaStream_t s) {
+    return p.wr == 1 ? pa_launch<DT, HD, 1>(a, p, work, s) : pa_launch<DT, HD, 4>(a, p, work, s);
+}
+template <int DT>
+static cudaError_t pa_launch(const PackedArgs &a, const PaPlan &p, void *work, cudaStream_t s) {
+    return p.hd == 32 ? pa_launch<DT, 32>(a, p, work, s) : p.hd == 64 ? pa_launch<DT, 64>(a, p, work, s)
+           : p.hd == 128 ? pa_launch<DT, 128>(a, p, work, s) : pa_launch<DT, 256>(a, p, work, s);
+}
+
+static PaPlan plan_of(int dtype, const PackedArgs &a, int sms) {
+    return dtype == DT_F32 ? pa_plan<DT_F32>(a, sms) : dtype == DT_F16 ? pa_plan<DT_F16>(a, sms) : pa_plan<DT_BF16>(a, sms);
+}
+
+size_t packed_attend_workspace(int dtype, const PackedArgs &a, int sms) {
+    const PaPlan p = plan_of(dtype, a, sms);
+    return sizeof(int) * KA_BLOCKS + sizeof(float) * 2 * p.blocks * p.part;
+}
+
+cudaError_t launch_packed_attend(int dtype, const PackedArgs &a, int sms, void *encode, void *work, cudaStream_t s, uint64_t *launches) {
+    (*launches)++;
+    const PaPlan p = plan_of(dtype, a, sms);
+    return dtype == DT_F32 ? pa_launch<DT_F32>(a, p, work, s) : dtype == DT_F16 ? pa_launch<DT_F16>(a, p, work, s) : pa_launch<DT_BF16>(a, p, work, s);
+}
+
+}  // namespace tcu

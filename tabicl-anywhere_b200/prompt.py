@@ -15,8 +15,14 @@ class _Fp4(ctypes.Structure):
     _fields_ = [("codes", _void), ("scales", _void), ("rows", _i32), ("k", _i32), ("format", _i32), ("unit", _float)]
 
 
+class _Packed(ctypes.Structure):
+    _fields_ = [("seqs", _i32), ("q_rows", _i32), ("k_rows", _i32), ("max_q", _i32), ("max_k", _i32), ("q_starts", _void),
+                ("k_starts", _void)]
+
+
 def signatures():
-    m = ctypes.POINTER(_Fp4)
+    m, b = ctypes.POINTER(_Fp4), ctypes.POINTER(_Packed)
+    rows = [_void, _i64, _i64]
     return {
         "tcu_fp4_code_bytes": (_size, [_int, _int]),
         "tcu_fp4_scale_bytes": (_size, [_int, _int, _int]),
@@ -24,6 +30,9 @@ def signatures():
         "tcu_fp4_load_device": (_int, [_void, m, _int, _void, _i64, _void]),
         "tcu_fp4_linear_workspace": (_size, [_void, m, m, _int]),
         "tcu_fp4_linear_device": (_int, [_void, m, m, _int, _void, _i64, _void, _int, _void, _i64, _void, _size, _void]),
+        "tcu_packed_attend_workspace": (_size, [_void, b, _int, _int, _int, _int]),
+        "tcu_packed_attend_device": (_int, [_void, b, _int, _int, _int, _int, *rows, *rows, *rows, *rows, _float, _int, _int, _void, _void,
+                                            _size, _void]),
     }
 
 
@@ -66,4 +75,29 @@ class Fp4:
         """y = act(x W^T + bias) + residual with this matrix as W, x another Fp4; act 1 is GELU, the residual may be y itself."""
         r = _lib().tcu_fp4_linear_device(self.gpu._h, self._m, x._m, dtype, y_ptr, ldy, bias, act, residual, ldr, work, work_bytes,
                                          stream)
+        return r if r == 0 else self.gpu.check(r)
+
+
+class Packed:
+    """`seqs` sequences of different lengths, one behind the other: query rows q_starts[s]..q_starts[s + 1] of `q_rows` and keys and
+    values k_starts[s]..k_starts[s + 1] of `k_rows` (int32 on the device; k_starts_ptr None: the queries' own), at most max_q and
+    max_k each."""
+
+    def __init__(self, gpu, seqs, q_rows, k_rows, max_q, max_k, q_starts_ptr, k_starts_ptr=None):
+        self.gpu = gpu
+        self._p = _Packed(seqs, q_rows, k_rows, max_q, max_k, q_starts_ptr, k_starts_ptr)
+
+    def attend_workspace(self, dtype, q_heads, heads, width):
+        """Bytes of working memory that `attend` needs (zeroed before its first use)."""
+        n = _lib().tcu_packed_attend_workspace(self.gpu._h, self._p, dtype, q_heads, heads, width)
+        if n == _REFUSED:
+            self.gpu.check(-1)
+        return n
+
+    def attend(self, dtype, q_heads, heads, width, q_ptr, q_row, q_head, k_ptr, k_row, k_head, v_ptr, v_row, v_head, out_ptr, o_row, o_head,
+               scale, causal=False, window=0, lse=None, work=None, work_bytes=0, stream=None):
+        """Softmax attention of the query rows over their sequences' keys and values; lse (optional): f32 [q_rows][q_heads]."""
+        r = _lib().tcu_packed_attend_device(self.gpu._h, self._p, dtype, q_heads, heads, width, q_ptr, q_row, q_head, k_ptr, k_row, k_head,
+                                            v_ptr, v_row, v_head, out_ptr, o_row, o_head, scale, causal, window, lse, work, work_bytes,
+                                            stream)
         return r if r == 0 else self.gpu.check(r)

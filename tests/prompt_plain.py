@@ -64,3 +64,24 @@ def stored(code, byte):
     r, s = np.arange(rows)[:, None], np.arange(count)[None]
     place = (r // 128 * (count // 4) + s // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + s % 4
     return code[:, 0::2] | (code[:, 1::2] << 4), place
+
+
+def attend(q, k, v, q_lens, k_lens, heads, scale, causal, window):
+    """q [rows, q_heads, width], k and v [keys, heads, width] in 64 bits, sequences one behind the other: outputs and log-sum-exp.
+    A key that a row does not see has no part in it, whatever it holds."""
+    out, lse = np.zeros(q.shape), np.full(q.shape[:2], -np.inf)
+    each, q0, k0 = q.shape[1] // heads, 0, 0
+    for n, length in zip(q_lens, k_lens):
+        for i in range(n):
+            hi = max(0, min(length, length - n + i + 1)) if causal else length
+            lo = max(0, length - n + i + 1 - window) if window else 0
+            if hi <= lo:
+                continue
+            for h in range(q.shape[1]):
+                s = scale * (k[k0 + lo:k0 + hi, h // each] @ q[q0 + i, h])
+                top = s.max()
+                p = np.exp(s - top)
+                lse[q0 + i, h] = top + np.log(p.sum())
+                out[q0 + i, h] = p @ v[k0 + lo:k0 + hi, h // each] / p.sum()
+        q0, k0 = q0 + n, k0 + length
+    return out, lse

@@ -220,3 +220,74 @@ def test_linear(gpu, dtype, name, rows, n, k):
     rng = np.random.default_rng(rows * 7 + n + k)
     ux, uw = (0.37, 0.0021) if name == "nv" else (1.0, 1.0)
     check_linear(gpu, rng, dtype, FORMATS[name], rows, n, k, act=rows % 2, bias=n % 3 > 0, residual=k % 3 > 0, ux=ux, uw=uw)
+
+
+# ---- attention of packed rows ---------------------------------------------------------------------------------------
+
+def check_attend(gpu, dtype, q_lens, k_lens, q_heads, heads, width, causal, window, scale=None, spoil=None, pad=0, at=0, seed=0, lse=True,
+                 own_rows=False, extra=2):
+    """Random rows; `spoil` may change the arrays (f64, as the type holds them) before they go to the device. pad, at: strides and
+    starts that are not aligned. extra: rows behind the last sequence."""
+    code, tt = DT[dtype]
+    rng = np.random.default_rng(seed + sum(q_lens) + 7 * sum(k_lens) + width)
+    tq, tk = sum(q_lens) + extra, sum(k_lens) + extra
+    q, k, v = (rounded(rng.normal(0, 1, (n, h, width)), tt) for n, h in ((tq, q_heads), (tk, heads), (tk, heads)))
+    if spoil:
+        spoil(q, k, v)
+    scale = 1 / np.sqrt(width) if scale is None else scale
+    put = lambda x: torch.as_strided(torch.full((x.shape[0] * (x.shape[1] * (width + pad) + pad) + at + 8,), float("nan"), dtype=tt, device="cuda"),
+                                     x.shape, (x.shape[1] * (width + pad) + pad, width + pad, 1), at)  # noqa: E731
+    qd, kd, vd, od = put(q), put(k), put(v), put(q)
+    for t, x in ((qd, q), (kd, k), (vd, v)):
+        t.copy_(dev(x))
+    od.fill_(9)
+    ld = torch.full((tq, q_heads), 9.0, device="cuda")
+    starts = lambda lens: dev(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32))  # noqa: E731
+    qs, ks = starts(q_lens), starts(k_lens)
+    p = tcu.Packed(gpu, len(q_lens), tq, tk, max(q_lens), max(k_lens), qs.data_ptr(), None if own_rows else ks.data_ptr())
+    work = torch.zeros(p.attend_workspace(code, q_heads, heads, width), dtype=torch.uint8, device="cuda")
+    p.attend(code, q_heads, heads, width, qd.data_ptr(), qd.stride(0), qd.stride(1), kd.data_ptr(), kd.stride(0), kd.stride(1), vd.data_ptr(),
+             vd.stride(0), vd.stride(1), od.data_ptr(), od.stride(0), od.stride(1), float(np.float32(scale)), causal=causal, window=window,
+             lse=ld.data_ptr() if lse else None, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    assert not work[:8192].any()  # left as the next call needs them
+    n = sum(q_lens)
+    got, got_lse = host(od), host(ld)
+    assert (got[n:] == 9).all() and (got_lse[n:] == 9).all()  # rows behind the last sequence
+    with np.errstate(all="ignore"):
+        want, want_lse = plain.attend(q[:n], k, v, q_lens, k_lens, heads, float(np.float32(scale)), causal, window)
+        # what each weight may be off by, relative: its score's rounding (products of f32 held to 2^-21, each of the width's sums to 2^-23
+        # of the largest), the weight's to the type, the exponential's; an output is off by that of sum p |v|, and its own rounding
+        kmax = max([1e-30] + [np.abs(x[np.isfinite(x)]).max() for x in (k,) if np.isfinite(x).any()])
+        qmax = np.abs(np.where(np.isfinite(q[:n]), q[:n], 0)).sum(-1)
+        score = abs(scale) * qmax * kmax * (2.0**-20 if dtype == "f32" else 2.0**-22) + 2.0**-20
+        weight = score + 2.0**-20 + (0 if dtype == "f32" else ULP[dtype])
+        size, _ = plain.attend(q[:n], k, np.abs(v), q_lens, k_lens, heads, float(np.float32(scale)), causal, window)
+        size = np.where(np.isfinite(size), size, 0)
+        tol = 2 * weight[..., None] * size + 1.01 * ULP[dtype] * np.abs(np.where(np.isfinite(want), want, 0)) + 2 * TINY[dtype] + 2.0**-126
+        fine = np.isfinite(want)
+        assert np.array_equal(np.isnan(got[:n]), np.isnan(want)), "NaN where there is none, or none where there is one"
+        assert np.array_equal(got[:n][~fine & ~np.isnan(want)], want[~fine & ~np.isnan(want)])
+        assert (np.abs(got[:n] - want)[fine] <= tol[fine]).all(), np.max(np.abs(got[:n] - want)[fine] / tol[fine])
+        if lse:
+            a, b = got_lse[:n], want_lse
+            fine = np.isfinite(b)
+            assert np.array_equal(np.isnan(a), np.isnan(b)) and np.array_equal(a[~fine & ~np.isnan(b)], b[~fine & ~np.isnan(b)])
+            assert (np.abs(a - b)[fine] <= (score + 2.0**-20 + 2.0**-22 * np.abs(b))[fine]).all()
+        else:
+            assert (got_lse == 9).all()
+    return got[:n]
+
+
+LENS = [  # query rows, keys
+    ([1], [1]), ([1], [300]), ([1, 1, 1], [0, 1, 700]), ([3], [3]), ([5, 0, 17], [5, 9, 17]), ([16], [64]), ([17], [65]), ([33, 1, 64], [33, 200, 64]),
+    ([129], [129]), ([128, 256], [128, 256]), ([300, 40], [333, 40]), ([7, 4], [3, 0]), ([200], [190]), ([2, 90], [1000, 90]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_heads,heads,width", [(1, 1, 64), (4, 2, 128), (6, 2, 32), (8, 1, 96), (3, 1, 8), (2, 2, 256), (4, 4, 120)])
+@pytest.mark.parametrize("mask", ["all", "causal", "window"])
+@pytest.mark.parametrize("lens", LENS, ids=lambda x: "x".join(map(str, x[0])) + "-" + "x".join(map(str, x[1])))
+def test_attend(gpu, dtype, q_heads, heads, width, mask, lens):
+    check_attend(gpu, dtype, *lens, q_heads, heads, width, mask != "all", 11 if mask == "window" else 0)
