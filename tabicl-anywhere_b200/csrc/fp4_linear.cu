@@ -70,6 +70,21 @@ __device__ __forceinline__ void fl_bulk(uint32_t to, const void *from, uint32_t 
                  : "memory");
 }
 
+// GELU. For 16-bit results the quotient and the exponential are the unit's own (2^-21 off), and the formula for |x| >= 0.5 serves
+// all: 1.5e-7 off in erf.
+template <int DT>
+__device__ __forceinline__ float fl_gelu(float v) {
+    if constexpr (DT == DT_F32) return gelu1(v);
+    const float a = fabsf(v) * 0.70710678118654752440f;
+    float t, e;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(0.3275911f, a, 1.f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(a * a * -1.44269504088896340736f));
+    float p = fmaf(1.0614054f, t, -1.4531521f);
+    p = fmaf(p, t, 1.4214138f), p = fmaf(p, t, -0.28449674f), p = fmaf(p, t, 0.2548296f);
+    const float half = 0.5f * p * t * e;  // of 1 - erf(a)
+    return v * (v < 0.f ? half : 1.f - half);
+}
+
 // Tile t's place: groups of `group` row tiles, in them the row tiles innermost, so that blocks at work at the same time share
 // weights and rows in L2.
 __device__ __forceinline__ int2 fl_place(const FlPlan &p, int t) {
@@ -221,7 +236,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
             }
             const bool whole = s0 == 0 && s1 == p.steps;
             bool last = true;
-            if (!whole && !abort_flag) {
+            if (!whole) {
                 // parts: each block's into its slot (the tile's first block's into its second slot, the others' into their first)
                 const long long u0 = (long long)t * p.steps;
                 const int b0 = (int)ka_div((u0 + 1) * gridDim.x - 1, p.total), b1 = (int)ka_div((u0 + p.steps) * gridDim.x - 1, p.total);
@@ -257,15 +272,28 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
                 const float bias = a.bias ? Elem<DT>::get(reinterpret_cast<const T *>(a.bias)[n]) : 0.f;
                 T *y = reinterpret_cast<T *>(a.y) + (size_t)row0 * a.ldy + n;
                 const T *r = reinterpret_cast<const T *>(a.residual) + (a.residual ? (size_t)row0 * a.ldr + n : 0);
-                const int rows = min(own, a.rows - row0);
+                // 16 values at a time, the others moved up behind them: code for all 128 would not stay in the instruction caches
+                // (a call of one row took 24 us so)
+#pragma unroll 1
+                for (int rows = min(own, a.rows - row0); rows > 0; rows -= 16) {
+                    float f[16];
+                    if (a.residual) {
 #pragma unroll
-                for (int i = 0; i < 128; i++) {
-                    if (i < rows) {
-                        float f = fmaf(v[i], a.alpha, bias);
-                        if (a.act) f = gelu1(f);
-                        if (a.residual) f += Elem<DT>::get(r[(size_t)i * a.ldr]);
-                        y[(size_t)i * a.ldy] = Elem<DT>::put(f);
+                        for (int i = 0; i < 16; i++) f[i] = i < rows ? Elem<DT>::get(r[(size_t)i * a.ldr]) : 0.f;
+                        r += (size_t)16 * a.ldr;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) f[i] = 0.f;
                     }
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        float g = fmaf(v[i], a.alpha, bias);
+                        if (a.act) g = fl_gelu<DT>(g);
+                        if (i < rows) y[(size_t)i * a.ldy] = Elem<DT>::put(g + f[i]);
+                    }
+                    y += (size_t)16 * a.ldy;
+#pragma unroll
+                    for (int i = 0; i < 112; i++) v[i] = v[i + 16];
                 }
             }
             pos += s1 - s0;

@@ -53,7 +53,9 @@ __device__ __forceinline__ long long ka_div(long long a, long long b) {  // not 
     return ((a | b) >> 32) ? a / b : (long long)((uint32_t)a / (uint32_t)b);
 }
 
-template <int R, int ALIGN, int STEP>
+// EXTRA: a unit counts as so many steps more than it has, its first ones, which are none: what it costs besides its steps (its
+// queries, its output), so that blocks with many short units have as much to do as those with few long ones.
+template <int R, int ALIGN, int STEP, int EXTRA = 0>
 struct KaCut {
     struct Span {
         int lo_min, lo_max, hi_min, hi_max, base, steps;  // what the tile's first and last rows see; where its steps begin
@@ -64,7 +66,7 @@ struct KaCut {
         Span p;
         p.lo_min = ka_lo(a, s, first), p.lo_max = ka_lo(a, s, last), p.hi_min = ka_hi(a, s, first), p.hi_max = ka_hi(a, s, last);
         p.base = p.lo_min & ~(ALIGN - 1);
-        p.steps = p.hi_max > p.lo_min ? (p.hi_max - p.base + STEP - 1) / STEP : 1;  // no keys: a step that writes zeros
+        p.steps = (p.hi_max > p.lo_min ? (p.hi_max - p.base + STEP - 1) / STEP : 1) + EXTRA;  // no keys: a step that writes zeros
         return p;
     }
     template <class A>

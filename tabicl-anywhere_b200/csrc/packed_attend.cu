@@ -406,13 +406,23 @@ static PaPlan plan_of(int dtype, const PackedArgs &a, int sms) {
     return dtype == DT_F32 ? pa_plan<DT_F32>(a, sms) : dtype == DT_F16 ? pa_plan<DT_F16>(a, sms) : pa_plan<DT_BF16>(a, sms);
 }
 
+// Many rows of a 16-bit type: the tensor-core kernel's, where TMA can fetch the keys and values.
+static bool pa_many(int dtype, const PackedArgs &a) {
+    return dtype != DT_F32 && a.width <= 128 && a.q_heads / a.c.heads <= 4096 && (long long)a.max_rows * (a.q_heads / a.c.heads) > 64;
+}
+
 size_t packed_attend_workspace(int dtype, const PackedArgs &a, int sms) {
     const PaPlan p = plan_of(dtype, a, sms);
-    return sizeof(int) * KA_BLOCKS + sizeof(float) * 2 * p.blocks * p.part;
+    const size_t own = sizeof(int) * KA_BLOCKS + sizeof(float) * 2 * p.blocks * p.part;
+    return pa_many(dtype, a) ? std::max(own, packed_attend_tc_workspace(a, sms)) : own;
 }
 
 cudaError_t launch_packed_attend(int dtype, const PackedArgs &a, int sms, void *encode, void *work, cudaStream_t s, uint64_t *launches) {
     (*launches)++;
+    if (pa_many(dtype, a)) {
+        const cudaError_t e = launch_packed_attend_tc(dtype, a, sms, encode, work, s);
+        if (e != cudaErrorNotSupported) return e;
+    }
     const PaPlan p = plan_of(dtype, a, sms);
     return dtype == DT_F32 ? pa_launch<DT_F32>(a, p, work, s) : dtype == DT_F16 ? pa_launch<DT_F16>(a, p, work, s) : pa_launch<DT_BF16>(a, p, work, s);
 }
