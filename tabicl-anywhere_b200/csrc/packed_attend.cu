@@ -17,8 +17,9 @@ constexpr int PA_THREADS = 128;
 // Steps a block takes at least: shorter parts of a unit are more to join.
 constexpr int PA_STEPS = 4;
 
-template <int DT, int HD, int WR>
+template <int DT, int HD_, int WR>
 struct PaShape {
+    static constexpr int HD = HD_;
     using T = typename Elem<DT>::T;
     static constexpr bool F32 = DT == DT_F32;
     using Raw = std::conditional_t<F32, uint32_t, uint16_t>;
@@ -82,13 +83,18 @@ __device__ __forceinline__ void pa_copy(uint8_t *to, const void *base, long long
     constexpr int PER = 16 / (int)sizeof(Raw);
     const Raw *from = reinterpret_cast<const Raw *>(base);
     if (wide) {
-        const int pieces = width / PER;
-        for (int i = threadIdx.x; i < C::BK * pieces; i += PA_THREADS) {
-            const int r = i / pieces, c = i - r * pieces;
-            const bool in = r >= lo && r < hi;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(pa_smem(to + r * C::PITCH + c * 16)),
-                         "l"(in ? from + first + r * row + c * PER : from), "r"(in ? 16 : 0)
-                         : "memory");
+        // a thread the same 16 bytes of every ROWS-th row
+        constexpr int LANES = C::HD / PER, ROWS = PA_THREADS / LANES;
+        const int c = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
+        if (c * PER < width) {
+            const Raw *at = from + first + r0 * row + c * PER;
+            const uint32_t dst = pa_smem(to + r0 * C::PITCH + c * 16);
+#pragma unroll
+            for (int x = 0; x < C::BK / ROWS; x++, at += ROWS * row) {
+                const int r = r0 + x * ROWS;
+                const bool in = r >= lo && r < hi;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + x * ROWS * C::PITCH), "l"(in ? at : from), "r"(in ? 16 : 0) : "memory");
+            }
         }
     } else {
         for (int i = threadIdx.x; i < C::BK * width; i += PA_THREADS) {
