@@ -33,6 +33,9 @@ cudaError_t launch_packed_attend(int dtype, const PackedArgs &a, int sms, void *
 // The same on the tensor cores, for many rows of a 16-bit type. Not taken: cudaErrorNotSupported, nothing launched.
 size_t packed_attend_tc_workspace(const PackedArgs &a, int sms);
 cudaError_t launch_packed_attend_tc(int dtype, const PackedArgs &a, int sms, void *encode, void *work, cudaStream_t s);
+// For many rows of f32.
+size_t packed_attend_tc32_workspace(const PackedArgs &a, int sms);
+cudaError_t launch_packed_attend_tc32(const PackedArgs &a, int sms, void *work, cudaStream_t s, uint64_t *launches);
 
 #ifdef __CUDACC__
 

@@ -417,13 +417,20 @@ static bool pa_many(int dtype, const PackedArgs &a) {
     return dtype != DT_F32 && a.width <= 128 && a.q_heads / a.c.heads <= 4096 && (long long)a.max_rows * (a.q_heads / a.c.heads) > 64;
 }
 
+// Many rows of f32: the tensor-core kernel's, whose split keys and values take as much memory again as they do, up to 1 GB.
+static bool pa_many32(int dtype, const PackedArgs &a, int sms) {
+    return dtype == DT_F32 && a.width <= 128 && (long long)a.max_rows * (a.q_heads / a.c.heads) > 64 && packed_attend_tc32_workspace(a, sms) <= 1u << 30;
+}
+
 size_t packed_attend_workspace(int dtype, const PackedArgs &a, int sms) {
+    if (pa_many32(dtype, a, sms)) return packed_attend_tc32_workspace(a, sms);
     const PaPlan p = plan_of(dtype, a, sms);
     const size_t own = sizeof(int) * KA_BLOCKS + sizeof(float) * 2 * p.blocks * p.part;
     return pa_many(dtype, a) ? std::max(own, packed_attend_tc_workspace(a, sms)) : own;
 }
 
 cudaError_t launch_packed_attend(int dtype, const PackedArgs &a, int sms, void *encode, void *work, cudaStream_t s, uint64_t *launches) {
+    if (pa_many32(dtype, a, sms)) return launch_packed_attend_tc32(a, sms, work, s, launches);
     (*launches)++;
     if (pa_many(dtype, a)) {
         const cudaError_t e = launch_packed_attend_tc(dtype, a, sms, encode, work, s);
