@@ -19,11 +19,10 @@ namespace tcu {
 constexpr int FL_THREADS = 384, FL_M = 128, FL_STEP = 256, FL_STAGES = 8;
 constexpr int FL_A = FL_M * FL_STEP / 2;  // bytes of a step's weights
 constexpr size_t FL_SMEM = 225 * 1024;
-// Steps a block takes at least where a product has fewer tiles than SMs.
-constexpr int FL_MIN_STEPS = 2;
+constexpr int FL_MIN_STEPS = 2;  // of a tile that is cut
 
 struct FlPlan {
-    int nt, row_tiles, feat_tiles, steps, stages, nacc, chunk, blocks, quads, group;
+    int nt, row_tiles, feat_tiles, steps, stages, nacc, chunk, blocks, quads, group, split;
     unsigned stage_bytes, sf_a, sf_b, slot, acc_cols;
     long long total;
 };
@@ -104,7 +103,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
     __shared__ __align__(8) uint64_t m_full[FL_STAGES], m_empty[FL_STAGES], m_acc[2], m_free[2], m_done;
     __shared__ uint32_t tslot;
     __shared__ volatile int abort_flag;
-    __shared__ int s_last;
+    __shared__ volatile int s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = (smem_addr(smraw) + 1023u) & ~1023u;
     if (warp == 2) {
@@ -128,8 +127,10 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
         if (!ok) abort_flag = 1;
         return ok;
     };
-    long long pos = ka_div(p.total * blockIdx.x, gridDim.x);
-    const long long end = ka_div(p.total * (blockIdx.x + 1), gridDim.x);
+    // the block's steps: an even share of all, or of whole tiles
+    const long long per = p.split ? 1 : p.steps, all = p.total / per;
+    long long pos = ka_div(all * blockIdx.x, gridDim.x) * per;
+    const long long end = ka_div(all * (blockIdx.x + 1), gridDim.x) * per;
 
     if (warp == 0) {
         int at = 0;
@@ -235,65 +236,75 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
                 mbar_arrive(&m_free[acc]);
             }
             const bool whole = s0 == 0 && s1 == p.steps;
-            bool last = true;
-            if (!whole) {
+            const int n = place.y * FL_M + quad * 32 + lane, row0 = place.x * p.nt + c0;
+            const float bias = a.bias && n < a.n ? Elem<DT>::get(reinterpret_cast<const T *>(a.bias)[n]) : 0.f;
+            T *y = reinterpret_cast<T *>(a.y) + (size_t)row0 * a.ldy + n;
+            const T *r = reinterpret_cast<const T *>(a.residual) + (a.residual ? (size_t)row0 * a.ldr + n : 0);
+            // 16 rows' outputs from their sums, of which `rows` there are
+            auto put = [&](const float *sum, int rows) {
+                float f[16];
+                if (a.residual) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) f[i] = i < rows ? Elem<DT>::get(r[(size_t)i * a.ldr]) : 0.f;
+                    r += (size_t)16 * a.ldr;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) f[i] = 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float g = fmaf(sum[i], a.alpha, bias);
+                    if (a.act) g = fl_gelu<DT>(g);
+                    if (i < rows) y[(size_t)i * a.ldy] = Elem<DT>::put(g + f[i]);
+                }
+                y += (size_t)16 * a.ldy;
+            };
+            const int rows = n < a.n && !abort_flag ? min(own, a.rows - row0) : 0;
+            if (whole) {
+                // 16 values at a time, the others moved up behind them: code for all 128 would not stay in the instruction caches (a
+                // call of one row took 24 us so)
+#pragma unroll 1
+                for (int there = rows; there > 0; there -= 16) {
+                    put(v, there);
+#pragma unroll
+                    for (int i = 0; i < 112; i++) v[i] = v[i + 16];
+                }
+            } else {
                 // parts: each block's into its slot (the tile's first block's into its second slot, the others' into their first)
                 const long long u0 = (long long)t * p.steps;
                 const int b0 = (int)ka_div((u0 + 1) * gridDim.x - 1, p.total), b1 = (int)ka_div((u0 + p.steps) * gridDim.x - 1, p.total);
                 const size_t size = (size_t)FL_M * p.nt;
-                const int at = c0 * FL_M + quad * 32 + lane;
-                float *to = part + (2 * (size_t)blockIdx.x + (s0 == 0)) * size + at;
+                float *at = part + c0 * FL_M + quad * 32 + lane, *to = at + (2 * (size_t)blockIdx.x + (s0 == 0)) * size;
 #pragma unroll
-                for (int i = 0; i < 128; i++)
-                    if (i < own) __stcg(to + i * FL_M, v[i]);
-                __threadfence();
+                for (int g = 0; g < 8; g++)
+                    if (g * 16 < own) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) __stcg(to + (g * 16 + i) * FL_M, v[g * 16 + i]);
+                    }
                 kt_bar(1, 256);
                 if (tid == 128) {
-                    const int n = atomicAdd(&arrived[b0], 1);
-                    s_last = n == b1 - b0;
+                    __threadfence();  // (after the barrier: for all that the block has stored)
+                    const int before = atomicAdd(&arrived[b0], 1);
+                    s_last = before == b1 - b0;
                     if (s_last) arrived[b0] = 0;
                     __threadfence();
                 }
                 kt_bar(1, 256);
-                last = s_last != 0;
-                if (last) {
-#pragma unroll
-                    for (int i = 0; i < 128; i++) v[i] = 0.f;
-                    for (int b = b0; b <= b1; b++) {
-                        const float *in = part + (2 * (size_t)b + (b == b0)) * size + at;
-#pragma unroll
-                        for (int i = 0; i < 128; i++)
-                            if (i < own) v[i] += __ldcg(in + i * FL_M);
-                    }
-                }
-            }
-            const int n = place.y * FL_M + quad * 32 + lane, row0 = place.x * p.nt + c0;
-            if (last && n < a.n && !abort_flag) {
-                const float bias = a.bias ? Elem<DT>::get(reinterpret_cast<const T *>(a.bias)[n]) : 0.f;
-                T *y = reinterpret_cast<T *>(a.y) + (size_t)row0 * a.ldy + n;
-                const T *r = reinterpret_cast<const T *>(a.residual) + (a.residual ? (size_t)row0 * a.ldr + n : 0);
-                // 16 values at a time, the others moved up behind them: code for all 128 would not stay in the instruction caches
-                // (a call of one row took 24 us so)
+                if (s_last) {
 #pragma unroll 1
-                for (int rows = min(own, a.rows - row0); rows > 0; rows -= 16) {
-                    float f[16];
-                    if (a.residual) {
+                    for (int g = 0; g < own && g < rows; g += 16) {
+                        float sum[16] = {};
+#pragma unroll 1
+                        for (int b = b0; b <= b1; b++) {
+                            const float *in = at + (2 * (size_t)b + (b == b0)) * size + g * FL_M;
+                            float x[16];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) f[i] = i < rows ? Elem<DT>::get(r[(size_t)i * a.ldr]) : 0.f;
-                        r += (size_t)16 * a.ldr;
-                    } else {
+                            for (int i = 0; i < 16; i++) x[i] = __ldcg(in + i * FL_M);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) f[i] = 0.f;
+                            for (int i = 0; i < 16; i++) sum[i] += x[i];
+                        }
+                        put(sum, rows - g);
                     }
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        float g = fmaf(v[i], a.alpha, bias);
-                        if (a.act) g = fl_gelu<DT>(g);
-                        if (i < rows) y[(size_t)i * a.ldy] = Elem<DT>::put(g + f[i]);
-                    }
-                    y += (size_t)16 * a.ldy;
-#pragma unroll
-                    for (int i = 0; i < 112; i++) v[i] = v[i + 16];
                 }
             }
             pos += s1 - s0;
@@ -311,16 +322,32 @@ static FlPlan fl_plan(int dtype, const Fp4LinearArgs &a, int sms) {
     const bool nv = a.format == FP4_NV;
     const int kp = fp4_padded(a.k), qs = nv ? 4 : 2;
     p.quads = fp4_quads(a.k, a.format), p.steps = (kp + FL_STEP - 1) / FL_STEP;
+    p.feat_tiles = (a.n + FL_M - 1) / FL_M;
+    // How many rows a tile has, and whether tiles are cut: what takes the fewest cycles as measured. A step's copies come at some 60
+    // bytes a cycle and SM; an output costs its block some 12 cycles a row of the tile, a cut tile's parts three times that.
+    const int widest = std::min(dtype == DT_F32 ? 128 : 256, (a.rows + 15) / 16 * 16);
+    double best = 0;
+    p.nt = 0;
+    for (int nt : {16, 32, 48, 64, 96, 128, 256, widest}) {
+        if (nt > widest || (nt > 128 && nt != 256 && nt != widest) || (a.rows > nt && nt % 128)) continue;
+        if (nt > 128) nt = 256;
+        const long long tiles = (long long)((a.rows + nt - 1) / nt) * p.feat_tiles;
+        const double step = 330 + 2.2 * nt, out = 1000 + 12.0 * nt, each = (double)tiles / sms;
+        for (int split = 0; split < 2; split++) {
+            const long long blocks = std::min<long long>(sms, split ? (tiles * p.steps + FL_MIN_STEPS - 1) / FL_MIN_STEPS : tiles);
+            const double turns = split ? (double)tiles / blocks : std::ceil((double)tiles / blocks);
+            const double cost = turns * p.steps * step + std::ceil(each) * out + (split ? 6000 + 36.0 * nt : 0);
+            if (!p.nt || cost < best) best = cost, p.nt = nt, p.split = split, p.blocks = (int)blocks;
+        }
+    }
     // f32 results: the matrix unit does not round its sums to nearest, so a sum runs over 4 steps in it, from there on in
     // registers; two narrower accumulators in turn, so that the unit does not wait for them to be read
-    const int most = dtype == DT_F32 ? 128 : 256;
-    p.nt = a.rows > most ? most : a.rows > 128 ? 256 : a.rows > 64 ? 128 : (a.rows + 15) / 16 * 16;
     p.chunk = dtype == DT_F32 ? 4 : p.steps;
     p.nacc = p.nt > 128 ? 1 : 2;
     int cols = 32;
     while (cols < p.nt) cols *= 2;
     p.acc_cols = (unsigned)(cols * p.nacc);
-    p.row_tiles = (a.rows + p.nt - 1) / p.nt, p.feat_tiles = (a.n + FL_M - 1) / FL_M;
+    p.row_tiles = (a.rows + p.nt - 1) / p.nt;
     p.sf_a = (unsigned)(FL_A + p.nt * 128), p.sf_b = p.sf_a + qs * 512;
     p.stage_bytes = (p.sf_b + qs * 512 * (p.nt > 128 ? 2 : 1) + 1023) / 1024 * 1024;
     p.slot = (unsigned)(qs * (4 + (p.nt > 128 ? 8 : 4)));
@@ -328,7 +355,6 @@ static FlPlan fl_plan(int dtype, const Fp4LinearArgs &a, int sms) {
     p.stages = std::min<int>(p.stages, (int)((512 - p.acc_cols) / p.slot));
     p.group = 8;
     p.total = (long long)p.row_tiles * p.feat_tiles * p.steps;
-    p.blocks = (int)std::min<long long>(sms, (p.total + FL_MIN_STEPS - 1) / FL_MIN_STEPS);
     return p;
 }
 
