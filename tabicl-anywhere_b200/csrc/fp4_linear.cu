@@ -8,7 +8,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <cstring>
+#include <type_traits>
 
 #include "device.cuh"
 #include "fp4.cuh"
@@ -52,8 +52,8 @@ __device__ __forceinline__ void fl_mma(uint32_t d, uint64_t a, uint64_t b, uint3
             : "memory");
 }
 // 512 bytes of scales (32 rows of 16) to 4 columns of tensor memory, once for each warp's lanes.
-__device__ __forceinline__ void fl_scales(uint32_t to, uint32_t from) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(smem_desc(from, 16, 128)) : "memory");
+__device__ __forceinline__ void fl_scales(uint32_t to, uint64_t from) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void fl_expect(uint64_t *m, uint32_t bytes) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}\n" ::"r"(smem_addr(m)), "r"(bytes) : "memory");
@@ -122,10 +122,8 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
     fence_after_sync();
     const uint32_t tmem = tslot, sf0 = tmem + p.acc_cols;
     auto wait_warp = [&](uint64_t *m, uint32_t parity) {
-        bool ok = mbar_test_wait(m, parity) || (!abort_flag && mbar_wait(m, parity, KT_WAIT));
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) abort_flag = 1;
-        return ok;
+        if (!mbar_test_wait(m, parity) && !abort_flag && !mbar_wait(m, parity, KT_WAIT)) abort_flag = 1;
+        __syncwarp();
     };
     // the block's steps: an even share of all, or of whole tiles
     const long long per = p.split ? 1 : p.steps, all = p.total / per;
@@ -133,20 +131,16 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
     const long long end = ka_div(all * (blockIdx.x + 1), gridDim.x) * per;
 
     if (warp == 0) {
-        int at = 0;
-        bool on = true;
-        while (pos < end && on) {
+        int at = 0, slot = 0;
+        uint32_t turn = 0;  // how often the slots have been filled (its lowest bit: a division by a number of slots known at run time costs more)
+        while (pos < end) {
             const int t = (int)ka_div(pos, p.steps), s0 = (int)(pos - (long long)t * p.steps), s1 = (int)min((long long)p.steps, s0 + end - pos);
             const int2 place = fl_place(p, t);
             const uint8_t *wa = a.w_scales + (size_t)place.y * p.quads * 512;
             const int row_block = place.x * p.nt / 128, blocks = min((p.nt + 127) / 128, (a.rows + 127) / 128 - row_block);
             const uint8_t *xa = a.x_scales + (size_t)row_block * p.quads * 512;
             for (int s = s0; s < s1; s++, at++) {
-                const int slot = at % p.stages;
-                if (at >= p.stages && !wait_warp(&m_empty[slot], (uint32_t)(at / p.stages - 1) & 1u)) {
-                    on = false;
-                    break;
-                }
+                if (turn) wait_warp(&m_empty[slot], (turn - 1) & 1u);
                 const int quads = min(QS, p.quads - s * QS);
                 if (elect_one()) {
                     const uint32_t to = base + slot * p.stage_bytes;
@@ -158,47 +152,67 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
                         fl_bulk(to + p.sf_b + b * QS * 512, xa + ((size_t)b * p.quads + s * QS) * 512, quads * 512, &m_full[slot]);
                 }
                 __syncwarp();
+                if (++slot == p.stages) slot = 0, turn++;
             }
             pos += s1 - s0;
         }
         // what was asked for lands before the block lets go of shared memory
         for (int i = max(0, at - p.stages); i < at; i++) mbar_wait(&m_full[i % p.stages], (uint32_t)(i / p.stages) & 1u, KT_WAIT);
     } else if (warp == 1) {
-        int at = 0, c = 0;
+        int c = 0, slot = 0;
+        uint32_t turn = 0;
         const bool two = p.nt > 128;
+        const uint64_t da0 = fl_desc(base), db0 = fl_desc(base + FL_A), sfa0 = smem_desc(base + p.sf_a, 16, 128), sfb0 = smem_desc(base + p.sf_b, 16, 128);
+        const uint32_t id0 = fl_idesc(p.nt, NV, 0), id2 = fl_idesc(p.nt, NV, 2);
+        // a step's scales to tensor memory, then its products; Q blocks of 4 scales, a number known when compiled for all but a row's
+        // last step (descriptors worked out in a loop cost the issuing thread about a hundred cycles each)
+        auto issue = [&](auto blocks, int quads, uint32_t d, uint32_t off, uint32_t sa, bool first) {
+            constexpr int Q = decltype(blocks)::value;
+            const uint64_t da = da0 + off, db = db0 + off, fa = sfa0 + off, fb = sfb0 + off;
+            const uint32_t sb = sa + QS * 4;
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                if (q >= quads) break;
+                fl_scales(sa + q * 4, fa + q * 32);
+                if (two)
+                    fl_scales(sb + q * 8, fb + q * 32), fl_scales(sb + q * 8 + 4, fb + (QS + q) * 32);
+                else
+                    fl_scales(sb + q * 4, fb + q * 32);
+            }
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+                if (q >= quads) break;
+                const uint32_t qa = sa + q * 4, qb = sb + q * (two ? 8 : 4);
+                if constexpr (NV) {
+                    fl_mma<NV>(d, da + q * 2, db + q * 2, id0, qa, qb, !first || q > 0);
+                } else {
+                    fl_mma<NV>(d, da + q * 4, db + q * 4, id0, qa, qb, !first || q > 0);
+                    fl_mma<NV>(d, da + q * 4 + 2, db + q * 4 + 2, id2, qa, qb, 1);
+                }
+            }
+        };
         while (pos < end) {
             const int t = (int)ka_div(pos, p.steps), s0 = (int)(pos - (long long)t * p.steps), s1 = (int)min((long long)p.steps, s0 + end - pos);
             for (int from = s0; from < s1; from += p.chunk, c++) {
-                const int to = min(s1, from + p.chunk), acc = c % p.nacc;
-                if (c >= p.nacc) wait_warp(&m_free[acc], (uint32_t)(c / p.nacc - 1) & 1u);
+                const int to = min(s1, from + p.chunk), acc = c & (p.nacc - 1), turns = c >> (p.nacc - 1);
+                if (turns) wait_warp(&m_free[acc], (uint32_t)(turns - 1) & 1u);
                 fence_after_sync();
                 const uint32_t d = tmem + acc * (p.acc_cols / p.nacc);
-                for (int s = from; s < to; s++, at++) {
-                    const int slot = at % p.stages;
-                    wait_warp(&m_full[slot], (uint32_t)(at / p.stages) & 1u);
+                for (int s = from; s < to; s++) {
+                    wait_warp(&m_full[slot], turn & 1u);
                     fence_after_sync();
                     const int quads = min(QS, p.quads - s * QS);
+                    const uint32_t off = (slot * p.stage_bytes) >> 4, sa = sf0 + slot * p.slot;
                     if (elect_one()) {
-                        const uint32_t in = base + slot * p.stage_bytes, sa = sf0 + slot * p.slot, sb = sa + QS * 4;
-                        for (int q = 0; q < quads; q++) {
-                            fl_scales(sa + q * 4, in + p.sf_a + q * 512);
-                            fl_scales(sb + q * (two ? 8 : 4), in + p.sf_b + q * 512);
-                            if (two) fl_scales(sb + q * 8 + 4, in + p.sf_b + (QS + q) * 512);
-                        }
-                        const uint64_t da = fl_desc(in), db = fl_desc(in + FL_A);
-                        for (int q = 0; q < quads; q++) {
-                            const uint32_t qa = sa + q * 4, qb = sb + q * (two ? 8 : 4);
-                            if constexpr (NV) {
-                                fl_mma<NV>(d, da + q * 2, db + q * 2, fl_idesc(p.nt, true, 0), qa, qb, s > from || q > 0);
-                            } else {
-                                fl_mma<NV>(d, da + q * 4, db + q * 4, fl_idesc(p.nt, false, 0), qa, qb, s > from || q > 0);
-                                fl_mma<NV>(d, da + q * 4 + 2, db + q * 4 + 2, fl_idesc(p.nt, false, 2), qa, qb, 1);
-                            }
-                        }
+                        if (quads == QS)
+                            issue(std::integral_constant<int, QS>{}, QS, d, off, sa, s == from);
+                        else
+                            issue(std::integral_constant<int, QS - 1>{}, quads, d, off, sa, s == from);
                         mma_commit(&m_empty[slot]);
                         if (s == to - 1) mma_commit(&m_acc[acc]);
                     }
                     __syncwarp();
+                    if (++slot == p.stages) slot = 0, turn++;
                 }
             }
             pos += s1 - s0;
@@ -218,8 +232,8 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
 #pragma unroll
             for (int i = 0; i < 128; i++) v[i] = 0.f;
             for (int from = s0; from < s1; from += p.chunk, c++) {
-                const int acc = c % p.nacc;
-                wait_warp(&m_acc[acc], (uint32_t)(c / p.nacc) & 1u);
+                const int acc = c & (p.nacc - 1);
+                wait_warp(&m_acc[acc], (uint32_t)(c >> (p.nacc - 1)) & 1u);
                 fence_after_sync();
                 const uint32_t d = tmem + acc * (p.acc_cols / p.nacc) + c0 + ((uint32_t)(quad * 32) << 16);
 #pragma unroll
