@@ -177,7 +177,8 @@ __global__ void __launch_bounds__(FP_THREADS, 8) k_fp4_pack(Fp4Args a, unsigned 
     const bool on = id < total;
     const unsigned row = on ? fp_div(id, div) : 0, part = on ? id - row * per : 0;
     __shared__ float stage[FP_THREADS / 32][32 * FP_PITCH];
-    const bool beside = !wide && __all_sync(0xffffffffu, on && row == __shfl_sync(0xffffffffu, row, 0));
+    const unsigned row0 = __shfl_sync(0xffffffffu, row, 0);  // (by every lane, those past the end too)
+    const bool beside = __all_sync(0xffffffffu, !wide && on && row == row0);
     const T *from = reinterpret_cast<const T *>(a.x) + (size_t)row * a.ldx + part * 16;
     float v[16];
     float top = load16<DT>(from, on ? a.k - (int)part * 16 : 0, wide, beside, stage[threadIdx.x >> 5], v);
@@ -240,7 +241,8 @@ __global__ void __launch_bounds__(FP_THREADS) k_fp4_load(Fp4Args a, unsigned per
     const bool on = id < total;
     const unsigned row = on ? fp_div(id, div) : 0, part = on ? id - row * per : 0, s = NV ? part : part / 2;
     const int there = a.k - (int)part * 16;
-    const bool beside = !wide && __all_sync(0xffffffffu, on && row == __shfl_sync(0xffffffffu, row, 0));
+    const unsigned row0 = __shfl_sync(0xffffffffu, row, 0);  // (by every lane, those past the end too)
+    const bool beside = __all_sync(0xffffffffu, !wide && on && row == row0);
     if (!beside && (!on || there <= 0)) return;
     const uint2 codes = __ldg(reinterpret_cast<const uint2 *>(a.codes) + id);
     const uint32_t byte = a.scales[((size_t)(row / 128) * quads + s / 4) * 512 + row % 32 * 16 + row % 128 / 32 * 4 + s % 4];

@@ -19,7 +19,6 @@ namespace tcu {
 constexpr int FL_THREADS = 384, FL_M = 128, FL_STEP = 256, FL_STAGES = 8;
 constexpr int FL_A = FL_M * FL_STEP / 2;  // bytes of a step's weights
 constexpr size_t FL_SMEM = 225 * 1024;
-constexpr int FL_MIN_STEPS = 2;  // of a tile that is cut
 
 struct FlPlan {
     int nt, row_tiles, feat_tiles, steps, stages, nacc, chunk, blocks, quads, group, split;
@@ -106,6 +105,10 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
     __shared__ volatile int s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = (smem_addr(smraw) + 1023u) & ~1023u;
+    if (tid == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+    }
     if (warp == 2) {
         tmem_alloc(&tslot, 512);
         tmem_relinquish();
@@ -337,21 +340,24 @@ static FlPlan fl_plan(int dtype, const Fp4LinearArgs &a, int sms) {
     const int kp = fp4_padded(a.k), qs = nv ? 4 : 2;
     p.quads = fp4_quads(a.k, a.format), p.steps = (kp + FL_STEP - 1) / FL_STEP;
     p.feat_tiles = (a.n + FL_M - 1) / FL_M;
-    // How many rows a tile has, and whether tiles are cut: what takes the fewest cycles as measured. A step's copies come at some 60
-    // bytes a cycle and SM; an output costs its block some 12 cycles a row of the tile, a cut tile's parts three times that.
+    // How many rows a tile has, and over how many blocks it is cut: what takes the fewest cycles, from what was measured (8 to 4096
+    // rows): a step 420 and 3 a row of the tile, a tile's output 1000 and 12 a row; the parts of a cut tile 7000 and 100 a row for
+    // storing and waiting, and each part 600 and 25 a row in the block that joins them (2048 x 1024 x 4096: whole tiles of 128 rows
+    // 15.6 us, cut over all SMs 27.2; of 256 rows 20.9 and 39.3. 4096 x 14336 x 8192: of 256 rows 255 us, of 128 330).
     const int widest = std::min(dtype == DT_F32 ? 128 : 256, (a.rows + 15) / 16 * 16);
     double best = 0;
     p.nt = 0;
     for (int nt : {16, 32, 48, 64, 96, 128, 256, widest}) {
-        if (nt > widest || (nt > 128 && nt != 256 && nt != widest) || (a.rows > nt && nt % 128)) continue;
         if (nt > 128) nt = 256;
+        if (nt > 128 ? widest <= 128 : nt > widest || (a.rows > nt && nt % 128)) continue;  // (a tile begins with a block of scales)
         const long long tiles = (long long)((a.rows + nt - 1) / nt) * p.feat_tiles;
-        const double step = 330 + 2.2 * nt, out = 1000 + 12.0 * nt, each = (double)tiles / sms;
-        for (int split = 0; split < 2; split++) {
-            const long long blocks = std::min<long long>(sms, split ? (tiles * p.steps + FL_MIN_STEPS - 1) / FL_MIN_STEPS : tiles);
-            const double turns = split ? (double)tiles / blocks : std::ceil((double)tiles / blocks);
-            const double cost = turns * p.steps * step + std::ceil(each) * out + (split ? 6000 + 36.0 * nt : 0);
-            if (!p.nt || cost < best) best = cost, p.nt = nt, p.split = split, p.blocks = (int)blocks;
+        const double step = 420 + 3.0 * nt, out = 1000 + 12.0 * nt;
+        for (int parts = 1; parts <= 32 && parts <= p.steps; parts *= 2) {
+            if (parts > 1 && tiles * parts > 2 * sms) break;
+            const long long blocks = std::min<long long>(sms, tiles * parts);
+            const double turns = parts > 1 ? (double)tiles / blocks : std::ceil((double)tiles / blocks);
+            const double cost = turns * p.steps * step + std::ceil(turns) * out + (parts > 1 ? 7000 + 100.0 * nt + parts * (600 + 25.0 * nt) : 0);
+            if (!p.nt || cost < best) best = cost, p.nt = nt, p.split = parts > 1, p.blocks = (int)blocks;
         }
     }
     // f32 results: the matrix unit does not round its sums to nearest, so a sum runs over 4 steps in it, from there on in

@@ -132,6 +132,31 @@ def test_pack_and_load(gpu, dtype, name, k, unit):
         assert (out[rest] == 9).all()                            # nothing beside the rows
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("name", ["mx", "nv"])
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 130), (3, 130), (5, 2050), (2, 513), (7, 600), (131, 50)])
+@pytest.mark.parametrize("pad", [0, 1, 6])
+def test_pack_few_rows(gpu, dtype, name, rows, k, pad):
+    """Sizes whose last threads have nothing to do, and a warp's may have rows of their own; aligned and not."""
+    code, tt = DT[dtype]
+    fmt = FORMATS[name]
+    x = rounded(np.random.default_rng(rows + k).normal(0, 1, (rows, k)), tt)
+    unit = float(np.float32(np.abs(x).max() / 2688)) if fmt == plain.NV else 1.0
+    xd = torch.as_strided(torch.zeros(rows * (k + pad) + 8, dtype=tt, device="cuda"), (rows, k), (k + pad, 1), pad % 4)
+    xd.copy_(dev(x))
+    m = Matrix(gpu, rows, k, fmt, unit, fill=0xA5)
+    m.m.pack(code, xd.data_ptr(), k + pad, stream=1)
+    y = torch.full((rows, k + pad), 9.0, dtype=tt, device="cuda")
+    m.m.load(code, y.data_ptr(), k + pad, stream=1)
+    sync(gpu)
+    want_codes, byte = plain.quantise(x, fmt, unit)
+    packed, place = plain.stored(want_codes, byte)
+    assert np.array_equal(m.codes.cpu().numpy().reshape(rows, -1), packed)
+    assert np.array_equal(m.scales.cpu().numpy()[place], byte)
+    want = rounded(rounded(plain.values(want_codes, byte, fmt, 1.0, k) * unit, torch.float32), tt)
+    assert np.array_equal(host(y[:, :k]), want) and (y[:, k:] == 9).all()
+
+
 def test_pack_writes_no_row_behind_the_last(gpu):
     """Scales of rows that the matrix does not have are left as they were."""
     m = Matrix(gpu, 130, 64, plain.NV, fill=0xA5)
@@ -148,6 +173,7 @@ def test_pack_writes_no_row_behind_the_last(gpu):
 LINEAR = [  # rows, n, k
     (1, 1, 1), (1, 128, 128), (1, 1024, 512), (3, 200, 130), (8, 4097, 700), (16, 256, 256), (17, 130, 2050), (33, 100, 512),
     (64, 1000, 1000), (65, 129, 384), (127, 300, 100), (128, 512, 1024), (129, 513, 640), (256, 128, 64), (257, 1000, 2000), (600, 700, 900),
+    (8, 300, 33000), (33, 64, 20000), (150, 130, 16400),  # few tiles of many steps: cut
 ]
 
 
