@@ -381,6 +381,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
         for (;;) {
             const Piece &p = take();
             if (p.n < 0 || abort_flag) break;
+            // (a tile without rows too: its threads' word that they are done with a buffer must not be counted for the next but one)
+            wait_warp(&mQ[units & 1], units / 2 & 1u);
             const int nq = p.nq[q], r0 = p.r0 + q * BQ, rows = min(BQ, p.sr.n * each - r0);
             const bool there = row < rows;
             // row r of the tile in memory, 8 coordinates from this lane's on

@@ -77,11 +77,12 @@ def attend(q, k, v, q_lens, k_lens, heads, scale, causal, window):
             lo = max(0, length - n + i + 1 - window) if window else 0
             if hi <= lo:
                 continue
-            for h in range(q.shape[1]):
-                s = scale * (k[k0 + lo:k0 + hi, h // each] @ q[q0 + i, h])
-                top = s.max()
-                p = np.exp(s - top)
-                lse[q0 + i, h] = top + np.log(p.sum())
-                out[q0 + i, h] = p @ v[k0 + lo:k0 + hi, h // each] / p.sum()
+            qi, ks, vs = q[q0 + i].reshape(heads, each, -1), k[k0 + lo:k0 + hi], v[k0 + lo:k0 + hi]
+            s = scale * np.einsum("nhw,hew->hen", ks, qi)
+            top = s.max(-1, keepdims=True)
+            p = np.exp(s - top)
+            total = p.sum(-1, keepdims=True)
+            lse[q0 + i] = (top + np.log(total)).reshape(-1)
+            out[q0 + i] = (np.einsum("hen,nhw->hew", p, vs) / total).reshape(q.shape[1:])
         q0, k0 = q0 + n, k0 + length
     return out, lse

@@ -317,3 +317,12 @@ LENS = [  # query rows, keys
 @pytest.mark.parametrize("lens", LENS, ids=lambda x: "x".join(map(str, x[0])) + "-" + "x".join(map(str, x[1])))
 def test_attend(gpu, dtype, q_heads, heads, width, mask, lens):
     check_attend(gpu, dtype, *lens, q_heads, heads, width, mask != "all", 11 if mask == "window" else 0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_heads,heads,width", [(40, 40, 64), (24, 24, 128), (60, 20, 64), (64, 16, 32)])
+@pytest.mark.parametrize("lens", [[300, 20, 563], [130], [257, 1, 1, 390]], ids=str)
+@pytest.mark.parametrize("causal", [False, True])
+def test_attend_many_units(gpu, dtype, q_heads, heads, width, lens, causal):
+    """Blocks with many pieces of work each, among them tiles with few rows beside tiles with none."""
+    check_attend(gpu, dtype, lens, lens, q_heads, heads, width, causal, 0, own_rows=causal)
