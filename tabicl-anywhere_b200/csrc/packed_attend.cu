@@ -14,8 +14,9 @@
 namespace tcu {
 
 constexpr int PA_THREADS = 128;
-// Steps a block takes at least: shorter parts of a unit are more to join.
-constexpr int PA_STEPS = 4;
+// What a unit costs besides its steps, in steps, and the steps that a block takes at least: so that units of one step are a block's
+// each (21 rows of 32 heads on 8 of width 256: 81 us with four units a block), and shorter parts of longer ones are not joined.
+constexpr int PA_EXTRA = 4, PA_STEPS = 5;
 
 template <int DT, int HD_, int WR>
 struct PaShape {
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
     using C = PaShape<DT, HD, WR>;
     using T = typename C::T;
     using Raw = typename C::Raw;
-    using Cut = KaCut<C::R, 1, C::BK>;
+    using Cut = KaCut<C::R, 1, C::BK, PA_EXTRA>;
     constexpr int R = C::R, KW = C::KW, BK = C::BK, OWN = C::OWN, NT = OWN / 8, NO = HD / 8, STAGES = C::STAGES, PITCH = C::PITCH, CP = C::CP;
     extern __shared__ __align__(16) uint8_t sm[];
     uint8_t *Qs = sm + (size_t)STAGES * 2 * C::TILE;
@@ -123,17 +124,47 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
     while (pl.pos < pl.end) {
         const KaRows sr = ka_rows(a, pl.seq);
         const auto sp = Cut::span(a, sr, each, pl.rt);
-        const int n = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), j0 = sp.base + pl.skip * BK, k0 = a.k_starts[pl.seq];
+        // `count` of the unit's steps as they are cut, n of keys
+        const int count = (int)min((long long)(sp.steps - pl.skip), pl.end - pl.pos), skipped = max(0, pl.skip - PA_EXTRA);
+        const int n = max(0, pl.skip + count - PA_EXTRA) - skipped, j0 = sp.base + skipped * BK, k0 = a.k_starts[pl.seq];
         const int r0 = pl.rt * R, rows = min(R, sr.n * each - r0);
         __syncthreads();  // the piece before is done with shared memory
         if (a.width < HD) {
             for (int i = tid; i < (int)(C::SMEM / 16); i += PA_THREADS) reinterpret_cast<uint4 *>(sm)[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
         }
-        for (int i = tid; i < rows * a.width; i += PA_THREADS) {
-            const int r = i / a.width, c = i - r * a.width, p = r0 + r;
-            *reinterpret_cast<Raw *>(Qs + r * PITCH + c * sizeof(T)) =
-                reinterpret_cast<const Raw *>(a.q)[(long long)(sr.first + p / each) * a.q_row + (long long)(pl.head * each + p % each) * a.q_head + c];
+        {
+            // the queries, 16 bytes a thread, 8 on their way together (one after the other they took 200 us for 64 rows of 256)
+            constexpr int PER = 16 / (int)sizeof(Raw), LANES = HD / PER, ROWS = PA_THREADS / LANES, N = R / ROWS < 1 ? 1 : R / ROWS, TURN = N < 8 ? N : 8;
+            const int c = tid % LANES, first = tid / LANES;
+#pragma unroll 1
+            for (int x = 0; x < N; x += TURN) {
+                uint4 w[TURN];
+#pragma unroll
+                for (int y = 0; y < TURN; y++) w[y] = make_uint4(0, 0, 0, 0);
+                auto from = [&](int y) {
+                    const int p = r0 + first + (x + y) * ROWS, i = p / each;
+                    return reinterpret_cast<const Raw *>(a.q) + (long long)(sr.first + i) * a.q_row + (long long)(pl.head * each + p - i * each) * a.q_head + c * PER;
+                };
+                if (wide & 4) {
+#pragma unroll
+                    for (int y = 0; y < TURN; y++)
+                        if (first + (x + y) * ROWS < rows && c * PER < a.width) w[y] = __ldg(reinterpret_cast<const uint4 *>(from(y)));
+                } else {
+#pragma unroll
+                    for (int y = 0; y < TURN; y++)
+                        if (first + (x + y) * ROWS < rows && c * PER < a.width) {
+                            __align__(16) Raw e[PER];
+                            const Raw *q = from(y);
+#pragma unroll
+                            for (int z = 0; z < PER; z++) e[z] = q[z];
+                            w[y] = *reinterpret_cast<const uint4 *>(e);
+                        }
+                }
+#pragma unroll
+                for (int y = 0; y < TURN; y++)
+                    if (first + (x + y) * ROWS < R) *reinterpret_cast<uint4 *>(Qs + (first + (x + y) * ROWS) * PITCH + c * 16) = w[y];
+            }
         }
         auto load = [&](int i) {
             const int at = j0 + i * BK, slot = i % STAGES;
@@ -291,9 +322,9 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
             for (int c = 0; c < NO; c++) *reinterpret_cast<float2 *>(oc + r * CP + 8 * c + 2 * t) = make_float2(o[c][2 * x], o[c][2 * x + 1]);
         }
         __syncthreads();
-        const bool whole = n == sp.steps;
+        const bool whole = count == sp.steps;
         const int2 who = Cut::sharers(pl, pl.pos - pl.skip, sp.steps);
-        const int cols = (a.width + 3) / 4;
+        constexpr int cols = HD / 4;  // of 4 columns
         // one row's `parts` states joined in 4 columns; at(p): where part p's outputs of the row lie, its maximum and its sum
         auto join = [&](int parts, auto at, float4 &v, float &M, float &L) {
             M = -INFINITY, L = 0.f, v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -315,6 +346,7 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
             float *mine = part + Cut::slot(blockIdx.x, pl.skip == 0) * C::PART;
             for (int i = tid; i < rows * cols; i += PA_THREADS) {
                 const int r = i / cols, c = (i - r * cols) * 4;
+                if (c >= a.width) continue;
                 float4 v;
                 float M, L;
                 join(KW, [&](int p) { return From{oc + (p * R + r) * CP + c, mc + p * R + r, lc + p * R + r}; }, v, M, L);
@@ -336,7 +368,8 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
             for (int i = tid; i < R; i += PA_THREADS) s_bad[i] = 0;
             __syncthreads();
             for (int i = tid; i < rows * cols; i += PA_THREADS) {
-                const int r = i / cols, c = (i - r * cols) * 4, p = r0 + r, hq = pl.head * each + p % each, row = sr.first + p / each;
+                const int r = i / cols, c = (i - r * cols) * 4, p = r0 + r, in = p / each, hq = pl.head * each + p - in * each, row = sr.first + in;
+                if (c >= a.width) continue;
                 float4 v;
                 float M, L;
                 if (whole)
@@ -350,18 +383,17 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
                 const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
                 T *out = reinterpret_cast<T *>(a.out) + row * a.o_row + hq * a.o_head + c;
 #pragma unroll
-                for (int x = 0; x < 4; x++)
-                    if (c + x < a.width) {
-                        out[x] = Elem<DT>::put(y[x]);
-                        if (y[x] != y[x]) s_bad[r] = 1;
-                    }
+                for (int x = 0; x < 4; x++) {  // (a width is a multiple of 8)
+                    out[x] = Elem<DT>::put(y[x]);
+                    if (y[x] != y[x]) s_bad[r] = 1;
+                }
                 if (c == 0 && a.lse) a.lse[(size_t)row * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M) + log2f(L)) * 0.69314718055994530942f;
             }
             __syncthreads();
             for (int r = warp; r < rows; r += PA_THREADS / 32)
                 if (s_bad[r]) pa_repair<DT>(a, sr, pl.seq, (r0 + r) / each, pl.head * each + (r0 + r) % each);
         }
-        Cut::next(pl, a, each, sr.n, n);
+        Cut::next(pl, a, each, sr.n, count);
     }
 }
 
@@ -387,11 +419,11 @@ static PaPlan pa_plan(const PackedArgs &a, int sms) {
 template <int DT, int HD, int WR>
 static cudaError_t pa_launch(const PackedArgs &a, const PaPlan &p, void *work, cudaStream_t s) {
     const size_t size = sizeof(typename Elem<DT>::T);
-    // keys' and values' rows in whole 16-byte pieces: bits 0 and 1
+    // keys', values' and queries' rows in whole 16-byte pieces: bits 0 to 2
     auto whole = [&](const void *x, long long row, long long head) {
         return ((uintptr_t)x | (size_t)row * size | (size_t)head * size | (size_t)a.width * size) % 16 == 0;
     };
-    const int wide = (whole(a.k, a.k_row, a.k_head) ? 1 : 0) | (whole(a.v, a.v_row, a.v_head) ? 2 : 0);
+    const int wide = (whole(a.k, a.k_row, a.k_head) ? 1 : 0) | (whole(a.v, a.v_row, a.v_head) ? 2 : 0) | (whole(a.q, a.q_row, a.q_head) ? 4 : 0);
     const cudaError_t e = allow_dynamic_smem((const void *)k_packed_attend<DT, HD, WR>, p.smem);
     if (e != cudaSuccess) return e;
     int *arrived = reinterpret_cast<int *>(work);
