@@ -203,20 +203,33 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
                 for (int y = 0; y < 4; y++) s[x][y] = 0.f;
             if constexpr (C::F32) {
                 const float *qf = reinterpret_cast<const float *>(Qs + (16 * wr + g) * PITCH);
-#pragma unroll 2
-                for (int c = 0; c < HD; c += 8) {
-                    uint32_t h[4], lw[4];
-                    pa_split(qf[c + t], h[0], lw[0]), pa_split(qf[8 * PITCH / 4 + c + t], h[1], lw[1]);
-                    pa_split(qf[c + t + 4], h[2], lw[2]), pa_split(qf[8 * PITCH / 4 + c + t + 4], h[3], lw[3]);
+                // (32 coordinates' sums at a time in the unit, which does not round them to nearest; these are added here)
+#pragma unroll 1
+                for (int c0 = 0; c0 < HD; c0 += 32) {
+                    float part[NT][4];
 #pragma unroll
-                    for (int x = 0; x < NT; x++) {
-                        const float *kf = reinterpret_cast<const float *>(ks + (8 * x + g) * PITCH) + c + t;
-                        uint32_t bh[2], bl[2];
-                        pa_split(kf[0], bh[0], bl[0]), pa_split(kf[4], bh[1], bl[1]);
-                        pa_mma<DT>(s[x], lw, bh[0], bh[1]);
-                        pa_mma<DT>(s[x], h, bl[0], bl[1]);
-                        pa_mma<DT>(s[x], h, bh[0], bh[1]);
+                    for (int x = 0; x < NT; x++)
+#pragma unroll
+                        for (int y = 0; y < 4; y++) part[x][y] = 0.f;
+#pragma unroll
+                    for (int c = c0; c < c0 + 32; c += 8) {
+                        uint32_t h[4], lw[4];
+                        pa_split(qf[c + t], h[0], lw[0]), pa_split(qf[8 * PITCH / 4 + c + t], h[1], lw[1]);
+                        pa_split(qf[c + t + 4], h[2], lw[2]), pa_split(qf[8 * PITCH / 4 + c + t + 4], h[3], lw[3]);
+#pragma unroll
+                        for (int x = 0; x < NT; x++) {
+                            const float *kf = reinterpret_cast<const float *>(ks + (8 * x + g) * PITCH) + c + t;
+                            uint32_t bh[2], bl[2];
+                            pa_split(kf[0], bh[0], bl[0]), pa_split(kf[4], bh[1], bl[1]);
+                            pa_mma<DT>(part[x], lw, bh[0], bh[1]);
+                            pa_mma<DT>(part[x], h, bl[0], bl[1]);
+                            pa_mma<DT>(part[x], h, bh[0], bh[1]);
+                        }
                     }
+#pragma unroll
+                    for (int x = 0; x < NT; x++)
+#pragma unroll
+                        for (int y = 0; y < 4; y++) s[x][y] += part[x][y];
                 }
             } else {
                 const uint32_t qa = pa_smem(Qs + (16 * wr + (lane & 15)) * PITCH + (lane >> 4) * 16);

@@ -49,12 +49,12 @@ __device__ __forceinline__ void pt_tie(float (&v)[32]) {
     for (int i = 0; i < 32; i += 8)
         asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7])::"memory");
 }
-// Two f32 at a time: x * y + z, x + y; and the largest of three.
-__device__ __forceinline__ float2 pt_fma2(float2 x, float2 y, float2 z) {
+// Two f32 at a time: x * y, x + y; and the largest of three.
+__device__ __forceinline__ float2 pt_mul2(float2 x, float2 y) {
     float2 d;
-    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}\n"
+    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}\n"
         : "=f"(d.x), "=f"(d.y)
-        : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
+        : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
     return d;
 }
 __device__ __forceinline__ float2 pt_add2(float2 x, float2 y) {
@@ -457,7 +457,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                     uint32_t h[16];
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
-                        const float2 t = pt_fma2(make_float2(x[32 * b + 2 * k], x[32 * b + 2 * k + 1]), sl2, mm2);
+                        // (the product rounded as the reference's was: of scores past 2^23 the rest would be more than 1)
+                        const float2 t = pt_add2(pt_mul2(make_float2(x[32 * b + 2 * k], x[32 * b + 2 * k + 1]), sl2), mm2);
                         const float2 w = make_float2(kt_ex2(t.x), kt_ex2(t.y));
                         sum[k & 1] = pt_add2(sum[k & 1], w);
                         h[k] = pt_pair<DT>(w.x, w.y);

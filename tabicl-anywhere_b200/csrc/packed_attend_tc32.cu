@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
             const int r = min(row, rows - 1), ri = (r0 + r) / each, hq = pl.head * each + (r0 + r) % each;  // rows past the end repeat the last
             const int my_hi = ka_hi(a, sr, ri) - p.j0, my_lo = ka_lo(a, sr, ri) - p.j0;
             const float rowfac = put_q(sr, ri, hq);
-            // ---- softmax: S(i) -> 2^14 P(i) = 2^(S - m + 14) over S(i), and the factor of what was before ----
+            // ---- softmax: S(i) -> 2^14 P(i) = 2^(S - m + 14) over S(i) (of scores that do not resolve 14: P(i)), and the factor of what was before ----
             float mrun = -INFINITY, lrun = 0.f;
 #pragma unroll 1
             for (int i = at; i < at + p.n; i++) {
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
 #pragma unroll
                 for (int k = 0; k < 64; k++) top[k & 3] = fmaxf(top[k & 3], x[k]);
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                const float mnew = fmaxf(mrun, mx * c1), mm = mnew == -INFINITY ? 0.f : mnew - 14.f;
+                const float mnew = fmaxf(mrun, mx * c1), mm = mnew == -INFINITY ? 0.f : fabsf(mnew) < 1048576.f ? mnew - 14.f : mnew;
                 const float f = mrun == -INFINITY ? 0.f : kt_ex2(mrun - mnew);
                 float psum[4] = {};
 #pragma unroll
@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                     uint32_t w[32];
 #pragma unroll
                     for (int k = 0; k < 32; k++) {
-                        x[32 * b + k] = kt_ex2(fmaf(x[32 * b + k], c1, -mm));
+                        // (the product rounded as the reference's was: of scores past 2^23 the rest would be more than 1)
+                        x[32 * b + k] = kt_ex2(__fmul_rn(x[32 * b + k], c1) - mm);
                         psum[k & 3] += x[32 * b + k];
                     }
                     // P goes where the scores were: of every 16 keys, hi and lo

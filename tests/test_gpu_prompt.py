@@ -326,3 +326,370 @@ def test_attend(gpu, dtype, q_heads, heads, width, mask, lens):
 def test_attend_many_units(gpu, dtype, q_heads, heads, width, lens, causal):
     """Blocks with many pieces of work each, among them tiles with few rows beside tiles with none."""
     check_attend(gpu, dtype, lens, lens, q_heads, heads, width, causal, 0, own_rows=causal)
+
+
+FEW, MANY = ([5, 1, 12], [40, 70, 12]), ([150, 90], [190, 90])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens", [FEW, MANY], ids=["few", "many"])
+@pytest.mark.parametrize("width", [64, 128, 256])
+@pytest.mark.parametrize("what", ["nan", "inf", "queries", "behind"])
+def test_attend_hides_what_is_not_seen(gpu, dtype, lens, width, what):
+    """NaN and infinities in keys and values reach the rows that see them and no others, in the same tile or the next sequence;
+    behind the last sequence nobody's."""
+    ends = np.cumsum(lens[1])
+
+    def spoil(q, k, v):
+        if what == "nan":
+            v[ends[0] - 3, 0, 5], k[ends[1] - 2, 1, 3], v[ends[0], 1] = np.nan, np.nan, np.nan
+        elif what == "inf":
+            v[ends[0] - 3, 0], v[ends[0], 1, 7], k[ends[1] - 1, 0, 0] = np.inf, -np.inf, np.inf
+        elif what == "queries":
+            q[1, 2, 0], q[4, 0] = np.nan, 0
+        else:
+            k[ends[-1]:], v[ends[-1]:] = np.nan, np.inf
+    check_attend(gpu, dtype, *lens, 4, 2, width, True, 0, spoil=spoil)
+    if what != "inf":  # (a plain sum of infinities of one sign and other numbers has no weights of nothing)
+        check_attend(gpu, dtype, *lens, 4, 2, width, True, 9, spoil=spoil)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens", [FEW, MANY], ids=["few", "many"])
+@pytest.mark.parametrize("pad,at", [(1, 0), (0, 1), (3, 5), (8, 8), (4, 4)])
+def test_attend_strides(gpu, dtype, lens, pad, at):
+    for width in (64, 120):
+        check_attend(gpu, dtype, *lens, 6, 3, width, True, 0, pad=pad, at=at)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens", [FEW, MANY], ids=["few", "many"])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 4.0])
+def test_attend_scales(gpu, dtype, lens, scale):
+    check_attend(gpu, dtype, *lens, 4, 2, 64, True, 0, scale=scale)
+    check_attend(gpu, dtype, *lens, 6, 2, 128, False, 0, scale=scale, lse=False)
+
+
+@pytest.mark.parametrize("lens", [FEW, MANY], ids=["few", "many"])
+def test_attend_f32_of_every_size(gpu, lens):
+    """Keys and values whose tiles are many powers of two apart: each tile of 64 keys is held to its own largest."""
+    def spoil(q, k, v):
+        for j in range(0, len(v), 64):
+            v[j:j + 64] *= 10.0 ** (((j // 64) * 7) % 33 - 15)
+        q[:2] *= 1e18
+        k[:70] *= 1e-18
+    check_attend(gpu, "f32", [lens[0][0]], [lens[1][0]], 4, 2, 128, False, 0, spoil=lambda q, k, v: v.__imul__(1e30))
+    check_attend(gpu, "f32", [lens[0][0]], [lens[1][0]], 4, 2, 64, False, 0, spoil=lambda q, k, v: v.__imul__(1e-33))
+
+    def apart(q, k, v):  # rows 0..63 of the keys are seen by all rows, of small values; those behind have large ones
+        v[64:128] *= 1e25
+        q *= 1e-3
+    check_attend(gpu, "f32", [lens[0][0]], [lens[1][0]], 4, 2, 128, True, 0, spoil=apart)
+    check_attend(gpu, "f32", [lens[0][0]], [lens[1][0]], 4, 2, 128, False, 0, spoil=spoil)
+
+
+def torch_attend(q, k, v, scale):
+    """One sequence, every row sees every key, in 64 bits on the GPU."""
+    each = q.shape[1] // k.shape[1]
+    s = torch.einsum("nhw,mhw->hnm", q.double(), k.double().repeat_interleave(each, 1)) * scale
+    return torch.einsum("hnm,mhw->nhw", torch.softmax(s, -1), v.double().repeat_interleave(each, 1)), torch.logsumexp(s, -1).t()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,keys,width", [(1, 100_000, 128), (3, 33_333, 64), (130, 20_001, 128), (300, 9_999, 64), (1, 30_000, 256)])
+def test_attend_long(gpu, dtype, rows, keys, width):
+    code, tt = DT[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(keys)
+    q, k, v = (torch.randn(n, h, width, generator=gen, device="cuda").to(tt) for n, h in ((rows, 4), (keys, 2), (keys, 2)))
+    qs, ks = (torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (rows, keys))
+    p = tcu.Packed(gpu, 1, rows, keys, rows, keys, qs.data_ptr(), ks.data_ptr())
+    work = torch.zeros(p.attend_workspace(code, 4, 2, width), dtype=torch.uint8, device="cuda")
+    out, lse = torch.empty_like(q), torch.empty(rows, 4, device="cuda")
+    first = None
+    for _ in range(2):  # the same to the last bit again: parts are joined in their order
+        p.attend(code, 4, 2, width, q.data_ptr(), 4 * width, width, k.data_ptr(), 2 * width, width, v.data_ptr(), 2 * width, width, out.data_ptr(),
+                 4 * width, width, width**-0.5, lse=lse.data_ptr(), work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+        sync(gpu)
+        assert first is None or torch.equal(first, out)
+        first = out.clone()
+    want, want_lse = torch_attend(q, k, v, width**-0.5)
+    # an output is a sum of thousands of values of either sign: errors of its weights (2^-8, 2^-11 of them, of either sign too) add as
+    # their squares do, and so do the values: relative to the root of the sum of p^2 v^2 a weight's error is a rounding
+    off = (out.double() - want).norm() / want.norm()
+    assert off <= {"f32": 2e-6, "f16": 2.0 * 2**-11, "bf16": 2.0 * 2**-8}[dtype], off
+    assert (lse.double() - want_lse).abs().max() <= 2.0**-18
+
+
+def test_attend_past_32_bits(gpu):
+    """Keys and values whose rows begin up to 2^32 elements apart."""
+    rows, keys, w = 100, 200, 64
+    step = 21_500_000  # 200 rows of it: 4.3e9 elements
+    big = torch.zeros(keys * step + 1024, dtype=torch.float16, device="cuda")
+    k = torch.as_strided(big, (keys, 1, w), (step, w, 1), 0)
+    v = torch.as_strided(big, (keys, 1, w), (step, w, 1), 512)
+    q = torch.randn(rows, 1, w, device="cuda").half()
+    k.copy_(torch.randn(keys, 1, w, device="cuda")), v.copy_(torch.randn(keys, 1, w, device="cuda"))
+    want, want_lse = torch_attend(q, k.contiguous(), v.contiguous(), 0.125)
+    for n in (1, rows):
+        qs, ks = (torch.tensor([0, x], dtype=torch.int32, device="cuda") for x in (n, keys))
+        p = tcu.Packed(gpu, 1, n, keys, n, keys, qs.data_ptr(), ks.data_ptr())
+        work = torch.zeros(p.attend_workspace(1, 1, 1, w), dtype=torch.uint8, device="cuda")
+        out, lse = torch.zeros_like(q), torch.zeros(rows, 1, device="cuda")
+        p.attend(1, 1, 1, w, q.data_ptr(), w, w, k.data_ptr(), step, w, v.data_ptr(), step, w, out.data_ptr(), w, w, 0.125, lse=lse.data_ptr(),
+                 work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+        sync(gpu)
+        # 11 bits of a weight and of an output, of values up to 4.5
+        assert (out[:n].double() - want[:n]).abs().max() <= 2 * 2.0**-11 * 4.5
+        assert (lse[:n].double() - want_lse[:n]).abs().max() <= 2.0**-18
+        assert not out[n:].any()
+
+
+@pytest.mark.parametrize("q_starts,k_starts", [([0, 200, 90], [0, 90, 180]), ([0, 90, 180], [0, 250, 180]), ([-4, 90, 180], [0, 90, 180]),
+                                               ([0, 90, 2**31 - 1], [0, 90, 180]), ([0, 90, 180], [90, 0, 2**30])])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attend_reports_bad_starts(gpu, dtype, q_starts, k_starts):
+    """A sequence whose rows or keys lie outside what was said is left alone and reported; the others are worked out."""
+    code, tt = DT[dtype]
+    q = torch.randn(180, 2, 64, device="cuda").to(tt)
+    out = torch.full_like(q, 9.0)
+    qs, ks = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (q_starts, k_starts))
+    p = tcu.Packed(gpu, 2, 180, 180, 90, 90, qs.data_ptr(), ks.data_ptr())
+    work = torch.zeros(p.attend_workspace(code, 2, 2, 64), dtype=torch.uint8, device="cuda")
+    p.attend(code, 2, 2, 64, q.data_ptr(), 128, 64, q.data_ptr(), 128, 64, q.data_ptr(), 128, 64, out.data_ptr(), 128, 64, 0.125,
+             work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    torch.cuda.synchronize()
+    with pytest.raises(tcu.TcuError, match="outside its range"):
+        gpu.sync()
+    good = [s for s in range(2) if 0 <= q_starts[s] <= q_starts[s + 1] <= 180 and q_starts[s + 1] - q_starts[s] <= 90
+            and 0 <= k_starts[s] <= k_starts[s + 1] <= 180 and k_starts[s + 1] - k_starts[s] <= 90]
+    done = torch.zeros(180, dtype=torch.bool, device="cuda")
+    for s in good:
+        rows, keys = slice(q_starts[s], q_starts[s + 1]), slice(k_starts[s], k_starts[s + 1])
+        want, _ = torch_attend(q[rows], q[keys], q[keys], 0.125)
+        assert (out[rows].double() - want).abs().max() <= 2.0**-8
+        done[rows] = True
+    assert (out[~done] == 9).all()
+    gpu.sync()
+
+
+def test_attend_refusals(gpu):
+    t = torch.zeros(64, 4, 64, device="cuda")
+    s = torch.tensor([0, 64], dtype=torch.int32, device="cuda")
+    p = tcu.Packed(gpu, 1, 64, 64, 64, 64, s.data_ptr(), s.data_ptr())
+    work = torch.zeros(p.attend_workspace(0, 4, 4, 64), dtype=torch.uint8, device="cuda")
+    x = t.data_ptr()
+    ok = dict(dtype=0, q_heads=4, heads=4, width=64, q_ptr=x, q_row=256, q_head=64, k_ptr=x, k_row=256, k_head=64, v_ptr=x, v_row=256, v_head=64,
+              out_ptr=x, o_row=256, o_head=64, scale=1.0, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    for match, kw in [("dtype", dict(dtype=3)), ("heads", dict(heads=3)), ("heads", dict(heads=0)), ("heads", dict(q_heads=0)), ("width", dict(width=12)),
+                      ("width", dict(width=264)), ("width", dict(width=0)), ("window", dict(window=3)), ("window", dict(causal=True, window=-1)),
+                      ("scale", dict(scale=float("nan"))), ("scale", dict(scale=float("inf"))), ("strides", dict(k_row=-1)), ("null", dict(q_ptr=None)),
+                      ("null", dict(v_ptr=None)), ("null", dict(out_ptr=None)), ("aligned", dict(k_ptr=x + 2)), ("aligned", dict(out_ptr=x + 1)),
+                      ("working memory", dict(work_bytes=8)), ("working memory", dict(work=None)), ("aligned", dict(work=work.data_ptr() + 4))]:
+        with pytest.raises(tcu.TcuError, match=match):
+            p.attend(**{**ok, **kw})
+    for bad in (dict(seqs=-1), dict(seqs=70_000), dict(q_rows=-1), dict(max_k=-1), dict(q_rows=2**30)):
+        b = tcu.Packed(gpu, **{**dict(seqs=1, q_rows=64, k_rows=64, max_q=64, max_k=64, q_starts_ptr=s.data_ptr()), **bad})
+        with pytest.raises(tcu.TcuError):
+            b.attend_workspace(0, 4, 4, 64)
+    with pytest.raises(tcu.TcuError, match="null"):
+        tcu.Packed(gpu, 1, 64, 64, 64, 64, None).attend(**ok)
+    for none in (dict(seqs=0), dict(q_rows=0), dict(max_q=0)):  # nothing to do
+        b = tcu.Packed(gpu, **{**dict(seqs=1, q_rows=64, k_rows=64, max_q=64, max_k=64, q_starts_ptr=None), **none})
+        assert b.attend_workspace(0, 4, 4, 64) == 0
+        b.attend(**{**ok, "work": None, "work_bytes": 0})
+    p.attend(**ok)
+    sync(gpu)
+
+
+def test_fp4_refusals(gpu):
+    t = torch.zeros(65536, dtype=torch.uint8, device="cuda")
+    x = t.data_ptr()
+    ok = dict(rows=4, k=64, format=tcu.NV, codes_ptr=x, scales_ptr=x, unit=1.0)
+    for match, kw in [("rows", dict(rows=0)), ("rows", dict(k=0)), ("rows", dict(k=2**25)), ("rows", dict(rows=2**24, k=4096)), ("format", dict(format=2)),
+                      ("unit", dict(unit=0.0)), ("unit", dict(unit=float("nan"))), ("unit", dict(unit=1e31)), ("unit", dict(unit=-1.0)),
+                      ("unit", dict(format=tcu.MX, unit=2.0)), ("null", dict(codes_ptr=None)), ("null", dict(scales_ptr=None)),
+                      ("aligned", dict(codes_ptr=x + 8)), ("aligned", dict(scales_ptr=x + 4))]:
+        m = tcu.Fp4(gpu, **{**ok, **kw})
+        for call in (lambda: m.pack(0, x, 2**26, stream=1), lambda: m.load(0, x, 2**26, stream=1), lambda: m.linear_workspace(m, 0)):
+            with pytest.raises(tcu.TcuError, match=match):
+                call()
+    m = tcu.Fp4(gpu, **ok)
+    for match, a in [("dtype", (3, x, 64)), ("null", (0, None, 64)), ("stride", (0, x, 63)), ("aligned", (0, x + 2, 64))]:
+        with pytest.raises(tcu.TcuError, match=match):
+            m.pack(*a, stream=1)
+        with pytest.raises(tcu.TcuError, match=match):
+            m.load(*a, stream=1)
+    work = torch.zeros(m.linear_workspace(m, 0), dtype=torch.uint8, device="cuda")
+    w = dict(work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    for match, a, kw in [("dtype", (m, 5, x, 4), w), ("null", (m, 0, None, 4), w), ("stride", (m, 0, x, 3), w), ("stride", (m, 0, x, 4), dict(w, residual=x, ldr=3)),
+                         ("act", (m, 0, x, 4), dict(w, act=2)), ("aligned", (m, 0, x + 2, 4), w), ("aligned", (m, 0, x, 4), dict(w, bias=x + 1)),
+                         ("working memory", (m, 0, x, 4), dict(w, work_bytes=16)), ("working memory", (m, 0, x, 4), dict(w, work=None)),
+                         ("format", (tcu.Fp4(gpu, **{**ok, "format": tcu.MX}), 0, x, 4), w), ("format", (tcu.Fp4(gpu, **{**ok, "k": 65}), 0, x, 4), w),
+                         ("units", (tcu.Fp4(gpu, **{**ok, "unit": 1e-30}), 0, x, 4), w)]:
+        with pytest.raises(tcu.TcuError, match=match):
+            (tcu.Fp4(gpu, **{**ok, "unit": 1e-30}) if match == "units" else m).linear(*a, **kw)
+    assert tcu.Fp4.code_bytes(0, 4) == 0 and tcu.Fp4.code_bytes(2**25, 2**24) == 0 and tcu.Fp4.scale_bytes(4, 4, 2) == 0
+    sync(gpu)
+
+
+@pytest.mark.parametrize("name", ["mx", "nv"])
+@pytest.mark.parametrize("rows", [5, 40, 200])
+def test_linear_keeps_rows_apart(gpu, name, rows):
+    """A NaN scale in a row of x or of W makes that row's or column's outputs NaN and no others."""
+    fmt = FORMATS[name]
+    rng = np.random.default_rng(rows)
+    x, xv = random_matrix(rng, gpu, rows, 300, fmt)
+    w, wv = random_matrix(rng, gpu, 150, 300, fmt)
+    for m, row in ((x, 3), (w, 129)):
+        m.scales[row // 128 * (m.scales.numel() // (-(-(rows if m is x else 150) // 128))) + row % 32 * 16 + row % 128 // 32 * 4 + 1] = 255 if fmt == plain.MX else 127
+    y = torch.zeros(rows, 150, device="cuda")
+    work = torch.zeros(w.m.linear_workspace(x.m, 0), dtype=torch.uint8, device="cuda")
+    w.m.linear(x.m, 0, y.data_ptr(), 150, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    got = host(y)
+    assert np.isnan(got[3]).all() and np.isnan(got[:, 129]).all()
+    fine = np.ones((rows, 150), bool)
+    fine[3], fine[:, 129] = False, False
+    want, size = xv @ wv.T, np.abs(xv) @ np.abs(wv).T
+    assert (np.abs(got - want) <= 30 * 2.0**-23 * size)[fine].all()
+
+
+# ---- a run of them together -----------------------------------------------------------------------------------------
+
+def gelu(x):
+    return 0.5 * x * (1 + torch.erf(x / 2**0.5))
+
+
+class Layer:
+    """A prompt's layer on the operators: projection, attention, the cache's store, output with residual, feed-forward, answer."""
+
+    def __init__(self, gpu, dtype, lens, d, q_heads, heads, width, ff, classes, fmt):
+        self.gpu, self.lens, self.fmt = gpu, lens, fmt
+        self.code, self.tt = DT[dtype]
+        self.hq, self.h, self.w, self.d, self.ff, self.classes = q_heads, heads, width, d, ff, classes
+        gen = torch.Generator(device="cuda").manual_seed(5)
+        rand = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+        n = sum(lens)
+        self.x = rand(n, d).to(self.tt)
+        self.weights = {}
+        for name, rows, cols in (("qkv", (q_heads + 2 * heads) * width, d), ("out", d, q_heads * width), ("up", ff, d), ("down", d, ff), ("head", classes, d)):
+            self.weights[name] = (self.matrix(rows, cols), (0.1 * rand(rows)).to(self.tt))
+            w = (rand(rows, cols) / cols**0.5).to(self.tt)
+            self.weights[name][0].pack(self.code, w, float(w.abs().max()) / 2688 if fmt == tcu.NV else 1.0)
+        self.inputs = {k: self.matrix(n, c) for k, c in (("x", d), ("a", q_heads * width), ("h", d), ("f", ff), ("y", d))}
+        new = lambda *s, dt=self.tt: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+        self.qkv, self.att, self.hid, self.up, self.y = new(n, q_heads + 2 * heads, width), new(n, q_heads * width), new(n, d), new(n, ff), new(n, d)
+        self.logits, self.lp, self.lse = new(n, classes), new(n, 1, dt=torch.float32), new(n, q_heads, dt=torch.float32)
+        self.labels = torch.randint(0, classes, (n, 1), generator=gen, device="cuda").int()
+        self.starts = torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int32, device="cuda")
+        self.packed = tcu.Packed(gpu, len(lens), n, n, max(lens), max(lens), self.starts.data_ptr())
+        pages = -(-n // 64) + 1
+        self.pool = torch.zeros(pages * tcu.Kv4Cache.page_bytes(heads, width, 64, 32), dtype=torch.uint8, device="cuda")
+        self.cache = tcu.Kv4Cache(gpu, self.pool.data_ptr(), pages, heads=heads, width=width, page=64, group=32)
+        self.slots = torch.arange(n, device="cuda")
+        need = max([self.packed.attend_workspace(self.code, q_heads, heads, width)] +
+                   [self.weights[k][0].m.m.linear_workspace(self.inputs[i].m.m, self.code) for k, i in (("qkv", "x"), ("out", "a"), ("up", "h"), ("down", "f"), ("head", "y"))])
+        self.work = torch.zeros(need, dtype=torch.uint8, device="cuda")  # one block serves them all
+
+    def matrix(self, rows, cols):
+        layer = self
+
+        class Held:
+            def __init__(self):
+                self.rows, self.cols, self.m = rows, cols, None
+
+            def pack(self, code, x, unit, stream=1):
+                if self.m is None:
+                    self.m = Matrix(layer.gpu, rows, cols, layer.fmt, unit)
+                self.m.m.pack(code, x.data_ptr(), cols, stream=stream)
+
+            def values(self):
+                y = torch.empty(rows, cols, device="cuda")
+                self.m.m.load(0, y.data_ptr(), cols, stream=1)
+                return y.double()
+        held = Held()
+        held.m = Matrix(layer.gpu, rows, cols, layer.fmt, 1.0 if layer.fmt == tcu.MX else 2.0**-9)
+        return held
+
+    def linear(self, name, inp, src, out, stream, act=0, residual=None):
+        self.inputs[inp].pack(self.code, src, None, stream)
+        w, b = self.weights[name]
+        w.m.m.linear(self.inputs[inp].m.m, self.code, out.data_ptr(), w.rows, bias=b.data_ptr(), act=act,
+                     residual=residual.data_ptr() if residual is not None else None, ldr=w.rows, work=self.work.data_ptr(),
+                     work_bytes=self.work.numel(), stream=stream)
+
+    def run(self, stream):
+        hq, h, w, es = self.hq, self.h, self.w, self.x.element_size()
+        row = (hq + 2 * h) * w
+        self.linear("qkv", "x", self.x, self.qkv, stream)
+        q = self.qkv.data_ptr()
+        k, v = q + hq * w * es, q + (hq + h) * w * es
+        self.packed.attend(self.code, hq, h, w, q, row, w, k, row, w, v, row, w, self.att.data_ptr(), hq * w, w, w**-0.5, causal=True,
+                           lse=self.lse.data_ptr(), work=self.work.data_ptr(), work_bytes=self.work.numel(), stream=stream)
+        self.cache.store(self.code, len(self.slots), self.slots.data_ptr(), k, row, w, v, row, w, stream=stream)
+        self.linear("out", "a", self.att, self.hid, stream, residual=self.x)
+        self.linear("up", "h", self.hid, self.up, stream, act=1)
+        self.linear("down", "f", self.up, self.y, stream, residual=self.hid)
+        self.linear("head", "y", self.y, self.logits, stream)
+        self.gpu.label_logprobs(self.code, self.logits.data_ptr(), len(self.slots), self.classes, self.classes, self.labels.data_ptr(), 1,
+                                self.lp.data_ptr(), stream=stream)
+
+    def check(self, tol):
+        """Each stage against 64 bits from what the stage before has left."""
+        def linear(name, inp):
+            w, b = self.weights[name]
+            return self.inputs[inp].values() @ w.values().t() + b.double()
+        near = lambda a, b: (a.double() - b).norm() <= tol * b.norm()  # noqa: E731
+        qkv = self.qkv.double().view(len(self.x), -1, self.w)
+        assert near(self.qkv.view(len(self.x), -1), linear("qkv", "x"))
+        at = 0
+        for n in self.lens:
+            q, k, v = qkv[at:at + n].split([self.hq, self.h, self.h], 1)
+            each = self.hq // self.h
+            s = torch.einsum("nhw,mhw->hnm", q, k.repeat_interleave(each, 1)) * self.w**-0.5
+            s.masked_fill_(torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -torch.inf)
+            want = torch.einsum("hnm,mhw->nhw", torch.softmax(s, -1), v.repeat_interleave(each, 1))
+            assert near(self.att[at:at + n], want.reshape(n, -1))
+            assert (self.lse[at:at + n].double() - torch.logsumexp(s, -1).t()).abs().max() < 1e-4
+            at += n
+        assert near(self.hid, linear("out", "a") + self.x.double())
+        assert near(self.up, gelu(linear("up", "h")))
+        assert near(self.y, linear("down", "f") + self.hid.double())
+        assert near(self.logits, linear("head", "y"))
+        want = torch.log_softmax(self.logits.double(), -1).gather(1, self.labels.long())
+        assert (self.lp.double() - want).abs().max() < 1e-4
+        k, v = torch.empty(len(self.x), self.h, self.w, device="cuda"), torch.empty(len(self.x), self.h, self.w, device="cuda")
+        self.cache.load(0, len(self.slots), self.slots.data_ptr(), k.data_ptr(), self.h * self.w, self.w, v.data_ptr(), self.h * self.w, self.w, stream=1)
+        torch.cuda.synchronize()
+        assert (k.double() - qkv[:, self.hq:self.hq + self.h]).norm() <= 0.1 * k.double().norm()  # (what four bits hold)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("fmt", ["mx", "nv"])
+def test_a_prompts_layer(gpu, dtype, fmt):
+    """Projection to answer on the caller's stream, again in a graph with other inputs, and beside itself on two streams."""
+    # a stage's rounding to its type, of values of which most are near the largest; f32: sums of some 500 products
+    tol = {"f32": 4e-6, "f16": 2 * 2.0**-11, "bf16": 2 * 2.0**-8}[dtype]
+    layer = Layer(gpu, dtype, [200, 1, 37, 130], 512, 8, 2, 64, 1000, 300, FORMATS[fmt])
+    layer.run(1)
+    sync(gpu)
+    layer.check(tol)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            layer.run(side.cuda_stream)
+        layer.x.copy_(torch.randn_like(layer.x))
+        graph.replay(), graph.replay()
+    sync(gpu)
+    layer.check(tol)
+    want = layer.y.clone()
+    other = Layer(gpu, dtype, [200, 1, 37, 130], 512, 8, 2, 64, 1000, 300, FORMATS[fmt])
+    other.x.copy_(layer.x)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for one, s in zip((layer, other), streams):
+            one.run(s.cuda_stream)
+    sync(gpu)
+    assert torch.equal(layer.y, want) and torch.equal(other.y, want)
