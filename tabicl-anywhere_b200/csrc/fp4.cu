@@ -1,5 +1,9 @@
 // Matrices in microscaled four-bit floating point: quantised, and read back. Both move bytes: a value of 2 or 4 bytes there,
 // half a byte and its share of a scale here.
+//
+// A block's scale and its numbers are those of exact arithmetic: a power of two divides exactly; for an e4m3 scale times the unit
+// the quotient is taken in f32 from both sides of its error, and where the two sides give different codes the border between them,
+// times scale and unit, is compared in 64 bits, which hold it (2 + 4 + 24 bits) exactly.
 #include "fp4.cuh"
 
 namespace tcu {
@@ -169,7 +173,8 @@ __device__ __forceinline__ float load16(const typename Elem<DT>::T *p, int there
 }
 
 // A thread quantises 16 neighbours: a block of FP4_NV, half a block of FP4_MX. 4 or 8 threads make a word of scales. Bound by its
-// instructions, some 130 for 16 values (8192 x 8192 bf16: BOTHTIMES).
+// instructions (8192 x 8192 bf16 to FP4_NV: 38 us, issue active in 71%, 172 MB at 4.5 TB/s; read back 29 us). Trying every value
+// against 64-bit borders where one of 16 was within 2^-20 of one took 69 us, with the values kept in local memory for it 52.
 template <int DT, bool NV>
 __global__ void __launch_bounds__(FP_THREADS, 8) k_fp4_pack(Fp4Args a, unsigned per, FpDiv div, unsigned total, int quads, int wide, float inv_six) {
     using T = typename Elem<DT>::T;

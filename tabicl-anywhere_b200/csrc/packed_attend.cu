@@ -1,11 +1,12 @@
-// Attention of packed rows over keys and values as they are, for few rows of any type, and for what the tensor-core kernel
-// (packed_attend_tc.cu) does not take: f32, widths above 128, rows that TMA cannot fetch.
+// Attention of packed rows over keys and values as they are, for few rows of any type, and for what the tensor-core kernels
+// (packed_attend_tc.cu, packed_attend_tc32.cu) do not take: widths above 128, 16-bit rows that TMA cannot fetch.
 //
 // 16 or 64 query rows of one key head (the heads that share it side by side) against steps of 64 keys (f32: 32) that come by
 // asynchronous copies. With 16 rows the four warps share a step's keys, with 64 its rows. One pass: running maxima and sums, the
 // output in registers, the matrix products by warp (16-bit operands as they are; f32 as two tf32, of 11 bits each, in three
 // products). A call of few rows streams its keys and values, so it is bound by memory; the steps of all sequences are cut evenly
-// over the blocks (kv4_plan.cuh), whose parts the last of them joins in order.
+// over the blocks (kv4_plan.cuh), whose parts the last of them joins in order. 32 requests of 0 to 16,383 bf16 tokens, 32 heads on 8 of
+// width 128: 188 us for 1.05 GB, 5.6 TB/s (343 us with a division for every 16 bytes copied).
 #include <algorithm>
 #include <type_traits>
 

@@ -8,6 +8,8 @@
 // registers, so every sum across steps is taken in f32 with rounding to nearest (the matrix unit's own accumulation is not: over
 // 10,000 keys it would cost 2.8e-5 of an output). As in the attention over the four-bit cache (kv4_attend_tc.cu), whose two
 // warpgroups that widen codes are not needed here.
+// 2048 rows over 10,000 keys, 4 heads of 128: 165 us, 0.25 PFLOP/s of scores and sums (0.76 of products), 15 of them the split; by
+// warps' products (packed_attend.cu) 1040. Bound by latency: a step's products, softmax and fold follow one another.
 #include <algorithm>
 
 #include "kv4_tc.cuh"
