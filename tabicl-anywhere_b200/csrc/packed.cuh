@@ -72,6 +72,7 @@ __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int 
         d *= a.scale;
         const float top = fmaxf(m, d), ref = top == -INFINITY ? 0.f : top, f = m == -INFINITY ? 0.f : expf(m - ref), p = expf(d - ref);
         l = l * f + p, m = top;
+        if (l != l) break;  // whatever follows, every output is NaN (all lanes have the same score)
 #pragma unroll
         for (int c = 0; c < 8; c++)
             if (lane + 32 * c < a.width) o[c] = fmaf(p, Elem<DT>::get(v[lane + 32 * c]), f == 1.f ? o[c] : o[c] * f);

@@ -328,6 +328,56 @@ def test_attend_many_units(gpu, dtype, q_heads, heads, width, lens, causal):
     check_attend(gpu, dtype, lens, lens, q_heads, heads, width, causal, 0, own_rows=causal)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("q_heads,width", [(129, 64), (150, 32), (128, 128), (16, 64), (5, 128), (300, 64)])
+def test_attend_many_heads_on_one(gpu, dtype, q_heads, width):
+    """More heads of a token than a tile has rows, and numbers that do not divide it."""
+    check_attend(gpu, dtype, [3, 40], [3, 70], q_heads, 1, width, True, 0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attend_many_sequences(gpu, dtype):
+    rng = np.random.default_rng(0)
+    check_attend(gpu, dtype, [1] * 3000, list(rng.integers(0, 5, 3000)), 2, 1, 32, False, 0)
+    lens = list(rng.integers(0, 3, 1500)) + [70]
+    check_attend(gpu, dtype, lens, lens, 2, 2, 64, True, 0, own_rows=True)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [3, 100])
+def test_attend_starts_behind_the_first_row(gpu, dtype, rows):
+    """Rows and keys before the first sequence's are nobody's."""
+    code, tt = DT[dtype]
+    q, k, v = (torch.randn(n, 2, 64, device="cuda").to(tt) for n in (rows + 7, 140, 140))
+    k[:9], v[:9] = float("nan"), float("inf")
+    out = torch.full_like(q, 9.0)
+    qs, ks = torch.tensor([7, rows + 7], dtype=torch.int32, device="cuda"), torch.tensor([9, 139], dtype=torch.int32, device="cuda")
+    p = tcu.Packed(gpu, 1, rows + 7, 140, rows, 130, qs.data_ptr(), ks.data_ptr())
+    work = torch.zeros(p.attend_workspace(code, 2, 2, 64), dtype=torch.uint8, device="cuda")
+    p.attend(code, 2, 2, 64, q.data_ptr(), 128, 64, k.data_ptr(), 128, 64, v.data_ptr(), 128, 64, out.data_ptr(), 128, 64, 0.125,
+             work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    want, _ = torch_attend(q[7:], k[9:139], v[9:139], 0.125)
+    assert (out[:7] == 9).all() and (out[7:].double() - want).abs().max() <= 2 * ULP["bf16"] * 4.5  # (a weight's rounding, of values up to 4.5)
+
+
+def test_linear_of_many_rows(gpu):
+    """More rows than a 16-bit number counts, and a product of a matrix with itself."""
+    rng = np.random.default_rng(1)
+    x, xv = random_matrix(rng, gpu, 70_001, 64, plain.NV)
+    w, wv = random_matrix(rng, gpu, 40, 64, plain.NV)
+    for m, mv in ((w, wv), (None, None)):
+        if m is None:
+            x, xv = random_matrix(rng, gpu, 300, 64, plain.MX)
+            m, mv = x, xv
+        y = torch.zeros(len(xv), len(mv), dtype=torch.bfloat16, device="cuda")
+        work = torch.zeros(m.m.linear_workspace(x.m, 2), dtype=torch.uint8, device="cuda")
+        m.m.linear(x.m, 2, y.data_ptr(), len(mv), work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+        sync(gpu)
+        want, size = xv @ mv.T, np.abs(xv) @ np.abs(mv).T
+        assert (np.abs(host(y) - want) <= 9 * 2.0**-23 * size + 1.01 * ULP["bf16"] * np.abs(want)).all()
+
+
 FEW, MANY = ([5, 1, 12], [40, 70, 12]), ([150, 90], [190, 90])
 
 
