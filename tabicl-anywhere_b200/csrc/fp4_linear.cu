@@ -6,8 +6,8 @@
 // copies and go on to tensor memory. W on the unit's side of 128 serves one row and thousands alike: few rows make a narrow
 // tile, and the weights stream at the memory's rate with no instruction of a thread's spent on them.
 // What bounds it: of many rows the matrix unit (4096 x 14336 x 8192 bf16 out: 259 us, 3.7 PFLOP/s, its pipe busy in 76%); of few the
-// weights (8 rows of that: 15.6 us, 66 MB at 4.2 TB/s, of which 4 us are start and output); below that launch and latency (one row,
-// 1024 x 512: 6.9 us). A step's issue in a loop that worked out its descriptors and divided by the number of slots took 353 and
+// weights (8 rows of that: 14.6 us, 66 MB at 4.5 TB/s, of which 4 us are start and output); below that launch and latency (one row,
+// 1024 x 512: 6.5 us). A step's issue in a loop that worked out its descriptors and divided by the number of slots took 353 and
 // 24 us, outputs in code for all of a thread's 128 sums 930 us (the instruction caches did not hold it).
 #include <cudaTypedefs.h>
 
@@ -96,8 +96,8 @@ __device__ __forceinline__ int2 fl_place(const FlPlan &p, int t) {
 
 // Warp 0: the copies; warp 1: the products; warps 4-11: sums from tensor memory, joining and output, a thread one output of
 // half the tile's rows. The steps of all tiles in a row are cut evenly over the blocks; parts of a tile meet in the working
-// memory, and the last block to arrive joins them in order.
-template <int DT, bool NV>
+// memory, and the last block to arrive joins them in order. OWN: rows of a tile that a thread takes at most.
+template <int DT, bool NV, int OWN>
 __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, FlPlan p, const __grid_constant__ CUtensorMap map_w,
                                                               const __grid_constant__ CUtensorMap map_x, float *part, int *arrived) {
     using T = typename Elem<DT>::T;
@@ -235,16 +235,37 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
         while (pos < end) {
             const int t = (int)ka_div(pos, p.steps), s0 = (int)(pos - (long long)t * p.steps), s1 = (int)min((long long)p.steps, s0 + end - pos);
             const int2 place = fl_place(p, t);
-            float v[128];
+            const bool whole = s0 == 0 && s1 == p.steps;
+            const int n = place.y * FL_M + quad * 32 + lane, row0 = place.x * p.nt + c0;
+            const float bias = a.bias && n < a.n ? Elem<DT>::get(reinterpret_cast<const T *>(a.bias)[n]) : 0.f;
+            T *y = reinterpret_cast<T *>(a.y) + (size_t)row0 * a.ldy + n;
+            const T *r = reinterpret_cast<const T *>(a.residual) + (a.residual ? (size_t)row0 * a.ldr + n : 0);
+            // The residual of a narrow tile of a 16-bit type is loaded whole before its products are waited for, two rows a register: a
+            // load waits for the copies asked for before it, some 3,000 cycles (4096 x 8192 x 2048, bf16: 65 us without a residual, 115
+            // to 125 so, 152 with one asked for 16 rows ahead, 160 in tiles of 256 rows, whose sums leave no registers for either).
+            constexpr bool EARLY = OWN <= 64 && DT != DT_F32;
+            uint32_t held[EARLY ? OWN / 2 : 1];
+            if constexpr (EARLY) {
+                const int rows = a.residual && n < a.n ? min(own, a.rows - row0) : 0;
+                const uint16_t *q = reinterpret_cast<const uint16_t *>(r);
 #pragma unroll
-            for (int i = 0; i < 128; i++) v[i] = 0.f;
+                for (int i = 0; i < OWN / 2; i++) held[i] = 0;
+                if (rows > 0) {
+#pragma unroll
+                    for (int i = 0; i < OWN / 2; i++)
+                        held[i] = (2 * i < rows ? q[(size_t)(2 * i) * a.ldr] : 0u) | (2 * i + 1 < rows ? (uint32_t)q[(size_t)(2 * i + 1) * a.ldr] << 16 : 0u);
+                }
+            }
+            float v[OWN];
+#pragma unroll
+            for (int i = 0; i < OWN; i++) v[i] = 0.f;
             for (int from = s0; from < s1; from += p.chunk, c++) {
                 const int acc = c & (p.nacc - 1);
                 wait_warp(&m_acc[acc], (uint32_t)(c >> (p.nacc - 1)) & 1u);
                 fence_after_sync();
                 const uint32_t d = tmem + acc * (p.acc_cols / p.nacc) + c0 + ((uint32_t)(quad * 32) << 16);
 #pragma unroll
-                for (int g = 0; g < 8; g++) {
+                for (int g = 0; g < OWN / 16; g++) {
                     if (g * 16 < own) {
                         float x[16];
                         tmem_ld16(d + g * 16, x);
@@ -256,21 +277,30 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
                 fence_before_sync();
                 mbar_arrive(&m_free[acc]);
             }
-            const bool whole = s0 == 0 && s1 == p.steps;
-            const int n = place.y * FL_M + quad * 32 + lane, row0 = place.x * p.nt + c0;
-            const float bias = a.bias && n < a.n ? Elem<DT>::get(reinterpret_cast<const T *>(a.bias)[n]) : 0.f;
-            T *y = reinterpret_cast<T *>(a.y) + (size_t)row0 * a.ldy + n;
-            const T *r = reinterpret_cast<const T *>(a.residual) + (a.residual ? (size_t)row0 * a.ldr + n : 0);
-            // 16 rows' outputs from their sums, of which `rows` there are
+            // 16 rows' outputs from their sums, of which `rows` there are; f32 residuals are asked for 16 rows ahead
+            constexpr bool AHEAD = DT == DT_F32;
+            float next[16];
+            auto ask = [&](int rows) {
+                if (!a.residual) return;
+#pragma unroll
+                for (int i = 0; i < 16; i++) next[i] = i < rows ? Elem<DT>::get(r[(size_t)i * a.ldr]) : 0.f;
+                r += (size_t)16 * a.ldr;
+            };
             auto put = [&](const float *sum, int rows) {
                 float f[16];
-                if (a.residual) {
+                if (EARLY && a.residual) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) f[i] = i < rows ? Elem<DT>::get(r[(size_t)i * a.ldr]) : 0.f;
-                    r += (size_t)16 * a.ldr;
+                    for (int i = 0; i < 16; i++) {
+                        const uint16_t h = (uint16_t)(held[i / 2] >> (i & 1) * 16);
+                        f[i] = Elem<DT>::get(*reinterpret_cast<const T *>(&h));
+                    }
+#pragma unroll
+                    for (int i = 0; i < OWN / 2 - 8; i++) held[i] = held[i + 8];
                 } else {
+                    if constexpr (!AHEAD) ask(rows);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) f[i] = 0.f;
+                    for (int i = 0; i < 16; i++) f[i] = a.residual ? next[i] : 0.f;
+                    if constexpr (AHEAD) ask(rows - 16);
                 }
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
@@ -281,6 +311,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
                 y += (size_t)16 * a.ldy;
             };
             const int rows = n < a.n && !abort_flag ? min(own, a.rows - row0) : 0;
+            if constexpr (AHEAD) ask(rows);
             if (whole) {
                 // 16 values at a time, the others moved up behind them: code for all 128 would not stay in the instruction caches (a
                 // call of one row took 24 us so)
@@ -288,7 +319,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
                 for (int there = rows; there > 0; there -= 16) {
                     put(v, there);
 #pragma unroll
-                    for (int i = 0; i < 112; i++) v[i] = v[i + 16];
+                    for (int i = 0; i < OWN - 16; i++) v[i] = v[i + 16];
                 }
             } else {
                 // parts: each block's into its slot (the tile's first block's into its second slot, the others' into their first)
@@ -297,7 +328,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
                 const size_t size = (size_t)FL_M * p.nt;
                 float *at = part + c0 * FL_M + quad * 32 + lane, *to = at + (2 * (size_t)blockIdx.x + (s0 == 0)) * size;
 #pragma unroll
-                for (int g = 0; g < 8; g++)
+                for (int g = 0; g < OWN / 16; g++)
                     if (g * 16 < own) {
 #pragma unroll
                         for (int i = 0; i < 16; i++) __stcg(to + (g * 16 + i) * FL_M, v[g * 16 + i]);
@@ -345,7 +376,7 @@ static FlPlan fl_plan(int dtype, const Fp4LinearArgs &a, int sms) {
     p.quads = fp4_quads(a.k, a.format), p.steps = (kp + FL_STEP - 1) / FL_STEP;
     p.feat_tiles = (a.n + FL_M - 1) / FL_M;
     // How many rows a tile has, and over how many blocks it is cut: what takes the fewest cycles, from what was measured (8 to 4096
-    // rows): a step 420 and 3 a row of the tile, a tile's output 1000 and 12 a row; the parts of a cut tile 7000 and 100 a row for
+    // rows): a step 420 and 3 a row of the tile, a tile's output 1000 and 12 a row, 20000 more for a residual in a tile of 256; the parts of a cut tile 7000 and 100 a row for
     // storing and waiting, and each part 600 and 25 a row in the block that joins them (2048 x 1024 x 4096: whole tiles of 128 rows
     // 15.6 us, cut over all SMs 27.2; of 256 rows 20.9 and 39.3. 4096 x 14336 x 8192: of 256 rows 255 us, of 128 330).
     const int widest = std::min(dtype == DT_F32 ? 128 : 256, (a.rows + 15) / 16 * 16);
@@ -355,7 +386,7 @@ static FlPlan fl_plan(int dtype, const Fp4LinearArgs &a, int sms) {
         if (nt > 128) nt = 256;
         if (nt > 128 ? widest <= 128 : nt > widest || (a.rows > nt && nt % 128)) continue;  // (a tile begins with a block of scales)
         const long long tiles = (long long)((a.rows + nt - 1) / nt) * p.feat_tiles;
-        const double step = 420 + 3.0 * nt, out = 1000 + 12.0 * nt;
+        const double step = 420 + 3.0 * nt, out = 1000 + 12.0 * nt + (a.residual && nt > 128 ? 20000 : 0);
         for (int parts = 1; parts <= 32 && parts <= p.steps; parts *= 2) {
             if (parts > 1 && tiles * parts > 2 * sms) break;
             const long long blocks = std::min<long long>(sms, tiles * parts);
@@ -383,8 +414,15 @@ static FlPlan fl_plan(int dtype, const Fp4LinearArgs &a, int sms) {
 }
 
 size_t fp4_linear_workspace(int dtype, const Fp4LinearArgs &a, int sms) {
-    const FlPlan p = fl_plan(dtype, a, sms);
-    return sizeof(int) * KA_BLOCKS + (size_t)p.blocks * 2 * FL_M * p.nt * sizeof(float);
+    // (for a call with a residual and for one without: the plan is not the same)
+    Fp4LinearArgs b = a;
+    size_t parts = 0;
+    for (const void *residual : {(const void *)nullptr, (const void *)&b}) {
+        b.residual = residual;
+        const FlPlan p = fl_plan(dtype, b, sms);
+        parts = std::max(parts, p.split ? (size_t)p.blocks * 2 * FL_M * p.nt * sizeof(float) : 0);
+    }
+    return sizeof(int) * KA_BLOCKS + parts;
 }
 
 static bool fl_map(void *encode, CUtensorMap *m, const uint8_t *codes, int rows, int k, int box) {
@@ -395,14 +433,20 @@ static bool fl_map(void *encode, CUtensorMap *m, const uint8_t *codes, int rows,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DT, bool NV>
+template <int DT, bool NV, int OWN>
 static cudaError_t launch(const Fp4LinearArgs &a, const FlPlan &p, const CUtensorMap &w, const CUtensorMap &x, void *work, cudaStream_t s) {
     const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
-    const cudaError_t e = allow_dynamic_smem((const void *)k_fp4_linear<DT, NV>, FL_SMEM);
+    const cudaError_t e = allow_dynamic_smem((const void *)k_fp4_linear<DT, NV, OWN>, FL_SMEM);
     if (e != cudaSuccess) return e;
     int *arrived = reinterpret_cast<int *>(work);
-    k_fp4_linear<DT, NV><<<p.blocks, FL_THREADS, smem, s>>>(a, p, w, x, reinterpret_cast<float *>(arrived + KA_BLOCKS), arrived);
+    k_fp4_linear<DT, NV, OWN><<<p.blocks, FL_THREADS, smem, s>>>(a, p, w, x, reinterpret_cast<float *>(arrived + KA_BLOCKS), arrived);
     return cudaGetLastError();
+}
+template <int DT, bool NV>
+static cudaError_t launch(const Fp4LinearArgs &a, const FlPlan &p, const CUtensorMap &w, const CUtensorMap &x, void *work, cudaStream_t s) {
+    if constexpr (DT != DT_F32)
+        if (p.nt > 128) return launch<DT, NV, 128>(a, p, w, x, work, s);
+    return launch<DT, NV, 64>(a, p, w, x, work, s);
 }
 
 cudaError_t launch_fp4_linear(int dtype, const Fp4LinearArgs &a, int sms, void *encode, void *work, cudaStream_t s, uint64_t *launches) {
