@@ -8,6 +8,7 @@ any machine with the driver, next to whatever runtime the host process (PyTorch,
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -45,15 +46,18 @@ def build(force=False, verbose=False):
     # an object is rebuilt when it is older than its source, any header or this script
     newest_dep = max(os.path.getmtime(p) for p in [os.path.join(CSRC, h) for h in HEADERS] +
                      [os.path.join(HERE, "..", "include", "tabicl_b200.h"), os.path.abspath(__file__)])
+    commands = []
     for src in SOURCES:
         obj = os.path.join(bdir, src + ".o")
         path = os.path.join(CSRC, src)
         if force or not os.path.exists(obj) or os.path.getmtime(obj) < max(newest_dep, os.path.getmtime(path)):
-            cmd = [NVCC, *FLAGS, "-c", path, "-o", obj]
+            commands.append([NVCC, *FLAGS, "-c", path, "-o", obj])
             if verbose:
-                print(" ".join(cmd))
-            subprocess.run(cmd, check=True)
+                print(" ".join(commands[-1]))
         objs.append(obj)
+    # a few sources at a time: the attention's variants take a minute each
+    with ThreadPoolExecutor(max(1, min(4, os.cpu_count() or 1))) as pool:
+        list(pool.map(lambda cmd: subprocess.run(cmd, check=True), commands))
     tmp = LIB + ".tmp"
     cmd = [NVCC, *FLAGS, "-shared", *objs, "-o", tmp]
     if verbose:
