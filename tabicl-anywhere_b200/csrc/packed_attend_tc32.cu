@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
             const int r = min(row, rows - 1), ri = (r0 + r) / each, hq = pl.head * each + (r0 + r) % each;  // rows past the end repeat the last
             const int my_hi = ka_hi(a, sr, ri) - p.j0, my_lo = ka_lo(a, sr, ri) - p.j0;
             const float rowfac = put_q(sr, ri, hq);
-            // ---- softmax: S(i) -> 2^14 P(i) = 2^(S - m + 14) over S(i) (of scores that do not resolve 14: P(i)), and the factor of what was before ----
+            // ---- softmax: S(i) -> 2^14 P(i), P(i) = 2^(S - m), over S(i), and the factor of what was before ----
             float mrun = -INFINITY, lrun = 0.f;
 #pragma unroll 1
             for (int i = at; i < at + p.n; i++) {
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
 #pragma unroll
                 for (int k = 0; k < 64; k++) top[k & 3] = fmaxf(top[k & 3], x[k]);
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                const float mnew = fmaxf(mrun, mx * c1), mm = mnew == -INFINITY ? 0.f : fabsf(mnew) < 1048576.f ? mnew - 14.f : mnew;
+                const float mnew = fmaxf(mrun, mx * c1), mm = mnew == -INFINITY ? 0.f : mnew;
                 const float f = mrun == -INFINITY ? 0.f : kt_ex2(mrun - mnew);
                 float psum[4] = {};
 #pragma unroll
@@ -349,9 +349,11 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                         x[32 * b + k] = kt_ex2(__fmul_rn(x[32 * b + k], c1) - mm);
                         psum[k & 3] += x[32 * b + k];
                     }
-                    // P goes where the scores were: of every 16 keys, hi and lo
+                    // P goes where the scores were: of every 16 keys, hi and lo. (Its 2^14, which keeps small weights' bits, is a factor of its
+                    // own: 14 in the exponent would be lost beside scores past 2^20, and not be the same from step to step.)
 #pragma unroll
-                    for (int k = 0; k < 16; k++) split_pair(x[32 * b + 2 * k], x[32 * b + 2 * k + 1], w[k / 8 * 16 + k % 8], w[k / 8 * 16 + 8 + k % 8]);
+                    for (int k = 0; k < 16; k++)
+                        split_pair(x[32 * b + 2 * k] * 16384.f, x[32 * b + 2 * k + 1] * 16384.f, w[k / 8 * 16 + k % 8], w[k / 8 * 16 + 8 + k % 8]);
                     tmem_st32u(tsp + 32 * b, w);
                 }
                 tmem_wait_st();
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                 lrun = fmaf(lrun, f, (psum[0] + psum[1]) + (psum[2] + psum[3]));
                 mrun = mnew;
             }
-            rowx[0][row] = mrun, rowx[1][row] = lrun * 6.103515625e-5f;  // 2^-14
+            rowx[0][row] = mrun, rowx[1][row] = lrun;
             kt_bar(2, 256);
             at += p.n;
             Cut::next(pl, a, each, sr.n, p.count);
