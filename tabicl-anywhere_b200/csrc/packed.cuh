@@ -50,7 +50,8 @@ __device__ __forceinline__ KaRows ka_rows(const PackedArgs &a, int seq) {
 
 // One row's output and log-sum-exp by one warp, from the keys that it sees and no others. The products of a tile's weights and
 // values take every value of the tile times a weight, 0 for a row that does not see it, and 0 times an infinity or a NaN is
-// NaN; so a row whose output holds a NaN is worked out again here, and is NaN still only if what it sees makes it so.
+// NaN; so a row whose output holds a NaN is worked out again here, and is NaN still only if what it sees makes it so. Products q k
+// near the largest have an exact difference, however large they are; scale and exponential take that.
 template <int DT>
 __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int seq, int i, int hq) {
     using T = typename Elem<DT>::T;
@@ -59,7 +60,8 @@ __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int 
     float x[8], o[8];
 #pragma unroll
     for (int c = 0; c < 8; c++) x[c] = lane + 32 * c < a.width ? Elem<DT>::get(q[lane + 32 * c]) : 0.f, o[c] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    const float scale = fabsf(a.scale);
+    float m = -INFINITY, l = 0.f;  // the largest product (of the scale's sign), the sum of weights
     for (int j = ka_lo(a, s, i); j < hi; j++) {
         const T *k = reinterpret_cast<const T *>(a.k) + (long long)(k0 + j) * a.k_row + head * a.k_head;
         const T *v = reinterpret_cast<const T *>(a.v) + (long long)(k0 + j) * a.v_row + head * a.v_head;
@@ -69,8 +71,8 @@ __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int 
             if (lane + 32 * c < a.width) d = fmaf(x[c], Elem<DT>::get(k[lane + 32 * c]), d);
 #pragma unroll
         for (int b = 16; b; b >>= 1) d += __shfl_xor_sync(0xffffffffu, d, b);
-        d *= a.scale;
-        const float top = fmaxf(m, d), ref = top == -INFINITY ? 0.f : top, f = m == -INFINITY ? 0.f : expf(m - ref), p = expf(d - ref);
+        d = a.scale < 0.f ? -d : d;
+        const float top = fmaxf(m, d), ref = top == -INFINITY ? 0.f : top, f = m == -INFINITY ? 0.f : expf((m - ref) * scale), p = expf((d - ref) * scale);
         l = l * f + p, m = top;
         if (l != l) break;  // whatever follows, every output is NaN (all lanes have the same score)
 #pragma unroll
@@ -81,7 +83,7 @@ __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int 
 #pragma unroll
     for (int c = 0; c < 8; c++)
         if (lane + 32 * c < a.width) out[lane + 32 * c] = Elem<DT>::put(l != 0.f ? o[c] / l : 0.f);
-    if (a.lse && lane == 0) a.lse[(size_t)(s.first + i) * a.q_heads + hq] = (m == -INFINITY ? 0.f : m) + logf(l);
+    if (a.lse && lane == 0) a.lse[(size_t)(s.first + i) * a.q_heads + hq] = (m == -INFINITY ? 0.f : m * scale) + logf(l);
 }
 
 #endif

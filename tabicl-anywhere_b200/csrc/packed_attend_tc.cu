@@ -7,7 +7,9 @@
 // (its products of 64 columns wait for shared memory), but tensor memory then holds one slot a tile, and scores, softmax and
 // output of a step follow one another: 5,700 cycles for 128 keys.
 // A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8, so O is rarely
-// rescaled. The steps of all units are cut evenly over the blocks (kv4_plan.cuh).
+// rescaled. A weight's exponent is one multiply-add, so it has what the reference's rounding left: no matter, since all of a row's
+// weights have it, as long as it is small. Rows whose reference is past 2^24 are worked out again by themselves (the differences
+// of products rounded first, a subtraction a score more, take 3% longer for all others). The steps of all units are cut evenly over the blocks (kv4_plan.cuh).
 // What bounds it: 4096 bf16 tokens, 32 heads on 8 of width 128, causal, take 163 us, 0.84 PFLOP/s: a step of 64 keys 1,700 cycles, of
 // which the products need 1,350 and the exponentials of both tiles 1,024; a unit's output 6,500, a block's start 13,000. f16, 16 heads
 // of width 64, 16 sequences of 1 to 2048 tokens: 146 us, the softmax (1,600 cycles a step) and the ends of units. Registers spilled
@@ -54,12 +56,12 @@ __device__ __forceinline__ void pt_tie(float (&v)[32]) {
     for (int i = 0; i < 32; i += 8)
         asm volatile("" : "+f"(v[i]), "+f"(v[i + 1]), "+f"(v[i + 2]), "+f"(v[i + 3]), "+f"(v[i + 4]), "+f"(v[i + 5]), "+f"(v[i + 6]), "+f"(v[i + 7])::"memory");
 }
-// Two f32 at a time: x * y, x + y; and the largest of three.
-__device__ __forceinline__ float2 pt_mul2(float2 x, float2 y) {
+// Two f32 at a time: x * y + z, x + y; and the largest of three.
+__device__ __forceinline__ float2 pt_fma2(float2 x, float2 y, float2 z) {
     float2 d;
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}\n"
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}\n"
         : "=f"(d.x), "=f"(d.y)
-        : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+        : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
     return d;
 }
 __device__ __forceinline__ float2 pt_add2(float2 x, float2 y) {
@@ -462,8 +464,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                     uint32_t h[16];
 #pragma unroll
                     for (int k = 0; k < 16; k++) {
-                        // (the product rounded as the reference's was: of scores past 2^23 the rest would be more than 1)
-                        const float2 t = pt_add2(pt_mul2(make_float2(x[32 * b + 2 * k], x[32 * b + 2 * k + 1]), sl2), mm2);
+                        const float2 t = pt_fma2(make_float2(x[32 * b + 2 * k], x[32 * b + 2 * k + 1]), sl2, mm2);
                         const float2 w = make_float2(kt_ex2(t.x), kt_ex2(t.y));
                         sum[k & 1] = pt_add2(sum[k & 1], w);
                         h[k] = pt_pair<DT>(w.x, w.y);
@@ -501,8 +502,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                     *cell(row, 4 * b + y) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             };
-            // the warp's rows from there to memory; those with a NaN once more by themselves
+            // the warp's rows from there to memory; those with a NaN or scores past 2^24 once more by themselves
             auto flush = [&](float M, float L) {
+                bad |= M != -INFINITY && !(fabsf(M) < 16777216.f);
                 __syncwarp();
 #pragma unroll 4
                 for (int x = 0; x < 32; x += ROWS) {

@@ -67,3 +67,29 @@ def test_attend_large_scores(gpu, dtype, rows, width, keys, scores, rest):
     assert (np.abs(got - want) <= 2 * weight * size + 1.01 * ULP[dtype] * np.abs(want)).all()
     # one rounding of a number so large, and a small logarithm's
     assert (np.abs(lse - want_lse) <= 2.0**-23 * np.abs(want_lse) + 2.0**-19).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [5, 100], ids=["few", "many"])
+@pytest.mark.parametrize("size", [1e3, 1e4, 1e5, 1e7, 1e12])
+def test_attend_scores_of_every_size(gpu, dtype, rows, size):
+    """Rows of scores up to 10^12, whatever falls between: every weight is that of a score resolved to 2^-22 of its magnitude."""
+    rng = np.random.default_rng(int(size))
+    width, keys = 64, 300
+    up = {"f32": size, "f16": min(size, 1e4), "bf16": size}[dtype]
+    q, k, v = (rounded(rng.normal(0, 1, (n, 1, width)), DT[dtype][1]) for n in (rows, keys, keys))
+    q[:, :, 1:], k[:, :, 1:] = 0, 0  # (one product a score: nothing of a sum is lost)
+    q = rounded(q * up, DT[dtype][1])
+    got, lse = attend(gpu, dtype, q, k, v, 0.25)
+    s = 0.25 * q[:, 0, :1] * k[None, :, 0, 0]
+    # each score off by up to `off` either way: a weight by e^(2 off), an output by what its weights' bounds leave it
+    off = np.abs(s).max(1, keepdims=True) * 2.0**-22 + 2.0**-20
+    low, high = np.exp(s - off - (s + off).max(1, keepdims=True)), np.exp(np.minimum(s + off - (s - off).max(1, keepdims=True), 700))
+    high = np.minimum(high / low.sum(1, keepdims=True).clip(1e-300), 1.0)
+    bound = high @ np.abs(v[:, 0])
+    assert np.isfinite(got).all() and (np.abs(got[:, 0]) <= bound * (1 + 2 * ULP[dtype]) + 2.0**-20).all()
+    want, want_lse = plain.attend(q, k, v, [rows], [keys], 1, 0.25, False, 0)
+    fine = off[:, 0] < 0.02
+    reach = (np.exp(2 * off) - 1 + 2 * (ULP[dtype] if dtype != "f32" else 0) + 2.0**-19) * plain.attend(q, k, np.abs(v), [rows], [keys], 1, 0.25, False, 0)[0][:, 0]
+    assert (np.abs(got[:, 0] - want[:, 0]) <= reach + 1.01 * ULP[dtype] * np.abs(want[:, 0]))[fine].all()
+    assert (np.abs(lse - want_lse) <= off + 2.0**-22 * np.abs(want_lse)).all()
