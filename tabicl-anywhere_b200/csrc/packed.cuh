@@ -48,42 +48,158 @@ __device__ __forceinline__ KaRows ka_rows(const PackedArgs &a, int seq) {
     return r;
 }
 
-// One row's output and log-sum-exp by one warp, from the keys that it sees and no others. The products of a tile's weights and
-// values take every value of the tile times a weight, 0 for a row that does not see it, and 0 times an infinity or a NaN is
-// NaN; so a row whose output holds a NaN is worked out again here, and is NaN still only if what it sees makes it so. Products q k
-// near the largest have an exact difference, however large they are; scale and exponential take that.
-template <int DT>
+// x + y, and what its rounding left into rest (0 beside infinities).
+__device__ __forceinline__ float pa_add(float x, float y, float &rest) {
+    const float t = x + y, z = t - x, e = (x - (t - z)) + (y - z);
+    rest += e == e ? e : 0.f;
+    return t;
+}
+// One row's output and log-sum-exp by one warp, from the keys that it sees and no others, U of them at a time. The products of a
+// tile's weights and values take every value of the tile times a weight, 0 for a row that does not see it, and 0 times an infinity
+// or a NaN is NaN; so a row whose output holds a NaN is worked out again here, and is NaN still only if what it sees makes it so.
+// Products q k near the largest have an exact difference, however large they are; scale and exponential take that. Sums keep what
+// their roundings leave, and weights are divided by as many as there may be keys, so that no sum leaves the values' range. (A key
+// in 0.1 us; one at a time, with the whole chain of a load, five exchanges and two exponentials for each, 0.65.)
+template <int DT, int HD>
 __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int seq, int i, int hq) {
     using T = typename Elem<DT>::T;
-    const int lane = threadIdx.x & 31, each = a.q_heads / a.c.heads, head = hq / each, hi = ka_hi(a, s, i), k0 = a.k_starts[seq];
-    const T *q = reinterpret_cast<const T *>(a.q) + (s.first + i) * a.q_row + hq * a.q_head;
-    float x[8], o[8];
+    constexpr int C = HD / 32, U = C > 4 ? 4 : 8;
+    const int lane = threadIdx.x & 31, each = a.q_heads / a.c.heads, head = hq / each, lo = ka_lo(a, s, i), hi = ka_hi(a, s, i);
+    const long long k0 = a.k_starts[seq];
+    const T *q = reinterpret_cast<const T *>(a.q) + (s.first + i) * a.q_row + hq * a.q_head + lane;
+    const T *k = reinterpret_cast<const T *>(a.k) + k0 * a.k_row + head * a.k_head + lane;
+    const T *v = reinterpret_cast<const T *>(a.v) + k0 * a.v_row + head * a.v_head + lane;
+    float x[C], o[C], o_rest[C];
 #pragma unroll
-    for (int c = 0; c < 8; c++) x[c] = lane + 32 * c < a.width ? Elem<DT>::get(q[lane + 32 * c]) : 0.f, o[c] = 0.f;
-    const float scale = fabsf(a.scale);
-    float m = -INFINITY, l = 0.f;  // the largest product (of the scale's sign), the sum of weights
-    for (int j = ka_lo(a, s, i); j < hi; j++) {
-        const T *k = reinterpret_cast<const T *>(a.k) + (long long)(k0 + j) * a.k_row + head * a.k_head;
-        const T *v = reinterpret_cast<const T *>(a.v) + (long long)(k0 + j) * a.v_row + head * a.v_head;
-        float d = 0.f;
+    for (int c = 0; c < C; c++) x[c] = lane + 32 * c < a.width ? Elem<DT>::get(q[32 * c]) : 0.f, o[c] = o_rest[c] = 0.f;
+    const float scale = fabsf(a.scale), part = __uint_as_float((unsigned)(95 + __clz(max(1, hi - lo))) << 23);  // 2^-(bits of the number of keys)
+    float m = -INFINITY, l = 0.f, l_rest = 0.f;  // the largest product (of the scale's sign), the sum of weights
+    bool dead = false;                           // every output is NaN, whatever follows
+#pragma unroll 1
+    for (int j = lo; j < hi; j += U) {
+        float d[U], top = m;
 #pragma unroll
-        for (int c = 0; c < 8; c++)
-            if (lane + 32 * c < a.width) d = fmaf(x[c], Elem<DT>::get(k[lane + 32 * c]), d);
+        for (int u = 0; u < U; u++) {
+            const T *from = k + min(j + u, hi - 1) * a.k_row;
+            d[u] = 0.f;
 #pragma unroll
-        for (int b = 16; b; b >>= 1) d += __shfl_xor_sync(0xffffffffu, d, b);
-        d = a.scale < 0.f ? -d : d;
-        const float top = fmaxf(m, d), ref = top == -INFINITY ? 0.f : top, f = m == -INFINITY ? 0.f : expf((m - ref) * scale), p = expf((d - ref) * scale);
-        l = l * f + p, m = top;
-        if (l != l) break;  // whatever follows, every output is NaN (all lanes have the same score)
+            for (int c = 0; c < C; c++)
+                if (lane + 32 * c < a.width) d[u] = fmaf(x[c], Elem<DT>::get(from[32 * c]), d[u]);
+        }
 #pragma unroll
-        for (int c = 0; c < 8; c++)
-            if (lane + 32 * c < a.width) o[c] = fmaf(p, Elem<DT>::get(v[lane + 32 * c]), f == 1.f ? o[c] : o[c] * f);
+        for (int b = 16; b; b >>= 1)
+#pragma unroll
+            for (int u = 0; u < U; u++) d[u] += __shfl_xor_sync(0xffffffffu, d[u], b);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            d[u] = j + u >= hi ? -INFINITY : a.scale < 0.f ? -d[u] : d[u];
+            top = fmaxf(top, d[u]);
+        }
+        const float ref = top == -INFINITY ? 0.f : top;
+        if (top != m) {
+            const float f = m == -INFINITY ? 0.f : expf((m - ref) * scale);
+            l *= f, l_rest *= f;
+#pragma unroll
+            for (int c = 0; c < C; c++) o[c] *= f, o_rest[c] *= f;
+            m = top;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            d[u] = j + u < hi ? expf((d[u] - ref) * scale) : 0.f;
+            sum += d[u];
+        }
+        l = pa_add(l, sum, l_rest);
+        if (l != l) break;  // every output is NaN (all lanes have the same scores)
+        if (dead) continue;
+        float y[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) y[c] = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const T *from = v + min(j + u, hi - 1) * a.v_row;
+#pragma unroll
+            for (int c = 0; c < C; c++)
+                if (lane + 32 * c < a.width && j + u < hi) y[c] = fmaf(d[u] * part, Elem<DT>::get(from[32 * c]), y[c]);
+        }
+        dead = true;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            o[c] = pa_add(o[c], y[c], o_rest[c]);
+            dead &= o[c] != o[c] || lane + 32 * c >= a.width;
+        }
+        dead = __all_sync(0xffffffffu, dead);
+        if (dead && !a.lse) break;
     }
-    T *out = reinterpret_cast<T *>(a.out) + (s.first + i) * a.o_row + hq * a.o_head;
+    l += l_rest;
+    T *out = reinterpret_cast<T *>(a.out) + (s.first + i) * a.o_row + hq * a.o_head + lane;
 #pragma unroll
-    for (int c = 0; c < 8; c++)
-        if (lane + 32 * c < a.width) out[lane + 32 * c] = Elem<DT>::put(l != 0.f ? o[c] / l : 0.f);
+    for (int c = 0; c < C; c++)
+        if (lane + 32 * c < a.width) out[32 * c] = Elem<DT>::put(l != l ? l : l != 0.f ? (o[c] + o_rest[c]) / (l * part) : 0.f);
     if (a.lse && lane == 0) a.lse[(size_t)(s.first + i) * a.q_heads + hq] = (m == -INFINITY ? 0.f : m * scale) + logf(l);
+}
+
+// After a block's work, where some of its outputs hold a NaN: the units that it has written once more, the rows with a NaN that
+// may not be one worked out again. It may be wrong only where the unit's values hold an infinity (a weight that was rounded to
+// nothing has a part in that) or a NaN that not all of its rows see, or (f32, whose operands are split) its keys or the row's
+// queries an infinity; rows that see a NaN in keys or values that all see are left as they are. `all`: every such row. From p the
+// block's pieces begin; joined: whether it has written the unit that it shares with the blocks before, after it. By W warps (which
+// have all the registers that the kernel was compiled for), for which no bounded wait waits: a row may take as long as it has keys.
+template <int DT, int HD, int R, int STEP, int EXTRA, int W, class Cut>
+__device__ __noinline__ void pa_mend(const PackedArgs &a, typename Cut::Place p, const int *joined, bool all, int *dirty) {
+    using T = typename Elem<DT>::T;
+    const int tid = threadIdx.x % (32 * W), warp = tid >> 5, lane = tid & 31, each = a.q_heads / a.c.heads;
+    const size_t size = sizeof(T);
+    const bool wide_k = !(((uintptr_t)a.k | (size_t)a.k_row * size | (size_t)a.k_head * size) & 15);
+    const bool wide_v = !(((uintptr_t)a.v | (size_t)a.v_row * size | (size_t)a.v_head * size) & 15);
+    auto infinite = [](float x) { return fabsf(x) == INFINITY; };
+    auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory"); };
+    while (p.pos < p.end) {
+        const KaRows s = ka_rows(a, p.seq);
+        const auto sp = Cut::span(a, s, each, p.rt);
+        const int count = (int)min((long long)(sp.steps - p.skip), p.end - p.pos);
+        if (count == sp.steps || joined[p.skip == 0]) {
+            const int r0 = p.rt * R, rows = min(R, s.n * each - r0), end = min(s.len, sp.base + (sp.steps - EXTRA) * STEP);
+            meet();
+            if (tid == 0) *dirty = all;
+            meet();
+            if (!all) {
+                const int pieces = a.width / 8;
+                const long long k0 = a.k_starts[p.seq] + sp.base;
+                bool found = false;
+                for (int x = tid; x < (end - sp.base) * pieces && !found; x += 32 * W) {
+                    const int j = x / pieces, c = (x - j * pieces) * 8;
+                    float e[8];
+                    load8<DT>(reinterpret_cast<const T *>(a.v) + (k0 + j) * a.v_row + p.head * a.v_head + c, wide_v, e);
+                    const bool hidden = sp.base + j < sp.lo_max || sp.base + j >= sp.hi_min;
+#pragma unroll
+                    for (int y = 0; y < 8; y++) found |= infinite(e[y]) || (hidden && e[y] != e[y]);
+                    if constexpr (DT == DT_F32) {
+                        load8<DT>(reinterpret_cast<const T *>(a.k) + (k0 + j) * a.k_row + p.head * a.k_head + c, wide_k, e);
+#pragma unroll
+                        for (int y = 0; y < 8; y++) found |= infinite(e[y]);
+                    }
+                }
+                if (found) *dirty = 1;
+                meet();
+            }
+            const bool some = *reinterpret_cast<volatile int *>(dirty);
+            for (int r = warp; r < rows; r += W) {
+                const int i = (r0 + r) / each, hq = p.head * each + (r0 + r) % each;
+                const T *out = reinterpret_cast<const T *>(a.out) + (s.first + i) * a.o_row + hq * a.o_head;
+                const T *q = reinterpret_cast<const T *>(a.q) + (s.first + i) * a.q_row + hq * a.q_head;
+                bool nan = false, inf = false;
+                for (int c = lane; c < a.width; c += 32) {
+                    const float y = Elem<DT>::get(out[c]);
+                    nan |= y != y;
+                    if constexpr (DT == DT_F32) inf |= infinite(q[c]);
+                }
+                nan = __any_sync(0xffffffffu, nan), inf = __any_sync(0xffffffffu, inf);
+                if (nan && (some || inf)) pa_repair<DT, HD>(a, s, p.seq, i, hq);
+            }
+        }
+        Cut::next(p, a, each, s.n, count);
+    }
 }
 
 #endif

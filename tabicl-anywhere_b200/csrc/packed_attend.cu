@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
             }
             __syncthreads();
             for (int r = warp; r < rows; r += PA_THREADS / 32)
-                if (s_bad[r]) pa_repair<DT>(a, sr, pl.seq, (r0 + r) / each, pl.head * each + (r0 + r) % each);
+                if (s_bad[r]) pa_repair<DT, HD>(a, sr, pl.seq, (r0 + r) / each, pl.head * each + (r0 + r) % each);
         }
         Cut::next(pl, a, each, sr.n, count);
     }

@@ -116,6 +116,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
     __shared__ uint32_t tslot;
     __shared__ volatile int abort_flag;
     __shared__ int s_unit[4], s_last;
+    // for the rows that are worked out again at the end: where the block's pieces began, the units that it has joined, whether some
+    // of its outputs are NaN, and whether of rows whose scores were too large
+    __shared__ typename Cut::Place s_place;
+    __shared__ int s_joined[2], s_dirty;
+    __shared__ volatile int s_bad, s_large;
     __shared__ long long s_sum[PT_THREADS / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
     const int each = a.q_heads / a.c.heads;
@@ -134,7 +139,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
         for (int i = 0; i < PT_RING; i++) mbar_init(&mPiece[i], 1), mbar_init(&mPieceFree[i], 15);
         mbar_init(&mJoin, 2 * BQ);
         mbar_init_fence();
-        abort_flag = 0;
+        abort_flag = 0, s_joined[0] = s_joined[1] = s_bad = s_large = 0, s_place = pl;
     }
     fence_before_sync();
     __syncthreads();
@@ -486,7 +491,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
             const bool whole = p.whole;
             if (nq) wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u);
             fence_after_sync();
-            float inv = whole ? (l != 0.f ? 1.f / l : 0.f) : 1.f;
+            auto inverse_of = [&](float M, float L) {
+                if (there && M != -INFINITY && !(fabsf(M) < 16777216.f)) {
+                    s_large = 1;
+                    return __uint_as_float(0x7fc00000u);  // (its outputs are NaN until then)
+                }
+                return L != 0.f ? 1.f / L : 0.f;
+            };
+            float inv = whole ? inverse_of(m, l) : 1.f;
             bool bad = false;
             // 32 columns from 32 b on to the row's place in shared memory
             auto put = [&](int b, const float (&o)[32]) {
@@ -502,9 +514,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                     *cell(row, 4 * b + y) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             };
-            // the warp's rows from there to memory; those with a NaN or scores past 2^24 once more by themselves
+            // the warp's rows from there to memory
             auto flush = [&](float M, float L) {
-                bad |= M != -INFINITY && !(fabsf(M) < 16777216.f);
                 __syncwarp();
 #pragma unroll 4
                 for (int x = 0; x < 32; x += ROWS) {
@@ -521,11 +532,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 }
                 const int i_row = there ? token(row) : 0, hq = p.head * each + (there ? r0 + row - i_row * each : 0);
                 if (there && a.lse) a.lse[(size_t)(p.sr.first + i_row) * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M) + log2f(L)) * 0.69314718055994530942f;
-                __syncwarp();
-                for (unsigned again = __ballot_sync(0xffffffffu, bad && there); again; again &= again - 1) {
-                    const int x = __ffs(again) - 1;
-                    pa_repair<DT>(a, p.sr, p.seq, __shfl_sync(0xffffffffu, i_row, x), __shfl_sync(0xffffffffu, hq, x));
-                }
+                if (bad && there) s_bad = 1;
             };
             const size_t prow = q * BQ + row;
             float *mine = part + Cut::slot(blockIdx.x, p.begins) * C::PART;
@@ -556,7 +563,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 if (tid == 0) {
                     const int before = atomicAdd(&arrived[who.x], 1);
                     s_last = before == who.y - 1;
-                    if (s_last) arrived[who.x] = 0;
+                    if (s_last) arrived[who.x] = 0, s_joined[p.begins] = 1;
                     __threadfence();
                 }
                 meet();
@@ -570,7 +577,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                             const float pm = __ldcg(from(b) + PT_R * HD + prow), ps = __ldcg(from(b) + PT_R * (HD + 1) + prow);
                             if (pm != -INFINITY || ps != 0.f) L = fmaf(kt_ex2(pm - ref), ps, L);
                         }
-                    inv = L != 0.f ? 1.f / L : 0.f;
+                    inv = inverse_of(M, L);
 #pragma unroll 1
                     for (int y = 0; y < HD / 32; y++) {
                         float o[32];
@@ -602,6 +609,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
     if (tid == 0 && abort_flag) *reinterpret_cast<volatile int *>(a.err_wait) = 1;
     fence_after_sync();
     if (warp == 8) tmem_dealloc(tmem, 512);
+    if (warp < 8 && s_bad && !abort_flag) pa_mend<DT, HD, PT_R, PT_BK, EXTRA, 8, Cut>(a, s_place, s_joined, s_large, &s_dirty);
 }
 
 template <int HD>

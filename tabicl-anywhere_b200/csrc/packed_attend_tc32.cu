@@ -121,6 +121,11 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
     __shared__ uint32_t tslot;
     __shared__ volatile int abort_flag;
     __shared__ int s_unit[4], s_last;
+    // for the rows that are worked out again at the end: where the block's pieces began, the units that it has joined, whether some
+    // of its outputs are NaN
+    __shared__ typename Cut::Place s_place;
+    __shared__ int s_joined[2], s_dirty;
+    __shared__ volatile int s_bad;
     __shared__ long long s_sum[PS_THREADS / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2, row = tid & (BQ - 1);
     const int each = a.q_heads / a.c.heads;
@@ -139,7 +144,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
         mbar_init(&mPV, 1), mbar_init(&mOfree, BQ);
         for (int i = 0; i < 3; i++) mbar_init(&mDone[i], 1);
         mbar_init_fence();
-        abort_flag = 0;
+        abort_flag = 0, s_joined[0] = s_joined[1] = s_bad = 0, s_place = pl;
     }
     fence_before_sync();
     __syncthreads();
@@ -427,7 +432,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                 kt_bar(3, 128);
                 if (row == 0) {
                     s_last = atomicAdd(arrived + who.x, 1) == who.y - 1;
-                    if (s_last) arrived[who.x] = 0;  // ready for the next call
+                    if (s_last) arrived[who.x] = 0, s_joined[pl.skip == 0] = 1;  // ready for the next call
                 }
                 kt_bar(3, 128);
                 write = write && s_last;
@@ -467,11 +472,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                 }
                 if (a.lse) a.lse[(size_t)(sr.first + ri) * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M) + log2f(L)) * 0.69314718055994530942f;
             }
-            __syncwarp();
-            for (unsigned again = __ballot_sync(0xffffffffu, bad); again; again &= again - 1) {
-                const int x = __ffs(again) - 1;
-                pa_repair<DT_F32>(a, sr, pl.seq, __shfl_sync(0xffffffffu, ri, x), __shfl_sync(0xffffffffu, hq, x));
-            }
+            if (bad) s_bad = 1;
             at += p.n;
             Cut::next(pl, a, each, sr.n, p.count);
         }
@@ -481,6 +482,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
     if (tid == 0 && abort_flag) *reinterpret_cast<volatile int *>(a.err_wait) = 1;
     fence_after_sync();
     if (warp == 8) tmem_dealloc(tmem, 512);
+    if (wg == 1 && s_bad && !abort_flag) pa_mend<DT_F32, HD, PS_BQ, PS_BK, PS_EXTRA, 4, Cut>(a, s_place, s_joined, false, &s_dirty);
 }
 
 // Working memory: counters, parts, the tiles' powers of two, the tiles.

@@ -93,3 +93,77 @@ def test_attend_scores_of_every_size(gpu, dtype, rows, size):
     reach = (np.exp(2 * off) - 1 + 2 * (ULP[dtype] if dtype != "f32" else 0) + 2.0**-19) * plain.attend(q, k, np.abs(v), [rows], [keys], 1, 0.25, False, 0)[0][:, 0]
     assert (np.abs(got[:, 0] - want[:, 0]) <= reach + 1.01 * ULP[dtype] * np.abs(want[:, 0]))[fine].all()
     assert (np.abs(lse - want_lse) <= off + 2.0**-22 * np.abs(want_lse)).all()
+
+
+# ---- what is worked out again ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,keys,width", [(3, 5_000, 64), (130, 5_000, 64), (130, 5_000, 128), (300, 700, 128), (130, 700, 256)])
+@pytest.mark.parametrize("what", ["value", "values", "infinite", "hidden", "key", "hidden key", "queries"])
+def test_attend_odd_numbers_over_many_keys(gpu, dtype, rows, keys, width, what):
+    """A NaN or an infinity in one value of a long sequence, where all rows see it or some: in the columns that it reaches, and no others."""
+    tt = DT[dtype][1]
+    gen = torch.Generator(device="cuda").manual_seed(keys)
+    q, k, v = (torch.randn(n, h, width, generator=gen, device="cuda").to(tt) for n, h in ((rows, 2), (keys, 1), (keys, 1)))
+    last = keys - rows // 2  # a key that the second half of the rows sees (causal)
+    if what == "value":
+        v[40, 0, 5] = float("nan")
+    elif what == "values":
+        v[40, 0, :] = float("nan")
+    elif what == "infinite":
+        v[40, 0, 5], v[41, 0, 6] = float("inf"), -float("inf")
+    elif what == "hidden":
+        v[last, 0, 3], v[last, 0, 9] = float("nan"), float("inf")
+    elif what == "key":
+        k[40, 0, 3] = float("nan")
+    elif what == "hidden key":
+        k[last, 0, 3] = float("nan")
+    else:
+        q[1, 1, 7], q[2, 0, 3] = float("nan"), float("inf")
+    scale, causal = width**-0.5, "hidden" in what
+    got, lse = attend(gpu, dtype, q, k, v, scale, causal)
+    seen = torch.ones(rows, keys, dtype=torch.bool, device="cuda")
+    if causal:
+        seen = torch.arange(keys, device="cuda")[None] <= torch.arange(rows, device="cuda")[:, None] + keys - rows
+    s = torch.einsum("nhw,mw->hnm", q.double(), k[:, 0].double()) * scale
+    s = torch.where(seen, s, torch.full_like(s, -float("inf")))
+    p = torch.softmax(s, -1)
+    # a hidden value has no part, whatever it is; a seen one has its weight's, however small
+    fine = torch.where(torch.isfinite(v[:, 0]), v[:, 0].double(), torch.zeros((), device="cuda").double())
+    want = torch.einsum("hnm,mw->nhw", p, fine)
+    for j in (40, 41, last):
+        odd = torch.where(torch.isfinite(v[j, 0]), torch.zeros((), device="cuda"), v[j, 0].float()).double()
+        want += torch.where(seen[:, j, None, None], odd, torch.zeros((), device="cuda").double()) + torch.zeros_like(want)
+    top = s.max(-1, keepdim=True).values
+    want, want_lse = want.cpu().numpy(), (top + torch.exp(s - top).sum(-1, keepdim=True).log())[..., 0].t().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(np.isnan(lse), np.isnan(want_lse))
+    some = np.isfinite(want)
+    assert np.array_equal(got[~some & ~np.isnan(want)], want[~some & ~np.isnan(want)])
+    # as in a long attention without them: beside the root of the sum of squares a weight's error is a rounding
+    if some.any():
+        off = np.linalg.norm(got[some] - want[some]) / np.linalg.norm(want[some])
+        assert off <= {"f32": 2e-6, "f16": 2.0 * 2**-11, "bf16": 2.0 * 2**-8}[dtype], off
+    assert (np.abs(lse - want_lse)[np.isfinite(want_lse)] <= 2.0**-18).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attend_works_out_rows_over_very_many_keys(gpu, dtype):
+    """Rows that see a NaN, and rows that must not, over more keys than a wait for them would have patience for."""
+    tt = DT[dtype][1]
+    rows, keys, width = 100, 150_000, 64
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(n, 1, width, generator=gen, device="cuda").to(tt) for n in (rows, keys, keys))
+    v[7, 0, 5], v[keys - 20, 0, 3] = float("nan"), float("nan")  # seen by all; by the last 20 rows
+    got, lse = attend(gpu, dtype, q, k, v, 0.125, True)
+    seen = torch.arange(keys, device="cuda")[None] <= torch.arange(rows, device="cuda")[:, None] + keys - rows
+    s = torch.einsum("nw,mw->nm", q[:, 0].double(), k[:, 0].double()) * 0.125
+    s = torch.where(seen, s, torch.full_like(s, -float("inf")))
+    v[7, 0, 5], v[keys - 20, 0, 3] = 0, 0
+    want = (torch.softmax(s, -1) @ v[:, 0].double()).cpu().numpy()
+    want[:, 5] = np.nan
+    want[-20:, 3] = np.nan
+    assert np.array_equal(np.isnan(got[:, 0]), np.isnan(want))
+    some = ~np.isnan(want)
+    off = np.linalg.norm((got[:, 0] - want)[some]) / np.linalg.norm(want[some])
+    assert off <= {"f32": 2e-6, "f16": 2.0 * 2**-11}[dtype], off
+    assert np.abs(lse[:, 0] - torch.logsumexp(s, -1).cpu().numpy()).max() <= 2.0**-18
