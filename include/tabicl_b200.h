@@ -155,7 +155,8 @@ TCU_API int tcu_represent_device(tcu_model *m, float *tok, int rows, float *rep,
 TCU_API int tcu_sync(tcu_ctx *ctx, void *stream);
 /* Test hook (no counterpart in the reference): the next one-kernel stage launch on this context starts as if a
  * wait had given up, so that the give-up path (every CTA leaving at its next barrier after its copies land) and
- * its report can be exercised without making any wait run out. */
+ * its report can be exercised without making any wait run out. A call of tcu_fp4_linear_device or
+ * tcu_packed_attend_device that comes before it takes it instead (its tensor-core kernels: every other CTA). */
 TCU_API int tcu_debug_abort_next(tcu_ctx *ctx);
 
 /* ---- a whole member: its problems and the class tree (src/predict.rs:638-699) ----------------------------------- */

@@ -273,7 +273,7 @@ class Gpu:
         return self.check(lib().tcu_sync(self._h, stream))
 
     def debug_abort_next(self):
-        """Test hook: the next one-kernel stage launch starts as if a wait had given up."""
+        """Test hook: the next one-kernel stage launch, or prompt operator before it, starts as if a wait had given up."""
         return self.check(lib().tcu_debug_abort_next(self._h))
 
 

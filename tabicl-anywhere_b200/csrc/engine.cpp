@@ -90,7 +90,7 @@ struct tcu_ctx {
     // store 1 into their slot; the host reads them without synchronising): ERR_SLOTS ints, see err_slot_names.
     int *err_host = nullptr;
     int *err_mapped = nullptr;     // the same slots' device address
-    bool abort_next = false;       // test hook: the next one-kernel stage launch starts aborted
+    bool abort_next = false;       // test hook: the next one-kernel stage or prompt operator's launch starts aborted
     unsigned *dev_scan = nullptr;  // scratch of the per-layer magnitude scan
     // uploads from bundles: two pinned staging buffers and a stream of their own (a piece is read from the source
     // while the one before is copied), used by one upload at a time and not under `mu`
@@ -3533,6 +3533,7 @@ int tcu_fp4_linear_device(tcu_ctx *ctx, const tcu_fp4 *w, const tcu_fp4 *x, int 
         if (need && (!work || work_bytes < need)) fail(TCU_ERR_ARG, "fp4_linear: needs " + std::to_string(need) + " bytes of working memory");
         check_aligned("fp4_linear", "working memory", work, 16);
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        a.give_up = ctx->abort_next, ctx->abort_next = false;
         Launch{ctx, s}(launch_fp4_linear(dtype, a, ctx->sms, (void *)tensor_map_encoder(), work, s, &ctx->launches), "fp4_linear");
         return TCU_OK;
     });
@@ -3593,6 +3594,7 @@ int tcu_packed_attend_device(tcu_ctx *ctx, const tcu_packed *p, int dtype, int q
         if (need && (!work || work_bytes < need)) fail(TCU_ERR_ARG, "packed_attend: needs " + std::to_string(need) + " bytes of working memory");
         check_aligned("packed_attend", "working memory", work, 16);
         cudaStream_t s = stream ? (cudaStream_t)stream : ctx->stream;
+        a.give_up = ctx->abort_next, ctx->abort_next = false;
         Launch{ctx, s}(launch_packed_attend(dtype, a, ctx->sms, (void *)tensor_map_encoder(), work, s, &ctx->launches), "packed_attend");
         return TCU_OK;
     });

@@ -33,6 +33,7 @@ struct Fp4LinearArgs {
     void *y = nullptr;
     long long ldy = 0, ldr = 0;
     int *err_wait = nullptr;  // report slot: set to 1 when a kernel gave up waiting
+    int give_up = 0;          // test hook: every other block begins as if a wait had given up
 };
 
 cudaError_t launch_fp4_pack(int dtype, const Fp4Args &a, cudaStream_t s, uint64_t *launches);

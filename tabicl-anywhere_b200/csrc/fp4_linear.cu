@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
         for (int i = 0; i < 2; i++) mbar_init(&m_acc[i], 1), mbar_init(&m_free[i], 256);
         mbar_init(&m_done, 1);
         mbar_init_fence();
-        abort_flag = 0;
+        abort_flag = a.give_up & blockIdx.x & 1;
     }
     fence_before_sync();
     __syncthreads();
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
     const long long end = ka_div(all * (blockIdx.x + 1), gridDim.x) * per;
 
     if (warp == 0) {
-        int at = 0, slot = 0;
+        int asked = 0, slot = 0;  // (asked: steps whose copies have been asked for; none after a wait has given up)
         uint32_t turn = 0;  // how often the slots have been filled (its lowest bit: a division by a number of slots known at run time costs more)
         while (pos < end) {
             const int t = (int)ka_div(pos, p.steps), s0 = (int)(pos - (long long)t * p.steps), s1 = (int)min((long long)p.steps, s0 + end - pos);
@@ -146,8 +146,10 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
             const uint8_t *wa = a.w_scales + (size_t)place.y * p.quads * 512;
             const int row_block = place.x * p.nt / 128, blocks = min((p.nt + 127) / 128, (a.rows + 127) / 128 - row_block);
             const uint8_t *xa = a.x_scales + (size_t)row_block * p.quads * 512;
-            for (int s = s0; s < s1; s++, at++) {
+            for (int s = s0; s < s1; s++) {
                 if (turn) wait_warp(&m_empty[slot], (turn - 1) & 1u);
+                if (__any_sync(0xffffffffu, abort_flag != 0)) break;
+                asked++;
                 const int quads = min(QS, p.quads - s * QS);
                 if (elect_one()) {
                     const uint32_t to = base + slot * p.stage_bytes;
@@ -164,7 +166,7 @@ __global__ void __launch_bounds__(FL_THREADS, 1) k_fp4_linear(Fp4LinearArgs a, F
             pos += s1 - s0;
         }
         // what was asked for lands before the block lets go of shared memory
-        for (int i = max(0, at - p.stages); i < at; i++) mbar_wait(&m_full[i % p.stages], (uint32_t)(i / p.stages) & 1u, KT_WAIT);
+        for (int i = max(0, asked - p.stages); i < asked; i++) mbar_wait(&m_full[i % p.stages], (uint32_t)(i / p.stages) & 1u, KT_WAIT);
     } else if (warp == 1) {
         int c = 0, slot = 0;
         uint32_t turn = 0;

@@ -24,6 +24,7 @@ struct PackedArgs {
     float *lse = nullptr;     // [rows][q_heads], or null
     int *err = nullptr;       // report slot: set to 1 on starts outside their range
     int *err_wait = nullptr;  // report slot: set to 1 when a kernel gave up waiting
+    int give_up = 0;          // test hook: every other block of a kernel with bounded waits begins as if one had given up
 };
 
 // Working memory of a call (the KA_BLOCKS counters, and parts after them), whichever kernel takes it, and the call. `encode` is

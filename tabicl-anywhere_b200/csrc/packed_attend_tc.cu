@@ -90,8 +90,9 @@ __device__ __forceinline__ uint32_t pt_pair(float x, float y) {
 // Warps 0-3, 4-7: softmax of the first and second tile, a thread a query row; warps 8, 9: the tiles' products S; warps 10, 11:
 // their products P V (a warp for both tiles' was what a step took longest in: a wait and its bookkeeping cost some hundred
 // cycles); warp 12: the copies; warp 13 clears the values behind a sequence's end; warp 14 walks the block's pieces of units and
-// hands them to the others, so that these have registers for their work alone; warp 15 brings the next piece's queries. Every wait is bounded, and one that gives up raises the block's abort flag, after which every wait returns at once and
-// the roles run to the end without results.
+// hands them to the others, so that these have registers for their work alone; warp 15 brings the next piece's queries. Every
+// wait is bounded, and one that gives up raises the block's abort flag, after which every wait returns at once, the roles leave
+// with the piece that they have, nothing more is asked for, and the block counts itself among those that share its units.
 template <int HD, int DT>
 __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a, const __grid_constant__ CUtensorMap map_k,
                                                                     const __grid_constant__ CUtensorMap map_v,
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
     // for the rows that are worked out again at the end: where the block's pieces began, the units that it has joined, whether some
     // of its outputs are NaN, and whether of rows whose scores were too large
     __shared__ typename Cut::Place s_place;
-    __shared__ int s_joined[2], s_dirty;
+    __shared__ int s_joined[2], s_counted[2], s_dirty;  // (s_counted: whether the block has counted itself among those that share them)
     __shared__ volatile int s_bad, s_large;
     __shared__ long long s_sum[PT_THREADS / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
         for (int i = 0; i < PT_RING; i++) mbar_init(&mPiece[i], 1), mbar_init(&mPieceFree[i], 15);
         mbar_init(&mJoin, 2 * BQ);
         mbar_init_fence();
-        abort_flag = 0, s_joined[0] = s_joined[1] = s_bad = s_large = 0, s_place = pl;
+        abort_flag = a.give_up & blockIdx.x & 1, s_counted[0] = s_counted[1] = s_joined[0] = s_joined[1] = s_bad = s_large = 0, s_place = pl;
     }
     fence_before_sync();
     __syncthreads();
@@ -150,6 +151,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
         if (!mbar_test_wait(m, parity) && !abort_flag && !mbar_wait(m, parity, KT_WAIT)) abort_flag = 1;
         __syncwarp();
     };
+    auto stopped = [&] { return __any_sync(0xffffffffu, abort_flag != 0); };
     // the next piece, from which every warp of a role takes what it needs; `taken` once it has
     int turns = 0;
     auto take = [&]() -> const Piece & {
@@ -194,6 +196,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 Cut::next(pl, a, each, sr.n, count);
             }
         } else if (warp == 12) {
+            int k_asked = 0, v_asked = 0;  // steps whose copies have been asked for
             for (;;) {
                 const Piece &p = take();
                 const int n = p.n, z0 = p.k0 + p.j0, head = p.head;
@@ -202,6 +205,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 for (int i = 0; i < n; i++) {
                     const int slot = (at + i) % NS, turn = (at + i) / NS, z = z0 + i * BK;
                     if (turn) wait_warp(&mKfree[slot], (uint32_t)(turn - 1) & 1u);
+                    if (stopped()) break;
+                    k_asked++;
                     if (elect_one()) {
                         pt_expect(&mK[slot], TILE);
 #pragma unroll
@@ -209,6 +214,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                     }
                     __syncwarp();
                     if (turn) wait_warp(&mVfree[slot], (uint32_t)(turn - 1) & 1u);
+                    if (stopped()) break;
+                    v_asked++;
                     if (elect_one()) {
                         pt_expect(&mV[slot], TILE);
 #pragma unroll
@@ -219,10 +226,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 at += n;
             }
             // what was asked for lands before the block lets go of shared memory
-            for (int i = max(0, at - NS); i < at; i++) {
-                mbar_wait(&mK[i % NS], (uint32_t)(i / NS) & 1u, KT_WAIT);
-                mbar_wait(&mV[i % NS], (uint32_t)(i / NS) & 1u, KT_WAIT);
-            }
+            for (int i = max(0, k_asked - NS); i < k_asked; i++) mbar_wait(&mK[i % NS], (uint32_t)(i / NS) & 1u, KT_WAIT);
+            for (int i = max(0, v_asked - NS); i < v_asked; i++) mbar_wait(&mV[i % NS], (uint32_t)(i / NS) & 1u, KT_WAIT);
         } else if (warp == 15) {
             // the rows' queries: by TMA (by_map), or in 16-byte pieces, asynchronously where they are aligned and not to change sign
             constexpr int LANES = HD / 8, ROWS = 32 / LANES;  // lanes a row, rows at a time
@@ -240,6 +245,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 if (n < 0 || abort_flag) break;
                 const int b = units & 1;
                 if (units >= 2) wait_warp(&mQfree[b], (units / 2 - 1) & 1u);
+                if (stopped()) break;
                 units++;
                 if (by_map) {
                     if (lane == 0) {
@@ -561,6 +567,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 __threadfence();
                 meet();
                 if (tid == 0) {
+                    s_counted[p.begins] = 1;
                     const int before = atomicAdd(&arrived[who.x], 1);
                     s_last = before == who.y - 1;
                     if (s_last) arrived[who.x] = 0, s_joined[p.begins] = 1;
@@ -606,7 +613,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
     }
     fence_before_sync();
     __syncthreads();
-    if (tid == 0 && abort_flag) *reinterpret_cast<volatile int *>(a.err_wait) = 1;
+    if (tid == 0 && abort_flag) {
+        *reinterpret_cast<volatile int *>(a.err_wait) = 1;
+        // the counters are to be zero when all blocks are done, whatever became of this one's parts
+        for (auto p = s_place; p.pos < p.end;) {
+            const KaRows s = ka_rows(a, p.seq);
+            const int steps = Cut::span(a, s, each, p.rt).steps, count = (int)min((long long)(steps - p.skip), p.end - p.pos);
+            if (count != steps && !s_counted[p.skip == 0]) {
+                const int2 who = Cut::sharers(p, p.pos - p.skip, steps);
+                if (atomicAdd(&arrived[who.x], 1) == who.y - 1) arrived[who.x] = 0;
+            }
+            Cut::next(p, a, each, s.n, count);
+        }
+    }
     fence_after_sync();
     if (warp == 8) tmem_dealloc(tmem, 512);
     if (warp < 8 && s_bad && !abort_flag) pa_mend<DT, HD, PT_R, PT_BK, EXTRA, 8, Cut>(a, s_place, s_joined, s_large, &s_dirty);

@@ -107,8 +107,8 @@ __global__ void __launch_bounds__(256) k_packed_split(PackedArgs a, uint8_t *til
 
 // Warps 0-3: softmax, a thread a query row; warps 4-7: the fold of each step's P V, a thread a row; warps 8, 9 issue the S products
 // of even and odd steps, warp 10 the P V products; warp 11: the copies. They hand over through mbarriers; every wait is bounded,
-// and one that gives up raises the block's abort flag, after which every wait returns at once and the roles, which walk the same
-// pieces of units and meet at the same barriers, run to the end without results.
+// and one that gives up raises the block's abort flag, after which every wait returns at once, nothing more is asked for, and the roles,
+// which walk the same pieces of units and meet at the same barriers, run to the end without results.
 template <int HD>
 __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs a, const uint8_t *tiles, const int2 *units, float *part, int *arrived) {
     using C = PsShape<HD>;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
         mbar_init(&mPV, 1), mbar_init(&mOfree, BQ);
         for (int i = 0; i < 3; i++) mbar_init(&mDone[i], 1);
         mbar_init_fence();
-        abort_flag = 0, s_joined[0] = s_joined[1] = s_bad = 0, s_place = pl;
+        abort_flag = a.give_up & blockIdx.x & 1, s_joined[0] = s_joined[1] = s_bad = 0, s_place = pl;
     }
     fence_before_sync();
     __syncthreads();
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
     if (wg == 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
         if (warp == 11) {
+            int asked = 0;  // steps whose copies have been asked for
             while (pl.pos < pl.end) {
                 const KaRows sr = ka_rows(a, pl.seq);
                 const auto sp = Cut::span(a, sr, each, pl.rt);
@@ -220,6 +221,8 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                     const uint32_t ph = (uint32_t)(at / NS) & 1u;
                     const int2 e = __ldg(units + first + i);
                     if (at >= NS) wait_warp(&mKfree[slot], ph ^ 1u), wait_warp(&mVfree[slot], ph ^ 1u);
+                    if (__any_sync(0xffffffffu, abort_flag != 0)) continue;
+                    asked++;
                     if (lane == 0) {
                         // (read by the softmax and the fold after they have seen products of this step; four steps on they are done with it)
                         *reinterpret_cast<volatile int *>(&teK[at & 7]) = e.x, *reinterpret_cast<volatile int *>(&teV[at & 7]) = e.y;
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                 Cut::next(pl, a, each, sr.n, p.count);
             }
             // what was asked for lands before the block lets go of shared memory
-            for (int i = max(0, at - NS); i < at; i++) {
+            for (int i = max(0, asked - NS); i < asked; i++) {
                 mbar_wait(&mK[i % NS], (uint32_t)(i / NS) & 1u, KT_WAIT);
                 mbar_wait(&mV[i % NS], (uint32_t)(i / NS) & 1u, KT_WAIT);
             }

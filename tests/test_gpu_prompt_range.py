@@ -167,3 +167,59 @@ def test_attend_works_out_rows_over_very_many_keys(gpu, dtype):
     off = np.linalg.norm((got[:, 0] - want)[some]) / np.linalg.norm(want[some])
     assert off <= {"f32": 2e-6, "f16": 2.0 * 2**-11}[dtype], off
     assert np.abs(lse[:, 0] - torch.logsumexp(s, -1).cpu().numpy()).max() <= 2.0**-18
+
+
+# ---- waits that give up ---------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_lens,k_lens,heads", [([100], [9_000], 1), ([300, 1, 900], [300, 70, 900], 4), ([2000], [2000], 2), ([150] * 20, [150] * 20, 8)])
+def test_attend_that_gives_up_leaves_its_counters(gpu, dtype, q_lens, k_lens, heads):
+    """Every other block gives up: the next call reports it, and finds the working memory as any call leaves it."""
+    code, tt = DT[dtype]
+    w, rows, keys = 64, sum(q_lens), sum(k_lens)
+    q, k, v = (torch.randn(n, heads, w, device="cuda").to(tt) for n in (rows, keys, keys))
+    qs, ks = (dev(np.concatenate([[0], np.cumsum(x)]).astype(np.int32)) for x in (q_lens, k_lens))
+    p = tcu.Packed(gpu, len(q_lens), rows, keys, max(q_lens), max(k_lens), qs.data_ptr(), ks.data_ptr())
+    work = torch.zeros(p.attend_workspace(code, heads, heads, w), dtype=torch.uint8, device="cuda")
+
+    def go():
+        out = torch.full_like(q, 9.0)
+        p.attend(code, heads, heads, w, q.data_ptr(), heads * w, w, k.data_ptr(), heads * w, w, v.data_ptr(), heads * w, w, out.data_ptr(),
+                 heads * w, w, 0.125, causal=True, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+        torch.cuda.synchronize()
+        return out
+    want = go()
+    gpu.sync()
+    for _ in range(2):
+        gpu.debug_abort_next()
+        go()
+        assert not work[:8192].any()
+        with pytest.raises(tcu.TcuError, match="gave up") as e:
+            gpu.sync()
+        assert e.value.code == -3
+        assert torch.equal(go(), want) and not work[:8192].any()
+        gpu.sync()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,n,k", [(8, 300, 33_000), (33, 64, 20_000), (600, 700, 900), (2, 40_000, 256)])
+def test_linear_that_gives_up_leaves_its_counters(gpu, dtype, rows, n, k):
+    code, tt = DT[dtype]
+    rng = np.random.default_rng(k)
+    x, w = (base.random_matrix(rng, gpu, r, k, plain.NV)[0] for r in (rows, n))
+    work = torch.zeros(w.m.linear_workspace(x.m, code), dtype=torch.uint8, device="cuda")
+
+    def go():
+        y = torch.full((rows, n), 9.0, dtype=tt, device="cuda")
+        w.m.linear(x.m, code, y.data_ptr(), n, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+        torch.cuda.synchronize()
+        return y
+    want = go()
+    gpu.sync()
+    gpu.debug_abort_next()
+    go()
+    assert not work[:8192].any()
+    with pytest.raises(tcu.TcuError, match="gave up"):
+        gpu.sync()
+    assert torch.equal(go(), want)
+    gpu.sync()
