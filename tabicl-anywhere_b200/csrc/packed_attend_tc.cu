@@ -606,6 +606,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                     flush(M, L);
                 }
             }
+            fence_async_smem();  // (outputs were stored where copies will write)
             mbar_arrive(&mQfree[units & 1]);
             units++;
             taken();
