@@ -5,7 +5,8 @@
 // asynchronous copies. With 16 rows the four warps share a step's keys, with 64 its rows. One pass: running maxima and sums, the
 // output in registers, the matrix products by warp (16-bit operands as they are; f32 as two tf32, of 11 bits each, in three
 // products). A call of few rows streams its keys and values, so it is bound by memory; the steps of all sequences are cut evenly
-// over the blocks (kv4_plan.cuh), whose parts the last of them joins in order. 32 requests of 0 to 16,383 bf16 tokens, 32 heads on 8 of
+// over the blocks (kv4_plan.cuh), whose parts the last of them joins in order. f16 weights are multiplied by 2^15, so that they fill
+// f16's range. 32 requests of 0 to 16,383 bf16 tokens, 32 heads on 8 of
 // width 128: 188 us for 1.05 GB, 5.6 TB/s (343 us with a division for every 16 bytes copied).
 #include <algorithm>
 #include <type_traits>
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, wr = warp % WR, kw = warp / WR;
     const int each = a.q_heads / a.c.heads;
     const float sl = a.scale * 1.44269504088896340736f;
+    constexpr float UP = DT == DT_F16 ? 0x1p15f : 1.f, DOWN = 1.f / UP;  // what 16-bit weights are multiplied by, their outputs at the end
     auto pl = Cut::template place<PA_THREADS>(a, each, PA_STEPS, s_sum, s_unit);
     while (pl.pos < pl.end) {
         const KaRows sr = ka_rows(a, pl.seq);
@@ -307,8 +309,8 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
                 const uint32_t va = pa_smem(vs + (lane & 15) * PITCH + (lane >> 4) * 16);
 #pragma unroll
                 for (int x = 0; x < NT; x += 2) {
-                    const uint32_t p[4] = {pa_pair<DT>(s[x][0], s[x][1]), pa_pair<DT>(s[x][2], s[x][3]), pa_pair<DT>(s[x + 1][0], s[x + 1][1]),
-                                           pa_pair<DT>(s[x + 1][2], s[x + 1][3])};
+                    const uint32_t p[4] = {pa_pair<DT>(s[x][0] * UP, s[x][1] * UP), pa_pair<DT>(s[x][2] * UP, s[x][3] * UP),
+                                           pa_pair<DT>(s[x + 1][0] * UP, s[x + 1][1] * UP), pa_pair<DT>(s[x + 1][2] * UP, s[x + 1][3] * UP)};
 #pragma unroll
                     for (int c = 0; c < NO; c += 2) {
                         uint32_t b[4];
@@ -394,7 +396,7 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
                         return From{b + r * HD + c, b + R * HD + r, b + R * HD + R + r};
                     }, v, M, L);
                 const float inv = L != 0.f ? 1.f / L : 0.f;
-                const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+                const float y[4] = {v.x * inv * DOWN, v.y * inv * DOWN, v.z * inv * DOWN, v.w * inv * DOWN};
                 T *out = reinterpret_cast<T *>(a.out) + row * a.o_row + hq * a.o_head + c;
 #pragma unroll
                 for (int x = 0; x < 4; x++) {  // (a width is a multiple of 8)

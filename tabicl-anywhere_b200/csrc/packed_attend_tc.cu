@@ -6,9 +6,11 @@
 // brings them (values as an operand whose coordinates are contiguous). A step of 128 keys would keep the matrix unit busier
 // (its products of 64 columns wait for shared memory), but tensor memory then holds one slot a tile, and scores, softmax and
 // output of a step follow one another: 5,700 cycles for 128 keys.
-// A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8, so O is rarely
-// rescaled. A weight's exponent is one multiply-add, so it has what the reference's rounding left: no matter, since all of a row's
-// weights have it, as long as it is small. Rows whose reference is past 2^24 are worked out again by themselves (the differences
+// A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8 (f16: 2^4), so O is
+// rarely rescaled. f16 weights are 2^11 times as large as that, so that they fill f16's range: one is held to 11 bits, and to 2^-36
+// of the largest, below which values of 60,000 would show the loss (16 sequences of f16 tokens: 152 us; with a lag of 2^2 and 2^13
+// 158, of 2^8 and 2^7 151.5, without 150). A weight's exponent is one multiply-add, so it has what the reference's rounding left: no matter, since all of a row's
+// weights have it, as long as it is small. Rows whose reference is past 2^22 are worked out again by themselves (the differences
 // of products rounded first, a subtraction a score more, take 3% longer for all others). The steps of all units are cut evenly over the blocks (kv4_plan.cuh).
 // What bounds it: 4096 bf16 tokens, 32 heads on 8 of width 128, causal, take 163 us, 0.84 PFLOP/s: a step of 64 keys 1,700 cycles, of
 // which the products need 1,350 and the exponentials of both tiles 1,024; a unit's output 6,500, a block's start 13,000. f16, 16 heads
@@ -100,6 +102,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
     using C = PtShape<HD>;
     using T = typename Elem<DT>::T;
     constexpr int EXTRA = C::EXTRA;
+    // a weight's exponent beside the reference at most when that is moved, and how far it may grow before it is moved again
+    constexpr float SHIFT = DT == DT_F16 ? 11.f : 0.f, LAG = DT == DT_F16 ? 4.f : 8.f;
     using Cut = KaCut<PT_R, 1, PT_BK, EXTRA>;
     constexpr int BQ = PT_BQ, BK = PT_BK, NS = C::NS, TILE = C::TILE, QTILE = C::QTILE;
     constexpr uint32_t TS = 0, TO = 256;  // tensor memory: [tile][2 slots] of S / P, then [tile] of O
@@ -381,6 +385,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
         const int q = wg, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, tO = tmem + lanes + TO + q * HD;
         const float sl = fminf(fmaxf(fabsf(a.scale) * 1.44269504088896340736f, FLT_MIN), FLT_MAX);  // (positive, so that -infinity stays itself)
+        constexpr float UNSHIFT = DT == DT_F16 ? 0x1p-11f : 1.f;
         const bool wide_o = (((uintptr_t)a.out | (size_t)a.o_row * 2 | (size_t)a.o_head * 2) & 15) == 0;
         uint32_t units = 0, meetings = 0;
         // both tiles' threads (a barrier whose wait is bounded too)
@@ -446,8 +451,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int k = 0; k < 32; k++) top[k & 3] = pt_max3(top[k & 3], x[2 * k], x[2 * k + 1]);
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl;
-                if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl - SHIFT;
+                if (__any_sync(0xffffffffu, mx > m + LAG)) {
                     const float mnew = fmaxf(m, mx), f = m == -INFINITY ? 0.f : kt_ex2(m - mnew);
                     if (i > 0) {  // O, once the product before has been added to it
                         wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u);
@@ -498,7 +503,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
             if (nq) wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u);
             fence_after_sync();
             auto inverse_of = [&](float M, float L) {
-                if (there && M != -INFINITY && !(fabsf(M) < 16777216.f)) {
+                if (there && M != -INFINITY && !(fabsf(M) < 4194304.f)) {
                     s_large = 1;
                     return __uint_as_float(0x7fc00000u);  // (its outputs are NaN until then)
                 }
@@ -537,7 +542,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                     }
                 }
                 const int i_row = there ? token(row) : 0, hq = p.head * each + (there ? r0 + row - i_row * each : 0);
-                if (there && a.lse) a.lse[(size_t)(p.sr.first + i_row) * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M) + log2f(L)) * 0.69314718055994530942f;
+                if (there && a.lse) a.lse[(size_t)(p.sr.first + i_row) * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M + SHIFT) + log2f(L * UNSHIFT)) * 0.69314718055994530942f;
                 if (bad && there) s_bad = 1;
             };
             const size_t prow = q * BQ + row;

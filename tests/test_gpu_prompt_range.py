@@ -223,3 +223,22 @@ def test_linear_that_gives_up_leaves_its_counters(gpu, dtype, rows, n, k):
         gpu.sync()
     assert torch.equal(go(), want)
     gpu.sync()
+
+
+# ---- values near a type's ends --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,width", [(5, 64), (100, 64), (100, 128), (5, 256)])
+@pytest.mark.parametrize("down", [14, 18, 22, 26, 30])
+@pytest.mark.parametrize("where", ["step", "steps"])
+def test_attend_f16_small_weights_of_large_values(gpu, rows, width, down, where):
+    """A weight of f16 is held to 2^-36 of the row's largest, not to f16's own smallest: values of 60,000 beside it are felt."""
+    keys = 200
+    q, k, v = np.zeros((rows, 1, width)), np.zeros((keys, 1, width)), np.zeros((keys, 1, width))
+    q[:, :, 0], k[:, :, 0] = 1, -500
+    k[7, 0, 0] = 0
+    at = 9 if where == "step" else 150
+    k[at, 0, 0], v[at, 0] = -down, np.linspace(30_000, 60_000, width).round(-2)
+    v = rounded(v, torch.float16)
+    got, _ = attend(gpu, "f16", q, k, v, LN2)
+    want, _ = plain.attend(q, k, v, [rows], [keys], 1, LN2, False, 0)
+    assert (np.abs(got - want) <= (2.0**-11 + 2.0**-19) * np.abs(want) + 2.0**-36 * 60_000 + 1.01 * 2.0**-11 * np.abs(want) + 2.0**-25).all()
