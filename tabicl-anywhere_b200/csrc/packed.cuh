@@ -57,9 +57,10 @@ __device__ __forceinline__ float pa_add(float x, float y, float &rest) {
 }
 // One row's output and log-sum-exp by one warp, from the keys that it sees and no others, U of them at a time. The products of a
 // tile's weights and values take every value of the tile times a weight, 0 for a row that does not see it, and 0 times an infinity
-// or a NaN is NaN; so a row whose output holds a NaN is worked out again here, and is NaN still only if what it sees makes it so.
+// or a NaN is NaN; so a row whose output holds a NaN is worked out again here, and is NaN still only if what it sees makes it so
+// (and a row whose weighted sum passed f32 before it was divided).
 // Products q k near the largest have an exact difference, however large they are; scale and exponential take that. Sums keep what
-// their roundings leave, and weights are divided by as many as there may be keys, so that no sum leaves the values' range. (A key
+// their roundings leave, and weights are scaled down where the values' sums come near f32's end. (A key
 // in 0.1 us; one at a time, with the whole chain of a load, five exchanges and two exponentials for each, 0.65.)
 template <int DT, int HD>
 __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int seq, int i, int hq) {
@@ -73,7 +74,8 @@ __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int 
     float x[C], o[C], o_rest[C];
 #pragma unroll
     for (int c = 0; c < C; c++) x[c] = lane + 32 * c < a.width ? Elem<DT>::get(q[32 * c]) : 0.f, o[c] = o_rest[c] = 0.f;
-    const float scale = fabsf(a.scale), part = __uint_as_float((unsigned)(95 + __clz(max(1, hi - lo))) << 23);  // 2^-(bits of the number of keys)
+    const float scale = fabsf(a.scale);
+    float part = 0.0625f;                        // what weights are multiplied by for this lane's outputs: U values have a sum
     float m = -INFINITY, l = 0.f, l_rest = 0.f;  // the largest product (of the scale's sign), the sum of weights
     bool dead = false;                           // every output is NaN, whatever follows
 #pragma unroll 1
@@ -124,10 +126,17 @@ __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int 
                 if (lane + 32 * c < a.width && j + u < hi) y[c] = fmaf(d[u] * part, Elem<DT>::get(from[32 * c]), y[c]);
         }
         dead = true;
+        bool near_end = false;
 #pragma unroll
         for (int c = 0; c < C; c++) {
             o[c] = pa_add(o[c], y[c], o_rest[c]);
             dead &= o[c] != o[c] || lane + 32 * c >= a.width;
+            near_end |= fabsf(o[c]) > 0x1p100f && finite_f(o[c]);
+        }
+        if (near_end) {
+            part *= 0x1p-28f;
+#pragma unroll
+            for (int c = 0; c < C; c++) o[c] *= 0x1p-28f, o_rest[c] *= 0x1p-28f;
         }
         dead = __all_sync(0xffffffffu, dead);
         if (dead && !a.lse) break;
@@ -140,14 +149,16 @@ __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int 
     if (a.lse && lane == 0) a.lse[(size_t)(s.first + i) * a.q_heads + hq] = (m == -INFINITY ? 0.f : m * scale) + logf(l);
 }
 
-// After a block's work, where some of its outputs hold a NaN: the units that it has written once more, the rows with a NaN that
-// may not be one worked out again. It may be wrong only where the unit's values hold an infinity (a weight that was rounded to
+// After a block's work, where some of its outputs are not finite: the units that it has written once more, the rows that may be
+// wrong worked out again. A NaN may be wrong only where the unit's values hold an infinity (a weight that was rounded to
 // nothing has a part in that) or a NaN that not all of its rows see, or (f32, whose operands are split) its keys or the row's
-// queries an infinity; rows that see a NaN in keys or values that all see are left as they are. `all`: every such row. From p the
+// queries an infinity; rows that see a NaN in keys or values that all see are left as they are. Infinities and NaN alike may
+// be wrong where values are so large that their weighted sums (weights up to 1 / by) may pass f32. `all`: every row that is not
+// finite. From p the
 // block's pieces begin; joined: whether it has written the unit that it shares with the blocks before, after it. By W warps (which
 // have all the registers that the kernel was compiled for), for which no bounded wait waits: a row may take as long as it has keys.
 template <int DT, int HD, int R, int STEP, int EXTRA, int W, class Cut>
-__device__ __noinline__ void pa_mend(const PackedArgs &a, typename Cut::Place p, const int *joined, bool all, int *dirty) {
+__device__ __noinline__ void pa_mend(const PackedArgs &a, typename Cut::Place p, const int *joined, bool all, float by, int *dirty) {
     using T = typename Elem<DT>::T;
     const int tid = threadIdx.x % (32 * W), warp = tid >> 5, lane = tid & 31, each = a.q_heads / a.c.heads;
     const size_t size = sizeof(T);
@@ -162,41 +173,43 @@ __device__ __noinline__ void pa_mend(const PackedArgs &a, typename Cut::Place p,
         if (count == sp.steps || joined[p.skip == 0]) {
             const int r0 = p.rt * R, rows = min(R, s.n * each - r0), end = min(s.len, sp.base + (sp.steps - EXTRA) * STEP);
             meet();
-            if (tid == 0) *dirty = all;
+            if (tid == 0) *dirty = all ? 2 : 0;
             meet();
             if (!all) {
                 const int pieces = a.width / 8;
                 const long long k0 = a.k_starts[p.seq] + sp.base;
-                bool found = false;
-                for (int x = tid; x < (end - sp.base) * pieces && !found; x += 32 * W) {
-                    const int j = x / pieces, c = (x - j * pieces) * 8;
+                // values that may be behind a wrong NaN, and such whose sums may pass f32 (f32's own kernel scales them)
+                const float limit = DT == DT_BF16 ? FLT_MAX * by / max(1, end - sp.base) : INFINITY;
+                bool found = false, large = false;
+                for (long long x = tid; x < (long long)(end - sp.base) * pieces && !large; x += 32 * W) {
+                    const int j = (int)(x / pieces), c = (int)(x - (long long)j * pieces) * 8;
                     float e[8];
                     load8<DT>(reinterpret_cast<const T *>(a.v) + (k0 + j) * a.v_row + p.head * a.v_head + c, wide_v, e);
                     const bool hidden = sp.base + j < sp.lo_max || sp.base + j >= sp.hi_min;
 #pragma unroll
-                    for (int y = 0; y < 8; y++) found |= infinite(e[y]) || (hidden && e[y] != e[y]);
+                    for (int y = 0; y < 8; y++) found |= infinite(e[y]) || (hidden && e[y] != e[y]), large |= fabsf(e[y]) > limit && !infinite(e[y]);
                     if constexpr (DT == DT_F32) {
                         load8<DT>(reinterpret_cast<const T *>(a.k) + (k0 + j) * a.k_row + p.head * a.k_head + c, wide_k, e);
 #pragma unroll
                         for (int y = 0; y < 8; y++) found |= infinite(e[y]);
                     }
                 }
-                if (found) *dirty = 1;
+                if (found || large) atomicMax(dirty, large ? 2 : 1);
                 meet();
             }
-            const bool some = *reinterpret_cast<volatile int *>(dirty);
+            const int some = *reinterpret_cast<volatile int *>(dirty);
             for (int r = warp; r < rows; r += W) {
                 const int i = (r0 + r) / each, hq = p.head * each + (r0 + r) % each;
                 const T *out = reinterpret_cast<const T *>(a.out) + (s.first + i) * a.o_row + hq * a.o_head;
                 const T *q = reinterpret_cast<const T *>(a.q) + (s.first + i) * a.q_row + hq * a.q_head;
-                bool nan = false, inf = false;
+                bool nan = false, end = false, inf = false;
                 for (int c = lane; c < a.width; c += 32) {
                     const float y = Elem<DT>::get(out[c]);
-                    nan |= y != y;
+                    nan |= y != y, end |= infinite(y);
                     if constexpr (DT == DT_F32) inf |= infinite(q[c]);
                 }
-                nan = __any_sync(0xffffffffu, nan), inf = __any_sync(0xffffffffu, inf);
-                if (nan && (some || inf)) pa_repair<DT, HD>(a, s, p.seq, i, hq);
+                nan = __any_sync(0xffffffffu, nan), end = __any_sync(0xffffffffu, end), inf = __any_sync(0xffffffffu, inf);
+                if ((nan && (some || inf)) || (end && some > 1)) pa_repair<DT, HD>(a, s, p.seq, i, hq);
             }
         }
         Cut::next(p, a, each, s.n, count);

@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
     __shared__ volatile int abort_flag;
     __shared__ int s_unit[4], s_last;
     // for the rows that are worked out again at the end: where the block's pieces began, the units that it has joined, whether some
-    // of its outputs are NaN, and whether of rows whose scores were too large
+    // of its outputs are not finite, and whether of rows whose scores were too large
     __shared__ typename Cut::Place s_place;
     __shared__ int s_joined[2], s_counted[2], s_dirty;  // (s_counted: whether the block has counted itself among those that share them)
     __shared__ volatile int s_bad, s_large;
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 return L != 0.f ? 1.f / L : 0.f;
             };
             float inv = whole ? inverse_of(m, l) : 1.f;
-            bool bad = false;
+            float2 odd = make_float2(0.f, 0.f);  // NaN once an output is not finite
             // 32 columns from 32 b on to the row's place in shared memory
             auto put = [&](int b, const float (&o)[32]) {
 #pragma unroll
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         const float y0 = o[8 * y + 2 * k] * inv, y1 = o[8 * y + 2 * k + 1] * inv;
-                        bad |= 32 * b + 8 * y < a.width && (y0 != y0 || y1 != y1);
+                        odd = pt_fma2(make_float2(y0, y1), make_float2(0.f, 0.f), odd);
                         w[k] = pt_pair<DT>(y0, y1);
                     }
                     *cell(row, 4 * b + y) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 }
                 const int i_row = there ? token(row) : 0, hq = p.head * each + (there ? r0 + row - i_row * each : 0);
                 if (there && a.lse) a.lse[(size_t)(p.sr.first + i_row) * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M + SHIFT) + log2f(L * UNSHIFT)) * 0.69314718055994530942f;
-                if (bad && there) s_bad = 1;
+                if (odd.x + odd.y != 0.f && there) s_bad = 1;
             };
             const size_t prow = q * BQ + row;
             float *mine = part + Cut::slot(blockIdx.x, p.begins) * C::PART;
@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
     }
     fence_after_sync();
     if (warp == 8) tmem_dealloc(tmem, 512);
-    if (warp < 8 && s_bad && !abort_flag) pa_mend<DT, HD, PT_R, PT_BK, EXTRA, 8, Cut>(a, s_place, s_joined, s_large, &s_dirty);
+    if (warp < 8 && s_bad && !abort_flag) pa_mend<DT, HD, PT_R, PT_BK, EXTRA, 8, Cut>(a, s_place, s_joined, s_large, 0x1p-8f, &s_dirty);
 }
 
 template <int HD>

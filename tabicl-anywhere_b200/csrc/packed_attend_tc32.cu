@@ -419,9 +419,12 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
             // ---- the row's output, or its part of it ----
             const bool whole = p.count == sp.steps;
             float M = rowx[0][row], L = rowx[1][row];
+            // (divided by the sum before it leaves its unit, a part too: the weighted sum of values near f32's largest may pass that)
             const float un0 = kt_pow2(unit / 2 - PS_T), un1 = kt_pow2(unit - unit / 2 - 14);
+            auto inverse = [](float sum) { return sum != 0.f ? 1.f / sum : 0.f; };  // 0 when no key is seen, NaN when a score is
+            const float inv = inverse(L);
 #pragma unroll
-            for (int k = 0; k < HD; k++) o[k] = o[k] * un0 * un1;
+            for (int k = 0; k < HD; k++) o[k] = o[k] * inv * un0 * un1;
             bool write = row < rows;
             if (!whole) {
                 const int2 who = Cut::sharers(pl, pl.pos - pl.skip, sp.steps);
@@ -443,14 +446,16 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                     __threadfence();
                     M = -INFINITY, L = 0.f;
                     for (int b = 0; b < who.y; b++) M = fmaxf(M, __ldcg(reinterpret_cast<const float2 *>(part) + Cut::slot(who.x + b, b == 0) * BQ + row).x);
+                    auto weight = [&](float2 x) { return x.x == -INFINITY ? x.y : x.y * kt_ex2(x.x - M); };  // (without keys 0, and a NaN sum stays one)
+                    for (int b = 0; b < who.y; b++) L += weight(__ldcg(reinterpret_cast<const float2 *>(part) + Cut::slot(who.x + b, b == 0) * BQ + row));
+                    const float all = inverse(L);
 #pragma unroll
                     for (int k = 0; k < HD; k++) o[k] = 0.f;
                     for (int b = 0; b < who.y; b++) {
                         const size_t from = Cut::slot(who.x + b, b == 0);
                         const float2 x = __ldcg(reinterpret_cast<const float2 *>(part) + from * BQ + row);
-                        const float f = x.x == -INFINITY ? (x.y != 0.f ? x.y : 0.f) : kt_ex2(x.x - M);  // (a NaN sum stays one)
                         if (x.x == -INFINITY && x.y == 0.f) continue;
-                        L = fmaf(x.y, f, L);
+                        const float f = weight(x) * all;
 #pragma unroll
                         for (int k = 0; k < HD; k += 4) {
                             const float4 y = __ldcg(reinterpret_cast<const float4 *>(po + from * BQ * HD + (k / 4 * BQ + row) * 4));
@@ -462,7 +467,6 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
             }
             bool bad = false;
             if (write && !abort_flag) {
-                const float inv = L != 0.f ? 1.f / L : 0.f;  // L is 0 when no key is seen, NaN when a score is
                 const bool wide = !(((uintptr_t)a.out & 15) || ((a.o_row | a.o_head) & 3));
                 float *to = reinterpret_cast<float *>(a.out) + (long long)(sr.first + ri) * a.o_row + (long long)hq * a.o_head;
 #pragma unroll
@@ -470,7 +474,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                     if (b >= a.width) break;
                     float v[8];
 #pragma unroll
-                    for (int x = 0; x < 8; x++) v[x] = L != 0.f ? o[b + x] * inv : 0.f, bad |= v[x] != v[x];
+                    for (int x = 0; x < 8; x++) v[x] = L != 0.f ? o[b + x] : 0.f, bad |= v[x] != v[x];
                     store8<DT_F32>(to + b, wide, v);
                 }
                 if (a.lse) a.lse[(size_t)(sr.first + ri) * a.q_heads + hq] = ((M == -INFINITY ? 0.f : M) + log2f(L)) * 0.69314718055994530942f;
@@ -485,7 +489,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
     if (tid == 0 && abort_flag) *reinterpret_cast<volatile int *>(a.err_wait) = 1;
     fence_after_sync();
     if (warp == 8) tmem_dealloc(tmem, 512);
-    if (wg == 1 && s_bad && !abort_flag) pa_mend<DT_F32, HD, PS_BQ, PS_BK, PS_EXTRA, 4, Cut>(a, s_place, s_joined, false, &s_dirty);
+    if (wg == 1 && s_bad && !abort_flag) pa_mend<DT_F32, HD, PS_BQ, PS_BK, PS_EXTRA, 4, Cut>(a, s_place, s_joined, false, 1.f, &s_dirty);
 }
 
 // Working memory: counters, parts, the tiles' powers of two, the tiles.

@@ -242,3 +242,25 @@ def test_attend_f16_small_weights_of_large_values(gpu, rows, width, down, where)
     got, _ = attend(gpu, "f16", q, k, v, LN2)
     want, _ = plain.attend(q, k, v, [rows], [keys], 1, LN2, False, 0)
     assert (np.abs(got - want) <= (2.0**-11 + 2.0**-19) * np.abs(want) + 2.0**-36 * 60_000 + 1.01 * 2.0**-11 * np.abs(want) + 2.0**-25).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,width", [(5, 64), (100, 64), (100, 128), (100, 256)])
+@pytest.mark.parametrize("keys", [70, 3000])
+@pytest.mark.parametrize("end", ["largest", "smallest"])
+def test_attend_values_near_the_ends(gpu, dtype, rows, width, keys, end):
+    """Weighted sums that pass a type's end before they are divided: an output is never further out than the values. And values that
+    are small, which nothing that is done for those may lose."""
+    rng = np.random.default_rng(keys)
+    end = {"largest": 60_000.0 if dtype == "f16" else 3e38, "smallest": 1e-5 if dtype == "f16" else 1e-33}[end]
+    q, k = (rounded(rng.normal(0, 1, (n, 2, width)), DT[dtype][1]) for n in (rows, keys))
+    v = rounded(rng.uniform(0.9, 1, (keys, 2, width)) * end, DT[dtype][1])
+    v[:, 1] *= np.where(rng.random((keys, 1)) < 0.5, -1, 1)
+    scale = width**-0.5
+    got, _ = attend(gpu, dtype, q, k, v, scale)
+    want, _ = plain.attend(q, k, v, [rows], [keys], 2, scale, False, 0)
+    size, _ = plain.attend(q, k, np.abs(v), [rows], [keys], 2, scale, False, 0)
+    score = scale * np.abs(q).sum(-1).max() * np.abs(k).max() * 2.0**-20
+    weight = score + 2.0**-19 + (0 if dtype == "f32" else ULP[dtype]) + (keys // 16 + 8) * 2.0**-24
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want) <= 2 * weight * size + 1.01 * ULP[dtype] * np.abs(want) + 2 * base.TINY[dtype] + 2.0**-126).all()
