@@ -21,6 +21,7 @@ constexpr int PS_BQ = 128, PS_BK = 64, PS_NS = 3, PS_THREADS = 384;
 constexpr int PS_STEPS = 8;  // steps a block takes at least
 constexpr int PS_EXTRA = 2;  // what a unit costs besides its steps, in steps
 constexpr int PS_T = 13;     // split values are below 2^T
+constexpr int NONE = -4000;  // the exponent of a unit that nothing has
 constexpr uint32_t PS_TQ = 0, PS_TS = 128, PS_TO = 384;
 
 template <int HD>
@@ -115,7 +116,8 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
     using Cut = KaCut<PS_BQ, PS_BK, PS_BK, PS_EXTRA>;
     constexpr int BQ = PS_BQ, BK = PS_BK, NS = PS_NS, BLOCK = C::BLOCK;
     extern __shared__ uint8_t smraw[];
-    __shared__ float fr[4][BQ], rowx[2][BQ], qmax[2][BQ];
+    __shared__ float2 fr[4][BQ];
+    __shared__ float rowx[2][BQ], qmax[2][BQ];
     __shared__ int teK[8], teV[8];
     __shared__ __align__(8) uint64_t mK[NS], mV[NS], mKfree[NS], mVfree[NS], mS[NS], mP[NS], mSlot[NS], mF[4], mPV, mOfree, mDone[3];
     __shared__ uint32_t tslot;
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
             const int r = min(row, rows - 1), ri = (r0 + r) / each, hq = pl.head * each + (r0 + r) % each;  // rows past the end repeat the last
             const int my_hi = ka_hi(a, sr, ri) - p.j0, my_lo = ka_lo(a, sr, ri) - p.j0;
             const float rowfac = put_q(sr, ri, hq);
-            // ---- softmax: S(i) -> 2^14 P(i), P(i) = 2^(S - m), over S(i), and the factor of what was before ----
+            // ---- softmax: S(i) -> 2^14 P(i), P(i) = 2^(S - the step's largest), over S(i), and the factors of what was before and of the step ----
             float mrun = -INFINITY, lrun = 0.f;
 #pragma unroll 1
             for (int i = at; i < at + p.n; i++) {
@@ -345,8 +347,9 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
 #pragma unroll
                 for (int k = 0; k < 64; k++) top[k & 3] = fmaxf(top[k & 3], x[k]);
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                const float mnew = fmaxf(mrun, mx * c1), mm = mnew == -INFINITY ? 0.f : mnew;
-                const float f = mrun == -INFINITY ? 0.f : kt_ex2(mrun - mnew);
+                // (weights beside the step's own largest: a step far below the row's largest keeps its bits, for values may be as far above)
+                const float mstep = __fmul_rn(mx, c1), mnew = fmaxf(mrun, mstep), mm = mstep == -INFINITY ? 0.f : mstep;
+                const float f = mrun == -INFINITY ? 0.f : kt_ex2(mrun - mnew), h = mstep == -INFINITY ? 0.f : kt_ex2(mstep - mnew);
                 float psum[4] = {};
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
@@ -365,11 +368,11 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                     tmem_st32u(tsp + 32 * b, w);
                 }
                 tmem_wait_st();
-                fr[i & 3][row] = f;
+                fr[i & 3][row] = make_float2(f, h);
                 fence_before_sync();
                 mbar_arrive(&mP[sl]);
                 mbar_arrive(&mF[i & 3]);
-                lrun = fmaf(lrun, f, (psum[0] + psum[1]) + (psum[2] + psum[3]));
+                lrun = fmaf(lrun, f, ((psum[0] + psum[1]) + (psum[2] + psum[3])) * h);
                 mrun = mnew;
             }
             rowx[0][row] = mrun, rowx[1][row] = lrun;
@@ -386,9 +389,9 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
             const int r0 = pl.rt * BQ, rows = min(BQ, sr.n * each - r0);
             const int r = min(row, rows - 1), ri = (r0 + r) / each, hq = pl.head * each + (r0 + r) % each;  // rows past the end repeat the last
             put_q(sr, ri, hq);
-            // ---- fold: O = O f + P V, in units of the tile's power of two ----
+            // ---- fold: O = O f + P V h, O in a unit of the row's, a power of two ----
             float o[HD];
-            int unit = 0;
+            int unit = NONE;
 #pragma unroll
             for (int k = 0; k < HD; k++) o[k] = 0.f;
 #pragma unroll 1
@@ -397,13 +400,18 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
                 wait_warp(&mF[i & 3], (uint32_t)(i >> 2) & 1u);
                 fence_after_sync();
                 const int e = *reinterpret_cast<volatile int *>(&teV[i & 7]);
-                // in the larger unit of the two, whatever is smaller scaled down
-                float f = fr[i & 3][row], g = 1.f;
-                if (i == at) unit = e;
-                if (e > unit)
-                    f *= kt_pow2(max(-126, unit - e)), unit = e;
-                else
-                    g = kt_pow2(max(-126, e - unit));
+                // Each side in its own unit (the factors' powers of two go there), then both in the larger of the two, what is far below gone.
+                // A factor of 0 (keys that are not seen, scores far below) has no unit: it has no say in that.
+                const float2 fh = fr[i & 3][row];
+                auto level = [](float x, int &exponent) {
+                    const uint32_t w = __float_as_uint(x);
+                    exponent = w ? (int)(w >> 23) - 127 : NONE;
+                    return w ? __uint_as_float((w & 0x7fffffu) | 0x3f800000u) : 0.f;
+                };
+                int old, step;
+                float f = level(fh.x, old), g = level(fh.y, step);
+                old += unit, step += e, unit = max(max(old, step), NONE);
+                f = old < unit - 126 ? 0.f : f * kt_pow2(old - unit), g = step < unit - 126 ? 0.f : g * kt_pow2(step - unit);
 #pragma unroll
                 for (int c = 0; c < HD / 32; c++) {
                     float x[32];
@@ -420,7 +428,8 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
             const bool whole = p.count == sp.steps;
             float M = rowx[0][row], L = rowx[1][row];
             // (divided by the sum before it leaves its unit, a part too: the weighted sum of values near f32's largest may pass that)
-            const float un0 = kt_pow2(unit / 2 - PS_T), un1 = kt_pow2(unit - unit / 2 - 14);
+            unit -= PS_T + 14;
+            const float un0 = unit < -252 ? 0.f : kt_pow2(unit / 2), un1 = unit < -252 ? 0.f : kt_pow2(unit - unit / 2);
             auto inverse = [](float sum) { return sum != 0.f ? 1.f / sum : 0.f; };  // 0 when no key is seen, NaN when a score is
             const float inv = inverse(L);
 #pragma unroll

@@ -264,3 +264,53 @@ def test_attend_values_near_the_ends(gpu, dtype, rows, width, keys, end):
     weight = score + 2.0**-19 + (0 if dtype == "f32" else ULP[dtype]) + (keys // 16 + 8) * 2.0**-24
     assert np.isfinite(got).all()
     assert (np.abs(got - want) <= 2 * weight * size + 1.01 * ULP[dtype] * np.abs(want) + 2 * base.TINY[dtype] + 2.0**-126).all()
+
+
+# ---- tiles of very different values (f32) ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("small,large", [(2.0**-111, 2.0**126), (2.0**126, 2.0**-111), (2.0**-60, 2.0**100), (2.0**-20, 2.0**20)])
+@pytest.mark.parametrize("mask", ["causal", "window", "weights"])
+def test_attend_f32_tiles_apart(gpu, width, small, large, mask):
+    """Values of 64 keys beside others up to 2^237 as large, which a row does not see, or weighs with nothing: it keeps its own to
+    2^-35 of the largest of their 64."""
+    rng = np.random.default_rng(1)
+    n = 128
+    q, k, v = (rounded(rng.normal(0, 1, (n, 1, width)).clip(-1.9, 1.9), torch.float32) for _ in range(3))
+    v[:64] *= small
+    v[64:] *= large
+    if mask == "weights":  # rows of either sign: the keys of one half are nothing to them
+        q[:, 0, 0], k[:64, 0, 0], k[64:, 0, 0] = np.where(np.arange(n) % 2, 1.0, -1.0), 2000, -2000
+    causal, window, scale = mask != "weights", 20 if mask == "window" else 0, 0.125
+    got, _ = attend(gpu, "f32", q, k, v, scale, causal, window)
+    want, _ = plain.attend(q, k, v, [n], [n], 1, scale, causal, window)
+    size, _ = plain.attend(q, k, np.abs(v), [n], [n], 1, scale, causal, window)
+    # the scores' rounding (a weight's: 64 or 128 products of up to 2^11 each held to 2^-21), and what 64 neighbours share
+    kmax = 2000 if mask == "weights" else 2
+    weight = scale * np.abs(q).sum(-1).max() * kmax * 2.0**-20 + 2.0**-19
+    seen = np.zeros((n, 2))  # the largest of the two tiles that the row has something from
+    for i in range(n):
+        lo, hi = (max(0, i + 1 - window) if window else 0, i + 1) if causal else (0, n)
+        for t, (a, b) in enumerate(((0, 64), (64, 128))):
+            there = min(hi, b) > max(lo, a) and (causal or (i % 2 == 1) == (t == 0))
+            seen[i, t] = (small, large)[t] * 2 if there else 0
+    tol = 2 * weight * size + 2.0**-34 * seen.max(1)[:, None, None] + 2.0**-148
+    assert (np.abs(got - want) <= tol).all(), np.max(np.abs(got - want) / tol)
+
+
+@pytest.mark.parametrize("rows,width", [(5, 64), (100, 64), (100, 128)])
+@pytest.mark.parametrize("down,up", [(30, 20), (40, 60), (100, 110), (120, 90)])
+@pytest.mark.parametrize("first", [True, False])
+def test_attend_f32_small_weights_of_large_values(gpu, rows, width, down, up, first):
+    """A step whose weights are far below the row's largest, of values as far above the others: it is felt."""
+    keys = 192
+    rng = np.random.default_rng(down)
+    q, k, v = np.zeros((rows, 1, width)), np.zeros((keys, 1, width)), rounded(rng.uniform(0.5, 1, (keys, 1, width)), torch.float32)
+    q[:, :, 0], k[:, :, 0] = 1, -500
+    a, b = (7, 150) if first else (150, 7)
+    k[a, 0, 0], k[b, 0, 0] = 0, -down
+    v[b] *= 2.0**up
+    got, _ = attend(gpu, "f32", q, k, v, LN2)
+    want, _ = plain.attend(q, k, v, [rows], [keys], 1, LN2, False, 0)
+    # (a weight's exponential, 2^-19; what 64 neighbours of the values share, times the weight that they have at most)
+    assert (np.abs(got - want) <= 2.0**-18 * np.abs(want) + 2.0**-34 * 2.0 ** max(up - down, 0)).all()
