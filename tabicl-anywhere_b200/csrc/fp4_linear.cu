@@ -397,9 +397,10 @@ static FlPlan fl_plan(int dtype, const Fp4LinearArgs &a, int sms) {
             if (!p.nt || cost < best) best = cost, p.nt = nt, p.split = parts > 1, p.blocks = (int)blocks;
         }
     }
-    // f32 results: the matrix unit does not round its sums to nearest, so a sum runs over 4 steps in it, from there on in
-    // registers; two narrower accumulators in turn, so that the unit does not wait for them to be read
-    p.chunk = dtype == DT_F32 ? 4 : p.steps;
+    // The matrix unit rounds its sums towards zero, so a sum runs over a number of steps in it, from there on in registers: f32 results
+    // over 4, with two narrower accumulators in turn, so that the unit does not wait for them to be read; 16-bit ones over 64, whose
+    // 256 additions leave 2^-17 of a sum of one sign (all of 262,144 columns: 2^-14, a seventh of a half of f16's last place).
+    p.chunk = dtype == DT_F32 ? 4 : std::min(64, p.steps);
     p.nacc = p.nt > 128 ? 1 : 2;
     int cols = 32;
     while (cols < p.nt) cols *= 2;

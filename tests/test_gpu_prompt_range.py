@@ -314,3 +314,34 @@ def test_attend_f32_small_weights_of_large_values(gpu, rows, width, down, up, fi
     want, _ = plain.attend(q, k, v, [rows], [keys], 1, LN2, False, 0)
     # (a weight's exponential, 2^-19; what 64 neighbours of the values share, times the weight that they have at most)
     assert (np.abs(got - want) <= 2.0**-18 * np.abs(want) + 2.0**-34 * 2.0 ** max(up - down, 0)).all()
+
+
+# ---- long sums ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_linear_long_rows_have_no_bias(gpu, dtype):
+    """Thousands of products of one sign: the matrix unit rounds its sums towards zero, so a result is made of sums of at most
+    256 of its additions (each off by a unit in the last place of f32 at most, half of one on average): 2^-16 on average."""
+    code, tt = DT[dtype]
+    rows, n, k = 16, 150 * 128, 2**18
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    numbers = torch.tensor(plain.NUMBERS, device="cuda")
+    power = torch.randint(-14, -4, (k // 32,), device="cuda", generator=gen)  # of the scales, the same for all rows (sums then need more than 24 bits)
+    mats = []
+    for r in (rows, n):
+        codes = torch.randint(0, 256, (r, k // 2), dtype=torch.uint8, device="cuda", generator=gen) & 0x77
+        scales = (power + 127).to(torch.uint8).view(1, k // 128, 1, 4).expand(-(-r // 128), -1, 128, -1).contiguous()
+        mats.append((tcu.Fp4(gpu, r, k, tcu.MX, codes.data_ptr(), scales.data_ptr()), codes, scales))
+    want = torch.zeros(rows, n, dtype=torch.float64, device="cuda")
+    for at in range(0, k, 2**12):
+        by = torch.pow(2.0, power[at // 32:(at + 2**12) // 32].double()).repeat_interleave(32)
+        xv, wv = (numbers[torch.stack([c & 7, c >> 4], -1).flatten(1).long()].double() * by for c in (m[1][:, at // 2:at // 2 + 2**11] for m in mats))
+        want += xv @ wv.t()
+    x, w = mats[0][0], mats[1][0]
+    y = torch.zeros(rows, n, dtype=tt, device="cuda")
+    work = torch.zeros(w.linear_workspace(x, code), dtype=torch.uint8, device="cuda")
+    w.linear(x, code, y.data_ptr(), n, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    off = (y.double() - want) / want
+    assert off.abs().max() <= ULP[dtype] + 2.0**-14
+    assert off.mean().abs() <= 2.0**-16, off.mean()
