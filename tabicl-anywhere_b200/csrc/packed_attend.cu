@@ -9,6 +9,7 @@
 // f16's range. Rows whose weighted sum passes f32 before it is divided are worked out again by themselves. 32 requests of 0 to 16,383 bf16 tokens, 32 heads on 8 of
 // width 128: 188 us for 1.05 GB, 5.6 TB/s (343 us with a division for every 16 bytes copied).
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "packed.cuh"
@@ -19,6 +20,9 @@ constexpr int PA_THREADS = 128;
 // What a unit costs besides its steps, in steps, and the steps that a block takes at least: so that units of one step are a block's
 // each (21 rows of 32 heads on 8 of width 256: 81 us with four units a block), and shorter parts of longer ones are not joined.
 constexpr int PA_EXTRA = 4, PA_STEPS = 5;
+// Steps of 16-bit keys over which a product's sums run in the matrix unit, which rounds them towards zero (1.1e-7 of one an
+// addition, of values of one sign); from there on they are added in the working memory.
+constexpr int PA_FOLD = 128;
 
 template <int DT, int HD_, int WR>
 struct PaShape {
@@ -32,6 +36,7 @@ struct PaShape {
     static constexpr int TILE = BK * PITCH, CP = HD + 4;
     static constexpr size_t SMEM = (size_t)STAGES * 2 * TILE + R * PITCH;
     static constexpr size_t PART = (size_t)R * (HD + 2);  // floats of a part: outputs, maxima, sums
+    static constexpr size_t SUMS = (size_t)PA_THREADS * HD / 2;  // floats of a block's folded sums
     static_assert((size_t)64 * CP * 4 + 512 <= (size_t)STAGES * 2 * TILE, "the warps' outputs meet where keys and values were");
 };
 
@@ -108,7 +113,7 @@ __device__ __forceinline__ void pa_copy(uint8_t *to, const void *base, long long
 }
 
 template <int DT, int HD, int WR>
-__global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int wide, float *part, int *arrived) {
+__global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int wide, float *part, float *sums, int *arrived) {
     using C = PaShape<DT, HD, WR>;
     using T = typename C::T;
     using Raw = typename C::Raw;
@@ -194,130 +199,151 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
 #pragma unroll
             for (int x = 0; x < 4; x++) o[i][x] = 0.f;
 
-        for (int i = 0; i < n; i++) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
-            __syncthreads();
-            load(i + STAGES - 1);
-            const uint8_t *ks = sm + (size_t)(i % STAGES) * 2 * C::TILE + kw * OWN * PITCH, *vs = ks + C::TILE;
-            float s[NT][4];
-#pragma unroll
-            for (int x = 0; x < NT; x++)
-#pragma unroll
-                for (int y = 0; y < 4; y++) s[x][y] = 0.f;
-            if constexpr (C::F32) {
-                const float *qf = reinterpret_cast<const float *>(Qs + (16 * wr + g) * PITCH);
-                // (32 coordinates' sums at a time in the unit, which does not round them to nearest; these are added here)
+        // the sums of the steps before, and the maxima that they are relative to
+        float4 *kept = reinterpret_cast<float4 *>(sums) + blockIdx.x * (C::SUMS / 4) + tid;
+        float m_kept[2] = {-INFINITY, -INFINITY};
+        auto kept_by = [&](int x) { return m_kept[x] == -INFINITY ? 0.f : pa_ex2(m_kept[x] - m[x]); };
+        constexpr int FOLD = C::F32 ? INT_MAX : PA_FOLD;
 #pragma unroll 1
-                for (int c0 = 0; c0 < HD; c0 += 32) {
-                    float part[NT][4];
-#pragma unroll
-                    for (int x = 0; x < NT; x++)
-#pragma unroll
-                        for (int y = 0; y < 4; y++) part[x][y] = 0.f;
-#pragma unroll
-                    for (int c = c0; c < c0 + 32; c += 8) {
-                        uint32_t h[4], lw[4];
-                        pa_split(qf[c + t], h[0], lw[0]), pa_split(qf[8 * PITCH / 4 + c + t], h[1], lw[1]);
-                        pa_split(qf[c + t + 4], h[2], lw[2]), pa_split(qf[8 * PITCH / 4 + c + t + 4], h[3], lw[3]);
-#pragma unroll
-                        for (int x = 0; x < NT; x++) {
-                            const float *kf = reinterpret_cast<const float *>(ks + (8 * x + g) * PITCH) + c + t;
-                            uint32_t bh[2], bl[2];
-                            pa_split(kf[0], bh[0], bl[0]), pa_split(kf[4], bh[1], bl[1]);
-                            pa_mma<DT>(part[x], lw, bh[0], bh[1]);
-                            pa_mma<DT>(part[x], h, bl[0], bl[1]);
-                            pa_mma<DT>(part[x], h, bh[0], bh[1]);
-                        }
-                    }
-#pragma unroll
-                    for (int x = 0; x < NT; x++)
-#pragma unroll
-                        for (int y = 0; y < 4; y++) s[x][y] += part[x][y];
-                }
-            } else {
-                const uint32_t qa = pa_smem(Qs + (16 * wr + (lane & 15)) * PITCH + (lane >> 4) * 16);
-                const uint32_t ka = pa_smem(ks + ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16);
-#pragma unroll
-                for (int c = 0; c < HD / 16; c++) {
-                    uint32_t q[4];
-                    pa_ldsm(qa + c * 32, q);
-#pragma unroll
-                    for (int x = 0; x < NT; x += 2) {
-                        uint32_t b[4];
-                        pa_ldsm(ka + 8 * x * PITCH + c * 32, b);
-                        pa_mma<DT>(s[x], q, b[0], b[1]), pa_mma<DT>(s[x + 1], q, b[2], b[3]);
-                    }
-                }
-            }
-            // scores in units of log2; what a row does not see goes, whatever it is
-            const int at = j0 + i * BK + kw * OWN + 2 * t;
-            const bool edge = j0 + i * BK < sp.lo_max || j0 + (i + 1) * BK > sp.hi_min || rows < R;
-            float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int x = 0; x < NT; x++)
-#pragma unroll
-                for (int y = 0; y < 4; y++) {
-                    const int j = at + 8 * x + (y & 1);
-                    float v = s[x][y] * sl;
-                    if (edge && (j < lo[y >> 1] || j >= hi[y >> 1])) v = -INFINITY;
-                    s[x][y] = v, top[y >> 1] = fmaxf(top[y >> 1], v);
-                }
-            float f[2], ref[2];
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-                top[x] = fmaxf(fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2)), m[x]);
-                ref[x] = top[x] == -INFINITY ? 0.f : top[x];
-                f[x] = m[x] == -INFINITY ? 0.f : pa_ex2(m[x] - ref[x]);
-            }
-            if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
-#pragma unroll
-                for (int x = 0; x < NO; x++)
-#pragma unroll
-                    for (int y = 0; y < 4; y++)
-                        if (m[y >> 1] != -INFINITY) o[x][y] *= f[y >> 1];
-                l[0] *= f[0], l[1] *= f[1], m[0] = top[0], m[1] = top[1];
-            }
-#pragma unroll
-            for (int x = 0; x < NT; x++)
-#pragma unroll
-                for (int y = 0; y < 4; y++) s[x][y] = pa_ex2(s[x][y] - ref[y >> 1]), l[y >> 1] += s[x][y];
-            if constexpr (C::F32) {
-                // A fragment's k takes the keys in the order in which a thread has their weights: k = t key 2 t, k = t + 4 key 2 t + 1.
-                // The unit does not round its sums to nearest, so each step's are its own, added here (over 10,000 keys 2.8e-5 of
-                // an output otherwise).
-                uint32_t h[NT][4], lw[NT][4];
+        for (int i0 = 0; i0 < n; i0 += FOLD) {
+            for (int i = i0; i < n && i - i0 < FOLD; i++) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+                __syncthreads();
+                load(i + STAGES - 1);
+                const uint8_t *ks = sm + (size_t)(i % STAGES) * 2 * C::TILE + kw * OWN * PITCH, *vs = ks + C::TILE;
+                float s[NT][4];
 #pragma unroll
                 for (int x = 0; x < NT; x++)
-                    pa_split(s[x][0], h[x][0], lw[x][0]), pa_split(s[x][2], h[x][1], lw[x][1]), pa_split(s[x][1], h[x][2], lw[x][2]), pa_split(s[x][3], h[x][3], lw[x][3]);
+#pragma unroll
+                    for (int y = 0; y < 4; y++) s[x][y] = 0.f;
+                if constexpr (C::F32) {
+                    const float *qf = reinterpret_cast<const float *>(Qs + (16 * wr + g) * PITCH);
+                    // (32 coordinates' sums at a time in the unit, which does not round them to nearest; these are added here)
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HD; c0 += 32) {
+                        float part[NT][4];
+#pragma unroll
+                        for (int x = 0; x < NT; x++)
+#pragma unroll
+                            for (int y = 0; y < 4; y++) part[x][y] = 0.f;
+#pragma unroll
+                        for (int c = c0; c < c0 + 32; c += 8) {
+                            uint32_t h[4], lw[4];
+                            pa_split(qf[c + t], h[0], lw[0]), pa_split(qf[8 * PITCH / 4 + c + t], h[1], lw[1]);
+                            pa_split(qf[c + t + 4], h[2], lw[2]), pa_split(qf[8 * PITCH / 4 + c + t + 4], h[3], lw[3]);
+#pragma unroll
+                            for (int x = 0; x < NT; x++) {
+                                const float *kf = reinterpret_cast<const float *>(ks + (8 * x + g) * PITCH) + c + t;
+                                uint32_t bh[2], bl[2];
+                                pa_split(kf[0], bh[0], bl[0]), pa_split(kf[4], bh[1], bl[1]);
+                                pa_mma<DT>(part[x], lw, bh[0], bh[1]);
+                                pa_mma<DT>(part[x], h, bl[0], bl[1]);
+                                pa_mma<DT>(part[x], h, bh[0], bh[1]);
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < NT; x++)
+#pragma unroll
+                            for (int y = 0; y < 4; y++) s[x][y] += part[x][y];
+                    }
+                } else {
+                    const uint32_t qa = pa_smem(Qs + (16 * wr + (lane & 15)) * PITCH + (lane >> 4) * 16);
+                    const uint32_t ka = pa_smem(ks + ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16);
+#pragma unroll
+                    for (int c = 0; c < HD / 16; c++) {
+                        uint32_t q[4];
+                        pa_ldsm(qa + c * 32, q);
+#pragma unroll
+                        for (int x = 0; x < NT; x += 2) {
+                            uint32_t b[4];
+                            pa_ldsm(ka + 8 * x * PITCH + c * 32, b);
+                            pa_mma<DT>(s[x], q, b[0], b[1]), pa_mma<DT>(s[x + 1], q, b[2], b[3]);
+                        }
+                    }
+                }
+                // scores in units of log2; what a row does not see goes, whatever it is
+                const int at = j0 + i * BK + kw * OWN + 2 * t;
+                const bool edge = j0 + i * BK < sp.lo_max || j0 + (i + 1) * BK > sp.hi_min || rows < R;
+                float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const int j = at + 8 * x + (y & 1);
+                        float v = s[x][y] * sl;
+                        if (edge && (j < lo[y >> 1] || j >= hi[y >> 1])) v = -INFINITY;
+                        s[x][y] = v, top[y >> 1] = fmaxf(top[y >> 1], v);
+                    }
+                float f[2], ref[2];
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+                    top[x] = fmaxf(fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2)), m[x]);
+                    ref[x] = top[x] == -INFINITY ? 0.f : top[x];
+                    f[x] = m[x] == -INFINITY ? 0.f : pa_ex2(m[x] - ref[x]);
+                }
+                if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+#pragma unroll
+                    for (int x = 0; x < NO; x++)
+#pragma unroll
+                        for (int y = 0; y < 4; y++)
+                            if (m[y >> 1] != -INFINITY) o[x][y] *= f[y >> 1];
+                    l[0] *= f[0], l[1] *= f[1], m[0] = top[0], m[1] = top[1];
+                }
+#pragma unroll
+                for (int x = 0; x < NT; x++)
+#pragma unroll
+                    for (int y = 0; y < 4; y++) s[x][y] = pa_ex2(s[x][y] - ref[y >> 1]), l[y >> 1] += s[x][y];
+                if constexpr (C::F32) {
+                    // A fragment's k takes the keys in the order in which a thread has their weights: k = t key 2 t, k = t + 4 key 2 t + 1.
+                    // The unit does not round its sums to nearest, so each step's are its own, added here (over 10,000 keys 2.8e-5 of
+                    // an output otherwise).
+                    uint32_t h[NT][4], lw[NT][4];
+#pragma unroll
+                    for (int x = 0; x < NT; x++)
+                        pa_split(s[x][0], h[x][0], lw[x][0]), pa_split(s[x][2], h[x][1], lw[x][1]), pa_split(s[x][1], h[x][2], lw[x][2]), pa_split(s[x][3], h[x][3], lw[x][3]);
+#pragma unroll
+                    for (int c = 0; c < NO; c++) {
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int x = 0; x < NT; x++) {
+                            const float *vf = reinterpret_cast<const float *>(vs + (8 * x + 2 * t) * PITCH) + 8 * c + g;
+                            uint32_t bh[2], bl[2];
+                            pa_split(vf[0], bh[0], bl[0]), pa_split(vf[PITCH / 4], bh[1], bl[1]);
+                            pa_mma<DT>(sum, lw[x], bh[0], bh[1]);
+                            pa_mma<DT>(sum, h[x], bl[0], bl[1]);
+                            pa_mma<DT>(sum, h[x], bh[0], bh[1]);
+                        }
+#pragma unroll
+                        for (int y = 0; y < 4; y++) o[c][y] += sum[y];
+                    }
+                } else {
+                    const uint32_t va = pa_smem(vs + (lane & 15) * PITCH + (lane >> 4) * 16);
+#pragma unroll
+                    for (int x = 0; x < NT; x += 2) {
+                        const uint32_t p[4] = {pa_pair<DT>(s[x][0] * UP, s[x][1] * UP), pa_pair<DT>(s[x][2] * UP, s[x][3] * UP),
+                                               pa_pair<DT>(s[x + 1][0] * UP, s[x + 1][1] * UP), pa_pair<DT>(s[x + 1][2] * UP, s[x + 1][3] * UP)};
+#pragma unroll
+                        for (int c = 0; c < NO; c += 2) {
+                            uint32_t b[4];
+                            pa_ldsm_t(va + 8 * x * PITCH + c * 16, b);
+                            pa_mma<DT>(o[c], p, b[0], b[1]), pa_mma<DT>(o[c + 1], p, b[2], b[3]);
+                        }
+                    }
+                }
+            }
+            if (!C::F32 && n > FOLD) {
+                const bool more = n - i0 > FOLD;
+                const float f0 = kept_by(0), f1 = kept_by(1);
 #pragma unroll
                 for (int c = 0; c < NO; c++) {
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int x = 0; x < NT; x++) {
-                        const float *vf = reinterpret_cast<const float *>(vs + (8 * x + 2 * t) * PITCH) + 8 * c + g;
-                        uint32_t bh[2], bl[2];
-                        pa_split(vf[0], bh[0], bl[0]), pa_split(vf[PITCH / 4], bh[1], bl[1]);
-                        pa_mma<DT>(sum, lw[x], bh[0], bh[1]);
-                        pa_mma<DT>(sum, h[x], bl[0], bl[1]);
-                        pa_mma<DT>(sum, h[x], bh[0], bh[1]);
-                    }
-#pragma unroll
-                    for (int y = 0; y < 4; y++) o[c][y] += sum[y];
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (i0) v = __ldcg(kept + c * PA_THREADS);
+                    v = make_float4(fmaf(v.x, f0, o[c][0]), fmaf(v.y, f0, o[c][1]), fmaf(v.z, f1, o[c][2]), fmaf(v.w, f1, o[c][3]));
+                    if (more) __stcg(kept + c * PA_THREADS, v), v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    o[c][0] = v.x, o[c][1] = v.y, o[c][2] = v.z, o[c][3] = v.w;
                 }
-            } else {
-                const uint32_t va = pa_smem(vs + (lane & 15) * PITCH + (lane >> 4) * 16);
-#pragma unroll
-                for (int x = 0; x < NT; x += 2) {
-                    const uint32_t p[4] = {pa_pair<DT>(s[x][0] * UP, s[x][1] * UP), pa_pair<DT>(s[x][2] * UP, s[x][3] * UP),
-                                           pa_pair<DT>(s[x + 1][0] * UP, s[x + 1][1] * UP), pa_pair<DT>(s[x + 1][2] * UP, s[x + 1][3] * UP)};
-#pragma unroll
-                    for (int c = 0; c < NO; c += 2) {
-                        uint32_t b[4];
-                        pa_ldsm_t(va + 8 * x * PITCH + c * 16, b);
-                        pa_mma<DT>(o[c], p, b[0], b[1]), pa_mma<DT>(o[c + 1], p, b[2], b[3]);
-                    }
-                }
+                m_kept[0] = m[0], m_kept[1] = m[1];
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -415,12 +441,12 @@ __global__ void __launch_bounds__(PA_THREADS) k_packed_attend(PackedArgs a, int 
 
 struct PaPlan {
     int hd, wr, blocks;
-    size_t smem, part;
+    size_t smem, part, sums;
 };
 template <int DT, int HD, int WR>
 static PaPlan pa_plan(int sms) {
     using C = PaShape<DT, HD, WR>;
-    return PaPlan{HD, WR, std::min(KA_BLOCKS, sms * std::max(1, std::min(4, (int)(224 * 1024 / (C::SMEM + 2048))))), C::SMEM, C::PART};
+    return PaPlan{HD, WR, std::min(KA_BLOCKS, sms * std::max(1, std::min(4, (int)(224 * 1024 / (C::SMEM + 2048))))), C::SMEM, C::PART, DT == DT_F32 ? 0 : C::SUMS};
 }
 template <int DT, int HD>
 static PaPlan pa_plan(const PackedArgs &a, int sms) {
@@ -443,7 +469,8 @@ static cudaError_t pa_launch(const PackedArgs &a, const PaPlan &p, void *work, c
     const cudaError_t e = allow_dynamic_smem((const void *)k_packed_attend<DT, HD, WR>, p.smem);
     if (e != cudaSuccess) return e;
     int *arrived = reinterpret_cast<int *>(work);
-    k_packed_attend<DT, HD, WR><<<p.blocks, PA_THREADS, p.smem, s>>>(a, wide, reinterpret_cast<float *>(arrived + KA_BLOCKS), arrived);
+    float *parts = reinterpret_cast<float *>(arrived + KA_BLOCKS);
+    k_packed_attend<DT, HD, WR><<<p.blocks, PA_THREADS, p.smem, s>>>(a, wide, parts, parts + 2 * p.blocks * p.part, arrived);
     return cudaGetLastError();
 }
 template <int DT, int HD>
@@ -473,7 +500,8 @@ static bool pa_many32(int dtype, const PackedArgs &a, int sms) {
 size_t packed_attend_workspace(int dtype, const PackedArgs &a, int sms) {
     if (pa_many32(dtype, a, sms)) return packed_attend_tc32_workspace(a, sms);
     const PaPlan p = plan_of(dtype, a, sms);
-    const size_t own = sizeof(int) * KA_BLOCKS + sizeof(float) * 2 * p.blocks * p.part;
+    // (folded sums only where a sequence may be long enough)
+    const size_t own = sizeof(int) * KA_BLOCKS + sizeof(float) * p.blocks * (2 * p.part + (a.max_len > PA_FOLD * 64 ? p.sums : 0));
     return pa_many(dtype, a) ? std::max(own, packed_attend_tc_workspace(a, sms)) : own;
 }
 

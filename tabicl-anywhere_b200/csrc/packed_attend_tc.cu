@@ -12,6 +12,8 @@
 // 158, of 2^8 and 2^7 151.5, without 150). A weight's exponent is one multiply-add, so it has what the reference's rounding left: no matter, since all of a row's
 // weights have it, as long as it is small. Rows whose reference is past 2^22 are worked out again by themselves (the differences
 // of products rounded first, a subtraction a score more, take 3% longer for all others). The steps of all units are cut evenly over the blocks (kv4_plan.cuh).
+// The matrix unit rounds its sums towards zero (1.1e-7 of one an addition, of values of one sign), so the output is taken from it
+// every 8192 keys and added to what came before in the working memory: without that, outputs over 131,072 keys were 8.7e-4 too low.
 // What bounds it: 4096 bf16 tokens, 32 heads on 8 of width 128, causal, take 163 us, 0.84 PFLOP/s: a step of 64 keys 1,700 cycles, of
 // which the products need 1,350 and the exponentials of both tiles 1,024; a unit's output 6,500, a block's start 13,000. f16, 16 heads
 // of width 64, 16 sequences of 1 to 2048 tokens: 146 us, the softmax (1,600 cycles a step) and the ends of units. Registers spilled
@@ -29,6 +31,7 @@ namespace tcu {
 constexpr int PT_R = 256, PT_BQ = 128, PT_BK = 64, PT_THREADS = 512;
 constexpr int PT_STEPS = 8;  // steps a block takes at least
 constexpr int PT_RING = 4;   // pieces on their way to the roles
+constexpr int PT_FOLD = 128; // steps that the output is summed over in tensor memory
 
 template <int HD>
 struct PtShape {
@@ -86,6 +89,25 @@ __device__ __forceinline__ uint32_t pt_pair(float x, float y) {
     } else {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
         return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+
+// A row's output in tensor memory added to what `to` holds of it (HD columns, 4 of all rows beside one another), that times f.
+template <int HD>
+__device__ __noinline__ void pt_fold(uint32_t tO, float *to, float f, bool first) {
+#pragma unroll 1
+    for (int b = 0; b < HD / 16; b++) {
+        float o[16];
+        tmem_ld16(tO + 16 * b, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; k++) asm volatile("" : "+f"(o[k])::"memory");  // (not used before the wait)
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+            float4 *at = reinterpret_cast<float4 *>(to + (4 * b + k / 4) * PT_R * 4);
+            const float4 v = first ? make_float4(0.f, 0.f, 0.f, 0.f) : __ldcg(at);
+            __stcg(at, make_float4(fmaf(v.x, f, o[k]), fmaf(v.y, f, o[k + 1]), fmaf(v.z, f, o[k + 2]), fmaf(v.w, f, o[k + 3])));
+        }
     }
 }
 
@@ -358,7 +380,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                             const uint64_t d = dV + ((slot * TILE) >> 4);
                             if (elect_one()) {
 #pragma unroll
-                                for (int k = 0; k < BK / 16; k++) mma_f16_ta(tO, tS + (c & 1) * BK + 8 * k, d + ((k * 2048) >> 4), idO, i > 0 || k > 0);
+                                for (int k = 0; k < BK / 16; k++) mma_f16_ta(tO, tS + (c & 1) * BK + 8 * k, d + ((k * 2048) >> 4), idO, i % PT_FOLD > 0 || k > 0);
                                 mma_commit(&mSlot[q][c & 1]);
                                 mma_commit(&mVfree[slot]);
                             }
@@ -424,6 +446,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
             }
             float m = -INFINITY, l = 0.f;  // the row's reference (log2), its sum of weights
             float x[64];                   // a step's scores
+            // where the row's output is folded to, for a part of a unit the part's own place (for a whole one that of the block's last part,
+            // which comes after all of those), and the reference it has there
+            float *fold = part + Cut::slot(blockIdx.x, p.whole || p.begins) * C::PART + (q * BQ + row) * 4, m_fold = -INFINITY;
+            auto fold_by = [&] { return m_fold == -INFINITY ? 0.f : kt_ex2(m_fold - m); };
             auto fetch = [&](int i, float (&to)[64]) {  // once S(i) is there: on their way until the next wait for loads
                 wait_warp(&mS[q][i & 1], (uint32_t)(i >> 1) & 1u);
                 fence_after_sync();
@@ -439,62 +465,71 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 arrived_all(x);
             }
 #pragma unroll 1
-            for (int i = 0; i < nq; i++, c++) {
-                const int key0 = i * BK;
-                const uint32_t tS = tmem + lanes + TS + (2 * q + (c & 1)) * BK;
-                if (__any_sync(0xffffffffu, key0 < my_lo || key0 + BK > my_hi)) {
-                    const int low = my_lo - key0, high = my_hi - key0;
-#pragma unroll
-                    for (int k = 0; k < 64; k++)
-                        if (k < low || k >= high) x[k] = -INFINITY;
+            for (int i0 = 0; i0 < nq; i0 += PT_FOLD) {
+                if (i0) {  // (the next product begins a sum of its own)
+                    wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u);
+                    fence_after_sync();
+                    pt_fold<HD>(tO, fold, fold_by(), i0 == PT_FOLD);
+                    m_fold = m;
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int k = 0; k < 32; k++) top[k & 3] = pt_max3(top[k & 3], x[2 * k], x[2 * k + 1]);
-                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl - SHIFT;
-                if (__any_sync(0xffffffffu, mx > m + LAG)) {
-                    const float mnew = fmaxf(m, mx), f = m == -INFINITY ? 0.f : kt_ex2(m - mnew);
-                    if (i > 0) {  // O, once the product before has been added to it
-                        wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u);
-                        fence_after_sync();
 #pragma unroll 1
-                        for (int b = 0; b < HD / 16; b++) {
-                            float o[16];
-                            tmem_ld16(tO + 16 * b, o);
-                            tmem_wait_ld();
+                for (int i = i0, i1 = min(nq, i0 + PT_FOLD); i < i1; i++, c++) {
+                    const int key0 = i * BK;
+                    const uint32_t tS = tmem + lanes + TS + (2 * q + (c & 1)) * BK;
+                    if (__any_sync(0xffffffffu, key0 < my_lo || key0 + BK > my_hi)) {
+                        const int low = my_lo - key0, high = my_hi - key0;
 #pragma unroll
-                            for (int k = 0; k < 16; k++) asm volatile("" : "+f"(o[k])::"memory");  // (not used before the wait)
-                            uint32_t w[16];
+                        for (int k = 0; k < 64; k++)
+                            if (k < low || k >= high) x[k] = -INFINITY;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                            for (int k = 0; k < 16; k++) w[k] = __float_as_uint(o[k] * f);
-                            tmem_st16u(tO + 16 * b, w);
+                    for (int k = 0; k < 32; k++) top[k & 3] = pt_max3(top[k & 3], x[2 * k], x[2 * k + 1]);
+                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sl - SHIFT;
+                    if (__any_sync(0xffffffffu, mx > m + LAG)) {
+                        const float mnew = fmaxf(m, mx), f = m == -INFINITY ? 0.f : kt_ex2(m - mnew);
+                        if (i > 0) {  // O, once the product before has been added to it
+                            wait_warp(&mSlot[q][(c - 1) & 1], (uint32_t)((c - 1) >> 1) & 1u);
+                            fence_after_sync();
+#pragma unroll 1
+                            for (int b = 0; b < HD / 16; b++) {
+                                float o[16];
+                                tmem_ld16(tO + 16 * b, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 16; k++) asm volatile("" : "+f"(o[k])::"memory");  // (not used before the wait)
+                                uint32_t w[16];
+#pragma unroll
+                                for (int k = 0; k < 16; k++) w[k] = __float_as_uint(o[k] * f);
+                                tmem_st16u(tO + 16 * b, w);
+                            }
                         }
+                        l *= f, m = mnew;
                     }
-                    l *= f, m = mnew;
-                }
-                const float mm = m == -INFINITY ? 0.f : m;
-                const float2 sl2 = make_float2(sl, sl), mm2 = make_float2(-mm, -mm);
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    const float mm = m == -INFINITY ? 0.f : m;
+                    const float2 sl2 = make_float2(sl, sl), mm2 = make_float2(-mm, -mm);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    uint32_t h[16];
+                    for (int b = 0; b < 2; b++) {
+                        uint32_t h[16];
 #pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        const float2 t = pt_fma2(make_float2(x[32 * b + 2 * k], x[32 * b + 2 * k + 1]), sl2, mm2);
-                        const float2 w = make_float2(kt_ex2(t.x), kt_ex2(t.y));
-                        sum[k & 1] = pt_add2(sum[k & 1], w);
-                        h[k] = pt_pair<DT>(w.x, w.y);
+                        for (int k = 0; k < 16; k++) {
+                            const float2 t = pt_fma2(make_float2(x[32 * b + 2 * k], x[32 * b + 2 * k + 1]), sl2, mm2);
+                            const float2 w = make_float2(kt_ex2(t.x), kt_ex2(t.y));
+                            sum[k & 1] = pt_add2(sum[k & 1], w);
+                            h[k] = pt_pair<DT>(w.x, w.y);
+                        }
+                        tmem_st16u(tS + 16 * b, h);  // over scores that have been read
                     }
-                    tmem_st16u(tS + 16 * b, h);  // over scores that have been read
-                }
-                tmem_wait_st();
-                fence_before_sync();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&mP[q][c & 1]);
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                if (i + 1 < nq) {
-                    fetch(c + 1, x);
-                    arrived_all(x);
+                    tmem_wait_st();
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&mP[q][c & 1]);
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    if (i + 1 < nq) {
+                        fetch(c + 1, x);
+                        arrived_all(x);
+                    }
                 }
             }
 
@@ -555,6 +590,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_packed_attend_tc(PackedArgs a
                 if (!nq) {
 #pragma unroll
                     for (int k = 0; k < 32; k++) o[k] = 0.f;
+                }
+                if (nq > PT_FOLD) {
+                    const float f = fold_by();
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(fold + (8 * b + k / 4) * PT_R * 4));
+                        o[k] = fmaf(v.x, f, o[k]), o[k + 1] = fmaf(v.y, f, o[k + 1]), o[k + 2] = fmaf(v.z, f, o[k + 2]), o[k + 3] = fmaf(v.w, f, o[k + 3]);
+                    }
                 }
                 if (whole) {
                     put(b, o);

@@ -345,3 +345,31 @@ def test_linear_long_rows_have_no_bias(gpu, dtype):
     off = (y.double() - want) / want
     assert off.abs().max() <= ULP[dtype] + 2.0**-14
     assert off.mean().abs() <= 2.0**-16, off.mean()
+
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,heads,keys,width", [(8192, 8, 131_072, 64), (5000, 8, 70_001, 128), (40, 300, 131_072, 64), (1, 600, 270_000, 128), (100, 40, 70_000, 256)])
+def test_attend_many_keys_have_no_bias(gpu, dtype, rows, heads, keys, width):
+    """Tens of thousands of values of one sign a row, in units that blocks do not share: sums of at most 512 additions in the matrix
+    unit, each off by a unit in the last place of f32 at most: 2^-14. (Heads of few rows share their keys in memory.)"""
+    code, tt = DT[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    kh = heads if rows > 64 and width < 256 else 1
+    q, k = torch.randn(rows, heads, width, generator=gen, device="cuda").to(tt), (0.1 * torch.randn(keys, kh, width, generator=gen, device="cuda")).to(tt)
+    v = (1 + 0.25 * torch.rand(keys, kh, width, generator=gen, device="cuda")).to(tt)
+    k[:200] *= 3  # (the largest scores are not the last)
+    qs, ks = (torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (rows, keys))
+    p = tcu.Packed(gpu, 1, rows, keys, rows, keys, qs.data_ptr(), ks.data_ptr())
+    work = torch.zeros(p.attend_workspace(code, heads, heads, width), dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(q)
+    step = width if kh > 1 else 0
+    p.attend(code, heads, heads, width, q.data_ptr(), heads * width, width, k.data_ptr(), kh * width, step, v.data_ptr(), kh * width, step, out.data_ptr(),
+             heads * width, width, width**-0.5, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    for h in (0, heads // 2, heads - 1):
+        s = q[:200, h].double() @ k[:, h % kh].double().t() * width**-0.5
+        want = torch.softmax(s, -1) @ v[:, h % kh].double()
+        off = (out[:200, h].double() - want) / want
+        assert off.abs().max() <= ULP[dtype] + 2.0**-13
+        assert off.mean().abs() <= 2.0**-14 + ULP[dtype] / off.numel() ** 0.5
