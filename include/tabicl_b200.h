@@ -524,7 +524,7 @@ TCU_API int tcu_fp4_load_device(tcu_ctx *ctx, const tcu_fp4 *m, int dtype, void 
 TCU_API size_t tcu_fp4_linear_workspace(tcu_ctx *ctx, const tcu_fp4 *w, const tcu_fp4 *x, int dtype); /* (size_t)-1: refused */
 /* y = act(x W^T + bias) + residual [x's rows][W's rows], act 0 (none) or 1 (GELU, src/kern.rs:285-290); bias and residual may
  * be NULL, and the residual may be y itself. y, bias and residual are of one type; sums are taken in f32. x and W are of one
- * format and k. A scale NaN in a row of x, or of W, makes that row's, or column's, outputs NaN, and no other. */
+ * format and k; the product of their units is a normal f32 number. A scale NaN in a row of x, or of W, makes that row's, or column's, outputs NaN, and no other. */
 TCU_API int tcu_fp4_linear_device(tcu_ctx *ctx, const tcu_fp4 *w, const tcu_fp4 *x, int dtype, void *y, int64_t ldy, const void *bias,
                                   int act, const void *residual, int64_t ldr, void *work, size_t work_bytes, void *stream);
 
@@ -545,7 +545,7 @@ TCU_API size_t tcu_packed_attend_workspace(tcu_ctx *ctx, const tcu_packed *p, in
  * and held to 2^-36 of the row's largest); f32 operands have 22 bits.
  * Of more than 64 rows of a key head in a sequence, f32 keys and values are held to 2^-35 of the largest in magnitude among 64
  * neighbours of their sequence (widths up to 128; the working memory then holds them once more, up to 1 GB of it). Scores are
- * resolved to 2^-23 of their magnitude. Strides in elements. */
+ * resolved to 2^-23 of their magnitude. q_rows * q_heads up to 2^31 - 2^16. Strides in elements, not negative. */
 TCU_API int tcu_packed_attend_device(tcu_ctx *ctx, const tcu_packed *p, int dtype, int q_heads, int heads, int width, const void *q,
                                      int64_t q_row, int64_t q_head, const void *k, int64_t k_row, int64_t k_head, const void *v,
                                      int64_t v_row, int64_t v_head, void *out, int64_t o_row, int64_t o_head, float scale, int causal,

@@ -3547,7 +3547,8 @@ static PackedArgs packed_args(const tcu_packed *p, int dtype, int q_heads, int h
     if (width < 8 || width > 256 || width % 8) fail(TCU_ERR_ARG, "packed_attend: width must be a multiple of 8, up to 256");
     if (p->seqs < 0 || p->seqs > 65535 || p->q_rows < 0 || p->k_rows < 0 || p->max_q < 0 || p->max_k < 0)
         fail(TCU_ERR_ARG, "packed_attend: 0..65535 sequences, rows and lengths not negative");
-    if ((long long)p->q_rows * q_heads > 0x7fffffffLL / 256) fail(TCU_ERR_ARG, "packed_attend: too many query rows for one call");
+    // (rows of a key head are counted in 32 bits, and whole tiles of them)
+    if ((long long)p->q_rows * q_heads > 0x7fff0000LL) fail(TCU_ERR_ARG, "packed_attend: query rows times query heads up to 2^31 - 2^16");
     PackedArgs a;
     a.c.heads = heads, a.seqs = p->seqs, a.rows = p->q_rows, a.k_rows = p->k_starts ? p->k_rows : p->q_rows;
     // (no sequence has more rows than there are)

@@ -373,3 +373,30 @@ def test_attend_many_keys_have_no_bias(gpu, dtype, rows, heads, keys, width):
         off = (out[:200, h].double() - want) / want
         assert off.abs().max() <= ULP[dtype] + 2.0**-13
         assert off.mean().abs() <= 2.0**-14 + ULP[dtype] / off.numel() ** 0.5
+
+
+# ---- many rows, many sequences --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_attend_more_rows_than_24_bits_count(gpu, dtype):
+    """270,000 tokens of 64 heads: 17 million rows."""
+    rows, heads, w, n = 270_000, 64, 8, 90
+    code, tt = DT[dtype]
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(rows, h, w, generator=gen, device="cuda").to(tt) for h in (heads, 2, 2))
+    starts = torch.arange(0, rows + 1, n, dtype=torch.int32, device="cuda")
+    p = tcu.Packed(gpu, rows // n, rows, rows, n, n, starts.data_ptr())
+    work = torch.zeros(p.attend_workspace(code, heads, 2, w), dtype=torch.uint8, device="cuda")
+    out = torch.full_like(q, 9.0)
+    p.attend(code, heads, 2, w, q.data_ptr(), heads * w, w, k.data_ptr(), 2 * w, w, v.data_ptr(), 2 * w, w, out.data_ptr(), heads * w, w, 0.3,
+             causal=True, work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    qq, kk, vv = (x.view(rows // n, n, -1, w).double().transpose(1, 2) for x in (q, k, v))
+    for at in range(0, rows // n, 500):
+        x, y, z = qq[at:at + 500], kk[at:at + 500].repeat_interleave(32, 1), vv[at:at + 500].repeat_interleave(32, 1)
+        s = (x @ y.transpose(-1, -2)) * 0.3
+        s.masked_fill_(torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1), -float("inf"))
+        want = torch.softmax(s, -1) @ z
+        got = out.view(rows // n, n, heads, w)[at:at + 500].transpose(1, 2).double()
+        # a weight's rounding of values up to 6, the output's
+        assert (got - want).abs().max() <= (2.0**-17 if dtype == "f32" else 3 * 2.0**-11) * 6
