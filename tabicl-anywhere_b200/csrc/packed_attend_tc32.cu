@@ -36,13 +36,31 @@ __device__ __forceinline__ long long ps_tile(const PackedArgs &a, int seq, int h
     return (long long)head * ps_slots(a.k_rows, a.seqs) + a.k_starts[seq] / PS_BK + seq + i;
 }
 
-// A block splits one tile. Rows behind a sequence's end are zeros.
+// A block splits one tile, found by its sequence and place in that (the grid's third coordinate and its first), or, where that would
+// be mostly blocks of nothing (sequences much shorter than the longest may be), by where it lies among all, whose sequence the block's
+// threads look for: 1000 sequences of 100 keys, of which one might have had 100,000, 3.5 ms by the first and 0.4 by the second.
+// Rows behind a sequence's end are zeros.
 template <int HD>
-__global__ void __launch_bounds__(256) k_packed_split(PackedArgs a, uint8_t *tiles, int2 *units, int wide) {
+__global__ void __launch_bounds__(256) k_packed_split(PackedArgs a, uint8_t *tiles, int2 *units, int wide, int by_place) {
     using C = PsShape<HD>;
     extern __shared__ __align__(16) uint8_t sm[];
     __shared__ float top[2][8];
-    const int seq = blockIdx.z, head = blockIdx.y, tile = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    __shared__ int s_seq;
+    const int head = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int seq = blockIdx.z, tile = blockIdx.x;
+    if (by_place) {
+        if (tid == 0) s_seq = -1;
+        __syncthreads();
+        for (int i = tid; i < a.seqs; i += 256) {
+            const KaRows s = ka_rows(a, i);
+            const int from = tile - (a.k_starts[i] / PS_BK + i);
+            if (s.ok && from >= 0 && from * PS_BK < s.len) s_seq = i;
+        }
+        __syncthreads();
+        seq = s_seq;
+        if (seq < 0) return;
+        tile -= a.k_starts[seq] / PS_BK + seq;
+    }
     const KaRows sr = ka_rows(a, seq);
     if (!sr.ok || !sr.n || tile * PS_BK >= sr.len) return;
     constexpr int LANES = HD / 4, ROWS = 256 / LANES, N = PS_BK / ROWS;  // threads a row, rows at a time, rows a thread
@@ -526,7 +544,12 @@ static cudaError_t ps_launch(const PackedArgs &a, int sms, uint8_t *work, cudaSt
     cudaError_t e = allow_dynamic_smem((const void *)k_packed_split<HD>, PsShape<HD>::TILE);
     if (e == cudaSuccess) e = allow_dynamic_smem((const void *)k_packed_attend_tc32<HD>, PsShape<HD>::SMEM);
     if (e != cudaSuccess) return e;
-    if (a.max_len) k_packed_split<HD><<<dim3((a.max_len + PS_BK - 1) / PS_BK, a.c.heads, a.seqs), 256, PsShape<HD>::TILE, s>>>(a, work + w.tiles, units, wide);
+    if (a.max_len) {
+        const long long each = (a.max_len + PS_BK - 1LL) / PS_BK, places = ps_slots(a.k_rows, a.seqs);
+        const bool by_place = each * a.seqs > 4 * places;
+        const dim3 grid((unsigned)(by_place ? places : each), a.c.heads, by_place ? 1 : a.seqs);
+        k_packed_split<HD><<<grid, 256, PsShape<HD>::TILE, s>>>(a, work + w.tiles, units, wide, by_place);
+    }
     k_packed_attend_tc32<HD><<<std::min(KA_BLOCKS, sms), PS_THREADS, PsShape<HD>::SMEM, s>>>(a, work + w.tiles, units, reinterpret_cast<float *>(work + w.parts),
                                                                                              reinterpret_cast<int *>(work));
     return cudaGetLastError();

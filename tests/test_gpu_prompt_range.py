@@ -400,3 +400,22 @@ def test_attend_more_rows_than_24_bits_count(gpu, dtype):
         got = out.view(rows // n, n, heads, w)[at:at + 500].transpose(1, 2).double()
         # a weight's rounding of values up to 6, the output's
         assert (got - want).abs().max() <= (2.0**-17 if dtype == "f32" else 3 * 2.0**-11) * 6
+
+
+@pytest.mark.parametrize("q_lens,k_lens,longest", [([70] * 300, [70] * 300, 21_000), ([100, 0, 3, 80] * 40, [90, 7, 0, 130] * 40, 9_080),
+                                                   ([66] * 700, [65] * 699 + [20_000], 20_000)])
+def test_attend_f32_longest_far_above_the_others(gpu, q_lens, k_lens, longest):
+    """Sequences that might have been much longer than they are: their keys are found by where they lie."""
+    rng = np.random.default_rng(len(q_lens))
+    rows, keys = sum(q_lens), sum(k_lens)
+    q, k, v = (rng.normal(0, 1, (n, 2, 64)).astype(np.float32) for n in (rows, keys, keys))
+    qd, kd, vd = (dev(x) for x in (q, k, v))
+    qs, ks = (dev(np.concatenate([[0], np.cumsum(x)]).astype(np.int32)) for x in (q_lens, k_lens))
+    p = tcu.Packed(gpu, len(q_lens), rows, keys, max(q_lens), longest, qs.data_ptr(), ks.data_ptr())
+    work = torch.zeros(p.attend_workspace(0, 2, 2, 64), dtype=torch.uint8, device="cuda")
+    out = torch.full_like(qd, 9.0)
+    p.attend(0, 2, 2, 64, qd.data_ptr(), 128, 64, kd.data_ptr(), 128, 64, vd.data_ptr(), 128, 64, out.data_ptr(), 128, 64, 0.125, causal=True,
+             work=work.data_ptr(), work_bytes=work.numel(), stream=1)
+    sync(gpu)
+    want, _ = plain.attend(q.astype(np.float64), k.astype(np.float64), v.astype(np.float64), q_lens, k_lens, 2, 0.125, True, 0)
+    assert np.abs(host(out) - want).max() <= 2.0**-17 * 5
