@@ -419,3 +419,22 @@ def test_attend_f32_longest_far_above_the_others(gpu, q_lens, k_lens, longest):
     sync(gpu)
     want, _ = plain.attend(q.astype(np.float64), k.astype(np.float64), v.astype(np.float64), q_lens, k_lens, 2, 0.125, True, 0)
     assert np.abs(host(out) - want).max() <= 2.0**-17 * 5
+
+
+# ---- masks and residuals that span whole tiles ----------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lens", [([700], [700]), ([300, 500], [900, 650]), ([150, 40], [1000, 70])], ids=str)
+@pytest.mark.parametrize("q_heads,heads,width", [(2, 2, 64), (4, 1, 128), (2, 1, 256)])
+@pytest.mark.parametrize("window", [64, 200, 333, 640])
+def test_attend_wide_windows(gpu, dtype, lens, q_heads, heads, width, window):
+    """Windows of several steps of keys: steps that a row's tile sees whole, in part and not at all."""
+    base.check_attend(gpu, dtype, *lens, q_heads, heads, width, True, window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("name", ["mx", "nv"])
+@pytest.mark.parametrize("rows,n,k", [(1500, 3000, 300), (2100, 5000, 512), (4096, 1000, 256), (777, 9001, 130)])
+def test_linear_residual_of_many_rows(gpu, dtype, name, rows, n, k):
+    rng = np.random.default_rng(rows)
+    base.check_linear(gpu, rng, dtype, base.FORMATS[name], rows, n, k, act=1, bias=True, residual=True)
