@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
             const int r = min(row, rows - 1), ri = (r0 + r) / each, hq = pl.head * each + (r0 + r) % each;  // rows past the end repeat the last
             const int my_hi = ka_hi(a, sr, ri) - p.j0, my_lo = ka_lo(a, sr, ri) - p.j0;
             const float rowfac = put_q(sr, ri, hq);
-            // ---- softmax: S(i) -> 2^14 P(i), P(i) = 2^(S - the step's largest), over S(i), and the factors of what was before and of the step ----
+            // ---- softmax: S(i) -> P(i) = 2^(S - r), r 14 below the step's largest, over S(i), and the factors of what was before and of the step ----
             float mrun = -INFINITY, lrun = 0.f;
 #pragma unroll 1
             for (int i = at; i < at + p.n; i++) {
@@ -365,24 +365,24 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
 #pragma unroll
                 for (int k = 0; k < 64; k++) top[k & 3] = fmaxf(top[k & 3], x[k]);
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                // (weights beside the step's own largest: a step far below the row's largest keeps its bits, for values may be as far above)
-                const float mstep = __fmul_rn(mx, c1), mnew = fmaxf(mrun, mstep), mm = mstep == -INFINITY ? 0.f : mstep;
-                const float f = mrun == -INFINITY ? 0.f : kt_ex2(mrun - mnew), h = mstep == -INFINITY ? 0.f : kt_ex2(mstep - mnew);
+                // (weights beside a number of the step's own: a step far below the row's largest keeps its bits, for values may be as far
+                // above; 2^14 for the largest, so that small ones keep theirs; of scores that do not resolve 14, 1. The step's factor knows
+                // which it was; a multiplication by 2^14 for each weight takes 2% longer.)
+                const float mstep = __fmul_rn(mx, c1), mnew = fmaxf(mrun, mstep), mm = mstep == -INFINITY ? 0.f : fabsf(mstep) < 1048576.f ? mstep - 14.f : mstep;
+                const float f = mrun == -INFINITY ? 0.f : kt_ex2(mrun - mnew), h = mstep == -INFINITY ? 0.f : kt_ex2(mm - mnew);
                 float psum[4] = {};
 #pragma unroll
                 for (int b = 0; b < 2; b++) {
                     uint32_t w[32];
 #pragma unroll
                     for (int k = 0; k < 32; k++) {
-                        // (the product rounded as the reference's was: of scores past 2^23 the rest would be more than 1)
+                        // (the product rounded as the largest's was: of scores past 2^23 the rest would be more than 1)
                         x[32 * b + k] = kt_ex2(__fmul_rn(x[32 * b + k], c1) - mm);
                         psum[k & 3] += x[32 * b + k];
                     }
-                    // P goes where the scores were: of every 16 keys, hi and lo. (Its 2^14, which keeps small weights' bits, is a factor of its
-                    // own: 14 in the exponent would be lost beside scores past 2^20, and not be the same from step to step.)
+                    // P goes where the scores were: of every 16 keys, hi and lo
 #pragma unroll
-                    for (int k = 0; k < 16; k++)
-                        split_pair(x[32 * b + 2 * k] * 16384.f, x[32 * b + 2 * k + 1] * 16384.f, w[k / 8 * 16 + k % 8], w[k / 8 * 16 + 8 + k % 8]);
+                    for (int k = 0; k < 16; k++) split_pair(x[32 * b + 2 * k], x[32 * b + 2 * k + 1], w[k / 8 * 16 + k % 8], w[k / 8 * 16 + 8 + k % 8]);
                     tmem_st32u(tsp + 32 * b, w);
                 }
                 tmem_wait_st();
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) k_packed_attend_tc32(PackedArgs
             const bool whole = p.count == sp.steps;
             float M = rowx[0][row], L = rowx[1][row];
             // (divided by the sum before it leaves its unit, a part too: the weighted sum of values near f32's largest may pass that)
-            unit -= PS_T + 14;
+            unit -= PS_T;
             const float un0 = unit < -252 ? 0.f : kt_pow2(unit / 2), un1 = unit < -252 ? 0.f : kt_pow2(unit - unit / 2);
             auto inverse = [](float sum) { return sum != 0.f ? 1.f / sum : 0.f; };  // 0 when no key is seen, NaN when a score is
             const float inv = inverse(L);
