@@ -541,8 +541,8 @@ TCU_API size_t tcu_packed_attend_workspace(tcu_ctx *ctx, const tcu_packed *p, in
  * sequence's n sees the keys up to (keys - n + i), and with window > 0 only the last `window` of those. A row that sees nothing
  * gives zeros. What a row does not see has no part in its result, NaN and infinities neither. lse (may be NULL): [q_rows][q_heads],
  * the logarithm of the sum of e^score, -infinity for a row that sees nothing. width: a multiple of 8, up to 256. Sums, weights'
- * sums and lse are f32 for every type; the weights that multiply 16-bit values are rounded to their type (f16:
- * and held to 2^-36 of the row's largest); f32 operands have 22 bits.
+ * sums and lse are f32 for every type; the weights that multiply 16-bit values are rounded to their type (f16: and held to 2^-36 of
+ * the row's largest); f32 operands have 22 bits.
  * Of more than 64 rows of a key head in a sequence, f32 keys and values are held to 2^-35 of the largest in magnitude among 64
  * neighbours of their sequence (widths up to 128; the working memory then holds them once more, up to 1 GB of it). Scores are
  * resolved to 2^-23 of their magnitude. q_rows * q_heads up to 2^31 - 2^16. Strides in elements, not negative. */

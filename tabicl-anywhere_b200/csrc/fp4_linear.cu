@@ -5,7 +5,7 @@
 // rows of x (its B), K in steps of 256 columns, 128 bytes of codes a row, by TMA into shared memory; the scales come by bulk
 // copies and go on to tensor memory. W on the unit's side of 128 serves one row and thousands alike: few rows make a narrow
 // tile, and the weights stream at the memory's rate with no instruction of a thread's spent on them.
-// What bounds it: of many rows the matrix unit (4096 x 14336 x 8192 bf16 out: 259 us, 3.7 PFLOP/s, its pipe busy in 76%); of few the
+// What bounds it: of many rows the matrix unit (4096 x 14336 x 8192 bf16 out: 259 us, 3.7 PFLOP/s, its queue busy in 74%, its tensor pipe in 54%); of few the
 // weights (8 rows of that: 14.6 us, 66 MB at 4.5 TB/s, of which 4 us are start and output); below that launch and latency (one row,
 // 1024 x 512: 6.5 us). A step's issue in a loop that worked out its descriptors and divided by the number of slots took 353 and
 // 24 us, outputs in code for all of a thread's 128 sums 930 us (the instruction caches did not hold it).

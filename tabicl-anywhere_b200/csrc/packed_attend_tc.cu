@@ -9,14 +9,15 @@
 // A row's weights are relative to a reference that follows its largest score only when that has grown by 2^8 (f16: 2^4), so O is
 // rarely rescaled. f16 weights are 2^11 times as large as that, so that they fill f16's range: one is held to 11 bits, and to 2^-36
 // of the largest, below which values of 60,000 would show the loss (16 sequences of f16 tokens: 152 us; with a lag of 2^2 and 2^13
-// 158, of 2^8 and 2^7 151.5, without 150). A weight's exponent is one multiply-add, so it has what the reference's rounding left: no matter, since all of a row's
-// weights have it, as long as it is small. Rows whose reference is past 2^22 are worked out again by themselves (the differences
-// of products rounded first, a subtraction a score more, take 3% longer for all others). The steps of all units are cut evenly over the blocks (kv4_plan.cuh).
+// 158, of 2^8 and 2^7 151.5, without 150). A weight's exponent is one multiply-add, so it has what the reference's rounding left: no
+// matter, since all of a row's weights have it, as long as it is small. Rows whose reference is past 2^22 are worked out again by
+// themselves (products rounded before the reference is subtracted take 3% longer for all others). The steps of all units are cut
+// evenly over the blocks (kv4_plan.cuh).
 // The matrix unit rounds its sums towards zero (1.1e-7 of one an addition, of values of one sign), so the output is taken from it
 // every 8192 keys and added to what came before in the working memory: without that, outputs over 131,072 keys were 8.7e-4 too low.
-// What bounds it: 4096 bf16 tokens, 32 heads on 8 of width 128, causal, take 163 us, 0.84 PFLOP/s: a step of 64 keys 1,700 cycles, of
+// What bounds it: 4096 bf16 tokens, 32 heads on 8 of width 128, causal, take 162 us, 0.85 PFLOP/s: a step of 64 keys 1,700 cycles, of
 // which the products need 1,350 and the exponentials of both tiles 1,024; a unit's output 6,500, a block's start 13,000. f16, 16 heads
-// of width 64, 16 sequences of 1 to 2048 tokens: 146 us, the softmax (1,600 cycles a step) and the ends of units. Registers spilled
+// of width 64, 16 sequences of 1 to 2048 tokens: 145 us, the softmax (1,600 cycles a step) and the ends of units. Registers spilled
 // in the roles that issue products cost 450 us for the first case, units cut by their steps alone 228. A polynomial in the place of
 // every third to sixth exponential, and the two tiles' exponentials in turns, changed nothing.
 #include <cudaTypedefs.h>

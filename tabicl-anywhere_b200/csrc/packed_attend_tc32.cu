@@ -4,11 +4,11 @@
 // kernel before, into tiles of 64 keys of one head as the matrix unit reads them, each tile scaled by a power of two of its own
 // that keeps it inside f16; every block of 128 query rows of that head then brings them by two copies a step.
 // 128 query rows of one key head (the heads that share it side by side) against 64 keys at a time: S = Q K^T with Q in tensor
-// memory; the weights P go back to tensor memory over S and multiply the values; each step's P V is folded into the output in
-// registers, so every sum across steps is taken in f32 with rounding to nearest (the matrix unit's own accumulation is not: over
+// memory; the weights P, relative to a number of the step's own, go back to tensor memory over S and multiply the values; each step's
+// P V is folded into the output in registers, in a unit of the row's own, so every sum across steps is taken in f32 with rounding to nearest (the matrix unit's own accumulation is not: over
 // 10,000 keys it would cost 2.8e-5 of an output). As in the attention over the four-bit cache (kv4_attend_tc.cu), whose two
 // warpgroups that widen codes are not needed here.
-// 2048 rows over 10,000 keys, 4 heads of 128: 165 us, 0.25 PFLOP/s of scores and sums (0.76 of products), 15 of them the split; by
+// 2048 rows over 10,000 keys, 4 heads of 128: 164 us, 0.26 PFLOP/s of scores and sums (0.76 of products), 15 of them the split; by
 // warps' products (packed_attend.cu) 1040. Bound by latency: a step's products, softmax and fold follow one another.
 #include <algorithm>
 
