@@ -60,8 +60,8 @@ __device__ __forceinline__ float pa_add(float x, float y, float &rest) {
 // or a NaN is NaN; so a row whose output holds a NaN is worked out again here, and is NaN still only if what it sees makes it so
 // (and a row whose weighted sum passed f32 before it was divided).
 // Products q k near the largest have an exact difference, however large they are; scale and exponential take that. Sums keep what
-// their roundings leave, and weights are scaled down where the values' sums come near f32's end. (A key
-// in 0.1 us; one at a time, with the whole chain of a load, five exchanges and two exponentials for each, 0.65.)
+// their roundings leave, and weights are scaled down where the values' sums come near f32's end. (A key in 0.1 us; one at a time,
+// with the whole chain of a load, five exchanges and two exponentials for each, 0.65.)
 template <int DT, int HD>
 __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int seq, int i, int hq) {
     using T = typename Elem<DT>::T;
@@ -154,8 +154,7 @@ __device__ __noinline__ void pa_repair(const PackedArgs &a, const KaRows s, int 
 // nothing has a part in that) or a NaN that not all of its rows see, or (f32, whose operands are split) its keys or the row's
 // queries an infinity; rows that see a NaN in keys or values that all see are left as they are. Infinities and NaN alike may
 // be wrong where values are so large that their weighted sums (weights up to 1 / by) may pass f32. `all`: every row that is not
-// finite. From p the
-// block's pieces begin; joined: whether it has written the unit that it shares with the blocks before, after it. By W warps (which
+// finite. From p the block's pieces begin; joined: whether it has written the unit that it shares with the blocks before, after it. By W warps (which
 // have all the registers that the kernel was compiled for), for which no bounded wait waits: a row may take as long as it has keys.
 template <int DT, int HD, int R, int STEP, int EXTRA, int W, class Cut>
 __device__ __noinline__ void pa_mend(const PackedArgs &a, typename Cut::Place p, const int *joined, bool all, float by, int *dirty) {
@@ -171,7 +170,7 @@ __device__ __noinline__ void pa_mend(const PackedArgs &a, typename Cut::Place p,
         const auto sp = Cut::span(a, s, each, p.rt);
         const int count = (int)min((long long)(sp.steps - p.skip), p.end - p.pos);
         if (count == sp.steps || joined[p.skip == 0]) {
-            const int r0 = p.rt * R, rows = min(R, s.n * each - r0), end = min(s.len, sp.base + (sp.steps - EXTRA) * STEP);
+            const int r0 = p.rt * R, rows = min(R, s.n * each - r0), end = (int)min((long long)s.len, sp.base + (long long)(sp.steps - EXTRA) * STEP);
             meet();
             if (tid == 0) *dirty = all ? 2 : 0;
             meet();
